@@ -45,6 +45,7 @@ FER_JIT_INTENT_FUSION_RELU = 1
 FER_JIT_INTENT_FUSION_MUL_SIGMOID_INPUT = 2
 
 FER_ROWS_SOFTMAX, FER_ROWS_LAYER_NORM, FER_ROWS_FAST = 1, 2, 4
+FER_ROTARY_INTERLEAVED, FER_ROTARY_AXIS_FREQS, FER_ROTARY_INVERSE = 1, 2, 4
 (FER_CHAIN_LOAD, FER_CHAIN_AFFINE, FER_CHAIN_ADD_SCALAR, FER_CHAIN_MUL_SCALAR, FER_CHAIN_RELU, FER_CHAIN_SIGMOID,
  FER_CHAIN_EXP, FER_CHAIN_TANH, FER_CHAIN_GELU_TANH, FER_CHAIN_SILU, FER_CHAIN_NEG, FER_CHAIN_ABS, FER_CHAIN_CLAMP,
  FER_CHAIN_ADD, FER_CHAIN_SUB, FER_CHAIN_MUL, FER_CHAIN_DIV, FER_CHAIN_MAX, FER_CHAIN_MIN, FER_CHAIN_RELU_LT,
@@ -175,6 +176,65 @@ class fer_gemm_request_t(C.Structure):
                 ("memory_regime", C.c_uint32)]
 
 
+class fer_rotary_args_t(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("positions", C.c_void_p), ("x_stride", C.c_size_t),
+                ("out_stride", C.c_size_t), ("rows", C.c_int), ("heads", C.c_int), ("head_dim", C.c_int),
+                ("rotary_dim", C.c_int), ("axes", C.c_int), ("sections", C.c_int * 4), ("base", C.c_float),
+                ("flags", C.c_uint32), ("dtype", C.c_uint32)]
+
+
+class fer_paged_view_t(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
+                ("batch", C.c_int), ("max_pages", C.c_int), ("pages", C.c_int), ("kv_heads", C.c_int),
+                ("page_size", C.c_int), ("head_dim", C.c_int), ("dtype", C.c_uint32)]
+
+
+class fer_paged_store_args_t(C.Structure):
+    _fields_ = [("k_rows", C.c_void_p), ("v_rows", C.c_void_p), ("k_stride", C.c_size_t), ("v_stride", C.c_size_t),
+                ("rows", C.c_int), ("n_seq", C.c_int), ("offsets", C.c_void_p), ("new_lengths", C.c_void_p),
+                ("weights", C.c_void_p), ("positions", C.c_void_p), ("seen", C.c_void_p), ("new_seen", C.c_void_p)]
+
+
+class fer_paged_attention_args_t(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_size_t), ("out_stride", C.c_size_t),
+                ("n_seq", C.c_int), ("heads", C.c_int), ("scale", C.c_float), ("lse", C.c_void_p),
+                ("weights", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class fer_paged_evict_args_t(C.Structure):
+    _fields_ = [("budget", C.c_int), ("recent", C.c_int), ("weights", C.c_void_p), ("positions", C.c_void_p),
+                ("seen", C.c_void_p), ("new_lengths", C.c_void_p), ("new_weights", C.c_void_p),
+                ("new_positions", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class fer_rotary_request_t(C.Structure):
+    _fields_ = [("x", C.c_uint64), ("out", C.c_uint64), ("positions", C.c_uint64), ("x_col", C.c_uint32),
+                ("out_col", C.c_uint32), ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32),
+                ("axes", C.c_uint32), ("sections", C.c_uint32 * 4), ("base", C.c_float), ("flags", C.c_uint32)]
+
+
+class fer_paged_cache_t(C.Structure):
+    _fields_ = [("k", C.c_uint64), ("v", C.c_uint64), ("page_table", C.c_uint64), ("lengths", C.c_uint64)]
+
+
+class fer_paged_store_request_t(C.Structure):
+    _fields_ = [("cache", fer_paged_cache_t), ("k_rows", C.c_uint64), ("v_rows", C.c_uint64), ("offsets", C.c_uint64),
+                ("new_lengths", C.c_uint64), ("weights", C.c_uint64), ("positions", C.c_uint64), ("seen", C.c_uint64),
+                ("new_seen", C.c_uint64), ("k_col", C.c_uint32), ("v_col", C.c_uint32)]
+
+
+class fer_paged_attention_request_t(C.Structure):
+    _fields_ = [("cache", fer_paged_cache_t), ("q", C.c_uint64), ("out", C.c_uint64), ("lse", C.c_uint64),
+                ("weights", C.c_uint64), ("workspace", C.c_uint64), ("q_col", C.c_uint32), ("out_col", C.c_uint32),
+                ("heads", C.c_uint32), ("scale", C.c_float)]
+
+
+class fer_paged_evict_request_t(C.Structure):
+    _fields_ = [("cache", fer_paged_cache_t), ("weights", C.c_uint64), ("positions", C.c_uint64), ("seen", C.c_uint64),
+                ("new_lengths", C.c_uint64), ("new_weights", C.c_uint64), ("new_positions", C.c_uint64),
+                ("workspace", C.c_uint64), ("budget", C.c_uint32), ("recent", C.c_uint32)]
+
+
 class fer_transformer_config_t(C.Structure):
     _fields_ = [("layers", C.c_uint32), ("d_model", C.c_uint32), ("heads", C.c_uint32), ("ffn", C.c_uint32),
                 ("vocab", C.c_uint32), ("max_tokens", C.c_uint32), ("eps", C.c_float), ("reserved", C.c_uint32)]
@@ -275,6 +335,10 @@ CAPI_PROTOTYPES = {
     "fer_submit_rows": (S, [P, C.POINTER(fer_rows_request_t), pu64]),
     "fer_jit_run_chain_f32": (S, [P, C.POINTER(fer_chain_op_t), u32, pu64, u32, u64, pu64]),
     "fer_submit_gemm": (S, [P, C.POINTER(fer_gemm_request_t), pu64]),
+    "fer_submit_rotary": (S, [P, C.POINTER(fer_rotary_request_t), pu64]),
+    "fer_submit_paged_store": (S, [P, C.POINTER(fer_paged_store_request_t), pu64]),
+    "fer_submit_paged_attention": (S, [P, C.POINTER(fer_paged_attention_request_t), pu64]),
+    "fer_submit_paged_evict": (S, [P, C.POINTER(fer_paged_evict_request_t), pu64]),
     "fer_transformer_create": (S, [P, C.POINTER(fer_transformer_config_t), pu64]),
     "fer_transformer_init_weights": (S, [P, u64, u64, f32]),
     "fer_transformer_weight_buffer": (S, [P, u64, pu64]),
@@ -361,6 +425,12 @@ KERNEL_PROTOTYPES = {
     "ptx_tensor_reduce_f32_noalloc": (C.c_int, [P, P, sz, C.c_int, P]),
     # include/fercuda/b200/ext.h (native launchers)
     "fer_fill_normal_bf16": (C.c_int, [P, sz, u64, f32, P]),
+    "fer_rotary": (C.c_int, [C.POINTER(fer_rotary_args_t), P]),
+    "fer_paged_store": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_store_args_t), P, P]),
+    "fer_paged_attention_workspace_bytes": (sz, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "fer_paged_attention": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_attention_args_t), P, P]),
+    "fer_paged_evict_workspace_bytes": (sz, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "fer_paged_evict": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_evict_args_t), P, P]),
 }
 
 _LIBS: dict[str, C.CDLL] = {}
@@ -447,6 +517,22 @@ def transformer_shard(global_batch: int, world: int, rank: int) -> tuple[int, in
     return first.value, count.value
 
 
+def paged_cache(k: int, v: int, page_table: int, lengths: int) -> fer_paged_cache_t:
+    """A paged key-value cache of four buffer ids."""
+    return fer_paged_cache_t(k, v, page_table, lengths)
+
+
+def paged_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_slots: int,
+                                    weights: bool = False) -> int:
+    """Bytes of workspace of Session.paged_attention; max_slots is max_pages * page_size."""
+    return kernels().fer_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim, max_slots, 1 if weights else 0)
+
+
+def paged_evict_workspace_bytes(batch: int, kv_heads: int, max_slots: int, budget: int) -> int:
+    """Bytes of workspace of Session.paged_evict."""
+    return kernels().fer_paged_evict_workspace_bytes(batch, kv_heads, max_slots, budget)
+
+
 class Session:
     """Thin owner of a fer_session_t* with the calls the tests and the bench need."""
 
@@ -501,6 +587,10 @@ class Session:
         check("fer_get_session_stream", self.call("fer_get_session_stream", C.byref(s)))
         return s.value
 
+    def set_stream(self, handle: int) -> None:
+        """Queues the session's work on another CUDA stream (a cudaStream_t as an integer)."""
+        check("fer_set_session_stream", self.call("fer_set_session_stream", handle))
+
     def comm_init(self, uid: bytes, rank: int, world: int, timeout_ms: int = 0) -> None:
         buf = (C.c_uint8 * COMM_UNIQUE_ID_BYTES).from_buffer_copy(uid)
         check("fer_comm_init", self.call("fer_comm_init", buf, rank, world, timeout_ms))
@@ -541,6 +631,44 @@ class Session:
         r = fer_gemm_request_t(a, b, out, 0, FER_MEMORY_AUTO)
         job = C.c_uint64()
         check("fer_submit_gemm", self.call("fer_submit_gemm", C.byref(r), C.byref(job)))
+        return job.value
+
+    def rotary(self, x: int, out: int, positions: int, heads: int, head_dim: int, *, sections=(0,), rotary_dim: int = 0,
+               base: float = 10000.0, x_col: int = 0, out_col: int = 0, interleaved: bool = False,
+               axis_freqs: bool = False, inverse: bool = False) -> int:
+        """fer_submit_rotary; one section per axis, (0,) for a single axis over the whole rotary_dim."""
+        if not 1 <= len(sections) <= 4:
+            raise ValueError("rotary takes 1 to 4 axes")
+        flags = ((FER_ROTARY_INTERLEAVED if interleaved else 0) | (FER_ROTARY_AXIS_FREQS if axis_freqs else 0) |
+                 (FER_ROTARY_INVERSE if inverse else 0))
+        r = fer_rotary_request_t(x, out, positions, x_col, out_col, heads, head_dim, rotary_dim, len(sections),
+                                 (C.c_uint32 * 4)(*sections), base, flags)
+        job = C.c_uint64()
+        check("fer_submit_rotary", self.lib.fer_submit_rotary(self.ptr, C.byref(r), C.byref(job)))
+        return job.value
+
+    def paged_store(self, cache: fer_paged_cache_t, k_rows: int, v_rows: int, *, k_col: int = 0, v_col: int = 0,
+                    offsets: int = 0, new_lengths: int = 0, weights: int = 0, positions: int = 0, seen: int = 0,
+                    new_seen: int = 0) -> int:
+        r = fer_paged_store_request_t(cache, k_rows, v_rows, offsets, new_lengths, weights, positions, seen, new_seen,
+                                      k_col, v_col)
+        job = C.c_uint64()
+        check("fer_submit_paged_store", self.lib.fer_submit_paged_store(self.ptr, C.byref(r), C.byref(job)))
+        return job.value
+
+    def paged_attention(self, cache: fer_paged_cache_t, q: int, out: int, heads: int, *, workspace: int,
+                        q_col: int = 0, out_col: int = 0, scale: float = 0.0, lse: int = 0, weights: int = 0) -> int:
+        r = fer_paged_attention_request_t(cache, q, out, lse, weights, workspace, q_col, out_col, heads, scale)
+        job = C.c_uint64()
+        check("fer_submit_paged_attention", self.lib.fer_submit_paged_attention(self.ptr, C.byref(r), C.byref(job)))
+        return job.value
+
+    def paged_evict(self, cache: fer_paged_cache_t, budget: int, recent: int, weights: int, positions: int, seen: int,
+                    *, workspace: int, new_lengths: int = 0, new_weights: int = 0, new_positions: int = 0) -> int:
+        r = fer_paged_evict_request_t(cache, weights, positions, seen, new_lengths, new_weights, new_positions,
+                                      workspace, budget, recent)
+        job = C.c_uint64()
+        check("fer_submit_paged_evict", self.lib.fer_submit_paged_evict(self.ptr, C.byref(r), C.byref(job)))
         return job.value
 
     def import_ptr(self, dtype: int, shape, ptr: int) -> int:

@@ -217,6 +217,152 @@ fer_status_t fer_transformer_prefill(fer_session_t* session, uint64_t model, uin
 fer_status_t fer_transformer_decode(fer_session_t* session, uint64_t model, uint64_t cache, uint64_t tokens,
                                     uint64_t logits, uint64_t* out_job_id);
 
+/* ---- rotary positions --------------------------------------------------------
+ * Turns the heads of x [rows, cols] (f32, f16 or bf16) by their rows'
+ * positions into out [rows, cols of its own], same dtype: head h is columns
+ * x_col + h * head_dim .. of x and out_col + h * head_dim .. of out, the other
+ * columns of out are left as they are. out may be x with the same column (in
+ * place) or with columns that do not overlap; any other overlap is refused.
+ * Query and key heads that lie side by side in a fused activation take one
+ * call. positions: i32 [rows] (one axis) or [rows, axes], axes 1 to 4 (time,
+ * height, width of video tokens). Of each head the first rotary_dim elements
+ * turn (0: all), the rest is copied. Pair i is elements i and i + rotary_dim/2,
+ * or 2i and 2i+1 with FER_ROTARY_INTERLEAVED. The pairs are dealt to the axes in order,
+ * sections[a] to axis a, together rotary_dim / 2 (one axis: sections[0] 0
+ * stands for all). Pair i turns by position * base^(-i / (rotary_dim / 2)); with
+ * FER_ROTARY_AXIS_FREQS the j-th pair of axis a by position * base^(-j /
+ * sections[a]). FER_ROTARY_INVERSE turns back, which is also the gradient of
+ * the call without it. base: > 0 and finite. */
+#define FER_ROTARY_INTERLEAVED 1u
+#define FER_ROTARY_AXIS_FREQS 2u
+#define FER_ROTARY_INVERSE 4u
+
+typedef struct fer_rotary_request {
+    uint64_t x;
+    uint64_t out;
+    uint64_t positions;
+    uint32_t x_col;
+    uint32_t out_col;
+    uint32_t heads;
+    uint32_t head_dim;       /* even, at most 1024 */
+    uint32_t rotary_dim;
+    uint32_t axes;
+    uint32_t sections[4];
+    float base;
+    uint32_t flags;          /* FER_ROTARY_* bits */
+} fer_rotary_request_t;
+
+fer_status_t fer_submit_rotary(fer_session_t* session, const fer_rotary_request_t* req, uint64_t* out_job_id);
+
+/* ---- paged key-value cache -----------------------------------------------------
+ * Keys and values of many sequences in pages handed out by the caller: k and v
+ * f16 or bf16 [pages, kv_heads, page_size, head_dim] (page_size a power of two
+ * from 8 to 256, head_dim 64, 128 or 256), page_table i32 [batch, max_pages],
+ * lengths i32 [batch]. Slot s of sequence b is row s % page_size of page
+ * page_table[b][s / page_size]; slots 0 .. lengths[b] - 1 are held, and the
+ * table's entries behind them are not read. A page id or a length out of range
+ * sets error bit 4 (fer_session_device_errors): slots of such a page count as
+ * not held, a length is clamped to 0 .. max_pages * page_size. Attention may
+ * read pages that several sequences share; pages that store or evict write
+ * must have one place in one sequence.
+ * Two optional arrays per slot follow a sequence's slots: weights f32 and
+ * positions i32, both [batch, kv_heads, max_pages * page_size]; seen i32
+ * [batch] counts the tokens a sequence ever had (its next position).
+ * Work is queued on the session stream; while that stream is captured the calls are
+ * refused (the launchers of native.h can be captured). Outputs must not
+ * overlap inputs or one another except where a line below says so. */
+typedef struct fer_paged_cache {
+    uint64_t k;
+    uint64_t v;
+    uint64_t page_table;
+    uint64_t lengths;
+} fer_paged_cache_t;
+
+/* Appends keys and values: head h of a row is columns k_col + h * head_dim ..
+ * of k_rows [rows, cols] and v_col + h * head_dim .. of v_rows (the cache's
+ * dtype; both may be one fused activation). offsets i32 [sequences + 1]: rows
+ * offsets[b] .. offsets[b+1] - 1 go behind sequence b's held slots, rows behind
+ * the last offset belong to nobody; 0: row b is the one new token of sequence
+ * b. Sequences and rows may be fewer than batch. new_lengths receives the
+ * lengths (0, or the cache's own: in place). weights (0: none) get 0 and
+ * positions (0: none) seen[b] + i for the i-th new row; seen is then required
+ * and new_seen (0 or seen: in place) receives seen[b] + the new rows. Rows
+ * that do not fit in max_pages * page_size are dropped and set error bit 4. */
+typedef struct fer_paged_store_request {
+    fer_paged_cache_t cache;
+    uint64_t k_rows;
+    uint64_t v_rows;
+    uint64_t offsets;
+    uint64_t new_lengths;
+    uint64_t weights;
+    uint64_t positions;
+    uint64_t seen;
+    uint64_t new_seen;
+    uint32_t k_col;
+    uint32_t v_col;
+} fer_paged_store_request_t;
+
+fer_status_t fer_submit_paged_store(fer_session_t* session, const fer_paged_store_request_t* req, uint64_t* out_job_id);
+
+/* One new token's attention for the first rows(q) sequences: query head h of
+ * row b is columns q_col + h * head_dim .. of q [rows, cols] (the cache's
+ * dtype) and its result the columns out_col + h * head_dim .. of out [rows,
+ * cols]; heads is a multiple of kv_heads and head h reads key head h / (heads
+ * / kv_heads). out = softmax(scale q.k) v over the held slots (store the new
+ * token's key first), f32 statistics; scale 0: 1 / sqrt(head_dim). lse
+ * (0: none) f32 [rows, heads]: log sum exp(scale q.k). weights (0: none): each
+ * held slot's probabilities, summed over the heads that share it, are added
+ * to it. A sequence without slots, or whose scores are all -inf, gives zeros
+ * and lse -inf. Bit-identical run to run; a sequence's results do not depend
+ * on the rest of the batch. q and out may be one buffer with columns that do not
+ * overlap. workspace: u8 buffer (16-byte aligned) of at least
+ * fer_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim,
+ * max_pages * page_size, weights != 0) bytes, any contents; calls on different
+ * streams need one each. */
+typedef struct fer_paged_attention_request {
+    fer_paged_cache_t cache;
+    uint64_t q;
+    uint64_t out;
+    uint64_t lse;
+    uint64_t weights;
+    uint64_t workspace;
+    uint32_t q_col;
+    uint32_t out_col;
+    uint32_t heads;
+    float scale;
+} fer_paged_attention_request_t;
+
+fer_status_t fer_submit_paged_attention(fer_session_t* session, const fer_paged_attention_request_t* req,
+                                        uint64_t* out_job_id);
+
+/* Cuts every sequence of more than `budget` slots down to `budget`, each key
+ * head for itself: slots whose position is at least seen[b] - recent are kept
+ * first, then those of the largest weight (NaN is the least; ties, and a
+ * surplus of recent slots, go to the lowest slot). Kept slots before `budget`
+ * stay; the i-th kept slot behind it moves (key, value, weight, position) into
+ * the i-th freed slot before it, so the order of slots is no order of
+ * positions. budget >= 1, recent <= budget. new_lengths, new_weights and
+ * new_positions receive the results (each 0 or the old one: in place; separate ones
+ * also receive what stayed); keys and values move in place, and everything
+ * behind a sequence's new length is left as it was. Pages behind
+ * ceil(budget / page_size) are free for other sequences afterwards. workspace: u8 buffer (16-byte aligned) of
+ * fer_paged_evict_workspace_bytes(batch, kv_heads, max_pages * page_size,
+ * budget) bytes, any contents; calls on different streams need one each. */
+typedef struct fer_paged_evict_request {
+    fer_paged_cache_t cache;
+    uint64_t weights;
+    uint64_t positions;
+    uint64_t seen;
+    uint64_t new_lengths;
+    uint64_t new_weights;
+    uint64_t new_positions;
+    uint64_t workspace;
+    uint32_t budget;
+    uint32_t recent;
+} fer_paged_evict_request_t;
+
+fer_status_t fer_submit_paged_evict(fer_session_t* session, const fer_paged_evict_request_t* req, uint64_t* out_job_id);
+
 /* Per-kernel-class timing of forwards: while enabled, every forward records a
  * CUDA event pair around each of its launches on the session stream; reading
  * synchronises the stream and sums the elapsed times. Enabling resets. */

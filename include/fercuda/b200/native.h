@@ -147,6 +147,125 @@ cudaError_t fer_decode_kv_attention(const void* qkv_dec, void* k_cache, void* v_
                                     cudaStream_t s);
 cudaError_t fer_device_int_add(int* d_len, int v, cudaStream_t s);
 cudaError_t fer_device_int_set(int* d_len, int v, cudaStream_t s);
+/* ---- rotary positions -------------------------------------------------------------
+ * Rotates the first rotary_dim elements of each of `heads` heads of every row
+ * of x [rows, heads * head_dim] (rows x_stride elements apart) into out (rows
+ * out_stride apart; out == x with equal strides rotates in place, other
+ * overlaps are not allowed); the rest of a head is copied. Pair i (i <
+ * rotary_dim / 2) is elements (i, i + rotary_dim / 2) of the head, or (2i,
+ * 2i + 1) with FER_ROTARY_FLAG_INTERLEAVED; it turns by positions[row][axis]
+ * * base^-e. Pairs are dealt to the axes in order, sections[a] each
+ * (sections add up to rotary_dim / 2); e = i / (rotary_dim / 2), or with
+ * FER_ROTARY_FLAG_AXIS_FREQS j / sections[axis] for the j-th pair of its
+ * axis. FER_ROTARY_FLAG_INVERSE turns back: the inverse, and the gradient.
+ * Angles are reduced in 64 bits, products are f32, rounded once to the
+ * output. dtype: fer_buffer_dtype_t f32, f16 or bf16. */
+#define FER_ROTARY_FLAG_INTERLEAVED 1u
+#define FER_ROTARY_FLAG_AXIS_FREQS 2u
+#define FER_ROTARY_FLAG_INVERSE 4u
+typedef struct fer_rotary_args {
+    const void* x;
+    void* out;
+    const int32_t* positions;    /* [rows, axes] */
+    size_t x_stride, out_stride; /* elements */
+    int rows, heads, head_dim, rotary_dim, axes;
+    int sections[4];
+    float base;
+    uint32_t flags;
+    uint32_t dtype;
+} fer_rotary_args_t;
+cudaError_t fer_rotary(const fer_rotary_args_t* args, cudaStream_t s);
+
+/* ---- paged key-value cache ----------------------------------------------------------
+ * K and V in pages [pages][kv_heads][page_size][head_dim] (f16 or bf16, 16-byte
+ * aligned); slot s of sequence b is row s % page_size of page
+ * page_table[b][s / page_size], and slots 0 .. lengths[b] - 1 are held.
+ * page_size is a power of two from 8 to 256, head_dim 64, 128 or 256. A page
+ * id outside [0, pages), or a length outside [0, max_pages * page_size], that
+ * a kernel meets sets error bit 4; slots of such a page are skipped (as if
+ * not held) and the length is clamped. Entries behind the last held slot are
+ * not read. Pages that fer_paged_store or fer_paged_evict write belong to one
+ * place of one sequence; fer_paged_attention only reads pages, which may be
+ * shared. */
+typedef struct fer_paged_view {
+    void* k;
+    void* v;
+    const int32_t* page_table;   /* [batch, max_pages] */
+    const int32_t* lengths;      /* [batch] */
+    int batch, max_pages, pages, kv_heads, page_size, head_dim;
+    uint32_t dtype;
+} fer_paged_view_t;
+/* Appends rows: sequence b < n_seq takes rows offsets[b] .. offsets[b+1] - 1
+ * (offsets NULL: row b), its i-th row to slot lengths[b] + i. k_rows / v_rows
+ * [rows, kv_heads * head_dim], k_stride / v_stride elements apart. Rows behind
+ * offsets[n_seq] belong to nobody. new_lengths (may be the view's lengths)
+ * receives the lengths after the call. Optional: weights f32 and positions
+ * i32, both [batch, kv_heads, max_pages * page_size], receive 0 and seen[b] + i for
+ * each new slot, and new_seen (may be seen) seen[b] + the new rows. Rows that
+ * do not fit set error bit 4 and are dropped. */
+typedef struct fer_paged_store_args {
+    const void* k_rows;
+    const void* v_rows;
+    size_t k_stride, v_stride;
+    int rows, n_seq;
+    const int32_t* offsets;      /* [n_seq + 1] or NULL */
+    int32_t* new_lengths;
+    float* weights;              /* NULL: none */
+    int32_t* positions;          /* NULL: none; else seen and new_seen are given */
+    const int32_t* seen;
+    int32_t* new_seen;
+} fer_paged_store_args_t;
+cudaError_t fer_paged_store(const fer_paged_view_t* cache, const fer_paged_store_args_t* args, uint32_t* err,
+                            cudaStream_t s);
+/* Attention of one query per sequence b < n_seq over its held slots, heads
+ * (a multiple of kv_heads; consecutive heads share a key head) of q [n_seq,
+ * heads * head_dim] (q_stride elements apart), into out (out_stride apart,
+ * not overlapping q): softmax(scale q.k) v, f32 statistics, rounded once. lse
+ * (optional) [n_seq, heads]: log of the sum of exp(scale q.k). weights
+ * (optional) f32 [batch, kv_heads, max_pages * page_size]: each held slot's
+ * probabilities, summed over the heads that share it in head order, are
+ * added. A sequence of no slots gives zeros, lse -inf. Deterministic, and a
+ * sequence's results do not depend on the others in the batch. workspace:
+ * fer_paged_attention_workspace_bytes, 16-byte aligned, any contents; two
+ * calls (or graph replays) that may run at the same time need one each. */
+typedef struct fer_paged_attention_args {
+    const void* q;
+    void* out;
+    size_t q_stride, out_stride;
+    int n_seq, heads;
+    float scale;                 /* 0: 1 / sqrt(head_dim) */
+    float* lse;
+    float* weights;
+    void* workspace;
+    size_t workspace_bytes;
+} fer_paged_attention_args_t;
+size_t fer_paged_attention_workspace_bytes(int n_seq, int heads, int kv_heads, int head_dim, int max_slots,
+                                           int with_weights);
+cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const fer_paged_attention_args_t* args, uint32_t* err,
+                                cudaStream_t s);
+/* Cuts every sequence of more than `budget` slots down to `budget`, for each
+ * key head on its own. Kept are the slots whose position is at least
+ * seen[b] - recent, then those of the largest weight (NaN is the least; ties
+ * and a surplus of recent slots go to the lowest slot). Kept slots before
+ * `budget` stay where they are, and the i-th kept slot behind it moves into
+ * the i-th freed slot before it: its key, value, weight and position. new_*
+ * (each may be the array it continues) receive the results; slots behind a
+ * sequence's new length are left as they were. workspace:
+ * fer_paged_evict_workspace_bytes, rules as above. */
+typedef struct fer_paged_evict_args {
+    int budget, recent;          /* 1 <= budget, 0 <= recent <= budget */
+    const float* weights;
+    const int32_t* positions;
+    const int32_t* seen;         /* [batch] */
+    int32_t* new_lengths;
+    float* new_weights;
+    int32_t* new_positions;
+    void* workspace;
+    size_t workspace_bytes;
+} fer_paged_evict_args_t;
+size_t fer_paged_evict_workspace_bytes(int batch, int kv_heads, int max_slots, int budget);
+cudaError_t fer_paged_evict(const fer_paged_view_t* cache, const fer_paged_evict_args_t* args, uint32_t* err,
+                            cudaStream_t s);
 /* Per-token layer norm, x f32 [T, d] -> out bf16, d one of 128, 256, ..., 4096. */
 cudaError_t fer_ln_bf16(const float* x, const float* g, const float* b, void* out, int T, int d, float eps,
                         cudaStream_t s);
