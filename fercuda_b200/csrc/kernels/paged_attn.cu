@@ -2,15 +2,34 @@
 //
 // For a query head h with key head h / group: s_j = scale q.k_j over the held
 // slots j, out = sum_j p_j v_j with p = exp(s - lse). Every key and value is
-// read once per pass over a group of heads and takes 4 flops a head and
-// element, so the pass is bound by HBM reads of the cache.
+// read once for all heads of a group and takes 4 flops a head and element, so
+// the pass is bound by HBM reads of the cache.
+//
+// Split. A sequence's slots are cut into chunks at fixed places; a unit of
+// work is (sequence, key head, block of 8 or 16 query heads, chunk). Every CTA
+// counts the units from the lengths and takes an equal, contiguous run of
+// them, so ragged batches and tables much wider than the lengths are shared
+// out evenly without the host knowing the lengths. A unit's maximum m, l = sum
+// 2^(s - m) and o = sum 2^(s - m) v go to the workspace in f32 (or, with one
+// chunk, the result to the output), and a second kernel adds a head's chunks
+// in order. Which CTA took a unit does not change its arithmetic: results are
+// the same run to run and for any batch.
+//
+// Inside a unit each of four warps takes every fourth slab of 16 (head_dim 64:
+// 32) slots through a ring of its own, filled by 16-byte asynchronous copies
+// that run on into the next unit; no barrier but the one at a unit's end.
+// Scores are S^T = K Q^T and outputs O^T = V^T P on 16-bit tensor-core tiles
+// with f32 accumulation: with slots as rows the 8 columns are the heads, so a
+// group of up to 8 heads wastes nothing it would have to read, and the
+// softmax of a head is a reduction over rows that stays in a warp. (One query
+// gives 8 or 16 columns a tile at best, 1/16 of the 128 rows a tcgen05 tile
+// has, and the tiles here run at a few per cent of the tensor pipe anyway.)
+// P is kept as the sum of two 16-bit numbers, so it has 16 bits or more:
+// rounding it once would have added half of the output's own rounding error.
 //
 // Scores are kept in base-2 units (scale * log2 e folded into one factor).
-// The slots are cut into chunks; a CTA per (sequence, key head, chunk) writes
-// the chunk's maximum m, l = sum 2^(s - m) and o = sum 2^(s - m) v in f32, and
-// a second kernel adds a head's chunks in order. When weights are wanted the
-// scores go to the workspace as well, and a third kernel adds 2^(s - lse) of a
-// group's heads, in head order, once lse is known.
+// When weights are wanted they go to the workspace as well, and the second
+// kernel adds 2^(s - lse) of a group's heads, in head order.
 //
 // A chunk whose scores are all -inf has l = 0 and counts as empty (m = 0 in
 // its exponents, so no inf - inf); l = 0 over all chunks gives zeros.
@@ -20,12 +39,17 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace {
 
 using fer::dev::Paged;
-constexpr int kThreads = 128;
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kFinish = 256;        // threads of the second kernel
+constexpr int kFinishSlots = 1024;  // slots of weights a CTA of it takes
+constexpr int kSegments = 1024;     // entries of the unit table in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -37,174 +61,650 @@ struct AttnParams {
     const void* q;
     void* out;
     size_t qs, os;
-    int heads, group, chunk, chunks;
+    int n_seq, heads, group, blocks, chunk, chunks;   // blocks: head blocks a key head
     float scale2;        // scale * log2 e
     float* lse;
     float* weights;
     float* part_ml;      // [n_seq * heads][chunks][2]
     float* part_o;       // [n_seq * heads][chunks][head_dim]
     float* scores;       // [n_seq * heads][max_slots], with weights
-    float* lse2;         // [n_seq * heads], with weights
     uint32_t* err;
 };
 
-__device__ __forceinline__ float2 widen(__half2 v) { return __half22float2(v); }
-__device__ __forceinline__ float2 widen(__nv_bfloat162 v) { return __bfloat1622float2(v); }
-template <typename T> struct Two;
-template <> struct Two<__half> { using P = __half2; };
-template <> struct Two<__nv_bfloat16> { using P = __nv_bfloat162; };
-
-template <bool MAX>
-__device__ __forceinline__ float block_reduce(float v, float* sh) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        const float o = __shfl_xor_sync(0xffffffffu, v, off);
-        v = MAX ? fmaxf(v, o) : v + o;
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
+    const int n = take ? 16 : 0;   // 0: the 16 bytes are zeroed
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+// Transposes an 8 x 8 tile of 16-bit elements spread over the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && __is_same(T, __half))
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (x, y), not negative, as two 16-bit numbers each: cut off, and what that
+// leaves. Both parts are at least the smallest positive number, so that an
+// infinite value gives an infinite product and not 0 x inf; NaN stays NaN.
+// f16 parts are of 2^14 x, which keeps 2^-38 and up; the sum over v is scaled
+// back at a unit's end.
+template <typename T>
+constexpr float kScaleP = __is_same(T, __half) ? 16384.0f : 1.0f;
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    if constexpr (__is_same(T, __half)) {
+        x *= kScaleP<T>;
+        y *= kScaleP<T>;
+        float hx, hy;
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
+            : "=f"(hx), "=f"(hy)
+            : "r"(hi));
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(y - hy), "f"(x - hx));
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(hi) : "r"(0x00010001u));
+        asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(lo) : "r"(0x00010001u));
+    } else {
+        const uint32_t ux = __float_as_uint(x), uy = __float_as_uint(y);
+        hi = __byte_perm(ux, uy, 0x7632);
+        const float rx = x - __uint_as_float(ux & 0xffff0000u), ry = y - __uint_as_float(uy & 0xffff0000u);
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(ry), "f"(rx));
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(hi) : "r"(0x00800080u));
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(lo) : "r"(0x00800080u));
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return MAX ? fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3])) : (sh[0] + sh[1]) + (sh[2] + sh[3]);
 }
 
-// grid (chunks, kv_heads, n_seq)
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attn_chunk(const Paged c, const AttnParams p) {
-    using P2 = typename Two<T>::P;
-    __shared__ float s_q[D], s_p[512], s_red[4];
-    __shared__ int s_page[512 / 8];
-    const int t = threadIdx.x, b = blockIdx.z, hk = blockIdx.y;
-    fer::dev::pdl_begin();
-    bool bad;
-    const int len = c.length(b, &bad);
-    if (bad && t == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
-    const int j0 = blockIdx.x * p.chunk;
-    if (j0 >= len) return;
-    const int n = min(p.chunk, len - j0);
-    for (int i = t; i <= (n - 1) >> c.shift; i += kThreads) {
-        s_page[i] = c.page(b, j0 + (i << c.shift));
-        if (s_page[i] < 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+// How a head_dim is cut: slots a slab, slabs in flight a warp.
+template <int D> struct Cut {
+    static constexpr int kSlab = D == 64 ? 32 : 16;
+    static constexpr int kStages = D == 256 ? 2 : 3;
+    static constexpr int kRow = 2 * D;                       // bytes
+    static constexpr int kStage = 2 * kSlab * kRow;          // keys, then values
+    static constexpr int kRing = kWarps * kStages * kStage;
+    template <int NT> static constexpr int merge() { return 2 * 32 * 4 * (NT * (D / 16 * 4 + 4)); }
+    template <int NT> static constexpr int smem() { return kRing + merge<NT>() + 4 * (kSegments + 1); }
+};
+
+// The units before every segment of sequences; kept in shared memory.
+struct Units {
+    const int* cum;   // [segments + 1]
+    int segments, seg;
+};
+
+// One unit, the same for all threads of a warp.
+struct Unit {
+    int b, hk, blk, chunk, chunks, k0, n;
+};
+
+__device__ __forceinline__ Unit find_unit(const Paged& c, const AttnParams& p, const Units& t, int u) {
+    int lo = 0, hi = t.segments;            // the last segment that starts at or before u
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (t.cum[mid] <= u) lo = mid;
+        else hi = mid;
     }
+    int r = u - t.cum[lo];
+    int b = lo * t.seg, len = 0, nch = 0;
+    bool bad;
+    for (;; ++b) {
+        len = c.length(b, &bad);
+        nch = (len + p.chunk - 1) / p.chunk;
+        const int here = nch * c.kv_heads * p.blocks;
+        if (r < here || b + 1 >= p.n_seq) break;
+        r -= here;
+    }
+    Unit x;
+    x.b = b;
+    x.chunks = nch;
+    const int hb = r / nch;
+    x.chunk = r - hb * nch;
+    x.hk = hb / p.blocks;
+    x.blk = hb - x.hk * p.blocks;
+    x.k0 = x.chunk * p.chunk;
+    x.n = min(p.chunk, len - x.k0);
+    return x;
+}
+
+// Page ids of a unit's chunk (up to 64 pages): lane i holds those of its i-th
+// and (i + 32)-th page, -1 where no slot is held or the table has no page.
+struct ChunkPages {
+    int a, b;
+    __device__ __forceinline__ int of(const Paged& c, int slot) const {
+        const int i = slot >> c.shift;
+        const int x = __shfl_sync(0xffffffffu, a, i & 31), y = __shfl_sync(0xffffffffu, b, i & 31);
+        return i < 32 ? x : y;
+    }
+    __device__ __forceinline__ bool all_good(const Paged& c, int n) const {
+        const int lane = threadIdx.x & 31, last = (n - 1) >> c.shift;
+        return !__any_sync(0xffffffffu, (lane <= last && a < 0) || (lane + 32 <= last && b < 0));
+    }
+};
+
+__device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x) {
+    const int lane = threadIdx.x & 31, last = (x.n - 1) >> c.shift;
+    ChunkPages g{-1, -1};
+    if (lane <= last) g.a = c.page(x.b, x.k0 + (lane << c.shift));
+    if (lane + 32 <= last) g.b = c.page(x.b, x.k0 + ((lane + 32) << c.shift));
+    return g;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const AttnParams p) {
+    using C = Cut<D>;
+    constexpr int kB = D / 16;                  // 16-wide blocks of a row
+    constexpr int kPieces = D / 8;              // 16-byte pieces of a row
+    constexpr int kRowsPer = 32 / kPieces;      // rows a warp copies at once
+    constexpr int kSub = C::kSlab / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int s_sum[kWarps];
+    float* merge = reinterpret_cast<float*>(smem + C::kRing);
+    int* cum = reinterpret_cast<int*>(smem + C::kRing + C::template merge<NT>());
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    fer::dev::pdl_begin();
+
+    // how many units each segment of sequences has, and the sums before them
+    Units table{cum, 0, 0};
+    table.seg = (p.n_seq + kSegments - 1) / kSegments;
+    table.segments = (p.n_seq + table.seg - 1) / table.seg;
+    int carry = 0;
+    for (int s0 = 0; s0 < table.segments; s0 += kThreads) {
+        int mine = 0;
+        const int s = s0 + t;
+        if (s < table.segments) {
+            for (int b = s * table.seg; b < min(p.n_seq, (s + 1) * table.seg); ++b) {
+                bool bad;
+                const int len = c.length(b, &bad);
+                if (bad && blockIdx.x == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+                mine += (len + p.chunk - 1) / p.chunk * c.kv_heads * p.blocks;
+            }
+        }
+        int x = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, off);
+            if (lane >= off) x += y;
+        }
+        if (lane == 31) s_sum[w] = x;
+        __syncthreads();
+        int before = carry;
+        for (int i = 0; i < kWarps; ++i) {
+            if (i < w) before += s_sum[i];
+            carry += s_sum[i];
+        }
+        if (s < table.segments) cum[s] = before + x - mine;
+        __syncthreads();
+    }
+    const int total = carry;
+    // sequences that hold nothing have no unit: their results are written here
+    for (int b = blockIdx.x; b < p.n_seq; b += gridDim.x) {
+        bool bad;
+        if (c.length(b, &bad) > 0) continue;
+        T* o = static_cast<T*>(p.out) + b * p.os;
+        for (int i = t; i < p.heads * D; i += kThreads) o[i] = static_cast<T>(0.0f);
+        if (p.lse)
+            for (int i = t; i < p.heads; i += kThreads) p.lse[static_cast<size_t>(b) * p.heads + i] = -INFINITY;
+    }
+    const int u0 = static_cast<int>(static_cast<long long>(total) * blockIdx.x / gridDim.x);
+    const int u1 = static_cast<int>(static_cast<long long>(total) * (blockIdx.x + 1) / gridDim.x);
+    if (u0 >= u1) return;
+
+    const uint32_t ring = fer::dev::smem_addr(smem) + w * C::kStages * C::kStage;
     const T* kc = static_cast<const T*>(c.k);
     const T* vc = static_cast<const T*>(c.v);
-    for (int g = 0; g < p.group; ++g) {
-        const int h = hk * p.group + g;
-        const size_t bh = static_cast<size_t>(b) * p.heads + h;
-        __syncthreads();
-        for (int i = t; i < D; i += kThreads)
-            s_q[i] = static_cast<float>(static_cast<const T*>(p.q)[b * p.qs + static_cast<size_t>(h) * D + i]);
-        __syncthreads();
-        float m = -INFINITY;
-        for (int j = t; j < n; j += kThreads) {
-            const int id = s_page[j >> c.shift];
-            float s = -INFINITY;
-            if (id >= 0) {
-                const P2* row = reinterpret_cast<const P2*>(kc + c.row(id, hk, j0 + j));
-                float dot = 0.0f;
-#pragma unroll 8
-                for (int i = 0; i < D / 2; ++i) {
-                    const float2 f = widen(row[i]);
-                    dot = fmaf(f.x, s_q[2 * i], dot);
-                    dot = fmaf(f.y, s_q[2 * i + 1], dot);
+
+    // what is being loaded: unit lu, slab li of it; its pages, and the next unit's on their way
+    int lu = u0, li = w, loads = 0;
+    Unit lx = find_unit(c, p, table, u0);
+    ChunkPages lp = load_pages(c, lx);
+    Unit nx = lx;
+    ChunkPages np = lp;
+    if (u0 + 1 < u1) {
+        nx = find_unit(c, p, table, u0 + 1);
+        np = load_pages(c, nx);
+    }
+    auto issue = [&]() {
+        while (lu < u1 && li * C::kSlab >= lx.n) {   // no slab of this unit is left for this warp
+            ++lu;
+            li = w;
+            lx = nx;
+            lp = np;
+            if (lu + 1 < u1) {
+                nx = find_unit(c, p, table, lu + 1);
+                np = load_pages(c, nx);
+            }
+        }
+        if (lu < u1) {
+            const uint32_t st = ring + (loads % C::kStages) * C::kStage;
+            const int piece = lane % kPieces;
+#pragma unroll
+            for (int i = 0; i < C::kSlab / kRowsPer; ++i) {
+                const int r = i * kRowsPer + lane / kPieces;
+                const int slot = li * C::kSlab + r;
+                const int id = lp.of(c, slot < lx.n ? slot : lx.n - 1);
+                const bool take = slot < lx.n && id >= 0;
+                const size_t at = take ? c.row(id, lx.hk, slot) + piece * 8 : 0;
+                const uint32_t to = st + r * C::kRow + ((piece ^ (r & 7)) << 4);
+                cp16(to, kc + at, take);
+                cp16(to + C::kSlab * C::kRow, vc + at, take);
+            }
+            li += kWarps;
+            ++loads;
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) issue();
+
+    int used = 0;
+    uint32_t qf[NT][kB][2];
+    int last_b = -1, last_hk = -1, last_blk = -1;
+    for (int u = u0; u < u1; ++u) {
+        const Unit x = find_unit(c, p, table, u);
+        const int h0 = x.hk * p.group + x.blk * 8 * NT;          // first head of the block
+        const int nh = min(8 * NT, p.group - x.blk * 8 * NT);    // its heads
+        if (x.b != last_b || x.hk != last_hk || x.blk != last_blk) {
+            last_b = x.b, last_hk = x.hk, last_blk = x.blk;
+            // columns (heads) lane / 4, rows (dims) 2 (lane % 4) + {0, 1} and 8 more
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int g = nt * 8 + lane / 4;
+                const T* q = static_cast<const T*>(p.q) + x.b * p.qs + static_cast<size_t>(h0 + (g < nh ? g : 0)) * D;
+                const bool even = (reinterpret_cast<uintptr_t>(q) & 3) == 0;
+#pragma unroll
+                for (int k = 0; k < kB; ++k)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint16_t* at = reinterpret_cast<const uint16_t*>(q + 16 * k + 8 * e + 2 * (lane & 3));
+                        uint32_t v;
+                        if (even) v = *reinterpret_cast<const uint32_t*>(at);
+                        else v = at[0] | static_cast<uint32_t>(at[1]) << 16;
+                        qf[nt][k][e] = g < nh ? v : 0u;
+                    }
+            }
+        }
+        const ChunkPages pg = load_pages(c, x);
+        const bool good = pg.all_good(c, x.n);
+        if (!good && w == 0 && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+
+        float m[NT][2], l[NT][2], o[NT][kB][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kB; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.0f;
+        }
+        for (int i = w; i * C::kSlab < x.n; i += kWarps) {
+            cp_wait<C::kStages - 2>();
+            __syncwarp();
+            issue();
+            const uint32_t st = ring + (used % C::kStages) * C::kStage;
+            ++used;
+#pragma unroll
+            for (int sub = 0; sub < kSub; ++sub) {
+                float s[NT][4];
+                {
+                    float s2[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
+                    const int r = sub * 16 + (lane & 15);
+#pragma unroll
+                    for (int k = 0; k < kB; ++k) {
+                        uint32_t a[4];
+                        ldsm4(a, st + r * C::kRow + (((2 * k + (lane >> 4)) ^ (r & 7)) << 4));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma<T>(k & 1 ? s2[nt] : s[nt], a, qf[nt][k][0], qf[nt][k][1]);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * p.scale2;
                 }
-                s = dot * p.scale2;
+                const int j = i * C::kSlab + sub * 16 + lane / 4;   // this lane's slots of the chunk: j, j + 8
+                bool on0 = j < x.n, on1 = j + 8 < x.n;
+                if (!good) {
+                    const int p0 = pg.of(c, min(j, x.n - 1)), p1 = pg.of(c, min(j + 8, x.n - 1));
+                    on0 = on0 && p0 >= 0;
+                    on1 = on1 && p1 >= 0;
+                }
+                bool grew = false;
+                float next[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (!on0) s[nt][e] = -INFINITY;
+                        if (!on1) s[nt][2 + e] = -INFINITY;
+                        float v = fmaxf(s[nt][e], s[nt][2 + e]);
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                        next[nt][e] = fmaxf(m[nt][e], v);
+                        grew |= next[nt][e] > m[nt][e];
+                    }
+                if (p.scores) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int g = nt * 8 + 2 * (lane & 3) + e;
+                            float* row = p.scores + (static_cast<size_t>(x.b) * p.heads + h0 + g) * c.max_slots() + x.k0;
+                            if (g < nh && j < x.n) row[j] = s[nt][e];
+                            if (g < nh && j + 8 < x.n) row[j + 8] = s[nt][2 + e];
+                        }
+                }
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float f = ex2(m[nt][e] - (next[nt][e] == -INFINITY ? 0.0f : next[nt][e]));
+                            m[nt][e] = next[nt][e];
+                            l[nt][e] *= f;
+#pragma unroll
+                            for (int k = 0; k < kB; ++k) o[nt][k][e] *= f, o[nt][k][2 + e] *= f;
+                        }
+                }
+                uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float base = m[nt][e] == -INFINITY ? 0.0f : m[nt][e];
+                        s[nt][e] = ex2(s[nt][e] - base);
+                        s[nt][2 + e] = ex2(s[nt][2 + e] - base);
+                        l[nt][e] += s[nt][e] + s[nt][2 + e];
+                    }
+                    split2<T>(s[nt][0], s[nt][1], hi[nt][0], lo[nt][0]);
+                    split2<T>(s[nt][2], s[nt][3], hi[nt][1], lo[nt][1]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        hi[nt][e] = transpose8(hi[nt][e]);
+                        lo[nt][e] = transpose8(lo[nt][e]);
+                    }
+                }
+                const int r = sub * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                for (int k = 0; k < kB; ++k) {
+                    uint32_t a[4];
+                    ldsm4_t(a, st + C::kSlab * C::kRow + r * C::kRow + (((2 * k + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma<T>(o[nt][k], a, lo[nt][0], lo[nt][1]);
+                        mma<T>(o[nt][k], a, hi[nt][0], hi[nt][1]);
+                    }
+                }
             }
-            s_p[j] = s;
-            if (p.scores) p.scores[bh * c.max_slots() + j0 + j] = s;
-            m = fmaxf(m, s);
         }
-        m = block_reduce<true>(m, s_red);
-        const float base = m == -INFINITY ? 0.0f : m;
-        float l = 0.0f;
-        for (int j = t; j < n; j += kThreads) {
-            const float e = exp2f(s_p[j] - base);
-            s_p[j] = e;
-            l += e;
-        }
-        l = block_reduce<false>(l, s_red);
-        const size_t at = bh * p.chunks + blockIdx.x;
-        if (t == 0) {
-            p.part_ml[2 * at] = m;
-            p.part_ml[2 * at + 1] = l;
-        }
-        for (int i = t; i < D / 2; i += kThreads) {
-            float2 o = make_float2(0.0f, 0.0f);
-            for (int j = 0; j < n; ++j) {
-                const int id = s_page[j >> c.shift];
-                if (id < 0) continue;
-                const float2 f = widen(reinterpret_cast<const P2*>(vc + c.row(id, hk, j0 + j))[i]);
-                o.x = fmaf(s_p[j], f.x, o.x);
-                o.y = fmaf(s_p[j], f.y, o.y);
+
+        // the warps' parts: 2 and 3 into 0 and 1, then 1 into 0
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
+                l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
             }
-            reinterpret_cast<float2*>(p.part_o + at * D)[i] = o;
+        constexpr int kRegs = NT * (kB * 4 + 4);
+#pragma unroll
+        for (int half = 2; half >= 1; half >>= 1) {
+            float* slot = merge + (w & 1) * kRegs * 32 + lane;
+            if (w >= half && w < 2 * half) {
+                float* at = half == 2 ? slot : merge + lane;
+                int i = 0;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        at[32 * i++] = m[nt][e];
+                        at[32 * i++] = l[nt][e];
+                    }
+#pragma unroll
+                    for (int k = 0; k < kB; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) at[32 * i++] = o[nt][k][e];
+                }
+            }
+            __syncthreads();
+            if (w < half) {
+                const float* at = half == 2 ? slot : merge + lane;
+                int i = 0;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float fa[2], fb[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float om = at[32 * i++], ol = at[32 * i++];
+                        const float top = fmaxf(m[nt][e], om), base = top == -INFINITY ? 0.0f : top;
+                        fa[e] = ex2(m[nt][e] - base);
+                        fb[e] = ex2(om - base);
+                        m[nt][e] = top;
+                        l[nt][e] = l[nt][e] * fa[e] + ol * fb[e];
+                    }
+#pragma unroll
+                    for (int k = 0; k < kB; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[nt][k][e] = o[nt][k][e] * fa[e & 1] + at[32 * i++] * fb[e & 1];
+                }
+            }
+            __syncthreads();
+        }
+        if (w == 0) {
+            constexpr float kBack = 1.0f / kScaleP<T>;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int g = nt * 8 + 2 * (lane & 3) + e;
+                    if (g >= nh) continue;
+                    const size_t bh = static_cast<size_t>(x.b) * p.heads + h0 + g;
+                    const size_t at = bh * p.chunks + x.chunk;
+                    const bool whole = x.chunks == 1;
+                    const float inv = l[nt][e] == 0.0f ? 0.0f : 1.0f / l[nt][e];
+                    if (lane < 4) {
+                        p.part_ml[2 * at] = m[nt][e];
+                        p.part_ml[2 * at + 1] = l[nt][e];
+                        if (whole && p.lse)
+                            p.lse[bh] = l[nt][e] == 0.0f ? -INFINITY : (m[nt][e] + log2f(l[nt][e])) * kLn2;
+                    }
+                    T* out = static_cast<T*>(p.out) + x.b * p.os + static_cast<size_t>(h0 + g) * D;
+                    float* po = p.part_o + at * D;
+#pragma unroll
+                    for (int k = 0; k < kB; ++k)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const int d = 16 * k + 8 * r + lane / 4;
+                            const float v = o[nt][k][2 * r + e] * kBack;
+                            if (whole) out[d] = static_cast<T>(l[nt][e] == 0.0f ? 0.0f : v * inv);
+                            else po[d] = v;
+                        }
+                }
         }
     }
+    cp_wait<0>();
 }
 
-// grid (heads, n_seq), D threads: a head's chunks added in order
+// log2 of a head's total sum of powers, from its chunks' (m, l), by one warp;
+// -inf where nothing counts. The maximum's base goes to *base.
+__device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float* base, float* sum) {
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY;
+    for (int i = lane; i < chunks; i += 32) top = fmaxf(top, ml[2 * i]);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float b = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f;
+    for (int i = lane; i < chunks; i += 32) l += ml[2 * i + 1] * ex2(ml[2 * i] - b);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    *base = b;
+    *sum = l;
+    return l == 0.0f ? -INFINITY : b + log2f(l);
+}
+
+// grid (group + weight tiles, kv_heads, n_seq). The first `group` CTAs of a
+// (key head, sequence) add one head's chunks each (in order within a warp,
+// then the warps in order); the others add probabilities to kFinishSlots
+// slots' weights each.
 template <typename T, int D>
-__global__ void __launch_bounds__(D) attn_join(const Paged c, const AttnParams p) {
+__global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
+    constexpr int kW = kFinish / 32, kV = D / 32;    // warps; dims a lane
+    __shared__ float s_o[kW][D];
+    __shared__ float s_lse[kFinish];
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    const int b = blockIdx.z, hk = blockIdx.y;
     fer::dev::pdl_begin();
-    const int b = blockIdx.y, h = blockIdx.x, t = threadIdx.x;
     bool bad;
     const int len = c.length(b, &bad);
     const int chunks = (len + p.chunk - 1) / p.chunk;
-    const size_t bh = static_cast<size_t>(b) * p.heads + h;
-    const float* ml = p.part_ml + 2 * bh * p.chunks;
-    const float* po = p.part_o + bh * p.chunks * D;
-    float M = -INFINITY;
-    for (int i = 0; i < chunks; ++i) M = fmaxf(M, ml[2 * i]);
-    const float base = M == -INFINITY ? 0.0f : M;
-    float l = 0.0f, o = 0.0f;
-    for (int i = 0; i < chunks; ++i) {
-        const float w = exp2f(ml[2 * i] - base);
-        l = fmaf(ml[2 * i + 1], w, l);
-        o = fmaf(po[static_cast<size_t>(i) * D + t], w, o);
-    }
-    static_cast<T*>(p.out)[b * p.os + static_cast<size_t>(h) * D + t] = static_cast<T>(l == 0.0f ? 0.0f : o / l);
-    if (t == 0) {
-        const float lse2 = l == 0.0f ? -INFINITY : base + log2f(l);
-        if (p.lse) p.lse[bh] = lse2 * kLn2;
-        if (p.lse2) p.lse2[bh] = lse2;
-    }
-}
-
-// grid (slot tiles, kv_heads, n_seq)
-__global__ void __launch_bounds__(kThreads) attn_weights(const Paged c, const AttnParams p) {
-    fer::dev::pdl_begin();
-    const int b = blockIdx.z, hk = blockIdx.y;
-    bool bad;
-    const int len = c.length(b, &bad);
-    const size_t most = static_cast<size_t>(c.max_slots());
-    for (int j = blockIdx.x * kThreads + threadIdx.x; j < len; j += gridDim.x * kThreads) {
-        float w = 0.0f;
-        for (int g = 0; g < p.group; ++g) {
-            const size_t bh = static_cast<size_t>(b) * p.heads + hk * p.group + g;
-            const float lse2 = p.lse2[bh];
-            if (lse2 != -INFINITY) w += exp2f(p.scores[bh * most + j] - lse2);
+    const size_t bh0 = static_cast<size_t>(b) * p.heads + static_cast<size_t>(hk) * p.group;
+    if (static_cast<int>(blockIdx.x) < p.group) {
+        if (chunks <= 1) return;                      // written already
+        const size_t bh = bh0 + blockIdx.x;
+        const float* ml = p.part_ml + 2 * bh * p.chunks;
+        const float* po = p.part_o + bh * p.chunks * D;
+        float base, l;
+        const float lse2 = chunks_lse2(ml, chunks, &base, &l);
+        float o[kV];
+#pragma unroll
+        for (int e = 0; e < kV; ++e) o[e] = 0.0f;
+#pragma unroll 4
+        for (int i = w; i < chunks; i += kW) {
+            const float f = ex2(ml[2 * i] - base);
+#pragma unroll
+            for (int e = 0; e < kV; ++e) o[e] = fmaf(po[static_cast<size_t>(i) * D + e * 32 + lane], f, o[e]);
         }
-        p.weights[(static_cast<size_t>(b) * c.kv_heads + hk) * most + j] += w;
+#pragma unroll
+        for (int e = 0; e < kV; ++e) s_o[w][e * 32 + lane] = o[e];
+        __syncthreads();
+        for (int d = t; d < D; d += kFinish) {
+            float v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kW; ++i) v += s_o[i][d];
+            static_cast<T*>(p.out)[b * p.os + (static_cast<size_t>(hk) * p.group + blockIdx.x) * D + d] =
+                static_cast<T>(l == 0.0f ? 0.0f : v / l);
+        }
+        if (t == 0 && p.lse) p.lse[bh] = lse2 * kLn2;
+        return;
+    }
+    const int j0 = (blockIdx.x - p.group) * kFinishSlots;
+    if (j0 >= len) return;
+    const size_t most = static_cast<size_t>(c.max_slots());
+    constexpr int kEach = kFinishSlots / kFinish;
+    float sum[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sum[e] = 0.0f;
+    for (int g0 = 0; g0 < p.group; g0 += kFinish) {
+        const int ng = min(kFinish, p.group - g0);
+        __syncthreads();
+        for (int g = w; g < ng; g += kW) {
+            float base, l;
+            const float v = chunks_lse2(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks, &base, &l);
+            if (lane == 0) s_lse[g] = v;
+        }
+        __syncthreads();
+        for (int g = 0; g < ng; ++g) {
+            if (s_lse[g] == -INFINITY) continue;
+            const float* row = p.scores + (bh0 + g0 + g) * most;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int j = j0 + e * kFinish + t;
+                if (j < len) sum[e] += ex2(row[j] - s_lse[g]);
+            }
+        }
+    }
+    float* out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int j = j0 + e * kFinish + t;
+        if (j < len) out[j] += sum[e];
     }
 }
 
-template <typename T, int D>
-cudaError_t run(const Paged& c, const AttnParams& p, int n_seq, cudaStream_t s) {
+// CTAs of a kernel that fit on the current device at once; 0 on an error. The
+// answer is kept per device, where the shared-memory limit is also set.
+constexpr int kDevices = 64;
+int resident(const void* kernel, int smem, std::atomic<int>* known) {
+    int dev = 0, n = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
+    if (const int k = known[dev].load(std::memory_order_relaxed)) return k;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return 0;
+    known[dev].store(n * sms, std::memory_order_relaxed);
+    return n * sms;
+}
+
+template <typename T, int D, int NT>
+cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     using fer::host::launch_pdl;
-    cudaError_t e = launch_pdl(attn_chunk<T, D>, dim3(p.chunks, c.kv_heads, n_seq), dim3(kThreads), 0, s, c, p);
-    if (e == cudaSuccess) e = launch_pdl(attn_join<T, D>, dim3(p.heads, n_seq), dim3(D), 0, s, c, p);
-    if (e == cudaSuccess && p.weights) {
-        const int tiles = (c.max_pages << c.shift) / 1024 + 1;
-        e = launch_pdl(attn_weights, dim3(tiles, c.kv_heads, n_seq), dim3(kThreads), 0, s, c, p);
+    constexpr int smem = Cut<D>::template smem<NT>();
+    static std::atomic<int> known[kDevices];
+    const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT>), smem, known);
+    if (ctas <= 0) return cudaErrorInvalidConfiguration;
+    const long long most = static_cast<long long>(p.n_seq) * c.kv_heads * p.blocks * p.chunks;
+    cudaError_t e = launch_pdl(attn_units<T, D, NT>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
+                               dim3(kThreads), smem, s, c, p);
+    if (e == cudaSuccess && (p.weights || p.chunks > 1)) {
+        const int tiles = p.weights ? (c.max_slots() - 1) / kFinishSlots + 1 : 0;
+        e = launch_pdl(attn_finish<T, D>, dim3(p.group + tiles, c.kv_heads, p.n_seq), dim3(kFinish), 0, s, c, p);
     }
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+template <typename T, int D>
+cudaError_t run_heads(const Paged& c, AttnParams& p, cudaStream_t s) {
+    if (p.group <= 8) {
+        p.blocks = 1;
+        return run<T, D, 1>(c, p, s);
+    }
+    p.blocks = (p.group + 15) / 16;
+    return run<T, D, 2>(c, p, s);
+}
+
 template <typename T>
-cudaError_t run_dim(const Paged& c, const AttnParams& p, int n_seq, cudaStream_t s) {
+cudaError_t run_dim(const Paged& c, AttnParams& p, cudaStream_t s) {
     switch (c.head_dim) {
-        case 64: return run<T, 64>(c, p, n_seq, s);
-        case 128: return run<T, 128>(c, p, n_seq, s);
-        default: return run<T, 256>(c, p, n_seq, s);
+        case 64: return run_heads<T, 64>(c, p, s);
+        case 128: return run_heads<T, 128>(c, p, s);
+        default: return run_heads<T, 256>(c, p, s);
     }
 }
 
@@ -218,7 +718,7 @@ extern "C" size_t fer_paged_attention_workspace_bytes(int n_seq, int heads, int 
     const size_t bh = static_cast<size_t>(n_seq) * heads;
     const size_t chunks = (max_slots - 1) / chunk_of(max_slots) + 1;
     size_t n = up16(bh * chunks * 2 * sizeof(float)) + up16(bh * chunks * head_dim * sizeof(float));
-    if (with_weights) n += up16(bh * sizeof(float)) + up16(bh * max_slots * sizeof(float));
+    if (with_weights) n += up16(bh * max_slots * sizeof(float));
     return n;
 }
 
@@ -235,7 +735,10 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 2) return cudaErrorInvalidValue;
     if (a->n_seq == 0) return cudaSuccess;
     if (c.kv_heads > 65535 || a->n_seq > 65535) return cudaErrorNotSupported;
-    const int max_slots = c.max_pages << c.shift;
+    const int max_slots = c.max_slots();
+    // units are counted in 31 bits
+    if (static_cast<long long>(a->n_seq) * a->heads * ((max_slots - 1) / chunk_of(max_slots) + 1) > 0x7fffffffll)
+        return cudaErrorNotSupported;
     const size_t need = fer_paged_attention_workspace_bytes(a->n_seq, a->heads, c.kv_heads, c.head_dim, max_slots,
                                                             a->weights != nullptr);
     if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_bytes < need)
@@ -245,6 +748,7 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     p.out = a->out;
     p.qs = a->q_stride;
     p.os = a->out_stride;
+    p.n_seq = a->n_seq;
     p.heads = a->heads;
     p.group = a->heads / c.kv_heads;
     p.chunk = chunk_of(max_slots);
@@ -259,11 +763,6 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     w += up16(bh * p.chunks * 2 * sizeof(float));
     p.part_o = reinterpret_cast<float*>(w);
     w += up16(bh * p.chunks * c.head_dim * sizeof(float));
-    if (a->weights) {
-        p.lse2 = reinterpret_cast<float*>(w);
-        w += up16(bh * sizeof(float));
-        p.scores = reinterpret_cast<float*>(w);
-    }
-    return c.head_dim && cache->dtype == 1 ? run_dim<__half>(c, p, a->n_seq, s)
-                                           : run_dim<__nv_bfloat16>(c, p, a->n_seq, s);
+    if (a->weights) p.scores = reinterpret_cast<float*>(w);
+    return cache->dtype == 1 ? run_dim<__half>(c, p, s) : run_dim<__nv_bfloat16>(c, p, s);
 }
