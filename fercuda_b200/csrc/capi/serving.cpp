@@ -100,7 +100,7 @@ fer_status_t open_cache(const Session& S, const fer_paged_cache_t& r, Cache* c) 
     if (k.dims[2] < 8 || k.dims[2] > 256 || (k.dims[2] & (k.dims[2] - 1)))
         return invalid("paged cache page_size must be a power of two from 8 to 256");
     if (k.dims[0] > INT_MAX || k.dims[1] > 65535 || t.dims[0] > 65535 ||
-        static_cast<uint64_t>(t.dims[1]) * k.dims[2] > INT_MAX - 1024)
+        static_cast<uint64_t>(t.dims[1]) * k.dims[2] > INT_MAX - 65536)
         return invalid("paged cache is too large");
     if ((reinterpret_cast<uintptr_t>(c->k->ptr) | reinterpret_cast<uintptr_t>(c->v->ptr)) % 16)
         return invalid("paged cache keys and values must be 16-byte aligned");

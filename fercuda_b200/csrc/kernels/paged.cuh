@@ -54,7 +54,7 @@ inline cudaError_t paged_params(const fer_paged_view_t* c, fer::dev::Paged* p) {
     while (shift < 8 && (1 << shift) != c->page_size) ++shift;
     if ((1 << shift) != c->page_size) return cudaErrorNotSupported;
     // slots of a sequence, (sequence, head) pairs and pages are counted in 31 bits
-    if ((static_cast<long long>(c->max_pages) << shift) > 0x7fffffffll - 1024 ||
+    if ((static_cast<long long>(c->max_pages) << shift) > 0x7fffffffll - 65536 ||
         static_cast<long long>(c->batch) * c->kv_heads > 0x7fffffffll)
         return cudaErrorNotSupported;
     p->k = c->k;

@@ -419,18 +419,18 @@ def check_evict(c, budget, recent, w, p, seen, before, now):
     k, v, ow, op = before
     nk, nv, nw, npos, nlen = now
     ek, ev, ew, ep = k.clone(), v.clone(), nw.cpu().clone(), npos.cpu().clone()
-    hw, hp = w.cpu().numpy(), p.cpu().numpy()
+    hw, hp, table = w.cpu(), p.cpu(), c.table.cpu()
     for b, n in enumerate(c.lens):
         assert int(nlen[b]) == min(n, budget)
         for h in range(c.H):
-            stay, moves = ref.evict(hw[b, h], hp[b, h], n, budget, recent, int(seen[b]))
+            stay, moves = ref.evict(hw[b, h].numpy(), hp[b, h].numpy(), n, budget, recent, int(seen[b]))
+            to = torch.tensor(stay + [t for _, t in moves], dtype=torch.long)
+            at = torch.tensor(stay + [a for a, _ in moves], dtype=torch.long)
             ew[b, h, :min(n, budget)] = 0
-            for s in stay:
-                ew[b, h, s], ep[b, h, s] = w[b, h, s].item(), int(p[b, h, s])
-            for a, t in moves:
-                ew[b, h, t], ep[b, h, t] = w[b, h, a].item(), int(p[b, h, a])
-                pa, pt = int(c.table[b, a // c.P]), int(c.table[b, t // c.P])
-                ek[pt, h, t % c.P], ev[pt, h, t % c.P] = k[pa, h, a % c.P], v[pa, h, a % c.P]
+            ew[b, h, to], ep[b, h, to] = hw[b, h, at], hp[b, h, at]
+            to, at = to[len(stay):], at[len(stay):]
+            pa, pt = table[b, at // c.P].long(), table[b, to // c.P].long()
+            ek[pt, h, to % c.P], ev[pt, h, to % c.P] = k[pa, h, at % c.P], v[pa, h, at % c.P]
             for got, old in ((nw, ow), (npos, op)):          # behind the new length nothing is written
                 assert ref.same_bits(got[b, h, min(n, budget):], old[b, h, min(n, budget):])
     assert ref.same_bits(nk, ek) and ref.same_bits(nv, ev)
@@ -485,7 +485,9 @@ def test_evict(session, kind, dtype, D, H, page, lens, budget, recent, shuffled,
     check_evict(c, budget, recent, w0, p0, seen, before, now)
 
 
-@pytest.mark.parametrize("n,budget", [(40001, 39999), (40001, 5000), (33000, 17), (8193, 8192)])
+@pytest.mark.parametrize("n,budget", [(40001, 39999), (40001, 5000), (33000, 17), (8193, 8192), (1025, 1000),
+                                      (140001, 139990), (140001, 6000),
+                                      (400001, 399000), (400001, 70000)])   # the last two do not fit shared memory
 def test_evict_long(session, n, budget):
     c = ref.Cache([n, n // 2], 1, 64, 64, BF16)
     w = weights_for("spread", 2, 1, c.slots, seed=n).cuda()
