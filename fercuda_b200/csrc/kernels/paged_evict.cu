@@ -21,10 +21,10 @@
 // read it. When a head can have at most 32 moves (a cache that is cut back every few
 // tokens) the warp also makes them, and one launch does it all.
 //
-// Above (evict_select): a CTA a head, from 48K slots on a cluster of 2 to 8,
+// Above (evict_select): a CTA a head, from 32K slots on a cluster of 2 to 8,
 // with the keys in shared memory, and three digits of 11, 11 and 10 bits counted there; the
 // other CTAs' counts are read through distributed shared memory. Beyond 8 x
-// 48K slots the keys are made again for every pass.
+// 32K slots the keys are made again for every pass.
 //
 // The moves (evict_move): a warp resolves 32 moves at once, a lane each, then
 // copies their rows with kAhead 16-byte loads a lane in flight.
@@ -44,10 +44,12 @@ constexpr uint32_t kAll = 0xffffffffu;
 constexpr int kSmall = 1024;                 // slots that a warp's registers hold
 constexpr int kSelect = 1024;                // threads of a selecting CTA
 constexpr int kWarps = kSelect / 32;
-constexpr int kMostKeys = 48 * 1024;         // keys a CTA holds in shared memory
+constexpr int kMostKeys = 32 * 1024;         // keys a CTA holds in shared memory
+constexpr int kCopies = 3;                   // of the first digit's counts, by lane: less contention
 constexpr int kBins = 2048;
 constexpr int kMove = 256;
 constexpr int kFusedMoves = 32;
+constexpr int kFewDropped = 4;               // slots too many that are found one by one
 
 struct EvictParams {
     int budget, recent, cap;     // cap: moves a (sequence, key head) can have
@@ -181,13 +183,39 @@ __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictPar
         // the largest cut with at least `budget` keys at or above it
         uint32_t cut = 0u;
         int above = n;   // keys >= cut
-        for (int bit = 31; bit >= 0 && above != p.budget; --bit) {
-            const uint32_t next = cut | 1u << bit;
-            int m = 0;
+        if (n - p.budget <= kFewDropped) {
+            // up from the least key, one value at a time
+            for (uint32_t from = 0u;;) {
+                uint32_t least = kAll;
 #pragma unroll
-            for (int i = 0; i < KEYS; ++i) m += key[i] >= next ? 1 : 0;   // next > 0: slots behind n do not count
-            m = __reduce_add_sync(kAll, m);
-            if (m >= p.budget) cut = next, above = m;
+                for (int i = 0; i < KEYS; ++i)
+                    if (32 * i + lane < n && key[i] >= from) least = min(least, key[i]);
+                least = __reduce_min_sync(kAll, least);
+                int m = 0;
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) m += 32 * i + lane < n && key[i] == least ? 1 : 0;
+                m = __reduce_add_sync(kAll, m);
+                cut = least;
+                if (above - m < p.budget || least == kAll) break;
+                above -= m;
+                from = least + 1u;
+            }
+        } else {
+            // bit by bit, from the highest in which keys differ
+            uint32_t differ = 0u, any = __shfl_sync(kAll, key[0], 0);
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) differ |= 32 * i + lane < n ? key[i] ^ any : 0u;
+            differ = __reduce_or_sync(kAll, differ);
+            const int top = 31 - __clz(differ);   // -1: all keys are alike
+            cut = any & ~low_bits(top + 1);
+            for (int bit = top; bit >= 0 && above != p.budget; --bit) {
+                const uint32_t next = cut | 1u << bit;
+                int m[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) m[i & 3] += key[i] >= next ? 1 : 0;   // next > 0: not those behind n
+                const int sum = __reduce_add_sync(kAll, (m[0] + m[1]) + (m[2] + m[3]));
+                if (sum >= p.budget) cut = next, above = sum;
+            }
         }
         const uint32_t held = low_bits((n - lane + 31) >> 5), front = low_bits((p.budget - lane + 31) >> 5);
         uint32_t kept = 0u, equal = 0u;   // bit i: slot 32 i + lane
@@ -254,17 +282,21 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
 }
 
 // grid (cluster CTAs, kv_heads, batch). CTA r of a cluster has the slots [lo,
-// hi), warp w of it the run [a, z) of those: runs are in slot order.
-__global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const EvictParams p, const int room) {
-    extern __shared__ uint32_t s_key[];       // [room], the CTA's keys where they fit
-    __shared__ __align__(8) int s_hist[3][kBins];
+// hi). They are passed over in rounds of 32 slots a thread; the key of slot lo
+// + j lies at word j + 4 (j / 32) of shared memory, so that threads read their
+// 32 in 16-byte pieces without bank conflicts. Without HELD the keys of a
+// round are made again from the arrays.
+template <bool HELD>
+__global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const EvictParams p) {
+    extern __shared__ __align__(16) uint32_t s_key[];
+    __shared__ __align__(8) int s_hist[kCopies + 2][kBins];
     __shared__ int s_scan[32];
     __shared__ int s_digit, s_above, s_here;
     __shared__ int s_eq, s_last;              // read by the cluster's other CTAs, as are the next two
     __shared__ int s_holes, s_movers;
     const cg::cluster_group cluster = cg::this_cluster();
     const int rank = blockIdx.x, ctas = gridDim.x;
-    const int t = threadIdx.x, lane = t & 31, w = t >> 5, b = blockIdx.z;
+    const int t = threadIdx.x, lane = t & 31, b = blockIdx.z;
     const size_t bh = static_cast<size_t>(b) * c.kv_heads + blockIdx.y;
     fer::dev::pdl_begin();
     bool bad;
@@ -280,19 +312,31 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     const int each = ((n - 1) / ctas + 1 + 127) & ~127;
     const int lo = static_cast<int>(min(static_cast<long long>(n), static_cast<long long>(rank) * each));
     const int hi = min(n - lo, each) + lo;
-    const bool held = each <= room;
-    const int run = ((hi - lo + kWarps - 1) / kWarps + 31) & ~31;
-    const int a = min(hi, lo + w * run), z = min(hi, a + run);
-    auto key_at = [&](int j) { return held ? s_key[j - lo] : key_of(h.w[j], h.pos[j], first); };
+    // this thread's 32 slots of a round, `mine` on: fn(i, key); i counts to a constant
+    auto each_key = [&](int mine, auto fn) {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(s_key + (mine - lo) / 32 * 36 + i);
+                fn(i, v.x), fn(i + 1, v.y), fn(i + 2, v.z), fn(i + 3, v.w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int j = min(mine + i, hi - 1);
+                fn(i, key_of(h.w[j], h.pos[j], first));
+            }
+        }
+    };
     auto meet = [&]() {
         if (ctas > 1) cluster.sync();
         else __syncthreads();
     };
-    for (int i = t; i < 3 * kBins; i += kSelect) (&s_hist[0][0])[i] = 0;
+    for (int i = t; i < (kCopies + 2) * kBins; i += kSelect) (&s_hist[0][0])[i] = 0;
     if (t == 0) s_last = -1;
     __syncthreads();
     // keys, and the count of their first digit; kBatch loads in flight
-    constexpr int kBatch = 4;
+    constexpr int kBatch = 8;
     for (int j0 = lo + t; j0 < hi; j0 += kBatch * kSelect) {
         float wt[kBatch];
         int pos[kBatch];
@@ -307,8 +351,8 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
             const int j = j0 + k * kSelect;
             if (j >= hi) break;
             const uint32_t key = key_of(wt[k], pos[k], first);
-            if (held) s_key[j - lo] = key;
-            atomicAdd(&s_hist[0][key >> 21], 1);
+            if constexpr (HELD) s_key[(j - lo) + (j - lo) / 32 * 4] = key;
+            atomicAdd(&s_hist[lane % kCopies][key >> 21], 1);
             if (j < p.budget) {
                 if (h.nw != h.w) h.nw[j] = wt[k];
                 if (h.np != h.pos) h.np[j] = pos[k];
@@ -320,12 +364,20 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
 #pragma unroll
     for (int d = 0; d < 3; ++d) {
         const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bins = d == 2 ? 1024 : 2048;
+        int* hist = s_hist[d == 0 ? 0 : kCopies + d - 1];
         if (d > 0) {
             const uint32_t mask = d == 1 ? 0xffe00000u : 0xfffffc00u;   // the digits found so far
-#pragma unroll 4
-            for (int j = lo + t; j < hi; j += kSelect) {
-                const uint32_t key = key_at(j);
-                if ((key & mask) == cut) atomicAdd(&s_hist[d][(key >> shift) & (bins - 1)], 1);
+            for (int mine = lo + 32 * t; mine < hi; mine += 32 * kSelect)
+                each_key(mine, [&](int i, uint32_t key) {
+                    if ((key & mask) == cut && mine + i < hi) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
+                });
+        } else {
+            __syncthreads();
+            for (int i = t; i < kBins; i += kSelect) {
+                int n0 = hist[i];
+#pragma unroll
+                for (int k = 1; k < kCopies; ++k) n0 += s_hist[k][i];
+                hist[i] = n0;
             }
         }
         meet();
@@ -337,7 +389,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 if (r >= ctas) break;
-                const int2 v = *reinterpret_cast<const int2*>(cluster.map_shared_rank(&s_hist[d][0], r) + bins - kPer * (t + 1));
+                const int2 v = *reinterpret_cast<const int2*>(cluster.map_shared_rank(hist, r) + bins - kPer * (t + 1));
                 count[0] += v.y, count[1] += v.x;
             }
         }
@@ -355,27 +407,34 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         left -= s_above;
         equal = s_here;
         __syncthreads();
+        if (left == equal) break;   // every key that begins like the cut is kept
     }
     // of the slots whose key is the cut the first `left` are kept: those up to `last`
     int last = n;
     if (left < equal) {   // the same for the whole cluster
-        int eq = 0;
-        for (int j = a + lane; j < z; j += 32) eq += key_at(j) == cut ? 1 : 0;
-        eq = __reduce_add_sync(kAll, eq);
-        int total;
-        int before = __shfl_sync(kAll, block_scan(lane == 0 ? eq : 0, s_scan, &total), 0);
-        if (t == 0) s_eq = total;
-        meet();
-        for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&s_eq, r);
-        if (before < left && left <= before + eq) {   // the last one lies in this warp's run
-            for (int j0 = a; j0 < z; j0 += 32) {
-                const uint32_t row = __ballot_sync(kAll, j0 + lane < z && key_at(min(j0 + lane, z - 1)) == cut);
-                if (before + __popc(row) >= left) {
-                    if ((row >> lane & 1u) && before + __popc(row & low_bits(lane)) + 1 == left) s_last = j0 + lane;
-                    break;
-                }
-                before += __popc(row);
+        auto word_of = [&](int mine) {
+            uint32_t word = 0u;
+            if (mine < hi) each_key(mine, [&](int i, uint32_t key) { word |= (key == cut ? 1u : 0u) << i; });
+            return word & low_bits(hi - mine);
+        };
+        int before = 0, total;
+        if (ctas > 1) {
+            int mine = 0;
+            for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) mine += __popc(word_of(r0 + 32 * t));
+            block_scan(mine, s_scan, &total);
+            if (t == 0) s_eq = total;
+            cluster.sync();
+            for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&s_eq, r);
+        }
+        for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) {
+            uint32_t word = word_of(r0 + 32 * t);
+            const int here = __popc(word);
+            const int at = before + block_scan(here, s_scan, &total);
+            if (at < left && left <= at + here) {   // the last one is this thread's
+                for (int k = at + 1; k < left; ++k) word &= word - 1u;
+                s_last = r0 + 32 * t + __ffs(word) - 1;
             }
+            before += total;
         }
         meet();
         for (int r = 0; r < ctas; ++r) {
@@ -383,46 +442,53 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
             if (v >= 0) last = v;
         }
     }
-    auto kept_at = [&](int j) {
-        const uint32_t key = key_at(j);
-        return key > cut || (key == cut && j <= last);
+    // Freed slots before the budget and kept ones behind it: each thread has
+    // its word of kept slots, and one scan of both counts gives its places in
+    // the lists.
+    int holes = 0, movers = 0;    // of this CTA so far
+    auto rounds = [&](int hole0, int mover0, bool list) {
+        for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) {
+            const int mine = r0 + 32 * t;
+            uint32_t word = 0u;
+            if (mine < hi) {
+                each_key(mine, [&](int i, uint32_t key) { word |= (key >= cut ? 1u : 0u) << i; });
+                if (last < mine + 31) {   // equal ones behind the last are not kept
+                    uint32_t equals = 0u;
+                    each_key(mine, [&](int i, uint32_t key) { equals |= (key == cut ? 1u : 0u) << i; });
+                    word &= ~equals | low_bits(last + 1 - mine);
+                }
+            }
+            word &= low_bits(hi - mine);
+            const uint32_t before = low_bits(p.budget - mine);
+            uint32_t hole = ~word & before & low_bits(hi - mine), move = word & ~before;
+            int total;
+            const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
+            if (list) {
+                int h0 = hole0 + holes + (at & 0xffff), m0 = mover0 + movers + (at >> 16);
+                for (; hole; hole &= hole - 1u, ++h0)
+                    if (h0 < p.cap) h.to[h0] = mine + __ffs(hole) - 1;
+                for (; move; move &= move - 1u, ++m0)
+                    if (m0 < p.cap) h.from[m0] = mine + __ffs(move) - 1;
+            }
+            holes += total & 0xffff;
+            movers += total >> 16;
+        }
     };
-    // freed slots before the budget and kept ones behind it, counted, then listed
-    int holes = 0, movers = 0;
-#pragma unroll 4
-    for (int j = a + lane; j < z; j += 32) {
-        const bool kept = kept_at(j);
-        holes += !kept && j < p.budget ? 1 : 0;
-        movers += kept && j >= p.budget ? 1 : 0;
+    int hole0 = 0, mover0 = 0;    // of the CTAs before
+    if (ctas > 1) {
+        rounds(0, 0, false);
+        if (t == 0) s_holes = holes, s_movers = movers;
+        cluster.sync();
+        for (int r = 0; r < rank; ++r) {
+            hole0 += *cluster.map_shared_rank(&s_holes, r);
+            mover0 += *cluster.map_shared_rank(&s_movers, r);
+        }
+        holes = movers = 0;
     }
-    holes = __reduce_add_sync(kAll, holes);
-    movers = __reduce_add_sync(kAll, movers);
-    int all_holes, all_movers;
-    int hole0 = __shfl_sync(kAll, block_scan(lane == 0 ? holes : 0, s_scan, &all_holes), 0);
-    int mover0 = __shfl_sync(kAll, block_scan(lane == 0 ? movers : 0, s_scan, &all_movers), 0);
-    if (t == 0) s_holes = all_holes, s_movers = all_movers;
-    meet();
-    int before_h = 0, before_m = 0;
-    for (int r = 0; r < rank; ++r) {
-        before_h += *cluster.map_shared_rank(&s_holes, r);
-        before_m += *cluster.map_shared_rank(&s_movers, r);
-    }
-    hole0 += before_h;
-    mover0 += before_m;
-#pragma unroll 4
-    for (int j0 = a; j0 < z; j0 += 32) {
-        const int j = j0 + lane;
-        const bool kept = j < z && kept_at(j), front = j < p.budget;
-        const uint32_t hole = __ballot_sync(kAll, j < z && !kept && front), move = __ballot_sync(kAll, kept && !front);
-        const int nh = hole0 + __popc(hole & low_bits(lane)), nm = mover0 + __popc(move & low_bits(lane));
-        if ((hole >> lane & 1u) && nh < p.cap) h.to[nh] = j;
-        if ((move >> lane & 1u) && nm < p.cap) h.from[nm] = j;
-        hole0 += __popc(hole);
-        mover0 += __popc(move);
-    }
+    rounds(hole0, mover0, true);
     // all alike, unless the arrays changed meanwhile
     if (rank == ctas - 1 && t == 0)
-        p.counts[bh] = min(before_m + all_movers, min(before_h + all_holes, p.cap));
+        p.counts[bh] = min(mover0 + movers, min(hole0 + holes, p.cap));
     if (ctas > 1) cluster.sync();   // no CTA leaves while another may read its shared memory
 }
 
@@ -498,22 +564,24 @@ cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
         // which is what one SM takes to read 10,000 more slots
         unsigned ctas = 1;
         while (ctas < 8 && static_cast<long long>(ctas) * kMostKeys < max_slots) ctas *= 2;
-        long long room = ((max_slots - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
-        if (room > kMostKeys) room = 0;
-        int keys = static_cast<int>(room);
+        const int each = ((max_slots - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
+        const bool held = each <= kMostKeys;
+        const size_t smem = held ? static_cast<size_t>(each) / 32 * 36 * 4 : 0;
+        const void* kernel = held ? reinterpret_cast<const void*>(evict_select<true>)
+                                  : reinterpret_cast<const void*>(evict_select<false>);
         static std::atomic<bool> set[kDevices];
         int dev = 0;
         e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
         if (dev >= kDevices || !set[dev].load(std::memory_order_relaxed)) {
-            e = cudaFuncSetAttribute(evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kMostKeys);
+            e = cudaFuncSetAttribute(evict_select<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     kMostKeys / 32 * 36 * 4);
             if (e != cudaSuccess) return e;
             if (dev < kDevices) set[dev].store(true, std::memory_order_relaxed);
         }
         Paged view = c;
-        void* args[] = {&view, &p, &keys};
-        e = launch_cluster(reinterpret_cast<const void*>(evict_select), dim3(ctas, c.kv_heads, batch), kSelect,
-                           4 * static_cast<size_t>(keys), ctas, s, args);
+        void* args[] = {&view, &p};
+        e = launch_cluster(kernel, dim3(ctas, c.kv_heads, batch), kSelect, smem, ctas, s, args);
         if (e != cudaSuccess) return e;
     }
     const dim3 grid((p.cap + kMove - 1) / kMove + (p.cap == 0), c.kv_heads, batch);
