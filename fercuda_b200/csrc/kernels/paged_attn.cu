@@ -47,8 +47,8 @@ namespace {
 using fer::dev::Paged;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kFinish = 256;        // threads of the second kernel
-constexpr int kFinishSlots = 1024;  // slots of weights a CTA of it takes
+constexpr int kFinish = 512;        // threads of the second kernel
+constexpr int kFinishSlots = 2048;  // slots of weights a CTA of it takes
 constexpr int kSegments = 1024;     // entries of the unit table in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -153,8 +153,7 @@ template <int D> struct Cut {
     static constexpr int kRow = 2 * D;                       // bytes
     static constexpr int kStage = 2 * kSlab * kRow;          // keys, then values
     static constexpr int kRing = kWarps * kStages * kStage;
-    template <int NT> static constexpr int merge() { return 2 * 32 * 4 * (NT * (D / 16 * 4 + 4)); }
-    template <int NT> static constexpr int smem() { return kRing + merge<NT>() + 4 * (kSegments + 1); }
+    static constexpr int kSmem = kRing + 4 * (kSegments + 1);
 };
 
 // The units before every segment of sequences; kept in shared memory.
@@ -163,9 +162,9 @@ struct Units {
     int segments, seg;
 };
 
-// One unit, the same for all threads of a warp.
+// One unit.
 struct Unit {
-    int b, hk, blk, chunk, chunks, k0, n;
+    int b, hk, blk, chunk, chunks, n;   // n: slots
 };
 
 __device__ __forceinline__ Unit find_unit(const Paged& c, const AttnParams& p, const Units& t, int u) {
@@ -192,10 +191,31 @@ __device__ __forceinline__ Unit find_unit(const Paged& c, const AttnParams& p, c
     x.chunk = r - hb * nch;
     x.hk = hb / p.blocks;
     x.blk = hb - x.hk * p.blocks;
-    x.k0 = x.chunk * p.chunk;
-    x.n = min(p.chunk, len - x.k0);
+    x.n = min(p.chunk, len - x.chunk * p.chunk);
     return x;
 }
+
+// The units of a run, found 32 at a time, one a lane, and handed to the whole
+// warp one by one.
+struct UnitRun {
+    int from = -1;   // unit of lane 0
+    Unit x{};
+    __device__ __forceinline__ Unit get(const Paged& c, const AttnParams& p, const Units& t, int u, int last) {
+        if (from < 0 || u >= from + 32) {
+            from = u;
+            x = find_unit(c, p, t, min(u + static_cast<int>(threadIdx.x & 31), last));
+        }
+        const int i = u - from;
+        Unit y;
+        y.b = __shfl_sync(0xffffffffu, x.b, i);
+        y.hk = __shfl_sync(0xffffffffu, x.hk, i);
+        y.blk = __shfl_sync(0xffffffffu, x.blk, i);
+        y.chunk = __shfl_sync(0xffffffffu, x.chunk, i);
+        y.chunks = __shfl_sync(0xffffffffu, x.chunks, i);
+        y.n = __shfl_sync(0xffffffffu, x.n, i);
+        return y;
+    }
+};
 
 // Page ids of a unit's chunk (up to 64 pages): lane i holds those of its i-th
 // and (i + 32)-th page, -1 where no slot is held or the table has no page.
@@ -212,11 +232,11 @@ struct ChunkPages {
     }
 };
 
-__device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x) {
+__device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x, int k0) {
     const int lane = threadIdx.x & 31, last = (x.n - 1) >> c.shift;
     ChunkPages g{-1, -1};
-    if (lane <= last) g.a = c.page(x.b, x.k0 + (lane << c.shift));
-    if (lane + 32 <= last) g.b = c.page(x.b, x.k0 + ((lane + 32) << c.shift));
+    if (lane <= last) g.a = c.page(x.b, k0 + (lane << c.shift));
+    if (lane + 32 <= last) g.b = c.page(x.b, k0 + ((lane + 32) << c.shift));
     return g;
 }
 
@@ -229,8 +249,8 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
     constexpr int kSub = C::kSlab / 16;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_sum[kWarps];
-    float* merge = reinterpret_cast<float*>(smem + C::kRing);
-    int* cum = reinterpret_cast<int*>(smem + C::kRing + C::template merge<NT>());
+    __shared__ float s_ml[kWarps][8 * NT][2];
+    int* cum = reinterpret_cast<int*>(smem + C::kRing);
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     fer::dev::pdl_begin();
 
@@ -280,34 +300,41 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
     const int u1 = static_cast<int>(static_cast<long long>(total) * (blockIdx.x + 1) / gridDim.x);
     if (u0 >= u1) return;
 
-    const uint32_t ring = fer::dev::smem_addr(smem) + w * C::kStages * C::kStage;
+    uint8_t* const my_ring = smem + w * C::kStages * C::kStage;
+    const uint32_t ring = fer::dev::smem_addr(my_ring);
     const T* kc = static_cast<const T*>(c.k);
     const T* vc = static_cast<const T*>(c.v);
 
-    // what is being loaded: unit lu, slab li of it; its pages, and the next unit's on their way
+    // What is being loaded: unit lu, slab li of it; its pages, and the next
+    // unit's on their way. Bit i of `broken`: the slab in stage i is of a unit
+    // with a page id out of range.
+    UnitRun load_run, run;
     int lu = u0, li = w, loads = 0;
-    Unit lx = find_unit(c, p, table, u0);
-    ChunkPages lp = load_pages(c, lx);
-    Unit nx = lx;
-    ChunkPages np = lp;
-    if (u0 + 1 < u1) {
-        nx = find_unit(c, p, table, u0 + 1);
-        np = load_pages(c, nx);
-    }
+    uint32_t broken = 0u;
+    Unit lx = load_run.get(c, p, table, u0, u1 - 1), nx = lx;
+    ChunkPages lp = load_pages(c, lx, lx.chunk * p.chunk), np = lp;
+    bool lgood = true;
+    auto look_ahead = [&]() {
+        lgood = lp.all_good(c, lx.n);
+        if (!lgood && w == 0 && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+        if (lu + 1 < u1) {
+            nx = load_run.get(c, p, table, lu + 1, u1 - 1);
+            np = load_pages(c, nx, nx.chunk * p.chunk);
+        }
+    };
+    look_ahead();
     auto issue = [&]() {
         while (lu < u1 && li * C::kSlab >= lx.n) {   // no slab of this unit is left for this warp
-            ++lu;
             li = w;
             lx = nx;
             lp = np;
-            if (lu + 1 < u1) {
-                nx = find_unit(c, p, table, lu + 1);
-                np = load_pages(c, nx);
-            }
+            if (++lu < u1) look_ahead();
         }
         if (lu < u1) {
-            const uint32_t st = ring + (loads % C::kStages) * C::kStage;
+            const int stage = loads % C::kStages;
+            const uint32_t st = ring + stage * C::kStage;
             const int piece = lane % kPieces;
+            broken = (broken & ~(1u << stage)) | (lgood ? 0u : 1u << stage);
 #pragma unroll
             for (int i = 0; i < C::kSlab / kRowsPer; ++i) {
                 const int r = i * kRowsPer + lane / kPieces;
@@ -327,36 +354,40 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
 #pragma unroll
     for (int i = 0; i < C::kStages - 1; ++i) issue();
 
+    // Queries as columns (heads lane / 4) of rows (dims 2 (lane % 4) + {0, 1}
+    // and 8 more); those of the next unit are loaded a unit ahead where the
+    // registers allow it.
+    constexpr bool kAhead = NT * kB <= 8;
+    uint32_t qf[NT][kB][2], qn[NT][kB][2];
+    auto load_q = [&](const Unit& x, uint32_t (&q)[NT][kB][2]) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int g = x.blk * 8 * NT + nt * 8 + lane / 4;
+            const bool real = g < p.group;
+            const T* row = static_cast<const T*>(p.q) + x.b * p.qs + (static_cast<size_t>(x.hk) * p.group + (real ? g : 0)) * D;
+            const bool even = (reinterpret_cast<uintptr_t>(row) & 3) == 0;
+#pragma unroll
+            for (int k = 0; k < kB; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint16_t* at = reinterpret_cast<const uint16_t*>(row + 16 * k + 8 * e + 2 * (lane & 3));
+                    uint32_t v;
+                    if (even) v = *reinterpret_cast<const uint32_t*>(at);
+                    else v = at[0] | static_cast<uint32_t>(at[1]) << 16;
+                    q[nt][k][e] = real ? v : 0u;
+                }
+        }
+    };
     int used = 0;
-    uint32_t qf[NT][kB][2];
-    int last_b = -1, last_hk = -1, last_blk = -1;
+    Unit x = run.get(c, p, table, u0, u1 - 1);
+    load_q(x, qf);
     for (int u = u0; u < u1; ++u) {
-        const Unit x = find_unit(c, p, table, u);
         const int h0 = x.hk * p.group + x.blk * 8 * NT;          // first head of the block
         const int nh = min(8 * NT, p.group - x.blk * 8 * NT);    // its heads
-        if (x.b != last_b || x.hk != last_hk || x.blk != last_blk) {
-            last_b = x.b, last_hk = x.hk, last_blk = x.blk;
-            // columns (heads) lane / 4, rows (dims) 2 (lane % 4) + {0, 1} and 8 more
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int g = nt * 8 + lane / 4;
-                const T* q = static_cast<const T*>(p.q) + x.b * p.qs + static_cast<size_t>(h0 + (g < nh ? g : 0)) * D;
-                const bool even = (reinterpret_cast<uintptr_t>(q) & 3) == 0;
-#pragma unroll
-                for (int k = 0; k < kB; ++k)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint16_t* at = reinterpret_cast<const uint16_t*>(q + 16 * k + 8 * e + 2 * (lane & 3));
-                        uint32_t v;
-                        if (even) v = *reinterpret_cast<const uint32_t*>(at);
-                        else v = at[0] | static_cast<uint32_t>(at[1]) << 16;
-                        qf[nt][k][e] = g < nh ? v : 0u;
-                    }
-            }
-        }
-        const ChunkPages pg = load_pages(c, x);
-        const bool good = pg.all_good(c, x.n);
-        if (!good && w == 0 && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+        const int k0 = x.chunk * p.chunk;
+        const Unit next = u + 1 < u1 ? run.get(c, p, table, u + 1, u1 - 1) : x;
+        const bool turn = next.b != x.b || next.hk != x.hk || next.blk != x.blk;
+        if (kAhead && turn) load_q(next, qn);
 
         float m[NT][2], l[NT][2], o[NT][kB][4];
 #pragma unroll
@@ -367,6 +398,7 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
             for (int k = 0; k < kB; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.0f;
         }
         for (int i = w; i * C::kSlab < x.n; i += kWarps) {
+            const bool good = !(broken >> (used % C::kStages) & 1u);
             cp_wait<C::kStages - 2>();
             __syncwarp();
             issue();
@@ -397,6 +429,7 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
                 const int j = i * C::kSlab + sub * 16 + lane / 4;   // this lane's slots of the chunk: j, j + 8
                 bool on0 = j < x.n, on1 = j + 8 < x.n;
                 if (!good) {
+                    const ChunkPages pg = load_pages(c, x, k0);
                     const int p0 = pg.of(c, min(j, x.n - 1)), p1 = pg.of(c, min(j + 8, x.n - 1));
                     on0 = on0 && p0 >= 0;
                     on1 = on1 && p1 >= 0;
@@ -422,7 +455,7 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             const int g = nt * 8 + 2 * (lane & 3) + e;
-                            float* row = p.scores + (static_cast<size_t>(x.b) * p.heads + h0 + g) * c.max_slots() + x.k0;
+                            float* row = p.scores + (static_cast<size_t>(x.b) * p.heads + h0 + g) * c.max_slots() + k0;
                             if (g < nh && j < x.n) row[j] = s[nt][e];
                             if (g < nh && j + 8 < x.n) row[j + 8] = s[nt][2 + e];
                         }
@@ -471,7 +504,12 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
             }
         }
 
-        // the warps' parts: 2 and 3 into 0 and 1, then 1 into 0
+        // The warps' parts meet in shared memory: each warp's o, a row of dims a
+        // head, in the stage of its ring that nothing is loaded into before
+        // its next slab. Eights of dims are swapped by head pair against bank conflicts.
+        float* const my_o = reinterpret_cast<float*>(my_ring + ((used + C::kStages - 1) % C::kStages) * C::kStage);
+        static_assert(8 * NT * D * 4 <= C::kStage);
+        __syncwarp();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -479,109 +517,103 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
-            }
-        constexpr int kRegs = NT * (kB * 4 + 4);
-#pragma unroll
-        for (int half = 2; half >= 1; half >>= 1) {
-            float* slot = merge + (w & 1) * kRegs * 32 + lane;
-            if (w >= half && w < 2 * half) {
-                float* at = half == 2 ? slot : merge + lane;
-                int i = 0;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        at[32 * i++] = m[nt][e];
-                        at[32 * i++] = l[nt][e];
-                    }
-#pragma unroll
-                    for (int k = 0; k < kB; ++k)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) at[32 * i++] = o[nt][k][e];
+                const int g = nt * 8 + 2 * (lane & 3) + e;
+                if (g >= nh) continue;
+                if (lane < 4) {
+                    s_ml[w][g][0] = m[nt][e];
+                    s_ml[w][g][1] = l[nt][e];
                 }
+#pragma unroll
+                for (int k = 0; k < kB; ++k)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        my_o[g * D + ((16 * k + 8 * r + lane / 4) ^ ((lane & 3) << 3))] = o[nt][k][2 * r + e];
             }
-            __syncthreads();
-            if (w < half) {
-                const float* at = half == 2 ? slot : merge + lane;
-                int i = 0;
+        if (lane == 0) s_sum[w] = used;
+        __syncthreads();
+        const float* part[kWarps];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float fa[2], fb[2];
+        for (int i = 0; i < kWarps; ++i)
+            part[i] = reinterpret_cast<const float*>(smem + (i * C::kStages + (s_sum[i] + C::kStages - 1) % C::kStages) * C::kStage);
+        const bool whole = x.chunks == 1;
+        const size_t bh0 = static_cast<size_t>(x.b) * p.heads + h0;
+        for (int i = t; i < nh * (D / 4); i += kThreads) {
+            const int g = i / (D / 4), d = i % (D / 4) * 4;
+            float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float om = at[32 * i++], ol = at[32 * i++];
-                        const float top = fmaxf(m[nt][e], om), base = top == -INFINITY ? 0.0f : top;
-                        fa[e] = ex2(m[nt][e] - base);
-                        fb[e] = ex2(om - base);
-                        m[nt][e] = top;
-                        l[nt][e] = l[nt][e] * fa[e] + ol * fb[e];
-                    }
+            for (int v = 0; v < kWarps; ++v) top = fmaxf(top, s_ml[v][g][0]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (int k = 0; k < kB; ++k)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            o[nt][k][e] = o[nt][k][e] * fa[e & 1] + at[32 * i++] * fb[e & 1];
-                }
+            for (int v = 0; v < kWarps; ++v) {
+                const float f = ex2(s_ml[v][g][0] - base);
+                const float4 y = *reinterpret_cast<const float4*>(part[v] + g * D + (d ^ ((g >> 1 & 3) << 3)));
+                sum += s_ml[v][g][1] * f;
+                a.x += y.x * f, a.y += y.y * f, a.z += y.z * f, a.w += y.w * f;
             }
-            __syncthreads();
-        }
-        if (w == 0) {
             constexpr float kBack = 1.0f / kScaleP<T>;
+            const size_t at = (bh0 + g) * p.chunks + x.chunk;
+            if (d == 0) {
+                p.part_ml[2 * at] = top;
+                p.part_ml[2 * at + 1] = sum;
+                if (whole && p.lse) p.lse[bh0 + g] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+            }
+            if (whole) {
+                const float f = sum == 0.0f ? 0.0f : kBack / sum;
+                T* out = static_cast<T*>(p.out) + x.b * p.os + static_cast<size_t>(h0 + g) * D + d;
+                const float v[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int g = nt * 8 + 2 * (lane & 3) + e;
-                    if (g >= nh) continue;
-                    const size_t bh = static_cast<size_t>(x.b) * p.heads + h0 + g;
-                    const size_t at = bh * p.chunks + x.chunk;
-                    const bool whole = x.chunks == 1;
-                    const float inv = l[nt][e] == 0.0f ? 0.0f : 1.0f / l[nt][e];
-                    if (lane < 4) {
-                        p.part_ml[2 * at] = m[nt][e];
-                        p.part_ml[2 * at + 1] = l[nt][e];
-                        if (whole && p.lse)
-                            p.lse[bh] = l[nt][e] == 0.0f ? -INFINITY : (m[nt][e] + log2f(l[nt][e])) * kLn2;
-                    }
-                    T* out = static_cast<T*>(p.out) + x.b * p.os + static_cast<size_t>(h0 + g) * D;
-                    float* po = p.part_o + at * D;
-#pragma unroll
-                    for (int k = 0; k < kB; ++k)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const int d = 16 * k + 8 * r + lane / 4;
-                            const float v = o[nt][k][2 * r + e] * kBack;
-                            if (whole) out[d] = static_cast<T>(l[nt][e] == 0.0f ? 0.0f : v * inv);
-                            else po[d] = v;
-                        }
-                }
+                for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(sum == 0.0f ? 0.0f : v[e] * f);
+            } else {
+                *reinterpret_cast<float4*>(p.part_o + at * D + d) =
+                    make_float4(a.x * kBack, a.y * kBack, a.z * kBack, a.w * kBack);
+            }
         }
+        __syncthreads();
+        if (turn) {
+            if constexpr (kAhead) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < kB; ++k) qf[nt][k][0] = qn[nt][k][0], qf[nt][k][1] = qn[nt][k][1];
+            } else {
+                load_q(next, qf);
+            }
+        }
+        x = next;
     }
     cp_wait<0>();
 }
 
 // log2 of a head's total sum of powers, from its chunks' (m, l), by one warp;
-// -inf where nothing counts. The maximum's base goes to *base.
+// -inf where nothing counts. The base of the sum, and the sum, go to the two
+// others.
 __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float* base, float* sum) {
     const int lane = threadIdx.x & 31;
-    float top = -INFINITY;
-    for (int i = lane; i < chunks; i += 32) top = fmaxf(top, ml[2 * i]);
+    float top = -INFINITY, l = 0.0f;
+    for (int i = lane; i < chunks; i += 32) {
+        const float2 v = *reinterpret_cast<const float2*>(ml + 2 * i);
+        const float next = fmaxf(top, v.x), b = next == -INFINITY ? 0.0f : next;
+        l = l * ex2(top - b) + v.y * ex2(v.x - b);
+        top = next;
+    }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float b = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
-    for (int i = lane; i < chunks; i += 32) l += ml[2 * i + 1] * ex2(ml[2 * i] - b);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    *base = b;
+    for (int off = 16; off > 0; off >>= 1) {
+        const float ot = __shfl_xor_sync(0xffffffffu, top, off), ol = __shfl_xor_sync(0xffffffffu, l, off);
+        const float next = fmaxf(top, ot), b = next == -INFINITY ? 0.0f : next;
+        // the same sum in both lanes of a pair
+        l = l * ex2(top - b) + ol * ex2(ot - b);
+        top = next;
+    }
+    *base = top == -INFINITY ? 0.0f : top;
     *sum = l;
-    return l == 0.0f ? -INFINITY : b + log2f(l);
+    return l == 0.0f ? -INFINITY : *base + log2f(l);
 }
 
 // grid (group + weight tiles, kv_heads, n_seq). The first `group` CTAs of a
 // (key head, sequence) add one head's chunks each (in order within a warp,
 // then the warps in order); the others add probabilities to kFinishSlots
-// slots' weights each.
+// slots' weights each, four slots a thread.
 template <typename T, int D>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
     constexpr int kW = kFinish / 32, kV = D / 32;    // warps; dims a lane
@@ -598,25 +630,26 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
         if (chunks <= 1) return;                      // written already
         const size_t bh = bh0 + blockIdx.x;
         const float* ml = p.part_ml + 2 * bh * p.chunks;
-        const float* po = p.part_o + bh * p.chunks * D;
+        const float* po = p.part_o + bh * p.chunks * D + lane;
         float base, l;
         const float lse2 = chunks_lse2(ml, chunks, &base, &l);
         float o[kV];
 #pragma unroll
         for (int e = 0; e < kV; ++e) o[e] = 0.0f;
+        if (w < chunks) {
 #pragma unroll 4
-        for (int i = w; i < chunks; i += kW) {
-            const float f = ex2(ml[2 * i] - base);
+            for (int i = w; i < chunks; i += kW) {
+                const float f = ex2(ml[2 * i] - base);
 #pragma unroll
-            for (int e = 0; e < kV; ++e) o[e] = fmaf(po[static_cast<size_t>(i) * D + e * 32 + lane], f, o[e]);
+                for (int e = 0; e < kV; ++e) o[e] = fmaf(po[static_cast<size_t>(i) * D + e * 32], f, o[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < kV; ++e) s_o[w][e * 32 + lane] = o[e];
         }
-#pragma unroll
-        for (int e = 0; e < kV; ++e) s_o[w][e * 32 + lane] = o[e];
         __syncthreads();
         for (int d = t; d < D; d += kFinish) {
             float v = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kW; ++i) v += s_o[i][d];
+            for (int i = 0; i < min(kW, chunks); ++i) v += s_o[i][d];
             static_cast<T*>(p.out)[b * p.os + (static_cast<size_t>(hk) * p.group + blockIdx.x) * D + d] =
                 static_cast<T>(l == 0.0f ? 0.0f : v / l);
         }
@@ -625,11 +658,10 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
     }
     const int j0 = (blockIdx.x - p.group) * kFinishSlots;
     if (j0 >= len) return;
-    const size_t most = static_cast<size_t>(c.max_slots());
-    constexpr int kEach = kFinishSlots / kFinish;
-    float sum[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) sum[e] = 0.0f;
+    const int j = j0 + 4 * t;
+    const size_t most = static_cast<size_t>(c.max_slots());   // a multiple of 8: rows start at 16 bytes
+    static_assert(kFinishSlots == 4 * kFinish);
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int g0 = 0; g0 < p.group; g0 += kFinish) {
         const int ng = min(kFinish, p.group - g0);
         __syncthreads();
@@ -639,21 +671,27 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
             if (lane == 0) s_lse[g] = v;
         }
         __syncthreads();
+        if (j >= len) continue;
+#pragma unroll 4
         for (int g = 0; g < ng; ++g) {
-            if (s_lse[g] == -INFINITY) continue;
-            const float* row = p.scores + (bh0 + g0 + g) * most;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                const int j = j0 + e * kFinish + t;
-                if (j < len) sum[e] += ex2(row[j] - s_lse[g]);
-            }
+            const float4 s = *reinterpret_cast<const float4*>(p.scores + (bh0 + g0 + g) * most + j);
+            const float lse2 = s_lse[g];
+            if (lse2 == -INFINITY) continue;
+            sum[0] += ex2(s.x - lse2);
+            sum[1] += ex2(s.y - lse2);
+            sum[2] += ex2(s.z - lse2);
+            sum[3] += ex2(s.w - lse2);
         }
     }
-    float* out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most;
+    float* out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most + j;
+    if (j + 3 < len && reinterpret_cast<uintptr_t>(p.weights) % 16 == 0) {
+        float4 v = *reinterpret_cast<float4*>(out);
+        v.x += sum[0], v.y += sum[1], v.z += sum[2], v.w += sum[3];
+        *reinterpret_cast<float4*>(out) = v;
+    } else {
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        const int j = j0 + e * kFinish + t;
-        if (j < len) out[j] += sum[e];
+        for (int e = 0; e < 4; ++e)
+            if (j + e < len) out[e] += sum[e];
     }
 }
 
@@ -675,7 +713,7 @@ int resident(const void* kernel, int smem, std::atomic<int>* known) {
 template <typename T, int D, int NT>
 cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     using fer::host::launch_pdl;
-    constexpr int smem = Cut<D>::template smem<NT>();
+    constexpr int smem = Cut<D>::kSmem;
     static std::atomic<int> known[kDevices];
     const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT>), smem, known);
     if (ctas <= 0) return cudaErrorInvalidConfiguration;

@@ -499,6 +499,20 @@ def test_evict_long(session, n, budget):
     check_evict(c, budget, min(budget, 128), w0, p0, i32(c.lens), before, (c.k, c.v, w, p, c.lengths))
 
 
+@pytest.mark.parametrize("n", [900, 5003])
+def test_evict_arrays_at_odd_addresses(session, n):
+    """Weights and positions that start 4 bytes behind a 16-byte boundary."""
+    c = ref.Cache([n, n - 7], 2, 64, 32, F16)
+    w0 = weights_for("ties", 2, 2, c.slots).cuda()
+    p0 = torch.arange(c.slots, dtype=torch.int32, device="cuda").repeat(2, 2, 1)
+    before = (c.k.cpu().clone(), c.v.cpu().clone(), w0.clone(), p0.clone())
+    room = [torch.empty(w0.numel() + 1, dtype=t, device="cuda") for t in (torch.float32, torch.int32)]
+    w, p = (r[1:].view(w0.shape) for r in room)
+    w.copy_(w0), p.copy_(p0)
+    run_evict(session, c, n // 2, 50, w, p, c.lengths.clone())
+    check_evict(c, n // 2, 50, w0, p0, i32(c.lens), before, (c.k, c.v, w, p, c.lengths))
+
+
 def test_more_recent_slots_than_the_budget(session):
     """Positions that claim to be recent everywhere: the lowest slots are kept."""
     c = ref.Cache([50], 1, 64, 16, BF16)
