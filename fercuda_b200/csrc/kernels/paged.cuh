@@ -18,7 +18,7 @@ struct Paged {
     int max_pages, pages, kv_heads, head_dim;
     int shift;   // log2 of the page size
 
-    __device__ __forceinline__ int page_size() const { return 1 << shift; }
+    __host__ __device__ __forceinline__ int page_size() const { return 1 << shift; }
     __host__ __device__ __forceinline__ int max_slots() const { return max_pages << shift; }
     // A sequence's length, clamped to what its row of the table can hold.
     __device__ __forceinline__ int length(int b, bool* bad) const {

@@ -7,17 +7,16 @@
 //
 // Split. A sequence's slots are cut into chunks at fixed places; a unit of
 // work is (sequence, key head, block of 8 or 16 query heads, chunk). Every CTA
-// counts the units from the lengths and takes an equal, contiguous run of
-// them, so ragged batches and tables much wider than the lengths are shared
+// counts the units and their cost from the lengths and takes a contiguous run
+// of equal cost, so ragged batches and tables much wider than the lengths are shared
 // out evenly without the host knowing the lengths. A unit's maximum m, l = sum
 // 2^(s - m) and o = sum 2^(s - m) v go to the workspace in f32 (or, with one
 // chunk, the result to the output), and a second kernel adds a head's chunks
 // in order. Which CTA took a unit does not change its arithmetic: results are
 // the same run to run and for any batch.
 //
-// Inside a unit each of four warps takes every fourth slab of 16 (head_dim 64:
-// 32) slots through a ring of its own, filled by 16-byte asynchronous copies
-// that run on into the next unit; no barrier but the one at a unit's end.
+// Inside a unit each of four warps takes every fourth slab of 16 slots through a ring of its own, filled by tensor copies of page rows
+// that run on into the next unit; the warps meet at a unit's end only.
 // Scores are S^T = K Q^T and outputs O^T = V^T P on 16-bit tensor-core tiles
 // with f32 accumulation: with slots as rows the 8 columns are the heads, so a
 // group of up to 8 heads wastes nothing it would have to read, and the
@@ -35,6 +34,7 @@
 // its exponents, so no inf - inf); l = 0 over all chunks gives zeros.
 #include "paged.cuh"
 #include "pdl.cuh"
+#include "tmap.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -47,9 +47,7 @@ namespace {
 using fer::dev::Paged;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kFinish = 512;        // threads of the second kernel
-constexpr int kFinishSlots = 2048;  // slots of weights a CTA of it takes
-constexpr int kSegments = 1024;     // entries of the unit table in shared memory
+constexpr int kSegments = 256;      // entries of the unit table in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -76,14 +74,13 @@ __device__ __forceinline__ float ex2(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
-    const int n = take ? 16 : 0;   // 0: the 16 bytes are zeroed
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Tensor copy of a box of rows of one page: 64 dims from x, rows from r.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int r, int head, int page,
+                                         uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r), "r"(head), "r"(page), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -146,21 +143,80 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     }
 }
 
-// How a head_dim is cut: slots a slab, slabs in flight a warp.
+// How a head_dim is cut: slots a slab, slabs in flight a warp, CTAs an SM. A
+// slab's rows lie in bands of 64 dims, each as the copies write it: piece c
+// (16 bytes) of row r at r * 128 + ((c ^ (r % 8)) * 16), so eight rows' pieces
+// of one column are in different banks.
 template <int D> struct Cut {
-    static constexpr int kSlab = D == 64 ? 32 : 16;
+    static constexpr int kSlab = 16;
     static constexpr int kStages = D == 256 ? 2 : 3;
-    static constexpr int kRow = 2 * D;                       // bytes
-    static constexpr int kStage = 2 * kSlab * kRow;          // keys, then values
+    template <int NT> static constexpr int ctas() { return D == 64 ? (NT == 1 ? 4 : 3) : D == 128 ? 2 : 1; }
+    static constexpr int kBand = kSlab * 128;
+    static constexpr int kHalf = D / 64 * kBand;             // keys; the values follow
+    static constexpr int kStage = 2 * kHalf;
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kSmem = kRing + 4 * (kSegments + 1);
+    static constexpr int kSmem = kRing + 1024;               // bands start at 1024 bytes
+    // Byte of piece c of row r in a half of a stage.
+    static __device__ __forceinline__ uint32_t at(int r, int c) {
+        return (c >> 3) * kBand + r * 128 + (((c ^ r) & 7) << 4);
+    }
 };
 
-// The units before every segment of sequences; kept in shared memory.
+// What a unit costs, in rounds of a slab for each warp: its rounds, and about
+// one more for its beginning and its end (measured: 2100 to 2450 cycles a
+// round, 1400 to 2000 around them).
+constexpr int kRound = 16 * kWarps;   // slots
+__host__ __device__ inline int rounds_of(int n) { return (n + kRound - 1) / kRound; }
+
+// The units and the cost before every segment of sequences; in shared memory.
 struct Units {
-    const int* cum;   // [segments + 1]
+    const int* units;
+    const int* cost;   // both [segments], ascending
     int segments, seg;
+
+    // The last segment that starts at or before v.
+    __device__ __forceinline__ int find(const int* list, int v) const {
+        int lo = 0, hi = segments;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (list[mid] <= v) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
 };
+
+// One sequence's units: head blocks, chunks of each, and the cost of a block.
+struct Seq {
+    int len, chunks, heads;
+    __device__ __forceinline__ Seq(const Paged& c, const AttnParams& p, int b) {
+        bool bad;
+        len = c.length(b, &bad);
+        chunks = (len + p.chunk - 1) / p.chunk;
+        heads = c.kv_heads * p.blocks;
+    }
+    __device__ __forceinline__ int units() const { return chunks * heads; }
+    __device__ __forceinline__ int block_cost() const { return rounds_of(len) + chunks; }
+    __device__ __forceinline__ int cost() const { return block_cost() * heads; }
+};
+
+// The first unit whose cost begins at or behind x.
+__device__ __forceinline__ int unit_at(const Paged& c, const AttnParams& p, const Units& t, int x) {
+    const int s = t.find(t.cost, x);
+    int u = t.units[s];
+    x -= t.cost[s];
+    for (int b = s * t.seg; b < min(p.n_seq, (s + 1) * t.seg); ++b) {
+        const Seq q(c, p, b);
+        if (x < q.cost()) {
+            const int block = x / q.block_cost(), rest = x - block * q.block_cost();
+            const int each = rounds_of(p.chunk) + 1;
+            return u + block * q.chunks + min((rest + each - 1) / each, q.chunks);
+        }
+        x -= q.cost();
+        u += q.units();
+    }
+    return u;
+}
 
 // One unit.
 struct Unit {
@@ -168,30 +224,22 @@ struct Unit {
 };
 
 __device__ __forceinline__ Unit find_unit(const Paged& c, const AttnParams& p, const Units& t, int u) {
-    int lo = 0, hi = t.segments;            // the last segment that starts at or before u
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (t.cum[mid] <= u) lo = mid;
-        else hi = mid;
-    }
-    int r = u - t.cum[lo];
-    int b = lo * t.seg, len = 0, nch = 0;
-    bool bad;
-    for (;; ++b) {
-        len = c.length(b, &bad);
-        nch = (len + p.chunk - 1) / p.chunk;
-        const int here = nch * c.kv_heads * p.blocks;
-        if (r < here || b + 1 >= p.n_seq) break;
-        r -= here;
+    const int s = t.find(t.units, u);
+    int r = u - t.units[s];
+    int b = s * t.seg;
+    Seq q(c, p, b);
+    while (r >= q.units() && b + 1 < p.n_seq) {
+        r -= q.units();
+        q = Seq(c, p, ++b);
     }
     Unit x;
     x.b = b;
-    x.chunks = nch;
-    const int hb = r / nch;
-    x.chunk = r - hb * nch;
+    x.chunks = q.chunks;
+    const int hb = q.chunks > 0 ? r / q.chunks : 0;
+    x.chunk = r - hb * q.chunks;
     x.hk = hb / p.blocks;
     x.blk = hb - x.hk * p.blocks;
-    x.n = min(p.chunk, len - x.chunk * p.chunk);
+    x.n = min(p.chunk, q.len - x.chunk * p.chunk);
     return x;
 }
 
@@ -241,118 +289,97 @@ __device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x, 
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
+    attn_units(const Paged c, const AttnParams p, const __grid_constant__ CUtensorMap k_map,
+               const __grid_constant__ CUtensorMap v_map) {
     using C = Cut<D>;
     constexpr int kB = D / 16;                  // 16-wide blocks of a row
-    constexpr int kPieces = D / 8;              // 16-byte pieces of a row
-    constexpr int kRowsPer = 32 / kPieces;      // rows a warp copies at once
-    constexpr int kSub = C::kSlab / 16;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int s_sum[kWarps];
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int s_units[kSegments], s_cost[kSegments], s_sum[kWarps], s_cost_sum[kWarps];
     __shared__ float s_ml[kWarps][8 * NT][2];
-    int* cum = reinterpret_cast<int*>(smem + C::kRing);
+    __shared__ uint64_t s_full[kWarps][C::kStages];
+    uint8_t* const smem = smem_raw + (-fer::dev::smem_addr(smem_raw) & 1023u);
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    if (lane == 0) {
+        for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&s_full[w][i], 1);
+        fer::dev::fence_mbar_init();
+    }
+    if (t == 0) {
+        fer::dev::prefetch_tmap(&k_map);
+        fer::dev::prefetch_tmap(&v_map);
+    }
     fer::dev::pdl_begin();
 
-    // how many units each segment of sequences has, and the sums before them
-    Units table{cum, 0, 0};
+    // how many units each segment of sequences has and what they cost, and the sums before them
+    Units table{s_units, s_cost, 0, 0};
     table.seg = (p.n_seq + kSegments - 1) / kSegments;
     table.segments = (p.n_seq + table.seg - 1) / table.seg;
+    int cost_carry = 0;
     int carry = 0;
     for (int s0 = 0; s0 < table.segments; s0 += kThreads) {
         int mine = 0;
+        int cost = 0;
         const int s = s0 + t;
         if (s < table.segments) {
             for (int b = s * table.seg; b < min(p.n_seq, (s + 1) * table.seg); ++b) {
-                bool bad;
-                const int len = c.length(b, &bad);
-                if (bad && blockIdx.x == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
-                mine += (len + p.chunk - 1) / p.chunk * c.kv_heads * p.blocks;
+                const Seq q(c, p, b);
+                mine += q.units();
+                cost += q.cost();
             }
         }
         int x = mine;
+        int y = cost;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x, off);
-            if (lane >= off) x += y;
+            const int x1 = __shfl_up_sync(0xffffffffu, x, off);
+            const int y1 = __shfl_up_sync(0xffffffffu, y, off);
+            if (lane >= off) x += x1, y += y1;
         }
-        if (lane == 31) s_sum[w] = x;
+        if (lane == 31) s_sum[w] = x, s_cost_sum[w] = y;
         __syncthreads();
-        int before = carry;
+        x += carry - mine;
+        y += cost_carry - cost;
         for (int i = 0; i < kWarps; ++i) {
-            if (i < w) before += s_sum[i];
+            if (i < w) x += s_sum[i], y += s_cost_sum[i];
             carry += s_sum[i];
+            cost_carry += s_cost_sum[i];
         }
-        if (s < table.segments) cum[s] = before + x - mine;
+        if (s < table.segments) s_units[s] = x, s_cost[s] = y;
         __syncthreads();
     }
-    const int total = carry;
     // sequences that hold nothing have no unit: their results are written here
     for (int b = blockIdx.x; b < p.n_seq; b += gridDim.x) {
         bool bad;
-        if (c.length(b, &bad) > 0) continue;
+        const int len = c.length(b, &bad);
+        if (bad && t == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+        if (len > 0) continue;
         T* o = static_cast<T*>(p.out) + b * p.os;
         for (int i = t; i < p.heads * D; i += kThreads) o[i] = static_cast<T>(0.0f);
         if (p.lse)
             for (int i = t; i < p.heads; i += kThreads) p.lse[static_cast<size_t>(b) * p.heads + i] = -INFINITY;
     }
-    const int u0 = static_cast<int>(static_cast<long long>(total) * blockIdx.x / gridDim.x);
-    const int u1 = static_cast<int>(static_cast<long long>(total) * (blockIdx.x + 1) / gridDim.x);
+    // this CTA's run: the units that begin in its equal part of the whole cost
+    int u0, u1;
+    {
+        const int x = static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(cost_carry)) *
+                                       (blockIdx.x + (lane & 1)) / gridDim.x);
+        const int u = x >= cost_carry ? carry : unit_at(c, p, table, x);
+        u0 = __shfl_sync(0xffffffffu, u, 0);
+        u1 = __shfl_sync(0xffffffffu, u, 1);
+    }
     if (u0 >= u1) return;
 
     uint8_t* const my_ring = smem + w * C::kStages * C::kStage;
     const uint32_t ring = fer::dev::smem_addr(my_ring);
-    const T* kc = static_cast<const T*>(c.k);
-    const T* vc = static_cast<const T*>(c.v);
-
-    // What is being loaded: unit lu, slab li of it; its pages, and the next
-    // unit's on their way. Bit i of `broken`: the slab in stage i is of a unit
-    // with a page id out of range.
-    UnitRun load_run, run;
-    int lu = u0, li = w, loads = 0;
-    uint32_t broken = 0u;
-    Unit lx = load_run.get(c, p, table, u0, u1 - 1), nx = lx;
-    ChunkPages lp = load_pages(c, lx, lx.chunk * p.chunk), np = lp;
-    bool lgood = true;
-    auto look_ahead = [&]() {
-        lgood = lp.all_good(c, lx.n);
-        if (!lgood && w == 0 && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
-        if (lu + 1 < u1) {
-            nx = load_run.get(c, p, table, lu + 1, u1 - 1);
-            np = load_pages(c, nx, nx.chunk * p.chunk);
-        }
-    };
-    look_ahead();
-    auto issue = [&]() {
-        while (lu < u1 && li * C::kSlab >= lx.n) {   // no slab of this unit is left for this warp
-            li = w;
-            lx = nx;
-            lp = np;
-            if (++lu < u1) look_ahead();
-        }
-        if (lu < u1) {
-            const int stage = loads % C::kStages;
-            const uint32_t st = ring + stage * C::kStage;
-            const int piece = lane % kPieces;
-            broken = (broken & ~(1u << stage)) | (lgood ? 0u : 1u << stage);
-#pragma unroll
-            for (int i = 0; i < C::kSlab / kRowsPer; ++i) {
-                const int r = i * kRowsPer + lane / kPieces;
-                const int slot = li * C::kSlab + r;
-                const int id = lp.of(c, slot < lx.n ? slot : lx.n - 1);
-                const bool take = slot < lx.n && id >= 0;
-                const size_t at = take ? c.row(id, lx.hk, slot) + piece * 8 : 0;
-                const uint32_t to = st + r * C::kRow + ((piece ^ (r & 7)) << 4);
-                cp16(to, kc + at, take);
-                cp16(to + C::kSlab * C::kRow, vc + at, take);
-            }
-            li += kWarps;
-            ++loads;
-        }
-        cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) issue();
+    // a box: rows of one page, 64 dims
+    const int box_rows = min(C::kSlab, c.page_size()), row_boxes = C::kSlab / box_rows;
+    const int my_box = lane / (D / 64) % row_boxes, my_band = lane % (D / 64);
+    const bool my_value = lane >= D / 64 * row_boxes;
+    const bool loader = lane < 2 * (D / 64) * row_boxes;
+    const CUtensorMap* const my_map = my_value ? &v_map : &k_map;
+    const uint32_t my_place = (my_value ? C::kHalf : 0) + my_band * C::kBand + my_box * box_rows * 128;
+    const uint32_t full0 = fer::dev::smem_addr(&s_full[w][0]);
+    bool alive = true;   // no wait of this warp has run out
 
     // Queries as columns (heads lane / 4) of rows (dims 2 (lane % 4) + {0, 1}
     // and 8 more); those of the next unit are loaded a unit ahead where the
@@ -378,9 +405,52 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
                 }
         }
     };
-    int used = 0;
-    Unit x = run.get(c, p, table, u0, u1 - 1);
+    // What is being loaded: unit lu, slab li of it; its pages, and the next
+    // unit's on their way. Bit i of `broken`: the slab in stage i is of a unit
+    // with a page id out of range.
+    UnitRun load_run;
+    int lu = u0, li = w, loads = 0;
+    uint32_t broken = 0u;
+    Unit lx = load_run.get(c, p, table, u0, u1 - 1), nx = lx;
+    UnitRun run = load_run;
+    ChunkPages lp = load_pages(c, lx, lx.chunk * p.chunk), np = lp;
+    Unit x = lx;   // what is being computed
     load_q(x, qf);
+    bool lgood = true;
+    auto look_ahead = [&]() {
+        lgood = lp.all_good(c, lx.n);
+        if (!lgood && w == 0 && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+        if (lu + 1 < u1) {
+            nx = load_run.get(c, p, table, lu + 1, u1 - 1);
+            np = load_pages(c, nx, nx.chunk * p.chunk);
+        }
+    };
+    look_ahead();
+    auto issue = [&]() {
+        while (lu < u1 && li * C::kSlab >= lx.n) {   // no slab of this unit is left for this warp
+            li = w;
+            lx = nx;
+            lp = np;
+            if (++lu < u1) look_ahead();
+        }
+        if (lu < u1) {
+            const int stage = loads % C::kStages;
+            broken = (broken & ~(1u << stage)) | (lgood ? 0u : 1u << stage);
+            // slots of no page are read as page `pages`, which is outside the map: zeros
+            const int slot = li * C::kSlab + my_box * box_rows;
+            const int id = lp.of(c, min(slot, p.chunk - 1));
+            if (lane == 0) fer::dev::mbar_arrive_expect_tx(&s_full[w][stage], C::kStage);
+            if (loader)
+                load_box(ring + stage * C::kStage + my_place, my_map, my_band * 64, slot & (c.page_size() - 1), lx.hk,
+                         id >= 0 ? id : c.pages, full0 + 8 * stage);
+            li += kWarps;
+            ++loads;
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) issue();
+
+    int used = 0;
     for (int u = u0; u < u1; ++u) {
         const int h0 = x.hk * p.group + x.blk * 8 * NT;          // first head of the block
         const int nh = min(8 * NT, p.group - x.blk * 8 * NT);    // its heads
@@ -399,13 +469,23 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
         }
         for (int i = w; i * C::kSlab < x.n; i += kWarps) {
             const bool good = !(broken >> (used % C::kStages) & 1u);
-            cp_wait<C::kStages - 2>();
+            const int stage = used % C::kStages;
+            if (alive) alive = fer::dev::mbar_wait(&s_full[w][stage], used / C::kStages & 1);
             __syncwarp();
             issue();
-            const uint32_t st = ring + (used % C::kStages) * C::kStage;
+            const uint32_t st = ring + stage * C::kStage;
             ++used;
-#pragma unroll
-            for (int sub = 0; sub < kSub; ++sub) {
+            const int rows = x.n - i * C::kSlab;
+            if (rows < C::kSlab) {   // the values behind the last slot count as zero, whatever is there
+                uint4* v = reinterpret_cast<uint4*>(my_ring + stage * C::kStage + C::kHalf);
+                for (int q = lane; q < D / 8 * (C::kSlab - rows); q += 32) {
+                    const int band = q / (8 * (C::kSlab - rows)), rest = q % (8 * (C::kSlab - rows));
+                    v[band * (C::kBand / 16) + 8 * rows + rest] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fer::dev::fence_proxy_async_smem();
+                __syncwarp();
+            }
+            {
                 float s[NT][4];
                 {
                     float s2[NT][4];
@@ -413,11 +493,11 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
-                    const int r = sub * 16 + (lane & 15);
+                    const int r = lane & 15;
 #pragma unroll
                     for (int k = 0; k < kB; ++k) {
                         uint32_t a[4];
-                        ldsm4(a, st + r * C::kRow + (((2 * k + (lane >> 4)) ^ (r & 7)) << 4));
+                        ldsm4(a, st + C::at(r, 2 * k + (lane >> 4)));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma<T>(k & 1 ? s2[nt] : s[nt], a, qf[nt][k][0], qf[nt][k][1]);
                     }
@@ -426,7 +506,7 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * p.scale2;
                 }
-                const int j = i * C::kSlab + sub * 16 + lane / 4;   // this lane's slots of the chunk: j, j + 8
+                const int j = i * C::kSlab + lane / 4;   // this lane's slots of the chunk: j, j + 8
                 bool on0 = j < x.n, on1 = j + 8 < x.n;
                 if (!good) {
                     const ChunkPages pg = load_pages(c, x, k0);
@@ -490,11 +570,11 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
                         lo[nt][e] = transpose8(lo[nt][e]);
                     }
                 }
-                const int r = sub * 16 + (lane & 7) + ((lane >> 4) << 3);
+                const int r = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
                 for (int k = 0; k < kB; ++k) {
                     uint32_t a[4];
-                    ldsm4_t(a, st + C::kSlab * C::kRow + r * C::kRow + (((2 * k + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+                    ldsm4_t(a, st + C::kHalf + C::at(r, 2 * k + ((lane >> 3) & 1)));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         mma<T>(o[nt][k], a, lo[nt][0], lo[nt][1]);
@@ -569,6 +649,7 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
                     make_float4(a.x * kBack, a.y * kBack, a.z * kBack, a.w * kBack);
             }
         }
+        fer::dev::fence_proxy_async_smem();   // before copies into the stages that held o
         __syncthreads();
         if (turn) {
             if constexpr (kAhead) {
@@ -582,7 +663,11 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
         }
         x = next;
     }
-    cp_wait<0>();
+    if (!alive) {   // let the last copies land, bounded as well, before the memory goes away
+        if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
+        for (int k = max(0, loads - C::kStages); k < loads; ++k)
+            fer::dev::mbar_wait(&s_full[w][k % C::kStages], k / C::kStages & 1);
+    }
 }
 
 // log2 of a head's total sum of powers, from its chunks' (m, l), by one warp;
@@ -591,10 +676,20 @@ __global__ void __launch_bounds__(kThreads) attn_units(const Paged c, const Attn
 __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float* base, float* sum) {
     const int lane = threadIdx.x & 31;
     float top = -INFINITY, l = 0.0f;
-    for (int i = lane; i < chunks; i += 32) {
-        const float2 v = *reinterpret_cast<const float2*>(ml + 2 * i);
-        const float next = fmaxf(top, v.x), b = next == -INFINITY ? 0.0f : next;
-        l = l * ex2(top - b) + v.y * ex2(v.x - b);
+    for (int i0 = lane; i0 < chunks; i0 += 32 * 8) {
+        float2 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = make_float2(-INFINITY, 0.0f);
+            if (i0 + 32 * k < chunks) v[k] = *reinterpret_cast<const float2*>(ml + 2 * (i0 + 32 * k));
+        }
+        float next = top;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) next = fmaxf(next, v[k].x);
+        const float b = next == -INFINITY ? 0.0f : next;
+        l *= ex2(top - b);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) l += v[k].y * ex2(v[k].x - b);
         top = next;
     }
 #pragma unroll
@@ -612,9 +707,9 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float*
 
 // grid (group + weight tiles, kv_heads, n_seq). The first `group` CTAs of a
 // (key head, sequence) add one head's chunks each (in order within a warp,
-// then the warps in order); the others add probabilities to kFinishSlots
-// slots' weights each, four slots a thread.
-template <typename T, int D>
+// then the warps in order); the others add probabilities to the
+// weights of four slots a thread.
+template <typename T, int D, int kFinish>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
     constexpr int kW = kFinish / 32, kV = D / 32;    // warps; dims a lane
     __shared__ float s_o[kW][D];
@@ -637,7 +732,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
 #pragma unroll
         for (int e = 0; e < kV; ++e) o[e] = 0.0f;
         if (w < chunks) {
-#pragma unroll 4
+#pragma unroll 8
             for (int i = w; i < chunks; i += kW) {
                 const float f = ex2(ml[2 * i] - base);
 #pragma unroll
@@ -656,11 +751,10 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
         if (t == 0 && p.lse) p.lse[bh] = lse2 * kLn2;
         return;
     }
-    const int j0 = (blockIdx.x - p.group) * kFinishSlots;
+    const int j0 = (blockIdx.x - p.group) * 4 * kFinish;
     if (j0 >= len) return;
     const int j = j0 + 4 * t;
     const size_t most = static_cast<size_t>(c.max_slots());   // a multiple of 8: rows start at 16 bytes
-    static_assert(kFinishSlots == 4 * kFinish);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int g0 = 0; g0 < p.group; g0 += kFinish) {
         const int ng = min(kFinish, p.group - g0);
@@ -710,6 +804,29 @@ int resident(const void* kernel, int smem, std::atomic<int>* known) {
     return n * sms;
 }
 
+// Boxes of 64 dims x `rows` rows of one page; 128-byte swizzle.
+bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int rows) {
+    const fer::host::EncodeTiledFn fn = fer::host::encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t page = static_cast<cuuint64_t>(c.page_size()), row = 2ull * c.head_dim;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), page, static_cast<cuuint64_t>(c.kv_heads),
+                                static_cast<cuuint64_t>(c.pages)};
+    const cuuint64_t strides[3] = {row, page * row, page * row * c.kv_heads};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, step[4] = {1, 1, 1, 1};
+    return fn(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides,
+              box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A warp a chunk at a time: four warps where a head has few chunks, sixteen
+// where there are many to read.
+template <typename T, int D, int THREADS>
+cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
+    const int tiles = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0;
+    return fer::host::launch_pdl(attn_finish<T, D, THREADS>, dim3(p.group + tiles, c.kv_heads, p.n_seq), dim3(THREADS),
+                                 0, s, c, p);
+}
+
 template <typename T, int D, int NT>
 cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     using fer::host::launch_pdl;
@@ -717,13 +834,15 @@ cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     static std::atomic<int> known[kDevices];
     const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT>), smem, known);
     if (ctas <= 0) return cudaErrorInvalidConfiguration;
+    CUtensorMap k_map, v_map;
+    const int rows = Cut<D>::kSlab < c.page_size() ? Cut<D>::kSlab : c.page_size();
+    const uint32_t dtype = __is_same(T, __half) ? 1 : 2;
+    if (!map_pages(&k_map, c, c.k, dtype, rows) || !map_pages(&v_map, c, c.v, dtype, rows)) return cudaErrorInvalidValue;
     const long long most = static_cast<long long>(p.n_seq) * c.kv_heads * p.blocks * p.chunks;
     cudaError_t e = launch_pdl(attn_units<T, D, NT>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
-                               dim3(kThreads), smem, s, c, p);
-    if (e == cudaSuccess && (p.weights || p.chunks > 1)) {
-        const int tiles = p.weights ? (c.max_slots() - 1) / kFinishSlots + 1 : 0;
-        e = launch_pdl(attn_finish<T, D>, dim3(p.group + tiles, c.kv_heads, p.n_seq), dim3(kFinish), 0, s, c, p);
-    }
+                               dim3(kThreads), smem, s, c, p, k_map, v_map);
+    if (e == cudaSuccess && (p.weights || p.chunks > 1))
+        e = p.chunks <= 32 ? finish<T, D, 128>(c, p, s) : finish<T, D, 512>(c, p, s);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -774,8 +893,9 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     if (a->n_seq == 0) return cudaSuccess;
     if (c.kv_heads > 65535 || a->n_seq > 65535) return cudaErrorNotSupported;
     const int max_slots = c.max_slots();
-    // units are counted in 31 bits
-    if (static_cast<long long>(a->n_seq) * a->heads * ((max_slots - 1) / chunk_of(max_slots) + 1) > 0x7fffffffll)
+    // units and their cost are counted in 31 bits
+    if (static_cast<long long>(a->n_seq) * a->heads * (rounds_of(max_slots) + (max_slots - 1) / chunk_of(max_slots) + 1) >
+        0x7fffffffll)
         return cudaErrorNotSupported;
     const size_t need = fer_paged_attention_workspace_bytes(a->n_seq, a->heads, c.kv_heads, c.head_dim, max_slots,
                                                             a->weights != nullptr);
