@@ -517,6 +517,9 @@ def transformer_shard(global_batch: int, world: int, rank: int) -> tuple[int, in
     return first.value, count.value
 
 
+_SECTIONS = C.c_uint32 * 4
+
+
 def paged_cache(k: int, v: int, page_table: int, lengths: int) -> fer_paged_cache_t:
     """A paged key-value cache of four buffer ids."""
     return fer_paged_cache_t(k, v, page_table, lengths)
@@ -538,6 +541,8 @@ class Session:
 
     def __init__(self, device: int = 0, pool_bytes: int = 256 << 20, regime: int = FER_MEMORY_CUSTOM_POOL):
         self.lib = capi()
+        self._job = C.c_uint64()
+        self._job_ref = C.byref(self._job)
         cfg = fer_pool_config_t()
         cfg.mutable_bytes = pool_bytes // 2
         cfg.immutable_bytes = pool_bytes - pool_bytes // 2
@@ -633,6 +638,13 @@ class Session:
         check("fer_submit_gemm", self.call("fer_submit_gemm", C.byref(r), C.byref(job)))
         return job.value
 
+    def _submit(self, fn, request) -> int:
+        """One fer_submit_* call; its job id."""
+        st = fn(self.ptr, C.byref(request), self._job_ref)
+        if st.code:
+            raise FerError(fn.__name__, st)
+        return self._job.value
+
     def rotary(self, x: int, out: int, positions: int, heads: int, head_dim: int, *, sections=(0,), rotary_dim: int = 0,
                base: float = 10000.0, x_col: int = 0, out_col: int = 0, interleaved: bool = False,
                axis_freqs: bool = False, inverse: bool = False) -> int:
@@ -641,35 +653,25 @@ class Session:
             raise ValueError("rotary takes 1 to 4 axes")
         flags = ((FER_ROTARY_INTERLEAVED if interleaved else 0) | (FER_ROTARY_AXIS_FREQS if axis_freqs else 0) |
                  (FER_ROTARY_INVERSE if inverse else 0))
-        r = fer_rotary_request_t(x, out, positions, x_col, out_col, heads, head_dim, rotary_dim, len(sections),
-                                 (C.c_uint32 * 4)(*sections), base, flags)
-        job = C.c_uint64()
-        check("fer_submit_rotary", self.lib.fer_submit_rotary(self.ptr, C.byref(r), C.byref(job)))
-        return job.value
+        return self._submit(self.lib.fer_submit_rotary, fer_rotary_request_t(
+            x, out, positions, x_col, out_col, heads, head_dim, rotary_dim, len(sections), _SECTIONS(*sections), base,
+            flags))
 
     def paged_store(self, cache: fer_paged_cache_t, k_rows: int, v_rows: int, *, k_col: int = 0, v_col: int = 0,
                     offsets: int = 0, new_lengths: int = 0, weights: int = 0, positions: int = 0, seen: int = 0,
                     new_seen: int = 0) -> int:
-        r = fer_paged_store_request_t(cache, k_rows, v_rows, offsets, new_lengths, weights, positions, seen, new_seen,
-                                      k_col, v_col)
-        job = C.c_uint64()
-        check("fer_submit_paged_store", self.lib.fer_submit_paged_store(self.ptr, C.byref(r), C.byref(job)))
-        return job.value
+        return self._submit(self.lib.fer_submit_paged_store, fer_paged_store_request_t(
+            cache, k_rows, v_rows, offsets, new_lengths, weights, positions, seen, new_seen, k_col, v_col))
 
     def paged_attention(self, cache: fer_paged_cache_t, q: int, out: int, heads: int, *, workspace: int,
                         q_col: int = 0, out_col: int = 0, scale: float = 0.0, lse: int = 0, weights: int = 0) -> int:
-        r = fer_paged_attention_request_t(cache, q, out, lse, weights, workspace, q_col, out_col, heads, scale)
-        job = C.c_uint64()
-        check("fer_submit_paged_attention", self.lib.fer_submit_paged_attention(self.ptr, C.byref(r), C.byref(job)))
-        return job.value
+        return self._submit(self.lib.fer_submit_paged_attention, fer_paged_attention_request_t(
+            cache, q, out, lse, weights, workspace, q_col, out_col, heads, scale))
 
     def paged_evict(self, cache: fer_paged_cache_t, budget: int, recent: int, weights: int, positions: int, seen: int,
                     *, workspace: int, new_lengths: int = 0, new_weights: int = 0, new_positions: int = 0) -> int:
-        r = fer_paged_evict_request_t(cache, weights, positions, seen, new_lengths, new_weights, new_positions,
-                                      workspace, budget, recent)
-        job = C.c_uint64()
-        check("fer_submit_paged_evict", self.lib.fer_submit_paged_evict(self.ptr, C.byref(r), C.byref(job)))
-        return job.value
+        return self._submit(self.lib.fer_submit_paged_evict, fer_paged_evict_request_t(
+            cache, weights, positions, seen, new_lengths, new_weights, new_positions, workspace, budget, recent))
 
     def import_ptr(self, dtype: int, shape, ptr: int) -> int:
         """Registers external device memory (e.g. a torch tensor) as a buffer."""

@@ -26,10 +26,13 @@ struct Paged {
         *bad = n < 0 || n > most;
         return n < 0 ? 0 : n > most ? most : n;
     }
+    __device__ __forceinline__ bool is_page(int id) const {
+        return static_cast<unsigned>(id) < static_cast<unsigned>(pages);
+    }
     // Page id of slot s of sequence b, -1 where the table holds none.
     __device__ __forceinline__ int page(int b, int s) const {
         const int id = table[static_cast<size_t>(b) * max_pages + (s >> shift)];
-        return static_cast<unsigned>(id) < static_cast<unsigned>(pages) ? id : -1;
+        return is_page(id) ? id : -1;
     }
     // First element of the row of slot s, given its page.
     __device__ __forceinline__ size_t row(int id, int h, int s) const {

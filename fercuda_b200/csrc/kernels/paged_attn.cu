@@ -47,7 +47,8 @@ namespace {
 using fer::dev::Paged;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kSegments = 256;      // entries of the unit table in shared memory
+constexpr int kSegments = 128;      // entries of the unit table in shared memory
+constexpr int kMeet = 2;            // heads whose parts meet at once
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -59,7 +60,10 @@ struct AttnParams {
     const void* q;
     void* out;
     size_t qs, os;
-    int n_seq, heads, group, blocks, chunk, chunks;   // blocks: head blocks a key head
+    int n_seq, heads, group, blocks, chunks;   // blocks: head blocks a key head
+    int chunk_log2;
+    __device__ __forceinline__ int chunk() const { return 1 << chunk_log2; }
+    __device__ __forceinline__ int chunks_of(int len) const { return (len + chunk() - 1) >> chunk_log2; }
     float scale2;        // scale * log2 e
     float* lse;
     float* weights;
@@ -155,16 +159,17 @@ template <int D> struct Cut {
     static constexpr int kHalf = D / 64 * kBand;             // keys; the values follow
     static constexpr int kStage = 2 * kHalf;
     static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kSmem = kRing + 1024;               // bands start at 1024 bytes
+    static constexpr int kMeetBytes = 2 * kWarps * kMeet * D * 4;
+    static constexpr int kSmem = kRing + kMeetBytes + 1024;  // bands start at 1024 bytes
     // Byte of piece c of row r in a half of a stage.
     static __device__ __forceinline__ uint32_t at(int r, int c) {
         return (c >> 3) * kBand + r * 128 + (((c ^ r) & 7) << 4);
     }
 };
 
-// What a unit costs, in rounds of a slab for each warp: its rounds, and about
-// one more for its beginning and its end (measured: 2100 to 2450 cycles a
-// round, 1400 to 2000 around them).
+// What a unit costs, in rounds of a slab for each warp: its rounds, and
+// kUnitCost more for its beginning and its end.
+constexpr int kUnitCost = 2;
 constexpr int kRound = 16 * kWarps;   // slots
 __host__ __device__ inline int rounds_of(int n) { return (n + kRound - 1) / kRound; }
 
@@ -192,11 +197,11 @@ struct Seq {
     __device__ __forceinline__ Seq(const Paged& c, const AttnParams& p, int b) {
         bool bad;
         len = c.length(b, &bad);
-        chunks = (len + p.chunk - 1) / p.chunk;
+        chunks = p.chunks_of(len);
         heads = c.kv_heads * p.blocks;
     }
     __device__ __forceinline__ int units() const { return chunks * heads; }
-    __device__ __forceinline__ int block_cost() const { return rounds_of(len) + chunks; }
+    __device__ __forceinline__ int block_cost() const { return rounds_of(len) + chunks * kUnitCost; }
     __device__ __forceinline__ int cost() const { return block_cost() * heads; }
 };
 
@@ -209,7 +214,7 @@ __device__ __forceinline__ int unit_at(const Paged& c, const AttnParams& p, cons
         const Seq q(c, p, b);
         if (x < q.cost()) {
             const int block = x / q.block_cost(), rest = x - block * q.block_cost();
-            const int each = rounds_of(p.chunk) + 1;
+            const int each = rounds_of(p.chunk()) + kUnitCost;
             return u + block * q.chunks + min((rest + each - 1) / each, q.chunks);
         }
         x -= q.cost();
@@ -239,7 +244,7 @@ __device__ __forceinline__ Unit find_unit(const Paged& c, const AttnParams& p, c
     x.chunk = r - hb * q.chunks;
     x.hk = hb / p.blocks;
     x.blk = hb - x.hk * p.blocks;
-    x.n = min(p.chunk, q.len - x.chunk * p.chunk);
+    x.n = min(p.chunk(), q.len - (x.chunk << p.chunk_log2));
     return x;
 }
 
@@ -265,8 +270,9 @@ struct UnitRun {
     }
 };
 
-// Page ids of a unit's chunk (up to 64 pages): lane i holds those of its i-th
-// and (i + 32)-th page, -1 where no slot is held or the table has no page.
+// Page ids of a unit's chunk (up to 64 pages) as the table has them: lane i
+// holds those of its i-th and (i + 32)-th page, -1 behind the last. They are
+// checked where they are used, so that a load for a later unit stays in flight.
 struct ChunkPages {
     int a, b;
     __device__ __forceinline__ int of(const Paged& c, int slot) const {
@@ -276,15 +282,16 @@ struct ChunkPages {
     }
     __device__ __forceinline__ bool all_good(const Paged& c, int n) const {
         const int lane = threadIdx.x & 31, last = (n - 1) >> c.shift;
-        return !__any_sync(0xffffffffu, (lane <= last && a < 0) || (lane + 32 <= last && b < 0));
+        return !__any_sync(0xffffffffu, (lane <= last && !c.is_page(a)) || (lane + 32 <= last && !c.is_page(b)));
     }
 };
 
 __device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x, int k0) {
     const int lane = threadIdx.x & 31, last = (x.n - 1) >> c.shift;
+    const int32_t* row = c.table + static_cast<size_t>(x.b) * c.max_pages + (k0 >> c.shift) + lane;
     ChunkPages g{-1, -1};
-    if (lane <= last) g.a = c.page(x.b, k0 + (lane << c.shift));
-    if (lane + 32 <= last) g.b = c.page(x.b, k0 + ((lane + 32) << c.shift));
+    if (lane <= last) g.a = row[0];
+    if (lane + 32 <= last) g.b = row[32];
     return g;
 }
 
@@ -296,9 +303,10 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
     constexpr int kB = D / 16;                  // 16-wide blocks of a row
     extern __shared__ uint8_t smem_raw[];
     __shared__ int s_units[kSegments], s_cost[kSegments], s_sum[kWarps], s_cost_sum[kWarps];
-    __shared__ float s_ml[kWarps][8 * NT][2];
+    __shared__ float s_ml[2][kWarps][8 * NT][2];
     __shared__ uint64_t s_full[kWarps][C::kStages];
     uint8_t* const smem = smem_raw + (-fer::dev::smem_addr(smem_raw) & 1023u);
+    float* const meet = reinterpret_cast<float*>(smem + C::kRing);   // [2][kWarps][kMeet][D]
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     if (lane == 0) {
         for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&s_full[w][i], 1);
@@ -382,16 +390,17 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
     bool alive = true;   // no wait of this warp has run out
 
     // Queries as columns (heads lane / 4) of rows (dims 2 (lane % 4) + {0, 1}
-    // and 8 more); those of the next unit are loaded a unit ahead where the
-    // registers allow it.
+    // and 8 more); columns behind the group's last head repeat its first and are
+    // left out at the end. Those of the next unit are loaded a unit ahead
+    // where the registers allow it.
     constexpr bool kAhead = NT * kB <= 8;
     uint32_t qf[NT][kB][2], qn[NT][kB][2];
     auto load_q = [&](const Unit& x, uint32_t (&q)[NT][kB][2]) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int g = x.blk * 8 * NT + nt * 8 + lane / 4;
-            const bool real = g < p.group;
-            const T* row = static_cast<const T*>(p.q) + x.b * p.qs + (static_cast<size_t>(x.hk) * p.group + (real ? g : 0)) * D;
+            const T* row = static_cast<const T*>(p.q) + x.b * p.qs +
+                           (static_cast<size_t>(x.hk) * p.group + (g < p.group ? g : 0)) * D;
             const bool even = (reinterpret_cast<uintptr_t>(row) & 3) == 0;
 #pragma unroll
             for (int k = 0; k < kB; ++k)
@@ -401,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
                     uint32_t v;
                     if (even) v = *reinterpret_cast<const uint32_t*>(at);
                     else v = at[0] | static_cast<uint32_t>(at[1]) << 16;
-                    q[nt][k][e] = real ? v : 0u;
+                    q[nt][k][e] = v;
                 }
         }
     };
@@ -413,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
     uint32_t broken = 0u;
     Unit lx = load_run.get(c, p, table, u0, u1 - 1), nx = lx;
     UnitRun run = load_run;
-    ChunkPages lp = load_pages(c, lx, lx.chunk * p.chunk), np = lp;
+    ChunkPages lp = load_pages(c, lx, lx.chunk << p.chunk_log2), np = lp;
     Unit x = lx;   // what is being computed
     load_q(x, qf);
     bool lgood = true;
@@ -422,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
         if (!lgood && w == 0 && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
         if (lu + 1 < u1) {
             nx = load_run.get(c, p, table, lu + 1, u1 - 1);
-            np = load_pages(c, nx, nx.chunk * p.chunk);
+            np = load_pages(c, nx, nx.chunk << p.chunk_log2);
         }
     };
     look_ahead();
@@ -438,23 +447,23 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
             broken = (broken & ~(1u << stage)) | (lgood ? 0u : 1u << stage);
             // slots of no page are read as page `pages`, which is outside the map: zeros
             const int slot = li * C::kSlab + my_box * box_rows;
-            const int id = lp.of(c, min(slot, p.chunk - 1));
+            const int id = lp.of(c, min(slot, p.chunk() - 1));
             if (lane == 0) fer::dev::mbar_arrive_expect_tx(&s_full[w][stage], C::kStage);
             if (loader)
                 load_box(ring + stage * C::kStage + my_place, my_map, my_band * 64, slot & (c.page_size() - 1), lx.hk,
-                         id >= 0 ? id : c.pages, full0 + 8 * stage);
+                         c.is_page(id) ? id : c.pages, full0 + 8 * stage);
             li += kWarps;
             ++loads;
         }
     };
 #pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) issue();
+    for (int i = 0; i < C::kStages; ++i) issue();
 
-    int used = 0;
+    int used = 0, turns = 0;
     for (int u = u0; u < u1; ++u) {
         const int h0 = x.hk * p.group + x.blk * 8 * NT;          // first head of the block
         const int nh = min(8 * NT, p.group - x.blk * 8 * NT);    // its heads
-        const int k0 = x.chunk * p.chunk;
+        const int k0 = x.chunk << p.chunk_log2;
         const Unit next = u + 1 < u1 ? run.get(c, p, table, u + 1, u1 - 1) : x;
         const bool turn = next.b != x.b || next.hk != x.hk || next.blk != x.blk;
         if (kAhead && turn) load_q(next, qn);
@@ -471,8 +480,6 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
             const bool good = !(broken >> (used % C::kStages) & 1u);
             const int stage = used % C::kStages;
             if (alive) alive = fer::dev::mbar_wait(&s_full[w][stage], used / C::kStages & 1);
-            __syncwarp();
-            issue();
             const uint32_t st = ring + stage * C::kStage;
             ++used;
             const int rows = x.n - i * C::kSlab;
@@ -511,8 +518,8 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
                 if (!good) {
                     const ChunkPages pg = load_pages(c, x, k0);
                     const int p0 = pg.of(c, min(j, x.n - 1)), p1 = pg.of(c, min(j + 8, x.n - 1));
-                    on0 = on0 && p0 >= 0;
-                    on1 = on1 && p1 >= 0;
+                    on0 = on0 && c.is_page(p0);
+                    on1 = on1 && c.is_page(p1);
                 }
                 bool grew = false;
                 float next[NT][2];
@@ -582,14 +589,16 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
                     }
                 }
             }
+            __syncwarp();
+            issue();   // into the stage that was just read
         }
 
-        // The warps' parts meet in shared memory: each warp's o, a row of dims a
-        // head, in the stage of its ring that nothing is loaded into before
-        // its next slab. Eights of dims are swapped by head pair against bank conflicts.
-        float* const my_o = reinterpret_cast<float*>(my_ring + ((used + C::kStages - 1) % C::kStages) * C::kStage);
-        static_assert(8 * NT * D * 4 <= C::kStage);
-        __syncwarp();
+        // The warps' parts meet in shared memory, kMeet heads at a time in two
+        // areas by turns, so that one barrier a time is enough: who writes an
+        // area again has passed the barrier behind its last readers.
+        const bool whole = x.chunks == 1;
+        const size_t bh0 = static_cast<size_t>(x.b) * p.heads + h0;
+        float(*const ml)[8 * NT][2] = s_ml[u & 1];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -597,60 +606,57 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
-                const int g = nt * 8 + 2 * (lane & 3) + e;
-                if (g >= nh) continue;
                 if (lane < 4) {
-                    s_ml[w][g][0] = m[nt][e];
-                    s_ml[w][g][1] = l[nt][e];
+                    ml[w][nt * 8 + 2 * lane + e][0] = m[nt][e];
+                    ml[w][nt * 8 + 2 * lane + e][1] = l[nt][e];
                 }
+            }
+#pragma unroll
+        for (int q = 0; q < 4 * NT; ++q) {   // heads 2 q and 2 q + 1, held by the lanes with lane % 4 == q % 4
+            if (2 * q >= nh) break;
+            float* const area = meet + turns * (kWarps * kMeet * D);
+            turns ^= 1;
+            if ((lane & 3) == (q & 3)) {
+                float* const mine = area + w * kMeet * D + lane / 4;
 #pragma unroll
                 for (int k = 0; k < kB; ++k)
 #pragma unroll
-                    for (int r = 0; r < 2; ++r)
-                        my_o[g * D + ((16 * k + 8 * r + lane / 4) ^ ((lane & 3) << 3))] = o[nt][k][2 * r + e];
+                    for (int e = 0; e < 4; ++e) mine[(e & 1) * D + 16 * k + 8 * (e >> 1)] = o[q / 4][k][e];
             }
-        if (lane == 0) s_sum[w] = used;
-        __syncthreads();
-        const float* part[kWarps];
+            __syncthreads();
+            for (int i = t; i < kMeet * (D / 4); i += kThreads) {
+                const int e = i / (D / 4), g = 2 * q + e, d = i % (D / 4) * 4;
+                if (g >= nh) continue;
+                float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i)
-            part[i] = reinterpret_cast<const float*>(smem + (i * C::kStages + (s_sum[i] + C::kStages - 1) % C::kStages) * C::kStage);
-        const bool whole = x.chunks == 1;
-        const size_t bh0 = static_cast<size_t>(x.b) * p.heads + h0;
-        for (int i = t; i < nh * (D / 4); i += kThreads) {
-            const int g = i / (D / 4), d = i % (D / 4) * 4;
-            float top = -INFINITY, sum = 0.0f;
+                for (int v = 0; v < kWarps; ++v) top = fmaxf(top, ml[v][g][0]);
+                const float base = top == -INFINITY ? 0.0f : top;
+                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int v = 0; v < kWarps; ++v) top = fmaxf(top, s_ml[v][g][0]);
-            const float base = top == -INFINITY ? 0.0f : top;
-            float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int v = 0; v < kWarps; ++v) {
+                    const float f = ex2(ml[v][g][0] - base);
+                    const float4 y = *reinterpret_cast<const float4*>(area + (v * kMeet + e) * D + d);
+                    sum += ml[v][g][1] * f;
+                    a.x += y.x * f, a.y += y.y * f, a.z += y.z * f, a.w += y.w * f;
+                }
+                constexpr float kBack = 1.0f / kScaleP<T>;
+                const size_t at = (bh0 + g) * p.chunks + x.chunk;
+                if (d == 0) {
+                    *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(top, sum);
+                    if (whole && p.lse) p.lse[bh0 + g] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+                }
+                if (whole) {
+                    const float f = sum == 0.0f ? 0.0f : kBack / sum;
+                    T* out = static_cast<T*>(p.out) + x.b * p.os + static_cast<size_t>(h0 + g) * D + d;
+                    const float v[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int v = 0; v < kWarps; ++v) {
-                const float f = ex2(s_ml[v][g][0] - base);
-                const float4 y = *reinterpret_cast<const float4*>(part[v] + g * D + (d ^ ((g >> 1 & 3) << 3)));
-                sum += s_ml[v][g][1] * f;
-                a.x += y.x * f, a.y += y.y * f, a.z += y.z * f, a.w += y.w * f;
-            }
-            constexpr float kBack = 1.0f / kScaleP<T>;
-            const size_t at = (bh0 + g) * p.chunks + x.chunk;
-            if (d == 0) {
-                p.part_ml[2 * at] = top;
-                p.part_ml[2 * at + 1] = sum;
-                if (whole && p.lse) p.lse[bh0 + g] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-            }
-            if (whole) {
-                const float f = sum == 0.0f ? 0.0f : kBack / sum;
-                T* out = static_cast<T*>(p.out) + x.b * p.os + static_cast<size_t>(h0 + g) * D + d;
-                const float v[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(sum == 0.0f ? 0.0f : v[e] * f);
-            } else {
-                *reinterpret_cast<float4*>(p.part_o + at * D + d) =
-                    make_float4(a.x * kBack, a.y * kBack, a.z * kBack, a.w * kBack);
+                    for (int k = 0; k < 4; ++k) out[k] = static_cast<T>(sum == 0.0f ? 0.0f : v[k] * f);
+                } else {
+                    *reinterpret_cast<float4*>(p.part_o + at * D + d) =
+                        make_float4(a.x * kBack, a.y * kBack, a.z * kBack, a.w * kBack);
+                }
             }
         }
-        fer::dev::fence_proxy_async_smem();   // before copies into the stages that held o
-        __syncthreads();
         if (turn) {
             if constexpr (kAhead) {
 #pragma unroll
@@ -719,7 +725,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
     fer::dev::pdl_begin();
     bool bad;
     const int len = c.length(b, &bad);
-    const int chunks = (len + p.chunk - 1) / p.chunk;
+    const int chunks = p.chunks_of(len);
     const size_t bh0 = static_cast<size_t>(b) * p.heads + static_cast<size_t>(hk) * p.group;
     if (static_cast<int>(blockIdx.x) < p.group) {
         if (chunks <= 1) return;                      // written already
@@ -894,7 +900,7 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     if (c.kv_heads > 65535 || a->n_seq > 65535) return cudaErrorNotSupported;
     const int max_slots = c.max_slots();
     // units and their cost are counted in 31 bits
-    if (static_cast<long long>(a->n_seq) * a->heads * (rounds_of(max_slots) + (max_slots - 1) / chunk_of(max_slots) + 1) >
+    if (static_cast<long long>(a->n_seq) * a->heads * (rounds_of(max_slots) + kUnitCost * ((max_slots - 1) / chunk_of(max_slots) + 1ll)) >
         0x7fffffffll)
         return cudaErrorNotSupported;
     const size_t need = fer_paged_attention_workspace_bytes(a->n_seq, a->heads, c.kv_heads, c.head_dim, max_slots,
@@ -909,8 +915,8 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     p.n_seq = a->n_seq;
     p.heads = a->heads;
     p.group = a->heads / c.kv_heads;
-    p.chunk = chunk_of(max_slots);
-    p.chunks = (max_slots - 1) / p.chunk + 1;
+    while ((1 << p.chunk_log2) < chunk_of(max_slots)) ++p.chunk_log2;
+    p.chunks = (max_slots - 1) / chunk_of(max_slots) + 1;
     p.scale2 = (a->scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c.head_dim)) : a->scale) * kLog2e;
     p.lse = a->lse;
     p.weights = a->weights;

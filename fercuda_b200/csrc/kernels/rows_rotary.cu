@@ -5,24 +5,33 @@
 // element once (2 x size bytes for 3 flops), so it is bound by HBM, and by
 // launch latency for a few rows.
 //
-// A CTA walks tiles of rows. For a tile it first puts the cosines and sines of
-// (row, pair) into shared memory, once for all heads: the frequency in turns
-// is f64, so position * frequency can be reduced to [-1/2, 1/2] turns exactly
-// before the f32 sine (an f32 angle of position 10^6 is off by 0.06 rad).
-// Then threads walk (row, head, unit) with V elements a load; a unit of the
-// half-split layout is V elements of the first half and the V that pair with
-// them. V is the widest that pointers, strides and sizes allow.
+// A warp takes a row (or, where rows are few, a part of its heads). Its lanes
+// compute the cosines and sines of the row's pairs once for all heads and
+// share them in shared memory; there is no barrier. The frequency in turns is f64, so
+// position * frequency can be reduced to [-1/2, 1/2] turns exactly before the
+// f32 sine (an f32 angle of position 10^6 is off by 0.06 rad). The first
+// kAhead loads a lane are in flight meanwhile.
+//
+// Lane (unit, head) turns the same unit of every hp-th head, so it reads its
+// cosines and sines once and keeps them in registers. Neighbouring lanes have
+// neighbouring units, then neighbouring heads: a warp reads the row front to
+// back. A unit of the half-split layout is V elements of the first half and
+// the V that pair with them; V is the widest that pointers, strides and sizes
+// allow.
 #include "elem.cuh"
 #include "pdl.cuh"
 
 #include "fercuda/b200/native.h"
 
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 2;   // units whose loads are in flight before the first is turned
+constexpr int kWarps = kThreads / 32;
+constexpr int kAhead = 4;   // loads a lane makes before it turns the first
 
 struct RotaryParams {
     const void* x;
@@ -31,34 +40,76 @@ struct RotaryParams {
     size_t xs, os;
     int rows, heads, head_dim, half, axes;
     int bound[4];     // first pair behind each axis
-    int tile;         // rows a tile
     int units;        // units a head, the copied tail's among them
+    int across;       // units a warp takes at once
+    int hp;           // heads a warp takes at once
+    int split;        // warps a row
+    int share;        // heads of one of them
     float base;
     uint32_t flags;
 };
 
+// Two neighbouring 16-bit elements as f32, and back, rounded to nearest even.
 template <typename T>
-__device__ __forceinline__ float to_f(T v) {
-    if constexpr (sizeof(T) == 4) return v;
-    else return static_cast<float>(v);
+__device__ __forceinline__ float2 widen2(uint32_t w) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow2(float x, float y) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 v = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
 }
 
-// V elements at an address that is a multiple of A of them.
+// V elements at an address that is a multiple of A of them, and as f32.
 template <typename T, int V, int A>
-struct alignas(sizeof(T) * A) Vec {
+struct alignas(sizeof(T) * A) Piece {
     T e[V];
+    __device__ __forceinline__ void get(float (&f)[V]) const {
+        if constexpr (sizeof(T) == 4 || V == 1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = static_cast<float>(e[i]);
+        } else {
+            uint32_t w[V / 2];
+            memcpy(w, e, sizeof(e));
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 v = widen2<T>(w[i]);
+                f[2 * i] = v.x, f[2 * i + 1] = v.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void put(const float (&f)[V]) {
+        if constexpr (sizeof(T) == 4 || V == 1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) e[i] = static_cast<T>(f[i]);
+        } else {
+            uint32_t w[V / 2];
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) w[i] = narrow2<T>(f[2 * i], f[2 * i + 1]);
+            memcpy(e, w, sizeof(e));
+        }
+    }
 };
 
 template <typename T, int V, int A, bool INTER>
-__global__ void __launch_bounds__(kThreads) rotary(const RotaryParams p) {
-    extern __shared__ double sh_freq[];                               // [half] turns a position
-    float2* sh_cs = reinterpret_cast<float2*>(sh_freq + p.half);      // [tile][half]
-    const int t = threadIdx.x;
-    const int turned = INTER ? 2 * p.half / V : p.half / V;           // units that turn; the rest are the tail
-    // the walk over (row, head, unit) in steps of kThreads, without a division a step
-    const int su = kThreads % p.units, sh = kThreads / p.units % p.heads, sr = kThreads / (p.units * p.heads);
+__global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
+    using P = Piece<T, V, A>;
+    constexpr int kPairs = INTER ? V / 2 : V;                         // pairs a unit
+    extern __shared__ __align__(16) double sh_freq[];                 // [half] turns a position
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int half4 = (p.half + 3) & ~3;
+    float2* const table = reinterpret_cast<float2*>(sh_freq + half4) + w * half4;   // this warp's cosines and sines
+    const int turned = p.half / kPairs;                               // units that turn; the rest are the tail
+    const int u0 = lane % p.across, h0 = lane / p.across;
+    const bool copy_tail = p.x != p.out;
     const double inv_two_pi = 0.15915494309189535;
-    for (int i = t; i < p.half; i += kThreads) {
+    for (int i = threadIdx.x; i < p.half; i += kThreads) {
         int a = 0, lo = 0;
         while (a + 1 < p.axes && i >= p.bound[a]) lo = p.bound[a++];
         const double e = (p.flags & FER_ROTARY_FLAG_AXIS_FREQS) ? static_cast<double>(i - lo) / (p.bound[a] - lo)
@@ -68,72 +119,82 @@ __global__ void __launch_bounds__(kThreads) rotary(const RotaryParams p) {
         sh_freq[i] = f;
     }
     fer::dev::pdl_begin();
-    const bool copy_tail = p.x != p.out;
-    const int tiles = (p.rows + p.tile - 1) / p.tile;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int r0 = tile * p.tile;
-        const int nr = min(p.tile, p.rows - r0);
-        __syncthreads();
-        for (int k = t; k < nr * p.half; k += kThreads) {
-            const int r = k / p.half, i = k - r * p.half;
-            int a = 0;
-            while (a + 1 < p.axes && i >= p.bound[a]) ++a;
-            const double turns = static_cast<double>(p.positions[static_cast<size_t>(r0 + r) * p.axes + a]) * sh_freq[i];
+    __syncthreads();
+    const long long items = static_cast<long long>(p.rows) * p.split;
+    for (long long item = static_cast<long long>(blockIdx.x) * kWarps + w; item < items;
+         item += static_cast<long long>(gridDim.x) * kWarps) {
+        const int r = static_cast<int>(p.split == 1 ? item : item / p.split);
+        const int part = p.split == 1 ? 0 : static_cast<int>(item - static_cast<long long>(r) * p.split);
+        const int end = min(p.heads, (part + 1) * p.share), first = part * p.share + h0;
+        const T* const row = static_cast<const T*>(p.x) + static_cast<size_t>(r) * p.xs;
+        T* const to = static_cast<T*>(p.out) + static_cast<size_t>(r) * p.os;
+        P a[kAhead], b[kAhead];
+        auto load = [&](int u, int hb) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int h = hb + k * p.hp;
+                if (h < end) {
+                    const T* src = row + h * p.head_dim + u * V;
+                    a[k] = *reinterpret_cast<const P*>(src);
+                    if (!INTER) b[k] = *reinterpret_cast<const P*>(src + p.half);
+                }
+            }
+        };
+        const bool lanes = h0 < p.hp;                                 // the lanes behind whole units rest
+        if (lanes && u0 < turned) load(u0, first);
+        const int32_t* const pos = p.positions + static_cast<size_t>(r) * p.axes;
+        __syncwarp();                                                 // the row before has been read out
+        for (int i = lane; i < p.half; i += 32) {
+            int x = 0;
+            while (x + 1 < p.axes && i >= p.bound[x]) ++x;
+            const double turns = static_cast<double>(pos[x]) * sh_freq[i];
             float s, c;
             sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-            sh_cs[k] = make_float2(c, s);
+            table[i] = make_float2(c, s);
         }
-        __syncthreads();
-        int u = t % p.units, h = t / p.units % p.heads, r = t / (p.units * p.heads);
-        while (r < nr) {
-            Vec<T, V, A> a[kAhead], b[kAhead];
-            int hu[kAhead], hh[kAhead], hr[kAhead];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                hu[k] = u, hh[k] = h, hr[k] = r;
-                if (r < nr) {
-                    const T* src = static_cast<const T*>(p.x) + static_cast<size_t>(r0 + r) * p.xs +
-                                   static_cast<size_t>(h) * p.head_dim;
-                    if (u < turned) {
-                        a[k] = *reinterpret_cast<const Vec<T, V, A>*>(src + u * V);
-                        if (!INTER) b[k] = *reinterpret_cast<const Vec<T, V, A>*>(src + p.half + u * V);
-                    } else if (copy_tail) {
-                        a[k] = *reinterpret_cast<const Vec<T, V, A>*>(src + 2 * p.half + (u - turned) * V);
-                    }
-                }
-                u += su;
-                h += sh;
-                r += sr;
-                if (u >= p.units) u -= p.units, ++h;
-                if (h >= p.heads) h -= p.heads, ++r;
+        __syncwarp();
+        if (!lanes) continue;
+        for (int u = u0; u < p.units; u += p.across) {
+            if (u >= turned) {
+                if (!copy_tail) break;
+                const int at = 2 * p.half + (u - turned) * V;
+                for (int h = first; h < end; h += p.hp)
+                    *reinterpret_cast<P*>(to + h * p.head_dim + at) = *reinterpret_cast<const P*>(row + h * p.head_dim + at);
+                continue;
             }
+            float2 cs[kPairs];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                if (hr[k] >= nr) continue;
-                T* dst = static_cast<T*>(p.out) + static_cast<size_t>(r0 + hr[k]) * p.os +
-                         static_cast<size_t>(hh[k]) * p.head_dim;
-                const float2* cs = sh_cs + hr[k] * p.half;
-                if (hu[k] >= turned) {
-                    if (copy_tail) *reinterpret_cast<Vec<T, V, A>*>(dst + 2 * p.half + (hu[k] - turned) * V) = a[k];
-                } else if constexpr (INTER) {
+            for (int e = 0; e < kPairs; ++e) cs[e] = table[u * kPairs + e];
+            for (int hb = first; hb < end; hb += kAhead * p.hp) {
+                if (u != u0 || hb != first) load(u, hb);
 #pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        const float2 w = cs[(hu[k] * V + e) / 2];
-                        const float x0 = to_f(a[k].e[e]), x1 = to_f(a[k].e[e + 1]);
-                        a[k].e[e] = static_cast<T>(x0 * w.x - x1 * w.y);
-                        a[k].e[e + 1] = static_cast<T>(x0 * w.y + x1 * w.x);
+                for (int k = 0; k < kAhead; ++k) {
+                    const int h = hb + k * p.hp;
+                    if (h >= end) break;
+                    T* dst = to + h * p.head_dim + u * V;
+                    float x[V], y[V];
+                    a[k].get(x);
+                    if constexpr (INTER) {
+#pragma unroll
+                        for (int e = 0; e < V; e += 2) {
+                            y[e] = x[e] * cs[e / 2].x - x[e + 1] * cs[e / 2].y;
+                            y[e + 1] = x[e] * cs[e / 2].y + x[e + 1] * cs[e / 2].x;
+                        }
+                        a[k].put(y);
+                        *reinterpret_cast<P*>(dst) = a[k];
+                    } else {
+                        float z[V];
+                        b[k].get(y);
+#pragma unroll
+                        for (int e = 0; e < V; ++e) {
+                            z[e] = x[e] * cs[e].y + y[e] * cs[e].x;
+                            x[e] = x[e] * cs[e].x - y[e] * cs[e].y;
+                        }
+                        a[k].put(x);
+                        b[k].put(z);
+                        *reinterpret_cast<P*>(dst) = a[k];
+                        *reinterpret_cast<P*>(dst + p.half) = b[k];
                     }
-                    *reinterpret_cast<Vec<T, V, A>*>(dst + hu[k] * V) = a[k];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        const float2 w = cs[hu[k] * V + e];
-                        const float x0 = to_f(a[k].e[e]), x1 = to_f(b[k].e[e]);
-                        a[k].e[e] = static_cast<T>(x0 * w.x - x1 * w.y);
-                        b[k].e[e] = static_cast<T>(x0 * w.y + x1 * w.x);
-                    }
-                    *reinterpret_cast<Vec<T, V, A>*>(dst + hu[k] * V) = a[k];
-                    *reinterpret_cast<Vec<T, V, A>*>(dst + p.half + hu[k] * V) = b[k];
                 }
             }
         }
@@ -144,15 +205,25 @@ template <typename T, int V, int A = V>
 cudaError_t launch(RotaryParams& p, cudaStream_t s) {
     const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
     p.units = (inter ? 2 * p.half : p.half) / V + (p.head_dim - 2 * p.half) / V;
-    // tiles of about four units a thread, at most 32 KB of cosines and sines
-    long long tile = 4ll * kThreads / (static_cast<long long>(p.units) * p.heads);
-    if (tile > 4096 / p.half) tile = 4096 / p.half;
-    p.tile = tile < 1 ? 1 : static_cast<int>(tile);
-    const int tiles = (p.rows + p.tile - 1) / p.tile;
-    const int grid = tiles < 148 * 6 ? tiles : 148 * 6;
-    const size_t smem = static_cast<size_t>(p.half) * (sizeof(double) + p.tile * sizeof(float2));
-    const cudaError_t e = inter ? fer::host::launch_pdl(rotary<T, V, A, true>, dim3(grid), dim3(kThreads), smem, s, p)
-                                : fer::host::launch_pdl(rotary<T, V, A, false>, dim3(grid), dim3(kThreads), smem, s, p);
+    p.across = p.units < 32 ? p.units : 32;
+    p.hp = 32 / p.across;
+    // a warp a row; where that leaves SMs without work, as many a row as have kAhead loads to make
+    const int turns = (p.heads + p.hp - 1) / p.hp;
+    int split = (148 * 2 * kWarps + p.rows - 1) / p.rows;
+    if (split > (turns + kAhead - 1) / kAhead) split = (turns + kAhead - 1) / kAhead;
+    p.share = ((turns + split - 1) / split) * p.hp;
+    p.split = (p.heads + p.share - 1) / p.share;
+    const long long ctas = (static_cast<long long>(p.rows) * p.split + kWarps - 1) / kWarps;
+    const int grid = static_cast<int>(ctas < 148 * 3 ? ctas : 148 * 3);
+    const size_t smem = static_cast<size_t>((p.half + 3) & ~3) * (sizeof(double) + kWarps * sizeof(float2));
+    cudaError_t e;
+    if constexpr (V > 1) {
+        if (inter) {
+            e = fer::host::launch_pdl(rotary<T, V, A, true>, dim3(grid), dim3(kThreads), smem, s, p);
+            return e != cudaSuccess ? e : cudaGetLastError();
+        }
+    }
+    e = fer::host::launch_pdl(rotary<T, V, A, false>, dim3(grid), dim3(kThreads), smem, s, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
