@@ -15,12 +15,16 @@
 // in order. Which CTA took a unit does not change its arithmetic: results are
 // the same run to run and for any batch.
 //
-// Inside a unit each of four warps takes every fourth slab of 16 slots through a ring of its own, filled by tensor copies of page rows
-// that run on into the next unit; the warps meet at a unit's end only.
-// Scores are S^T = K Q^T and outputs O^T = V^T P on 16-bit tensor-core tiles
-// with f32 accumulation: with slots as rows the 8 columns are the heads, so a
-// group of up to 8 heads wastes nothing it would have to read, and the
-// softmax of a head is a reduction over rows that stays in a warp. (One query
+// Inside a unit a warp loads rounds of 64 slots by tensor copies of page rows
+// into a ring, running on into the next units, and four warps compute. In a
+// round each of them takes 16 slots' scores for all heads, S^T = K Q^T; they
+// agree on the maxima, exchange their probabilities through shared memory as
+// ready operand fragments, and each then adds a quarter of the dims, O^T = V^T
+// P, over all 64 slots. So an output stays in one warp (no sums to be joined at a unit's end)
+// and takes few registers, and several CTAs share an SM and hide one
+// another's latencies. Products are 16-bit tensor-core tiles with f32
+// accumulation: with slots or dims as rows the 8 columns are the heads, so a
+// group of up to 8 heads wastes nothing it would have to read. (One query
 // gives 8 or 16 columns a tile at best, 1/16 of the 128 rows a tcgen05 tile
 // has, and the tiles here run at a few per cent of the tensor pipe anyway.)
 // P is kept as the sum of two 16-bit numbers, so it has 16 bits or more:
@@ -45,10 +49,10 @@
 namespace {
 
 using fer::dev::Paged;
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kSegments = 128;      // entries of the unit table in shared memory
-constexpr int kMeet = 2;            // heads whose parts meet at once
+constexpr int kWarps = 4;                        // that compute; one more loads
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kRound = 16 * kWarps;  // slots a round
+constexpr int kSegments = 128;       // entries of the unit table in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -98,6 +102,8 @@ __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t at) {
                  : "r"(at)
                  : "memory");
 }
+// Barrier of the computing warps.
+__device__ __forceinline__ void meet_warps() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); }
 // Transposes an 8 x 8 tile of 16-bit elements spread over the warp.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
@@ -147,30 +153,26 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     }
 }
 
-// How a head_dim is cut: slots a slab, slabs in flight a warp, CTAs an SM. A
-// slab's rows lie in bands of 64 dims, each as the copies write it: piece c
-// (16 bytes) of row r at r * 128 + ((c ^ (r % 8)) * 16), so eight rows' pieces
-// of one column are in different banks.
+// How a head_dim is cut: rounds in flight, CTAs an SM. A round's rows lie in
+// bands of 64 dims, each as the copies write it: piece c (16 bytes) of row r
+// at r * 128 + ((c ^ (r % 8)) * 16), so eight rows' pieces of one column are
+// in different banks.
 template <int D> struct Cut {
-    static constexpr int kSlab = 16;
-    static constexpr int kStages = D == 256 ? 2 : 3;
-    template <int NT> static constexpr int ctas() { return D == 64 ? (NT == 1 ? 4 : 3) : D == 128 ? 2 : 1; }
-    static constexpr int kBand = kSlab * 128;
+    static constexpr int kStages = D == 128 ? 2 : 3;
+    static constexpr int kCtas = D == 64 ? 4 : D == 128 ? 3 : 1;
+    static constexpr int kBand = kRound * 128;
     static constexpr int kHalf = D / 64 * kBand;             // keys; the values follow
     static constexpr int kStage = 2 * kHalf;
-    static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kMeetBytes = 2 * kWarps * kMeet * D * 4;
-    static constexpr int kSmem = kRing + kMeetBytes + 1024;  // bands start at 1024 bytes
+    static constexpr int kSmem = kStages * kStage + 1024;    // bands start at 1024 bytes
     // Byte of piece c of row r in a half of a stage.
     static __device__ __forceinline__ uint32_t at(int r, int c) {
         return (c >> 3) * kBand + r * 128 + (((c ^ r) & 7) << 4);
     }
 };
 
-// What a unit costs, in rounds of a slab for each warp: its rounds, and
-// kUnitCost more for its beginning and its end.
-constexpr int kUnitCost = 2;
-constexpr int kRound = 16 * kWarps;   // slots
+// What a unit costs, in rounds: its rounds, and kUnitCost more for its
+// beginning and its end.
+constexpr int kUnitCost = 1;
 __host__ __device__ inline int rounds_of(int n) { return (n + kRound - 1) / kRound; }
 
 // The units and the cost before every segment of sequences; in shared memory.
@@ -272,22 +274,23 @@ struct UnitRun {
 
 // Page ids of a unit's chunk (up to 64 pages) as the table has them: lane i
 // holds those of its i-th and (i + 32)-th page, -1 behind the last. They are
-// checked where they are used, so that a load for a later unit stays in flight.
+// checked where they are used, so that a load for a later unit stays in
+// flight. k0: first slot of the chunk.
 struct ChunkPages {
     int a, b;
-    __device__ __forceinline__ int of(const Paged& c, int slot) const {
-        const int i = slot >> c.shift;
+    __device__ __forceinline__ int of(const Paged& c, int k0, int slot) const {   // a slot of the chunk
+        const int i = ((k0 + slot) >> c.shift) - (k0 >> c.shift);
         const int x = __shfl_sync(0xffffffffu, a, i & 31), y = __shfl_sync(0xffffffffu, b, i & 31);
         return i < 32 ? x : y;
     }
-    __device__ __forceinline__ bool all_good(const Paged& c, int n) const {
-        const int lane = threadIdx.x & 31, last = (n - 1) >> c.shift;
+    __device__ __forceinline__ bool all_good(const Paged& c, const Unit& x, int k0) const {
+        const int lane = threadIdx.x & 31, last = ((k0 + x.n - 1) >> c.shift) - (k0 >> c.shift);
         return !__any_sync(0xffffffffu, (lane <= last && !c.is_page(a)) || (lane + 32 <= last && !c.is_page(b)));
     }
 };
 
 __device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x, int k0) {
-    const int lane = threadIdx.x & 31, last = (x.n - 1) >> c.shift;
+    const int lane = threadIdx.x & 31, last = ((k0 + x.n - 1) >> c.shift) - (k0 >> c.shift);
     const int32_t* row = c.table + static_cast<size_t>(x.b) * c.max_pages + (k0 >> c.shift) + lane;
     ChunkPages g{-1, -1};
     if (lane <= last) g.a = row[0];
@@ -296,20 +299,23 @@ __device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x, 
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
+__global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
     attn_units(const Paged c, const AttnParams p, const __grid_constant__ CUtensorMap k_map,
                const __grid_constant__ CUtensorMap v_map) {
     using C = Cut<D>;
     constexpr int kB = D / 16;                  // 16-wide blocks of a row
+    constexpr int kMine = D / 64;               // of them a warp's share of the output
     extern __shared__ uint8_t smem_raw[];
-    __shared__ int s_units[kSegments], s_cost[kSegments], s_sum[kWarps], s_cost_sum[kWarps];
-    __shared__ float s_ml[2][kWarps][8 * NT][2];
-    __shared__ uint64_t s_full[kWarps][C::kStages];
+    __shared__ int s_units[kSegments], s_cost[kSegments], s_sum[kWarps + 1], s_cost_sum[kWarps + 1];
+    __shared__ uint4 s_p[kWarps][NT][32];       // probabilities of 16 slots, as operand fragments
+    __shared__ float s_top[kWarps][8 * NT], s_l[kWarps][8 * NT];
+    __shared__ uint64_t s_full[C::kStages], s_empty[C::kStages];
+    __shared__ int s_good[C::kStages];          // the round's unit has no page id out of range
     uint8_t* const smem = smem_raw + (-fer::dev::smem_addr(smem_raw) & 1023u);
-    float* const meet = reinterpret_cast<float*>(smem + C::kRing);   // [2][kWarps][kMeet][D]
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-    if (lane == 0) {
-        for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&s_full[w][i], 1);
+    if (t < C::kStages) {
+        fer::dev::mbar_init(&s_full[t], 1);
+        fer::dev::mbar_init(&s_empty[t], kWarps);
         fer::dev::fence_mbar_init();
     }
     if (t == 0) {
@@ -347,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
         __syncthreads();
         x += carry - mine;
         y += cost_carry - cost;
-        for (int i = 0; i < kWarps; ++i) {
+        for (int i = 0; i <= kWarps; ++i) {
             if (i < w) x += s_sum[i], y += s_cost_sum[i];
             carry += s_sum[i];
             cost_carry += s_cost_sum[i];
@@ -377,23 +383,61 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
     }
     if (u0 >= u1) return;
 
-    uint8_t* const my_ring = smem + w * C::kStages * C::kStage;
-    const uint32_t ring = fer::dev::smem_addr(my_ring);
-    // a box: rows of one page, 64 dims
-    const int box_rows = min(C::kSlab, c.page_size()), row_boxes = C::kSlab / box_rows;
-    const int my_box = lane / (D / 64) % row_boxes, my_band = lane % (D / 64);
-    const bool my_value = lane >= D / 64 * row_boxes;
-    const bool loader = lane < 2 * (D / 64) * row_boxes;
-    const CUtensorMap* const my_map = my_value ? &v_map : &k_map;
-    const uint32_t my_place = (my_value ? C::kHalf : 0) + my_band * C::kBand + my_box * box_rows * 128;
-    const uint32_t full0 = fer::dev::smem_addr(&s_full[w][0]);
+    const uint32_t ring = fer::dev::smem_addr(smem);
     bool alive = true;   // no wait of this warp has run out
+    if (w == kWarps) {
+        // The loading warp: every unit's rounds in order, round q of the run
+        // into stage q % kStages. A box is rows of one page, 64 dims, a lane each.
+        const int box_rows = min(kRound, c.page_size()), row_boxes = kRound / box_rows;
+        const int boxes = 2 * (D / 64) * row_boxes;
+        const uint32_t full0 = fer::dev::smem_addr(&s_full[0]);
+        UnitRun run;
+        Unit x = run.get(c, p, table, u0, u1 - 1), next = x;
+        ChunkPages pages = load_pages(c, x, x.chunk << p.chunk_log2), ahead = pages;
+        int q = 0;
+        for (int u = u0; u < u1 && alive; ++u) {
+            if (u + 1 < u1) {   // the next unit's page ids are on their way meanwhile
+                next = run.get(c, p, table, u + 1, u1 - 1);
+                ahead = load_pages(c, next, next.chunk << p.chunk_log2);
+            }
+            const int k0 = x.chunk << p.chunk_log2;
+            const int good = pages.all_good(c, x, k0);
+            if (!good && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+            for (int r0 = 0; r0 < x.n; r0 += kRound, ++q) {
+                const int stage = q % C::kStages;
+                alive = __all_sync(0xffffffffu, fer::dev::mbar_wait(&s_empty[stage], (q / C::kStages & 1) ^ 1));
+                if (!alive) break;
+                if (lane == 0) {
+                    s_good[stage] = good;
+                    fer::dev::mbar_arrive_expect_tx(&s_full[stage], C::kStage);
+                }
+                for (int i = lane; i - lane < boxes; i += 32) {
+                    const int value = i >= boxes / 2, j = i - value * (boxes / 2);
+                    const int band = j % (D / 64), rows = j / (D / 64) * box_rows;
+                    // slots of no page are read as page `pages`, which is outside the map: zeros
+                    const int slot = r0 + min(rows, kRound - box_rows);
+                    const int id = pages.of(c, k0, slot);
+                    if (i < boxes)
+                        load_box(ring + stage * C::kStage + value * C::kHalf + band * C::kBand + rows * 128,
+                                 value ? &v_map : &k_map, band * 64, (k0 + slot) & (c.page_size() - 1), x.hk,
+                                 c.is_page(id) ? id : c.pages, full0 + 8 * stage);
+                }
+            }
+            x = next;
+            pages = ahead;
+        }
+        // the copies have landed before this warp leaves, whatever became of the others
+        for (int k = max(0, q - C::kStages); k < q; ++k)
+            alive = fer::dev::mbar_wait(&s_full[k % C::kStages], k / C::kStages & 1) && alive;
+        if (!alive && lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
+        return;
+    }
 
     // Queries as columns (heads lane / 4) of rows (dims 2 (lane % 4) + {0, 1}
     // and 8 more); columns behind the group's last head repeat its first and are
     // left out at the end. Those of the next unit are loaded a unit ahead
     // where the registers allow it.
-    constexpr bool kAhead = NT * kB <= 8;
+    constexpr bool kAhead = NT * kB <= 16;
     uint32_t qf[NT][kB][2], qn[NT][kB][2];
     auto load_q = [&](const Unit& x, uint32_t (&q)[NT][kB][2]) {
 #pragma unroll
@@ -414,52 +458,10 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
                 }
         }
     };
-    // What is being loaded: unit lu, slab li of it; its pages, and the next
-    // unit's on their way. Bit i of `broken`: the slab in stage i is of a unit
-    // with a page id out of range.
-    UnitRun load_run;
-    int lu = u0, li = w, loads = 0;
-    uint32_t broken = 0u;
-    Unit lx = load_run.get(c, p, table, u0, u1 - 1), nx = lx;
-    UnitRun run = load_run;
-    ChunkPages lp = load_pages(c, lx, lx.chunk << p.chunk_log2), np = lp;
-    Unit x = lx;   // what is being computed
+    UnitRun run;
+    Unit x = run.get(c, p, table, u0, u1 - 1);
     load_q(x, qf);
-    bool lgood = true;
-    auto look_ahead = [&]() {
-        lgood = lp.all_good(c, lx.n);
-        if (!lgood && w == 0 && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
-        if (lu + 1 < u1) {
-            nx = load_run.get(c, p, table, lu + 1, u1 - 1);
-            np = load_pages(c, nx, nx.chunk << p.chunk_log2);
-        }
-    };
-    look_ahead();
-    auto issue = [&]() {
-        while (lu < u1 && li * C::kSlab >= lx.n) {   // no slab of this unit is left for this warp
-            li = w;
-            lx = nx;
-            lp = np;
-            if (++lu < u1) look_ahead();
-        }
-        if (lu < u1) {
-            const int stage = loads % C::kStages;
-            broken = (broken & ~(1u << stage)) | (lgood ? 0u : 1u << stage);
-            // slots of no page are read as page `pages`, which is outside the map: zeros
-            const int slot = li * C::kSlab + my_box * box_rows;
-            const int id = lp.of(c, min(slot, p.chunk() - 1));
-            if (lane == 0) fer::dev::mbar_arrive_expect_tx(&s_full[w][stage], C::kStage);
-            if (loader)
-                load_box(ring + stage * C::kStage + my_place, my_map, my_band * 64, slot & (c.page_size() - 1), lx.hk,
-                         c.is_page(id) ? id : c.pages, full0 + 8 * stage);
-            li += kWarps;
-            ++loads;
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < C::kStages; ++i) issue();
-
-    int used = 0, turns = 0;
+    int q = 0;   // rounds of the run so far
     for (int u = u0; u < u1; ++u) {
         const int h0 = x.hk * p.group + x.blk * 8 * NT;          // first head of the block
         const int nh = min(8 * NT, p.group - x.blk * 8 * NT);    // its heads
@@ -468,137 +470,126 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
         const bool turn = next.b != x.b || next.hk != x.hk || next.blk != x.blk;
         if (kAhead && turn) load_q(next, qn);
 
-        float m[NT][2], l[NT][2], o[NT][kB][4];
+        // this lane's heads: 8 nt + 2 (lane % 4) + e. m is the same in all warps, l of this lane's slots
+        float m[NT][2], l[NT][2], o[NT][kMine][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kB; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.0f;
+            for (int k = 0; k < kMine; ++k) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.0f;
         }
-        for (int i = w; i * C::kSlab < x.n; i += kWarps) {
-            const bool good = !(broken >> (used % C::kStages) & 1u);
-            const int stage = used % C::kStages;
-            if (alive) alive = fer::dev::mbar_wait(&s_full[w][stage], used / C::kStages & 1);
+        for (int r0 = 0; r0 < x.n; r0 += kRound, ++q) {
+            const int stage = q % C::kStages;
+            if (alive) alive = fer::dev::mbar_wait(&s_full[stage], q / C::kStages & 1);
+            const bool good = s_good[stage];
             const uint32_t st = ring + stage * C::kStage;
-            ++used;
-            const int rows = x.n - i * C::kSlab;
-            if (rows < C::kSlab) {   // the values behind the last slot count as zero, whatever is there
-                uint4* v = reinterpret_cast<uint4*>(my_ring + stage * C::kStage + C::kHalf);
-                for (int q = lane; q < D / 8 * (C::kSlab - rows); q += 32) {
-                    const int band = q / (8 * (C::kSlab - rows)), rest = q % (8 * (C::kSlab - rows));
-                    v[band * (C::kBand / 16) + 8 * rows + rest] = make_uint4(0u, 0u, 0u, 0u);
-                }
+            const int rows = x.n - r0;           // held slots of the round, or more
+            if (rows < 16 * w + 16) {            // values behind the last slot count as zero, whatever is there
+                uint4* v = reinterpret_cast<uint4*>(smem + stage * C::kStage + C::kHalf);
+                const int from = max(rows, 16 * w), n = 8 * (16 * w + 16 - from);
+                for (int i = lane; i < D / 64 * n; i += 32)
+                    v[i / n * (C::kBand / 16) + 8 * from + i % n] = make_uint4(0u, 0u, 0u, 0u);
                 fer::dev::fence_proxy_async_smem();
-                __syncwarp();
             }
+            float s[NT][4];
             {
-                float s[NT][4];
-                {
-                    float s2[NT][4];
+                float s2[NT][4];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
-                    const int r = lane & 15;
+                    for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
+                const int r = 16 * w + (lane & 15);
 #pragma unroll
-                    for (int k = 0; k < kB; ++k) {
-                        uint32_t a[4];
-                        ldsm4(a, st + C::at(r, 2 * k + (lane >> 4)));
+                for (int k = 0; k < kB; ++k) {
+                    uint32_t a[4];
+                    ldsm4(a, st + C::at(r, 2 * k + (lane >> 4)));
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma<T>(k & 1 ? s2[nt] : s[nt], a, qf[nt][k][0], qf[nt][k][1]);
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * p.scale2;
+                    for (int nt = 0; nt < NT; ++nt) mma<T>(k & 1 ? s2[nt] : s[nt], a, qf[nt][k][0], qf[nt][k][1]);
                 }
-                const int j = i * C::kSlab + lane / 4;   // this lane's slots of the chunk: j, j + 8
-                bool on0 = j < x.n, on1 = j + 8 < x.n;
-                if (!good) {
-                    const ChunkPages pg = load_pages(c, x, k0);
-                    const int p0 = pg.of(c, min(j, x.n - 1)), p1 = pg.of(c, min(j + 8, x.n - 1));
-                    on0 = on0 && c.is_page(p0);
-                    on1 = on1 && c.is_page(p1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * p.scale2;
+            }
+            const int j = r0 + 16 * w + lane / 4;   // this lane's slots of the chunk: j, j + 8
+            bool on0 = j < x.n, on1 = j + 8 < x.n;
+            if (!good) {
+                const ChunkPages pg = load_pages(c, x, k0);
+                const int p0 = pg.of(c, k0, min(j, x.n - 1)), p1 = pg.of(c, k0, min(j + 8, x.n - 1));
+                on0 = on0 && c.is_page(p0);
+                on1 = on1 && c.is_page(p1);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (!on0) s[nt][e] = -INFINITY;
+                    if (!on1) s[nt][2 + e] = -INFINITY;
+                    float v = fmaxf(s[nt][e], s[nt][2 + e]);
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                    if (lane < 4) s_top[w][nt * 8 + 2 * lane + e] = v;
                 }
-                bool grew = false;
-                float next[NT][2];
+            if (p.scores) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        if (!on0) s[nt][e] = -INFINITY;
-                        if (!on1) s[nt][2 + e] = -INFINITY;
-                        float v = fmaxf(s[nt][e], s[nt][2 + e]);
-                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-                        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                        next[nt][e] = fmaxf(m[nt][e], v);
-                        grew |= next[nt][e] > m[nt][e];
+                        const int g = nt * 8 + 2 * (lane & 3) + e;
+                        float* row = p.scores + (static_cast<size_t>(x.b) * p.heads + h0 + g) * c.max_slots() + k0;
+                        if (g < nh && j < x.n) row[j] = s[nt][e];
+                        if (g < nh && j + 8 < x.n) row[j + 8] = s[nt][2 + e];
                     }
-                if (p.scores) {
+            }
+            meet_warps();
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int g = nt * 8 + 2 * (lane & 3) + e;
-                            float* row = p.scores + (static_cast<size_t>(x.b) * p.heads + h0 + g) * c.max_slots() + k0;
-                            if (g < nh && j < x.n) row[j] = s[nt][e];
-                            if (g < nh && j + 8 < x.n) row[j + 8] = s[nt][2 + e];
-                        }
+                for (int e = 0; e < 2; ++e) {
+                    float top = m[nt][e];
+#pragma unroll
+                    for (int v = 0; v < kWarps; ++v) top = fmaxf(top, s_top[v][nt * 8 + 2 * (lane & 3) + e]);
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    const float f = ex2(m[nt][e] - base);   // 1 where the maximum stays
+                    m[nt][e] = top;
+                    s[nt][e] = ex2(s[nt][e] - base);
+                    s[nt][2 + e] = ex2(s[nt][2 + e] - base);
+                    l[nt][e] = l[nt][e] * f + (s[nt][e] + s[nt][2 + e]);
+#pragma unroll
+                    for (int k = 0; k < kMine; ++k) o[nt][k][e] *= f, o[nt][k][2 + e] *= f;
                 }
-                if (__any_sync(0xffffffffu, grew)) {
+                uint4 f;
+                split2<T>(s[nt][0], s[nt][1], f.x, f.z);
+                split2<T>(s[nt][2], s[nt][3], f.y, f.w);
+                f.x = transpose8(f.x), f.y = transpose8(f.y), f.z = transpose8(f.z), f.w = transpose8(f.w);
+                s_p[w][nt][lane] = f;
+            }
+            meet_warps();
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+            for (int v = 0; v < kWarps; ++v) {
+                if (16 * v >= rows) break;
+                uint4 f[NT];
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float f = ex2(m[nt][e] - (next[nt][e] == -INFINITY ? 0.0f : next[nt][e]));
-                            m[nt][e] = next[nt][e];
-                            l[nt][e] *= f;
+                for (int nt = 0; nt < NT; ++nt) f[nt] = s_p[v][nt][lane];
+                const int r = 16 * v + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-                            for (int k = 0; k < kB; ++k) o[nt][k][e] *= f, o[nt][k][2 + e] *= f;
-                        }
-                }
-                uint32_t hi[NT][2], lo[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float base = m[nt][e] == -INFINITY ? 0.0f : m[nt][e];
-                        s[nt][e] = ex2(s[nt][e] - base);
-                        s[nt][2 + e] = ex2(s[nt][2 + e] - base);
-                        l[nt][e] += s[nt][e] + s[nt][2 + e];
-                    }
-                    split2<T>(s[nt][0], s[nt][1], hi[nt][0], lo[nt][0]);
-                    split2<T>(s[nt][2], s[nt][3], hi[nt][1], lo[nt][1]);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        hi[nt][e] = transpose8(hi[nt][e]);
-                        lo[nt][e] = transpose8(lo[nt][e]);
-                    }
-                }
-                const int r = (lane & 7) + ((lane >> 4) << 3);
-#pragma unroll
-                for (int k = 0; k < kB; ++k) {
+                for (int k = 0; k < kMine; ++k) {
                     uint32_t a[4];
-                    ldsm4_t(a, st + C::kHalf + C::at(r, 2 * k + ((lane >> 3) & 1)));
+                    ldsm4_t(a, st + C::kHalf + C::at(r, 2 * (w * kMine + k) + ((lane >> 3) & 1)));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma<T>(o[nt][k], a, lo[nt][0], lo[nt][1]);
-                        mma<T>(o[nt][k], a, hi[nt][0], hi[nt][1]);
+                        mma<T>(o[nt][k], a, f[nt].z, f[nt].w);
+                        mma<T>(o[nt][k], a, f[nt].x, f[nt].y);
                     }
                 }
             }
             __syncwarp();
-            issue();   // into the stage that was just read
+            if (lane == 0) fer::dev::mbar_arrive(&s_empty[stage]);
         }
 
-        // The warps' parts meet in shared memory, kMeet heads at a time in two
-        // areas by turns, so that one barrier a time is enough: who writes an
-        // area again has passed the barrier behind its last readers.
-        const bool whole = x.chunks == 1;
-        const size_t bh0 = static_cast<size_t>(x.b) * p.heads + h0;
-        float(*const ml)[8 * NT][2] = s_ml[u & 1];
+        // the unit's sums, and each warp's dims of its result
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -606,57 +597,38 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 4);
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 8);
                 l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], 16);
-                if (lane < 4) {
-                    ml[w][nt * 8 + 2 * lane + e][0] = m[nt][e];
-                    ml[w][nt * 8 + 2 * lane + e][1] = l[nt][e];
-                }
+                if (lane < 4) s_l[w][nt * 8 + 2 * lane + e] = l[nt][e];
             }
+        meet_warps();
+        const bool whole = x.chunks == 1;
+        constexpr float kBack = 1.0f / kScaleP<T>;
 #pragma unroll
-        for (int q = 0; q < 4 * NT; ++q) {   // heads 2 q and 2 q + 1, held by the lanes with lane % 4 == q % 4
-            if (2 * q >= nh) break;
-            float* const area = meet + turns * (kWarps * kMeet * D);
-            turns ^= 1;
-            if ((lane & 3) == (q & 3)) {
-                float* const mine = area + w * kMeet * D + lane / 4;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int k = 0; k < kB; ++k)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mine[(e & 1) * D + 16 * k + 8 * (e >> 1)] = o[q / 4][k][e];
-            }
-            __syncthreads();
-            for (int i = t; i < kMeet * (D / 4); i += kThreads) {
-                const int e = i / (D / 4), g = 2 * q + e, d = i % (D / 4) * 4;
+            for (int e = 0; e < 2; ++e) {
+                const int g = nt * 8 + 2 * (lane & 3) + e;
                 if (g >= nh) continue;
-                float top = -INFINITY, sum = 0.0f;
+                float sum = 0.0f;
 #pragma unroll
-                for (int v = 0; v < kWarps; ++v) top = fmaxf(top, ml[v][g][0]);
-                const float base = top == -INFINITY ? 0.0f : top;
-                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int v = 0; v < kWarps; ++v) sum += s_l[v][g];
+                const size_t bh = static_cast<size_t>(x.b) * p.heads + h0 + g, at = bh * p.chunks + x.chunk;
+                if (w == 0 && lane < 4) {
+                    *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(m[nt][e], sum);
+                    if (whole && p.lse) p.lse[bh] = sum == 0.0f ? -INFINITY : (m[nt][e] + log2f(sum)) * kLn2;
+                }
+                const float f = !whole ? kBack : sum == 0.0f ? 0.0f : kBack / sum;
+                T* const out = static_cast<T*>(p.out) + x.b * p.os + static_cast<size_t>(h0 + g) * D;
+                float* const part = p.part_o + at * D;
 #pragma unroll
-                for (int v = 0; v < kWarps; ++v) {
-                    const float f = ex2(ml[v][g][0] - base);
-                    const float4 y = *reinterpret_cast<const float4*>(area + (v * kMeet + e) * D + d);
-                    sum += ml[v][g][1] * f;
-                    a.x += y.x * f, a.y += y.y * f, a.z += y.z * f, a.w += y.w * f;
-                }
-                constexpr float kBack = 1.0f / kScaleP<T>;
-                const size_t at = (bh0 + g) * p.chunks + x.chunk;
-                if (d == 0) {
-                    *reinterpret_cast<float2*>(p.part_ml + 2 * at) = make_float2(top, sum);
-                    if (whole && p.lse) p.lse[bh0 + g] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-                }
-                if (whole) {
-                    const float f = sum == 0.0f ? 0.0f : kBack / sum;
-                    T* out = static_cast<T*>(p.out) + x.b * p.os + static_cast<size_t>(h0 + g) * D + d;
-                    const float v[4] = {a.x, a.y, a.z, a.w};
+                for (int k = 0; k < kMine; ++k)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) out[k] = static_cast<T>(sum == 0.0f ? 0.0f : v[k] * f);
-                } else {
-                    *reinterpret_cast<float4*>(p.part_o + at * D + d) =
-                        make_float4(a.x * kBack, a.y * kBack, a.z * kBack, a.w * kBack);
-                }
+                    for (int r = 0; r < 2; ++r) {
+                        const int d = 16 * (w * kMine + k) + 8 * r + lane / 4;
+                        const float v = o[nt][k][2 * r + e] * f;
+                        if (whole) out[d] = static_cast<T>(sum == 0.0f ? 0.0f : v);
+                        else part[d] = v;
+                    }
             }
-        }
         if (turn) {
             if constexpr (kAhead) {
 #pragma unroll
@@ -669,11 +641,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::template ctas<NT>())
         }
         x = next;
     }
-    if (!alive) {   // let the last copies land, bounded as well, before the memory goes away
-        if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
-        for (int k = max(0, loads - C::kStages); k < loads; ++k)
-            fer::dev::mbar_wait(&s_full[w][k % C::kStages], k / C::kStages & 1);
-    }
+    if (!alive && lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
 }
 
 // log2 of a head's total sum of powers, from its chunks' (m, l), by one warp;
@@ -841,7 +809,7 @@ cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT>), smem, known);
     if (ctas <= 0) return cudaErrorInvalidConfiguration;
     CUtensorMap k_map, v_map;
-    const int rows = Cut<D>::kSlab < c.page_size() ? Cut<D>::kSlab : c.page_size();
+    const int rows = kRound < c.page_size() ? kRound : c.page_size();
     const uint32_t dtype = __is_same(T, __half) ? 1 : 2;
     if (!map_pages(&k_map, c, c.k, dtype, rows) || !map_pages(&v_map, c, c.v, dtype, rows)) return cudaErrorInvalidValue;
     const long long most = static_cast<long long>(p.n_seq) * c.kv_heads * p.blocks * p.chunks;
