@@ -679,14 +679,15 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float*
     return l == 0.0f ? -INFINITY : *base + log2f(l);
 }
 
-// grid (group + weight tiles, kv_heads, n_seq). The first `group` CTAs of a
-// (key head, sequence) add one head's chunks each (in order within a warp,
-// then the warps in order); the others add probabilities to the
-// weights of four slots a thread.
+// grid (group * D / 32 + weight tiles, kv_heads, n_seq). The first CTAs of a
+// (key head, sequence) add one head's chunks for 32 dims each (in order within
+// a warp, then the warps in order); the others add probabilities to the
+// weights of four slots a thread. Both have what does not depend on the
+// total in flight before they wait for it.
 template <typename T, int D, int kFinish>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
-    constexpr int kW = kFinish / 32, kV = D / 32;    // warps; dims a lane
-    __shared__ float s_o[kW][D];
+    constexpr int kW = kFinish / 32, kBands = D / 32, kAhead = 16, kHeads = 4;
+    __shared__ float s_o[kW][32];
     __shared__ float s_lse[kFinish];
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     const int b = blockIdx.z, hk = blockIdx.y;
@@ -695,40 +696,48 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
     const int len = c.length(b, &bad);
     const int chunks = p.chunks_of(len);
     const size_t bh0 = static_cast<size_t>(b) * p.heads + static_cast<size_t>(hk) * p.group;
-    if (static_cast<int>(blockIdx.x) < p.group) {
+    if (static_cast<int>(blockIdx.x) < p.group * kBands) {
         if (chunks <= 1) return;                      // written already
-        const size_t bh = bh0 + blockIdx.x;
+        const int g = blockIdx.x / kBands, d = blockIdx.x % kBands * 32 + lane;
+        const size_t bh = bh0 + g;
         const float* ml = p.part_ml + 2 * bh * p.chunks;
-        const float* po = p.part_o + bh * p.chunks * D + lane;
-        float base, l;
+        const float* po = p.part_o + bh * p.chunks * D + d;
+        float v[kAhead], m[kAhead], base, l, o = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = w + k * kW;
+            v[k] = 0.0f, m[k] = -INFINITY;
+            if (i < chunks) v[k] = po[static_cast<size_t>(i) * D], m[k] = ml[2 * i];
+        }
         const float lse2 = chunks_lse2(ml, chunks, &base, &l);
-        float o[kV];
 #pragma unroll
-        for (int e = 0; e < kV; ++e) o[e] = 0.0f;
-        if (w < chunks) {
-#pragma unroll 8
-            for (int i = w; i < chunks; i += kW) {
-                const float f = ex2(ml[2 * i] - base);
-#pragma unroll
-                for (int e = 0; e < kV; ++e) o[e] = fmaf(po[static_cast<size_t>(i) * D + e * 32], f, o[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < kV; ++e) s_o[w][e * 32 + lane] = o[e];
-        }
+        for (int k = 0; k < kAhead; ++k)
+            if (w + k * kW < chunks) o = fmaf(v[k], ex2(m[k] - base), o);
+        for (int i = w + kAhead * kW; i < chunks; i += kW)
+            o = fmaf(po[static_cast<size_t>(i) * D], ex2(ml[2 * i] - base), o);
+        s_o[w][lane] = o;
         __syncthreads();
-        for (int d = t; d < D; d += kFinish) {
-            float v = 0.0f;
-            for (int i = 0; i < min(kW, chunks); ++i) v += s_o[i][d];
-            static_cast<T*>(p.out)[b * p.os + (static_cast<size_t>(hk) * p.group + blockIdx.x) * D + d] =
-                static_cast<T>(l == 0.0f ? 0.0f : v / l);
-        }
-        if (t == 0 && p.lse) p.lse[bh] = lse2 * kLn2;
+        if (w > 0) return;
+        o = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) o += s_o[i][lane];
+        static_cast<T*>(p.out)[b * p.os + (static_cast<size_t>(hk) * p.group + g) * D + d] =
+            static_cast<T>(l == 0.0f ? 0.0f : o / l);
+        if (d == 0 && p.lse) p.lse[bh] = lse2 * kLn2;
         return;
     }
-    const int j0 = (blockIdx.x - p.group) * 4 * kFinish;
+    const int j0 = (blockIdx.x - p.group * kBands) * 4 * kFinish;
     if (j0 >= len) return;
     const int j = j0 + 4 * t;
     const size_t most = static_cast<size_t>(c.max_slots());   // a multiple of 8: rows start at 16 bytes
+    const bool on = j < len, whole = j + 3 < len && reinterpret_cast<uintptr_t>(p.weights) % 16 == 0;
+    const float* const scores = p.scores + bh0 * most + j;
+    float* const out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most + j;
+    float4 s[kHeads], old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (whole) old = *reinterpret_cast<const float4*>(out);
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k)
+        if (on && k < p.group) s[k] = *reinterpret_cast<const float4*>(scores + k * most);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int g0 = 0; g0 < p.group; g0 += kFinish) {
         const int ng = min(kFinish, p.group - g0);
@@ -739,23 +748,25 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
             if (lane == 0) s_lse[g] = v;
         }
         __syncthreads();
-        if (j >= len) continue;
-#pragma unroll 4
-        for (int g = 0; g < ng; ++g) {
-            const float4 s = *reinterpret_cast<const float4*>(p.scores + (bh0 + g0 + g) * most + j);
-            const float lse2 = s_lse[g];
-            if (lse2 == -INFINITY) continue;
-            sum[0] += ex2(s.x - lse2);
-            sum[1] += ex2(s.y - lse2);
-            sum[2] += ex2(s.z - lse2);
-            sum[3] += ex2(s.w - lse2);
+        if (!on) continue;
+        for (int g = 0; g < ng; g += kHeads) {
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k)
+                if ((g0 > 0 || g > 0) && g + k < ng) s[k] = *reinterpret_cast<const float4*>(scores + (g0 + g + k) * most);
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k) {
+                if (g + k >= ng) break;
+                const float lse2 = s_lse[g + k];
+                if (lse2 == -INFINITY) continue;
+                sum[0] += ex2(s[k].x - lse2);
+                sum[1] += ex2(s[k].y - lse2);
+                sum[2] += ex2(s[k].z - lse2);
+                sum[3] += ex2(s[k].w - lse2);
+            }
         }
     }
-    float* out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most + j;
-    if (j + 3 < len && reinterpret_cast<uintptr_t>(p.weights) % 16 == 0) {
-        float4 v = *reinterpret_cast<float4*>(out);
-        v.x += sum[0], v.y += sum[1], v.z += sum[2], v.w += sum[3];
-        *reinterpret_cast<float4*>(out) = v;
+    if (whole) {
+        *reinterpret_cast<float4*>(out) = make_float4(old.x + sum[0], old.y + sum[1], old.z + sum[2], old.w + sum[3]);
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -797,8 +808,8 @@ bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int r
 template <typename T, int D, int THREADS>
 cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
     const int tiles = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0;
-    return fer::host::launch_pdl(attn_finish<T, D, THREADS>, dim3(p.group + tiles, c.kv_heads, p.n_seq), dim3(THREADS),
-                                 0, s, c, p);
+    return fer::host::launch_pdl(attn_finish<T, D, THREADS>, dim3(p.group * (D / 32) + tiles, c.kv_heads, p.n_seq),
+                                 dim3(THREADS), 0, s, c, p);
 }
 
 template <typename T, int D, int NT>
