@@ -679,17 +679,18 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float*
     return l == 0.0f ? -INFINITY : *base + log2f(l);
 }
 
-// grid (group * D / 32 + weight tiles, kv_heads, n_seq). The first CTAs of a
-// (key head, sequence) add one head's chunks for 32 dims each (in order within
-// a warp, then the warps in order); the others add probabilities to the
-// weights of four slots a thread. Both have what does not depend on the
-// total in flight before they wait for it.
-template <typename T, int D, int kFinish>
+// grid (group * D / DIMS + weight tiles, kv_heads, n_seq). The first CTAs of a
+// (key head, sequence) add one head's chunks for DIMS dims each: a warp takes
+// 32 of them and every kW-th chunk in order, then the warps' sums are added in
+// order. The others add probabilities to the weights of four slots a thread.
+// Both have what does not depend on the total in flight before they wait for
+// it.
+template <typename T, int D, int kFinish, int DIMS>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
-    constexpr int kW = kFinish / 32, kBands = D / 32, kAhead = 16, kHeads = 4;
-    __shared__ float s_o[kW][32];
+    constexpr int kIn = DIMS / 32, kW = kFinish / 32 / kIn, kBands = D / DIMS, kAhead = 16, kHeads = 4;
+    __shared__ float s_o[kW][DIMS];
     __shared__ float s_lse[kFinish];
-    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    const int t = threadIdx.x, lane = t & 31, w = (t >> 5) / kIn;
     const int b = blockIdx.z, hk = blockIdx.y;
     fer::dev::pdl_begin();
     bool bad;
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
     const size_t bh0 = static_cast<size_t>(b) * p.heads + static_cast<size_t>(hk) * p.group;
     if (static_cast<int>(blockIdx.x) < p.group * kBands) {
         if (chunks <= 1) return;                      // written already
-        const int g = blockIdx.x / kBands, d = blockIdx.x % kBands * 32 + lane;
+        const int g = blockIdx.x / kBands, in = t % DIMS, d = blockIdx.x % kBands * DIMS + in;
         const size_t bh = bh0 + g;
         const float* ml = p.part_ml + 2 * bh * p.chunks;
         const float* po = p.part_o + bh * p.chunks * D + d;
@@ -715,12 +716,14 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
             if (w + k * kW < chunks) o = fmaf(v[k], ex2(m[k] - base), o);
         for (int i = w + kAhead * kW; i < chunks; i += kW)
             o = fmaf(po[static_cast<size_t>(i) * D], ex2(ml[2 * i] - base), o);
-        s_o[w][lane] = o;
-        __syncthreads();
-        if (w > 0) return;
-        o = 0.0f;
+        if constexpr (kW > 1) {
+            s_o[w][in] = o;
+            __syncthreads();
+            if (w > 0) return;
+            o = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kW; ++i) o += s_o[i][lane];
+            for (int i = 0; i < kW; ++i) o += s_o[i][in];
+        }
         static_cast<T*>(p.out)[b * p.os + (static_cast<size_t>(hk) * p.group + g) * D + d] =
             static_cast<T>(l == 0.0f ? 0.0f : o / l);
         if (d == 0 && p.lse) p.lse[bh] = lse2 * kLn2;
@@ -742,7 +745,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
     for (int g0 = 0; g0 < p.group; g0 += kFinish) {
         const int ng = min(kFinish, p.group - g0);
         __syncthreads();
-        for (int g = w; g < ng; g += kW) {
+        for (int g = t >> 5; g < ng; g += kFinish / 32) {
             float base, l;
             const float v = chunks_lse2(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks, &base, &l);
             if (lane == 0) s_lse[g] = v;
@@ -803,12 +806,10 @@ bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int r
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A warp a chunk at a time: four warps where a head has few chunks, sixteen
-// where there are many to read.
-template <typename T, int D, int THREADS>
+template <typename T, int D, int THREADS, int DIMS>
 cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
     const int tiles = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0;
-    return fer::host::launch_pdl(attn_finish<T, D, THREADS>, dim3(p.group * (D / 32) + tiles, c.kv_heads, p.n_seq),
+    return fer::host::launch_pdl(attn_finish<T, D, THREADS, DIMS>, dim3(p.group * (D / DIMS) + tiles, c.kv_heads, p.n_seq),
                                  dim3(THREADS), 0, s, c, p);
 }
 
@@ -827,7 +828,8 @@ cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     cudaError_t e = launch_pdl(attn_units<T, D, NT>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
                                dim3(kThreads), smem, s, c, p, k_map, v_map);
     if (e == cudaSuccess && (p.weights || p.chunks > 1))
-        e = p.chunks <= 32 ? finish<T, D, 128>(c, p, s) : finish<T, D, 512>(c, p, s);
+        // few chunks: a head a CTA; many: sixteen warps for 32 dims, whose loads one SM could not have in flight
+        e = p.chunks <= 32 ? finish<T, D, 256, D>(c, p, s) : finish<T, D, 512, 32>(c, p, s);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
