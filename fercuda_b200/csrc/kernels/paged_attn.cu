@@ -646,24 +646,25 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
 
 // log2 of a head's total sum of powers, from its chunks' (m, l), by one warp;
 // -inf where nothing counts. The base of the sum, and the sum, go to the two
-// others.
+// others. BATCH loads a lane are in flight.
+template <int BATCH>
 __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float* base, float* sum) {
     const int lane = threadIdx.x & 31;
     float top = -INFINITY, l = 0.0f;
-    for (int i0 = lane; i0 < chunks; i0 += 32 * 8) {
-        float2 v[8];
+    for (int i0 = lane; i0 < chunks; i0 += 32 * BATCH) {
+        float2 v[BATCH];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < BATCH; ++k) {
             v[k] = make_float2(-INFINITY, 0.0f);
             if (i0 + 32 * k < chunks) v[k] = *reinterpret_cast<const float2*>(ml + 2 * (i0 + 32 * k));
         }
         float next = top;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) next = fmaxf(next, v[k].x);
+        for (int k = 0; k < BATCH; ++k) next = fmaxf(next, v[k].x);
         const float b = next == -INFINITY ? 0.0f : next;
         l *= ex2(top - b);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) l += v[k].y * ex2(v[k].x - b);
+        for (int k = 0; k < BATCH; ++k) l += v[k].y * ex2(v[k].x - b);
         top = next;
     }
 #pragma unroll
@@ -687,7 +688,8 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float*
 // it.
 template <typename T, int D, int kFinish, int DIMS>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
-    constexpr int kIn = DIMS / 32, kW = kFinish / 32 / kIn, kBands = D / DIMS, kAhead = 16, kHeads = 4;
+    constexpr int kIn = DIMS / 32, kW = kFinish / 32 / kIn, kBands = D / DIMS, kHeads = 4;
+    constexpr int kAhead = DIMS == D ? 8 : 16, kBatch = DIMS == D ? 1 : 8;
     __shared__ float s_o[kW][DIMS];
     __shared__ float s_lse[kFinish];
     const int t = threadIdx.x, lane = t & 31, w = (t >> 5) / kIn;
@@ -710,10 +712,11 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
             v[k] = 0.0f, m[k] = -INFINITY;
             if (i < chunks) v[k] = po[static_cast<size_t>(i) * D], m[k] = ml[2 * i];
         }
-        const float lse2 = chunks_lse2(ml, chunks, &base, &l);
+        const float lse2 = chunks_lse2<kBatch>(ml, chunks, &base, &l);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
             if (w + k * kW < chunks) o = fmaf(v[k], ex2(m[k] - base), o);
+#pragma unroll 4
         for (int i = w + kAhead * kW; i < chunks; i += kW)
             o = fmaf(po[static_cast<size_t>(i) * D], ex2(ml[2 * i] - base), o);
         if constexpr (kW > 1) {
@@ -747,7 +750,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
         __syncthreads();
         for (int g = t >> 5; g < ng; g += kFinish / 32) {
             float base, l;
-            const float v = chunks_lse2(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks, &base, &l);
+            const float v = chunks_lse2<kBatch>(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks, &base, &l);
             if (lane == 0) s_lse[g] = v;
         }
         __syncthreads();
