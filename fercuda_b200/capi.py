@@ -9,7 +9,9 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
+from typing import NamedTuple
 
 import numpy as np
 
@@ -335,10 +337,10 @@ CAPI_PROTOTYPES = {
     "fer_submit_rows": (S, [P, C.POINTER(fer_rows_request_t), pu64]),
     "fer_jit_run_chain_f32": (S, [P, C.POINTER(fer_chain_op_t), u32, pu64, u32, u64, pu64]),
     "fer_submit_gemm": (S, [P, C.POINTER(fer_gemm_request_t), pu64]),
-    "fer_submit_rotary": (S, [P, C.POINTER(fer_rotary_request_t), pu64]),
-    "fer_submit_paged_store": (S, [P, C.POINTER(fer_paged_store_request_t), pu64]),
-    "fer_submit_paged_attention": (S, [P, C.POINTER(fer_paged_attention_request_t), pu64]),
-    "fer_submit_paged_evict": (S, [P, C.POINTER(fer_paged_evict_request_t), pu64]),
+    "fer_submit_rotary": (S, [P, P, pu64]),   # fer_rotary_request_t*
+    "fer_submit_paged_store": (S, [P, P, pu64]),   # fer_paged_store_request_t*
+    "fer_submit_paged_attention": (S, [P, P, pu64]),   # fer_paged_attention_request_t*
+    "fer_submit_paged_evict": (S, [P, P, pu64]),   # fer_paged_evict_request_t*
     "fer_transformer_create": (S, [P, C.POINTER(fer_transformer_config_t), pu64]),
     "fer_transformer_init_weights": (S, [P, u64, u64, f32]),
     "fer_transformer_weight_buffer": (S, [P, u64, pu64]),
@@ -517,12 +519,25 @@ def transformer_shard(global_batch: int, world: int, rank: int) -> tuple[int, in
     return first.value, count.value
 
 
-_SECTIONS = C.c_uint32 * 4
+class PagedCache(NamedTuple):
+    """A paged key-value cache: four buffer ids."""
+    k: int
+    v: int
+    page_table: int
+    lengths: int
 
 
-def paged_cache(k: int, v: int, page_table: int, lengths: int) -> fer_paged_cache_t:
-    """A paged key-value cache of four buffer ids."""
-    return fer_paged_cache_t(k, v, page_table, lengths)
+def paged_cache(k: int, v: int, page_table: int, lengths: int) -> PagedCache:
+    return PagedCache(k, v, page_table, lengths)
+
+
+# The requests of the per-token calls, packed as their ctypes mirrors above lie
+# in memory: building one of those takes longer than the call.
+_NONE = (0, 0, 0, 0)
+_pack_rotary = struct.Struct("=3Q10IfI").pack
+_pack_store = struct.Struct("=12Q2I").pack
+_pack_attention = struct.Struct("=9Q3If").pack
+_pack_evict = struct.Struct("=11Q2I").pack
 
 
 def paged_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_slots: int,
@@ -638,9 +653,9 @@ class Session:
         check("fer_submit_gemm", self.call("fer_submit_gemm", C.byref(r), C.byref(job)))
         return job.value
 
-    def _submit(self, fn, request) -> int:
+    def _submit(self, fn, request: bytes) -> int:
         """One fer_submit_* call; its job id."""
-        st = fn(self.ptr, C.byref(request), self._job_ref)
+        st = fn(self.ptr, request, self._job_ref)
         if st.code:
             raise FerError(fn.__name__, st)
         return self._job.value
@@ -653,25 +668,25 @@ class Session:
             raise ValueError("rotary takes 1 to 4 axes")
         flags = ((FER_ROTARY_INTERLEAVED if interleaved else 0) | (FER_ROTARY_AXIS_FREQS if axis_freqs else 0) |
                  (FER_ROTARY_INVERSE if inverse else 0))
-        return self._submit(self.lib.fer_submit_rotary, fer_rotary_request_t(
-            x, out, positions, x_col, out_col, heads, head_dim, rotary_dim, len(sections), _SECTIONS(*sections), base,
-            flags))
+        axes = len(sections)
+        return self._submit(self.lib.fer_submit_rotary, _pack_rotary(
+            x, out, positions, x_col, out_col, heads, head_dim, rotary_dim, axes, *sections, *_NONE[axes:], base, flags))
 
-    def paged_store(self, cache: fer_paged_cache_t, k_rows: int, v_rows: int, *, k_col: int = 0, v_col: int = 0,
+    def paged_store(self, cache: PagedCache, k_rows: int, v_rows: int, *, k_col: int = 0, v_col: int = 0,
                     offsets: int = 0, new_lengths: int = 0, weights: int = 0, positions: int = 0, seen: int = 0,
                     new_seen: int = 0) -> int:
-        return self._submit(self.lib.fer_submit_paged_store, fer_paged_store_request_t(
-            cache, k_rows, v_rows, offsets, new_lengths, weights, positions, seen, new_seen, k_col, v_col))
+        return self._submit(self.lib.fer_submit_paged_store, _pack_store(
+            *cache, k_rows, v_rows, offsets, new_lengths, weights, positions, seen, new_seen, k_col, v_col))
 
-    def paged_attention(self, cache: fer_paged_cache_t, q: int, out: int, heads: int, *, workspace: int,
+    def paged_attention(self, cache: PagedCache, q: int, out: int, heads: int, *, workspace: int,
                         q_col: int = 0, out_col: int = 0, scale: float = 0.0, lse: int = 0, weights: int = 0) -> int:
-        return self._submit(self.lib.fer_submit_paged_attention, fer_paged_attention_request_t(
-            cache, q, out, lse, weights, workspace, q_col, out_col, heads, scale))
+        return self._submit(self.lib.fer_submit_paged_attention, _pack_attention(
+            *cache, q, out, lse, weights, workspace, q_col, out_col, heads, scale))
 
-    def paged_evict(self, cache: fer_paged_cache_t, budget: int, recent: int, weights: int, positions: int, seen: int,
+    def paged_evict(self, cache: PagedCache, budget: int, recent: int, weights: int, positions: int, seen: int,
                     *, workspace: int, new_lengths: int = 0, new_weights: int = 0, new_positions: int = 0) -> int:
-        return self._submit(self.lib.fer_submit_paged_evict, fer_paged_evict_request_t(
-            cache, weights, positions, seen, new_lengths, new_weights, new_positions, workspace, budget, recent))
+        return self._submit(self.lib.fer_submit_paged_evict, _pack_evict(
+            *cache, weights, positions, seen, new_lengths, new_weights, new_positions, workspace, budget, recent))
 
     def import_ptr(self, dtype: int, shape, ptr: int) -> int:
         """Registers external device memory (e.g. a torch tensor) as a buffer."""

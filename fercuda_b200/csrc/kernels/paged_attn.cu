@@ -36,8 +36,8 @@
 //
 // A chunk whose scores are all -inf has l = 0 and counts as empty (m = 0 in
 // its exponents, so no inf - inf); l = 0 over all chunks gives zeros.
+#include "launch.cuh"
 #include "paged.cuh"
-#include "pdl.cuh"
 #include "tmap.cuh"
 
 #include <cuda_bf16.h>
@@ -782,10 +782,9 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
 
 // CTAs of a kernel that fit on the current device at once; 0 on an error. The
 // answer is kept per device, where the shared-memory limit is also set.
-constexpr int kDevices = 64;
 int resident(const void* kernel, int smem, std::atomic<int>* known) {
     int dev = 0, n = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= fer::host::kMaxDevices) return 0;
     if (const int k = known[dev].load(std::memory_order_relaxed)) return k;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, smem) != cudaSuccess ||
@@ -812,15 +811,14 @@ bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int r
 template <typename T, int D, int THREADS, int DIMS>
 cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
     const int tiles = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0;
-    return fer::host::launch_pdl(attn_finish<T, D, THREADS, DIMS>, dim3(p.group * (D / DIMS) + tiles, c.kv_heads, p.n_seq),
-                                 dim3(THREADS), 0, s, c, p);
+    return fer::host::Direct<attn_finish<T, D, THREADS, DIMS>>::launch(
+        dim3(p.group * (D / DIMS) + tiles, c.kv_heads, p.n_seq), dim3(THREADS), 0, s, 1, c, p);
 }
 
 template <typename T, int D, int NT>
 cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
-    using fer::host::launch_pdl;
     constexpr int smem = Cut<D>::kSmem;
-    static std::atomic<int> known[kDevices];
+    static std::atomic<int> known[fer::host::kMaxDevices];
     const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT>), smem, known);
     if (ctas <= 0) return cudaErrorInvalidConfiguration;
     CUtensorMap k_map, v_map;
@@ -828,12 +826,12 @@ cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     const uint32_t dtype = __is_same(T, __half) ? 1 : 2;
     if (!map_pages(&k_map, c, c.k, dtype, rows) || !map_pages(&v_map, c, c.v, dtype, rows)) return cudaErrorInvalidValue;
     const long long most = static_cast<long long>(p.n_seq) * c.kv_heads * p.blocks * p.chunks;
-    cudaError_t e = launch_pdl(attn_units<T, D, NT>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
-                               dim3(kThreads), smem, s, c, p, k_map, v_map);
+    cudaError_t e = fer::host::Direct<attn_units<T, D, NT>>::launch(dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
+                                                                    dim3(kThreads), smem, s, 1, c, p, k_map, v_map);
     if (e == cudaSuccess && (p.weights || p.chunks > 1))
         // few chunks: a head a CTA; many: sixteen warps for 32 dims, whose loads one SM could not have in flight
         e = p.chunks <= 32 ? finish<T, D, 256, D>(c, p, s) : finish<T, D, 512, 32>(c, p, s);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return e;
 }
 
 template <typename T, int D>

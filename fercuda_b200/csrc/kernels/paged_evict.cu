@@ -28,8 +28,8 @@
 //
 // The moves (evict_move): a warp resolves 32 moves at once, a lane each, then
 // copies their rows with kAhead 16-byte loads a lane in flight.
+#include "launch.cuh"
 #include "paged.cuh"
-#include "pdl.cuh"
 
 #include <cooperative_groups.h>
 
@@ -516,48 +516,26 @@ int most_moves(int max_slots, int budget) {
 
 size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
 
-constexpr int kDevices = 64;
-
-cudaError_t launch_cluster(const void* kernel, dim3 grid, int threads, size_t smem, unsigned cluster, cudaStream_t s,
-                           void** args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = fer::host::pdl_enabled() ? 2 : 1;
-    fer_pdl_note_launch();
-    return cudaLaunchKernelExC(&cfg, kernel, args);
-}
-
-template <int D>
-const void* small_kernel(int max_slots) {
-    const void* k[] = {reinterpret_cast<const void*>(evict_small<D, 8>), reinterpret_cast<const void*>(evict_small<D, 16>),
-                       reinterpret_cast<const void*>(evict_small<D, 24>), reinterpret_cast<const void*>(evict_small<D, 32>)};
-    return k[(max_slots - 1) / 256];
+template <int D, int KEYS>
+cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t s) {
+    // two heads a CTA, up to eight CTAs a sequence
+    unsigned ctas = 1;
+    while (ctas < 8 && 4 * ctas <= static_cast<unsigned>(c.kv_heads)) ctas *= 2;
+    const int warps = (c.kv_heads + ctas - 1) / ctas < 8 ? (c.kv_heads + ctas - 1) / ctas : 8;
+    return fer::host::Direct<evict_small<D, KEYS>>::launch(dim3(ctas, batch), dim3(32 * warps), 0, s, ctas, c, p);
 }
 
 template <int D>
 cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
     cudaError_t e;
     const int max_slots = c.max_slots();
-    const bool small = max_slots <= kSmall;
-    if (small) {
+    const bool few = max_slots <= kSmall;
+    if (few) {
         p.fused = p.cap <= kFusedMoves;
-        // two heads a CTA, up to eight CTAs a sequence
-        unsigned ctas = 1;
-        while (ctas < 8 && 4 * ctas <= static_cast<unsigned>(c.kv_heads)) ctas *= 2;
-        const int warps = (c.kv_heads + ctas - 1) / ctas < 8 ? (c.kv_heads + ctas - 1) / ctas : 8;
-        Paged view = c;
-        void* args[] = {&view, &p};
-        e = launch_cluster(small_kernel<D>(max_slots), dim3(ctas, batch), 32 * warps, 0, ctas, s, args);
+        e = max_slots <= 256   ? small<D, 8>(c, p, batch, s)
+            : max_slots <= 512 ? small<D, 16>(c, p, batch, s)
+            : max_slots <= 768 ? small<D, 24>(c, p, batch, s)
+                               : small<D, 32>(c, p, batch, s);
         if (e != cudaSuccess || p.fused) return e;
     } else {
         // no more CTAs a head than its keys need: a step of a cluster (barrier, remote counts) takes about 2 us,
@@ -567,25 +545,23 @@ cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
         const int each = ((max_slots - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
         const bool held = each <= kMostKeys;
         const size_t smem = held ? static_cast<size_t>(each) / 32 * 36 * 4 : 0;
-        const void* kernel = held ? reinterpret_cast<const void*>(evict_select<true>)
-                                  : reinterpret_cast<const void*>(evict_select<false>);
-        static std::atomic<bool> set[kDevices];
+        static std::atomic<bool> set[fer::host::kMaxDevices];
         int dev = 0;
         e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
-        if (dev >= kDevices || !set[dev].load(std::memory_order_relaxed)) {
+        if (dev >= fer::host::kMaxDevices || !set[dev].load(std::memory_order_relaxed)) {
             e = cudaFuncSetAttribute(evict_select<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      kMostKeys / 32 * 36 * 4);
             if (e != cudaSuccess) return e;
-            if (dev < kDevices) set[dev].store(true, std::memory_order_relaxed);
+            if (dev < fer::host::kMaxDevices) set[dev].store(true, std::memory_order_relaxed);
         }
-        Paged view = c;
-        void* args[] = {&view, &p};
-        e = launch_cluster(kernel, dim3(ctas, c.kv_heads, batch), kSelect, smem, ctas, s, args);
+        const dim3 grid(ctas, c.kv_heads, batch);
+        e = held ? fer::host::Direct<evict_select<true>>::launch(grid, dim3(kSelect), smem, s, ctas, c, p)
+                 : fer::host::Direct<evict_select<false>>::launch(grid, dim3(kSelect), 0, s, ctas, c, p);
         if (e != cudaSuccess) return e;
     }
     const dim3 grid((p.cap + kMove - 1) / kMove + (p.cap == 0), c.kv_heads, batch);
-    return fer::host::launch_pdl(evict_move<D>, grid, dim3(kMove), 0, s, c, p, !small);
+    return fer::host::Direct<evict_move<D>>::launch(grid, dim3(kMove), 0, s, 1, c, p, !few);
 }
 
 }  // namespace
@@ -634,5 +610,5 @@ extern "C" cudaError_t fer_paged_evict(const fer_paged_view_t* cache, const fer_
         case 128: e = run<128>(c, p, cache->batch, s); break;
         default: e = run<256>(c, p, cache->batch, s); break;
     }
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return e;
 }

@@ -19,7 +19,7 @@
 // the V that pair with them; V is the widest that pointers, strides and sizes
 // allow.
 #include "elem.cuh"
-#include "pdl.cuh"
+#include "launch.cuh"
 
 #include "fercuda/b200/native.h"
 
@@ -219,12 +219,12 @@ cudaError_t launch(RotaryParams& p, cudaStream_t s) {
     cudaError_t e;
     if constexpr (V > 1) {
         if (inter) {
-            e = fer::host::launch_pdl(rotary<T, V, A, true>, dim3(grid), dim3(kThreads), smem, s, p);
-            return e != cudaSuccess ? e : cudaGetLastError();
+            e = fer::host::Direct<rotary<T, V, A, true>>::launch(dim3(grid), dim3(kThreads), smem, s, 1, p);
+            return e;
         }
     }
-    e = fer::host::launch_pdl(rotary<T, V, A, false>, dim3(grid), dim3(kThreads), smem, s, p);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    e = fer::host::Direct<rotary<T, V, A, false>>::launch(dim3(grid), dim3(kThreads), smem, s, 1, p);
+    return e;
 }
 
 // The widest power-of-two V elements that every address and size allows.

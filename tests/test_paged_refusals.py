@@ -142,3 +142,32 @@ def test_session_entries_refuse_null():
     for name in ("fer_submit_rotary", "fer_submit_paged_store", "fer_submit_paged_attention",
                  "fer_submit_paged_evict"):
         assert getattr(lib, name)(None, None, None).code == capi.FER_STATUS_INVALID_ARGUMENT
+
+
+def test_packed_requests_are_the_structs():
+    """The bytes that Session packs for a call are those of the ctypes mirror with the same values."""
+    got = {}
+
+    class Fake:
+        def __getattr__(self, name):
+            def fn(ptr, request, job):
+                got[name] = request
+                return capi.fer_status_t(0, None)
+            return fn
+
+    s = capi.Session.__new__(capi.Session)
+    s.lib, s.ptr, s._job, s._job_ref = Fake(), None, C.c_uint64(7), None
+    cache = capi.paged_cache(1, 2, 3, 4)
+    assert s.rotary(1, 2, 3, 4, 64, sections=(5, 6, 7), rotary_dim=36, base=1e6, x_col=8, out_col=9, interleaved=True,
+                    inverse=True) == 7
+    want = capi.fer_rotary_request_t(1, 2, 3, 8, 9, 4, 64, 36, 3, (C.c_uint32 * 4)(5, 6, 7), 1e6, 5)
+    assert got["fer_submit_rotary"] == bytes(want)
+    s.paged_store(cache, 5, 6, k_col=7, v_col=8, offsets=9, new_lengths=10, weights=11, positions=12, seen=13, new_seen=14)
+    want = capi.fer_paged_store_request_t(capi.fer_paged_cache_t(*cache), 5, 6, 9, 10, 11, 12, 13, 14, 7, 8)
+    assert got["fer_submit_paged_store"] == bytes(want)
+    s.paged_attention(cache, 5, 6, 7, workspace=8, q_col=9, out_col=10, scale=0.5, lse=11, weights=12)
+    want = capi.fer_paged_attention_request_t(capi.fer_paged_cache_t(*cache), 5, 6, 11, 12, 8, 9, 10, 7, 0.5)
+    assert got["fer_submit_paged_attention"] == bytes(want)
+    s.paged_evict(cache, 5, 6, 7, 8, 9, workspace=10, new_lengths=11, new_weights=12, new_positions=13)
+    want = capi.fer_paged_evict_request_t(capi.fer_paged_cache_t(*cache), 7, 8, 9, 11, 12, 13, 10, 5, 6)
+    assert got["fer_submit_paged_evict"] == bytes(want)
