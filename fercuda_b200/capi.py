@@ -666,7 +666,7 @@ class Session:
         """fer_submit_rotary; one section per axis, (0,) for a single axis over the whole rotary_dim."""
         if not 1 <= len(sections) <= 4:
             raise ValueError("rotary takes 1 to 4 axes")
-        flags = ((FER_ROTARY_INTERLEAVED if interleaved else 0) | (FER_ROTARY_AXIS_FREQS if axis_freqs else 0) |
+        flags = ((FER_ROTARY_INTERLEAVED if interleaved else 0) + (FER_ROTARY_AXIS_FREQS if axis_freqs else 0) +
                  (FER_ROTARY_INVERSE if inverse else 0))
         axes = len(sections)
         return self._submit(self.lib.fer_submit_rotary, _pack_rotary(

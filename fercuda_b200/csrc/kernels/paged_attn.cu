@@ -66,6 +66,7 @@ struct AttnParams {
     size_t qs, os;
     int n_seq, heads, group, blocks, chunks;   // blocks: head blocks a key head
     int chunk_log2;
+    int direct;          // every unit there can be has a CTA of its own
     __device__ __forceinline__ int chunk() const { return 1 << chunk_log2; }
     __device__ __forceinline__ int chunks_of(int len) const { return (len + chunk() - 1) >> chunk_log2; }
     float scale2;        // scale * log2 e
@@ -324,43 +325,6 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
     }
     fer::dev::pdl_begin();
 
-    // how many units each segment of sequences has and what they cost, and the sums before them
-    Units table{s_units, s_cost, 0, 0};
-    table.seg = (p.n_seq + kSegments - 1) / kSegments;
-    table.segments = (p.n_seq + table.seg - 1) / table.seg;
-    int cost_carry = 0;
-    int carry = 0;
-    for (int s0 = 0; s0 < table.segments; s0 += kThreads) {
-        int mine = 0;
-        int cost = 0;
-        const int s = s0 + t;
-        if (s < table.segments) {
-            for (int b = s * table.seg; b < min(p.n_seq, (s + 1) * table.seg); ++b) {
-                const Seq q(c, p, b);
-                mine += q.units();
-                cost += q.cost();
-            }
-        }
-        int x = mine;
-        int y = cost;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int x1 = __shfl_up_sync(0xffffffffu, x, off);
-            const int y1 = __shfl_up_sync(0xffffffffu, y, off);
-            if (lane >= off) x += x1, y += y1;
-        }
-        if (lane == 31) s_sum[w] = x, s_cost_sum[w] = y;
-        __syncthreads();
-        x += carry - mine;
-        y += cost_carry - cost;
-        for (int i = 0; i <= kWarps; ++i) {
-            if (i < w) x += s_sum[i], y += s_cost_sum[i];
-            carry += s_sum[i];
-            cost_carry += s_cost_sum[i];
-        }
-        if (s < table.segments) s_units[s] = x, s_cost[s] = y;
-        __syncthreads();
-    }
     // sequences that hold nothing have no unit: their results are written here
     for (int b = blockIdx.x; b < p.n_seq; b += gridDim.x) {
         bool bad;
@@ -372,16 +336,65 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
         if (p.lse)
             for (int i = t; i < p.heads; i += kThreads) p.lse[static_cast<size_t>(b) * p.heads + i] = -INFINITY;
     }
-    // this CTA's run: the units that begin in its equal part of the whole cost
-    int u0, u1;
-    {
-        const int x = static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(cost_carry)) *
-                                       (blockIdx.x + (lane & 1)) / gridDim.x);
-        const int u = x >= cost_carry ? carry : unit_at(c, p, table, x);
-        u0 = __shfl_sync(0xffffffffu, u, 0);
-        u1 = __shfl_sync(0xffffffffu, u, 1);
+    Units table{s_units, s_cost, 0, 0};
+    UnitRun run;
+    int u0 = 0, u1 = 1;
+    if (p.direct) {
+        // no table: this CTA's unit by its index
+        const int heads = c.kv_heads * p.blocks, chunk = blockIdx.x % p.chunks, hb = blockIdx.x / p.chunks;
+        const int b = hb / heads, h = hb - b * heads;
+        const Seq q(c, p, b);
+        if (chunk >= q.chunks) return;
+        run.from = 0;
+        run.x = Unit{b, h / p.blocks, h % p.blocks, chunk, q.chunks, min(p.chunk(), q.len - (chunk << p.chunk_log2))};
+        __syncthreads();   // the barriers are set up
+    } else {
+        // how many units each segment of sequences has and what they cost, and the sums before them
+        table.seg = (p.n_seq + kSegments - 1) / kSegments;
+        table.segments = (p.n_seq + table.seg - 1) / table.seg;
+        int cost_carry = 0;
+        int carry = 0;
+        for (int s0 = 0; s0 < table.segments; s0 += kThreads) {
+            int mine = 0;
+            int cost = 0;
+            const int s = s0 + t;
+            if (s < table.segments) {
+                for (int b = s * table.seg; b < min(p.n_seq, (s + 1) * table.seg); ++b) {
+                    const Seq q(c, p, b);
+                    mine += q.units();
+                    cost += q.cost();
+                }
+            }
+            int x = mine;
+            int y = cost;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int x1 = __shfl_up_sync(0xffffffffu, x, off);
+                const int y1 = __shfl_up_sync(0xffffffffu, y, off);
+                if (lane >= off) x += x1, y += y1;
+            }
+            if (lane == 31) s_sum[w] = x, s_cost_sum[w] = y;
+            __syncthreads();
+            x += carry - mine;
+            y += cost_carry - cost;
+            for (int i = 0; i <= kWarps; ++i) {
+                if (i < w) x += s_sum[i], y += s_cost_sum[i];
+                carry += s_sum[i];
+                cost_carry += s_cost_sum[i];
+            }
+            if (s < table.segments) s_units[s] = x, s_cost[s] = y;
+            __syncthreads();
+        }
+        // this CTA's run: the units that begin in its equal part of the whole cost
+        {
+            const int x = static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(cost_carry)) *
+                                           (blockIdx.x + (lane & 1)) / gridDim.x);
+            const int u = x >= cost_carry ? carry : unit_at(c, p, table, x);
+            u0 = __shfl_sync(0xffffffffu, u, 0);
+            u1 = __shfl_sync(0xffffffffu, u, 1);
+        }
+        if (u0 >= u1) return;
     }
-    if (u0 >= u1) return;
 
     const uint32_t ring = fer::dev::smem_addr(smem);
     bool alive = true;   // no wait of this warp has run out
@@ -391,7 +404,6 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
         const int box_rows = min(kRound, c.page_size()), row_boxes = kRound / box_rows;
         const int boxes = 2 * (D / 64) * row_boxes;
         const uint32_t full0 = fer::dev::smem_addr(&s_full[0]);
-        UnitRun run;
         Unit x = run.get(c, p, table, u0, u1 - 1), next = x;
         ChunkPages pages = load_pages(c, x, x.chunk << p.chunk_log2), ahead = pages;
         int q = 0;
@@ -458,7 +470,6 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
                 }
         }
     };
-    UnitRun run;
     Unit x = run.get(c, p, table, u0, u1 - 1);
     load_q(x, qf);
     int q = 0;   // rounds of the run so far
@@ -816,7 +827,7 @@ cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
 }
 
 template <typename T, int D, int NT>
-cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
+cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
     constexpr int smem = Cut<D>::kSmem;
     static std::atomic<int> known[fer::host::kMaxDevices];
     const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT>), smem, known);
@@ -826,6 +837,7 @@ cudaError_t run(const Paged& c, const AttnParams& p, cudaStream_t s) {
     const uint32_t dtype = __is_same(T, __half) ? 1 : 2;
     if (!map_pages(&k_map, c, c.k, dtype, rows) || !map_pages(&v_map, c, c.v, dtype, rows)) return cudaErrorInvalidValue;
     const long long most = static_cast<long long>(p.n_seq) * c.kv_heads * p.blocks * p.chunks;
+    p.direct = most <= ctas;
     cudaError_t e = fer::host::Direct<attn_units<T, D, NT>>::launch(dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
                                                                     dim3(kThreads), smem, s, 1, c, p, k_map, v_map);
     if (e == cudaSuccess && (p.weights || p.chunks > 1))

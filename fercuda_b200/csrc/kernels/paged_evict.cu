@@ -16,9 +16,9 @@
 // lane-strided, finds the cut bit by bit: at most 32 counts, no shared memory
 // and no barrier, and it stops as soon as a cut leaves exactly the budget.
 // What a lane frees, keeps and moves are then 32-bit masks, and only the key
-// registers that hold such a slot in some lane cost a ballot. A sequence's
-// heads share a cluster, so that its length can be replaced once all have
-// read it. When a head can have at most 32 moves (a cache that is cut back every few
+// registers that hold such a slot in some lane cost a ballot. Where lengths are
+// replaced in place a sequence's heads share a cluster, and its length is replaced once
+// all have read it. When a head can have at most 32 moves (a cache that is cut back every few
 // tokens) the warp also makes them, and one launch does it all.
 //
 // Above (evict_select): a CTA a head, from 32K slots on a cluster of 2 to 8,
@@ -92,17 +92,16 @@ __device__ __forceinline__ Head head_of(const Paged& c, const EvictParams& p, si
 // Up to 32 moves of one head, move i0 + lane in each lane: their slots are
 // resolved to rows, a lane each, then all lanes copy row after row.
 template <int D>
-__device__ __forceinline__ void move_rows(const Paged& c, const EvictParams& p, const Head& h, int b, int hk,
-                                          bool mine, int from, int to) {
+__device__ __forceinline__ void move_rows(const Paged& c, const EvictParams& p, const Head& h, int hk, bool mine,
+                                          int from, int to, int pf, int pt) {   // pf, pt: their pages, as the table has them
     constexpr int kPieces = D / 8, kRows = 32 / kPieces, kAhead = 8;   // lanes a row, rows at once
     const int lane = threadIdx.x & 31, piece = lane % kPieces;
     unsigned long long src = 0, dst = 0;
     bool good = false;
     if (mine) {
-        const int pf = c.page(b, from), pt = c.page(b, to);
         h.nw[to] = h.w[from];
         h.np[to] = h.pos[from];
-        good = pf >= 0 && pt >= 0;
+        good = c.is_page(pf) && c.is_page(pt);
         if (good) src = c.row(pf, hk, from), dst = c.row(pt, hk, to);
         else fer::dev::report(p.err, fer::dev::kErrBadShape);
     }
@@ -139,8 +138,8 @@ __device__ __forceinline__ void copy_whole(const Head& h, int n, int t, int step
 // The low `n` bits, n clamped to 0 .. 32.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? kAll : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// grid (CTAs a sequence, batch), a cluster a sequence and a warp a head, for
-// max_slots <= 32 * KEYS. Slot 32 i + lane is key i of that lane.
+// grid (CTAs a sequence, batch), a warp a head, for max_slots <= 32 * KEYS;
+// where the length is replaced in place a sequence's CTAs are a cluster. Slot 32 i + lane is key i of that lane.
 template <int D, int KEYS>
 __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictParams p) {
     __shared__ int s_to[8][kFusedMoves], s_from[8][kFusedMoves];
@@ -152,6 +151,25 @@ __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictPar
     const int n = c.length(b, &bad);
     if (bad && threadIdx.x == 0 && blockIdx.x == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
     const long long first = static_cast<long long>(p.seen[b]) - p.recent;
+    // the sequence's page ids, lane-strided, for the moves of this kernel
+    constexpr int kPages = (32 * KEYS / 8 + 31) / 32;
+    int pages[kPages];
+    if (p.fused) {
+#pragma unroll
+        for (int i = 0; i < kPages; ++i) {
+            pages[i] = -1;
+            if (32 * i + lane < c.max_pages) pages[i] = c.table[static_cast<size_t>(b) * c.max_pages + 32 * i + lane];
+        }
+    }
+    auto page_of = [&](int i) {
+        int id = -1;
+#pragma unroll
+        for (int k = 0; k < kPages; ++k) {
+            const int v = __shfl_sync(kAll, pages[k], i & 31);
+            if (i >> 5 == k) id = v;
+        }
+        return id;
+    };
     for (int hk = blockIdx.x * warps + w; hk < c.kv_heads; hk += step) {
         const size_t bh = static_cast<size_t>(b) * c.kv_heads + hk;
         const Head h = head_of(c, p, bh);
@@ -254,13 +272,14 @@ __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictPar
         const int moved = min(count[0], min(count[1], p.cap));   // all alike
         if (p.fused) {
             __syncwarp();
-            move_rows<D>(c, p, h, b, hk, lane < moved, lane < moved ? from[lane] : 0, lane < moved ? to[lane] : 0);
+            const int f = lane < moved ? from[lane] : 0, g = lane < moved ? to[lane] : 0;
+            move_rows<D>(c, p, h, hk, lane < moved, f, g, page_of(f >> c.shift), page_of(g >> c.shift));
             __syncwarp();
         } else if (lane == 0) {
             p.counts[bh] = moved;
         }
     }
-    cluster.sync();   // every head has read the length
+    cluster.sync();   // every head of the cluster has read the length
     if (blockIdx.x == 0 && threadIdx.x == 0) p.new_lengths[b] = min(n, p.budget);
 }
 
@@ -506,7 +525,9 @@ __global__ void __launch_bounds__(kMove) evict_move(const Paged c, const EvictPa
     const int i = (blockIdx.x * (kMove / 32) + (threadIdx.x >> 5)) * 32 + lane;
     if (i - lane >= moved) return;
     const Head h = head_of(c, p, bh);
-    move_rows<D>(c, p, h, b, hk, i < moved, i < moved ? h.from[i] : 0, i < moved ? h.to[i] : 0);
+    const int from = i < moved ? h.from[i] : 0, to = i < moved ? h.to[i] : 0;
+    const int32_t* const row = c.table + static_cast<size_t>(b) * c.max_pages;
+    move_rows<D>(c, p, h, hk, i < moved, from, to, row[from >> c.shift], row[to >> c.shift]);
 }
 
 int most_moves(int max_slots, int budget) {
@@ -522,7 +543,8 @@ cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t 
     unsigned ctas = 1;
     while (ctas < 8 && 4 * ctas <= static_cast<unsigned>(c.kv_heads)) ctas *= 2;
     const int warps = (c.kv_heads + ctas - 1) / ctas < 8 ? (c.kv_heads + ctas - 1) / ctas : 8;
-    return fer::host::Direct<evict_small<D, KEYS>>::launch(dim3(ctas, batch), dim3(32 * warps), 0, s, ctas, c, p);
+    const unsigned cluster = p.new_lengths == c.lengths ? ctas : 1;
+    return fer::host::Direct<evict_small<D, KEYS>>::launch(dim3(ctas, batch), dim3(32 * warps), 0, s, cluster, c, p);
 }
 
 template <int D>
