@@ -58,7 +58,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // Slots a chunk: a function of the table's width alone, so that a sequence's
 // results do not depend on the batch.
-__host__ __device__ inline int chunk_of(int max_slots) { return max_slots > 32768 ? 512 : 256; }
+__host__ __device__ inline int chunk_of(int max_slots) { return max_slots > 65536 ? 512 : 256; }
 
 struct AttnParams {
     const void* q;

@@ -560,10 +560,11 @@ cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
                                : small<D, 32>(c, p, batch, s);
         if (e != cudaSuccess || p.fused) return e;
     } else {
-        // no more CTAs a head than its keys need: a step of a cluster (barrier, remote counts) takes about 2 us,
-        // which is what one SM takes to read 10,000 more slots
+        // As many CTAs a head as its keys need; up to eight where SMs would be left over, a CTA at least 4096 slots
+        // (32 heads of 32768 slots: 20 us with one CTA a head, 18 with four).
         unsigned ctas = 1;
         while (ctas < 8 && static_cast<long long>(ctas) * kMostKeys < max_slots) ctas *= 2;
+        while (ctas < 8 && 2ll * ctas * c.kv_heads * batch <= 148 && ctas * 4096ll < max_slots) ctas *= 2;
         const int each = ((max_slots - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
         const bool held = each <= kMostKeys;
         const size_t smem = held ? static_cast<size_t>(each) / 32 * 36 * 4 : 0;
