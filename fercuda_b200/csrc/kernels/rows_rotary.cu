@@ -209,7 +209,7 @@ cudaError_t launch(RotaryParams& p, cudaStream_t s) {
     p.hp = 32 / p.across;
     // a warp a row; where that leaves SMs without work, as many a row as have kAhead loads to make
     const int turns = (p.heads + p.hp - 1) / p.hp;
-    int split = (148 * 2 * kWarps + p.rows - 1) / p.rows;
+    int split = p.rows < 148 * 2 * kWarps ? (148 * 2 * kWarps - 1) / p.rows + 1 : 1;
     if (split > (turns + kAhead - 1) / kAhead) split = (turns + kAhead - 1) / kAhead;
     p.share = ((turns + split - 1) / split) * p.hp;
     p.split = (p.heads + p.share - 1) / p.share;

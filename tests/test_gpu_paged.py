@@ -7,6 +7,9 @@ that bound in f32. Pages are NaN outside the held slots, and table entries
 behind them are no page ids, so anything that is read there shows."""
 import ctypes as C
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -668,6 +671,50 @@ def test_captured_steps(session):
         for got, exp in zip((c.k, c.v, c.lengths, t["w"], t["p"], t["seen"], t["out"], t["lse"]), want):
             assert ref.same_bits(got, exp)
     assert int(err) == 0
+
+
+FIRST_USE = """
+import ctypes as C, sys
+sys.path.insert(0, {root!r})
+import torch
+from fercuda_b200 import capi
+from tests import paged_ref as ref
+lib = capi.kernels()
+c = ref.Cache([90, 300], 2, {dim}, 16, torch.bfloat16, max_pages=30)
+W = 2 * {dim}
+q = torch.randn(2, W, device="cuda").to(torch.bfloat16)
+out = torch.zeros_like(q)
+w, p = torch.zeros(2, 2, c.slots, device="cuda"), torch.zeros(2, 2, c.slots, dtype=torch.int32, device="cuda")
+seen = c.lengths.clone()
+size = max(lib.fer_paged_attention_workspace_bytes(2, 2, 2, {dim}, c.slots, 1), lib.fer_paged_evict_workspace_bytes(2, 2, c.slots, 60))
+ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+v = capi.fer_paged_view_t(c.k.data_ptr(), c.v.data_ptr(), c.table.data_ptr(), c.lengths.data_ptr(), 2, c.max_pages,
+                          c.k.shape[0], 2, 16, {dim}, capi.FER_DTYPE_BF16)
+a = capi.fer_rotary_args_t(q.data_ptr(), q.data_ptr(), seen.data_ptr(), W, W, 2, 2, {dim}, {dim}, 1, (C.c_int * 4)({dim} // 2),
+                           1e4, 0, capi.FER_DTYPE_BF16)
+x = capi.fer_paged_attention_args_t(q.data_ptr(), out.data_ptr(), W, W, 2, 2, 0.0, None, w.data_ptr(), ws.data_ptr(), size)
+e = capi.fer_paged_evict_args_t(60, 9, w.data_ptr(), p.data_ptr(), seen.data_ptr(), c.lengths.data_ptr(), w.data_ptr(),
+                                p.data_ptr(), ws.data_ptr(), size)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    rc = [lib.fer_rotary(C.byref(a), s), lib.fer_paged_attention(C.byref(v), C.byref(x), None, s),
+          lib.fer_paged_evict(C.byref(v), C.byref(e), None, s)]
+assert rc == [0, 0, 0], rc
+g.replay()
+torch.cuda.synchronize()
+print("ok", c.lengths.tolist(), float(out.float().abs().sum()) > 0)
+"""
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_first_use_under_capture(dim):
+    """A process whose first calls of the launchers are captured."""
+    root = str(Path(__file__).resolve().parents[1])
+    r = subprocess.run([sys.executable, "-c", FIRST_USE.format(root=root, dim=dim)], capture_output=True, text=True,
+                       timeout=240, cwd=root)
+    assert r.returncode == 0 and "ok [60, 60] True" in r.stdout, r.stdout + r.stderr
 
 
 def test_session_calls_are_refused_under_capture(session):
