@@ -10,6 +10,10 @@
 
 namespace fer::dev {
 
+// Fetches a line into L2. Only a hint: it may come before a programmatic
+// launch wait, as the value is read behind it.
+__device__ __forceinline__ void prefetch_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
+
 struct Paged {
     void* k;
     void* v;

@@ -83,7 +83,6 @@ __device__ __forceinline__ float ex2(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ void prefetch_l2(const void* at) { asm volatile("prefetch.global.L2 [%0];" ::"l"(at)); }
 // Tensor copy of a box of rows of one page: 64 dims from x, rows from r.
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int r, int head, int page,
                                          uint32_t bar) {
@@ -327,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
     // lengths and page ids into L2 while the kernel before still runs: only a hint, their values are read behind it
     {
         const size_t line = static_cast<size_t>(blockIdx.x) * kThreads + t, ids = static_cast<size_t>(p.n_seq) * c.max_pages;
-        if (line * 32 < ids) prefetch_l2(c.table + line * 32);
-        if (line * 32 < static_cast<size_t>(p.n_seq)) prefetch_l2(c.lengths + line * 32);
+        if (line * 32 < ids) fer::dev::prefetch_l2(c.table + line * 32);
+        if (line * 32 < static_cast<size_t>(p.n_seq)) fer::dev::prefetch_l2(c.lengths + line * 32);
     }
     fer::dev::pdl_begin();
 

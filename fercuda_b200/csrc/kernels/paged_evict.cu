@@ -146,6 +146,14 @@ __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictPar
     const cg::cluster_group cluster = cg::this_cluster();
     const int b = blockIdx.y, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int warps = blockDim.x >> 5, step = warps * gridDim.x;
+    if (blockIdx.x * warps + w < c.kv_heads) {   // the first head's arrays, and the page ids
+        const Head h = head_of(c, p, static_cast<size_t>(b) * c.kv_heads + blockIdx.x * warps + w);
+        if (32 * lane < c.max_slots()) {
+            fer::dev::prefetch_l2(h.w + 32 * lane);
+            fer::dev::prefetch_l2(h.pos + 32 * lane);
+        }
+        if (32 * lane < c.max_pages) fer::dev::prefetch_l2(c.table + static_cast<size_t>(b) * c.max_pages + 32 * lane);
+    }
     fer::dev::pdl_begin();
     bool bad;
     const int n = c.length(b, &bad);
@@ -317,6 +325,14 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     const int rank = blockIdx.x, ctas = gridDim.x;
     const int t = threadIdx.x, lane = t & 31, b = blockIdx.z;
     const size_t bh = static_cast<size_t>(b) * c.kv_heads + blockIdx.y;
+    {   // this CTA's part of a full row of the arrays
+        const Head h = head_of(c, p, bh);
+        const int part = (c.max_slots() - 1) / ctas + 1;
+        for (int j = 32 * t; j < part && rank * part + j < c.max_slots(); j += 32 * kSelect) {
+            fer::dev::prefetch_l2(h.w + rank * part + j);
+            fer::dev::prefetch_l2(h.pos + rank * part + j);
+        }
+    }
     fer::dev::pdl_begin();
     bool bad;
     const int n = c.length(b, &bad);
@@ -464,47 +480,67 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     // Freed slots before the budget and kept ones behind it: each thread has
     // its word of kept slots, and one scan of both counts gives its places in
     // the lists.
-    int holes = 0, movers = 0;    // of this CTA so far
-    auto rounds = [&](int hole0, int mover0, bool list) {
-        for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) {
-            const int mine = r0 + 32 * t;
-            uint32_t word = 0u;
-            if (mine < hi) {
-                each_key(mine, [&](int i, uint32_t key) { word |= (key >= cut ? 1u : 0u) << i; });
-                if (last < mine + 31) {   // equal ones behind the last are not kept
-                    uint32_t equals = 0u;
-                    each_key(mine, [&](int i, uint32_t key) { equals |= (key == cut ? 1u : 0u) << i; });
-                    word &= ~equals | low_bits(last + 1 - mine);
-                }
+    auto words = [&](int mine, uint32_t* hole, uint32_t* move) {
+        uint32_t word = 0u;
+        if (mine < hi) {
+            each_key(mine, [&](int i, uint32_t key) { word |= (key >= cut ? 1u : 0u) << i; });
+            if (last < mine + 31) {   // equal ones behind the last are not kept
+                uint32_t equals = 0u;
+                each_key(mine, [&](int i, uint32_t key) { equals |= (key == cut ? 1u : 0u) << i; });
+                word &= ~equals | low_bits(last + 1 - mine);
             }
-            word &= low_bits(hi - mine);
-            const uint32_t before = low_bits(p.budget - mine);
-            uint32_t hole = ~word & before & low_bits(hi - mine), move = word & ~before;
-            int total;
-            const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
-            if (list) {
-                int h0 = hole0 + holes + (at & 0xffff), m0 = mover0 + movers + (at >> 16);
-                for (; hole; hole &= hole - 1u, ++h0)
-                    if (h0 < p.cap) h.to[h0] = mine + __ffs(hole) - 1;
-                for (; move; move &= move - 1u, ++m0)
-                    if (m0 < p.cap) h.from[m0] = mine + __ffs(move) - 1;
-            }
-            holes += total & 0xffff;
-            movers += total >> 16;
         }
+        word &= low_bits(hi - mine);
+        const uint32_t before = low_bits(p.budget - mine);
+        *hole = ~word & before & low_bits(hi - mine);
+        *move = word & ~before;
     };
+    auto list = [&](int mine, uint32_t hole, uint32_t move, int h0, int m0) {
+        for (; hole; hole &= hole - 1u, ++h0)
+            if (h0 < p.cap) h.to[h0] = mine + __ffs(hole) - 1;
+        for (; move; move &= move - 1u, ++m0)
+            if (m0 < p.cap) h.from[m0] = mine + __ffs(move) - 1;
+    };
+    int holes = 0, movers = 0;    // of this CTA, or of its rounds so far
     int hole0 = 0, mover0 = 0;    // of the CTAs before
-    if (ctas > 1) {
-        rounds(0, 0, false);
+    auto earlier = [&]() {
         if (t == 0) s_holes = holes, s_movers = movers;
         cluster.sync();
         for (int r = 0; r < rank; ++r) {
             hole0 += *cluster.map_shared_rank(&s_holes, r);
             mover0 += *cluster.map_shared_rank(&s_movers, r);
         }
-        holes = movers = 0;
+    };
+    if constexpr (HELD) {   // one round
+        static_assert(kMostKeys <= 32 * kSelect);
+        const int mine = lo + 32 * t;
+        uint32_t hole, move;
+        int total;
+        words(mine, &hole, &move);
+        const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
+        holes = total & 0xffff;
+        movers = total >> 16;
+        if (ctas > 1) earlier();
+        list(mine, hole, move, hole0 + (at & 0xffff), mover0 + (at >> 16));
+    } else {
+#pragma unroll 1
+        for (int pass = ctas > 1 ? 0 : 1; pass < 2; ++pass) {
+            for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) {
+                const int mine = r0 + 32 * t;
+                uint32_t hole, move;
+                int total;
+                words(mine, &hole, &move);
+                const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
+                if (pass == 1) list(mine, hole, move, hole0 + holes + (at & 0xffff), mover0 + movers + (at >> 16));
+                holes += total & 0xffff;
+                movers += total >> 16;
+            }
+            if (pass == 0) {
+                earlier();
+                holes = movers = 0;
+            }
+        }
     }
-    rounds(hole0, mover0, true);
     // all alike, unless the arrays changed meanwhile
     if (rank == ctas - 1 && t == 0)
         p.counts[bh] = min(mover0 + movers, min(hole0 + holes, p.cap));
