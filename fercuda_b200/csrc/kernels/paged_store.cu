@@ -5,10 +5,11 @@
 // for prompts and by launch latency for a decode step.
 //
 // A CTA takes a run of rows. One thread a row finds its sequence (binary
-// search in the offsets), slot and page; then the threads walk (row, head,
-// 16-byte piece) of keys and of values, so reads are contiguous along a row
-// and writes along a head's row in its page. Weights and positions are walked
-// with the row innermost: consecutive slots of a head are consecutive.
+// search in the offsets), slot and page; then a warp takes a row (several warps where
+// rows are few) and walks its 16-byte pieces, kAhead of keys and of values in
+// flight a lane: reads are contiguous along a row and writes along a head's
+// row in its page. Weights and positions are walked with the row innermost:
+// consecutive slots of a head are consecutive.
 //
 // Lengths: a CTA of a step (one row a sequence) is the only reader of its
 // sequences' lengths and writes the new ones itself, in place or not. With
@@ -24,7 +25,9 @@ namespace {
 
 using fer::dev::Paged;
 constexpr int kThreads = 256;
-constexpr int kMaxRows = 32;   // rows a CTA at most
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxRows = 16;   // rows a CTA at most
+constexpr int kAhead = 4;
 
 struct StoreParams {
     const uint16_t* k_rows;
@@ -103,17 +106,32 @@ __global__ void __launch_bounds__(kThreads) store_rows(const Paged c, const Stor
     }
     if (bad) fer::dev::report(p.err, bad);
     __syncthreads();
-    const int pieces = c.head_dim / kPer, per_row = c.kv_heads * pieces;
-    for (int i = t; i < nr * per_row; i += kThreads) {
-        const int j = i / per_row, q = i - j * per_row;
-        const int h = q / pieces, e = q - h * pieces;
+    // head_dim is a power of two: piece q of a row is piece q % pieces of head q / pieces
+    const int pieces = c.head_dim / kPer, log = 31 - __clz(pieces), per_row = c.kv_heads << log;
+    const int lane = t & 31, w = t >> 5, share = max(1, kWarps / p.run);   // warps a row
+    for (int j = w / share; j < nr; j += max(1, kWarps / share)) {
         if (s_page[j] < 0) continue;
-        const size_t from = static_cast<size_t>(q) * kPer;
-        const Piece kk = *reinterpret_cast<const Piece*>(p.k_rows + (r0 + static_cast<size_t>(j)) * p.ks + from);
-        const Piece vv = *reinterpret_cast<const Piece*>(p.v_rows + (r0 + static_cast<size_t>(j)) * p.vs + from);
-        const size_t to = c.row(s_page[j], h, s_slot[j]) + static_cast<size_t>(e) * kPer;
-        *reinterpret_cast<Piece*>(static_cast<uint16_t*>(c.k) + to) = kk;
-        *reinterpret_cast<Piece*>(static_cast<uint16_t*>(c.v) + to) = vv;
+        const Piece* const kr = reinterpret_cast<const Piece*>(p.k_rows + (r0 + static_cast<size_t>(j)) * p.ks);
+        const Piece* const vr = reinterpret_cast<const Piece*>(p.v_rows + (r0 + static_cast<size_t>(j)) * p.vs);
+        const size_t to = c.row(s_page[j], 0, s_slot[j]) / kPer, head = static_cast<size_t>(pieces) << c.shift;
+        Piece* const kp = static_cast<Piece*>(c.k) + to;
+        Piece* const vp = static_cast<Piece*>(c.v) + to;
+        for (int q0 = (w % share) * 32 + lane; q0 < per_row; q0 += 32 * share * kAhead) {
+            Piece kk[kAhead], vv[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int q = q0 + 32 * share * k;
+                if (q < per_row) kk[k] = kr[q], vv[k] = vr[q];
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int q = q0 + 32 * share * k;
+                if (q >= per_row) break;
+                const size_t at = (q >> log) * head + (q & (pieces - 1));
+                kp[at] = kk[k];
+                vp[at] = vv[k];
+            }
+        }
     }
     if (p.weights || p.positions) {
         const size_t most = static_cast<size_t>(c.max_slots());
@@ -174,9 +192,9 @@ extern "C" cudaError_t fer_paged_store(const fer_paged_view_t* cache, const fer_
     p.seen = a->seen;
     p.new_seen = a->positions || a->seen ? a->new_seen : nullptr;
     p.err = err;
-    // about 32 KB of keys and values a CTA
-    int run = static_cast<int>(16384 / (width * 2));
-    p.run = run < 1 ? 1 : run > kMaxRows ? kMaxRows : run;
+    // kMaxRows rows a CTA, fewer (and more warps a row) where that would leave SMs without work
+    p.run = kMaxRows;
+    while (p.run > 1 && a->rows < 148 * 2 * p.run) p.run /= 2;
     const bool in_place = a->new_lengths == cache->lengths || (p.new_seen && p.new_seen == a->seen);
     const bool later = a->offsets && in_place;
     cudaError_t e = cudaSuccess;
