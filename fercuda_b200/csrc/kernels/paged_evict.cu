@@ -26,7 +26,7 @@
 // other CTAs' counts are read through distributed shared memory. Beyond 8 x
 // 32K slots the keys are made again for every pass.
 //
-// The moves (evict_move): a warp resolves 32 moves at once, a lane each, then
+// The moves (evict_move): a warp resolves 16 moves at once, a lane each, then
 // copies their rows with kAhead 16-byte loads a lane in flight.
 #include "launch.cuh"
 #include "paged.cuh"
@@ -48,6 +48,7 @@ constexpr int kMostKeys = 32 * 1024;         // keys a CTA holds in shared memor
 constexpr int kCopies = 3;                   // of the first digit's counts, by lane: less contention
 constexpr int kBins = 2048;
 constexpr int kMove = 256;
+constexpr int kWarpMoves = 16;
 constexpr int kFusedMoves = 32;
 constexpr int kFewDropped = 4;               // slots too many that are found one by one
 
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     if (ctas > 1) cluster.sync();   // no CTA leaves while another may read its shared memory
 }
 
-// grid (move tiles, kv_heads, batch), a warp 32 moves
+// grid (move tiles, kv_heads, batch), a warp kWarpMoves moves
 template <int D>
 __global__ void __launch_bounds__(kMove) evict_move(const Paged c, const EvictParams p, const bool lengths) {
     fer::dev::pdl_begin();
@@ -558,12 +559,13 @@ __global__ void __launch_bounds__(kMove) evict_move(const Paged c, const EvictPa
         p.new_lengths[b] = min(c.length(b, &bad), p.budget);
     }
     const int moved = p.counts[bh];
-    const int i = (blockIdx.x * (kMove / 32) + (threadIdx.x >> 5)) * 32 + lane;
-    if (i - lane >= moved) return;
+    const int i0 = (blockIdx.x * (kMove / 32) + (threadIdx.x >> 5)) * kWarpMoves, i = i0 + lane;
+    if (i0 >= moved) return;
+    const bool mine = lane < kWarpMoves && i < moved;
     const Head h = head_of(c, p, bh);
-    const int from = i < moved ? h.from[i] : 0, to = i < moved ? h.to[i] : 0;
+    const int from = mine ? h.from[i] : 0, to = mine ? h.to[i] : 0;
     const int32_t* const row = c.table + static_cast<size_t>(b) * c.max_pages;
-    move_rows<D>(c, p, h, hk, i < moved, from, to, row[from >> c.shift], row[to >> c.shift]);
+    move_rows<D>(c, p, h, hk, mine, from, to, row[from >> c.shift], row[to >> c.shift]);
 }
 
 int most_moves(int max_slots, int budget) {
@@ -619,7 +621,8 @@ cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
                  : fer::host::Direct<evict_select<false>>::launch(grid, dim3(kSelect), 0, s, ctas, c, p);
         if (e != cudaSuccess) return e;
     }
-    const dim3 grid((p.cap + kMove - 1) / kMove + (p.cap == 0), c.kv_heads, batch);
+    constexpr int kTile = kMove / 32 * kWarpMoves;
+    const dim3 grid((p.cap + kTile - 1) / kTile + (p.cap == 0), c.kv_heads, batch);
     return fer::host::Direct<evict_move<D>>::launch(grid, dim3(kMove), 0, s, 1, c, p, !few);
 }
 
