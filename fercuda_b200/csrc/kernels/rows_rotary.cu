@@ -18,8 +18,13 @@
 // back. A unit of the half-split layout is V elements of the first half and
 // the V that pair with them; V is the widest that pointers, strides and sizes
 // allow.
+//
+// Measured: 32768 rows of 32 heads x 64 bf16 45.6 us, 5.9 TB/s (90% of the HBM
+// copy rate); 10007 rows of 40 heads x 128 f16 with three axes 39.0 us, 5.3
+// TB/s; one row 4.8 us, the host's time for the call. A CTA a tile of rows
+// with one table and barriers took 64.7 and 56.5 us.
 #include "elem.cuh"
-#include "launch.cuh"
+#include "pdl.cuh"
 
 #include "fercuda/b200/native.h"
 
@@ -219,11 +224,11 @@ cudaError_t launch(RotaryParams& p, cudaStream_t s) {
     cudaError_t e;
     if constexpr (V > 1) {
         if (inter) {
-            e = fer::host::Direct<rotary<T, V, A, true>>::launch(dim3(grid), dim3(kThreads), smem, s, 1, p);
+            e = fer::host::launch_pdl(rotary<T, V, A, true>, dim3(grid), dim3(kThreads), smem, s, p);
             return e;
         }
     }
-    e = fer::host::Direct<rotary<T, V, A, false>>::launch(dim3(grid), dim3(kThreads), smem, s, 1, p);
+    e = fer::host::launch_pdl(rotary<T, V, A, false>, dim3(grid), dim3(kThreads), smem, s, p);
     return e;
 }
 
