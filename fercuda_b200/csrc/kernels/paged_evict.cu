@@ -484,8 +484,10 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         }
     }
     // Freed slots before the budget and kept ones behind it: each thread has
-    // its word of kept slots, and one scan of both counts gives its places in
-    // the lists.
+    // its word of kept slots, and one scan of both counts, 16 bits each without
+    // a sign (a round can have 32768), gives its places in the lists.
+    auto low_half = [](int v) { return v & 0xffff; };
+    auto high_half = [](int v) { return static_cast<int>(static_cast<uint32_t>(v) >> 16); };
     auto words = [&](int mine, uint32_t* hole, uint32_t* move) {
         uint32_t word = 0u;
         if (mine < hi) {
@@ -524,10 +526,10 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         int total;
         words(mine, &hole, &move);
         const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
-        holes = total & 0xffff;
-        movers = total >> 16;
+        holes = low_half(total);
+        movers = high_half(total);
         if (ctas > 1) earlier();
-        list(mine, hole, move, hole0 + (at & 0xffff), mover0 + (at >> 16));
+        list(mine, hole, move, hole0 + low_half(at), mover0 + high_half(at));
     } else {
 #pragma unroll 1
         for (int pass = ctas > 1 ? 0 : 1; pass < 2; ++pass) {
@@ -537,9 +539,9 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
                 int total;
                 words(mine, &hole, &move);
                 const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
-                if (pass == 1) list(mine, hole, move, hole0 + holes + (at & 0xffff), mover0 + movers + (at >> 16));
-                holes += total & 0xffff;
-                movers += total >> 16;
+                if (pass == 1) list(mine, hole, move, hole0 + holes + low_half(at), mover0 + movers + high_half(at));
+                holes += low_half(total);
+                movers += high_half(total);
             }
             if (pass == 0) {
                 earlier();

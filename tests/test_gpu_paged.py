@@ -502,6 +502,18 @@ def test_evict_long(session, n, budget):
     check_evict(c, budget, min(budget, 128), w0, p0, i32(c.lens), before, (c.k, c.v, w, p, c.lengths))
 
 
+@pytest.mark.parametrize("n", [262144, 300000])   # in shared memory, and not
+def test_evict_of_the_older_half(session, n):
+    """Every slot of the recent half moves: whole rounds of 32768 slots."""
+    c = ref.Cache([n], 1, 64, 64, BF16)
+    w = weights_for("spread", 1, 1, c.slots, seed=n).cuda()
+    p = torch.arange(c.slots, dtype=torch.int32, device="cuda").repeat(1, 1, 1)
+    before = (c.k.cpu().clone(), c.v.cpu().clone(), w.clone(), p.clone())
+    w0, p0 = w.clone(), p.clone()
+    run_evict(session, c, n // 2, n // 2, w, p, c.lengths.clone())
+    check_evict(c, n // 2, n // 2, w0, p0, i32(c.lens), before, (c.k, c.v, w, p, c.lengths))
+
+
 @pytest.mark.parametrize("n", [900, 5003])
 def test_evict_arrays_at_odd_addresses(session, n):
     """Weights and positions that start 4 bytes behind a 16-byte boundary."""
