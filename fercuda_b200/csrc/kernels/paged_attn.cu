@@ -857,19 +857,17 @@ cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
                                           dim3(kThreads), smem, s, c, p, k_map, v_map);
     if (e == cudaSuccess && (p.weights || p.chunks > 1))
         // few chunks: a head a CTA; many: sixteen warps for 32 dims, whose loads one SM could not have in flight
-    // (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA)
+        // (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA)
         e = p.chunks <= 32 ? finish<T, D, 256, D>(c, p, s) : finish<T, D, 512, 32>(c, p, s);
     return e;
 }
 
+// Head blocks a key head: of up to 8 heads, or of up to 16 where it has more.
+int blocks_of(int group) { return group <= 8 ? 1 : (group - 1) / 16 + 1; }
+
 template <typename T, int D>
 cudaError_t run_heads(const Paged& c, AttnParams& p, cudaStream_t s) {
-    if (p.group <= 8) {
-        p.blocks = 1;
-        return run<T, D, 1>(c, p, s);
-    }
-    p.blocks = (p.group + 15) / 16;
-    return run<T, D, 2>(c, p, s);
+    return p.group <= 8 ? run<T, D, 1>(c, p, s) : run<T, D, 2>(c, p, s);
 }
 
 template <typename T>
@@ -910,8 +908,9 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     if (c.kv_heads > 65535 || a->n_seq > 65535) return cudaErrorNotSupported;
     const int max_slots = c.max_slots();
     // units and their cost are counted in 31 bits
-    if (static_cast<long long>(a->n_seq) * a->heads * (rounds_of(max_slots) + kUnitCost * ((max_slots - 1) / chunk_of(max_slots) + 1ll)) >
-        0x7fffffffll)
+    const int group = a->heads / c.kv_heads;
+    const long long blocks = static_cast<long long>(a->n_seq) * c.kv_heads * blocks_of(group);
+    if (blocks * (rounds_of(max_slots) + kUnitCost * ((max_slots - 1ll) / chunk_of(max_slots) + 1)) > 0x7fffffffll)
         return cudaErrorNotSupported;
     const size_t need = fer_paged_attention_workspace_bytes(a->n_seq, a->heads, c.kv_heads, c.head_dim, max_slots,
                                                             a->weights != nullptr);
@@ -924,7 +923,8 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     p.os = a->out_stride;
     p.n_seq = a->n_seq;
     p.heads = a->heads;
-    p.group = a->heads / c.kv_heads;
+    p.group = group;
+    p.blocks = blocks_of(group);
     while ((1 << p.chunk_log2) < chunk_of(max_slots)) ++p.chunk_log2;
     p.chunks = (max_slots - 1) / chunk_of(max_slots) + 1;
     p.scale2 = (a->scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c.head_dim)) : a->scale) * kLog2e;

@@ -12,24 +12,25 @@
 // read once; those before the budget are copied to their new arrays as they
 // pass (what is freed among them the moves overwrite, which are as many).
 //
-// Measured: 64 sequences x 16 heads of 64 cut from 513 to 512 slots 6.4 us (one
-// chain of latencies: arrays, cut, page ids, rows); 4 sequences of up to 32768 x 8
-// heads of 128 cut to 4096 35.4 us, of which 15 us are the selection and 17 us
-// the moves (54 MB read and written; 16.5 us at the copy rate).
+// Measured: 64 sequences x 16 heads of 64 cut from 513 to 512 slots 6.4 us
+// (one chain of latencies: arrays, cut, page ids, rows); 4 sequences of up to
+// 32768 x 8 heads of 128 cut to 4096 35.4 us, of which 15 us are the selection
+// and 17 us the moves (16.5 us for all bytes at the copy rate).
 //
 // Up to 1024 slots (evict_small): a warp a head with its keys in registers,
 // lane-strided, finds the cut bit by bit: at most 32 counts, no shared memory
 // and no barrier, and it stops as soon as a cut leaves exactly the budget.
 // What a lane frees, keeps and moves are then 32-bit masks, and only the key
-// registers that hold such a slot in some lane cost a ballot. Where lengths are
-// replaced in place a sequence's heads share a cluster, and its length is replaced once
-// all have read it. When a head can have at most 32 moves (a cache that is cut back every few
-// tokens) the warp also makes them, and one launch does it all.
+// registers that hold such a slot in some lane cost a ballot. Where lengths
+// are replaced in place a sequence's heads share a cluster, and its length is
+// replaced once all have read it. When a head can have at most 32 moves (a
+// cache that is cut back every few tokens) the warp also makes them, and one
+// launch does it all.
 //
-// Above (evict_select): a CTA a head, from 32K slots on a cluster of 2 to 8,
-// with the keys in shared memory, and three digits of 11, 11 and 10 bits counted there; the
-// other CTAs' counts are read through distributed shared memory. Beyond 8 x
-// 32K slots the keys are made again for every pass.
+// Above (evict_select): a CTA a head, or a cluster of 2 to 8 of them, with the
+// keys in shared memory, and three digits of 11, 11 and 10 bits counted there;
+// the other CTAs' counts are read through distributed shared memory. Beyond 8
+// x 32K slots the keys are made again for every pass.
 //
 // The moves (evict_move): a warp resolves 16 moves at once, a lane each, then
 // copies their rows with kAhead 16-byte loads a lane in flight.
@@ -145,7 +146,8 @@ __device__ __forceinline__ void copy_whole(const Head& h, int n, int t, int step
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? kAll : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // grid (CTAs a sequence, batch), a warp a head, for max_slots <= 32 * KEYS;
-// where the length is replaced in place a sequence's CTAs are a cluster. Slot 32 i + lane is key i of that lane.
+// where the length is replaced in place a sequence's CTAs are a cluster. Slot
+// 32 i + lane is key i of that lane.
 template <int D, int KEYS>
 __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictParams p) {
     __shared__ int s_to[8][kFusedMoves], s_from[8][kFusedMoves];

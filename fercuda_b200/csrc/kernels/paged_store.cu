@@ -5,11 +5,11 @@
 // for prompts and by launch latency for a decode step.
 //
 // A CTA takes a run of rows. One thread a row finds its sequence (binary
-// search in the offsets), slot and page; then a warp takes a row (several warps where
-// rows are few) and walks its 16-byte pieces, kAhead of keys and of values in
-// flight a lane: reads are contiguous along a row and writes along a head's
-// row in its page. Weights and positions are walked with the row innermost:
-// consecutive slots of a head are consecutive.
+// search in the offsets), slot and page; then a warp takes a row (several
+// warps where rows are few) and walks its 16-byte pieces, kAhead of keys and
+// of values in flight a lane: reads are contiguous along a row and writes
+// along a head's row in its page. Weights and positions are walked with the
+// row innermost: consecutive slots of a head are consecutive.
 //
 // Lengths: a CTA of a step (one row a sequence) is the only reader of its
 // sequences' lengths and writes the new ones itself, in place or not. With

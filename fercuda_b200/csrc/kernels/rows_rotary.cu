@@ -7,10 +7,10 @@
 //
 // A warp takes a row (or, where rows are few, a part of its heads). Its lanes
 // compute the cosines and sines of the row's pairs once for all heads and
-// share them in shared memory; there is no barrier. The frequency in turns is f64, so
-// position * frequency can be reduced to [-1/2, 1/2] turns exactly before the
-// f32 sine (an f32 angle of position 10^6 is off by 0.06 rad). The first
-// kAhead loads a lane are in flight meanwhile.
+// share them in shared memory; there is no barrier. The frequency in turns is
+// f64, so position * frequency can be reduced to [-1/2, 1/2] turns exactly
+// before the f32 sine (an f32 angle of position 10^6 is off by 0.06 rad). The
+// first kAhead loads a lane are in flight meanwhile.
 //
 // Lane (unit, head) turns the same unit of every hp-th head, so it reads its
 // cosines and sines once and keeps them in registers. Neighbouring lanes have

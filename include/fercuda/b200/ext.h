@@ -283,11 +283,12 @@ typedef struct fer_paged_cache {
  * dtype; both may be one fused activation). offsets i32 [sequences + 1]: rows
  * offsets[b] .. offsets[b+1] - 1 go behind sequence b's held slots, rows behind
  * the last offset belong to nobody; 0: row b is the one new token of sequence
- * b. Sequences and rows may be fewer than batch. new_lengths receives the
- * lengths (0, or the cache's own: in place). weights (0: none) get 0 and
- * positions (0: none) seen[b] + i for the i-th new row; seen is then required
- * and new_seen (0 or seen: in place) receives seen[b] + the new rows. Rows
- * that do not fit in max_pages * page_size are dropped and set error bit 4. */
+ * b. Sequences and rows may be fewer than batch; nothing is written for those
+ * left out. new_lengths receives the others' lengths (0, or the cache's own:
+ * in place). weights (0: none) get 0 and positions (0: none) seen[b] + i for
+ * the i-th new row; seen is then required and new_seen (0 or seen: in place)
+ * receives seen[b] + the new rows. Rows that do not fit in max_pages *
+ * page_size are dropped and set error bit 4. */
 typedef struct fer_paged_store_request {
     fer_paged_cache_t cache;
     uint64_t k_rows;
@@ -342,12 +343,13 @@ fer_status_t fer_submit_paged_attention(fer_session_t* session, const fer_paged_
  * stay; the i-th kept slot behind it moves (key, value, weight, position) into
  * the i-th freed slot before it, so the order of slots is no order of
  * positions. budget >= 1, recent <= budget. new_lengths, new_weights and
- * new_positions receive the results (each 0 or the old one: in place; separate ones
- * also receive what stayed); keys and values move in place, and everything
- * behind a sequence's new length is left as it was. Pages behind
- * ceil(budget / page_size) are free for other sequences afterwards. workspace: u8 buffer (16-byte aligned) of
- * fer_paged_evict_workspace_bytes(batch, kv_heads, max_pages * page_size,
- * budget) bytes, any contents; calls on different streams need one each. */
+ * new_positions receive the results (each 0 or the old one: in place; separate
+ * ones also receive what stayed); keys and values move in place, and
+ * everything behind a sequence's new length is left as it was. Pages behind
+ * ceil(budget / page_size) are free for other sequences afterwards. workspace:
+ * u8 buffer (16-byte aligned) of fer_paged_evict_workspace_bytes(batch,
+ * kv_heads, max_pages * page_size, budget) bytes, any contents; calls on
+ * different streams need one each. */
 typedef struct fer_paged_evict_request {
     fer_paged_cache_t cache;
     uint64_t weights;

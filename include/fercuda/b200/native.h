@@ -199,10 +199,10 @@ typedef struct fer_paged_view {
  * (offsets NULL: row b), its i-th row to slot lengths[b] + i. k_rows / v_rows
  * [rows, kv_heads * head_dim], k_stride / v_stride elements apart. Rows behind
  * offsets[n_seq] belong to nobody. new_lengths (may be the view's lengths)
- * receives the lengths after the call. Optional: weights f32 and positions
- * i32, both [batch, kv_heads, max_pages * page_size], receive 0 and seen[b] + i for
- * each new slot, and new_seen (may be seen) seen[b] + the new rows. Rows that
- * do not fit set error bit 4 and are dropped. */
+ * receives the n_seq sequences' lengths after the call. Optional: weights f32
+ * and positions i32, both [batch, kv_heads, max_pages * page_size], receive 0
+ * and seen[b] + i for each new slot, and new_seen (may be seen) seen[b] + the
+ * new rows. Rows that do not fit set error bit 4 and are dropped. */
 typedef struct fer_paged_store_args {
     const void* k_rows;
     const void* v_rows;

@@ -5,6 +5,7 @@ Copies and selections are exact. Attention is held to half a step of its type
 plus the arithmetic bound that tests/paged_ref.py derives; lse and weights to
 that bound in f32. Pages are NaN outside the held slots, and table entries
 behind them are no page ids, so anything that is read there shows."""
+import copy
 import ctypes as C
 import math
 import subprocess
@@ -150,6 +151,61 @@ def test_a_sequence_does_not_depend_on_its_batch(session, page, group):
         w1 = torch.zeros(1, 2, c.slots, device="cuda")
         o1, l1 = attend(session, one, q[b:b + 1].clone(), 2 * group, weights=w1)
         assert ref.same_bits(o1, out[b:b + 1]) and ref.same_bits(l1, lse[b:b + 1]) and ref.same_bits(w1, w[b:b + 1])
+
+
+@pytest.mark.parametrize("dtype,D,H,group,page,B,most", [
+    (BF16, 64, 8, 1, 16, 300, 700),      # more units than CTAs, segments of three sequences
+    (F16, 128, 4, 4, 32, 130, 1100),
+    (BF16, 256, 2, 12, 64, 129, 600),
+    (BF16, 64, 1, 20, 8, 1000, 40),
+    (F16, 128, 2, 16, 128, 150, 600)])
+def test_attention_of_large_ragged_batches(session, dtype, D, H, group, page, B, most):
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, most + 1, (B,), generator=g)
+    lens[torch.rand(B, generator=g) < 0.2] = 0             # runs of empty sequences, the first and last among them
+    lens[:2] = lens[-3:] = 0
+    lens = lens.tolist()
+    lens[B // 2] = most
+    c = ref.Cache(lens, H, D, page, dtype, seed=B)
+    q = queries(c, H * group)
+    w = torch.zeros(B, H, c.slots, device="cuda")
+    out, lse = attend(session, c, q, H * group, weights=w)
+    host = copy.copy(c)
+    host.k, host.v, host.table = c.k.cpu(), c.v.cpu(), c.table.cpu()
+    sums = check(host, q, H * group, out, lse)
+    now = w.cpu().double()
+    for (b, h), (want, rel) in sums.items():
+        assert bool(((now[b, h, :lens[b]] - want).abs() <= want * (rel + 2.0 ** -23) + 2.0 ** -140).all())
+        assert not now[b, h, lens[b]:].any()
+    b = B // 2
+    one = ref.Cache([most], H, D, page, dtype)
+    one.k, one.v, one.table, one.lengths = c.k, c.v, c.table[b:b + 1].clone(), c.lengths[b:b + 1].clone()
+    o1, l1 = attend(session, one, q[b:b + 1].clone(), H * group)
+    assert ref.same_bits(o1, out[b:b + 1]) and ref.same_bits(l1, lse[b:b + 1])
+
+
+def test_attention_of_a_large_batch_that_holds_nothing(session):
+    c = ref.Cache([0] * 700, 2, 64, 16, BF16, max_pages=40)
+    out, lse = attend(session, c, queries(c, 4), 4)
+    assert not out.any() and bool((lse == -math.inf).all())
+
+
+def test_bad_pages_in_a_large_batch(session):
+    """As above, where a CTA has several units."""
+    lens = [300] * 200
+    c = ref.Cache(lens, 4, 64, 16, BF16)
+    q = queries(c, 4)
+    good, gl = attend(session, c, q, 4)
+    c.table[70, 17] = -1                                   # a page of the second chunk
+    c.table[199, :19] = 10 ** 6
+    out, lse = attend(session, c, q, 4, errors=ERR_BAD)
+    others = [b for b in range(200) if b not in (70, 199)]
+    assert ref.same_bits(out[others], good[others]) and ref.same_bits(lse[others], gl[others])
+    assert not out[199].any() and bool((lse[199] == -math.inf).all())
+    one = copy.copy(c)
+    one.lens, one.table = [300], c.table[70:71].clone()
+    one.table[0, 17] = c.table[0, 0]                       # any page: the oracle leaves those slots out
+    check(one, q[70:71], 4, out[70:71], lse[70:71], skip={(0, s) for s in range(272, 288)})
 
 
 def test_fewer_rows_than_the_cache_has_sequences(session):
