@@ -333,14 +333,6 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     const int rank = blockIdx.x, ctas = gridDim.x;
     const int t = threadIdx.x, lane = t & 31, b = blockIdx.z;
     const size_t bh = static_cast<size_t>(b) * c.kv_heads + blockIdx.y;
-    {   // this CTA's part of a full row of the arrays
-        const Head h = head_of(c, p, bh);
-        const int part = (c.max_slots() - 1) / ctas + 1;
-        for (int j = 32 * t; j < part && rank * part + j < c.max_slots(); j += 32 * kSelect) {
-            fer::dev::prefetch_l2(h.w + rank * part + j);
-            fer::dev::prefetch_l2(h.pos + rank * part + j);
-        }
-    }
     fer::dev::pdl_begin();
     bool bad;
     const int n = c.length(b, &bad);

@@ -408,6 +408,34 @@ def test_store(session, dtype, D, H, page, lens, offsets, tail, cols, in_place):
         assert torch.equal(c.lengths, old_len) and torch.equal(seen, old_seen)
 
 
+@pytest.mark.parametrize("n_seq,ragged", [(400, True), (5000, False)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_store_of_many_rows(session, n_seq, ragged, in_place):
+    """More rows than a CTA takes, and runs of sequences that get none."""
+    g = torch.Generator().manual_seed(n_seq)
+    new = torch.randint(0, 30, (n_seq,), generator=g) * (torch.rand(n_seq, generator=g) < 0.8) if ragged else None
+    offsets = [3] + (3 + new.cumsum(0)).tolist() if ragged else None
+    lens = torch.randint(0, 34, (n_seq,), generator=g).tolist()
+    c = ref.Cache(lens, 2, 64, 16, BF16, max_pages=4)
+    grow_table(c)
+    n = offsets[-1] + 5 if ragged else n_seq
+    rows = torch.randn(n, 256, generator=g).to(BF16).cuda()
+    w = torch.full((n_seq, 2, c.slots), 5.0, device="cuda")
+    p = torch.full((n_seq, 2, c.slots), -5, dtype=torch.int32, device="cuda")
+    seen = c.lengths + 9
+    want = expect_store(c, rows, 0, 128, offsets, n_seq, w, p, seen)
+    new_len, new_seen = (c.lengths, seen) if in_place else (c.lengths.clone(), seen.clone())
+    with ref.Buffers(session) as B:
+        r = B(rows)
+        ids, bseen = c.ids(B), B(seen)
+        session.paged_store(ids, r, r, v_col=128, offsets=B(i32(offsets)) if ragged else 0,
+                            new_lengths=0 if in_place else B(new_len), weights=B(w), positions=B(p), seen=bseen,
+                            new_seen=0 if in_place else B(new_seen))
+    assert session.device_errors() == 0
+    for got, exp in zip((c.k, c.v, new_len, w, p, new_seen), want):
+        assert ref.same_bits(got, exp)
+
+
 def test_store_of_keys_and_values_alone(session):
     """No weights, no positions, keys and values in buffers of their own."""
     c = ref.Cache([10, 31], 2, 64, 16, BF16, max_pages=3)
@@ -518,6 +546,10 @@ def weights_for(kind, B, H, slots, seed=0):
     (F16, 128, 1, 8, [65, 64, 2], 1, 1, False),
     (BF16, 64, 3, 32, [300, 257, 1000], 256, 256, True),
     (BF16, 256, 2, 64, [130], 77, 0, True),
+    (BF16, 64, 40, 8, [536, 530, 513, 512, 30, 0], 512, 40, True),   # at most 32 moves, heads in turns
+    (F16, 64, 40, 8, [700, 600, 301], 300, 0, False),
+    (F16, 128, 5, 8, [1016, 1001, 1000], 1000, 5, True),
+    (BF16, 64, 40, 16, [5000, 1, 4097], 4000, 100, False),
     (F16, 64, 1, 128, [3000, 2999, 0], 900, 33, True)])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_evict(session, kind, dtype, D, H, page, lens, budget, recent, shuffled, in_place):
