@@ -317,10 +317,10 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
 }
 
 // grid (cluster CTAs, kv_heads, batch). CTA r of a cluster has the slots [lo,
-// hi). They are passed over in rounds of 32 slots a thread; the key of slot lo
-// + j lies at word j + 4 (j / 32) of shared memory, so that threads read their
-// 32 in 16-byte pieces without bank conflicts. Without HELD the keys of a
-// round are made again from the arrays.
+// hi). They are passed over in rounds of up to 32 slots a thread, shared out
+// evenly; the key of slot lo + j lies at word j + 4 (j / 32) of shared memory,
+// so that threads read 32 in 16-byte pieces without bank conflicts. Without
+// HELD the keys of a round are made again from the arrays.
 template <bool HELD>
 __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const EvictParams p) {
     extern __shared__ __align__(16) uint32_t s_key[];
@@ -347,12 +347,15 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     const int each = ((n - 1) / ctas + 1 + 127) & ~127;
     const int lo = static_cast<int>(min(static_cast<long long>(n), static_cast<long long>(rank) * each));
     const int hi = min(n - lo, each) + lo;
-    // this thread's 32 slots of a round, `mine` on: fn(i, key); i counts to a constant
+    // slots a thread takes in a round: all of the CTA's in one round where keys are held
+    const int run = HELD ? ((each - 1) / kSelect + 4) & ~3 : 32, round = run * kSelect;
+    // this thread's slots of a round, `mine` on: fn(i, key)
     auto each_key = [&](int mine, auto fn) {
         if constexpr (HELD) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const uint4 v = *reinterpret_cast<const uint4*>(s_key + (mine - lo) / 32 * 36 + i);
+#pragma unroll 2
+            for (int i = 0; i < run; i += 4) {
+                const int j = mine - lo + i;
+                const uint4 v = *reinterpret_cast<const uint4*>(s_key + j + j / 32 * 4);
                 fn(i, v.x), fn(i + 1, v.y), fn(i + 2, v.z), fn(i + 3, v.w);
             }
         } else {
@@ -402,7 +405,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         int* hist = s_hist[d == 0 ? 0 : kCopies + d - 1];
         if (d > 0) {
             const uint32_t mask = d == 1 ? 0xffe00000u : 0xfffffc00u;   // the digits found so far
-            for (int mine = lo + 32 * t; mine < hi; mine += 32 * kSelect)
+            for (int mine = lo + run * t; mine < hi; mine += round)
                 each_key(mine, [&](int i, uint32_t key) {
                     if ((key & mask) == cut && mine + i < hi) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
                 });
@@ -450,24 +453,24 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         auto word_of = [&](int mine) {
             uint32_t word = 0u;
             if (mine < hi) each_key(mine, [&](int i, uint32_t key) { word |= (key == cut ? 1u : 0u) << i; });
-            return word & low_bits(hi - mine);
+            return word & low_bits(min(run, hi - mine));
         };
         int before = 0, total;
         if (ctas > 1) {
             int mine = 0;
-            for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) mine += __popc(word_of(r0 + 32 * t));
+            for (int r0 = lo; r0 < hi; r0 += round) mine += __popc(word_of(r0 + run * t));
             block_scan(mine, s_scan, &total);
             if (t == 0) s_eq = total;
             cluster.sync();
             for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&s_eq, r);
         }
-        for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) {
-            uint32_t word = word_of(r0 + 32 * t);
+        for (int r0 = lo; r0 < hi; r0 += round) {
+            uint32_t word = word_of(r0 + run * t);
             const int here = __popc(word);
             const int at = before + block_scan(here, s_scan, &total);
             if (at < left && left <= at + here) {   // the last one is this thread's
                 for (int k = at + 1; k < left; ++k) word &= word - 1u;
-                s_last = r0 + 32 * t + __ffs(word) - 1;
+                s_last = r0 + run * t + __ffs(word) - 1;
             }
             before += total;
         }
@@ -486,15 +489,15 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         uint32_t word = 0u;
         if (mine < hi) {
             each_key(mine, [&](int i, uint32_t key) { word |= (key >= cut ? 1u : 0u) << i; });
-            if (last < mine + 31) {   // equal ones behind the last are not kept
+            if (last < mine + run - 1) {   // equal ones behind the last are not kept
                 uint32_t equals = 0u;
                 each_key(mine, [&](int i, uint32_t key) { equals |= (key == cut ? 1u : 0u) << i; });
                 word &= ~equals | low_bits(last + 1 - mine);
             }
         }
-        word &= low_bits(hi - mine);
-        const uint32_t before = low_bits(p.budget - mine);
-        *hole = ~word & before & low_bits(hi - mine);
+        const uint32_t all = low_bits(min(run, hi - mine)), before = low_bits(p.budget - mine);
+        word &= all;
+        *hole = ~word & before & all;
         *move = word & ~before;
     };
     auto list = [&](int mine, uint32_t hole, uint32_t move, int h0, int m0) {
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     };
     if constexpr (HELD) {   // one round
         static_assert(kMostKeys <= 32 * kSelect);
-        const int mine = lo + 32 * t;
+        const int mine = lo + run * t;
         uint32_t hole, move;
         int total;
         words(mine, &hole, &move);
@@ -527,8 +530,8 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     } else {
 #pragma unroll 1
         for (int pass = ctas > 1 ? 0 : 1; pass < 2; ++pass) {
-            for (int r0 = lo; r0 < hi; r0 += 32 * kSelect) {
-                const int mine = r0 + 32 * t;
+            for (int r0 = lo; r0 < hi; r0 += round) {
+                const int mine = r0 + run * t;
                 uint32_t hole, move;
                 int total;
                 words(mine, &hole, &move);
