@@ -327,13 +327,16 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     __shared__ __align__(8) int s_hist[kCopies + 2][kBins];
     __shared__ int s_scan[32];
     __shared__ int s_digit, s_above, s_here;
-    __shared__ int s_eq, s_last;              // read by the cluster's other CTAs, as are the next two
-    __shared__ int s_holes, s_movers;
+    __shared__ int s_eq, s_last;              // read by the cluster's other CTAs
+    __shared__ int s_holes[8], s_movers[8];   // every CTA's, written by them
     const cg::cluster_group cluster = cg::this_cluster();
     const int rank = blockIdx.x, ctas = gridDim.x;
     const int t = threadIdx.x, lane = t & 31, b = blockIdx.z;
     const size_t bh = static_cast<size_t>(b) * c.kv_heads + blockIdx.y;
+    for (int i = t; i < (kCopies + 2) * kBins; i += kSelect) (&s_hist[0][0])[i] = 0;
+    if (t == 0) s_last = -1;
     fer::dev::pdl_begin();
+    __syncthreads();
     bool bad;
     const int n = c.length(b, &bad);
     if (bad && t == 0 && rank == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
@@ -370,9 +373,6 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         if (ctas > 1) cluster.sync();
         else __syncthreads();
     };
-    for (int i = t; i < (kCopies + 2) * kBins; i += kSelect) (&s_hist[0][0])[i] = 0;
-    if (t == 0) s_last = -1;
-    __syncthreads();
     // keys, and the count of their first digit; kBatch loads in flight
     constexpr int kBatch = 8;
     for (int j0 = lo + t; j0 < hi; j0 += kBatch * kSelect) {
@@ -424,12 +424,15 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         static_assert(kPer == 2);
         int count[kPer] = {}, sum = 0;
         if (kPer * t < bins) {
+            int2 v[8];   // all in flight
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                if (r >= ctas) break;
-                const int2 v = *reinterpret_cast<const int2*>(cluster.map_shared_rank(hist, r) + bins - kPer * (t + 1));
-                count[0] += v.y, count[1] += v.x;
+                v[r] = make_int2(0, 0);
+                if (r < ctas)
+                    v[r] = *reinterpret_cast<const int2*>(cluster.map_shared_rank(hist, r) + bins - kPer * (t + 1));
             }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) count[0] += v[r].y, count[1] += v[r].x;
         }
         sum = count[0] + count[1];
         int total;
@@ -509,12 +512,12 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     int holes = 0, movers = 0;    // of this CTA, or of its rounds so far
     int hole0 = 0, mover0 = 0;    // of the CTAs before
     auto earlier = [&]() {
-        if (t == 0) s_holes = holes, s_movers = movers;
-        cluster.sync();
-        for (int r = 0; r < rank; ++r) {
-            hole0 += *cluster.map_shared_rank(&s_holes, r);
-            mover0 += *cluster.map_shared_rank(&s_movers, r);
+        if (t < ctas) {
+            *cluster.map_shared_rank(&s_holes[rank], t) = holes;
+            *cluster.map_shared_rank(&s_movers[rank], t) = movers;
         }
+        cluster.sync();   // the last: no CTA reads or writes another's shared memory behind it
+        for (int r = 0; r < rank; ++r) hole0 += s_holes[r], mover0 += s_movers[r];
     };
     if constexpr (HELD) {   // one round
         static_assert(kMostKeys <= 32 * kSelect);
@@ -549,7 +552,6 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     // all alike, unless the arrays changed meanwhile
     if (rank == ctas - 1 && t == 0)
         p.counts[bh] = min(mover0 + movers, min(hole0 + holes, p.cap));
-    if (ctas > 1) cluster.sync();   // no CTA leaves while another may read its shared memory
 }
 
 // grid (move tiles, kv_heads, batch), a warp kWarpMoves moves
