@@ -94,10 +94,11 @@ __device__ __forceinline__ float ex2(float v) {
 }
 // Tensor copy of a box of rows of one page: 64 dims from x, rows from r.
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int r, int head, int page,
-                                         uint32_t bar) {
+                                         uint32_t bar, uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
-            "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r), "r"(head), "r"(page), "r"(bar)
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::
+            "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r), "r"(head), "r"(page), "r"(bar), "l"(policy)
         : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
@@ -419,6 +420,11 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
         const int box_rows = min(kRound, c.page_size()), row_boxes = kRound / box_rows;
         const int boxes = 2 * (D / 64) * row_boxes;
         const uint32_t full0 = fer::dev::smem_addr(&s_full[0]);
+        // rows that are read once leave L2 first, so the parts and scores stay for the joining
+        // (two of 40003 slots with weights 38.3 -> 36.7 us, 131071 slots 95.2 -> 93.3)
+        uint64_t policy;
+        if (p.blocks == 1) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+        else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
         Unit x = run.get(c, p, table, u0, u1 - 1), next = x;
         ChunkPages pages = load_pages(c, x, x.chunk << p.chunk_log2), ahead = pages;
         int q = 0;
@@ -447,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
                     if (i < boxes)
                         load_box(ring + stage * C::kStage + value * C::kHalf + band * C::kBand + rows * 128,
                                  value ? &v_map : &k_map, band * 64, (k0 + slot) & (c.page_size() - 1), x.hk,
-                                 c.is_page(id) ? id : c.pages, full0 + 8 * stage);
+                                 c.is_page(id) ? id : c.pages, full0 + 8 * stage, policy);
                 }
             }
             x = next;
