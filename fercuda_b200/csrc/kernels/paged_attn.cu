@@ -677,10 +677,9 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
 }
 
 // log2 of a head's total sum of powers, from its chunks' (m, l), by one warp;
-// -inf where nothing counts. The base of the sum, and the sum, go to the two
-// others. BATCH loads a lane are in flight.
+// -inf where nothing counts. BATCH loads a lane are in flight.
 template <int BATCH>
-__device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float* base, float* sum) {
+__device__ __forceinline__ float chunks_lse2(const float* ml, int chunks) {
     const int lane = threadIdx.x & 31;
     float top = -INFINITY, l = 0.0f;
     for (int i0 = lane; i0 < chunks; i0 += 32 * BATCH) {
@@ -699,32 +698,30 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks, float*
         for (int k = 0; k < BATCH; ++k) l += v[k].y * ex2(v[k].x - b);
         top = next;
     }
+    float all = top;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        const float ot = __shfl_xor_sync(0xffffffffu, top, off), ol = __shfl_xor_sync(0xffffffffu, l, off);
-        const float next = fmaxf(top, ot), b = next == -INFINITY ? 0.0f : next;
-        // the same sum in both lanes of a pair
-        l = l * ex2(top - b) + ol * ex2(ot - b);
-        top = next;
-    }
-    *base = top == -INFINITY ? 0.0f : top;
-    *sum = l;
-    return l == 0.0f ? -INFINITY : *base + log2f(l);
+    for (int off = 16; off > 0; off >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, off));
+    const float base = all == -INFINITY ? 0.0f : all;
+    l *= ex2(top - base);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    return l == 0.0f ? -INFINITY : base + log2f(l);
 }
 
 // grid (group * D / DIMS + weight tiles, kv_heads, n_seq). The first CTAs of a
 // (key head, sequence) add one head's chunks for DIMS dims each: a warp takes
-// 32 of them and every kW-th chunk in order, then the warps' sums are added in
-// order. The others add probabilities to the weights of four slots a thread.
-// Both have what does not depend on the total in flight before they wait for
-// it.
+// every kW-th chunk in order, DIMS / 32 dims a lane, and the warps' sums,
+// each of a maximum of its own, are added in order. The others add
+// probabilities to the weights of four slots a thread, with what does not
+// depend on the total in flight before they wait for it.
 template <typename T, int D, int kFinish, int DIMS>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
-    constexpr int kIn = DIMS / 32, kW = kFinish / 32 / kIn, kBands = D / DIMS, kHeads = 4;
-    constexpr int kAhead = DIMS == D ? 8 : 16, kBatch = DIMS == D ? 1 : 8;
-    __shared__ float s_o[kW][DIMS];
+    constexpr int kW = kFinish / 32, kV = DIMS / 32, kBands = D / DIMS, kHeads = 4;
+    constexpr int kAhead = kV == 1 ? 16 : kV <= 4 ? 4 : 2, kBatch = DIMS == D ? 1 : 8;
+    __shared__ __align__(16) float s_o[kW][DIMS];
+    __shared__ float2 s_ml[kW];
     __shared__ float s_lse[kFinish];
-    const int t = threadIdx.x, lane = t & 31, w = (t >> 5) / kIn;
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     const int b = blockIdx.z, hk = blockIdx.y;
     fer::dev::pdl_begin();
     bool bad;
@@ -733,35 +730,56 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
     const size_t bh0 = static_cast<size_t>(b) * p.heads + static_cast<size_t>(hk) * p.group;
     if (static_cast<int>(blockIdx.x) < p.group * kBands) {
         if (chunks <= 1) return;                      // written already
-        const int g = blockIdx.x / kBands, in = t % DIMS, d = blockIdx.x % kBands * DIMS + in;
+        const int g = blockIdx.x / kBands, d0 = blockIdx.x % kBands * DIMS;
         const size_t bh = bh0 + g;
-        const float* ml = p.part_ml + 2 * bh * p.chunks;
-        const float* po = p.part_o + bh * p.chunks * D + d;
-        float v[kAhead], m[kAhead], base, l, o = 0.0f;
+        const float2* const ml = reinterpret_cast<const float2*>(p.part_ml) + bh * p.chunks;
+        struct alignas(4 * (kV < 4 ? kV : 4)) Dims { float e[kV]; };
+        const float* const po = p.part_o + bh * p.chunks * D + d0 + kV * lane;
+        float top = -INFINITY, l = 0.0f;
+        Dims o{};
+        for (int i0 = w; i0 < chunks; i0 += kW * kAhead) {
+            Dims v[kAhead];
+            float2 x[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int i = w + k * kW;
-            v[k] = 0.0f, m[k] = -INFINITY;
-            if (i < chunks) v[k] = po[static_cast<size_t>(i) * D], m[k] = ml[2 * i];
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + k * kW;
+                x[k] = make_float2(-INFINITY, 0.0f);
+                v[k] = Dims{};
+                if (i < chunks) x[k] = ml[i], v[k] = *reinterpret_cast<const Dims*>(po + static_cast<size_t>(i) * D);
+            }
+            float next = top;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) next = fmaxf(next, x[k].x);
+            const float base = next == -INFINITY ? 0.0f : next, f = ex2(top - base);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < kV; ++e) o.e[e] *= f;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const float y = ex2(x[k].x - base);
+                l = fmaf(x[k].y, y, l);
+#pragma unroll
+                for (int e = 0; e < kV; ++e) o.e[e] = fmaf(v[k].e[e], y, o.e[e]);
+            }
+            top = next;
         }
-        const float lse2 = chunks_lse2<kBatch>(ml, chunks, &base, &l);
+        *reinterpret_cast<Dims*>(&s_o[w][kV * lane]) = o;
+        if (lane == 0) s_ml[w] = make_float2(top, l);
+        __syncthreads();
+        if (t >= DIMS) return;
+        float all = -INFINITY, sum = 0.0f, out = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-            if (w + k * kW < chunks) o = fmaf(v[k], ex2(m[k] - base), o);
-#pragma unroll 4
-        for (int i = w + kAhead * kW; i < chunks; i += kW)
-            o = fmaf(po[static_cast<size_t>(i) * D], ex2(ml[2 * i] - base), o);
-        if constexpr (kW > 1) {
-            s_o[w][in] = o;
-            __syncthreads();
-            if (w > 0) return;
-            o = 0.0f;
+        for (int i = 0; i < kW; ++i) all = fmaxf(all, s_ml[i].x);
+        const float base = all == -INFINITY ? 0.0f : all;
 #pragma unroll
-            for (int i = 0; i < kW; ++i) o += s_o[i][in];
+        for (int i = 0; i < kW; ++i) {
+            const float y = ex2(s_ml[i].x - base);
+            sum = fmaf(s_ml[i].y, y, sum);
+            out = fmaf(s_o[i][t], y, out);
         }
-        static_cast<T*>(p.out)[b * p.os + (static_cast<size_t>(hk) * p.group + g) * D + d] =
-            static_cast<T>(l == 0.0f ? 0.0f : o / l);
-        if (d == 0 && p.lse) p.lse[bh] = lse2 * kLn2;
+        static_cast<T*>(p.out)[b * p.os + (static_cast<size_t>(hk) * p.group + g) * D + d0 + t] =
+            static_cast<T>(sum == 0.0f ? 0.0f : out / sum);
+        if (d0 + t == 0 && p.lse) p.lse[bh] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * kLn2;
         return;
     }
     const int j0 = (blockIdx.x - p.group * kBands) * 4 * kFinish;
@@ -781,8 +799,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
         const int ng = min(kFinish, p.group - g0);
         __syncthreads();
         for (int g = t >> 5; g < ng; g += kFinish / 32) {
-            float base, l;
-            const float v = chunks_lse2<kBatch>(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks, &base, &l);
+            const float v = chunks_lse2<kBatch>(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks);
             if (lane == 0) s_lse[g] = v;
         }
         __syncthreads();
