@@ -28,7 +28,7 @@
 // launch does it all.
 //
 // Above (evict_select): a CTA a head, or a cluster of 2 to 8 of them, with the
-// keys in shared memory, and three digits of 11, 11 and 10 bits counted there;
+// keys in shared memory, and three digits of 12, 12 and 8 bits counted there;
 // the other CTAs' counts are read through distributed shared memory. Beyond 8
 // x 32K slots the keys are made again for every pass.
 //
@@ -52,7 +52,7 @@ constexpr int kSelect = 1024;                // threads of a selecting CTA
 constexpr int kWarps = kSelect / 32;
 constexpr int kMostKeys = 32 * 1024;         // keys a CTA holds in shared memory
 constexpr int kCopies = 3;                   // of the first digit's counts, by lane: less contention
-constexpr int kBins = 2048;
+constexpr int kWords = 2048;                 // of a digit's counts
 constexpr int kMove = 256;
 constexpr int kWarpMoves = 16;
 constexpr int kFusedMoves = 32;
@@ -324,7 +324,7 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
 template <bool HELD>
 __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const EvictParams p) {
     extern __shared__ __align__(16) uint32_t s_key[];
-    __shared__ __align__(8) int s_hist[kCopies + 2][kBins];
+    __shared__ __align__(8) uint32_t s_hist[kCopies + 2][kWords];
     __shared__ int s_scan[32];
     __shared__ int s_digit, s_above, s_here;
     __shared__ int s_eq, s_last;              // read by the cluster's other CTAs
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     const int rank = blockIdx.x, ctas = gridDim.x;
     const int t = threadIdx.x, lane = t & 31, b = blockIdx.z;
     const size_t bh = static_cast<size_t>(b) * c.kv_heads + blockIdx.y;
-    for (int i = t; i < (kCopies + 2) * kBins; i += kSelect) (&s_hist[0][0])[i] = 0;
+    for (int i = t; i < (kCopies + 2) * kWords; i += kSelect) (&s_hist[0][0])[i] = 0u;
     if (t == 0) s_last = -1;
     fer::dev::pdl_begin();
     __syncthreads();
@@ -373,6 +373,14 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         if (ctas > 1) cluster.sync();
         else __syncthreads();
     };
+    // Digits of 12, 12 and 8 bits, two counts a word (a CTA's held keys are few
+    // enough); else of 11, 11 and 10, a word each.
+    constexpr int kPack = HELD ? 2 : 1;
+    constexpr int kShift[3] = {HELD ? 20 : 21, HELD ? 8 : 10, 0}, kBins[3] = {kPack * kWords, kPack * kWords, HELD ? 256 : 1024};
+    auto count_one = [&](uint32_t* hist, uint32_t bin) {
+        if constexpr (HELD) atomicAdd(&hist[bin >> 1], bin & 1 ? 0x10000u : 1u);
+        else atomicAdd(&hist[bin], 1u);
+    };
     // keys, and the count of their first digit; kBatch loads in flight
     constexpr int kBatch = 8;
     for (int j0 = lo + t; j0 < hi; j0 += kBatch * kSelect) {
@@ -390,7 +398,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
             if (j >= hi) break;
             const uint32_t key = key_of(wt[k], pos[k], first);
             if constexpr (HELD) s_key[(j - lo) + (j - lo) / 32 * 4] = key;
-            atomicAdd(&s_hist[lane % kCopies][key >> 21], 1);
+            count_one(s_hist[lane % kCopies], key >> kShift[0]);
             if (j < p.budget) {
                 if (h.nw != h.w) h.nw[j] = wt[k];
                 if (h.np != h.pos) h.np[j] = pos[k];
@@ -401,18 +409,18 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     int left = p.budget, equal = 0;   // slots to be found among the keys that begin like the cut, and how many those are
 #pragma unroll
     for (int d = 0; d < 3; ++d) {
-        const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bins = d == 2 ? 1024 : 2048;
-        int* hist = s_hist[d == 0 ? 0 : kCopies + d - 1];
+        const int shift = kShift[d], bins = kBins[d];
+        uint32_t* const hist = s_hist[d == 0 ? 0 : kCopies + d - 1];
         if (d > 0) {
-            const uint32_t mask = d == 1 ? 0xffe00000u : 0xfffffc00u;   // the digits found so far
+            const uint32_t mask = ~0u << kShift[d - 1];   // the digits found so far
             for (int mine = lo + run * t; mine < hi; mine += round)
                 each_key(mine, [&](int i, uint32_t key) {
-                    if ((key & mask) == cut && mine + i < hi) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1);
+                    if ((key & mask) == cut && mine + i < hi) count_one(hist, (key >> shift) & (bins - 1));
                 });
         } else {
             __syncthreads();
-            for (int i = t; i < kBins; i += kSelect) {
-                int n0 = hist[i];
+            for (int i = t; i < kWords; i += kSelect) {
+                uint32_t n0 = hist[i];
 #pragma unroll
                 for (int k = 1; k < kCopies; ++k) n0 += s_hist[k][i];
                 hist[i] = n0;
@@ -420,28 +428,41 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         }
         meet();
         // thread t has the kPer bins from kPer t on, counted from the top
-        constexpr int kPer = kBins / kSelect;
-        static_assert(kPer == 2);
-        int count[kPer] = {}, sum = 0;
+        constexpr int kPer = 2 * kPack;
+        static_assert(kPer * kSelect == kBins[0]);
+        int count[kPer] = {};
         if (kPer * t < bins) {
-            int2 v[8];   // all in flight
+            uint2 v[8];   // all in flight
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                v[r] = make_int2(0, 0);
+                v[r] = make_uint2(0u, 0u);
                 if (r < ctas)
-                    v[r] = *reinterpret_cast<const int2*>(cluster.map_shared_rank(hist, r) + bins - kPer * (t + 1));
+                    v[r] = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + (bins - kPer * (t + 1)) / kPack);
             }
 #pragma unroll
-            for (int r = 0; r < 8; ++r) count[0] += v[r].y, count[1] += v[r].x;
+            for (int r = 0; r < 8; ++r) {
+                if constexpr (HELD) {
+                    count[0] += v[r].y >> 16, count[1] += v[r].y & 0xffffu;
+                    count[2] += v[r].x >> 16, count[3] += v[r].x & 0xffffu;
+                } else {
+                    count[0] += v[r].y, count[1] += v[r].x;
+                }
+            }
         }
-        sum = count[0] + count[1];
-        int total;
+        int sum = 0, total;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += count[i];
         int before = block_scan(sum, s_scan, &total);
         if (before < left && left <= before + sum) {
-            const bool second = left > before + count[0];
-            s_digit = bins - 1 - (kPer * t + (second ? 1 : 0));
-            s_above = before + (second ? count[0] : 0);
-            s_here = second ? count[1] : count[0];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (before < left && left <= before + count[i]) {
+                    s_digit = bins - 1 - (kPer * t + i);
+                    s_above = before;
+                    s_here = count[i];
+                }
+                before += count[i];
+            }
         }
         __syncthreads();
         cut |= static_cast<uint32_t>(s_digit) << shift;
