@@ -14,7 +14,7 @@
 //
 // Measured: 64 sequences x 16 heads of 64 cut from 513 to 512 slots 6.4 us
 // (one chain of latencies: arrays, cut, page ids, rows); 4 sequences of up to
-// 32768 x 8 heads of 128 cut to 4096 35.4 us, of which 15 us are the selection
+// 32768 x 8 heads of 128 cut to 4096 32.2 us, of which 13 us are the selection
 // and 17 us the moves (16.5 us for all bytes at the copy rate).
 //
 // Up to 1024 slots (evict_small): a warp a head with its keys in registers,
@@ -32,8 +32,9 @@
 // the other CTAs' counts are read through distributed shared memory. Beyond 8
 // x 32K slots the keys are made again for every pass.
 //
-// The moves (evict_move): a warp resolves 16 moves at once, a lane each, then
-// copies their rows with kAhead 16-byte loads a lane in flight.
+// The moves (evict_move, or the selecting CTAs where heads come in waves): a
+// warp resolves up to 32 moves at once, a lane each, then copies their rows
+// with kAhead 16-byte loads a lane in flight.
 #include "paged.cuh"
 #include "pdl.cuh"
 
@@ -56,11 +57,13 @@ constexpr int kWords = 2048;                 // of a digit's counts
 constexpr int kMove = 256;
 constexpr int kWarpMoves = 16;
 constexpr int kFusedMoves = 32;
+constexpr int kFuseCtas = 2 * 148;           // selecting CTAs from which on they also move rows
 constexpr int kFewDropped = 4;               // slots too many that are found one by one
 
 struct EvictParams {
     int budget, recent, cap;     // cap: moves a (sequence, key head) can have
-    int fused;                   // the selecting warp moves rows
+    int fused;                   // the selecting kernel moves rows
+    int late;                    // lengths are replaced in place, by a kernel behind all of their readers
     const float* weights;
     const int32_t* positions;
     const int32_t* seen;
@@ -98,10 +101,10 @@ __device__ __forceinline__ Head head_of(const Paged& c, const EvictParams& p, si
 
 // Up to 32 moves of one head, move i0 + lane in each lane: their slots are
 // resolved to rows, a lane each, then all lanes copy row after row.
-template <int D>
+template <int D, int kAhead>
 __device__ __forceinline__ void move_rows(const Paged& c, const EvictParams& p, const Head& h, int hk, bool mine,
                                           int from, int to, int pf, int pt) {   // pf, pt: their pages, as the table has them
-    constexpr int kPieces = D / 8, kRows = 32 / kPieces, kAhead = 8;   // lanes a row, rows at once
+    constexpr int kPieces = D / 8, kRows = 32 / kPieces;   // lanes a row, rows at once
     const int lane = threadIdx.x & 31, piece = lane % kPieces;
     unsigned long long src = 0, dst = 0;
     bool good = false;
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictPar
         if (p.fused) {
             __syncwarp();
             const int f = lane < moved ? from[lane] : 0, g = lane < moved ? to[lane] : 0;
-            move_rows<D>(c, p, h, hk, lane < moved, f, g, page_of(f >> c.shift), page_of(g >> c.shift));
+            move_rows<D, 8>(c, p, h, hk, lane < moved, f, g, page_of(f >> c.shift), page_of(g >> c.shift));
             __syncwarp();
         } else if (lane == 0) {
             p.counts[bh] = moved;
@@ -321,7 +324,7 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
 // evenly; the key of slot lo + j lies at word j + 4 (j / 32) of shared memory,
 // so that threads read 32 in 16-byte pieces without bank conflicts. Without
 // HELD the keys of a round are made again from the arrays.
-template <bool HELD>
+template <int D, bool HELD>
 __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const EvictParams p) {
     extern __shared__ __align__(16) uint32_t s_key[];
     __shared__ __align__(8) uint32_t s_hist[kCopies + 2][kWords];
@@ -341,6 +344,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     const int n = c.length(b, &bad);
     if (bad && t == 0 && rank == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
     const Head h = head_of(c, p, bh);
+    if (p.fused && !p.late && t == 0 && rank == 0 && blockIdx.y == 0) p.new_lengths[b] = min(n, p.budget);
     if (n <= p.budget) {   // the same for the whole cluster
         copy_whole(h, n, rank * kSelect + t, ctas * kSelect);
         if (t == 0 && rank == 0) p.counts[bh] = 0;
@@ -571,8 +575,24 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         }
     }
     // all alike, unless the arrays changed meanwhile
-    if (rank == ctas - 1 && t == 0)
-        p.counts[bh] = min(mover0 + movers, min(hole0 + holes, p.cap));
+    if (!HELD || !p.fused) {
+        if (rank == ctas - 1 && t == 0) p.counts[bh] = min(mover0 + movers, min(hole0 + holes, p.cap));
+        return;
+    }
+    // the cluster's warps share the moves out among them
+    if (ctas > 1) {
+        holes = movers = 0;
+        for (int r = 0; r < ctas; ++r) holes += s_holes[r], movers += s_movers[r];
+    }
+    const int moved = min(movers, min(holes, p.cap));
+    const int share = max(1, min(32, (moved - 1) / (kWarps * ctas) + 1));
+    meet();   // the lists are written
+    const int32_t* const row = c.table + static_cast<size_t>(b) * c.max_pages;
+    for (int i0 = (rank * kWarps + (t >> 5)) * share; i0 < moved; i0 += kWarps * ctas * share) {
+        const bool mine = lane < share && i0 + lane < moved;
+        const int from = mine ? h.from[i0 + lane] : 0, to = mine ? h.to[i0 + lane] : 0;
+        move_rows<D, 4>(c, p, h, blockIdx.y, mine, from, to, row[from >> c.shift], row[to >> c.shift]);
+    }
 }
 
 // grid (move tiles, kv_heads, batch), a warp kWarpMoves moves
@@ -592,7 +612,14 @@ __global__ void __launch_bounds__(kMove) evict_move(const Paged c, const EvictPa
     const Head h = head_of(c, p, bh);
     const int from = mine ? h.from[i] : 0, to = mine ? h.to[i] : 0;
     const int32_t* const row = c.table + static_cast<size_t>(b) * c.max_pages;
-    move_rows<D>(c, p, h, hk, mine, from, to, row[from >> c.shift], row[to >> c.shift]);
+    move_rows<D, 8>(c, p, h, hk, mine, from, to, row[from >> c.shift], row[to >> c.shift]);
+}
+
+__global__ void __launch_bounds__(kMove) evict_lengths(const Paged c, const EvictParams p, const int batch) {
+    fer::dev::pdl_begin();
+    const int b = blockIdx.x * kMove + threadIdx.x;
+    bool bad;
+    if (b < batch) p.new_lengths[b] = min(c.length(b, &bad), p.budget);
 }
 
 int most_moves(int max_slots, int budget) {
@@ -647,28 +674,38 @@ cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
                                : small<D, 32>(c, p, batch, s);
         if (e != cudaSuccess || p.fused) return e;
     } else {
-        // As many CTAs a head as its keys need; up to eight where SMs would be left over, a CTA at least 4096 slots
-        // (32 heads of 32768 slots: 20 us with one CTA a head, 18 with four).
+        // As many CTAs a head as its keys need; more where SMs would be left over, a CTA at least 4096 slots
+        // (32 heads of 32768 slots: 20 us with one CTA a head, 18 with four). Eight only for up to eight heads:
+        // clusters of eight do not fill all SMs (16 heads of 32768 slots: 32 us in all with four, 44 with eight).
+        const long long heads = static_cast<long long>(c.kv_heads) * batch;
         unsigned ctas = 1;
         while (ctas < 8 && static_cast<long long>(ctas) * kMostKeys < max_slots) ctas *= 2;
-        while (ctas < 8 && 2ll * ctas * c.kv_heads * batch <= 148 && ctas * 4096ll < max_slots) ctas *= 2;
+        while (ctas < 4 && 2 * ctas * heads <= 148 && ctas * 4096ll < max_slots) ctas *= 2;
+        if (ctas == 4 && heads <= 8 && 4 * 4096 < max_slots) ctas = 8;
         const int each = ((max_slots - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
         const bool held = each <= kMostKeys;
+        // In several waves the moves of one head overlap the selection of others (512 heads of 8192 slots cut to
+        // 4096, rows of 64: 202 us in two kernels, 152 in one); in one wave they gain nothing (32 heads: 32.2 and
+        // 32.0) or, with few CTAs, are slower (1 head of 8192: 23.8 and 32.4).
+        p.fused = held && ctas * heads >= kFuseCtas;
+        p.late = p.new_lengths == c.lengths;
         const size_t smem = held ? static_cast<size_t>(each) / 32 * 36 * 4 : 0;
         static std::atomic<bool> set[fer::host::kMaxDevices];
         int dev = 0;
         e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
         if (dev >= fer::host::kMaxDevices || !set[dev].load(std::memory_order_relaxed)) {
-            e = cudaFuncSetAttribute(evict_select<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(evict_select<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      kMostKeys / 32 * 36 * 4);
             if (e != cudaSuccess) return e;
             if (dev < fer::host::kMaxDevices) set[dev].store(true, std::memory_order_relaxed);
         }
         const dim3 grid(ctas, c.kv_heads, batch);
-        e = held ? launch_cluster(evict_select<true>, grid, dim3(kSelect), smem, ctas, s, c, p)
-                 : launch_cluster(evict_select<false>, grid, dim3(kSelect), 0, ctas, s, c, p);
-        if (e != cudaSuccess) return e;
+        e = held ? launch_cluster(evict_select<D, true>, grid, dim3(kSelect), smem, ctas, s, c, p)
+                 : launch_cluster(evict_select<D, false>, grid, dim3(kSelect), 0, ctas, s, c, p);
+        if (e != cudaSuccess || (p.fused && !p.late)) return e;
+        if (p.fused)
+            return fer::host::launch_pdl(evict_lengths, dim3((batch + kMove - 1) / kMove), dim3(kMove), 0, s, c, p, batch);
     }
     constexpr int kTile = kMove / 32 * kWarpMoves;
     const dim3 grid((p.cap + kTile - 1) / kTile + (p.cap == 0), c.kv_heads, batch);
