@@ -28,7 +28,8 @@
 // launch does it all.
 //
 // Above (evict_select): a CTA a head, or a cluster of 2 to 8 of them, with the
-// keys in shared memory, and three digits of 12, 12 and 8 bits counted there;
+// keys in shared memory, and three digits of 12, 12 and 8 bits (or four of 10
+// in the smaller CTAs that short heads take where there are many) counted there;
 // the other CTAs' counts are read through distributed shared memory. Beyond 8
 // x 32K slots the keys are made again for every pass.
 //
@@ -49,11 +50,9 @@ namespace cg = cooperative_groups;
 using fer::dev::Paged;
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr int kSmall = 1024;                 // slots that a warp's registers hold
-constexpr int kSelect = 1024;                // threads of a selecting CTA
-constexpr int kWarps = kSelect / 32;
-constexpr int kMostKeys = 32 * 1024;         // keys a CTA holds in shared memory
+constexpr int kSelect = 1024, kSelectFew = 256;   // threads of a selecting CTA
+constexpr int kMostKeys = 32;                // keys a thread of it holds in shared memory
 constexpr int kCopies = 3;                   // of the first digit's counts, by lane: less contention
-constexpr int kWords = 2048;                 // of a digit's counts
 constexpr int kMove = 256;
 constexpr int kWarpMoves = 16;
 constexpr int kFusedMoves = 32;
@@ -303,6 +302,7 @@ __global__ void __launch_bounds__(256) evict_small(const Paged c, const EvictPar
 }
 
 // Exclusive prefix sum over the block, and the total.
+template <int kWarps>
 __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
     int x = v;
@@ -324,10 +324,15 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
 // evenly; the key of slot lo + j lies at word j + 4 (j / 32) of shared memory,
 // so that threads read 32 in 16-byte pieces without bank conflicts. Without
 // HELD the keys of a round are made again from the arrays.
-template <int D, bool HELD>
-__global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const EvictParams p) {
+template <int D, bool HELD, int kSelect>
+__global__ void __launch_bounds__(kSelect, 1024 / kSelect) evict_select(const Paged c, const EvictParams p) {
+    // Digits: with two counts a word (a CTA's held keys are few enough), four
+    // bins a thread, else two.
+    constexpr int kWarps = kSelect / 32, kWords = 2 * kSelect, kPack = HELD ? 2 : 1, kPer = 2 * kPack;
+    constexpr int kLog = (kSelect == 1024 ? 10 : 8) + kPack, kDigits = (31 + kLog) / kLog;
+    static_assert(kPer * kSelect == 1 << kLog);
     extern __shared__ __align__(16) uint32_t s_key[];
-    __shared__ __align__(8) uint32_t s_hist[kCopies + 2][kWords];
+    __shared__ __align__(8) uint32_t s_hist[kCopies + kDigits - 1][kWords];
     __shared__ int s_scan[32];
     __shared__ int s_digit, s_above, s_here;
     __shared__ int s_eq, s_last;              // read by the cluster's other CTAs
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     const int rank = blockIdx.x, ctas = gridDim.x;
     const int t = threadIdx.x, lane = t & 31, b = blockIdx.z;
     const size_t bh = static_cast<size_t>(b) * c.kv_heads + blockIdx.y;
-    for (int i = t; i < (kCopies + 2) * kWords; i += kSelect) (&s_hist[0][0])[i] = 0u;
+    for (int i = t; i < (kCopies + kDigits - 1) * kWords; i += kSelect) (&s_hist[0][0])[i] = 0u;
     if (t == 0) s_last = -1;
     fer::dev::pdl_begin();
     __syncthreads();
@@ -377,10 +382,6 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         if (ctas > 1) cluster.sync();
         else __syncthreads();
     };
-    // Digits of 12, 12 and 8 bits, two counts a word (a CTA's held keys are few
-    // enough); else of 11, 11 and 10, a word each.
-    constexpr int kPack = HELD ? 2 : 1;
-    constexpr int kShift[3] = {HELD ? 20 : 21, HELD ? 8 : 10, 0}, kBins[3] = {kPack * kWords, kPack * kWords, HELD ? 256 : 1024};
     auto count_one = [&](uint32_t* hist, uint32_t bin) {
         if constexpr (HELD) atomicAdd(&hist[bin >> 1], bin & 1 ? 0x10000u : 1u);
         else atomicAdd(&hist[bin], 1u);
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
             if (j >= hi) break;
             const uint32_t key = key_of(wt[k], pos[k], first);
             if constexpr (HELD) s_key[(j - lo) + (j - lo) / 32 * 4] = key;
-            count_one(s_hist[lane % kCopies], key >> kShift[0]);
+            count_one(s_hist[lane % kCopies], key >> (32 - kLog));
             if (j < p.budget) {
                 if (h.nw != h.w) h.nw[j] = wt[k];
                 if (h.np != h.pos) h.np[j] = pos[k];
@@ -412,11 +413,11 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
     uint32_t cut = 0u;
     int left = p.budget, equal = 0;   // slots to be found among the keys that begin like the cut, and how many those are
 #pragma unroll
-    for (int d = 0; d < 3; ++d) {
-        const int shift = kShift[d], bins = kBins[d];
+    for (int d = 0; d < kDigits; ++d) {
+        const int above = 32 - d * kLog, shift = max(0, above - kLog), bins = 1 << (above - shift);
         uint32_t* const hist = s_hist[d == 0 ? 0 : kCopies + d - 1];
         if (d > 0) {
-            const uint32_t mask = ~0u << kShift[d - 1];   // the digits found so far
+            const uint32_t mask = ~0u << above;   // the digits found so far
             for (int mine = lo + run * t; mine < hi; mine += round)
                 each_key(mine, [&](int i, uint32_t key) {
                     if ((key & mask) == cut && mine + i < hi) count_one(hist, (key >> shift) & (bins - 1));
@@ -432,8 +433,6 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         }
         meet();
         // thread t has the kPer bins from kPer t on, counted from the top
-        constexpr int kPer = 2 * kPack;
-        static_assert(kPer * kSelect == kBins[0]);
         int count[kPer] = {};
         if (kPer * t < bins) {
             uint2 v[8];   // all in flight
@@ -456,7 +455,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         int sum = 0, total;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) sum += count[i];
-        int before = block_scan(sum, s_scan, &total);
+        int before = block_scan<kWarps>(sum, s_scan, &total);
         if (before < left && left <= before + sum) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
@@ -487,7 +486,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         if (ctas > 1) {
             int mine = 0;
             for (int r0 = lo; r0 < hi; r0 += round) mine += __popc(word_of(r0 + run * t));
-            block_scan(mine, s_scan, &total);
+            block_scan<kWarps>(mine, s_scan, &total);
             if (t == 0) s_eq = total;
             cluster.sync();
             for (int r = 0; r < rank; ++r) before += *cluster.map_shared_rank(&s_eq, r);
@@ -495,7 +494,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         for (int r0 = lo; r0 < hi; r0 += round) {
             uint32_t word = word_of(r0 + run * t);
             const int here = __popc(word);
-            const int at = before + block_scan(here, s_scan, &total);
+            const int at = before + block_scan<kWarps>(here, s_scan, &total);
             if (at < left && left <= at + here) {   // the last one is this thread's
                 for (int k = at + 1; k < left; ++k) word &= word - 1u;
                 s_last = r0 + run * t + __ffs(word) - 1;
@@ -545,12 +544,12 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
         for (int r = 0; r < rank; ++r) hole0 += s_holes[r], mover0 += s_movers[r];
     };
     if constexpr (HELD) {   // one round
-        static_assert(kMostKeys <= 32 * kSelect);
+        static_assert(kMostKeys <= 32);
         const int mine = lo + run * t;
         uint32_t hole, move;
         int total;
         words(mine, &hole, &move);
-        const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
+        const int at = block_scan<kWarps>(__popc(hole) | __popc(move) << 16, s_scan, &total);
         holes = low_half(total);
         movers = high_half(total);
         if (ctas > 1) earlier();
@@ -563,7 +562,7 @@ __global__ void __launch_bounds__(kSelect, 1) evict_select(const Paged c, const 
                 uint32_t hole, move;
                 int total;
                 words(mine, &hole, &move);
-                const int at = block_scan(__popc(hole) | __popc(move) << 16, s_scan, &total);
+                const int at = block_scan<kWarps>(__popc(hole) | __popc(move) << 16, s_scan, &total);
                 if (pass == 1) list(mine, hole, move, hole0 + holes + low_half(at), mover0 + movers + high_half(at));
                 holes += low_half(total);
                 movers += high_half(total);
@@ -661,6 +660,25 @@ cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t 
     return launch_cluster(evict_small<D, KEYS>, dim3(ctas, batch), dim3(32 * warps), 0, cluster, s, c, p);
 }
 
+template <int D, bool HELD, int THREADS>
+cudaError_t select(const Paged& c, const EvictParams& p, unsigned ctas, int batch, cudaStream_t s) {
+    const auto kernel = evict_select<D, HELD, THREADS>;
+    const int each = ((c.max_slots() - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
+    const size_t smem = HELD ? static_cast<size_t>(each) / 32 * 36 * 4 : 0;
+    if (HELD) {
+        static std::atomic<bool> set[fer::host::kMaxDevices];
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev >= fer::host::kMaxDevices || !set[dev].load(std::memory_order_relaxed)) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostKeys * THREADS / 32 * 36 * 4);
+            if (e != cudaSuccess) return e;
+            if (dev < fer::host::kMaxDevices) set[dev].store(true, std::memory_order_relaxed);
+        }
+    }
+    return launch_cluster(kernel, dim3(ctas, c.kv_heads, batch), dim3(THREADS), smem, ctas, s, c, p);
+}
+
 template <int D>
 cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
     cudaError_t e;
@@ -679,30 +697,22 @@ cudaError_t run(const Paged& c, EvictParams& p, int batch, cudaStream_t s) {
         // clusters of eight do not fill all SMs (16 heads of 32768 slots: 32 us in all with four, 44 with eight).
         const long long heads = static_cast<long long>(c.kv_heads) * batch;
         unsigned ctas = 1;
-        while (ctas < 8 && static_cast<long long>(ctas) * kMostKeys < max_slots) ctas *= 2;
+        while (ctas < 8 && static_cast<long long>(ctas) * kMostKeys * kSelect < max_slots) ctas *= 2;
         while (ctas < 4 && 2 * ctas * heads <= 148 && ctas * 4096ll < max_slots) ctas *= 2;
         if (ctas == 4 && heads <= 8 && 4 * 4096 < max_slots) ctas = 8;
-        const int each = ((max_slots - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
-        const bool held = each <= kMostKeys;
         // In several waves the moves of one head overlap the selection of others (512 heads of 8192 slots cut to
         // 4096, rows of 64: 202 us in two kernels, 152 in one); in one wave they gain nothing (32 heads: 32.2 and
         // 32.0) or, with few CTAs, are slower (1 head of 8192: 23.8 and 32.4).
+        const bool held = max_slots <= static_cast<long long>(ctas) * kMostKeys * kSelect;
         p.fused = held && ctas * heads >= kFuseCtas;
         p.late = p.new_lengths == c.lengths;
-        const size_t smem = held ? static_cast<size_t>(each) / 32 * 36 * 4 : 0;
-        static std::atomic<bool> set[fer::host::kMaxDevices];
-        int dev = 0;
-        e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        if (dev >= fer::host::kMaxDevices || !set[dev].load(std::memory_order_relaxed)) {
-            e = cudaFuncSetAttribute(evict_select<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     kMostKeys / 32 * 36 * 4);
-            if (e != cudaSuccess) return e;
-            if (dev < fer::host::kMaxDevices) set[dev].store(true, std::memory_order_relaxed);
-        }
-        const dim3 grid(ctas, c.kv_heads, batch);
-        e = held ? launch_cluster(evict_select<D, true>, grid, dim3(kSelect), smem, ctas, s, c, p)
-                 : launch_cluster(evict_select<D, false>, grid, dim3(kSelect), 0, ctas, s, c, p);
+        // More heads than SMs, and short ones: several small CTAs an SM hide one another's latencies (1344 heads of
+        // 1560 slots cut to 542: 121 us with 1024 threads, 77 with 256; 320 of 8000 to 7990: 36 and 26). With many
+        // moves a head large CTAs in more waves overlap better (512 of 8192 to 4096: 153 and 174).
+        const bool small_ctas = heads > 148 && max_slots <= kMostKeys * kSelectFew && p.cap <= 2048;
+        e = !held        ? select<D, false, kSelect>(c, p, ctas, batch, s)
+            : small_ctas ? select<D, true, kSelectFew>(c, p, ctas, batch, s)
+                         : select<D, true, kSelect>(c, p, ctas, batch, s);
         if (e != cudaSuccess || (p.fused && !p.late)) return e;
         if (p.fused)
             return fer::host::launch_pdl(evict_lengths, dim3((batch + kMove - 1) / kMove), dim3(kMove), 0, s, c, p, batch);
