@@ -590,13 +590,15 @@ def test_evict_long(session, n, budget):
     check_evict(c, budget, min(budget, 128), w0, p0, i32(c.lens), before, (c.k, c.v, w, p, c.lengths))
 
 
-@pytest.mark.parametrize("D,H,page", [(64, 8, 16), (128, 4, 32), (256, 2, 8)])
+@pytest.mark.parametrize("D,H,page,heads,most,budget", [
+    (64, 8, 16, 320, 1500, 700), (128, 4, 32, 320, 1500, 700), (256, 2, 8, 160, 1500, 700),
+    (64, 4, 64, 300, 5200, 2400)])       # many moves a head
 @pytest.mark.parametrize("in_place", [False, True])
-def test_evict_of_large_batches(session, D, H, page, in_place):
-    """More heads than the GPU holds CTAs at once; some sequences need no cut."""
-    B = 320 // H
-    lens = torch.randint(500, 1500, (B,), generator=torch.Generator().manual_seed(H)).tolist()
-    lens[0], lens[-1] = 0, 1500
+def test_evict_of_large_batches(session, D, H, page, heads, most, budget, in_place):
+    """More heads than the GPU has SMs; some sequences need no cut."""
+    B = heads // H
+    lens = torch.randint(most // 3, most, (B,), generator=torch.Generator().manual_seed(H)).tolist()
+    lens[0], lens[-1] = 0, most
     c = ref.Cache(lens, H, D, page, BF16)
     w = weights_for("spread", B, H, c.slots, seed=H).cuda()
     w[torch.rand(w.shape, device="cuda") < 0.2] = 0.5
@@ -605,9 +607,9 @@ def test_evict_of_large_batches(session, D, H, page, in_place):
     mark = (torch.full_like(w, 123.0), torch.full_like(p, -9))
     before = (c.k.cpu().clone(), c.v.cpu().clone(), *((w0, p0) if in_place else mark))
     out = None if in_place else (torch.full_like(c.lengths, -1), *[t.clone() for t in mark])
-    run_evict(session, c, 700, 60, w, p, i32(lens), out)
+    run_evict(session, c, budget, 60, w, p, i32(lens), out)
     now = (c.k, c.v, w, p, c.lengths) if in_place else (c.k, c.v, out[1], out[2], out[0])
-    check_evict(c, 700, 60, w0, p0, i32(lens), before, now)
+    check_evict(c, budget, 60, w0, p0, i32(lens), before, now)
 
 
 @pytest.mark.parametrize("n", [262144, 300000])   # in shared memory, and not
