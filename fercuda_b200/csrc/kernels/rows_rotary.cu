@@ -17,7 +17,9 @@
 // neighbouring units, then neighbouring heads: a warp reads the row front to
 // back. A unit of the half-split layout is V elements of the first half and
 // the V that pair with them; V is the widest that pointers, strides and sizes
-// allow.
+// allow. What lies behind the turned part of a head is copied by itself, in the
+// widest pieces that fit it (16384 rows of 32 heads x 128 of which 64 turn: 61
+// us; 111 as further units of the turning lanes).
 //
 // Measured: 32768 rows of 32 heads x 64 bf16 45.6 us, 5.9 TB/s (90% of the HBM
 // copy rate); 10007 rows of 40 heads x 128 f16 with three axes 39.0 us, 5.3
@@ -37,6 +39,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kAhead = 4;   // loads a lane makes before it turns the first
+constexpr int kTailHeads = 4096;
 
 struct RotaryParams {
     const void* x;
@@ -45,9 +48,12 @@ struct RotaryParams {
     size_t xs, os;
     int rows, heads, head_dim, half, axes;
     int bound[4];     // first pair behind each axis
-    int units;        // units a head, the copied tail's among them
-    int across;       // units a warp takes at once
+    int units;        // that turn, a head
+    int across;       // of them a warp takes at once
     int hp;           // heads a warp takes at once
+    int tail;         // pieces behind the turned part of a head that are copied
+    int tail_bytes;   // of such a piece
+    uint32_t tail_inverse;   // ceil(2^32 / tail)
     int split;        // warps a row
     int share;        // heads of one of them
     float base;
@@ -102,7 +108,31 @@ struct alignas(sizeof(T) * A) Piece {
     }
 };
 
-template <typename T, int V, int A, bool INTER>
+// A warp copies the `tail` pieces behind the turned part of `heads` heads of a
+// row, `head` bytes apart.
+template <typename Bytes>
+__device__ __forceinline__ void copy_tail(const char* row, char* to, uint32_t head, int heads, uint32_t tail, uint32_t inverse) {
+    const Bytes* const src = reinterpret_cast<const Bytes*>(row);
+    Bytes* const dst = reinterpret_cast<Bytes*>(to);
+    head /= sizeof(Bytes);
+    const uint32_t n = heads * tail;
+    for (uint32_t i0 = threadIdx.x & 31; i0 < n; i0 += 32 * kAhead) {
+        Bytes v[kAhead];
+        uint32_t at[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            // i / tail: exact, as i * tail < kTailHeads * 1022^2 < 2^32; one piece a head has no such inverse
+            const uint32_t i = i0 + 32 * k, h = tail == 1 ? i : __umulhi(i, inverse);
+            at[k] = h * head + (i - h * tail);
+            if (i < n) v[k] = src[at[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (i0 + 32 * k < n) dst[at[k]] = v[k];
+    }
+}
+
+template <typename T, int V, int A, bool INTER, bool TAIL>
 __global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
     using P = Piece<T, V, A>;
     constexpr int kPairs = INTER ? V / 2 : V;                         // pairs a unit
@@ -110,9 +140,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int half4 = (p.half + 3) & ~3;
     float2* const table = reinterpret_cast<float2*>(sh_freq + half4) + w * half4;   // this warp's cosines and sines
-    const int turned = p.half / kPairs;                               // units that turn; the rest are the tail
     const int u0 = lane % p.across, h0 = lane / p.across;
-    const bool copy_tail = p.x != p.out;
     const double inv_two_pi = 0.15915494309189535;
     for (int i = threadIdx.x; i < p.half; i += kThreads) {
         int a = 0, lo = 0;
@@ -146,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
             }
         };
         const bool lanes = h0 < p.hp;                                 // the lanes behind whole units rest
-        if (lanes && u0 < turned) load(u0, first);
+        if (lanes) load(u0, first);
         const int32_t* const pos = p.positions + static_cast<size_t>(r) * p.axes;
         __syncwarp();                                                 // the row before has been read out
         for (int i = lane; i < p.half; i += 32) {
@@ -158,15 +186,20 @@ __global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
             table[i] = make_float2(c, s);
         }
         __syncwarp();
+        if constexpr (TAIL) {
+            const uint32_t head = p.head_dim * sizeof(T);
+            for (int h = part * p.share; h < end; h += kTailHeads) {
+                const int off = h * p.head_dim + 2 * p.half, n = min(kTailHeads, end - h);
+                const char* const src = reinterpret_cast<const char*>(row + off);
+                char* const dst = reinterpret_cast<char*>(to + off);
+                if (p.tail_bytes == 16) copy_tail<uint4>(src, dst, head, n, p.tail, p.tail_inverse);
+                else if (p.tail_bytes == 8) copy_tail<uint2>(src, dst, head, n, p.tail, p.tail_inverse);
+                else if (p.tail_bytes == 4) copy_tail<uint32_t>(src, dst, head, n, p.tail, p.tail_inverse);
+                else copy_tail<uint16_t>(src, dst, head, n, p.tail, p.tail_inverse);
+            }
+        }
         if (!lanes) continue;
         for (int u = u0; u < p.units; u += p.across) {
-            if (u >= turned) {
-                if (!copy_tail) break;
-                const int at = 2 * p.half + (u - turned) * V;
-                for (int h = first; h < end; h += p.hp)
-                    *reinterpret_cast<P*>(to + h * p.head_dim + at) = *reinterpret_cast<const P*>(row + h * p.head_dim + at);
-                continue;
-            }
             float2 cs[kPairs];
 #pragma unroll
             for (int e = 0; e < kPairs; ++e) cs[e] = table[u * kPairs + e];
@@ -209,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
 template <typename T, int V, int A = V>
 cudaError_t launch(RotaryParams& p, cudaStream_t s) {
     const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
-    p.units = (inter ? 2 * p.half : p.half) / V + (p.head_dim - 2 * p.half) / V;
+    p.units = (inter ? 2 * p.half : p.half) / V;
     p.across = p.units < 32 ? p.units : 32;
     p.hp = 32 / p.across;
     // a warp a row; where that leaves SMs without work, as many a row as have kAhead loads to make
@@ -221,15 +254,10 @@ cudaError_t launch(RotaryParams& p, cudaStream_t s) {
     const long long ctas = (static_cast<long long>(p.rows) * p.split + kWarps - 1) / kWarps;
     const int grid = static_cast<int>(ctas < 148 * 3 ? ctas : 148 * 3);
     const size_t smem = static_cast<size_t>((p.half + 3) & ~3) * (sizeof(double) + kWarps * sizeof(float2));
-    cudaError_t e;
-    if constexpr (V > 1) {
-        if (inter) {
-            e = fer::host::launch_pdl(rotary<T, V, A, true>, dim3(grid), dim3(kThreads), smem, s, p);
-            return e;
-        }
-    }
-    e = fer::host::launch_pdl(rotary<T, V, A, false>, dim3(grid), dim3(kThreads), smem, s, p);
-    return e;
+    void (*kernel)(RotaryParams) = p.tail ? rotary<T, V, A, false, true> : rotary<T, V, A, false, false>;
+    if constexpr (V > 1)
+        if (inter) kernel = p.tail ? rotary<T, V, A, true, true> : rotary<T, V, A, true, false>;
+    return fer::host::launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, s, p);
 }
 
 // The widest power-of-two V elements that every address and size allows.
@@ -237,9 +265,14 @@ template <typename T>
 cudaError_t dispatch(RotaryParams& p, cudaStream_t s) {
     const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
     const uintptr_t addr = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out);
-    size_t all = addr / sizeof(T) | p.xs | p.os | static_cast<size_t>(p.head_dim) |
-                 static_cast<size_t>(inter ? 2 * p.half : p.half);
-    if (2 * p.half != p.head_dim) all |= static_cast<size_t>(2 * p.half);
+    const size_t heads = addr / sizeof(T) | p.xs | p.os | static_cast<size_t>(p.head_dim);
+    const size_t all = heads | static_cast<size_t>(inter ? 2 * p.half : p.half);
+    if (p.x != p.out && p.head_dim > 2 * p.half) {
+        const size_t tail = (heads | static_cast<size_t>(2 * p.half)) * sizeof(T);
+        p.tail_bytes = static_cast<int>(tail % 16 == 0 ? 16 : tail & (0 - tail));
+        p.tail = (p.head_dim - 2 * p.half) * static_cast<int>(sizeof(T)) / p.tail_bytes;
+        p.tail_inverse = static_cast<uint32_t>(((1ull << 32) + p.tail - 1) / p.tail);
+    }
     constexpr int kMost = 16 / sizeof(T);
     if constexpr (kMost == 8)
         if (all % 8 == 0) return launch<T, 8>(p, s);

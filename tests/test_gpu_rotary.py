@@ -55,6 +55,27 @@ def test_matches_definition(session, dtype, rows, heads, head_dim, sections, rot
         assert torch.equal(got[..., rot:], x.double().view_as(want)[..., rot:])
 
 
+@pytest.mark.parametrize("dtype,rows,heads,head_dim,rot,col", [
+    (BF16, 9, 3, 72, 64, 0), (BF16, 9, 3, 72, 64, 1), (F32, 700, 5, 68, 64, 0), (F16, 40, 32, 128, 32, 8),
+    (BF16, 3, 9000, 34, 32, 0),            # one piece a head
+    (F16, 2, 5000, 1024, 2, 0), (F16, 2, 5000, 1024, 2, 1)])
+def test_copied_tails(session, dtype, rows, heads, head_dim, rot, col):
+    """What lies behind the turned part arrives as it is, and nothing is written beside the heads."""
+    g = torch.Generator().manual_seed(heads)
+    x = torch.randn(rows, heads * head_dim + 16, generator=g).to(dtype).cuda()
+    pos = torch.randint(0, 5000, (rows,), generator=g, dtype=torch.int32)
+    out = torch.full_like(x, 7.0)
+    call(session, x, out, pos.cuda(), heads, head_dim, rotary_dim=rot, x_col=col, out_col=col)
+    part = slice(col, col + heads * head_dim)
+    got, src = out[:, part].reshape(rows, heads, head_dim), x[:, part].reshape(rows, heads, head_dim)
+    assert ref.same_bits(got[..., rot:], src[..., rot:])
+    rest = out.clone()
+    rest[:, part] = 7.0
+    assert bool((rest == 7.0).all())
+    want, far = ref.rotary(src.cpu().view(rows, -1), pos[:, None], heads, head_dim, [rot // 2], rot, 1e4, False, False, False)
+    assert bool(((got.cpu().double() - want).abs() <= bound(src.cpu().view(rows, -1), want, far, dtype, heads, head_dim)).all())
+
+
 def test_far_and_negative_positions(session):
     pos = torch.tensor([0, 1, -1, 12345, -99999, 2 ** 24 + 1, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)
     x = torch.randn(8, 64, generator=torch.Generator().manual_seed(1))
