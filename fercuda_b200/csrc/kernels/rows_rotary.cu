@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kAhead = 4;   // loads a lane makes before it turns the first
+constexpr int kTailAhead = 4;
 constexpr int kTailHeads = 4096;
 
 struct RotaryParams {
@@ -116,24 +116,25 @@ __device__ __forceinline__ void copy_tail(const char* row, char* to, uint32_t he
     Bytes* const dst = reinterpret_cast<Bytes*>(to);
     head /= sizeof(Bytes);
     const uint32_t n = heads * tail;
-    for (uint32_t i0 = threadIdx.x & 31; i0 < n; i0 += 32 * kAhead) {
-        Bytes v[kAhead];
-        uint32_t at[kAhead];
+    for (uint32_t i0 = threadIdx.x & 31; i0 < n; i0 += 32 * kTailAhead) {
+        Bytes v[kTailAhead];
+        uint32_t at[kTailAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
+        for (int k = 0; k < kTailAhead; ++k) {
             // i / tail: exact, as i * tail < kTailHeads * 1022^2 < 2^32; one piece a head has no such inverse
             const uint32_t i = i0 + 32 * k, h = tail == 1 ? i : __umulhi(i, inverse);
             at[k] = h * head + (i - h * tail);
             if (i < n) v[k] = src[at[k]];
         }
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
+        for (int k = 0; k < kTailAhead; ++k)
             if (i0 + 32 * k < n) dst[at[k]] = v[k];
     }
 }
 
-template <typename T, int V, int A, bool INTER, bool TAIL>
-__global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
+// kAhead: loads a lane makes before it turns the first
+template <typename T, int V, int A, bool INTER, bool TAIL, int kAhead>
+__global__ void __launch_bounds__(kThreads, kAhead < 4 ? 4 : 3) rotary(const RotaryParams p) {
     using P = Piece<T, V, A>;
     constexpr int kPairs = INTER ? V / 2 : V;                         // pairs a unit
     extern __shared__ __align__(16) double sh_freq[];                 // [half] turns a position
@@ -239,25 +240,33 @@ __global__ void __launch_bounds__(kThreads, 3) rotary(const RotaryParams p) {
     }
 }
 
-template <typename T, int V, int A = V>
-cudaError_t launch(RotaryParams& p, cudaStream_t s) {
-    const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
-    p.units = (inter ? 2 * p.half : p.half) / V;
-    p.across = p.units < 32 ? p.units : 32;
-    p.hp = 32 / p.across;
+template <typename T, int V, int A, int kAhead>
+cudaError_t launch_ahead(RotaryParams& p, int turns, cudaStream_t s) {
     // a warp a row; where that leaves SMs without work, as many a row as have kAhead loads to make
-    const int turns = (p.heads + p.hp - 1) / p.hp;
+    constexpr int kCtas = kAhead < 4 ? 4 : 3;
     int split = p.rows < 148 * 2 * kWarps ? (148 * 2 * kWarps - 1) / p.rows + 1 : 1;
     if (split > (turns + kAhead - 1) / kAhead) split = (turns + kAhead - 1) / kAhead;
     p.share = ((turns + split - 1) / split) * p.hp;
     p.split = (p.heads + p.share - 1) / p.share;
     const long long ctas = (static_cast<long long>(p.rows) * p.split + kWarps - 1) / kWarps;
-    const int grid = static_cast<int>(ctas < 148 * 3 ? ctas : 148 * 3);
+    const int grid = static_cast<int>(ctas < 148 * kCtas ? ctas : 148 * kCtas);
     const size_t smem = static_cast<size_t>((p.half + 3) & ~3) * (sizeof(double) + kWarps * sizeof(float2));
-    void (*kernel)(RotaryParams) = p.tail ? rotary<T, V, A, false, true> : rotary<T, V, A, false, false>;
+    void (*kernel)(RotaryParams) = p.tail ? rotary<T, V, A, false, true, kAhead> : rotary<T, V, A, false, false, kAhead>;
     if constexpr (V > 1)
-        if (inter) kernel = p.tail ? rotary<T, V, A, true, true> : rotary<T, V, A, true, false>;
+        if (p.flags & FER_ROTARY_FLAG_INTERLEAVED)
+            kernel = p.tail ? rotary<T, V, A, true, true, kAhead> : rotary<T, V, A, true, false, kAhead>;
     return fer::host::launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, s, p);
+}
+
+template <typename T, int V, int A = V>
+cudaError_t launch(RotaryParams& p, cudaStream_t s) {
+    p.units = (p.flags & FER_ROTARY_FLAG_INTERLEAVED ? 2 * p.half : p.half) / V;
+    p.across = p.units < 32 ? p.units : 32;
+    p.hp = 32 / p.across;
+    // rows that give a lane two loads at most: more warps instead of more loads (32768 rows of 8 heads x 128: 36.9
+    // us with four loads and three CTAs an SM, 32.8 so)
+    const int turns = (p.heads + p.hp - 1) / p.hp;
+    return turns <= 2 ? launch_ahead<T, V, A, 2>(p, turns, s) : launch_ahead<T, V, A, 4>(p, turns, s);
 }
 
 // The widest power-of-two V elements that every address and size allows.
