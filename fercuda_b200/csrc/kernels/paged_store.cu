@@ -9,7 +9,8 @@
 // warps where rows are few) and walks its 16-byte pieces, kAhead of keys and
 // of values in flight a lane: reads are contiguous along a row and writes
 // along a head's row in its page. Weights and positions are walked with the
-// row innermost: consecutive slots of a head are consecutive.
+// row innermost: consecutive slots of a head are consecutive. Short rows are
+// walked as one run of pieces by the whole CTA.
 //
 // Lengths: a CTA of a step (one row a sequence) is the only reader of its
 // sequences' lengths and writes the new ones itself, in place or not. With
@@ -30,14 +31,16 @@ namespace {
 using fer::dev::Paged;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxRows = 16;   // rows a CTA at most
+constexpr int kMaxRows = 128;  // rows a CTA at most
 constexpr int kAhead = 4;
+constexpr int kShort = 32 * kAhead;   // pieces of a row below which a CTA's rows are walked as one
 
 struct StoreParams {
     const uint16_t* k_rows;
     const uint16_t* v_rows;
     size_t ks, vs;
     int rows, n_seq, run;      // run: rows a CTA
+    uint32_t inverse;          // ceil(2^32 / pieces of a row), for short ones
     const int32_t* offsets;
     int32_t* new_lengths;
     float* weights;
@@ -113,27 +116,56 @@ __global__ void __launch_bounds__(kThreads) store_rows(const Paged c, const Stor
     // head_dim is a power of two: piece q of a row is piece q % pieces of head q / pieces
     const int pieces = c.head_dim / kPer, log = 31 - __clz(pieces), per_row = c.kv_heads << log;
     const int lane = t & 31, w = t >> 5, share = max(1, kWarps / p.run);   // warps a row
-    for (int j = w / share; j < nr; j += max(1, kWarps / share)) {
-        if (s_page[j] < 0) continue;
-        const Piece* const kr = reinterpret_cast<const Piece*>(p.k_rows + (r0 + static_cast<size_t>(j)) * p.ks);
-        const Piece* const vr = reinterpret_cast<const Piece*>(p.v_rows + (r0 + static_cast<size_t>(j)) * p.vs);
-        const size_t to = c.row(s_page[j], 0, s_slot[j]) / kPer, head = static_cast<size_t>(pieces) << c.shift;
-        Piece* const kp = static_cast<Piece*>(c.k) + to;
-        Piece* const vp = static_cast<Piece*>(c.v) + to;
-        for (int q0 = (w % share) * 32 + lane; q0 < per_row; q0 += 32 * share * kAhead) {
+    if (per_row < kShort) {
+        // i / per_row: exact, as i * per_row < kMaxRows * kShort^2 < 2^32; one piece a row does not occur
+        const size_t head = static_cast<size_t>(pieces) << c.shift;
+        for (int i0 = t; i0 < nr * per_row; i0 += kThreads * kAhead) {
             Piece kk[kAhead], vv[kAhead];
+            int j[kAhead], q[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const int q = q0 + 32 * share * k;
-                if (q < per_row) kk[k] = kr[q], vv[k] = vr[q];
+                const int i = i0 + kThreads * k;
+                j[k] = static_cast<int>(__umulhi(static_cast<uint32_t>(i), p.inverse));
+                q[k] = i - j[k] * per_row;
+                if (i >= nr * per_row || s_page[j[k]] < 0) {
+                    j[k] = -1;
+                    continue;
+                }
+                const size_t r = r0 + static_cast<size_t>(j[k]);
+                kk[k] = reinterpret_cast<const Piece*>(p.k_rows + r * p.ks)[q[k]];
+                vv[k] = reinterpret_cast<const Piece*>(p.v_rows + r * p.vs)[q[k]];
             }
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const int q = q0 + 32 * share * k;
-                if (q >= per_row) break;
-                const size_t at = (q >> log) * head + (q & (pieces - 1));
-                kp[at] = kk[k];
-                vp[at] = vv[k];
+                if (j[k] < 0) continue;
+                const size_t at = c.row(s_page[j[k]], 0, s_slot[j[k]]) / kPer + (q[k] >> log) * head + (q[k] & (pieces - 1));
+                static_cast<Piece*>(c.k)[at] = kk[k];
+                static_cast<Piece*>(c.v)[at] = vv[k];
+            }
+        }
+    } else {
+        for (int j = w / share; j < nr; j += max(1, kWarps / share)) {
+            if (s_page[j] < 0) continue;
+            const Piece* const kr = reinterpret_cast<const Piece*>(p.k_rows + (r0 + static_cast<size_t>(j)) * p.ks);
+            const Piece* const vr = reinterpret_cast<const Piece*>(p.v_rows + (r0 + static_cast<size_t>(j)) * p.vs);
+            const size_t to = c.row(s_page[j], 0, s_slot[j]) / kPer, head = static_cast<size_t>(pieces) << c.shift;
+            Piece* const kp = static_cast<Piece*>(c.k) + to;
+            Piece* const vp = static_cast<Piece*>(c.v) + to;
+            for (int q0 = (w % share) * 32 + lane; q0 < per_row; q0 += 32 * share * kAhead) {
+                Piece kk[kAhead], vv[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int q = q0 + 32 * share * k;
+                    if (q < per_row) kk[k] = kr[q], vv[k] = vr[q];
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const int q = q0 + 32 * share * k;
+                    if (q >= per_row) break;
+                    const size_t at = (q >> log) * head + (q & (pieces - 1));
+                    kp[at] = kk[k];
+                    vp[at] = vv[k];
+                }
             }
         }
     }
@@ -196,15 +228,19 @@ extern "C" cudaError_t fer_paged_store(const fer_paged_view_t* cache, const fer_
     p.seen = a->seen;
     p.new_seen = a->positions || a->seen ? a->new_seen : nullptr;
     p.err = err;
-    // kMaxRows rows a CTA, fewer (and more warps a row) where that would leave SMs without work
-    p.run = kMaxRows;
+    const bool wide = rows_at % 16 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0;
+    const size_t per_row = wide ? width / 8 : width;
+    p.inverse = static_cast<uint32_t>(((1ull << 32) + per_row - 1) / per_row);
+    // 16 rows a CTA, more of short ones (of 8 pieces: 69.6 us for 131072 rows with 16, 20.5 with 128); fewer (and more
+    // warps a row) where that would leave SMs without work
+    p.run = 16;
+    while (p.run < kMaxRows && p.run * per_row < 1024) p.run *= 2;
     while (p.run > 1 && a->rows < 148 * 2 * p.run) p.run /= 2;
     const bool in_place = a->new_lengths == cache->lengths || (p.new_seen && p.new_seen == a->seen);
     const bool later = a->offsets && in_place;
     cudaError_t e = cudaSuccess;
     if (a->rows > 0 || !later) {
         const int grid = a->rows > 0 ? (a->rows - 1) / p.run + 1 : 1;
-        const bool wide = rows_at % 16 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0;
         e = wide ? fer::host::launch_pdl(store_rows<uint4>, dim3(grid), dim3(kThreads), 0, s, c, p, !later)
                  : fer::host::launch_pdl(store_rows<uint16_t>, dim3(grid), dim3(kThreads), 0, s, c, p, !later);
         if (e != cudaSuccess) return e;
