@@ -59,6 +59,8 @@ using fer::dev::Paged;
 constexpr int kWarps = 4;                        // that compute; one more loads
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kRound = 16 * kWarps;  // slots a round
+constexpr int kTiles = 148 * 16;     // CTAs that add weights, at least where there are that many tiles
+constexpr int kManyHeads = 148 * 4;  // heads whose joining fills the GPU with a CTA each
 constexpr int kSegments = 128;       // entries of the unit table in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -782,50 +784,54 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
         if (d0 + t == 0 && p.lse) p.lse[bh] = sum == 0.0f ? -INFINITY : (base + log2f(sum)) * kLn2;
         return;
     }
-    const int j0 = (blockIdx.x - p.group * kBands) * 4 * kFinish;
-    if (j0 >= len) return;
-    const int j = j0 + 4 * t;
     const size_t most = static_cast<size_t>(c.max_slots());   // a multiple of 8: rows start at 16 bytes
-    const bool on = j < len, whole = j + 3 < len && reinterpret_cast<uintptr_t>(p.weights) % 16 == 0;
-    const float* const scores = p.scores + bh0 * most + j;
-    float* const out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most + j;
-    float4 s[kHeads], old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (whole) old = *reinterpret_cast<const float4*>(out);
+    const int step = (gridDim.x - p.group * kBands) * 4 * kFinish;
+    for (int j0 = (blockIdx.x - p.group * kBands) * 4 * kFinish; j0 < len; j0 += step) {
+        const int j = j0 + 4 * t;
+        const bool on = j < len, whole = j + 3 < len && reinterpret_cast<uintptr_t>(p.weights) % 16 == 0;
+        const float* const scores = p.scores + bh0 * most + j;
+        float* const out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most + j;
+        float4 s[kHeads], old = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (whole) old = *reinterpret_cast<const float4*>(out);
 #pragma unroll
-    for (int k = 0; k < kHeads; ++k)
-        if (on && k < p.group) s[k] = *reinterpret_cast<const float4*>(scores + k * most);
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g0 = 0; g0 < p.group; g0 += kFinish) {
-        const int ng = min(kFinish, p.group - g0);
-        __syncthreads();
-        for (int g = t >> 5; g < ng; g += kFinish / 32) {
-            const float v = chunks_lse2<kBatch>(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks);
-            if (lane == 0) s_lse[g] = v;
-        }
-        __syncthreads();
-        if (!on) continue;
-        for (int g = 0; g < ng; g += kHeads) {
+        for (int k = 0; k < kHeads; ++k)
+            if (on && k < p.group) s[k] = *reinterpret_cast<const float4*>(scores + k * most);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int g0 = 0; g0 < p.group; g0 += kFinish) {
+            const int ng = min(kFinish, p.group - g0);
+            if (p.group > kFinish || j0 < step) {   // else the totals are there from the first tile
+                __syncthreads();
+                for (int g = w; g < ng; g += kW) {
+                    const float v = chunks_lse2<kBatch>(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks);
+                    if (lane == 0) s_lse[g] = v;
+                }
+                __syncthreads();
+            }
+            if (!on) continue;
+            for (int g = 0; g < ng; g += kHeads) {
 #pragma unroll
-            for (int k = 0; k < kHeads; ++k)
-                if ((g0 > 0 || g > 0) && g + k < ng) s[k] = *reinterpret_cast<const float4*>(scores + (g0 + g + k) * most);
+                for (int k = 0; k < kHeads; ++k)
+                    if ((g0 > 0 || g > 0) && g + k < ng)
+                        s[k] = *reinterpret_cast<const float4*>(scores + (g0 + g + k) * most);
 #pragma unroll
-            for (int k = 0; k < kHeads; ++k) {
-                if (g + k >= ng) break;
-                const float lse2 = s_lse[g + k];
-                if (lse2 == -INFINITY) continue;
-                sum[0] += ex2(s[k].x - lse2);
-                sum[1] += ex2(s[k].y - lse2);
-                sum[2] += ex2(s[k].z - lse2);
-                sum[3] += ex2(s[k].w - lse2);
+                for (int k = 0; k < kHeads; ++k) {
+                    if (g + k >= ng) break;
+                    const float lse2 = s_lse[g + k];
+                    if (lse2 == -INFINITY) continue;
+                    sum[0] += ex2(s[k].x - lse2);
+                    sum[1] += ex2(s[k].y - lse2);
+                    sum[2] += ex2(s[k].z - lse2);
+                    sum[3] += ex2(s[k].w - lse2);
+                }
             }
         }
-    }
-    if (whole) {
-        *reinterpret_cast<float4*>(out) = make_float4(old.x + sum[0], old.y + sum[1], old.z + sum[2], old.w + sum[3]);
-    } else {
+        if (whole) {
+            *reinterpret_cast<float4*>(out) = make_float4(old.x + sum[0], old.y + sum[1], old.z + sum[2], old.w + sum[3]);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (j + e < len) out[e] += sum[e];
+            for (int e = 0; e < 4; ++e)
+                if (j + e < len) out[e] += sum[e];
+        }
     }
 }
 
@@ -859,7 +865,11 @@ bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int r
 
 template <typename T, int D, int THREADS, int DIMS>
 cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
-    const int tiles = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0;
+    // as many tiles a (key head, sequence) as there are, within kTiles CTAs: a wide table has mostly empty ones
+    // (those 64 x 32 heads with weights: 66 us in all with every tile its CTA, 36 so)
+    const long long pairs = static_cast<long long>(c.kv_heads) * p.n_seq;
+    const int all = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0, least = static_cast<int>(kTiles / pairs) + 1;
+    const int tiles = all < least ? all : least;
     return fer::host::launch_pdl(attn_finish<T, D, THREADS, DIMS>, dim3(p.group * (D / DIMS) + tiles, c.kv_heads, p.n_seq),
                                  dim3(THREADS), 0, s, c, p);
 }
@@ -879,9 +889,10 @@ cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
     cudaError_t e = fer::host::launch_pdl(attn_units<T, D, NT>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
                                           dim3(kThreads), smem, s, c, p, k_map, v_map);
     if (e == cudaSuccess && (p.weights || p.chunks > 1))
-        // few chunks: a head a CTA; many: sixteen warps for 32 dims, whose loads one SM could not have in flight
-        // (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA)
-        e = p.chunks <= 32 ? finish<T, D, 256, D>(c, p, s) : finish<T, D, 512, 32>(c, p, s);
+        // few chunks or many heads: a head a CTA; else sixteen warps for 32 dims, whose loads one SM could not have
+        // in flight (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA; 64 x 32
+        // heads of up to 512 slots in a table of 32768: 52 us in all so, 32 with a head a CTA)
+        e = p.chunks <= 32 || static_cast<long long>(p.n_seq) * p.heads >= kManyHeads ? finish<T, D, 256, D>(c, p, s) : finish<T, D, 512, 32>(c, p, s);
     return e;
 }
 

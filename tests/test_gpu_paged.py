@@ -184,6 +184,22 @@ def test_attention_of_large_ragged_batches(session, dtype, D, H, group, page, B,
     assert ref.same_bits(o1, out[b:b + 1]) and ref.same_bits(l1, lse[b:b + 1])
 
 
+def test_attention_of_short_sequences_in_a_wide_table(session):
+    lens = torch.randint(0, 300, (100,), generator=torch.Generator().manual_seed(3)).tolist()
+    lens[7], lens[50] = 12001, 1025
+    c = ref.Cache(lens, 4, 64, 64, BF16, max_pages=256)
+    q = queries(c, 8)
+    w = torch.zeros(100, 4, c.slots, device="cuda")
+    out, lse = attend(session, c, q, 8, weights=w)
+    host = copy.copy(c)
+    host.k, host.v, host.table = c.k.cpu(), c.v.cpu(), c.table.cpu()
+    sums = check(host, q, 8, out, lse)
+    now = w.cpu().double()
+    for (b, h), (want, rel) in sums.items():
+        assert bool(((now[b, h, :lens[b]] - want).abs() <= want * (rel + 2.0 ** -23) + 2.0 ** -140).all())
+        assert not now[b, h, lens[b]:].any()
+
+
 def test_attention_of_a_large_batch_that_holds_nothing(session):
     c = ref.Cache([0] * 700, 2, 64, 16, BF16, max_pages=40)
     out, lse = attend(session, c, queries(c, 4), 4)
@@ -408,27 +424,29 @@ def test_store(session, dtype, D, H, page, lens, offsets, tail, cols, in_place):
         assert torch.equal(c.lengths, old_len) and torch.equal(seen, old_seen)
 
 
-@pytest.mark.parametrize("n_seq,ragged", [(400, True), (5000, False)])
+@pytest.mark.parametrize("n_seq,ragged,H,col", [(400, True, 2, 0), (5000, False, 2, 0), (400, True, 1, 0),
+                                                (400, True, 1, 3), (3000, False, 3, 8)])
 @pytest.mark.parametrize("in_place", [False, True])
-def test_store_of_many_rows(session, n_seq, ragged, in_place):
+def test_store_of_many_rows(session, n_seq, ragged, H, col, in_place):
     """More rows than a CTA takes, and runs of sequences that get none."""
     g = torch.Generator().manual_seed(n_seq)
     new = torch.randint(0, 30, (n_seq,), generator=g) * (torch.rand(n_seq, generator=g) < 0.8) if ragged else None
     offsets = [3] + (3 + new.cumsum(0)).tolist() if ragged else None
     lens = torch.randint(0, 34, (n_seq,), generator=g).tolist()
-    c = ref.Cache(lens, 2, 64, 16, BF16, max_pages=4)
+    c = ref.Cache(lens, H, 64, 16, BF16, max_pages=4)
     grow_table(c)
     n = offsets[-1] + 5 if ragged else n_seq
-    rows = torch.randn(n, 256, generator=g).to(BF16).cuda()
-    w = torch.full((n_seq, 2, c.slots), 5.0, device="cuda")
-    p = torch.full((n_seq, 2, c.slots), -5, dtype=torch.int32, device="cuda")
+    cols = (col, col + 64 * H)
+    rows = torch.randn(n, 128 * H + 8, generator=g).to(BF16).cuda()
+    w = torch.full((n_seq, H, c.slots), 5.0, device="cuda")
+    p = torch.full((n_seq, H, c.slots), -5, dtype=torch.int32, device="cuda")
     seen = c.lengths + 9
-    want = expect_store(c, rows, 0, 128, offsets, n_seq, w, p, seen)
+    want = expect_store(c, rows, *cols, offsets, n_seq, w, p, seen)
     new_len, new_seen = (c.lengths, seen) if in_place else (c.lengths.clone(), seen.clone())
     with ref.Buffers(session) as B:
         r = B(rows)
         ids, bseen = c.ids(B), B(seen)
-        session.paged_store(ids, r, r, v_col=128, offsets=B(i32(offsets)) if ragged else 0,
+        session.paged_store(ids, r, r, k_col=cols[0], v_col=cols[1], offsets=B(i32(offsets)) if ragged else 0,
                             new_lengths=0 if in_place else B(new_len), weights=B(w), positions=B(p), seen=bseen,
                             new_seen=0 if in_place else B(new_seen))
     assert session.device_errors() == 0
