@@ -519,13 +519,6 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
             const bool good = s_good[stage];
             const uint32_t st = ring + stage * C::kStage;
             const int rows = x.n - r0;           // held slots of the round, or more
-            if (rows < 16 * w + 16) {            // values behind the last slot count as zero, whatever is there
-                uint4* v = reinterpret_cast<uint4*>(smem + stage * C::kStage + C::kHalf);
-                const int from = max(rows, 16 * w), n = 8 * (16 * w + 16 - from);
-                for (int i = lane; i < D / 64 * n; i += 32)
-                    v[i / n * (C::kBand / 16) + 8 * from + i % n] = make_uint4(0u, 0u, 0u, 0u);
-                fer::dev::fence_proxy_async_smem();
-            }
             float s[NT][4];
             {
                 float s2[NT][4];
@@ -601,6 +594,13 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
                 s_p[w][nt][lane] = f;
             }
             meet_warps();
+            // the low parts' products in a sum of their own: chains of dependent products half as long
+            constexpr bool kTwo = NT == 1;
+            float low[NT][kMine][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < kMine; ++k) low[nt][k][0] = low[nt][k][1] = low[nt][k][2] = low[nt][k][3] = 0.0f;
 #pragma unroll
             for (int v = 0; v < kWarps; ++v) {
                 if (16 * v >= rows) break;
@@ -608,16 +608,30 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) f[nt] = s_p[v][nt][lane];
                 const int r = 16 * v + (lane & 7) + ((lane >> 4) << 3);
+                const int left = rows - 16 * v - 2 * (lane & 3);   // a lane has slots 0, 1, 8 and 9 from there
 #pragma unroll
                 for (int k = 0; k < kMine; ++k) {
                     uint32_t a[4];
                     ldsm4_t(a, st + C::kHalf + C::at(r, 2 * (w * kMine + k) + ((lane >> 3) & 1)));
+                    if (16 * v + 16 > rows) {   // values behind the last slot count as zero, whatever is there
+                        const uint32_t m0 = left > 1 ? ~0u : left > 0 ? 0xffffu : 0u;
+                        const uint32_t m1 = left > 9 ? ~0u : left > 8 ? 0xffffu : 0u;
+                        a[0] &= m0, a[1] &= m0, a[2] &= m1, a[3] &= m1;
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma<T>(o[nt][k], a, f[nt].z, f[nt].w);
+                        mma<T>(kTwo ? low[nt][k] : o[nt][k], a, f[nt].z, f[nt].w);
                         mma<T>(o[nt][k], a, f[nt].x, f[nt].y);
                     }
                 }
+            }
+            if constexpr (kTwo) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < kMine; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[nt][k][e] += low[nt][k][e];
             }
             __syncwarp();
             if (lane == 0) fer::dev::mbar_arrive(&s_empty[stage]);
