@@ -799,9 +799,9 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
         return;
     }
     const size_t most = static_cast<size_t>(c.max_slots());   // a multiple of 8: rows start at 16 bytes
-    const int step = (gridDim.x - p.group * kBands) * 4 * kFinish;
-    for (int j0 = (blockIdx.x - p.group * kBands) * 4 * kFinish; j0 < len; j0 += step) {
-        const int j = j0 + 4 * t;
+    const uint32_t step = (gridDim.x - p.group * kBands) * 4 * kFinish;   // j0 may pass 31 bits at the end
+    for (uint32_t j0 = (blockIdx.x - p.group * kBands) * 4 * kFinish; j0 < static_cast<uint32_t>(len); j0 += step) {
+        const int j = static_cast<int>(j0) + 4 * t;
         const bool on = j < len, whole = j + 3 < len && reinterpret_cast<uintptr_t>(p.weights) % 16 == 0;
         const float* const scores = p.scores + bh0 * most + j;
         float* const out = p.weights + (static_cast<size_t>(b) * c.kv_heads + hk) * most + j;

@@ -813,6 +813,34 @@ def test_captured_steps(session):
     assert int(err) == 0
 
 
+@pytest.mark.parametrize("lens,H,budget", [([5000, 3000, 20], 2, 1000), ([1500] * 160, 2, 700)])
+def test_captured_long_eviction(lens, H, budget):
+    """Selection in clusters, and with the moves in the same kernel, replayed from a graph in place."""
+    lib = capi.kernels()
+    c = ref.Cache(lens, H, 64, 64, BF16)
+    B, err = len(lens), torch.zeros(1, dtype=torch.int32, device="cuda")
+    w = weights_for("spread", B, H, c.slots).cuda()
+    p = torch.arange(c.slots, dtype=torch.int32, device="cuda").repeat(B, H, 1)
+    seen = c.lengths.clone()
+    size = lib.fer_paged_evict_workspace_bytes(B, H, c.slots, budget)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    v = views(c)
+    a = capi.fer_paged_evict_args_t(budget, 50, w.data_ptr(), p.data_ptr(), seen.data_ptr(), c.lengths.data_ptr(),
+                                    w.data_ptr(), p.data_ptr(), ws.data_ptr(), size)
+    state = (c.k, c.v, w, p, c.lengths)
+    before = [x.clone() for x in state]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert lib.fer_paged_evict(C.byref(v), C.byref(a), err.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    for _ in range(2):
+        for x, old in zip(state, before):
+            x.copy_(old)
+        graph.replay()
+        torch.cuda.synchronize()
+        check_evict(c, budget, 50, before[2], before[3], seen, [before[0].cpu(), before[1].cpu(), *before[2:4]], state)
+    assert int(err) == 0
+
+
 FIRST_USE = """
 import ctypes as C, sys
 sys.path.insert(0, {root!r})
