@@ -32,10 +32,10 @@
 // rounding it once would have added half of the output's own rounding error.
 //
 // Measured (HBM copy 6538 GB/s): 131071 slots x 8 key heads of 128 for 64
-// heads 93.8 us, 5.7 TB/s; 33 sequences of 0 to 8192 slots with weights 114.5
+// heads 92.5 us, 5.8 TB/s; 33 sequences of 0 to 8192 slots with weights 115
 // us (86 us at the copy rate); 64 sequences of 1 to 1024 slots x 16 heads of 64
-// 35.8 us (20.6): 3.5 us pass until the first rows arrive, CTAs end between 19
-// and 31 us as they have a unit more or less, and 5 us go to the joining.
+// 33.2 us (20.6): 3.5 us pass until the first rows arrive, CTAs end between 18
+// and 29 us as they have a unit more or less, and 5 us go to the joining.
 //
 // Scores are kept in base-2 units (scale * log2 e folded into one factor).
 // When weights are wanted they go to the workspace as well, and the second
