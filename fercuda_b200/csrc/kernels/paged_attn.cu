@@ -733,7 +733,9 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks) {
 template <typename T, int D, int kFinish, int DIMS>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
     constexpr int kW = kFinish / 32, kV = DIMS / 32, kBands = D / DIMS, kHeads = 4;
-    constexpr int kAhead = kV == 1 ? 16 : kV <= 4 ? 4 : 2, kBatch = DIMS == D ? 1 : 8;
+    // Chunks that share a maximum, and batches of lse's loads: functions of D and kFinish, so not of the batch.
+    constexpr int kStep = D <= 128 ? 4 : 2, kBatch = kFinish > 256 ? 8 : 1;
+    constexpr int kAhead = kV == 1 ? 16 : kStep;   // chunks in flight
     __shared__ __align__(16) float s_o[kW][DIMS];
     __shared__ float2 s_ml[kW];
     __shared__ float s_lse[kFinish];
@@ -763,21 +765,24 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
                 v[k] = Dims{};
                 if (i < chunks) x[k] = ml[i], v[k] = *reinterpret_cast<const Dims*>(po + static_cast<size_t>(i) * D);
             }
-            float next = top;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) next = fmaxf(next, x[k].x);
-            const float base = next == -INFINITY ? 0.0f : next, f = ex2(top - base);
-            l *= f;
+            for (int k0 = 0; k0 < kAhead; k0 += kStep) {
+                float next = top;
 #pragma unroll
-            for (int e = 0; e < kV; ++e) o.e[e] *= f;
+                for (int k = k0; k < k0 + kStep; ++k) next = fmaxf(next, x[k].x);
+                const float base = next == -INFINITY ? 0.0f : next, f = ex2(top - base);
+                l *= f;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const float y = ex2(x[k].x - base);
-                l = fmaf(x[k].y, y, l);
+                for (int e = 0; e < kV; ++e) o.e[e] *= f;
 #pragma unroll
-                for (int e = 0; e < kV; ++e) o.e[e] = fmaf(v[k].e[e], y, o.e[e]);
+                for (int k = k0; k < k0 + kStep; ++k) {
+                    const float y = ex2(x[k].x - base);
+                    l = fmaf(x[k].y, y, l);
+#pragma unroll
+                    for (int e = 0; e < kV; ++e) o.e[e] = fmaf(v[k].e[e], y, o.e[e]);
+                }
+                top = next;
             }
-            top = next;
         }
         *reinterpret_cast<Dims*>(&s_o[w][kV * lane]) = o;
         if (lane == 0) s_ml[w] = make_float2(top, l);
@@ -902,11 +907,15 @@ cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
     p.direct = most <= ctas;
     cudaError_t e = fer::host::launch_pdl(attn_units<T, D, NT>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
                                           dim3(kThreads), smem, s, c, p, k_map, v_map);
-    if (e == cudaSuccess && (p.weights || p.chunks > 1))
+    if (e == cudaSuccess && (p.weights || p.chunks > 1)) {
         // few chunks or many heads: a head a CTA; else sixteen warps for 32 dims, whose loads one SM could not have
         // in flight (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA; 64 x 32
         // heads of up to 512 slots in a table of 32768: 52 us in all so, 32 with a head a CTA)
-        e = p.chunks <= 32 || static_cast<long long>(p.n_seq) * p.heads >= kManyHeads ? finish<T, D, 256, D>(c, p, s) : finish<T, D, 512, 32>(c, p, s);
+        // Which warp takes which chunk, and with it every rounding, is a function of the table's width.
+        if (p.chunks <= 32) e = finish<T, D, 256, D>(c, p, s);
+        else if (static_cast<long long>(p.n_seq) * p.heads >= kManyHeads) e = finish<T, D, 512, D>(c, p, s);
+        else e = finish<T, D, 512, 32>(c, p, s);
+    }
     return e;
 }
 

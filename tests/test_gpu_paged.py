@@ -184,10 +184,11 @@ def test_attention_of_large_ragged_batches(session, dtype, D, H, group, page, B,
     assert ref.same_bits(o1, out[b:b + 1]) and ref.same_bits(l1, lse[b:b + 1])
 
 
-def test_attention_of_short_sequences_in_a_wide_table(session):
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_of_short_sequences_in_a_wide_table(session, D):
     lens = torch.randint(0, 300, (100,), generator=torch.Generator().manual_seed(3)).tolist()
     lens[7], lens[50] = 12001, 1025
-    c = ref.Cache(lens, 4, 64, 64, BF16, max_pages=256)
+    c = ref.Cache(lens, 4, D, 64, BF16, max_pages=256)
     q = queries(c, 8)
     w = torch.zeros(100, 4, c.slots, device="cuda")
     out, lse = attend(session, c, q, 8, weights=w)
@@ -198,6 +199,12 @@ def test_attention_of_short_sequences_in_a_wide_table(session):
     for (b, h), (want, rel) in sums.items():
         assert bool(((now[b, h, :lens[b]] - want).abs() <= want * (rel + 2.0 ** -23) + 2.0 ** -140).all())
         assert not now[b, h, lens[b]:].any()
+    for b in (7, 50, 51):                                  # alone in the same table: the same bits
+        one = copy.copy(c)
+        one.lens, one.table, one.lengths = lens[b:b + 1], c.table[b:b + 1].clone(), c.lengths[b:b + 1].clone()
+        w1 = torch.zeros(1, 4, c.slots, device="cuda")
+        o1, l1 = attend(session, one, q[b:b + 1].clone(), 8, weights=w1)
+        assert ref.same_bits(o1, out[b:b + 1]) and ref.same_bits(l1, lse[b:b + 1]) and ref.same_bits(w1, w[b:b + 1])
 
 
 def test_attention_of_a_large_batch_that_holds_nothing(session):
