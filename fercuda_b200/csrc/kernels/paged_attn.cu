@@ -726,15 +726,16 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks) {
 
 // grid (group * D / DIMS + weight tiles, kv_heads, n_seq). The first CTAs of a
 // (key head, sequence) add one head's chunks for DIMS dims each: a warp takes
-// every kW-th chunk in order, DIMS / 32 dims a lane, and the warps' sums,
-// each of a maximum of its own, are added in order. The others add
+// every kW-th chunk in order, DIMS / 32 dims a lane (and again for the next
+// start, where the CTA has fewer warps), and these kW sums, each of a maximum
+// of its own, are added in order. The others add
 // probabilities to the weights of four slots a thread, with what does not
 // depend on the total in flight before they wait for it.
-template <typename T, int D, int kFinish, int DIMS>
+template <typename T, int D, int kFinish, int DIMS, int kW>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
-    constexpr int kW = kFinish / 32, kV = DIMS / 32, kBands = D / DIMS, kHeads = 4;
-    // Chunks that share a maximum, and batches of lse's loads: functions of D and kFinish, so not of the batch.
-    constexpr int kStep = D <= 128 ? 4 : 2, kBatch = kFinish > 256 ? 8 : 1;
+    constexpr int kWarpsIn = kFinish / 32, kV = DIMS / 32, kBands = D / DIMS, kHeads = 4;
+    // Chunks that share a maximum, and batches of lse's loads: functions of D and kW, so not of the batch.
+    constexpr int kStep = D <= 128 ? 4 : 2, kBatch = kW > 8 ? 8 : 1;
     constexpr int kAhead = kV == 1 ? 16 : kStep;   // chunks in flight
     __shared__ __align__(16) float s_o[kW][DIMS];
     __shared__ float2 s_ml[kW];
@@ -753,39 +754,41 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
         const float2* const ml = reinterpret_cast<const float2*>(p.part_ml) + bh * p.chunks;
         struct alignas(4 * (kV < 4 ? kV : 4)) Dims { float e[kV]; };
         const float* const po = p.part_o + bh * p.chunks * D + d0 + kV * lane;
-        float top = -INFINITY, l = 0.0f;
-        Dims o{};
-        for (int i0 = w; i0 < chunks; i0 += kW * kAhead) {
-            Dims v[kAhead];
-            float2 x[kAhead];
+        for (int part = w; part < kW; part += kWarpsIn) {
+            float top = -INFINITY, l = 0.0f;
+            Dims o{};
+            for (int i0 = part; i0 < chunks; i0 += kW * kAhead) {
+                Dims v[kAhead];
+                float2 x[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const int i = i0 + k * kW;
-                x[k] = make_float2(-INFINITY, 0.0f);
-                v[k] = Dims{};
-                if (i < chunks) x[k] = ml[i], v[k] = *reinterpret_cast<const Dims*>(po + static_cast<size_t>(i) * D);
-            }
-#pragma unroll
-            for (int k0 = 0; k0 < kAhead; k0 += kStep) {
-                float next = top;
-#pragma unroll
-                for (int k = k0; k < k0 + kStep; ++k) next = fmaxf(next, x[k].x);
-                const float base = next == -INFINITY ? 0.0f : next, f = ex2(top - base);
-                l *= f;
-#pragma unroll
-                for (int e = 0; e < kV; ++e) o.e[e] *= f;
-#pragma unroll
-                for (int k = k0; k < k0 + kStep; ++k) {
-                    const float y = ex2(x[k].x - base);
-                    l = fmaf(x[k].y, y, l);
-#pragma unroll
-                    for (int e = 0; e < kV; ++e) o.e[e] = fmaf(v[k].e[e], y, o.e[e]);
+                for (int k = 0; k < kAhead; ++k) {
+                    const int i = i0 + k * kW;
+                    x[k] = make_float2(-INFINITY, 0.0f);
+                    v[k] = Dims{};
+                    if (i < chunks) x[k] = ml[i], v[k] = *reinterpret_cast<const Dims*>(po + static_cast<size_t>(i) * D);
                 }
-                top = next;
+#pragma unroll
+                for (int k0 = 0; k0 < kAhead; k0 += kStep) {
+                    float next = top;
+#pragma unroll
+                    for (int k = k0; k < k0 + kStep; ++k) next = fmaxf(next, x[k].x);
+                    const float base = next == -INFINITY ? 0.0f : next, f = ex2(top - base);
+                    l *= f;
+#pragma unroll
+                    for (int e = 0; e < kV; ++e) o.e[e] *= f;
+#pragma unroll
+                    for (int k = k0; k < k0 + kStep; ++k) {
+                        const float y = ex2(x[k].x - base);
+                        l = fmaf(x[k].y, y, l);
+#pragma unroll
+                        for (int e = 0; e < kV; ++e) o.e[e] = fmaf(v[k].e[e], y, o.e[e]);
+                    }
+                    top = next;
+                }
             }
+            *reinterpret_cast<Dims*>(&s_o[part][kV * lane]) = o;
+            if (lane == 0) s_ml[part] = make_float2(top, l);
         }
-        *reinterpret_cast<Dims*>(&s_o[w][kV * lane]) = o;
-        if (lane == 0) s_ml[w] = make_float2(top, l);
         __syncthreads();
         if (t >= DIMS) return;
         float all = -INFINITY, sum = 0.0f, out = 0.0f;
@@ -820,7 +823,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
             const int ng = min(kFinish, p.group - g0);
             if (p.group > kFinish || j0 < step) {   // else the totals are there from the first tile
                 __syncthreads();
-                for (int g = w; g < ng; g += kW) {
+                for (int g = w; g < ng; g += kWarpsIn) {
                     const float v = chunks_lse2<kBatch>(p.part_ml + 2 * (bh0 + g0 + g) * p.chunks, chunks);
                     if (lane == 0) s_lse[g] = v;
                 }
@@ -882,15 +885,15 @@ bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int r
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, int THREADS, int DIMS>
+template <typename T, int D, int THREADS, int DIMS, int kW>
 cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
     // as many tiles a (key head, sequence) as there are, within kTiles CTAs: a wide table has mostly empty ones
-    // (those 64 x 32 heads with weights: 66 us in all with every tile its CTA, 36 so)
+    // (those 64 x 32 heads with weights: 66 us in all with every tile its CTA, 37 so)
     const long long pairs = static_cast<long long>(c.kv_heads) * p.n_seq;
     const int all = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0, least = static_cast<int>(kTiles / pairs) + 1;
     const int tiles = all < least ? all : least;
-    return fer::host::launch_pdl(attn_finish<T, D, THREADS, DIMS>, dim3(p.group * (D / DIMS) + tiles, c.kv_heads, p.n_seq),
-                                 dim3(THREADS), 0, s, c, p);
+    return fer::host::launch_pdl(attn_finish<T, D, THREADS, DIMS, kW>,
+                                 dim3(p.group * (D / DIMS) + tiles, c.kv_heads, p.n_seq), dim3(THREADS), 0, s, c, p);
 }
 
 template <typename T, int D, int NT>
@@ -910,11 +913,11 @@ cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
     if (e == cudaSuccess && (p.weights || p.chunks > 1)) {
         // few chunks or many heads: a head a CTA; else sixteen warps for 32 dims, whose loads one SM could not have
         // in flight (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA; 64 x 32
-        // heads of up to 512 slots in a table of 32768: 52 us in all so, 32 with a head a CTA)
+        // heads of up to 512 slots in a table of 32768: 52 us in all so, 33 with a head a CTA)
         // Which warp takes which chunk, and with it every rounding, is a function of the table's width.
-        if (p.chunks <= 32) e = finish<T, D, 256, D>(c, p, s);
-        else if (static_cast<long long>(p.n_seq) * p.heads >= kManyHeads) e = finish<T, D, 512, D>(c, p, s);
-        else e = finish<T, D, 512, 32>(c, p, s);
+        if (p.chunks <= 32) e = finish<T, D, 256, D, 8>(c, p, s);
+        else if (static_cast<long long>(p.n_seq) * p.heads >= kManyHeads) e = finish<T, D, 256, D, 16>(c, p, s);
+        else e = finish<T, D, 512, 32, 16>(c, p, s);
     }
     return e;
 }
