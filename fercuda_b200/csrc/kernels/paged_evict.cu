@@ -36,6 +36,7 @@
 // The moves (evict_move, or the selecting CTAs where heads come in waves): a
 // warp resolves up to 32 moves at once, a lane each, then copies their rows
 // with kAhead 16-byte loads a lane in flight.
+#include "evict_keys.h"
 #include "paged.cuh"
 #include "pdl.cuh"
 
@@ -51,7 +52,7 @@ using fer::dev::Paged;
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr int kSmall = 1024;                 // slots that a warp's registers hold
 constexpr int kSelect = 1024, kSelectFew = 256;   // threads of a selecting CTA
-constexpr int kMostKeys = 32;                // keys a thread of it holds in shared memory
+using fer::evict::kMostKeys;
 constexpr int kCopies = 3;                   // of the first digit's counts, by lane: less contention
 constexpr int kMove = 256;
 constexpr int kWarpMoves = 16;
@@ -321,9 +322,8 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int* total) {
 
 // grid (cluster CTAs, kv_heads, batch). CTA r of a cluster has the slots [lo,
 // hi). They are passed over in rounds of up to 32 slots a thread, shared out
-// evenly; the key of slot lo + j lies at word j + 4 (j / 32) of shared memory,
-// so that threads read 32 in 16-byte pieces without bank conflicts. Without
-// HELD the keys of a round are made again from the arrays.
+// evenly; the key of slot lo + j lies at word word_of(j) of shared memory.
+// Without HELD the keys of a round are made again from the arrays.
 template <int D, bool HELD, int kSelect>
 __global__ void __launch_bounds__(kSelect, 1024 / kSelect) evict_select(const Paged c, const EvictParams p) {
     // Digits: with two counts a word (a CTA's held keys are few enough), four
@@ -356,18 +356,18 @@ __global__ void __launch_bounds__(kSelect, 1024 / kSelect) evict_select(const Pa
         return;
     }
     const long long first = static_cast<long long>(p.seen[b]) - p.recent;
-    const int each = ((n - 1) / ctas + 1 + 127) & ~127;
+    const int each = fer::evict::slots_of_cta(n, ctas);
     const int lo = static_cast<int>(min(static_cast<long long>(n), static_cast<long long>(rank) * each));
     const int hi = min(n - lo, each) + lo;
     // slots a thread takes in a round: all of the CTA's in one round where keys are held
-    const int run = HELD ? ((each - 1) / kSelect + 4) & ~3 : 32, round = run * kSelect;
+    const int run = HELD ? fer::evict::slots_of_thread(each, kSelect) : 32, round = run * kSelect;
     // this thread's slots of a round, `mine` on: fn(i, key)
     auto each_key = [&](int mine, auto fn) {
         if constexpr (HELD) {
 #pragma unroll 2
             for (int i = 0; i < run; i += 4) {
                 const int j = mine - lo + i;
-                const uint4 v = *reinterpret_cast<const uint4*>(s_key + j + j / 32 * 4);
+                const uint4 v = *reinterpret_cast<const uint4*>(s_key + fer::evict::word_of(j));
                 fn(i, v.x), fn(i + 1, v.y), fn(i + 2, v.z), fn(i + 3, v.w);
             }
         } else {
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kSelect, 1024 / kSelect) evict_select(const Pa
             const int j = j0 + k * kSelect;
             if (j >= hi) break;
             const uint32_t key = key_of(wt[k], pos[k], first);
-            if constexpr (HELD) s_key[(j - lo) + (j - lo) / 32 * 4] = key;
+            if constexpr (HELD) s_key[fer::evict::word_of(j - lo)] = key;
             count_one(s_hist[lane % kCopies], key >> (32 - kLog));
             if (j < p.budget) {
                 if (h.nw != h.w) h.nw[j] = wt[k];
@@ -663,15 +663,16 @@ cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t 
 template <int D, bool HELD, int THREADS>
 cudaError_t select(const Paged& c, const EvictParams& p, unsigned ctas, int batch, cudaStream_t s) {
     const auto kernel = evict_select<D, HELD, THREADS>;
-    const int each = ((c.max_slots() - 1) / static_cast<int>(ctas) + 1 + 127) & ~127;
-    const size_t smem = HELD ? static_cast<size_t>(each) / 32 * 36 * 4 : 0;
+    const int each = fer::evict::slots_of_cta(c.max_slots(), static_cast<int>(ctas));
+    const size_t smem = HELD ? sizeof(uint32_t) * fer::evict::words_of_cta(each, THREADS) : 0;
     if (HELD) {
         static std::atomic<bool> set[fer::host::kMaxDevices];
         int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
         if (dev >= fer::host::kMaxDevices || !set[dev].load(std::memory_order_relaxed)) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostKeys * THREADS / 32 * 36 * 4);
+            constexpr int most = sizeof(uint32_t) * fer::evict::words_of_cta(kMostKeys * THREADS, THREADS);
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
             if (e != cudaSuccess) return e;
             if (dev < fer::host::kMaxDevices) set[dev].store(true, std::memory_order_relaxed);
         }

@@ -1,0 +1,31 @@
+"""Paged-cache operators where a table is full to its last slot and where a
+rounding inside a kernel would show, against the 64-bit restatements of
+tests/paged_ref.py."""
+import pytest
+import torch
+
+from tests import paged_ref as ref
+from tests.test_gpu_paged import check_evict, run_evict, weights_for
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("batch,slots,cut", [
+    # a CTA of 256 threads a head, runs of 12, 20, 24 and 28 slots a thread
+    (160, 2176, 30), (160, 4864, 64), (160, 5248, 64), (160, 6400, 64), (160, 4608, 2000),
+    # of 1024 threads
+    (75, 8320, 64), (75, 20224, 64), (75, 24320, 10000), (75, 28288, 64),
+    # clusters of eight, and of four
+    (1, 8 * 8320, 100), (1, 8 * 20224, 100), (16, 4 * 8320, 20000)])
+def test_evict_from_a_full_table(session, batch, slots, cut):
+    """The longest sequences hold every slot of the table's width."""
+    lens = [slots] * min(batch, 2) + [40 + b for b in range(batch - 2)]
+    lens[-1] = slots
+    c = ref.Cache(lens, 1, 64, 64, torch.bfloat16)
+    assert c.slots == slots
+    w = weights_for("ties" if cut < 100 else "spread", batch, 1, slots, seed=slots).cuda()
+    p = torch.arange(slots, dtype=torch.int32, device="cuda").repeat(batch, 1, 1)
+    w0, p0 = w.clone(), p.clone()
+    before = (c.k.cpu().clone(), c.v.cpu().clone(), w0, p0)
+    run_evict(session, c, slots - cut, 50, w, p, c.lengths.clone())
+    check_evict(c, slots - cut, 50, w0, p0, torch.tensor(lens, dtype=torch.int32), before, (c.k, c.v, w, p, c.lengths))
