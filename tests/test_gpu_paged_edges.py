@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from tests import paged_ref as ref
-from tests.test_gpu_paged import check_evict, run_evict, weights_for
+from tests import paged_sharp as sharp
+from tests.test_gpu_paged import attend, check_evict, run_evict, weights_for
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +30,17 @@ def test_evict_from_a_full_table(session, batch, slots, cut):
     before = (c.k.cpu().clone(), c.v.cpu().clone(), w0, p0)
     run_evict(session, c, slots - cut, 50, w, p, c.lengths.clone())
     check_evict(c, slots - cut, 50, w0, p0, torch.tensor(lens, dtype=torch.int32), before, (c.k, c.v, w, p, c.lengths))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,H,group,page", [(64, 2, 1, 8), (64, 1, 9, 16), (128, 2, 4, 64), (128, 1, 16, 8),
+                                            (256, 1, 3, 32), (256, 2, 20, 16)])
+def test_attention_keeps_probabilities_in_two_parts(session, dtype, D, H, group, page):
+    """Scores are exact and values alike in size, so a P rounded once, or a lost
+    low part, would go past the bound (tests/test_paged_sharp_bound.py)."""
+    c = ref.Cache([1, 2, 3, 5, 8, 13, 16, 33, 64], H, D, page, dtype, seed=D + group)
+    q = sharp.fill(c, group, D + group).cuda()
+    out, _ = attend(session, c, q, H * group, scale=1.0)
+    out = out.cpu().double().view(len(c.lens), H, group, D)
+    for b, (p, v) in enumerate(sharp.answers(c, group)):
+        assert float((out[b] - p @ v).abs().max()) <= sharp.bound(c, b), (b, c.lens[b])
