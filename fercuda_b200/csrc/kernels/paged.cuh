@@ -7,6 +7,7 @@
 #include "sm100_util.cuh"
 
 #include <cstdint>
+#include <initializer_list>
 
 namespace fer::dev {
 
@@ -51,13 +52,19 @@ namespace fer::host {
 // Devices for which a launcher keeps what it asked the runtime once.
 constexpr int kMaxDevices = 64;
 
+// Whether all of these arrays of 32-bit numbers start at a multiple of 4 bytes (null does).
+inline bool words_aligned(std::initializer_list<const void*> arrays) {
+    uintptr_t at = 0;
+    for (const void* a : arrays) at |= reinterpret_cast<uintptr_t>(a);
+    return at % 4 == 0;
+}
+
 // Checks the view's sizes and pointers.
 inline cudaError_t paged_params(const fer_paged_view_t* c, fer::dev::Paged* p) {
     if (!c || !c->k || !c->v || !c->page_table || !c->lengths) return cudaErrorInvalidValue;
     if (c->batch <= 0 || c->max_pages <= 0 || c->pages <= 0 || c->kv_heads <= 0) return cudaErrorInvalidValue;
     if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16) return cudaErrorInvalidValue;
-    if ((reinterpret_cast<uintptr_t>(c->page_table) | reinterpret_cast<uintptr_t>(c->lengths)) % 4)
-        return cudaErrorInvalidValue;
+    if (!words_aligned({c->page_table, c->lengths})) return cudaErrorInvalidValue;
     if (c->dtype != 1 && c->dtype != 2) return cudaErrorNotSupported;
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return cudaErrorNotSupported;
     int shift = 3;

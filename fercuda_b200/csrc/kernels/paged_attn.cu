@@ -964,6 +964,7 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     if (a->q_stride < width || a->out_stride < width || !(a->scale >= 0.0f) || a->scale > 3.0e38f)
         return cudaErrorInvalidValue;
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 2) return cudaErrorInvalidValue;
+    if (!fer::host::words_aligned({a->lse, a->weights})) return cudaErrorInvalidValue;
     if (a->n_seq == 0) return cudaSuccess;
     if (c.kv_heads > 65535 || a->n_seq > 65535) return cudaErrorNotSupported;
     const int max_slots = c.max_slots();

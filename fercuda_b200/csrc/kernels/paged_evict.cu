@@ -740,6 +740,8 @@ extern "C" cudaError_t fer_paged_evict(const fer_paged_view_t* cache, const fer_
     if (!a || a->budget < 1 || a->recent < 0 || a->recent > a->budget || !a->weights || !a->positions || !a->seen ||
         !a->new_lengths || !a->new_weights || !a->new_positions)
         return cudaErrorInvalidValue;
+    if (!fer::host::words_aligned({a->weights, a->positions, a->seen, a->new_lengths, a->new_weights, a->new_positions}))
+        return cudaErrorInvalidValue;
     if (c.kv_heads > 65535 || cache->batch > 65535) return cudaErrorNotSupported;
     const int max_slots = c.max_slots();
     const size_t need = fer_paged_evict_workspace_bytes(cache->batch, c.kv_heads, max_slots, a->budget);

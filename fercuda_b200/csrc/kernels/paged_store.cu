@@ -207,6 +207,8 @@ extern "C" cudaError_t fer_paged_store(const fer_paged_view_t* cache, const fer_
     if (!a || a->rows < 0 || a->n_seq < 0 || a->n_seq > cache->batch || !a->new_lengths) return cudaErrorInvalidValue;
     if (!a->offsets && a->rows != a->n_seq) return cudaErrorInvalidValue;
     if (a->positions && (!a->seen || !a->new_seen)) return cudaErrorInvalidValue;
+    if (!fer::host::words_aligned({a->offsets, a->new_lengths, a->weights, a->positions, a->seen, a->new_seen}))
+        return cudaErrorInvalidValue;
     const size_t width = static_cast<size_t>(c.kv_heads) * c.head_dim;
     if (a->rows > 0 && (!a->k_rows || !a->v_rows || a->k_stride < width || a->v_stride < width))
         return cudaErrorInvalidValue;

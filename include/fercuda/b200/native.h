@@ -186,7 +186,7 @@ cudaError_t fer_rotary(const fer_rotary_args_t* args, cudaStream_t s);
  * not held) and the length is clamped. Entries behind the last held slot are
  * not read. Pages that fer_paged_store or fer_paged_evict write belong to one
  * place of one sequence; fer_paged_attention only reads pages, which may be
- * shared. */
+ * shared. Arrays of 32-bit numbers start at multiples of 4 bytes. */
 typedef struct fer_paged_view {
     void* k;
     void* v;

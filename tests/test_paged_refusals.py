@@ -101,6 +101,19 @@ def test_evict_refuses(change):
     assert evict(**change) == INVALID
 
 
+@pytest.mark.parametrize("at", [AT + 1, AT + 2])
+def test_misaligned_words_are_refused(at):
+    """A kernel would fault on these addresses."""
+    for name in ("offsets", "new_lengths", "weights", "seen", "new_seen"):
+        assert store(**{name: at}) == INVALID, name
+    assert store(positions=at, seen=AT, new_seen=AT) == store(positions=AT, seen=at, new_seen=AT) == INVALID
+    assert store(positions=AT, seen=AT, new_seen=at) == INVALID
+    for name in ("lse", "weights"):
+        assert attention(**{name: at}) == INVALID, name
+    for name in ("weights", "positions", "seen", "new_lengths", "new_weights", "new_positions"):
+        assert evict(**{name: at}) == INVALID, name
+
+
 def test_no_sequences_is_no_work():
     assert store() == attention() == OK
 
