@@ -287,7 +287,7 @@ fer_status_t submit_attention(Session& S, const fer_paged_attention_request_t& r
     if (rows > static_cast<uint64_t>(c.view.batch)) return invalid("paged attention has more rows than the cache");
     if (r.heads == 0 || r.heads % static_cast<uint32_t>(c.view.kv_heads) || r.heads > 65536)
         return invalid("paged attention heads must be a multiple of kv_heads, at most 65536");
-    if (!(r.scale >= 0.0f) || r.scale > 3.0e38f) return invalid("paged attention scale must be finite and not negative");
+    if (!(r.scale >= 0.0f) || r.scale > 2.0e38f) return invalid("paged attention scale must be from 0 to 2e38");
     const uint64_t width = static_cast<uint64_t>(r.heads) * c.view.head_dim;
     const Cols cq{q, r.q_col, width}, co{o, r.out_col, width};
     if (!cq.fits() || !co.fits()) return invalid("paged attention heads reach past the columns");

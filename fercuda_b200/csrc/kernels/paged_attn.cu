@@ -63,6 +63,7 @@ constexpr int kTiles = 148 * 16;     // CTAs that add weights, at least where th
 constexpr int kManyHeads = 148 * 4;  // heads whose joining fills the GPU with a CTA each
 constexpr int kSegments = 128;       // entries of the unit table in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMostScale = 2.0e38f;   // times log2 e it is still finite
 constexpr float kLn2 = 0.6931471805599453f;
 
 // Slots a chunk: a function of the table's width alone, so that a sequence's
@@ -961,7 +962,7 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     if (!a || !a->q || !a->out || a->n_seq < 0 || a->n_seq > cache->batch || a->heads <= 0 || a->heads % c.kv_heads)
         return cudaErrorInvalidValue;
     const size_t width = static_cast<size_t>(a->heads) * c.head_dim;
-    if (a->q_stride < width || a->out_stride < width || !(a->scale >= 0.0f) || a->scale > 3.0e38f)
+    if (a->q_stride < width || a->out_stride < width || !(a->scale >= 0.0f) || a->scale > kMostScale)
         return cudaErrorInvalidValue;
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out)) % 2) return cudaErrorInvalidValue;
     if (!fer::host::words_aligned({a->lse, a->weights})) return cudaErrorInvalidValue;

@@ -310,7 +310,7 @@ fer_status_t fer_submit_paged_store(fer_session_t* session, const fer_paged_stor
  * dtype) and its result the columns out_col + h * head_dim .. of out [rows,
  * cols]; heads is a multiple of kv_heads and head h reads key head h / (heads
  * / kv_heads). out = softmax(scale q.k) v over the held slots (store the new
- * token's key first), f32 statistics; scale 0: 1 / sqrt(head_dim). lse
+ * token's key first), f32 statistics; scale up to 2e38, 0: 1 / sqrt(head_dim). lse
  * (0: none) f32 [rows, heads]: log sum exp(scale q.k). weights (0: none): each
  * held slot's probabilities, summed over the heads that share it, are added
  * to it. A sequence without slots, or whose scores are all -inf, gives zeros

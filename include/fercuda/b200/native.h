@@ -233,7 +233,7 @@ typedef struct fer_paged_attention_args {
     void* out;
     size_t q_stride, out_stride;
     int n_seq, heads;
-    float scale;                 /* 0: 1 / sqrt(head_dim) */
+    float scale;                 /* up to 2e38; 0: 1 / sqrt(head_dim) */
     float* lse;
     float* weights;
     void* workspace;

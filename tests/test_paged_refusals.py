@@ -114,6 +114,12 @@ def test_misaligned_words_are_refused(at):
         assert evict(**{name: at}) == INVALID, name
 
 
+@pytest.mark.parametrize("scale,code", [(2.5e38, INVALID), (3.0e38, INVALID), (2.0e38, OK), (1e-45, OK)])
+def test_attention_takes_scales_with_a_finite_base_2_form(scale, code):
+    """scale * log2 e is one f32 factor; were it infinite, a product of 0 would give NaN."""
+    assert attention(scale=scale) == code
+
+
 def test_no_sequences_is_no_work():
     assert store() == attention() == OK
 
