@@ -8,6 +8,7 @@
 
 #include "fercuda/b200/native.h"
 
+#include <cfloat>
 #include <climits>
 #include <new>
 
@@ -175,7 +176,7 @@ fer_status_t submit_rotary(Session& S, const fer_rotary_request_t& r, uint64_t* 
     if (rot % 2 || rot > r.head_dim) return invalid("rotary_dim must be even and at most head_dim");
     if (r.flags & ~(FER_ROTARY_INTERLEAVED | FER_ROTARY_AXIS_FREQS | FER_ROTARY_INVERSE))
         return invalid("unknown rotary flags");
-    if (!(r.base > 0.0f) || r.base > 3.0e38f) return invalid("rotary base must be positive and finite");
+    if (!(r.base > 0.0f) || r.base > FLT_MAX) return invalid("rotary base must be positive and finite");
     uint64_t sum = 0;
     for (uint32_t i = 0; i < r.axes; ++i) sum += r.sections[i];
     const bool whole = r.axes == 1 && r.sections[0] == 0;

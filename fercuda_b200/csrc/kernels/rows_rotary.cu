@@ -30,6 +30,7 @@
 
 #include "fercuda/b200/native.h"
 
+#include <cfloat>
 #include <cstdint>
 #include <cstring>
 #include <type_traits>
@@ -298,7 +299,7 @@ extern "C" cudaError_t fer_rotary(const fer_rotary_args_t* a, cudaStream_t s) {
     if (a->rows < 0 || a->heads <= 0 || a->head_dim <= 0 || a->head_dim % 2 || a->rotary_dim <= 0 || a->rotary_dim % 2 ||
         a->rotary_dim > a->head_dim || a->axes < 1 || a->axes > 4 || a->head_dim > 1024 || a->heads > 65536)
         return cudaErrorInvalidValue;
-    if (!(a->base > 0.0f) || a->base > 3.0e38f || (a->flags & ~7u)) return cudaErrorInvalidValue;
+    if (!(a->base > 0.0f) || a->base > FLT_MAX || (a->flags & ~7u)) return cudaErrorInvalidValue;
     const size_t width = static_cast<size_t>(a->heads) * a->head_dim;
     if (a->x_stride < width || a->out_stride < width) return cudaErrorInvalidValue;
     if (a->x == a->out && a->x_stride != a->out_stride) return cudaErrorInvalidValue;

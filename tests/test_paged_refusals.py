@@ -31,6 +31,11 @@ def test_rotary_refuses(change):
     assert rotary(**change) == INVALID
 
 
+@pytest.mark.parametrize("base", [1e-45, 3.1e38, 3.4028234e38])
+def test_rotary_takes_every_finite_base(base):
+    assert rotary(base=base) == OK
+
+
 def test_rotary_takes_no_rows():
     assert rotary() == OK
 
