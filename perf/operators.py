@@ -11,6 +11,7 @@ may keep the attention weight summed so far and the position of its token,
 both [batch, kv_heads, slots].
 """
 import math
+import weakref
 
 import torch
 
@@ -194,8 +195,20 @@ def _prepare_cache(case, s, g):
     s["new_positions"] = torch.zeros_like(s["positions"])
 
 
+class _Registered:
+    """Buffer ids of tensors that the caller owns; they are freed with the state that holds this."""
+
+    def __init__(self, session, ids):
+        weakref.finalize(self, _release, session, ids).atexit = False
+
+
+def _release(session, ids):
+    for i in ids:
+        session.free(i)
+
+
 def _prepare_own(case, s):
-    """The session, and the tensors registered with it as buffers."""
+    """The session, and the tensors registered with it as buffers for as long as the state lives."""
     from fercuda_b200 import capi
     codes = {torch.float32: capi.FER_DTYPE_F32, torch.float16: capi.FER_DTYPE_F16, torch.bfloat16: capi.FER_DTYPE_BF16,
              torch.int32: capi.FER_DTYPE_I32, torch.uint8: capi.FER_DTYPE_U8}
@@ -214,6 +227,7 @@ def _prepare_own(case, s):
         s["workspace"] = torch.empty(size, dtype=torch.uint8, device="cuda")
     s["ids"] = ids = {k: session.import_ptr(codes[t.dtype], list(t.shape), t.data_ptr())
                       for k, t in s.items() if isinstance(t, torch.Tensor)}
+    s["registered"] = _Registered(session, list(ids.values()))
     ids.setdefault("workspace", 0)
     if case["op"] != "rotary":
         s["cache"] = capi.paged_cache(ids["k"], ids["v"], ids["table"], ids["lengths"])
