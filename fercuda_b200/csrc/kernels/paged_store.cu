@@ -61,8 +61,10 @@ __device__ __forceinline__ int new_rows(const StoreParams& p, int b) {
     return n < 0 ? 0 : n;
 }
 
-__device__ __forceinline__ void advance(const Paged& c, const StoreParams& p, int b, int len) {
-    const int n = new_rows(p, b), most = c.max_slots();
+__device__ __forceinline__ void advance(const Paged& c, const StoreParams& p, int b) {
+    bool off;
+    const int n = new_rows(p, b), most = c.max_slots(), len = c.length(b, &off);
+    if (off) fer::dev::report(p.err, fer::dev::kErrBadShape);   // of a sequence without new rows as well
     p.new_lengths[b] = n > most - len ? most : len + n;
     if (p.new_seen) p.new_seen[b] = p.seen[b] + n;
 }
@@ -180,21 +182,19 @@ __global__ void __launch_bounds__(kThreads) store_rows(const Paged c, const Stor
         }
     }
     if (!update) return;
-    bool off;
     if (p.offsets) {
         // n_seq sequences over all CTAs; nothing in this launch reads what is written
-        for (int b = blockIdx.x * kThreads + t; b < p.n_seq; b += gridDim.x * kThreads) advance(c, p, b, c.length(b, &off));
+        for (int b = blockIdx.x * kThreads + t; b < p.n_seq; b += gridDim.x * kThreads) advance(c, p, b);
     } else {
         // this CTA's own sequences; their lengths were read before the barrier
-        if (t < nr) advance(c, p, r0 + t, c.length(r0 + t, &off));
+        if (t < nr) advance(c, p, r0 + t);
     }
 }
 
 __global__ void __launch_bounds__(kThreads) advance_lengths(const Paged c, const StoreParams p) {
     fer::dev::pdl_begin();
-    bool off;
     const int b = blockIdx.x * kThreads + threadIdx.x;
-    if (b < p.n_seq) advance(c, p, b, c.length(b, &off));
+    if (b < p.n_seq) advance(c, p, b);
 }
 
 }  // namespace

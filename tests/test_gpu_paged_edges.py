@@ -10,6 +10,8 @@ from tests.test_gpu_paged import attend, check_evict, run_evict, weights_for
 
 pytestmark = pytest.mark.gpu
 
+ERR_BAD = 4
+
 
 @pytest.mark.parametrize("batch,slots,cut", [
     # a CTA of 256 threads a head, runs of 12, 20, 24 and 28 slots a thread
@@ -44,3 +46,23 @@ def test_attention_keeps_probabilities_in_two_parts(session, dtype, D, H, group,
     out = out.cpu().double().view(len(c.lens), H, group, D)
     for b, (p, v) in enumerate(sharp.answers(c, group)):
         assert float((out[b] - p @ v).abs().max()) <= sharp.bound(c, b), (b, c.lens[b])
+
+
+@pytest.mark.parametrize("bad,becomes", [(-3, 0), (10 ** 6, 64)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_store_reports_a_bad_length_without_rows(session, bad, becomes, in_place):
+    """A sequence that gets no row has its length clamped; that is reported as any other."""
+    c = ref.Cache([20, 30, 64], 2, 64, 16, torch.bfloat16)
+    c.lengths[1] = bad
+    k, v = c.k.clone(), c.v.clone()
+    rows = torch.randn(4, 2 * c.H * c.D, device="cuda").to(c.dtype)
+    offsets = torch.tensor([0, 4, 4, 4], dtype=torch.int32, device="cuda")
+    new = c.lengths if in_place else torch.full_like(c.lengths, -1)
+    with ref.Buffers(session) as B:
+        ids, r = c.ids(B), B(rows)
+        session.paged_store(ids, r, r, v_col=c.H * c.D, offsets=B(offsets), new_lengths=0 if in_place else B(new))
+    assert session.device_errors() == ERR_BAD
+    assert new.tolist() == [24, becomes, 64]
+    for pool, old, col in ((c.k, k, 0), (c.v, v, c.H * c.D)):
+        old[c.table[0, 1].item(), :, 4:8] = rows[:, col: col + c.H * c.D].view(4, c.H, c.D).transpose(0, 1)
+        assert ref.same_bits(pool, old)
