@@ -12,8 +12,10 @@
 // shared out evenly without the host knowing the lengths; where every unit
 // there can be has a CTA of its own, its index is the unit. A unit's maximum m,
 // l = sum 2^(s - m) and o = sum 2^(s - m) v go to the workspace in f32 (or,
-// with one chunk, the result to the output), and a second kernel adds a head's
-// chunks in order. Which CTA took a unit does not change its arithmetic:
+// with one chunk, the result to the output), and a second kernel joins a head's
+// chunks: 8 or 16 partial sums of every 8th or 16th chunk each, then those in
+// order. How many depends on the table's width, and how many chunks share a
+// maximum on head_dim. Which CTA took a unit does not change its arithmetic:
 // results are the same run to run and for any batch.
 //
 // Inside a unit a warp loads rounds of 64 slots by tensor copies of page rows
@@ -25,16 +27,19 @@
 // a unit's end) and takes few registers, and several CTAs share an SM and hide
 // one another's latencies. Products are 16-bit tensor-core tiles with f32
 // accumulation: with slots or dims as rows the 8 columns are the heads, so a
-// group of up to 8 heads wastes nothing it would have to read. (One query
-// gives 8 or 16 columns a tile at best, 1/16 of the 128 rows a tcgen05 tile
-// has, and the tiles here run at a few per cent of the tensor pipe anyway.)
+// group of up to 8 heads wastes nothing it would have to read. (A group of up
+// to 16 heads is 1/8 of the 128 rows a tcgen05 tile has, and the tiles here run
+// at a few per cent of the tensor pipe. Larger groups read their pages once
+// more, from L2, for every 16 heads: 64 heads over one key head, 64 sequences
+// of up to 2048 slots, take 47 us, ten times their bytes at the copy rate;
+// there heads as a tcgen05 tile's rows would fit.)
 // P is kept as the sum of two 16-bit numbers, so it has 16 bits or more:
 // rounding it once would have added half of the output's own rounding error.
 //
 // Measured (HBM copy 6538 GB/s): 131071 slots x 8 key heads of 128 for 64
-// heads 92.5 us, 5.8 TB/s; 33 sequences of 0 to 8192 slots with weights 115
+// heads 91 to 92.5 us, 5.8 TB/s; 33 sequences of 0 to 8192 slots with weights 115
 // us (86 us at the copy rate); 64 sequences of 1 to 1024 slots x 16 heads of 64
-// 33.2 us (20.6): 3.5 us pass until the first rows arrive, CTAs end between 18
+// 32 to 33.2 us (20.6): 3.5 us pass until the first rows arrive, CTAs end between 18
 // and 29 us as they have a unit more or less, and 5 us go to the joining.
 //
 // Scores are kept in base-2 units (scale * log2 e folded into one factor).
@@ -68,8 +73,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // Slots a chunk: a function of the table's width alone, so that a sequence's
 // results do not depend on the batch. Short chunks share the work out more
-// evenly, long ones write fewer parts: 2 x 40003 slots take 40.0 us in chunks
-// of 512 and 38.3 of 256, 131071 slots 95.5 of 512 and 113 of 256.
+// evenly, long ones write fewer parts: 2 x 40003 slots with weights take 39.2 us
+// in chunks of 512 and 36.6 of 256, 131071 slots 91.1 of 512 and 97.5 of 256.
 __host__ __device__ inline int chunk_of(int max_slots) { return max_slots > 65536 ? 512 : 256; }
 
 struct AttnParams {

@@ -16,11 +16,11 @@
 // sequences' lengths and writes the new ones itself, in place or not. With
 // offsets a sequence may span CTAs; then the first CTA's threads write the
 // new lengths when they go elsewhere, and a second small kernel when they
-// replace the old.
+// replace the old (2 us more).
 //
-// Measured: 37 prompts of 1 to 2048 rows of 8 heads x 128 f16 52.6 us, 91% of
-// the HBM copy rate; a step of 64 rows of 16 heads x 64 4.8 us, the host's time
-// for the call.
+// Measured: 37 prompts of 1 to 2048 rows of 8 heads x 128 f16 52.6 to 54.4 us,
+// 88 to 91% of the HBM copy rate; a step of 64 rows of 16 heads x 64 4.6 us, the
+// host's time for the call.
 #include "paged.cuh"
 #include "pdl.cuh"
 

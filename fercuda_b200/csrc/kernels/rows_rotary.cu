@@ -18,13 +18,13 @@
 // back. A unit of the half-split layout is V elements of the first half and
 // the V that pair with them; V is the widest that pointers, strides and sizes
 // allow. What lies behind the turned part of a head is copied by itself, in the
-// widest pieces that fit it (16384 rows of 32 heads x 128 of which 64 turn: 61
+// widest pieces that fit it (16384 rows of 32 heads x 128 of which 64 turn: 59
 // us; 111 as further units of the turning lanes).
 //
-// Measured: 32768 rows of 32 heads x 64 bf16 45.6 us, 5.9 TB/s (90% of the HBM
-// copy rate); 10007 rows of 40 heads x 128 f16 with three axes 39.0 us, 5.3
-// TB/s; one row 4.8 us, the host's time for the call. A CTA a tile of rows
-// with one table and barriers took 64.7 and 56.5 us.
+// Measured: 32768 rows of 32 heads x 64 bf16 45.6 to 48.6 us, 5.5 to 5.9 TB/s
+// (85 to 90% of the HBM copy rate); 10007 rows of 40 heads x 128 f16 with three
+// axes 39.0 us, 5.3 TB/s; one row 4.5 us, the host's time for the call. A CTA a
+// tile of rows with one table and barriers took 64.7 and 56.5 us.
 #include "elem.cuh"
 #include "pdl.cuh"
 

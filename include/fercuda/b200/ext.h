@@ -232,7 +232,7 @@ fer_status_t fer_transformer_decode(fer_session_t* session, uint64_t model, uint
  * stands for all). Pair i turns by position * base^(-i / (rotary_dim / 2)); with
  * FER_ROTARY_AXIS_FREQS the j-th pair of axis a by position * base^(-j /
  * sections[a]). FER_ROTARY_INVERSE turns back, which is also the gradient of
- * the call without it. base: > 0 and finite. */
+ * the call without it. base: > 0 and finite. heads: at most 65536. */
 #define FER_ROTARY_INTERLEAVED 1u
 #define FER_ROTARY_AXIS_FREQS 2u
 #define FER_ROTARY_INVERSE 4u
@@ -261,8 +261,10 @@ fer_status_t fer_submit_rotary(fer_session_t* session, const fer_rotary_request_
  * lengths i32 [batch]. Slot s of sequence b is row s % page_size of page
  * page_table[b][s / page_size]; slots 0 .. lengths[b] - 1 are held, and the
  * table's entries behind them are not read. A page id or a length out of range
- * sets error bit 4 (fer_session_device_errors): slots of such a page count as
- * not held, a length is clamped to 0 .. max_pages * page_size. Attention may
+ * sets error bit 4 (fer_session_device_errors): a length is clamped to 0 ..
+ * max_pages * page_size; attention counts slots of such a page as not held,
+ * store drops their keys and values, and evict, which selects among all slots,
+ * copies no row from or to one. batch and kv_heads: at most 65535. Attention may
  * read pages that several sequences share; pages that store or evict write
  * must have one place in one sequence.
  * Two optional arrays per slot follow a sequence's slots: weights f32 and
@@ -308,7 +310,7 @@ fer_status_t fer_submit_paged_store(fer_session_t* session, const fer_paged_stor
 /* One new token's attention for the first rows(q) sequences: query head h of
  * row b is columns q_col + h * head_dim .. of q [rows, cols] (the cache's
  * dtype) and its result the columns out_col + h * head_dim .. of out [rows,
- * cols]; heads is a multiple of kv_heads and head h reads key head h / (heads
+ * cols]; heads is a multiple of kv_heads, at most 65536, and head h reads key head h / (heads
  * / kv_heads). out = softmax(scale q.k) v over the held slots (store the new
  * token's key first), f32 statistics; scale up to 2e38, 0: 1 / sqrt(head_dim). lse
  * (0: none) f32 [rows, heads]: log sum exp(scale q.k). weights (0: none): each
@@ -319,7 +321,9 @@ fer_status_t fer_submit_paged_store(fer_session_t* session, const fer_paged_stor
  * overlap. workspace: u8 buffer (16-byte aligned) of at least
  * fer_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim,
  * max_pages * page_size, weights != 0) bytes, any contents; calls on different
- * streams need one each. */
+ * streams need one each. It goes by the table's width, not by what is held:
+ * 4 bytes a row, head and slot with weights, and 4 (head_dim + 2) a row, head
+ * and 256 slots (512 in tables of more than 65536). */
 typedef struct fer_paged_attention_request {
     fer_paged_cache_t cache;
     uint64_t q;
@@ -345,7 +349,10 @@ fer_status_t fer_submit_paged_attention(fer_session_t* session, const fer_paged_
  * positions. budget >= 1, recent <= budget. new_lengths, new_weights and
  * new_positions receive the results (each 0 or the old one: in place; separate
  * ones also receive what stayed); keys and values move in place, and
- * everything behind a sequence's new length is left as it was. Pages behind
+ * everything behind a sequence's new length is left as it was. (Store gives new
+ * slots the weight 0 and only attention of one token adds to it: right behind a
+ * prompt a cut keeps the recent and the lowest slots, unless the caller has put
+ * weights of its own into the array.) Pages behind
  * ceil(budget / page_size) are free for other sequences afterwards. workspace:
  * u8 buffer (16-byte aligned) of fer_paged_evict_workspace_bytes(batch,
  * kv_heads, max_pages * page_size, budget) bytes, any contents; calls on

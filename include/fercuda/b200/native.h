@@ -182,8 +182,9 @@ cudaError_t fer_rotary(const fer_rotary_args_t* args, cudaStream_t s);
  * page_table[b][s / page_size], and slots 0 .. lengths[b] - 1 are held.
  * page_size is a power of two from 8 to 256, head_dim 64, 128 or 256. A page
  * id outside [0, pages), or a length outside [0, max_pages * page_size], that
- * a kernel meets sets error bit 4; slots of such a page are skipped (as if
- * not held) and the length is clamped. Entries behind the last held slot are
+ * a kernel meets sets error bit 4; the length is clamped, attention skips slots
+ * of such a page (as if not held), store drops their rows and evict, which
+ * selects among all slots, copies no row from or to one. Entries behind the last held slot are
  * not read. Pages that fer_paged_store or fer_paged_evict write belong to one
  * place of one sequence; fer_paged_attention only reads pages, which may be
  * shared. Arrays of 32-bit numbers start at multiples of 4 bytes. */
