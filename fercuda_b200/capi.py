@@ -209,6 +209,36 @@ class fer_paged_evict_args_t(C.Structure):
                 ("new_positions", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class fer_norm_rotary_args_t(C.Structure):
+    _fields_ = [("rotary", fer_rotary_args_t), ("k_heads", C.c_int), ("q_gamma", C.c_void_p), ("k_gamma", C.c_void_p),
+                ("eps", C.c_float)]
+
+
+class fer_norm_rotary_grad_t(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("grad_stride", C.c_size_t), ("q_gamma_grad", C.c_void_p),
+                ("k_gamma_grad", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class fer_paged_plan_args_t(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("page_table", "lengths", "counts", "held", "seen", "free_pages", "free_state",
+                                          "new_held", "new_free_state", "offsets", "sequences", "positions", "slots")] + \
+               [(n, C.c_int) for n in ("batch", "max_pages", "pages", "page_size", "rows")]
+
+
+class fer_paged_window_args_t(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_size_t), ("out_stride", C.c_size_t),
+                ("rows", C.c_int), ("n_seq", C.c_int), ("heads", C.c_int), ("offsets", C.c_void_p), ("window", C.c_int),
+                ("sinks", C.c_int), ("scale", C.c_float), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class fer_paged_prefix_args_t(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_size_t), ("out_stride", C.c_size_t),
+                ("n_seq", C.c_int), ("heads", C.c_int), ("prefix_pages", C.c_void_p), ("prefix_length", C.c_void_p),
+                ("max_prefix_pages", C.c_int), ("scale", C.c_float), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
 class fer_rotary_request_t(C.Structure):
     _fields_ = [("x", C.c_uint64), ("out", C.c_uint64), ("positions", C.c_uint64), ("x_col", C.c_uint32),
                 ("out_col", C.c_uint32), ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32),
@@ -235,6 +265,35 @@ class fer_paged_evict_request_t(C.Structure):
     _fields_ = [("cache", fer_paged_cache_t), ("weights", C.c_uint64), ("positions", C.c_uint64), ("seen", C.c_uint64),
                 ("new_lengths", C.c_uint64), ("new_weights", C.c_uint64), ("new_positions", C.c_uint64),
                 ("workspace", C.c_uint64), ("budget", C.c_uint32), ("recent", C.c_uint32)]
+
+
+class fer_norm_rotary_request_t(C.Structure):
+    _fields_ = [("rotary", fer_rotary_request_t), ("q_gamma", C.c_uint64), ("k_gamma", C.c_uint64), ("k_heads", C.c_uint32),
+                ("eps", C.c_float)]
+
+
+class fer_norm_rotary_grad_request_t(C.Structure):
+    _fields_ = [("rotary", fer_rotary_request_t), ("q_gamma", C.c_uint64), ("k_gamma", C.c_uint64), ("grad", C.c_uint64),
+                ("q_gamma_grad", C.c_uint64), ("k_gamma_grad", C.c_uint64), ("workspace", C.c_uint64),
+                ("grad_col", C.c_uint32), ("k_heads", C.c_uint32), ("eps", C.c_float), ("reserved", C.c_uint32)]
+
+
+class fer_paged_plan_request_t(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("page_table", "lengths", "counts", "held", "free_pages", "free_state", "offsets",
+                                          "new_held", "new_free_state", "sequences", "positions", "slots", "seen")] + \
+               [("page_size", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class fer_paged_window_attention_request_t(C.Structure):
+    _fields_ = [("cache", fer_paged_cache_t), ("q", C.c_uint64), ("out", C.c_uint64), ("lse", C.c_uint64),
+                ("offsets", C.c_uint64), ("workspace", C.c_uint64), ("q_col", C.c_uint32), ("out_col", C.c_uint32),
+                ("heads", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32), ("scale", C.c_float)]
+
+
+class fer_paged_prefix_attention_request_t(C.Structure):
+    _fields_ = [("cache", fer_paged_cache_t), ("q", C.c_uint64), ("out", C.c_uint64), ("lse", C.c_uint64),
+                ("prefix_pages", C.c_uint64), ("prefix_length", C.c_uint64), ("workspace", C.c_uint64),
+                ("q_col", C.c_uint32), ("out_col", C.c_uint32), ("heads", C.c_uint32), ("scale", C.c_float)]
 
 
 class fer_transformer_config_t(C.Structure):
@@ -341,6 +400,11 @@ CAPI_PROTOTYPES = {
     "fer_submit_paged_store": (S, [P, P, pu64]),   # fer_paged_store_request_t*
     "fer_submit_paged_attention": (S, [P, P, pu64]),   # fer_paged_attention_request_t*
     "fer_submit_paged_evict": (S, [P, P, pu64]),   # fer_paged_evict_request_t*
+    "fer_submit_norm_rotary": (S, [P, P, pu64]),   # fer_norm_rotary_request_t*
+    "fer_submit_norm_rotary_grad": (S, [P, P, pu64]),   # fer_norm_rotary_grad_request_t*
+    "fer_submit_paged_plan": (S, [P, P, pu64]),   # fer_paged_plan_request_t*
+    "fer_submit_paged_window_attention": (S, [P, P, pu64]),   # fer_paged_window_attention_request_t*
+    "fer_submit_paged_prefix_attention": (S, [P, P, pu64]),   # fer_paged_prefix_attention_request_t*
     "fer_transformer_create": (S, [P, C.POINTER(fer_transformer_config_t), pu64]),
     "fer_transformer_init_weights": (S, [P, u64, u64, f32]),
     "fer_transformer_weight_buffer": (S, [P, u64, pu64]),
@@ -433,6 +497,14 @@ KERNEL_PROTOTYPES = {
     "fer_paged_attention": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_attention_args_t), P, P]),
     "fer_paged_evict_workspace_bytes": (sz, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "fer_paged_evict": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_evict_args_t), P, P]),
+    "fer_norm_rotary": (C.c_int, [C.POINTER(fer_norm_rotary_args_t), P]),
+    "fer_norm_rotary_grad_workspace_bytes": (sz, [C.c_int, C.c_int, C.c_int]),
+    "fer_norm_rotary_grad": (C.c_int, [C.POINTER(fer_norm_rotary_args_t), C.POINTER(fer_norm_rotary_grad_t), P]),
+    "fer_paged_plan": (C.c_int, [C.POINTER(fer_paged_plan_args_t), P, P]),
+    "fer_paged_window_attention_workspace_bytes": (sz, [C.c_int] * 8),
+    "fer_paged_window_attention": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_window_args_t), P, P]),
+    "fer_paged_prefix_attention_workspace_bytes": (sz, [C.c_int] * 6),
+    "fer_paged_prefix_attention": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_prefix_args_t), P, P]),
 }
 
 _LIBS: dict[str, C.CDLL] = {}
@@ -538,6 +610,11 @@ _pack_rotary = struct.Struct("=3Q10IfI").pack
 _pack_store = struct.Struct("=12Q2I").pack
 _pack_attention = struct.Struct("=9Q3If").pack
 _pack_evict = struct.Struct("=11Q2I").pack
+_pack_norm_rotary = struct.Struct("=3Q10IfI2QIf").pack
+_pack_norm_rotary_grad = struct.Struct("=3Q10IfI6Q2IfI").pack
+_pack_plan = struct.Struct("=13Q2I").pack
+_pack_window_attention = struct.Struct("=9Q5If").pack
+_pack_prefix_attention = struct.Struct("=10Q3If").pack
 
 
 def paged_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_slots: int,
@@ -549,6 +626,25 @@ def paged_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, head_d
 def paged_evict_workspace_bytes(batch: int, kv_heads: int, max_slots: int, budget: int) -> int:
     """Bytes of workspace of Session.paged_evict."""
     return kernels().fer_paged_evict_workspace_bytes(batch, kv_heads, max_slots, budget)
+
+
+def norm_rotary_grad_workspace_bytes(rows: int, heads: int, head_dim: int) -> int:
+    """Bytes of workspace of Session.norm_rotary_grad."""
+    return kernels().fer_norm_rotary_grad_workspace_bytes(rows, heads, head_dim)
+
+
+def paged_window_attention_workspace_bytes(rows: int, sequences: int, heads: int, kv_heads: int, head_dim: int,
+                                           max_slots: int, window: int, sinks: int) -> int:
+    """Bytes of workspace of Session.paged_window_attention; max_slots is max_pages * page_size."""
+    return kernels().fer_paged_window_attention_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_slots,
+                                                                window, sinks)
+
+
+def paged_prefix_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_slots: int,
+                                           max_prefix_slots: int) -> int:
+    """Bytes of workspace of Session.paged_prefix_attention; slots are pages * page_size."""
+    return kernels().fer_paged_prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim, max_slots,
+                                                                max_prefix_slots)
 
 
 class Session:
@@ -687,6 +783,52 @@ class Session:
                     *, workspace: int, new_lengths: int = 0, new_weights: int = 0, new_positions: int = 0) -> int:
         return self._submit(self.lib.fer_submit_paged_evict, _pack_evict(
             *cache, weights, positions, seen, new_lengths, new_weights, new_positions, workspace, budget, recent))
+
+    def norm_rotary(self, x: int, out: int, positions: int, heads: int, head_dim: int, *, k_heads: int = 0,
+                    q_gamma: int = 0, k_gamma: int = 0, eps: float = 1e-6, sections=(0,), rotary_dim: int = 0,
+                    base: float = 10000.0, x_col: int = 0, out_col: int = 0, interleaved: bool = False,
+                    axis_freqs: bool = False) -> int:
+        """fer_submit_norm_rotary; the last k_heads of the heads are key heads."""
+        if not 1 <= len(sections) <= 4:
+            raise ValueError("rotary takes 1 to 4 axes")
+        flags = (FER_ROTARY_INTERLEAVED if interleaved else 0) + (FER_ROTARY_AXIS_FREQS if axis_freqs else 0)
+        axes = len(sections)
+        return self._submit(self.lib.fer_submit_norm_rotary, _pack_norm_rotary(
+            x, out, positions, x_col, out_col, heads, head_dim, rotary_dim, axes, *sections, *_NONE[axes:], base, flags,
+            q_gamma, k_gamma, k_heads, eps))
+
+    def norm_rotary_grad(self, x: int, grad: int, out: int, positions: int, heads: int, head_dim: int, *, workspace: int,
+                         k_heads: int = 0, q_gamma: int = 0, k_gamma: int = 0, q_gamma_grad: int = 0,
+                         k_gamma_grad: int = 0, eps: float = 1e-6, sections=(0,), rotary_dim: int = 0,
+                         base: float = 10000.0, x_col: int = 0, grad_col: int = 0, out_col: int = 0,
+                         interleaved: bool = False, axis_freqs: bool = False) -> int:
+        """fer_submit_norm_rotary_grad: out receives the gradient of x."""
+        if not 1 <= len(sections) <= 4:
+            raise ValueError("rotary takes 1 to 4 axes")
+        flags = (FER_ROTARY_INTERLEAVED if interleaved else 0) + (FER_ROTARY_AXIS_FREQS if axis_freqs else 0)
+        axes = len(sections)
+        return self._submit(self.lib.fer_submit_norm_rotary_grad, _pack_norm_rotary_grad(
+            x, out, positions, x_col, out_col, heads, head_dim, rotary_dim, axes, *sections, *_NONE[axes:], base, flags,
+            q_gamma, k_gamma, grad, q_gamma_grad, k_gamma_grad, workspace, grad_col, k_heads, eps, 0))
+
+    def paged_plan(self, page_table: int, lengths: int, counts: int, held: int, free_pages: int, free_state: int,
+                   offsets: int, *, page_size: int, new_held: int = 0, new_free_state: int = 0, sequences: int = 0,
+                   positions: int = 0, slots: int = 0, seen: int = 0) -> int:
+        return self._submit(self.lib.fer_submit_paged_plan, _pack_plan(
+            page_table, lengths, counts, held, free_pages, free_state, offsets, new_held, new_free_state, sequences,
+            positions, slots, seen, page_size, 0))
+
+    def paged_window_attention(self, cache: PagedCache, q: int, out: int, heads: int, window: int, sinks: int, *,
+                               workspace: int, offsets: int = 0, q_col: int = 0, out_col: int = 0, scale: float = 0.0,
+                               lse: int = 0) -> int:
+        return self._submit(self.lib.fer_submit_paged_window_attention, _pack_window_attention(
+            *cache, q, out, lse, offsets, workspace, q_col, out_col, heads, window, sinks, scale))
+
+    def paged_prefix_attention(self, cache: PagedCache, prefix_pages: int, prefix_length: int, q: int, out: int,
+                               heads: int, *, workspace: int, q_col: int = 0, out_col: int = 0, scale: float = 0.0,
+                               lse: int = 0) -> int:
+        return self._submit(self.lib.fer_submit_paged_prefix_attention, _pack_prefix_attention(
+            *cache, q, out, lse, prefix_pages, prefix_length, workspace, q_col, out_col, heads, scale))
 
     def import_ptr(self, dtype: int, shape, ptr: int) -> int:
         """Registers external device memory (e.g. a torch tensor) as a buffer."""

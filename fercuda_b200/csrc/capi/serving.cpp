@@ -1,5 +1,8 @@
 // Serving operators of a paged key-value cache: fer_submit_rotary,
-// fer_submit_paged_store, fer_submit_paged_attention, fer_submit_paged_evict.
+// fer_submit_norm_rotary and its gradient, fer_submit_paged_plan,
+// fer_submit_paged_store, fer_submit_paged_attention,
+// fer_submit_paged_window_attention, fer_submit_paged_prefix_attention,
+// fer_submit_paged_evict.
 //
 // Unknown ids -> NOT_FOUND; wrong dtypes, ranks, shapes, columns and
 // overlapping outputs -> INVALID_ARGUMENT. Nothing is launched after a
@@ -10,6 +13,7 @@
 
 #include <cfloat>
 #include <climits>
+#include <initializer_list>
 #include <new>
 
 using fer::capi::Buffer;
@@ -156,7 +160,15 @@ bool capturing(const Session& S) {
 
 const char* const kCapturing = "session stream is being captured; use the launchers of native.h";
 
-fer_status_t submit_rotary(Session& S, const fer_rotary_request_t& r, uint64_t* out_job_id) {
+// The buffers and columns of a rotary request.
+struct Rotary {
+    Cols x, out;
+    const Buffer* positions = nullptr;
+    fer_rotary_args_t args{};
+};
+
+// Checks a rotary request whose flags are among `flags` and head_dim at most `most_dim`.
+fer_status_t open_rotary(const Session& S, const fer_rotary_request_t& r, uint32_t flags, uint32_t most_dim, Rotary* to) {
     const Buffer* x = S.find(r.x);
     const Buffer* o = S.find(r.out);
     const Buffer* pos = S.find(r.positions);
@@ -170,12 +182,12 @@ fer_status_t submit_rotary(Session& S, const fer_rotary_request_t& r, uint64_t* 
     if (pos->desc.dtype != FER_DTYPE_I32 || pos->desc.dims[0] != x->desc.dims[0] ||
         !((pos->desc.rank == 1 && r.axes == 1) || (pos->desc.rank == 2 && pos->desc.dims[1] == r.axes)))
         return invalid("rotary requires i32 positions [rows, axes]");
-    if (r.heads == 0 || r.heads > 65536 || r.head_dim == 0 || r.head_dim % 2 || r.head_dim > 1024)
-        return invalid("rotary requires 1 to 65536 heads of an even head_dim of at most 1024");
+    if (r.heads == 0 || r.heads > 65536 || r.head_dim == 0 || r.head_dim % 2 || r.head_dim > most_dim)
+        return invalid(most_dim == 1024 ? "rotary requires 1 to 65536 heads of an even head_dim of at most 1024"
+                                        : "norm and rotary require 1 to 65536 heads of an even head_dim of at most 256");
     const uint32_t rot = r.rotary_dim ? r.rotary_dim : r.head_dim;
     if (rot % 2 || rot > r.head_dim) return invalid("rotary_dim must be even and at most head_dim");
-    if (r.flags & ~(FER_ROTARY_INTERLEAVED | FER_ROTARY_AXIS_FREQS | FER_ROTARY_INVERSE))
-        return invalid("unknown rotary flags");
+    if (r.flags & ~flags) return invalid("unknown rotary flags");
     if (!(r.base > 0.0f) || r.base > FLT_MAX) return invalid("rotary base must be positive and finite");
     uint64_t sum = 0;
     for (uint32_t i = 0; i < r.axes; ++i) sum += r.sections[i];
@@ -187,7 +199,10 @@ fer_status_t submit_rotary(Session& S, const fer_rotary_request_t& r, uint64_t* 
     const bool in_place = x->ptr == o->ptr && x->desc.dims[1] == o->desc.dims[1] && r.x_col == r.out_col;
     if (!in_place && overlap(cx, co)) return invalid("rotary x and out overlap");
     if (overlap(o, pos)) return invalid("rotary out and positions overlap");
-    fer_rotary_args_t a{};
+    to->x = cx;
+    to->out = co;
+    to->positions = pos;
+    fer_rotary_args_t& a = to->args;
     a.x = cx.at();
     a.out = co.at();
     a.positions = static_cast<const int32_t*>(pos->ptr);
@@ -202,8 +217,160 @@ fer_status_t submit_rotary(Session& S, const fer_rotary_request_t& r, uint64_t* 
     a.base = r.base;
     a.flags = r.flags;
     a.dtype = x->desc.dtype;
+    return ok();
+}
+
+fer_status_t submit_rotary(Session& S, const fer_rotary_request_t& r, uint64_t* out_job_id) {
+    Rotary t;
+    const fer_status_t st =
+        open_rotary(S, r, FER_ROTARY_INTERLEAVED | FER_ROTARY_AXIS_FREQS | FER_ROTARY_INVERSE, 1024, &t);
+    if (st.code != FER_STATUS_OK) return st;
     if (capturing(S)) return invalid(kCapturing);
-    return finish(S, fer_rotary(&a, S.stream), out_job_id);
+    return finish(S, fer_rotary(&t.args, S.stream), out_job_id);
+}
+
+// What the norm adds to a rotary request: gammas, eps, and how many heads are keys.
+fer_status_t open_norm(const Session& S, const fer_rotary_request_t& r, uint64_t q_gamma, uint64_t k_gamma, uint32_t k_heads,
+                       float eps, Rotary* t, const Buffer* (&gamma)[2], fer_norm_rotary_args_t* a) {
+    const fer_status_t st = open_rotary(S, r, FER_ROTARY_INTERLEAVED | FER_ROTARY_AXIS_FREQS, 256, t);
+    if (st.code != FER_STATUS_OK) return st;
+    if (!find_optional(S, q_gamma, &gamma[0]) || !find_optional(S, k_gamma, &gamma[1])) return not_found("buffer id not found");
+    for (const Buffer* g : gamma) {
+        if (g && !is_vector(g, FER_DTYPE_F32, r.head_dim)) return invalid("norm gammas must be f32 [head_dim]");
+        if (g && overlap(g, t->out.buf)) return invalid("norm out and gammas overlap");
+    }
+    if (k_heads > r.heads) return invalid("norm has more key heads than heads");
+    if (!(eps >= 0.0f) || eps > FLT_MAX) return invalid("norm eps must be finite and not negative");
+    a->rotary = t->args;
+    a->k_heads = static_cast<int>(k_heads);
+    a->q_gamma = gamma[0] ? static_cast<const float*>(gamma[0]->ptr) : nullptr;
+    a->k_gamma = gamma[1] ? static_cast<const float*>(gamma[1]->ptr) : nullptr;
+    a->eps = eps;
+    return ok();
+}
+
+fer_status_t submit_norm_rotary(Session& S, const fer_norm_rotary_request_t& r, uint64_t* out_job_id) {
+    Rotary t;
+    const Buffer* gamma[2];
+    fer_norm_rotary_args_t a{};
+    const fer_status_t st = open_norm(S, r.rotary, r.q_gamma, r.k_gamma, r.k_heads, r.eps, &t, gamma, &a);
+    if (st.code != FER_STATUS_OK) return st;
+    if (capturing(S)) return invalid(kCapturing);
+    return finish(S, fer_norm_rotary(&a, S.stream), out_job_id);
+}
+
+fer_status_t submit_norm_rotary_grad(Session& S, const fer_norm_rotary_grad_request_t& r, uint64_t* out_job_id) {
+    Rotary t;
+    const Buffer* gamma[2];
+    fer_norm_rotary_args_t a{};
+    const fer_status_t st = open_norm(S, r.rotary, r.q_gamma, r.k_gamma, r.k_heads, r.eps, &t, gamma, &a);
+    if (st.code != FER_STATUS_OK) return st;
+    const Buffer* g = S.find(r.grad);
+    const Buffer* ws = S.find(r.workspace);
+    const Buffer* sum[2];
+    if (!g || !ws || !find_optional(S, r.q_gamma_grad, &sum[0]) || !find_optional(S, r.k_gamma_grad, &sum[1]))
+        return not_found("buffer id not found");
+    if (g->desc.dtype != t.x.buf->desc.dtype || g->desc.rank != 2 || g->desc.dims[0] != t.x.buf->desc.dims[0])
+        return invalid("norm gradient requires a rank-2 grad of x's dtype and rows");
+    const Cols cg{g, r.grad_col, t.x.n};
+    if (!cg.fits()) return invalid("norm gradient heads reach past the columns");
+    const bool in_place = g->ptr == t.out.buf->ptr && g->desc.dims[1] == t.out.buf->desc.dims[1] && cg.col == t.out.col;
+    if (!in_place && overlap(cg, t.out)) return invalid("norm gradient grad and out overlap");
+    if (ws->desc.dtype != FER_DTYPE_U8) return invalid("workspace must be a u8 buffer");
+    if (ws->bytes < fer_norm_rotary_grad_workspace_bytes(a.rotary.rows, a.rotary.heads, a.rotary.head_dim) ||
+        reinterpret_cast<uintptr_t>(ws->ptr) % 16)
+        return invalid("workspace is too small or not 16-byte aligned");
+    const Buffer* out[] = {t.out.buf, sum[0], sum[1], ws};
+    const Buffer* in[] = {t.x.buf, g, t.positions, gamma[0], gamma[1]};
+    for (int i = 0; i < 4; ++i) {
+        if (!out[i]) continue;
+        if (i > 0 && i < 3 && !is_vector(out[i], FER_DTYPE_F32, r.rotary.head_dim))
+            return invalid("norm gamma gradients must be f32 [head_dim]");
+        for (int j = 0; j < i; ++j)
+            if (out[j] && overlap(out[i], out[j])) return invalid("norm gradient buffers overlap");
+        for (const Buffer* b : in)   // out against the others was judged by columns
+            if (i > 0 && b && overlap(out[i], b)) return invalid("norm gradient buffers overlap");
+    }
+    fer_norm_rotary_grad_t d{};
+    d.grad = cg.at();
+    d.grad_stride = g->desc.dims[1];
+    d.q_gamma_grad = sum[0] ? static_cast<float*>(sum[0]->ptr) : nullptr;
+    d.k_gamma_grad = sum[1] ? static_cast<float*>(sum[1]->ptr) : nullptr;
+    d.workspace = ws->ptr;
+    d.workspace_bytes = ws->bytes;
+    if (capturing(S)) return invalid(kCapturing);
+    return finish(S, fer_norm_rotary_grad(&a, &d, S.stream), out_job_id);
+}
+
+fer_status_t submit_plan(Session& S, const fer_paged_plan_request_t& r, uint64_t* out_job_id) {
+    const Buffer* table = S.find(r.page_table);
+    const Buffer* len = S.find(r.lengths);
+    const Buffer* count = S.find(r.counts);
+    const Buffer* held = S.find(r.held);
+    const Buffer* ring = S.find(r.free_pages);
+    const Buffer* state = S.find(r.free_state);
+    const Buffer* off = S.find(r.offsets);
+    const Buffer *nheld, *nstate, *row[3], *seen;
+    if (!table || !len || !count || !held || !ring || !state || !off || !find_optional(S, r.new_held, &nheld) ||
+        !find_optional(S, r.new_free_state, &nstate) || !find_optional(S, r.sequences, &row[0]) ||
+        !find_optional(S, r.positions, &row[1]) || !find_optional(S, r.slots, &row[2]) || !find_optional(S, r.seen, &seen))
+        return not_found("buffer id not found");
+    if (!nheld) nheld = held;
+    if (!nstate) nstate = state;
+    if (table->desc.dtype != FER_DTYPE_I32 || table->desc.rank != 2) return invalid("paged plan requires an i32 rank-2 page table");
+    const uint64_t batch = table->desc.dims[0], max_pages = table->desc.dims[1];
+    for (const Buffer* b : {len, count, held, nheld, seen})
+        if (b && !is_vector(b, FER_DTYPE_I32, batch))
+            return invalid("paged plan requires i32 lengths, counts, held, new_held and seen [batch]");
+    if (ring->desc.dtype != FER_DTYPE_I32 || ring->desc.rank != 1) return invalid("paged plan requires i32 free_pages [pages]");
+    if (!is_vector(state, FER_DTYPE_I32, 2) || !is_vector(nstate, FER_DTYPE_I32, 2))
+        return invalid("paged plan requires i32 free_state and new_free_state [2]");
+    if (!is_vector(off, FER_DTYPE_I32, batch + 1)) return invalid("paged plan requires i32 offsets [batch + 1]");
+    uint64_t rows = 0;
+    for (const Buffer* b : row) {
+        if (!b) continue;
+        if (b->desc.dtype != FER_DTYPE_I32 || b->desc.rank != 1 || (rows && b->desc.dims[0] != rows) || b->desc.dims[0] > INT_MAX)
+            return invalid("paged plan requires i32 sequences, positions and slots of the same rows");
+        rows = b->desc.dims[0];
+    }
+    if (r.page_size < 8 || r.page_size > 256 || (r.page_size & (r.page_size - 1)))
+        return invalid("paged plan page_size must be a power of two from 8 to 256");
+    if (batch > 65535 || max_pages * r.page_size > INT_MAX - 65536 || ring->desc.dims[0] * static_cast<uint64_t>(r.page_size) > INT_MAX)
+        return invalid("paged plan is too large");
+    const Buffer* out[] = {table, ring, nheld, nstate, off, row[0], row[1], row[2]};
+    const Buffer* in[] = {len, count, held, state, seen};
+    for (int i = 0; i < 8; ++i) {
+        if (!out[i]) continue;
+        for (int j = 0; j < i; ++j)
+            if (out[j] && overlap(out[i], out[j])) return invalid("paged plan buffers overlap");
+        for (const Buffer* b : in) {
+            if (!b || !overlap(out[i], b)) continue;
+            if ((i == 2 && b == held && same(nheld, b)) || (i == 3 && b == state && same(nstate, b))) continue;
+            return invalid("paged plan buffers overlap");
+        }
+    }
+    const auto words = [](const Buffer* b) { return b ? static_cast<int32_t*>(b->ptr) : nullptr; };
+    fer_paged_plan_args_t a{};
+    a.page_table = words(table);
+    a.lengths = words(len);
+    a.counts = words(count);
+    a.held = words(held);
+    a.seen = words(seen);
+    a.free_pages = words(ring);
+    a.free_state = words(state);
+    a.new_held = words(nheld);
+    a.new_free_state = words(nstate);
+    a.offsets = words(off);
+    a.sequences = words(row[0]);
+    a.positions = words(row[1]);
+    a.slots = words(row[2]);
+    a.batch = static_cast<int>(batch);
+    a.max_pages = static_cast<int>(max_pages);
+    a.pages = static_cast<int>(ring->desc.dims[0]);
+    a.page_size = static_cast<int>(r.page_size);
+    a.rows = static_cast<int>(rows);
+    if (capturing(S)) return invalid(kCapturing);
+    return finish(S, fer_paged_plan(&a, S.dev_err, S.stream), out_job_id);
 }
 
 fer_status_t submit_store(Session& S, const fer_paged_store_request_t& r, uint64_t* out_job_id) {
@@ -326,6 +493,134 @@ fer_status_t submit_attention(Session& S, const fer_paged_attention_request_t& r
     return finish(S, fer_paged_attention(&c.view, &a, S.dev_err, S.stream), out_job_id);
 }
 
+// What the attention operators ask of queries and outputs: dtype, rows, columns, lse and scale; q and out as columns.
+fer_status_t open_rows(const Cache& c, const Buffer* q, const Buffer* o, const Buffer* lse, uint32_t heads, uint32_t q_col,
+                       uint32_t out_col, float scale, Cols* cq, Cols* co) {
+    if (q->desc.dtype != c.view.dtype || o->desc.dtype != c.view.dtype)
+        return invalid("paged attention requires q and out of the cache's dtype");
+    if (q->desc.rank != 2 || o->desc.rank != 2 || q->desc.dims[0] != o->desc.dims[0] || q->desc.dims[0] > INT_MAX)
+        return invalid("paged attention requires rank-2 q and out of the same rows");
+    if (heads == 0 || heads % static_cast<uint32_t>(c.view.kv_heads) || heads > 65536)
+        return invalid("paged attention heads must be a multiple of kv_heads, at most 65536");
+    if (!(scale >= 0.0f) || scale > 2.0e38f) return invalid("paged attention scale must be from 0 to 2e38");
+    const uint64_t width = static_cast<uint64_t>(heads) * c.view.head_dim;
+    *cq = Cols{q, q_col, width};
+    *co = Cols{o, out_col, width};
+    if (!cq->fits() || !co->fits()) return invalid("paged attention heads reach past the columns");
+    if (lse && !(lse->desc.dtype == FER_DTYPE_F32 && lse->desc.rank == 2 && lse->desc.dims[0] == q->desc.dims[0] &&
+                 lse->desc.dims[1] == heads))
+        return invalid("paged attention lse must be f32 [rows, heads]");
+    if (overlap(*cq, *co)) return invalid("paged attention q and out overlap");
+    return ok();
+}
+
+// A workspace of `need` bytes, and what is written (out, lse, it) apart from one another and from all that is read.
+fer_status_t check_written(const Cache& c, const Buffer* q, const Buffer* o, const Buffer* lse, const Buffer* ws, uint64_t need,
+                           std::initializer_list<const Buffer*> in) {
+    if (ws->desc.dtype != FER_DTYPE_U8) return invalid("workspace must be a u8 buffer");
+    if (ws->bytes < need || reinterpret_cast<uintptr_t>(ws->ptr) % 16)
+        return invalid("workspace is too small or not 16-byte aligned");
+    const Buffer* out[] = {o, lse, ws};
+    for (int i = 0; i < 3; ++i) {
+        if (!out[i]) continue;
+        if (c.touches(out[i]) || (i > 0 && overlap(out[i], q))) return invalid("paged attention buffers overlap");
+        for (const Buffer* b : in)
+            if (b && overlap(out[i], b)) return invalid("paged attention buffers overlap");
+        for (int j = 0; j < i; ++j)
+            if (out[j] && overlap(out[i], out[j])) return invalid("paged attention buffers overlap");
+    }
+    return ok();
+}
+
+fer_status_t submit_window(Session& S, const fer_paged_window_attention_request_t& r, uint64_t* out_job_id) {
+    Cache c;
+    fer_status_t st = open_cache(S, r.cache, &c);
+    if (st.code != FER_STATUS_OK) return st;
+    const Buffer* q = S.find(r.q);
+    const Buffer* o = S.find(r.out);
+    const Buffer* ws = S.find(r.workspace);
+    const Buffer *lse, *off;
+    if (!q || !o || !ws || !find_optional(S, r.lse, &lse) || !find_optional(S, r.offsets, &off))
+        return not_found("buffer id not found");
+    Cols cq, co;
+    st = open_rows(c, q, o, lse, r.heads, r.q_col, r.out_col, r.scale, &cq, &co);
+    if (st.code != FER_STATUS_OK) return st;
+    const uint64_t rows = q->desc.dims[0];
+    uint64_t n_seq = rows;
+    if (off) {
+        if (off->desc.dtype != FER_DTYPE_I32 || off->desc.rank != 1 || off->desc.dims[0] < 2)
+            return invalid("paged window attention requires i32 offsets [sequences + 1]");
+        n_seq = off->desc.dims[0] - 1;
+    }
+    if (n_seq > static_cast<uint64_t>(c.view.batch)) return invalid("paged window attention has more sequences than the cache");
+    if (r.window > INT_MAX || r.sinks > INT_MAX) return invalid("paged window attention window and sinks must be below 2^31");
+    fer_paged_window_args_t a{};
+    a.q = cq.at();
+    a.out = co.at();
+    a.q_stride = q->desc.dims[1];
+    a.out_stride = o->desc.dims[1];
+    a.rows = static_cast<int>(rows);
+    a.n_seq = static_cast<int>(n_seq);
+    a.heads = static_cast<int>(r.heads);
+    a.offsets = off ? static_cast<const int32_t*>(off->ptr) : nullptr;
+    a.window = static_cast<int>(r.window);
+    a.sinks = static_cast<int>(r.sinks);
+    a.scale = r.scale;
+    a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
+    a.workspace = ws->ptr;
+    a.workspace_bytes = ws->bytes;
+    st = check_written(c, q, o, lse, ws,
+                       fer_paged_window_attention_workspace_bytes(a.rows, a.n_seq, a.heads, c.view.kv_heads, c.view.head_dim,
+                                                                  static_cast<int>(c.max_slots), a.window, a.sinks),
+                       {off});
+    if (st.code != FER_STATUS_OK) return st;
+    if (capturing(S)) return invalid(kCapturing);
+    return finish(S, fer_paged_window_attention(&c.view, &a, S.dev_err, S.stream), out_job_id);
+}
+
+fer_status_t submit_prefix(Session& S, const fer_paged_prefix_attention_request_t& r, uint64_t* out_job_id) {
+    Cache c;
+    fer_status_t st = open_cache(S, r.cache, &c);
+    if (st.code != FER_STATUS_OK) return st;
+    const Buffer* q = S.find(r.q);
+    const Buffer* o = S.find(r.out);
+    const Buffer* ws = S.find(r.workspace);
+    const Buffer* pages = S.find(r.prefix_pages);
+    const Buffer* length = S.find(r.prefix_length);
+    const Buffer* lse;
+    if (!q || !o || !ws || !pages || !length || !find_optional(S, r.lse, &lse)) return not_found("buffer id not found");
+    Cols cq, co;
+    st = open_rows(c, q, o, lse, r.heads, r.q_col, r.out_col, r.scale, &cq, &co);
+    if (st.code != FER_STATUS_OK) return st;
+    if (q->desc.dims[0] > static_cast<uint64_t>(c.view.batch)) return invalid("paged attention has more rows than the cache");
+    if (pages->desc.dtype != FER_DTYPE_I32 || pages->desc.rank != 1 ||
+        static_cast<uint64_t>(pages->desc.dims[0]) * c.view.page_size > INT_MAX - 65536)
+        return invalid("paged prefix attention requires i32 prefix_pages [pages] of less than 2^31 slots");
+    if (!is_vector(length, FER_DTYPE_I32, 1)) return invalid("paged prefix attention requires i32 prefix_length [1]");
+    fer_paged_prefix_args_t a{};
+    a.q = cq.at();
+    a.out = co.at();
+    a.q_stride = q->desc.dims[1];
+    a.out_stride = o->desc.dims[1];
+    a.n_seq = static_cast<int>(q->desc.dims[0]);
+    a.heads = static_cast<int>(r.heads);
+    a.prefix_pages = static_cast<const int32_t*>(pages->ptr);
+    a.prefix_length = static_cast<const int32_t*>(length->ptr);
+    a.max_prefix_pages = static_cast<int>(pages->desc.dims[0]);
+    a.scale = r.scale;
+    a.lse = lse ? static_cast<float*>(lse->ptr) : nullptr;
+    a.workspace = ws->ptr;
+    a.workspace_bytes = ws->bytes;
+    st = check_written(c, q, o, lse, ws,
+                       fer_paged_prefix_attention_workspace_bytes(a.n_seq, a.heads, c.view.kv_heads, c.view.head_dim,
+                                                                  static_cast<int>(c.max_slots),
+                                                                  a.max_prefix_pages * c.view.page_size),
+                       {pages, length});
+    if (st.code != FER_STATUS_OK) return st;
+    if (capturing(S)) return invalid(kCapturing);
+    return finish(S, fer_paged_prefix_attention(&c.view, &a, S.dev_err, S.stream), out_job_id);
+}
+
 fer_status_t submit_evict(Session& S, const fer_paged_evict_request_t& r, uint64_t* out_job_id) {
     Cache c;
     const fer_status_t st = open_cache(S, r.cache, &c);
@@ -419,6 +714,26 @@ fer_status_t fer_submit_paged_attention(fer_session_t* session, const fer_paged_
 fer_status_t fer_submit_paged_evict(fer_session_t* session, const fer_paged_evict_request_t* req,
                                     uint64_t* out_job_id) {
     return entry(session, req, out_job_id, submit_evict);
+}
+
+fer_status_t fer_submit_norm_rotary(fer_session_t* session, const fer_norm_rotary_request_t* req, uint64_t* out_job_id) {
+    return entry(session, req, out_job_id, submit_norm_rotary);
+}
+
+fer_status_t fer_submit_norm_rotary_grad(fer_session_t* session, const fer_norm_rotary_grad_request_t* req, uint64_t* out_job_id) {
+    return entry(session, req, out_job_id, submit_norm_rotary_grad);
+}
+
+fer_status_t fer_submit_paged_plan(fer_session_t* session, const fer_paged_plan_request_t* req, uint64_t* out_job_id) {
+    return entry(session, req, out_job_id, submit_plan);
+}
+
+fer_status_t fer_submit_paged_window_attention(fer_session_t* session, const fer_paged_window_attention_request_t* req, uint64_t* out_job_id) {
+    return entry(session, req, out_job_id, submit_window);
+}
+
+fer_status_t fer_submit_paged_prefix_attention(fer_session_t* session, const fer_paged_prefix_attention_request_t* req, uint64_t* out_job_id) {
+    return entry(session, req, out_job_id, submit_prefix);
 }
 
 }  // extern "C"

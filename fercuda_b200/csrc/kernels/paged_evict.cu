@@ -628,28 +628,6 @@ int most_moves(int max_slots, int budget) {
 
 size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
 
-// As launch_pdl, in clusters of `cluster` CTAs along x.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, unsigned cluster, cudaStream_t s,
-                           Args&&... args) {
-    if (cluster == 1) return fer::host::launch_pdl(kern, grid, block, smem, s, std::forward<Args>(args)...);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = fer::host::pdl_enabled() ? 2 : 1;
-    fer_pdl_note_launch();   // the kernel triggers its dependents either way
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-
 template <int D, int KEYS>
 cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t s) {
     // two heads a CTA, up to eight CTAs a sequence
@@ -657,7 +635,7 @@ cudaError_t small(const Paged& c, const EvictParams& p, int batch, cudaStream_t 
     while (ctas < 8 && 4 * ctas <= static_cast<unsigned>(c.kv_heads)) ctas *= 2;
     const int warps = (c.kv_heads + ctas - 1) / ctas < 8 ? (c.kv_heads + ctas - 1) / ctas : 8;
     const unsigned cluster = p.new_lengths == c.lengths ? ctas : 1;
-    return launch_cluster(evict_small<D, KEYS>, dim3(ctas, batch), dim3(32 * warps), 0, cluster, s, c, p);
+    return fer::host::launch_pdl_cluster(evict_small<D, KEYS>, dim3(ctas, batch), dim3(32 * warps), 0, cluster, s, c, p);
 }
 
 template <int D, bool HELD, int THREADS>
@@ -677,7 +655,7 @@ cudaError_t select(const Paged& c, const EvictParams& p, unsigned ctas, int batc
             if (dev < fer::host::kMaxDevices) set[dev].store(true, std::memory_order_relaxed);
         }
     }
-    return launch_cluster(kernel, dim3(ctas, c.kv_heads, batch), dim3(THREADS), smem, ctas, s, c, p);
+    return fer::host::launch_pdl_cluster(kernel, dim3(ctas, c.kv_heads, batch), dim3(THREADS), smem, ctas, s, c, p);
 }
 
 template <int D>

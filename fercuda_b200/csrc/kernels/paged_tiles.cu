@@ -1,0 +1,1225 @@
+// Attention over a paged key-value cache in tensor-core tiles: rows of prompts or
+// single tokens with a sliding window and sinks, and a batch of single tokens
+// behind a prefix that all of them share.
+//
+// A row is one query head of one token. The rows that read the same keys, those
+// of one key head, lie side by side: token by token, each with its group of
+// query heads. A unit of work is up to 256 rows (two sub-tiles of 128, the
+// lanes of tensor memory; one of 128 where head_dim is 256) and a range of key
+// blocks. Per block S = Q K^T, P = 2^(scale S - m) and O += P V; a row's m, l = sum
+// P and O stay on chip for the whole range: 4 flops a row, slot and dim, and
+// each key and value is read once a unit. 256 rows a unit are 256 flops a byte
+// of keys and values, which is what the GPU's tensor rate needs of its HBM rate.
+//
+// Warps. One loads keys and values by tensor copies of page rows into a ring of
+// tiles, running on into the next units. One issues the products: S_x for
+// sub-tile x as soon as P_x V of the block before is issued, so that the tensor
+// cores work on one sub-tile while four warps take the other's softmax, a row a
+// thread. P replaces S in tensor memory and is the left operand from there. The
+// maximum a row subtracts is raised only when a block's exceeds it by 2^kSlack
+// (softmax does not depend on it), so O is seldom rescaled. Where a unit has at
+// most 128 rows, the two sub-tiles are the same rows with every other key block
+// each, added up at the end: single tokens keep both in flight and are bound by
+// HBM.
+//
+// P is rounded to 16 bits once, by half a step of the type at most, and l sums it
+// unrounded; where rows are few (kFine) what rounding leaves is multiplied as a
+// second operand, as the tensor cores wait for memory there anyway.
+//
+// Units are numbered from the lengths on the device, and CTA i of G takes i, 2G -
+// 1 - i, 2G + i, ...: prompts' units come longest first. Which CTA takes a unit
+// does not change its arithmetic. Where rows are few for the GPU a row's keys
+// are cut into several units, whose m, l and O go to the workspace in f32, and
+// a second kernel adds them in order; cuts are a function of the call's sizes.
+//
+// Slots that no row of a unit sees are zeroed in the value tile, and pages without
+// a visible slot are not looked up. A result that is NaN (an infinite value of
+// a slot that some rows of the tile see and others do not makes 0 x inf) is
+// computed again row by row over what the row sees.
+#include "f32x2.cuh"
+#include "paged.cuh"
+#include "pdl.cuh"
+#include "tmap.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+#include <climits>
+#include <cstdint>
+
+namespace {
+
+using fer::dev::Paged;
+
+constexpr int kSms = 148;
+constexpr int kSegments = 256;       // entries of the unit table
+constexpr int kUnitSlots = 3;        // units handed from the loading warp to the others
+constexpr int kBadRing = 16;         // key blocks whose flag is kept
+constexpr int kJoinWarps = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kMostScale = 2.0e38f;   // times log2 e it is still finite
+constexpr float kSlack = 7.0f;          // log2 units the subtracted maximum may lag
+
+// Sizes of a head_dim: keys a block, sub-tiles of rows, tiles of the ring.
+template <int D> struct Cut {
+    static constexpr int kKeys = D == 256 ? 64 : 128;
+    static constexpr int kSubs = D == 256 ? 1 : 2;
+    static constexpr int kRows = 128 * kSubs;
+    static constexpr int kBands = D / 64;
+    static constexpr int kTile = kKeys * D * 2;
+    static constexpr int kBand = kKeys * 128;        // 64 dims of a tile's keys
+    static constexpr int kStages = D == 64 ? 8 : 5;
+    static constexpr int kQ = 128 * D * 2;           // queries of a sub-tile
+    static constexpr int kSoft = 4 * kSubs;          // softmax warps
+    static constexpr int kThreads = 32 * (kSoft + 2);
+    static constexpr int kSmem = kSubs * kQ + kStages * kTile + 1024;
+    static constexpr uint32_t kColO = 256;           // O of sub-tile x at kColO + x D, S and P at 128 x
+    // rows up to which P's rounding is made up for
+    static constexpr int kFine = kSubs == 2 ? 128 : 64;
+};
+
+struct TileParams {
+    const void* q;
+    void* out;
+    size_t qs, os;
+    float* lse;
+    const int32_t* offsets;        // null: row b is sequence b's latest slot
+    int n_seq, rows, heads, group;
+    int window, sinks;             // INT_MAX: no window
+    float scale2;                  // scale * log2 e
+    int chunk;                     // key blocks a unit
+    int parts;                     // parts a row may have; 0: results go to out
+    float* part_ml;                // [rows * heads][parts][2]
+    float* part_o;                 // [rows * heads][parts][head_dim]
+    const int32_t* prefix_pages;   // null: no prefix
+    const int32_t* prefix_length;
+    int prefix_max, prefix_chunk, own_parts;
+    uint32_t* err;
+};
+
+// Some rows of one sequence (or of the whole batch, before the prefix), one key
+// head and a range of key blocks.
+struct Unit {
+    int tok0;          // row of q of the first token; < 0: no more units
+    int f0, nf;        // rows: token (f0 + i) / group, head hk * group + (f0 + i) % group
+    int hk, seq;       // seq -1: the prefix
+    int slot0;         // the first token's slot
+    int hi, lo, sink;  // visible to some row: slots below hi that are below sink or not below lo
+    int sb, wb0;       // key blocks: 0 .. sb - 1, then wb0 ..
+    int c0, c1;        // of them, counted in that order, the unit's
+    int part;          // -1: the only one of its rows
+};
+
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+struct Seq {
+    int len, n, tok0;
+    bool bad, broken;   // its length, its rows out of range
+    __device__ __forceinline__ Seq(const Paged& c, const TileParams& p, int b) {
+        len = c.length(b, &bad);
+        tok0 = b;
+        n = 1;
+        broken = false;
+        if (p.offsets) {
+            const int lo = p.offsets[b], hi = p.offsets[b + 1];
+            tok0 = min(max(lo, 0), p.rows);
+            n = min(max(hi, tok0), p.rows) - tok0;
+            broken = tok0 != lo || tok0 + n != hi;
+        }
+    }
+    __device__ __forceinline__ int tiles(const TileParams& p, int rows) const {
+        return static_cast<int>((static_cast<long long>(n) * p.group + rows - 1) / rows);
+    }
+};
+
+// The visible range and the key blocks of tile i of a sequence; returns how many blocks.
+template <int D>
+__device__ __forceinline__ int tile_range(const TileParams& p, const Seq& q, int i, Unit& u) {
+    using C = Cut<D>;
+    u.tok0 = q.tok0;
+    u.f0 = i * C::kRows;
+    u.nf = static_cast<int>(min(static_cast<long long>(C::kRows), static_cast<long long>(q.n) * p.group - u.f0));
+    u.slot0 = q.len - q.n;
+    const int first = u.slot0 + u.f0 / p.group, last = u.slot0 + (u.f0 + u.nf - 1) / p.group;
+    u.hi = max(last + 1, 0);
+    u.lo = p.window == INT_MAX ? 0 : max(first + 1 - p.window, 0);
+    u.sink = min(p.sinks, u.hi);
+    const int end = (u.hi + C::kKeys - 1) / C::kKeys;
+    u.wb0 = min(u.lo / C::kKeys, end);
+    u.sb = min((u.sink + C::kKeys - 1) / C::kKeys, u.wb0);
+    return u.sb + end - u.wb0;
+}
+
+__device__ __forceinline__ int chunks_of(int blocks, int chunk) { return blocks <= chunk ? 1 : (blocks - 1) / chunk + 1; }
+
+// Units of one key head of a sequence.
+template <int D>
+__device__ __forceinline__ int units_of(const TileParams& p, const Seq& q) {
+    const int tiles = q.tiles(p, Cut<D>::kRows);
+    if (p.parts == 0) return tiles;
+    int n = 0;
+    for (int i = 0; i < tiles; ++i) {
+        Unit u;
+        n += chunks_of(tile_range<D>(p, q, i, u), p.chunk);
+    }
+    return n;
+}
+
+// What the prefix is cut into.
+template <int D>
+struct Prefix {
+    int len = 0, tiles = 0, chunks = 0;
+    bool bad = false;
+    __device__ __forceinline__ Prefix(const Paged& c, const TileParams& p) {
+        if (!p.prefix_pages) return;
+        const int n = p.prefix_length[0], most = p.prefix_max << c.shift;
+        bad = n < 0 || n > most;
+        len = min(max(n, 0), most);
+        tiles = static_cast<int>((static_cast<long long>(p.n_seq) * p.group + Cut<D>::kRows - 1) / Cut<D>::kRows);
+        chunks = len > 0 ? chunks_of((len - 1) / Cut<D>::kKeys + 1, p.prefix_chunk) : 0;
+    }
+    __device__ __forceinline__ int units(const Paged& c) const { return c.kv_heads * tiles * chunks; }
+};
+
+// Unit x of the call; s_units: units before every segment of seg sequences.
+template <int D>
+__device__ __forceinline__ Unit find_unit(const Paged& c, const TileParams& p, const Prefix<D>& pre, const int* s_units,
+                                          int segments, int seg, int x) {
+    using C = Cut<D>;
+    Unit u{};
+    if (x < pre.units(c)) {
+        // tiles that read the same keys next to one another
+        const int t = x % pre.tiles, rest = x / pre.tiles, k = rest % pre.chunks;
+        u.hk = rest / pre.chunks;
+        u.seq = -1;
+        u.f0 = t * C::kRows;
+        u.nf = static_cast<int>(min(static_cast<long long>(C::kRows), static_cast<long long>(p.n_seq) * p.group - u.f0));
+        u.hi = pre.len;
+        const int blocks = (pre.len - 1) / C::kKeys + 1;
+        u.c0 = k * p.prefix_chunk;
+        u.c1 = min(blocks, u.c0 + p.prefix_chunk);
+        u.part = p.own_parts + k;
+        return u;
+    }
+    x -= pre.units(c);
+    int lo = 0, hi = segments;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_units[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    x -= s_units[lo];
+    int b = lo * seg;
+    Seq q(c, p, b);
+    int each = units_of<D>(p, q);
+    while (x >= each * c.kv_heads && b + 1 < p.n_seq) {
+        x -= each * c.kv_heads;
+        q = Seq(c, p, ++b);
+        each = units_of<D>(p, q);
+    }
+    u.seq = b;
+    u.hk = x / each;
+    x -= u.hk * each;
+    const int tiles = q.tiles(p, C::kRows);
+    int i = tiles - 1;   // the last tile sees most
+    int blocks;
+    if (p.parts == 0) {
+        i -= x;
+        blocks = tile_range<D>(p, q, i, u);
+        u.c1 = blocks;
+        u.part = -1;
+        return u;
+    }
+    for (;; --i) {
+        blocks = tile_range<D>(p, q, i, u);
+        const int n = chunks_of(blocks, p.chunk);
+        if (x < n || i == 0) {
+            u.c0 = x * p.chunk;
+            u.c1 = min(blocks, u.c0 + p.chunk);
+            u.part = n == 1 && !p.prefix_pages ? -1 : x;
+            return u;
+        }
+        x -= n;
+    }
+}
+
+__device__ __forceinline__ int block_of(const Unit& u, int i) { return i < u.sb ? i : u.wb0 + (i - u.sb); }
+// How a unit's blocks are shared: every other one to each sub-tile, or all to both.
+template <int D>
+__device__ __forceinline__ bool alternate(const Unit& u) { return Cut<D>::kSubs == 2 && u.nf <= 128; }
+
+// Place in the ring, from the unit's first, of a block's keys and of its values: K_0 V_0 K_1 V_1 ..., or where blocks
+// alternate K_0 K_1 V_0 K_2 V_1 ...
+__device__ __forceinline__ int at_k(bool alt, int i) { return alt && i > 0 ? 2 * i - 1 : 2 * i; }
+__device__ __forceinline__ int at_v(bool alt, int i, int nb) { return alt ? min(2 * i + 2, nb + i) : 2 * i + 1; }
+
+template <int STAGES>
+struct Shared {
+    uint64_t full[STAGES], empty[STAGES];
+    uint64_t unit_full[kUnitSlots], unit_empty[kUnitSlots];
+    uint64_t q_full, s_full[2], p_full[2], o_full[2];
+    Unit unit[kUnitSlots];
+    int bad[kBadRing];
+    int units[kSegments], sum[12];
+    float ml[2][128][2];
+    uint32_t tmem;
+    int stop, leave;
+};
+
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int r, int head, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r), "r"(head), "r"(page), "r"(fer::dev::smem_addr(bar))
+        : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle.
+__device__ __forceinline__ uint64_t sdesc(uint32_t at, uint32_t lbo, uint32_t sbo) {
+    return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 |
+           static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32 | 1ull << 46 | 2ull << 61;
+}
+// kind::f16, f32 sums, M = 128: N, type of both operands, and whether B has N as its contiguous dimension.
+__host__ __device__ constexpr uint32_t idesc(int n, bool bf16, bool b_by_n) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_by_n ? 1u << 16 : 0u) | (static_cast<uint32_t>(n) >> 3) << 17 |
+           (128u >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(fer::dev::smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of this thread's lane of tensor memory; the wait is in the statement, so no use can come before it.
+__device__ __forceinline__ void tmem_ld(uint32_t at, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at)
+        : "memory");
+}
+// 16 columns; completed by wait_st
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t u;
+    if constexpr (__is_same(T, __half)) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+    return u;
+}
+template <typename T>
+__device__ __forceinline__ void unpack2(uint32_t u, float& lo, float& hi) {
+    if constexpr (__is_same(T, __half)) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&u));
+        lo = v.x, hi = v.y;
+    } else {
+        lo = __uint_as_float(u << 16), hi = __uint_as_float(u & 0xffff0000u);
+    }
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, fer::dev::mbar_wait(bar, parity & 1u));
+}
+template <int N>
+__device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
+
+// The bits below n, all or none of them where n is past the ends.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Whether some row of a unit sees a slot of the page.
+__device__ __forceinline__ bool page_needed(const Paged& c, const Unit& u, int page) {
+    const int first = page << c.shift, last = first + c.page_size() - 1;
+    return first < u.hi && (last >= u.lo || first < u.sink);
+}
+__device__ __forceinline__ const int32_t* table_of(const Paged& c, const TileParams& p, const Unit& u) {
+    return u.seq < 0 ? p.prefix_pages : c.table + static_cast<size_t>(u.seq) * c.max_pages;
+}
+// A row's slots: below end, and below sink or not below begin.
+struct Sees {
+    int begin, end, sink;
+    __device__ __forceinline__ Sees(const TileParams& p, const Unit& u, int f) {
+        end = u.seq < 0 ? u.hi : u.slot0 + (u.f0 + f) / p.group + 1;
+        begin = p.window == INT_MAX || u.seq < 0 ? 0 : max(end - p.window, 0);
+        sink = p.sinks;
+    }
+    __device__ __forceinline__ bool operator()(int s) const { return s < end && (s >= begin || s < sink); }
+};
+__device__ __forceinline__ size_t q_row(const TileParams& p, const Unit& u, int f) {
+    return static_cast<size_t>(u.tok0) + (u.f0 + f) / p.group;
+}
+__device__ __forceinline__ int q_head(const TileParams& p, const Unit& u, int f) { return u.hk * p.group + (u.f0 + f) % p.group; }
+
+template <typename T>
+__device__ __forceinline__ void put(T* to, float v) { *to = static_cast<T>(v); }
+
+// One row over its slots of the unit's blocks, by a warp: m, l and this lane's dims (every 32nd) of O. A probability that
+// vanishes counts as the smallest number, so that it gives an infinite value its due.
+template <typename T, int D>
+__device__ __noinline__ void one_row(const Paged& c, const TileParams& p, const Unit& u, int f, float& m, float& l,
+                                     float (&o)[D / 32]) {
+    const int lane = threadIdx.x & 31;
+    const T* const q = static_cast<const T*>(p.q) + q_row(p, u, f) * p.qs + static_cast<size_t>(q_head(p, u, f)) * D;
+    const int32_t* const table = table_of(c, p, u);
+    const Sees sees(p, u, f);
+    m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.0f;
+    for (int k = u.c0; k < u.c1; ++k) {
+        const int s0 = block_of(u, k) * Cut<D>::kKeys;
+        for (int s = s0; s < s0 + Cut<D>::kKeys; ++s) {
+            if (!sees(s)) continue;
+            const int id = table[s >> c.shift];
+            if (!c.is_page(id)) continue;
+            const size_t at = c.row(id, u.hk, s);
+            float dot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+                dot = fmaf(static_cast<float>(q[i * 32 + lane]), static_cast<float>(static_cast<const T*>(c.k)[at + i * 32 + lane]), dot);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
+            dot *= p.scale2;
+            if (dot == -INFINITY) continue;
+            const float top = fmaxf(m, dot), base = top == -INFINITY ? 0.0f : top;
+            const float a = fmaxf(ex2(m - base), 1.17549435e-38f);
+            float w = ex2(dot - base);
+            if (w < 1.17549435e-38f) w = 1.17549435e-38f;   // NaN stays
+            m = top;
+            l = l * a + w;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+                o[i] = o[i] * a + w * static_cast<float>(static_cast<const T*>(c.v)[at + i * 32 + lane]);
+        }
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Cut<D>::kThreads, 1)
+    attn_tiles(const Paged c, const TileParams p, const __grid_constant__ CUtensorMap k_map,
+               const __grid_constant__ CUtensorMap v_map) {
+    using C = Cut<D>;
+    constexpr bool kBf16 = !__is_same(T, __half);
+    constexpr uint32_t kIdS = idesc(C::kKeys, kBf16, false), kIdO = idesc(D, kBf16, true);
+    // P is 2^(s - m + kUp): 16-bit floats of 5 exponent bits keep small ones so; with kSlack it stays below 2^15
+    constexpr float kUp = kBf16 ? 0.0f : 8.0f;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Shared<C::kStages> sh;
+    const uint32_t smem = (fer::dev::smem_addr(smem_raw) + 1023u) & ~1023u, ring = smem + C::kSubs * C::kQ;
+    uint8_t* const smem_at = smem_raw + (smem - fer::dev::smem_addr(smem_raw));
+    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+
+    if (t == 0) {
+        for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&sh.full[i], 1), fer::dev::mbar_init(&sh.empty[i], 1);
+        for (int i = 0; i < kUnitSlots; ++i)
+            fer::dev::mbar_init(&sh.unit_full[i], 1), fer::dev::mbar_init(&sh.unit_empty[i], C::kSoft + 1);
+        fer::dev::mbar_init(&sh.q_full, C::kSoft);
+        for (int i = 0; i < 2; ++i)
+            fer::dev::mbar_init(&sh.s_full[i], 1), fer::dev::mbar_init(&sh.p_full[i], 4), fer::dev::mbar_init(&sh.o_full[i], 1);
+        sh.stop = 0;
+        fer::dev::fence_mbar_init();
+        fer::dev::prefetch_tmap(&k_map);
+        fer::dev::prefetch_tmap(&v_map);
+    }
+    if (w == C::kSoft + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fer::dev::smem_addr(&sh.tmem)),
+                     "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fer::dev::pdl_begin();
+
+    // units before every segment of sequences
+    const Prefix<D> pre(c, p);
+    const int seg = (p.n_seq + kSegments - 1) / kSegments, segments = (p.n_seq + seg - 1) / seg;
+    {
+        int mine[(kSegments + C::kThreads - 1) / C::kThreads] = {};
+        bool bad = pre.bad, broken = false;
+        int carry = 0;
+        for (int k = 0, s0 = 0; s0 < segments; ++k, s0 += C::kThreads) {
+            const int s = s0 + t;
+            int n = 0;
+            if (s < segments)
+                for (int b = s * seg; b < min(p.n_seq, (s + 1) * seg); ++b) {
+                    const Seq q(c, p, b);
+                    bad = bad || q.bad;
+                    broken = broken || q.broken;
+                    if (!q.broken) n += units_of<D>(p, q) * c.kv_heads;
+                }
+            mine[k] = n;
+            int x = n;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, off);
+                if (lane >= off) x += y;
+            }
+            if (lane == 31) sh.sum[w] = x;
+            __syncthreads();
+            x += carry - n;
+            for (int i = 0; i < C::kThreads / 32; ++i) {
+                if (i < w) x += sh.sum[i];
+                carry += sh.sum[i];
+            }
+            if (s < segments) sh.units[s] = x;
+            __syncthreads();
+        }
+        // with offsets that cannot be nothing is done
+        broken = __syncthreads_or(broken);
+        if (t == 0) sh.sum[0] = broken ? 0 : carry;
+        if ((bad || broken) && blockIdx.x == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const int units = sh.sum[0] + pre.units(c), grid = static_cast<int>(gridDim.x);
+    const uint32_t tmem = sh.tmem;
+    volatile int* const stop = &sh.stop;
+    bool ok = true;
+
+    if (w == C::kSoft) {
+        // ---- units, and their keys and values. Pages of a block: one a lane.
+        const int box_rows = min(C::kKeys, c.page_size()), pages = C::kKeys / box_rows, boxes = pages * C::kBands;
+        uint32_t tile = 0, block = 0;   // so far
+        for (int k = 0; ok; ++k) {
+            const int slot = k % kUnitSlots;
+            ok = warp_wait(&sh.unit_empty[slot], (k / kUnitSlots & 1) ^ 1);
+            if (!ok || fer::dev::warp_flag(stop)) break;
+            const long long x = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
+            Unit u{};
+            u.tok0 = -1;
+            if (x < units) u = find_unit<D>(c, p, pre, sh.units, segments, seg, static_cast<int>(x));
+            if (lane == 0) {
+                sh.unit[slot] = u;
+                fer::dev::mbar_arrive(&sh.unit_full[slot]);
+            }
+            __syncwarp();
+            if (u.tok0 < 0) break;   // a later round has none either
+            const int32_t* const table = table_of(c, p, u);
+            const int nb = u.c1 - u.c0, lead = alternate<D>(u) ? 2 : 1;
+            // this lane's page of block i: -1 where there is none to read, -2 where its id is out of range
+            const auto page_at = [&](int i) {
+                if (i >= nb || lane >= pages) return -1;
+                const int page = ((block_of(u, u.c0 + i) * C::kKeys) >> c.shift) + lane;
+                if (!page_needed(c, u, page)) return -1;
+                const int id = table[page];
+                return c.is_page(id) ? id : -2;
+            };
+            const auto load = [&](int i, int mine, bool value) {
+                const int st = tile % C::kStages;
+                if (ok) ok = warp_wait(&sh.empty[st], (tile / C::kStages & 1) ^ 1);
+                if (!ok) return;
+                const bool bad = __any_sync(0xffffffffu, mine == -2);
+                if (lane == 0) {
+                    if (!value) {
+                        sh.bad[block % kBadRing] = bad;
+                        if (bad) fer::dev::report(p.err, fer::dev::kErrBadShape);
+                    }
+                    fer::dev::mbar_arrive_expect_tx(&sh.full[st], C::kTile);
+                }
+                __syncwarp();
+                const int s0 = block_of(u, u.c0 + i) * C::kKeys;
+                for (int j0 = 0; j0 < boxes; j0 += 32) {
+                    const int j = j0 + lane, pg = j / C::kBands, band = j % C::kBands;
+                    const int id = __shfl_sync(0xffffffffu, mine, pg & 31);
+                    // slots of no page are read as page `pages`, outside the map: zeros
+                    if (j < boxes)
+                        load_box(ring + st * C::kTile + band * C::kBand + pg * box_rows * 128, value ? &v_map : &k_map,
+                                 band * 64, s0 & (c.page_size() - 1), u.hk, id < 0 ? c.pages : id, &sh.full[st]);
+                }
+                ++tile;
+                if (!value) ++block;
+            };
+            // ids of four blocks: i .. i + 3 when values i are loaded
+            int id0 = page_at(0), id1 = page_at(1), id2 = page_at(2);
+            if (nb > 0) load(0, id0, false);
+            if (lead == 2 && nb > 1) load(1, id1, false);
+            for (int i = 0; i < nb && ok; ++i) {
+                const int id3 = page_at(i + 3);
+                load(i, id0, true);
+                if (i + lead < nb) load(i + lead, lead == 2 ? id2 : id1, false);
+                id0 = id1, id1 = id2, id2 = id3;
+            }
+        }
+        if (!ok) {
+            if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutSync);
+            *stop = 1;
+        }
+        // the copies have landed before this warp leaves, whatever became of the others
+        for (uint32_t i = tile > C::kStages ? tile - C::kStages : 0; i < tile; ++i)
+            if (!warp_wait(&sh.full[i % C::kStages], i / C::kStages)) {
+                if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
+                *stop = 1;
+            }
+    } else if (w == C::kSoft + 1) {
+        // ---- products
+        uint32_t base = 0;                 // tiles of the units before
+        uint32_t n_q = 0, n_p[2] = {0, 0}; // phases so far
+        for (int k = 0; ok; ++k) {
+            const int slot = k % kUnitSlots;
+            ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
+            if (!ok || fer::dev::warp_flag(stop)) break;
+            const Unit u = sh.unit[slot];
+            __syncwarp();
+            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
+            if (u.tok0 < 0) break;
+            const int nb = u.c1 - u.c0;
+            if (nb == 0) continue;
+            const bool alt = alternate<D>(u), both = C::kSubs == 2 && !alt, fine = u.nf <= C::kFine;
+            ok = warp_wait(&sh.q_full, n_q++);
+            const auto product_s = [&](int x, int i, bool last) {   // last: no other sub-tile reads the tile
+                const uint32_t at = base + at_k(alt, i);
+                const int st = at % C::kStages;
+                if (!ok || !(ok = warp_wait(&sh.full[st], at / C::kStages))) return;
+                fence_after();
+                if (lane == 0) {
+                    const uint32_t q = smem + (both ? x * C::kQ : 0), kk = ring + st * C::kTile;
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j)
+                        mma_ss(tmem + 128 * x, sdesc(q + (j / 4) * 16384 + (j % 4) * 32, 16, 1024),
+                               sdesc(kk + (j / 4) * C::kBand + (j % 4) * 32, 16, 1024), kIdS, j > 0);
+                    commit(&sh.s_full[x]);
+                    if (last) commit(&sh.empty[st]);
+                }
+                __syncwarp();
+            };
+            const auto product_o = [&](int x, int i, bool first, bool last, bool end) {
+                const uint32_t at = base + at_v(alt, i, nb);
+                const int st = at % C::kStages;
+                if (!ok || !(ok = warp_wait(&sh.p_full[x], n_p[x]++) && warp_wait(&sh.full[st], at / C::kStages))) return;
+                fence_after();
+                if (lane == 0) {
+                    const uint32_t o = tmem + C::kColO + x * D, pp = tmem + 128 * x, v = ring + st * C::kTile;
+#pragma unroll
+                    for (int j = 0; j < C::kKeys / 16; ++j)
+                        mma_ts(o, pp + 8 * j, sdesc(v + j * 2048, C::kBand, 1024), kIdO, !first || j > 0);
+                    if (fine)
+#pragma unroll
+                        for (int j = 0; j < C::kKeys / 16; ++j)
+                            mma_ts(o, pp + C::kKeys / 2 + 8 * j, sdesc(v + j * 2048, C::kBand, 1024), kIdO, 1);
+                    if (last) commit(&sh.empty[st]);
+                    if (end) commit(&sh.o_full[x]);
+                }
+                __syncwarp();
+            };
+            if (alt) {
+                product_s(0, 0, true);
+                if (nb > 1) product_s(1, 1, true);
+                for (int i = 0; i < nb && ok; ++i) {
+                    product_o(i & 1, i, i < 2, true, i + 2 >= nb);
+                    if (i + 2 < nb) product_s(i & 1, i + 2, true);
+                }
+            } else {
+                product_s(0, 0, !both);
+                if (both) product_s(1, 0, true);
+                for (int i = 0; i < nb && ok; ++i) {
+                    product_o(0, i, i == 0, !both, i + 1 == nb);
+                    if (i + 1 < nb) product_s(0, i + 1, !both);
+                    if (both) {
+                        product_o(1, i, i == 0, true, i + 1 == nb);
+                        if (i + 1 < nb) product_s(1, i + 1, true);
+                    }
+                }
+            }
+            base += 2 * nb;
+        }
+        if (!ok) {
+            if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
+            *stop = 1;
+        }
+    } else {
+        // ---- softmax, a row a thread
+        const int x = w >> 2, r = t & 127;
+        const uint32_t row_at = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16), s_at = row_at + 128 * x;
+        uint32_t base = 0, block = 0, n_s = 0, n_o = 0;
+        const bool wide_q = (reinterpret_cast<uintptr_t>(p.q) | (p.qs * 2)) % 16 == 0;
+        const bool wide_o = (reinterpret_cast<uintptr_t>(p.out) | (p.os * 2)) % 16 == 0;
+        for (int k = 0;; ++k) {
+            const int slot = k % kUnitSlots;
+            ok = ok && warp_wait(&sh.unit_full[slot], k / kUnitSlots);
+            // both sub-tiles' warps leave together: each unit has barriers for all of them
+            if (!ok) *stop = 1;
+            meet<32 * C::kSoft>();   // and the unit before is done with its queries, sums and results
+            if (t == 0) sh.leave = *stop;
+            meet<32 * C::kSoft>();
+            if (sh.leave) {
+                if (!ok && lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutMma);
+                break;
+            }
+            const Unit u = sh.unit[slot];
+            __syncwarp();
+            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
+            if (u.tok0 < 0) break;
+            const int nb = u.c1 - u.c0;
+            const bool alt = alternate<D>(u), fine = u.nf <= C::kFine;
+            if (nb > 0) {
+                constexpr int kPieces = D / 8;
+                for (int i = t; i < u.nf * kPieces; i += 32 * C::kSoft) {
+                    const int f = i / kPieces, pc = i % kPieces;
+                    const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + q_row(p, u, f) * p.qs +
+                                          static_cast<size_t>(q_head(p, u, f)) * D + pc * 8;
+                    uint4 v;
+                    if (wide_q) {
+                        v = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        uint32_t e[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) e[j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
+                        v = make_uint4(e[0], e[1], e[2], e[3]);
+                    }
+                    *reinterpret_cast<uint4*>(smem_at + (f >> 7) * C::kQ + (pc >> 3) * 16384 + (f & 127) * 128 +
+                                              (((pc ^ f) & 7) << 4)) = v;
+                }
+                fer::dev::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) fer::dev::mbar_arrive(&sh.q_full);
+            }
+            const int f = alt ? r : x * 128 + r, first = alt ? x : 0, step = alt ? 2 : 1;
+            const bool rows_here = (f & ~31) < u.nf;                       // of the warp
+            const Sees sees(p, u, min(f, u.nf - 1));
+            // what every row of the warp sees, for blocks that need no mask
+            const int all_end = __reduce_min_sync(0xffffffffu, sees.end), all_begin = __reduce_max_sync(0xffffffffu, sees.begin);
+            float m = -INFINITY, l = 0.0f;
+            const int32_t* const table = table_of(c, p, u);
+            for (int i = first; i < nb; i += step) {
+                if (ok) ok = warp_wait(&sh.s_full[x], n_s);
+                ++n_s;
+                fence_after();
+                const int s0 = block_of(u, u.c0 + i) * C::kKeys;
+                if (rows_here && ok) {
+                    const bool plain = s0 + C::kKeys <= all_end && (s0 >= all_begin || s0 + C::kKeys <= sees.sink);
+                    const bool bad = sh.bad[(block + i) % kBadRing] != 0;
+                    // [b0, e0) of the window and [0, k0) of the sinks, within the block
+                    const int b0 = sees.begin - s0, e0 = sees.end - s0, k0 = min(sees.sink, sees.end) - s0;
+                    const auto scores = [&](int j, float (&v)[32]) {   // 32 of the block, -inf where the row sees none
+                        tmem_ld(s_at + 32 * j, v);
+                        if (plain && !bad) return;
+                        uint32_t on = (below(e0 - 32 * j) & ~below(b0 - 32 * j)) | below(k0 - 32 * j);
+                        if (bad)
+                            for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
+                                const int page = (s0 + 32 * j + e) >> c.shift;
+                                if (!page_needed(c, u, page) || !c.is_page(table[page])) on &= ~(0xffu << e);
+                            }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(on >> e & 1u)) v[e] = -INFINITY;
+                    };
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < C::kKeys / 32; ++j) {
+                        float v[32];
+                        scores(j, v);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[e], v[e + 1]);
+                    }
+                    const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * p.scale2;
+                    const bool raise = top > m + kSlack;
+                    const float m1 = raise ? top : m, shift = m1 == -INFINITY ? 0.0f : m1;
+                    const float a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
+                    m = m1;
+                    if (i > first && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+                        for (int j = 0; j < D / 16; ++j) {
+                            uint32_t o[16];
+                            tmem_ld16(row_at + C::kColO + x * D + 16 * j, o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                            tmem_st16(row_at + C::kColO + x * D + 16 * j, o);
+                        }
+                    }
+                    const uint64_t sc2 = fer::dev::f2_splat(p.scale2), nm2 = fer::dev::f2_splat(kUp - shift);
+                    uint64_t sum[4] = {0, 0, 0, 0};
+                    uint32_t low[C::kKeys / 2];   // kept to the end: they lie over scores
+#pragma unroll
+                    for (int j = 0; j < C::kKeys / 32; ++j) {
+                        float v[32];
+                        uint32_t hi[16];
+                        scores(j, v);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float p0, p1;
+                            fer::dev::f2_unpack(fer::dev::f2_fma(fer::dev::f2_pack(v[e], v[e + 1]), sc2, nm2), p0, p1);
+                            p0 = ex2(p0), p1 = ex2(p1);
+                            sum[(e >> 1) & 3] = fer::dev::f2_add(sum[(e >> 1) & 3], fer::dev::f2_pack(p0, p1));
+                            hi[e >> 1] = pack2<T>(p0, p1);
+                            if (fine) {
+                                float h0, h1;
+                                unpack2<T>(hi[e >> 1], h0, h1);
+                                low[16 * j + (e >> 1)] = pack2<T>(p0 - h0, p1 - h1);
+                            }
+                        }
+                        tmem_st16(s_at + 16 * j, hi);
+                    }
+                    if (fine)
+#pragma unroll
+                        for (int j = 0; j < C::kKeys / 32; ++j)
+                            tmem_st16(s_at + C::kKeys / 2 + 16 * j, *reinterpret_cast<uint32_t(*)[16]>(low + 16 * j));
+                    float sm[8];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) fer::dev::f2_unpack(sum[j], sm[2 * j], sm[2 * j + 1]);
+                    l = l * a + (((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7])));
+                    wait_st();
+                }
+                // values of slots that no row sees count as zero, whatever is there
+                const bool behind = s0 + C::kKeys > u.hi, before = s0 < u.lo && s0 + C::kKeys > u.sink;
+                if ((behind || before) && ok) {
+                    const uint32_t at = base + at_v(alt, i, nb);
+                    const int st = at % C::kStages;
+                    ok = warp_wait(&sh.full[st], at / C::kStages);
+                    if (ok)
+                        for (int j = r; j < C::kKeys * (D / 8); j += 128) {
+                            const int e = j / (D / 8), pc = j % (D / 8), s = s0 + e;
+                            if (s < u.hi && (s >= u.lo || s < u.sink)) continue;
+                            *reinterpret_cast<uint4*>(smem_at + C::kSubs * C::kQ + st * C::kTile + (pc >> 3) * C::kBand +
+                                                      e * 128 + ((pc & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                        }
+                    fer::dev::fence_proxy_async_smem();
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) fer::dev::mbar_arrive(&sh.p_full[x]);
+            }
+            const bool mine = first < nb;
+            if (mine) {
+                if (ok) ok = warp_wait(&sh.o_full[x], n_o);
+                ++n_o;
+            }
+            fence_after();
+            base += 2 * nb, block += nb;
+
+            // the results: where blocks alternate each sub-tile's warps take half of the dims of both sums
+            float ml = m, wa = 1.0f, wb = 0.0f, total = l;
+            int d0 = 0, d1 = D;
+            uint32_t at_a = row_at + C::kColO + x * D, at_b = at_a;
+            if (alt) {
+                sh.ml[x][r][0] = m, sh.ml[x][r][1] = l;
+                meet<32 * C::kSoft>();
+                const float ma = sh.ml[0][r][0], mb = nb > 1 ? sh.ml[1][r][0] : -INFINITY;
+                ml = fmaxf(ma, mb);
+                const float base2 = ml == -INFINITY ? 0.0f : ml;
+                wa = ex2(ma - base2), wb = ex2(mb - base2);
+                total = sh.ml[0][r][1] * wa + (nb > 1 ? sh.ml[1][r][1] * wb : 0.0f);
+                d0 = x * (D / 2), d1 = d0 + D / 2;
+                at_a = row_at + C::kColO, at_b = at_a + D;
+                fence_after();
+            }
+            // (the barriers of a unit that ended early are not waited for: everything stops below)
+            const bool on = f < u.nf;
+            const int fr = min(f, u.nf - 1), head = q_head(p, u, fr);
+            const size_t tok = q_row(p, u, fr), bh = tok * p.heads + head, part = bh * p.parts + max(u.part, 0);
+            T* const out = static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D;
+            const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+            bool nan = false;
+            if (rows_here && ok) {
+#pragma unroll 1
+                for (int d = d0; d < d1; d += 32) {
+                    float o[32];
+                    if (nb > 0) {
+                        tmem_ld(at_a + d, o);
+                        if (alt && nb > 1) {
+                            float o1[32];
+                            tmem_ld(at_b + d, o1);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = fmaf(o[e], wa, o1[e] * wb);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        o[e] = nb > 0 ? o[e] * scale : 0.0f;
+                        nan = nan || !(o[e] - o[e] == 0.0f);   // infinite ones too: they may be 0 x inf elsewhere
+                    }
+                    if (on && u.part >= 0) {
+                        float4* const to = reinterpret_cast<float4*>(p.part_o + part * D + d);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                    } else if (on && wide_o) {
+                        uint4* const to = reinterpret_cast<uint4*>(out + d);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            to[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
+                                               pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+                    } else if (on) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) put(out + d + e, o[e]);
+                    }
+                    __syncwarp();
+                }
+                if (on && (!alt || x == 0)) {
+                    if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * part) = make_float2(ml, total);
+                    else if (p.lse) p.lse[bh] = total == 0.0f ? -INFINITY : (ml + (log2f(total) - kUp)) * kLn2;
+                }
+                unsigned again = __ballot_sync(0xffffffffu, on && nan && nb > 0);
+                while (again) {
+                    const int src = __ffs(again) - 1;
+                    again &= again - 1;
+                    const int g = (f & ~31) + src;
+                    float m2, l2, o2[D / 32];
+                    one_row<T, D>(c, p, u, g, m2, l2, o2);
+                    const int gh = q_head(p, u, g);
+                    const size_t gt = q_row(p, u, g), gp = (gt * p.heads + gh) * p.parts + max(u.part, 0);
+#pragma unroll
+                    for (int j = 0; j < D / 32; ++j) {
+                        const int d = 32 * j + lane;
+                        if (d < d0 || d >= d1) continue;
+                        if (u.part >= 0) p.part_o[gp * D + d] = o2[j];
+                        else put(static_cast<T*>(p.out) + gt * p.os + static_cast<size_t>(gh) * D + d, l2 == 0.0f ? 0.0f : o2[j] / l2);
+                    }
+                    // l is of 2^(s - m + kUp) elsewhere
+                    if (lane == 0 && u.part >= 0 && (!alt || x == 0))
+                        *reinterpret_cast<float2*>(p.part_ml + 2 * gp) = make_float2(m2 + kUp, l2);
+                    __syncwarp();
+                }
+            }
+            fence_before();
+        }
+    }
+
+    fence_before();
+    __syncthreads();
+    if (w == C::kSoft + 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// Adds the parts of every row that has several, one warp each: out = sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kJoinWarps) attn_join(const Paged c, const TileParams p, float up) {
+    constexpr int kV = D / 32;
+    struct alignas(4 * (kV < 4 ? kV : 4)) Dims { float e[kV]; };
+    fer::dev::pdl_begin();
+    const int lane = threadIdx.x & 31;
+    const long long item = static_cast<long long>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
+    if (item >= static_cast<long long>(p.rows) * p.heads) return;
+    const int tok = static_cast<int>(item / p.heads), head = static_cast<int>(item - static_cast<long long>(tok) * p.heads);
+    int own = 0, shared = 0;
+    {
+        // the row's sequence, and its tile's blocks
+        int b = tok;
+        if (p.offsets) {
+            int lo = 0, hi = p.n_seq;   // the last sequence that starts at or before the row
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (p.offsets[mid] <= tok) lo = mid;
+                else hi = mid;
+            }
+            b = lo;
+        }
+        const Seq q(c, p, b);
+        if (tok < q.tok0 || tok >= q.tok0 + q.n) return;   // of no sequence
+        const long long f = static_cast<long long>(tok - q.tok0) * p.group + head % p.group;
+        Unit u;
+        own = chunks_of(tile_range<D>(p, q, static_cast<int>(f / Cut<D>::kRows), u), p.chunk);
+    }
+    if (p.prefix_pages) shared = Prefix<D>(c, p).chunks;
+    else if (own == 1) return;   // written already
+    const float2* const ml = reinterpret_cast<const float2*>(p.part_ml) + item * p.parts;
+    const float* const po = p.part_o + item * p.parts * D + kV * lane;
+    const int n = own + shared;
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, ml[i < own ? i : p.own_parts + i - own].x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f;
+    Dims o{};
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const int at = i < own ? i : p.own_parts + i - own;
+        const float2 v = ml[at];
+        const Dims d = *reinterpret_cast<const Dims*>(po + static_cast<size_t>(at) * D);
+        const float y = ex2(v.x - base);
+        l = fmaf(v.y, y, l);
+        // a part without a key counts as nothing, and one that vanishes gives an infinite value its due
+        const float z = v.y == 0.0f ? 0.0f : fmaxf(y, 1.17549435e-38f);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) o.e[e] = fmaf(d.e[e], z, o.e[e]);
+    }
+    T* const out = static_cast<T*>(p.out) + static_cast<size_t>(tok) * p.os + static_cast<size_t>(head) * D + kV * lane;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) put(out + e, l == 0.0f ? 0.0f : o.e[e] * inv);
+    if (lane == 0 && p.lse) p.lse[item] = l == 0.0f ? -INFINITY : (base + (log2f(l) - up)) * kLn2;
+}
+
+// ---- host
+
+struct Split {
+    int chunk, parts;
+};
+
+constexpr int keys_of(int head_dim) { return head_dim == 256 ? 64 : 128; }
+constexpr int rows_of(int head_dim) { return head_dim == 256 ? 128 : 256; }
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// Cuts of a row's key blocks, of which there are at most `blocks`, where `units` tiles of rows and heads are to be
+// shared out and a tile has about tile_rows rows.
+Split split(long long units, long long blocks, long long tile_rows) {
+    Split s{INT_MAX, 0};
+    long long parts = 1;
+    if (tile_rows <= 64) parts = ceil_div(blocks, 8);            // a part costs little: even shares of ragged lengths
+    else if (units < 4 * kSms) parts = ceil_div(4 * kSms, units);
+    if (tile_rows > 64 && parts > ceil_div(blocks, 16)) parts = ceil_div(blocks, 16);
+    if (parts <= 1) return s;
+    s.chunk = static_cast<int>(ceil_div(blocks, parts));
+    s.parts = static_cast<int>(ceil_div(blocks, s.chunk));
+    return s;
+}
+
+Split window_split(long long rows, long long n_seq, int heads, int kv_heads, int head_dim, long long max_slots, long long window,
+                   long long sinks) {
+    const int keys = keys_of(head_dim), tile = rows_of(head_dim);
+    const long long group = heads / kv_heads;
+    long long blocks = ceil_div(max_slots, keys);
+    if (window > 0) {
+        const long long some = ceil_div(window + ceil_div(tile, group), keys) + 1 + ceil_div(sinks, keys);
+        if (some < blocks) blocks = some;
+    }
+    const long long tiles = n_seq > ceil_div(rows * group, tile) ? n_seq : ceil_div(rows * group, tile);
+    const long long each = ceil_div(rows, n_seq) * group;
+    return split(tiles * kv_heads, blocks, each < tile ? each : tile);
+}
+
+struct PrefixSplit {
+    Split own;
+    int chunk, parts;
+};
+
+PrefixSplit prefix_split(long long n_seq, int heads, int kv_heads, int head_dim, long long max_slots, long long max_prefix) {
+    const int keys = keys_of(head_dim), tile = rows_of(head_dim);
+    const long long group = heads / kv_heads;
+    PrefixSplit s{};
+    s.own = split(n_seq * kv_heads * ceil_div(group, tile), ceil_div(max_slots, keys), group < tile ? group : tile);
+    if (s.own.parts == 0) s.own = Split{INT_MAX, 1};
+    // a CTA's equal share of the prefix, if that is not less than a few blocks
+    const long long blocks = ceil_div(max_prefix, keys), tiles = kv_heads * ceil_div(n_seq * group, tile);
+    long long chunk = ceil_div(blocks * tiles, kSms);
+    if (chunk < 4) chunk = 4;
+    if (chunk > blocks) chunk = blocks;
+    s.chunk = static_cast<int>(chunk);
+    s.parts = static_cast<int>(ceil_div(blocks, chunk));
+    return s;
+}
+
+size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
+size_t parts_bytes(size_t rows, size_t heads, size_t head_dim, size_t parts) {
+    return up16(rows * heads * parts * 2 * sizeof(float)) + rows * heads * parts * head_dim * sizeof(float);
+}
+
+// Boxes of 64 dims x `rows` rows of one page; 128-byte swizzle.
+bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int rows) {
+    const fer::host::EncodeTiledFn fn = fer::host::encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t page = static_cast<cuuint64_t>(c.page_size()), row = 2ull * c.head_dim;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), page, static_cast<cuuint64_t>(c.kv_heads),
+                                static_cast<cuuint64_t>(c.pages)};
+    const cuuint64_t strides[3] = {row, page * row, page * row * c.kv_heads};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, step[4] = {1, 1, 1, 1};
+    return fn(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides,
+              box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Sets the shared-memory limit of a kernel once per device.
+cudaError_t allow(const void* kernel, int smem, std::atomic<bool>* known) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= fer::host::kMaxDevices) return cudaErrorInvalidDevice;
+    if (known[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) known[dev].store(true, std::memory_order_relaxed);
+    return e;
+}
+
+template <typename T, int D>
+cudaError_t run(const Paged& c, const TileParams& p, cudaStream_t s) {
+    using C = Cut<D>;
+    static std::atomic<bool> known[fer::host::kMaxDevices];
+    cudaError_t e = allow(reinterpret_cast<const void*>(attn_tiles<T, D>), C::kSmem, known);
+    if (e != cudaSuccess) return e;
+    CUtensorMap k_map, v_map;
+    const int rows = C::kKeys < c.page_size() ? C::kKeys : c.page_size();
+    const uint32_t dtype = __is_same(T, __half) ? 1 : 2;
+    if (!map_pages(&k_map, c, c.k, dtype, rows) || !map_pages(&v_map, c, c.v, dtype, rows)) return cudaErrorInvalidValue;
+    // no more CTAs than there can be units
+    const long long tiles = ceil_div(static_cast<long long>(p.rows) * p.group, C::kRows) + p.n_seq;
+    long long most = tiles * c.kv_heads * (p.parts > 0 ? p.parts : 1);
+    const int grid = static_cast<int>(most < kSms ? most : kSms);
+    e = fer::host::launch_pdl(attn_tiles<T, D>, dim3(grid), dim3(C::kThreads), C::kSmem, s, c, p, k_map, v_map);
+    if (e == cudaSuccess && p.parts > 0) {
+        const long long ctas = ceil_div(static_cast<long long>(p.rows) * p.heads, kJoinWarps);
+        e = fer::host::launch_pdl(attn_join<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(32 * kJoinWarps), 0, s, c, p,
+                                  __is_same(T, __half) ? 8.0f : 0.0f);
+    }
+    return e;
+}
+
+template <typename T>
+cudaError_t run_dim(const Paged& c, const TileParams& p, cudaStream_t s) {
+    switch (c.head_dim) {
+        case 64: return run<T, 64>(c, p, s);
+        case 128: return run<T, 128>(c, p, s);
+        default: return run<T, 256>(c, p, s);
+    }
+}
+
+// What both operators' arguments have in common.
+cudaError_t common(const fer_paged_view_t* cache, const void* q, void* out, size_t q_stride, size_t out_stride, int heads,
+                   float scale, const float* lse, Paged* c, TileParams* p) {
+    const cudaError_t e = fer::host::paged_params(cache, c);
+    if (e != cudaSuccess) return e;
+    if (!q || !out || heads <= 0 || heads % c->kv_heads || heads > 65536) return cudaErrorInvalidValue;
+    const size_t width = static_cast<size_t>(heads) * c->head_dim;
+    if (q_stride < width || out_stride < width || !(scale >= 0.0f) || scale > kMostScale) return cudaErrorInvalidValue;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 2 || !fer::host::words_aligned({lse}))
+        return cudaErrorInvalidValue;
+    if (c->kv_heads > 65535) return cudaErrorNotSupported;
+    p->q = q;
+    p->out = out;
+    p->qs = q_stride;
+    p->os = out_stride;
+    p->lse = const_cast<float*>(lse);
+    p->heads = heads;
+    p->group = heads / c->kv_heads;
+    p->scale2 = (scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c->head_dim)) : scale) * kLog2e;
+    return cudaSuccess;
+}
+
+cudaError_t go(const Paged& c, TileParams& p, uint32_t dtype, void* workspace, size_t bytes, cudaStream_t s) {
+    // units are counted in 31 bits, and so are the joining's CTAs
+    const long long tiles = ceil_div(static_cast<long long>(p.rows) * p.group, rows_of(c.head_dim)) + p.n_seq;
+    if (tiles * c.kv_heads * (p.parts > 0 ? p.parts : 1) > INT_MAX - 65536ll ||
+        static_cast<long long>(p.rows) * p.group > INT_MAX - 65536ll ||
+        ceil_div(static_cast<long long>(p.rows) * p.heads, kJoinWarps) > INT_MAX)
+        return cudaErrorNotSupported;
+    if (p.parts > 0) {
+        if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+            bytes < parts_bytes(p.rows, p.heads, c.head_dim, p.parts))
+            return cudaErrorInvalidValue;
+        p.part_ml = static_cast<float*>(workspace);
+        p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                            up16(static_cast<size_t>(p.rows) * p.heads * p.parts * 2 * sizeof(float)));
+    }
+    return dtype == 1 ? run_dim<__half>(c, p, s) : run_dim<__nv_bfloat16>(c, p, s);
+}
+
+bool sizes_ok(int heads, int kv_heads, int head_dim) {
+    return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128 || head_dim == 256);
+}
+
+}  // namespace
+
+extern "C" size_t fer_paged_window_attention_workspace_bytes(int rows, int n_seq, int heads, int kv_heads, int head_dim,
+                                                             int max_slots, int window, int sinks) {
+    if (rows <= 0 || n_seq <= 0 || max_slots <= 0 || window < 0 || sinks < 0 || !sizes_ok(heads, kv_heads, head_dim)) return 0;
+    const Split s = window_split(rows, n_seq, heads, kv_heads, head_dim, max_slots, window, sinks);
+    return s.parts > 0 ? parts_bytes(rows, heads, head_dim, s.parts) : 16;
+}
+
+extern "C" cudaError_t fer_paged_window_attention(const fer_paged_view_t* cache, const fer_paged_window_args_t* a, uint32_t* err,
+                                                  cudaStream_t s) {
+    if (!a) return cudaErrorInvalidValue;
+    Paged c{};
+    TileParams p{};
+    const cudaError_t e = common(cache, a->q, a->out, a->q_stride, a->out_stride, a->heads, a->scale, a->lse, &c, &p);
+    if (e != cudaSuccess) return e;
+    if (a->rows < 0 || a->n_seq < 0 || a->n_seq > cache->batch || a->window < 0 || a->sinks < 0 ||
+        (!a->offsets && a->rows != a->n_seq) || !fer::host::words_aligned({a->offsets}))
+        return cudaErrorInvalidValue;
+    if (a->rows == 0 || a->n_seq == 0) return cudaSuccess;
+    if (a->n_seq > 65535) return cudaErrorNotSupported;
+    p.offsets = a->offsets;
+    p.rows = a->rows;
+    p.n_seq = a->n_seq;
+    p.window = a->window > 0 ? a->window : INT_MAX;
+    p.sinks = a->window > 0 ? a->sinks : 0;
+    p.err = err;
+    const Split sp = window_split(a->rows, a->n_seq, a->heads, c.kv_heads, c.head_dim, c.max_slots(), a->window, a->sinks);
+    p.chunk = sp.chunk;
+    p.parts = sp.parts;
+    return go(c, p, cache->dtype, a->workspace, a->workspace_bytes, s);
+}
+
+extern "C" size_t fer_paged_prefix_attention_workspace_bytes(int n_seq, int heads, int kv_heads, int head_dim, int max_slots,
+                                                             int max_prefix_slots) {
+    if (n_seq <= 0 || max_slots <= 0 || max_prefix_slots <= 0 || !sizes_ok(heads, kv_heads, head_dim)) return 0;
+    const PrefixSplit s = prefix_split(n_seq, heads, kv_heads, head_dim, max_slots, max_prefix_slots);
+    return parts_bytes(n_seq, heads, head_dim, static_cast<size_t>(s.own.parts) + s.parts);
+}
+
+extern "C" cudaError_t fer_paged_prefix_attention(const fer_paged_view_t* cache, const fer_paged_prefix_args_t* a, uint32_t* err,
+                                                  cudaStream_t s) {
+    if (!a) return cudaErrorInvalidValue;
+    Paged c{};
+    TileParams p{};
+    const cudaError_t e = common(cache, a->q, a->out, a->q_stride, a->out_stride, a->heads, a->scale, a->lse, &c, &p);
+    if (e != cudaSuccess) return e;
+    if (!a->prefix_pages || !a->prefix_length || a->max_prefix_pages <= 0 || a->n_seq < 0 || a->n_seq > cache->batch ||
+        !fer::host::words_aligned({a->prefix_pages, a->prefix_length}))
+        return cudaErrorInvalidValue;
+    const long long most = static_cast<long long>(a->max_prefix_pages) << c.shift;
+    if (most > INT_MAX - 65536ll || a->n_seq > 65535) return cudaErrorNotSupported;
+    if (a->n_seq == 0) return cudaSuccess;
+    p.rows = p.n_seq = a->n_seq;
+    p.window = INT_MAX;
+    p.err = err;
+    p.prefix_pages = a->prefix_pages;
+    p.prefix_length = a->prefix_length;
+    p.prefix_max = a->max_prefix_pages;
+    const PrefixSplit sp = prefix_split(a->n_seq, a->heads, c.kv_heads, c.head_dim, c.max_slots(), most);
+    p.chunk = sp.own.chunk;
+    p.own_parts = sp.own.parts;
+    p.prefix_chunk = sp.chunk;
+    p.parts = sp.own.parts + sp.parts;
+    return go(c, p, cache->dtype, a->workspace, a->workspace_bytes, s);
+}

@@ -254,6 +254,48 @@ typedef struct fer_rotary_request {
 
 fer_status_t fer_submit_rotary(fer_session_t* session, const fer_rotary_request_t* req, uint64_t* out_job_id);
 
+/* Query and key heads normed and turned in one pass: each head of x becomes x /
+ * sqrt(mean(x^2) + eps) * gamma over all of its elements, and then turns as
+ * fer_submit_rotary's does. rotary: that call's request (x, out, columns, heads,
+ * positions and so on) without FER_ROTARY_INVERSE, head_dim at most 256; of its
+ * heads the last k_heads are key heads with k_gamma, the others query heads with
+ * q_gamma, f32 [head_dim] each (0: ones). f32 inside, rounded once. eps >= 0. */
+typedef struct fer_norm_rotary_request {
+    fer_rotary_request_t rotary;
+    uint64_t q_gamma;
+    uint64_t k_gamma;
+    uint32_t k_heads;
+    float eps;
+} fer_norm_rotary_request_t;
+
+fer_status_t fer_submit_norm_rotary(fer_session_t* session, const fer_norm_rotary_request_t* req, uint64_t* out_job_id);
+
+/* Its gradient. rotary, gammas, k_heads and eps as in the call, with x the
+ * call's x and out the gradient of x; grad [rows, cols] the gradient of the
+ * call's out, heads from column grad_col. out may be x, or grad, with the same
+ * column (in place) or with columns that do not overlap. q_gamma_grad and
+ * k_gamma_grad f32 [head_dim] (0: not wanted) receive the gradients of the
+ * gammas, summed over rows and heads in a fixed order. workspace: u8 buffer
+ * (16-byte aligned) of at least fer_norm_rotary_grad_workspace_bytes(rows,
+ * heads, head_dim) bytes, any contents; calls on different streams need one
+ * each. */
+typedef struct fer_norm_rotary_grad_request {
+    fer_rotary_request_t rotary;
+    uint64_t q_gamma;
+    uint64_t k_gamma;
+    uint64_t grad;
+    uint64_t q_gamma_grad;
+    uint64_t k_gamma_grad;
+    uint64_t workspace;
+    uint32_t grad_col;
+    uint32_t k_heads;
+    float eps;
+    uint32_t reserved;
+} fer_norm_rotary_grad_request_t;
+
+fer_status_t fer_submit_norm_rotary_grad(fer_session_t* session, const fer_norm_rotary_grad_request_t* req,
+                                         uint64_t* out_job_id);
+
 /* ---- paged key-value cache -----------------------------------------------------
  * Keys and values of many sequences in pages handed out by the caller: k and v
  * f16 or bf16 [pages, kv_heads, page_size, head_dim] (page_size a power of two
@@ -371,6 +413,111 @@ typedef struct fer_paged_evict_request {
 } fer_paged_evict_request_t;
 
 fer_status_t fer_submit_paged_evict(fer_session_t* session, const fer_paged_evict_request_t* req, uint64_t* out_job_id);
+
+/* The plan of a serving step, on the GPU from the requests' lengths: sequence b
+ * holds lengths[b] slots and asks for counts[b] new rows (all i32 [batch]; 0:
+ * none, and a length set to 0 gives a sequence's pages back); held[b] pages of
+ * its row of page_table i32 [batch, max_pages] are its own. free_pages i32
+ * [pages] is a ring, free_state i32 [2] the place where the free pages in it
+ * begin and their number. Sequences are served in order: one gets its rows if
+ * they need no new page, or if the pages that it and those before it ask for
+ * are no more than the ring has; else it gets none this time. New pages come
+ * from the ring's beginning, in order of sequences; pages behind those that a
+ * sequence needs (its slots, new rows among them, over page_size, rounded up)
+ * go back behind the ring's end, and can be taken from the next call on. Written:
+ * page_table and free_pages (in place), new_held and new_free_state (0 or the
+ * old one: in place), offsets i32 [batch + 1] (the first row of every sequence,
+ * as store and window attention take them), and for every row of the step's
+ * activation, each i32 [rows] and optional (0): sequences (-1 behind the last
+ * row), positions (what rotary takes: seen[b], or lengths[b] where seen is 0,
+ * and up; 0 behind the last), slots (page * page_size + the slot in the page; -1
+ * behind the last). page_size: a power of two from 8 to 256. Error bit 4: a
+ * length, count or number of pages out of range (clamped; more slots than a row
+ * of the table holds: no rows for that sequence), a page id or free_state out of
+ * range (no page moves then), more rows than the arrays have (dropped). */
+typedef struct fer_paged_plan_request {
+    uint64_t page_table;
+    uint64_t lengths;
+    uint64_t counts;
+    uint64_t held;
+    uint64_t free_pages;
+    uint64_t free_state;
+    uint64_t offsets;
+    uint64_t new_held;
+    uint64_t new_free_state;
+    uint64_t sequences;
+    uint64_t positions;
+    uint64_t slots;
+    uint64_t seen;
+    uint32_t page_size;
+    uint32_t reserved;
+} fer_paged_plan_request_t;
+
+fer_status_t fer_submit_paged_plan(fer_session_t* session, const fer_paged_plan_request_t* req, uint64_t* out_job_id);
+
+/* Attention of prompts' rows or single tokens over the cache, with a sliding
+ * window and sinks (store the new tokens' keys first). offsets i32 [sequences +
+ * 1]: rows offsets[b] .. offsets[b+1] - 1 of q [rows, cols] are the last slots
+ * of sequence b (rows without a slot, where it holds fewer, see nothing), rows
+ * behind the last offset belong to nobody and theirs of out and lse are left as
+ * they were; 0: row b is sequence b's last slot. A row in slot p sees the slots s
+ * <= p with s > p - window, or s < sinks; window 0: all s <= p. Pages in which
+ * no row of the call sees a slot are not read, nor are their entries, so
+ * their pages may have been given to others. head columns, heads, scale, lse
+ * and overlaps as in fer_submit_paged_attention; a row that sees nothing gives
+ * zeros and lse -inf. Probabilities are rounded to the cache's dtype once before they
+ * meet the values, sums are f32. Bit-identical run to run. Offsets that decrease
+ * or leave 0 .. rows set error bit 4, and the results are then not to be used.
+ * workspace: u8 buffer (16-byte aligned) of at least
+ * fer_paged_window_attention_workspace_bytes(rows, sequences, heads, kv_heads,
+ * head_dim, max_pages * page_size, window, sinks) bytes, any contents; calls on
+ * different streams need one each. */
+typedef struct fer_paged_window_attention_request {
+    fer_paged_cache_t cache;
+    uint64_t q;
+    uint64_t out;
+    uint64_t lse;
+    uint64_t offsets;
+    uint64_t workspace;
+    uint32_t q_col;
+    uint32_t out_col;
+    uint32_t heads;
+    uint32_t window;
+    uint32_t sinks;
+    float scale;
+} fer_paged_window_attention_request_t;
+
+fer_status_t fer_submit_paged_window_attention(fer_session_t* session, const fer_paged_window_attention_request_t* req,
+                                               uint64_t* out_job_id);
+
+/* One new token's attention for the first rows(q) sequences, all of them behind
+ * one prefix whose keys and values are read once for the whole batch: the slots
+ * 0 .. prefix_length - 1 (i32 [1]) of prefix_pages (i32 [pages], ids in the
+ * cache's pools), and then the sequence's own held slots as in
+ * fer_submit_paged_attention, under one softmax. The cache's table and lengths
+ * hold the sequences' own slots alone; a prefix enters its pages once, as a
+ * sequence of a cache view of its own. Other arguments and rules as
+ * fer_submit_paged_attention's (no weights); a prefix_length out of range is
+ * clamped and sets error bit 4. Bit-identical run to run. workspace: u8 buffer (16-byte aligned) of at least
+ * fer_paged_prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim,
+ * max_pages * page_size, prefix pages * page_size) bytes, any contents; calls on
+ * different streams need one each. */
+typedef struct fer_paged_prefix_attention_request {
+    fer_paged_cache_t cache;
+    uint64_t q;
+    uint64_t out;
+    uint64_t lse;
+    uint64_t prefix_pages;
+    uint64_t prefix_length;
+    uint64_t workspace;
+    uint32_t q_col;
+    uint32_t out_col;
+    uint32_t heads;
+    float scale;
+} fer_paged_prefix_attention_request_t;
+
+fer_status_t fer_submit_paged_prefix_attention(fer_session_t* session, const fer_paged_prefix_attention_request_t* req,
+                                               uint64_t* out_job_id);
 
 /* Per-kernel-class timing of forwards: while enabled, every forward records a
  * CUDA event pair around each of its launches on the session stream; reading

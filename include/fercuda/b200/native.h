@@ -176,6 +176,37 @@ typedef struct fer_rotary_args {
 } fer_rotary_args_t;
 cudaError_t fer_rotary(const fer_rotary_args_t* args, cudaStream_t s);
 
+/* Root-mean-square norm of each head and its rotary positions in one pass, as
+ * fer_rotary with flags INTERLEAVED and AXIS_FREQS only and head_dim at most 256:
+ * a head x becomes x / sqrt(mean(x^2) + eps) * gamma over all of its elements,
+ * then its first rotary_dim elements turn. The first heads - k_heads heads take
+ * q_gamma, the last k_heads k_gamma, f32 [head_dim] each (NULL: ones). f32
+ * inside, rounded once. eps >= 0.
+ * fer_norm_rotary_grad: rotary.x is the call's x, grad the gradient of its out
+ * (grad_stride elements apart), rotary.out receives the gradient of x (out ==
+ * grad or out == x with equal strides is allowed), q_gamma_grad / k_gamma_grad
+ * (NULL: not wanted) those of the gammas, summed over rows and heads in a fixed
+ * order. workspace: fer_norm_rotary_grad_workspace_bytes, 16-byte aligned, any
+ * contents; calls (or graph replays) that may run at the same time need one each. */
+typedef struct fer_norm_rotary_args {
+    fer_rotary_args_t rotary;
+    int k_heads;
+    const float* q_gamma;
+    const float* k_gamma;
+    float eps;
+} fer_norm_rotary_args_t;
+typedef struct fer_norm_rotary_grad {
+    const void* grad;
+    size_t grad_stride;
+    float* q_gamma_grad;
+    float* k_gamma_grad;
+    void* workspace;
+    size_t workspace_bytes;
+} fer_norm_rotary_grad_t;
+size_t fer_norm_rotary_grad_workspace_bytes(int rows, int heads, int head_dim);
+cudaError_t fer_norm_rotary(const fer_norm_rotary_args_t* args, cudaStream_t s);
+cudaError_t fer_norm_rotary_grad(const fer_norm_rotary_args_t* args, const fer_norm_rotary_grad_t* grad, cudaStream_t s);
+
 /* ---- paged key-value cache ----------------------------------------------------------
  * K and V in pages [pages][kv_heads][page_size][head_dim] (f16 or bf16, 16-byte
  * aligned); slot s of sequence b is row s % page_size of page
@@ -267,6 +298,88 @@ typedef struct fer_paged_evict_args {
 size_t fer_paged_evict_workspace_bytes(int batch, int kv_heads, int max_slots, int budget);
 cudaError_t fer_paged_evict(const fer_paged_view_t* cache, const fer_paged_evict_args_t* args, uint32_t* err,
                             cudaStream_t s);
+/* The plan of a step: sequence b < batch holds lengths[b] slots and asks for
+ * counts[b] new rows; its row of page_table has held[b] pages. free_pages is a
+ * ring of `pages` entries and free_state says where the free ones begin and how
+ * many there are. Sequences are served in order: b gets its rows if it needs no
+ * new page, or if all that it and the sequences before it ask for are no more
+ * than the ring has; else it gets none. Pages are taken from the ring's
+ * beginning in order of sequences; those behind what a sequence needs (ceil of
+ * its slots, with the new rows, over page_size) go back behind the ring's end.
+ * new_held and new_free_state (each may be the old one) receive the results,
+ * offsets [batch + 1] the first row of each sequence, and for every row i <
+ * rows sequences[i] (-1 behind the last), positions[i] (seen[b], or
+ * lengths[b], + its place among the sequence's rows; 0) and slots[i]
+ * (page * page_size + the slot in it; -1), each optional (NULL). Error bit 4: a
+ * length, count or page count out of range (clamped), more slots than a row of
+ * the table has (the sequence gets no rows), a page id out of range, more rows
+ * than `rows` (dropped), a free_state out of range (no page moves). */
+typedef struct fer_paged_plan_args {
+    int32_t* page_table;         /* [batch, max_pages] */
+    const int32_t* lengths;      /* [batch] */
+    const int32_t* counts;       /* [batch] */
+    const int32_t* held;         /* [batch] */
+    const int32_t* seen;         /* [batch] or NULL: lengths */
+    int32_t* free_pages;         /* [pages] */
+    const int32_t* free_state;   /* [2] */
+    int32_t* new_held;
+    int32_t* new_free_state;
+    int32_t* offsets;            /* [batch + 1] */
+    int32_t* sequences;          /* [rows] or NULL, as the next two */
+    int32_t* positions;
+    int32_t* slots;
+    int batch, max_pages, pages, page_size, rows;
+} fer_paged_plan_args_t;
+cudaError_t fer_paged_plan(const fer_paged_plan_args_t* args, uint32_t* err, cudaStream_t s);
+/* Attention of rows of prompts or single tokens over the view's cache, keys
+ * stored first: rows offsets[b] .. offsets[b+1] - 1 of q [rows, heads *
+ * head_dim] are the last slots of sequence b < n_seq (offsets NULL: row b is
+ * sequence b's last, and rows == n_seq). The row of slot p sees the slots s <= p
+ * with s > p - window or s < sinks; window 0: all s <= p. Pages without a slot
+ * that one of the call's rows sees are not read, nor are their entries. Other
+ * arguments as fer_paged_attention's; lse [rows, heads]. A row that sees nothing
+ * gives zeros, lse -inf; rows behind the last offset are left as they were.
+ * Offsets that decrease or leave 0 .. rows set error bit 4, and results are then
+ * not to be used. The same bits run to run. workspace:
+ * fer_paged_window_attention_workspace_bytes, rules as above. */
+typedef struct fer_paged_window_args {
+    const void* q;
+    void* out;
+    size_t q_stride, out_stride;
+    int rows, n_seq, heads;
+    const int32_t* offsets;      /* [n_seq + 1] or NULL */
+    int window, sinks;
+    float scale;
+    float* lse;
+    void* workspace;
+    size_t workspace_bytes;
+} fer_paged_window_args_t;
+size_t fer_paged_window_attention_workspace_bytes(int rows, int n_seq, int heads, int kv_heads, int head_dim,
+                                                  int max_slots, int window, int sinks);
+cudaError_t fer_paged_window_attention(const fer_paged_view_t* cache, const fer_paged_window_args_t* args, uint32_t* err,
+                                       cudaStream_t s);
+/* Attention of one query per sequence b < n_seq over the slots 0 ..
+ * *prefix_length - 1 of prefix_pages, pages of the same pools that all sequences
+ * share, and then the sequence's own held slots: one softmax over both. The
+ * prefix is read once for all. A prefix_length out of range is clamped with
+ * error bit 4. Other arguments as fer_paged_attention's. */
+typedef struct fer_paged_prefix_args {
+    const void* q;
+    void* out;
+    size_t q_stride, out_stride;
+    int n_seq, heads;
+    const int32_t* prefix_pages;   /* [max_prefix_pages] */
+    const int32_t* prefix_length;  /* [1] */
+    int max_prefix_pages;
+    float scale;
+    float* lse;
+    void* workspace;
+    size_t workspace_bytes;
+} fer_paged_prefix_args_t;
+size_t fer_paged_prefix_attention_workspace_bytes(int n_seq, int heads, int kv_heads, int head_dim, int max_slots,
+                                                  int max_prefix_slots);
+cudaError_t fer_paged_prefix_attention(const fer_paged_view_t* cache, const fer_paged_prefix_args_t* args, uint32_t* err,
+                                       cudaStream_t s);
 /* Per-token layer norm, x f32 [T, d] -> out bf16, d one of 128, 256, ..., 4096. */
 cudaError_t fer_ln_bf16(const float* x, const float* g, const float* b, void* out, int T, int d, float eps,
                         cudaStream_t s);
