@@ -53,7 +53,7 @@ namespace {
 using fer::dev::Paged;
 
 constexpr int kSms = 148;
-constexpr int kSegments = 256;       // entries of the unit table
+constexpr int kSegments = 128;       // entries of the unit table
 constexpr int kUnitSlots = 3;        // units handed from the loading warp to the others
 constexpr int kBadRing = 16;         // key blocks whose flag is kept
 constexpr int kJoinWarps = 8;
@@ -267,7 +267,6 @@ struct Shared {
     Unit unit[kUnitSlots];
     int bad[kBadRing];
     int units[kSegments], sum[12];
-    float ml[2][128][2];
     uint32_t tmem;
     int stop, leave;
 };
@@ -840,13 +839,16 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             int d0 = 0, d1 = D;
             uint32_t at_a = row_at + C::kColO + x * D, at_b = at_a;
             if (alt) {
-                sh.ml[x][r][0] = m, sh.ml[x][r][1] = l;
+                // the queries' second half is free in such a unit
+                float2* const sums = reinterpret_cast<float2*>(smem_at + (C::kSubs - 1) * C::kQ);
+                sums[t] = make_float2(m, l);
                 meet<32 * C::kSoft>();
-                const float ma = sh.ml[0][r][0], mb = nb > 1 ? sh.ml[1][r][0] : -INFINITY;
+                const float2 sa = sums[r], sb = sums[128 + r];
+                const float ma = sa.x, mb = sb.x;
                 ml = fmaxf(ma, mb);
                 const float base2 = ml == -INFINITY ? 0.0f : ml;
                 wa = ex2(ma - base2), wb = ex2(mb - base2);
-                total = sh.ml[0][r][1] * wa + (nb > 1 ? sh.ml[1][r][1] * wb : 0.0f);
+                total = sa.y * wa + sb.y * wb;
                 d0 = x * (D / 2), d1 = d0 + D / 2;
                 at_a = row_at + C::kColO, at_b = at_a + D;
                 fence_after();
