@@ -47,6 +47,7 @@
 #include <atomic>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 namespace {
 
@@ -61,6 +62,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMostScale = 2.0e38f;   // times log2 e it is still finite
 constexpr float kSlack = 7.0f;          // log2 units the subtracted maximum may lag
+constexpr int kPoly = 1, kPolyOf = 4;   // of so many pairs of exponentials so many go to the multipliers
 
 // Sizes of a head_dim: keys a block, sub-tiles of rows, tiles of the ring.
 template <int D> struct Cut {
@@ -70,15 +72,23 @@ template <int D> struct Cut {
     static constexpr int kBands = D / 64;
     static constexpr int kTile = kKeys * D * 2;
     static constexpr int kBand = kKeys * 128;        // 64 dims of a tile's keys
-    static constexpr int kStages = D == 64 ? 8 : 5;
+    static constexpr int kStages = D == 64 ? 8 : D == 128 ? 5 : 4;
     static constexpr int kQ = 128 * D * 2;           // queries of a sub-tile
     static constexpr int kSoft = 4 * kSubs;          // softmax warps
-    static constexpr int kThreads = 32 * (kSoft + 2);
-    static constexpr int kSmem = kSubs * kQ + kStages * kTile + 1024;
+    // Softmax warps, one that loads keys and values, one for each sub-tile that issues products, one that loads queries.
+    // Registers: of 168 a thread at launch the two groups of four softmax warps take 224 and leave the third group's warps
+    // 56. (One group has enough at launch.)
+    static constexpr bool kShift = kSubs == 2;
+    static constexpr int kThreads = 32 * (kSoft + kSubs + 2);
+    static constexpr int kRing = kSubs * kQ;         // where the ring begins
+    // Where a unit's warps add up their results: the second sub-tile's queries, which such a unit does not have, or 32 KB more
+    static constexpr int kMeet = D == 128 ? kQ : kRing + kStages * kTile;
+    static constexpr int kSmem = kRing + kStages * kTile + (D == 128 ? 0 : 32768) + 1024;
     static constexpr uint32_t kColO = 256;           // O of sub-tile x at kColO + x D, S and P at 128 x
     // rows up to which P's rounding is made up for
     static constexpr int kFine = kSubs == 2 ? 128 : 64;
 };
+constexpr int kFew = 32;   // rows that the four warps of a sub-tile share
 
 struct TileParams {
     const void* q;
@@ -254,21 +264,21 @@ __device__ __forceinline__ int block_of(const Unit& u, int i) { return i < u.sb 
 template <int D>
 __device__ __forceinline__ bool alternate(const Unit& u) { return Cut<D>::kSubs == 2 && u.nf <= 128; }
 
-// Place in the ring, from the unit's first, of a block's keys and of its values: K_0 V_0 K_1 V_1 ..., or where blocks
-// alternate K_0 K_1 V_0 K_2 V_1 ...
-__device__ __forceinline__ int at_k(bool alt, int i) { return alt && i > 0 ? 2 * i - 1 : 2 * i; }
+// Place in the ring, from the unit's first, of a block's values: K_0 V_0 K_1 V_1 ..., or where blocks alternate K_0 K_1
+// V_0 K_2 V_1 ...
 __device__ __forceinline__ int at_v(bool alt, int i, int nb) { return alt ? min(2 * i + 2, nb + i) : 2 * i + 1; }
 
 template <int STAGES>
 struct Shared {
     uint64_t full[STAGES], empty[STAGES];
     uint64_t unit_full[kUnitSlots], unit_empty[kUnitSlots];
-    uint64_t q_full, s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2];
     Unit unit[kUnitSlots];
     int bad[kBadRing];
     int units[kSegments], sum[12];
     uint32_t tmem;
     int stop, leave;
+    uint32_t again;   // rows to be computed again
 };
 
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int r, int head, int page, uint64_t* bar) {
@@ -277,6 +287,10 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
             "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r), "r"(head), "r"(page), "r"(fer::dev::smem_addr(bar))
         : "memory");
 }
+
+// 256 threads x 224 and 128 x 56 are the 384 x 168 of the launch.
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
 
 // Shared-memory matrix descriptor, 128-byte swizzle.
 __device__ __forceinline__ uint64_t sdesc(uint32_t at, uint32_t lbo, uint32_t sbo) {
@@ -310,21 +324,33 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 columns of this thread's lane of tensor memory; the wait is in the statement, so no use can come before it.
+// 32 columns of this thread's lane of tensor memory; there after wait_ld.
 __device__ __forceinline__ void tmem_ld(uint32_t at, float (&v)[32]) {
-    uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]),
+          "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]),
+          "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
         : "r"(at)
         : "memory");
+}
+// The loads into v have landed; v passes through the statements, so that no use comes before them.
+template <int N>
+__device__ __forceinline__ void wait_ld(float (&v)[N][32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int j = 0; j < N; ++j)
+        asm volatile(""
+                     : "+f"(v[j][0]), "+f"(v[j][1]), "+f"(v[j][2]), "+f"(v[j][3]), "+f"(v[j][4]), "+f"(v[j][5]), "+f"(v[j][6]),
+                       "+f"(v[j][7]), "+f"(v[j][8]), "+f"(v[j][9]), "+f"(v[j][10]), "+f"(v[j][11]), "+f"(v[j][12]),
+                       "+f"(v[j][13]), "+f"(v[j][14]), "+f"(v[j][15]), "+f"(v[j][16]), "+f"(v[j][17]), "+f"(v[j][18]),
+                       "+f"(v[j][19]), "+f"(v[j][20]), "+f"(v[j][21]), "+f"(v[j][22]), "+f"(v[j][23]), "+f"(v[j][24]),
+                       "+f"(v[j][25]), "+f"(v[j][26]), "+f"(v[j][27]), "+f"(v[j][28]), "+f"(v[j][29]), "+f"(v[j][30]),
+                       "+f"(v[j][31])
+                     :
+                     : "memory");
 }
 __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
     asm volatile(
@@ -376,6 +402,10 @@ __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(N)
 // The bits below n, all or none of them where n is past the ends.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(fer::dev::smem_addr(bar)), "r"(n) : "memory");
+}
+
 // Whether some row of a unit sees a slot of the page.
 __device__ __forceinline__ bool page_needed(const Paged& c, const Unit& u, int page) {
     const int first = page << c.shift, last = first + c.page_size() - 1;
@@ -398,6 +428,46 @@ __device__ __forceinline__ size_t q_row(const TileParams& p, const Unit& u, int 
     return static_cast<size_t>(u.tok0) + (u.f0 + f) / p.group;
 }
 __device__ __forceinline__ int q_head(const TileParams& p, const Unit& u, int f) { return u.hk * p.group + (u.f0 + f) % p.group; }
+
+// Whether a unit's queries are those of one sub-tile, which one warp loads ahead.
+template <int D>
+__device__ __forceinline__ bool loads_ahead(const Unit& u) { return Cut<D>::kSubs == 1 || u.nf <= 128; }
+// Piece i (8 elements) of a unit's queries, and its place.
+template <typename T, int D>
+__device__ __forceinline__ uint4 q_piece(const TileParams& p, const Unit& u, int i) {
+    const int f = i / (D / 8), pc = i % (D / 8);
+    const uint16_t* const src = reinterpret_cast<const uint16_t*>(p.q) + q_row(p, u, f) * p.qs +
+                                static_cast<size_t>(q_head(p, u, f)) * D + pc * 8;
+    if ((reinterpret_cast<uintptr_t>(p.q) | (p.qs * 2)) % 16 == 0) return *reinterpret_cast<const uint4*>(src);
+    uint32_t e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
+    return make_uint4(e[0], e[1], e[2], e[3]);
+}
+template <int D>
+__device__ __forceinline__ int q_place(int f, int pc) {
+    return (f >> 7) * Cut<D>::kQ + (pc >> 3) * 16384 + (f & 127) * 128 + (((pc ^ f) & 7) << 4);
+}
+
+// 2^t for two t of at most 126, on the multipliers and adders: t = n + f with |f| <= 1/2, n by rounding in the last bits of
+// an f32, 2^f by the polynomial of degree 4 with the least relative error (2.9e-6) among those with 2^0 = 1, and n added to
+// its exponent. Below -127 it gives 0.
+__device__ __forceinline__ void powers2(uint64_t t2, float& a, float& b) {
+    float t0, t1;
+    fer::dev::f2_unpack(t2, t0, t1);
+    const uint64_t t = fer::dev::f2_pack(fmaxf(t0, -127.0f), fmaxf(t1, -127.0f));
+    const uint64_t r = fer::dev::f2_add(t, fer::dev::f2_splat(12582912.0f));
+    const uint64_t f = fer::dev::f2_sub(t, fer::dev::f2_sub(r, fer::dev::f2_splat(12582912.0f)));
+    uint64_t y = fer::dev::f2_fma(f, fer::dev::f2_splat(0.009582853f), fer::dev::f2_splat(0.055906426f));
+    y = fer::dev::f2_fma(y, f, fer::dev::f2_splat(0.24024099f));
+    y = fer::dev::f2_fma(y, f, fer::dev::f2_splat(0.69312418f));
+    y = fer::dev::f2_fma(y, f, fer::dev::f2_splat(1.0f));
+    float r0, r1, y0, y1;
+    fer::dev::f2_unpack(r, r0, r1);
+    fer::dev::f2_unpack(y, y0, y1);
+    a = __uint_as_float(__float_as_uint(y0) + (__float_as_uint(r0) << 23));
+    b = __uint_as_float(__float_as_uint(y1) + (__float_as_uint(r1) << 23));
+}
 
 template <typename T>
 __device__ __forceinline__ void put(T* to, float v) { *to = static_cast<T>(v); }
@@ -444,7 +514,7 @@ __device__ __noinline__ void one_row(const Paged& c, const TileParams& p, const 
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
-    attn_tiles(const Paged c, const TileParams p, const __grid_constant__ CUtensorMap k_map,
+    attn_tiles(const __grid_constant__ Paged c, const __grid_constant__ TileParams p, const __grid_constant__ CUtensorMap k_map,
                const __grid_constant__ CUtensorMap v_map) {
     using C = Cut<D>;
     constexpr bool kBf16 = !__is_same(T, __half);
@@ -453,18 +523,20 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     constexpr float kUp = kBf16 ? 0.0f : 8.0f;
     extern __shared__ uint8_t smem_raw[];
     __shared__ Shared<C::kStages> sh;
-    const uint32_t smem = (fer::dev::smem_addr(smem_raw) + 1023u) & ~1023u, ring = smem + C::kSubs * C::kQ;
+    const uint32_t smem = (fer::dev::smem_addr(smem_raw) + 1023u) & ~1023u, ring = smem + C::kRing;
     uint8_t* const smem_at = smem_raw + (smem - fer::dev::smem_addr(smem_raw));
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
 
     if (t == 0) {
-        for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&sh.full[i], 1), fer::dev::mbar_init(&sh.empty[i], 1);
+        for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&sh.full[i], 1), fer::dev::mbar_init(&sh.empty[i], C::kSubs);
         for (int i = 0; i < kUnitSlots; ++i)
-            fer::dev::mbar_init(&sh.unit_full[i], 1), fer::dev::mbar_init(&sh.unit_empty[i], C::kSoft + 1);
+            fer::dev::mbar_init(&sh.unit_full[i], 1), fer::dev::mbar_init(&sh.unit_empty[i], C::kSoft + C::kSubs + 1);
         fer::dev::mbar_init(&sh.q_full, C::kSoft);
+        fer::dev::mbar_init(&sh.q_empty, C::kSubs);
         for (int i = 0; i < 2; ++i)
             fer::dev::mbar_init(&sh.s_full[i], 1), fer::dev::mbar_init(&sh.p_full[i], 4), fer::dev::mbar_init(&sh.o_full[i], 1);
         sh.stop = 0;
+        sh.again = 0;
         fer::dev::fence_mbar_init();
         fer::dev::prefetch_tmap(&k_map);
         fer::dev::prefetch_tmap(&v_map);
@@ -524,169 +596,233 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     volatile int* const stop = &sh.stop;
     bool ok = true;
 
-    if (w == C::kSoft) {
-        // ---- units, and their keys and values. Pages of a block: one a lane.
-        const int box_rows = min(C::kKeys, c.page_size()), pages = C::kKeys / box_rows, boxes = pages * C::kBands;
-        uint32_t tile = 0, block = 0;   // so far
-        for (int k = 0; ok; ++k) {
-            const int slot = k % kUnitSlots;
-            ok = warp_wait(&sh.unit_empty[slot], (k / kUnitSlots & 1) ^ 1);
-            if (!ok || fer::dev::warp_flag(stop)) break;
-            const long long x = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
-            Unit u{};
-            u.tok0 = -1;
-            if (x < units) u = find_unit<D>(c, p, pre, sh.units, segments, seg, static_cast<int>(x));
-            if (lane == 0) {
-                sh.unit[slot] = u;
-                fer::dev::mbar_arrive(&sh.unit_full[slot]);
-            }
-            __syncwarp();
-            if (u.tok0 < 0) break;   // a later round has none either
-            const int32_t* const table = table_of(c, p, u);
-            const int nb = u.c1 - u.c0, lead = alternate<D>(u) ? 2 : 1;
-            // this lane's page of block i: -1 where there is none to read, -2 where its id is out of range
-            const auto page_at = [&](int i) {
-                if (i >= nb || lane >= pages) return -1;
-                const int page = ((block_of(u, u.c0 + i) * C::kKeys) >> c.shift) + lane;
-                if (!page_needed(c, u, page)) return -1;
-                const int id = table[page];
-                return c.is_page(id) ? id : -2;
-            };
-            const auto load = [&](int i, int mine, bool value) {
-                const int st = tile % C::kStages;
-                if (ok) ok = warp_wait(&sh.empty[st], (tile / C::kStages & 1) ^ 1);
-                if (!ok) return;
-                const bool bad = __any_sync(0xffffffffu, mine == -2);
+    if (w >= C::kSoft) {
+        if constexpr (C::kShift) fewer_registers();   // all four warps of the group
+        if (w == C::kSoft) {
+            // ---- units, and their keys and values. Pages of a block: one a lane.
+            const int box_rows = min(C::kKeys, c.page_size()), pages = C::kKeys / box_rows, boxes = pages * C::kBands;
+            uint32_t tile = 0, block = 0;   // so far
+            for (int k = 0; ok; ++k) {
+                const int slot = k % kUnitSlots;
+                ok = warp_wait(&sh.unit_empty[slot], (k / kUnitSlots & 1) ^ 1);
+                if (!ok || fer::dev::warp_flag(stop)) break;
+                const long long x = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
+                Unit u{};
+                u.tok0 = -1;
+                if (x < units) u = find_unit<D>(c, p, pre, sh.units, segments, seg, static_cast<int>(x));
                 if (lane == 0) {
-                    if (!value) {
-                        sh.bad[block % kBadRing] = bad;
-                        if (bad) fer::dev::report(p.err, fer::dev::kErrBadShape);
-                    }
-                    fer::dev::mbar_arrive_expect_tx(&sh.full[st], C::kTile);
+                    sh.unit[slot] = u;
+                    fer::dev::mbar_arrive(&sh.unit_full[slot]);
                 }
                 __syncwarp();
-                const int s0 = block_of(u, u.c0 + i) * C::kKeys;
-                for (int j0 = 0; j0 < boxes; j0 += 32) {
-                    const int j = j0 + lane, pg = j / C::kBands, band = j % C::kBands;
-                    const int id = __shfl_sync(0xffffffffu, mine, pg & 31);
-                    // slots of no page are read as page `pages`, outside the map: zeros
-                    if (j < boxes)
-                        load_box(ring + st * C::kTile + band * C::kBand + pg * box_rows * 128, value ? &v_map : &k_map,
-                                 band * 64, s0 & (c.page_size() - 1), u.hk, id < 0 ? c.pages : id, &sh.full[st]);
+                if (u.tok0 < 0) break;   // a later round has none either
+                const int32_t* const table = table_of(c, p, u);
+                const int nb = u.c1 - u.c0, lead = alternate<D>(u) ? 2 : 1;
+                // this lane's page of block i: -1 where there is none to read, -2 where its id is out of range
+                const auto page_at = [&](int i) {
+                    if (i >= nb || lane >= pages) return -1;
+                    const int page = ((block_of(u, u.c0 + i) * C::kKeys) >> c.shift) + lane;
+                    if (!page_needed(c, u, page)) return -1;
+                    const int id = table[page];
+                    return c.is_page(id) ? id : -2;
+                };
+                const auto load = [&](int i, int mine, bool value) {
+                    const int st = tile % C::kStages;
+                    if (ok) ok = warp_wait(&sh.empty[st], (tile / C::kStages & 1) ^ 1);
+                    if (!ok) return;
+                    const bool bad = __any_sync(0xffffffffu, mine == -2);
+                    if (lane == 0) {
+                        if (!value) {
+                            sh.bad[block % kBadRing] = bad;
+                            if (bad) fer::dev::report(p.err, fer::dev::kErrBadShape);
+                        }
+                        fer::dev::mbar_arrive_expect_tx(&sh.full[st], C::kTile);
+                    }
+                    __syncwarp();
+                    const int s0 = block_of(u, u.c0 + i) * C::kKeys;
+                    for (int j0 = 0; j0 < boxes; j0 += 32) {
+                        const int j = j0 + lane, pg = j / C::kBands, band = j % C::kBands;
+                        const int id = __shfl_sync(0xffffffffu, mine, pg & 31);
+                        // slots of no page are read as page `pages`, outside the map: zeros
+                        if (j < boxes)
+                            load_box(ring + st * C::kTile + band * C::kBand + pg * box_rows * 128, value ? &v_map : &k_map,
+                                     band * 64, s0 & (c.page_size() - 1), u.hk, id < 0 ? c.pages : id, &sh.full[st]);
+                    }
+                    ++tile;
+                    if (!value) ++block;
+                };
+                // ids of four blocks: i .. i + 3 when values i are loaded
+                int id0 = page_at(0), id1 = page_at(1), id2 = page_at(2);
+                if (nb > 0) load(0, id0, false);
+                if (lead == 2 && nb > 1) load(1, id1, false);
+                for (int i = 0; i < nb && ok; ++i) {
+                    const int id3 = page_at(i + 3);
+                    load(i, id0, true);
+                    if (i + lead < nb) load(i + lead, lead == 2 ? id2 : id1, false);
+                    id0 = id1, id1 = id2, id2 = id3;
                 }
-                ++tile;
-                if (!value) ++block;
-            };
-            // ids of four blocks: i .. i + 3 when values i are loaded
-            int id0 = page_at(0), id1 = page_at(1), id2 = page_at(2);
-            if (nb > 0) load(0, id0, false);
-            if (lead == 2 && nb > 1) load(1, id1, false);
-            for (int i = 0; i < nb && ok; ++i) {
-                const int id3 = page_at(i + 3);
-                load(i, id0, true);
-                if (i + lead < nb) load(i + lead, lead == 2 ? id2 : id1, false);
-                id0 = id1, id1 = id2, id2 = id3;
             }
-        }
-        if (!ok) {
-            if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutSync);
-            *stop = 1;
-        }
-        // the copies have landed before this warp leaves, whatever became of the others
-        for (uint32_t i = tile > C::kStages ? tile - C::kStages : 0; i < tile; ++i)
-            if (!warp_wait(&sh.full[i % C::kStages], i / C::kStages)) {
-                if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
+            if (!ok) {
+                if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutSync);
                 *stop = 1;
             }
-    } else if (w == C::kSoft + 1) {
-        // ---- products
-        uint32_t base = 0;                 // tiles of the units before
-        uint32_t n_q = 0, n_p[2] = {0, 0}; // phases so far
-        for (int k = 0; ok; ++k) {
-            const int slot = k % kUnitSlots;
-            ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
-            if (!ok || fer::dev::warp_flag(stop)) break;
-            const Unit u = sh.unit[slot];
-            __syncwarp();
-            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
-            if (u.tok0 < 0) break;
-            const int nb = u.c1 - u.c0;
-            if (nb == 0) continue;
-            const bool alt = alternate<D>(u), both = C::kSubs == 2 && !alt, fine = u.nf <= C::kFine;
-            ok = warp_wait(&sh.q_full, n_q++);
-            const auto product_s = [&](int x, int i, bool last) {   // last: no other sub-tile reads the tile
-                const uint32_t at = base + at_k(alt, i);
-                const int st = at % C::kStages;
-                if (!ok || !(ok = warp_wait(&sh.full[st], at / C::kStages))) return;
-                fence_after();
-                if (lane == 0) {
-                    const uint32_t q = smem + (both ? x * C::kQ : 0), kk = ring + st * C::kTile;
+            // the copies have landed before this warp leaves, whatever became of the others
+            for (uint32_t i = tile > C::kStages ? tile - C::kStages : 0; i < tile; ++i)
+                if (!warp_wait(&sh.full[i % C::kStages], i / C::kStages)) {
+                    if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
+                    *stop = 1;
+                }
+        } else if (w > C::kSoft && w <= C::kSoft + C::kSubs) {
+            // ---- products of sub-tile x. Each of these warps sees every tile of the ring, so that none can lap it, and lets go
+            // of those that are the other's as soon as they are there.
+            const int x = w - C::kSoft - 1;
+            const uint32_t s_at = tmem + 128 * x, o_at = tmem + C::kColO + x * D;
+            uint32_t tile = 0, n_q = 0, n_p = 0;   // so far
+            const auto landed = [&](uint32_t i) {
+                if (ok) ok = warp_wait(&sh.full[i % C::kStages], i / C::kStages);
+            };
+            const auto skip = [&]() {
+                landed(tile);
+                if (lane == 0) fer::dev::mbar_arrive(&sh.empty[tile % C::kStages]);
+                ++tile;
+            };
+            for (int k = 0; ok; ++k) {
+                const int slot = k % kUnitSlots;
+                ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
+                if (!ok || fer::dev::warp_flag(stop)) break;
+                const int nf = sh.unit[slot].nf, nb = sh.unit[slot].c1 - sh.unit[slot].c0;
+                const bool end = sh.unit[slot].tok0 < 0;
+                __syncwarp();
+                if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
+                if (end) break;
+                if (nb == 0) continue;
+                const bool alt = C::kSubs == 2 && nf <= 128, fine = nf <= C::kFine && nf > kFew;
+                const uint64_t q_desc = sdesc(smem + (alt ? 0 : x * C::kQ), 16, 1024);
+                ok = warp_wait(&sh.q_full, n_q++);
+                // S of the tile; last: of the unit, so that other queries may come
+                const auto product_s = [&](uint32_t i, bool last) {
+                    const uint64_t kk = sdesc(ring + i % C::kStages * C::kTile, 16, 1024);
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j)
-                        mma_ss(tmem + 128 * x, sdesc(q + (j / 4) * 16384 + (j % 4) * 32, 16, 1024),
-                               sdesc(kk + (j / 4) * C::kBand + (j % 4) * 32, 16, 1024), kIdS, j > 0);
+                        mma_ss(s_at, q_desc + ((j / 4) * 16384 + (j % 4) * 32) / 16,
+                               kk + ((j / 4) * C::kBand + (j % 4) * 32) / 16, kIdS, j > 0);
                     commit(&sh.s_full[x]);
-                    if (last) commit(&sh.empty[st]);
-                }
-                __syncwarp();
-            };
-            const auto product_o = [&](int x, int i, bool first, bool last, bool end) {
-                const uint32_t at = base + at_v(alt, i, nb);
-                const int st = at % C::kStages;
-                if (!ok || !(ok = warp_wait(&sh.p_full[x], n_p[x]++) && warp_wait(&sh.full[st], at / C::kStages))) return;
-                fence_after();
-                if (lane == 0) {
-                    const uint32_t o = tmem + C::kColO + x * D, pp = tmem + 128 * x, v = ring + st * C::kTile;
+                    commit(&sh.empty[i % C::kStages]);
+                    if (last) commit(&sh.q_empty);
+                };
+                const auto product_o = [&](uint32_t i, bool first) {
+                    const uint64_t v = sdesc(ring + i % C::kStages * C::kTile, C::kBand, 1024);
 #pragma unroll
-                    for (int j = 0; j < C::kKeys / 16; ++j)
-                        mma_ts(o, pp + 8 * j, sdesc(v + j * 2048, C::kBand, 1024), kIdO, !first || j > 0);
+                    for (int j = 0; j < C::kKeys / 16; ++j) mma_ts(o_at, s_at + 8 * j, v + j * (2048 / 16), kIdO, !first || j > 0);
                     if (fine)
 #pragma unroll
                         for (int j = 0; j < C::kKeys / 16; ++j)
-                            mma_ts(o, pp + C::kKeys / 2 + 8 * j, sdesc(v + j * 2048, C::kBand, 1024), kIdO, 1);
-                    if (last) commit(&sh.empty[st]);
-                    if (end) commit(&sh.o_full[x]);
+                            mma_ts(o_at, s_at + C::kKeys / 2 + 8 * j, v + j * (2048 / 16), kIdO, 1);
+                    commit(&sh.empty[i % C::kStages]);
+                };
+                // K_0 V_0 K_1 V_1 ..., or K_0 K_1 V_0 K_2 V_1 ... where even blocks are sub-tile 0's: either way the values
+                // of a block are followed by the keys of this sub-tile's next
+                const int step = alt ? 2 : 1;
+                if (alt && x == 1) skip();                                   // K_0
+                if (alt && x == 1 && nb == 1) {
+                    skip();                                                  // V_0
+                    if (lane == 0) fer::dev::mbar_arrive(&sh.q_empty);
+                    continue;
                 }
-                __syncwarp();
-            };
-            if (alt) {
-                product_s(0, 0, true);
-                if (nb > 1) product_s(1, 1, true);
-                for (int i = 0; i < nb && ok; ++i) {
-                    product_o(i & 1, i, i < 2, true, i + 2 >= nb);
-                    if (i + 2 < nb) product_s(i & 1, i + 2, true);
+                landed(tile);
+                if (ok) {
+                    fence_after();
+                    if (lane == 0) product_s(tile, step >= nb - (alt ? x : 0));
+                    __syncwarp();
                 }
-            } else {
-                product_s(0, 0, !both);
-                if (both) product_s(1, 0, true);
-                for (int i = 0; i < nb && ok; ++i) {
-                    product_o(0, i, i == 0, !both, i + 1 == nb);
-                    if (i + 1 < nb) product_s(0, i + 1, !both);
-                    if (both) {
-                        product_o(1, i, i == 0, true, i + 1 == nb);
-                        if (i + 1 < nb) product_s(1, i + 1, true);
+                ++tile;
+                if (alt && x == 0 && nb > 1) skip();                         // K_1
+                for (int i = alt ? x : 0; i < nb; i += step) {
+                    if (alt && i > 0) {
+                        skip();                                              // the other's V_{i-1}
+                        if (i + 1 < nb) skip();                              // and K_{i+1}
                     }
+                    const bool more = i + step < nb;
+                    landed(tile);
+                    if (more) landed(tile + 1);
+                    if (ok) ok = warp_wait(&sh.p_full[x], n_p);
+                    ++n_p;
+                    if (ok) {
+                        fence_after();
+                        if (lane == 0) {
+                            product_o(tile, i < step);
+                            if (more) product_s(tile + 1, i + 2 * step >= nb);
+                            else commit(&sh.o_full[x]);
+                        }
+                        __syncwarp();
+                    }
+                    tile += more ? 2 : 1;
                 }
+                if (alt && (nb - 1) % 2 != x) skip();                        // the other's last values
             }
-            base += 2 * nb;
-        }
-        if (!ok) {
-            if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
-            *stop = 1;
+            if (!ok) {
+                if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
+                *stop = 1;
+            }
+        } else {
+            // ---- queries of units of at most 128 rows, read while the unit before still computes; few rows go to each
+            // quarter of the sub-tile
+            uint32_t n_q = 0;
+            for (int k = 0; ok; ++k) {
+                const int slot = k % kUnitSlots;
+                ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
+                if (!ok || fer::dev::warp_flag(stop)) break;
+                const Unit u = sh.unit[slot];
+                __syncwarp();
+                if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
+                if (u.tok0 < 0) break;
+                if (u.c1 == u.c0) continue;
+                const bool mine = loads_ahead<D>(u);
+                constexpr int kAhead = 4;
+                uint4 v[kAhead];
+                const int n = mine ? u.nf * (D / 8) : 0;
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (j * 32 + lane < n) v[j] = q_piece<T, D>(p, u, j * 32 + lane);
+                ok = warp_wait(&sh.q_empty, n_q++ ^ 1u);   // the unit before has multiplied its last keys
+                if (!mine) continue;
+                const int copies = u.nf <= kFew ? 4 : 1;
+                for (int i0 = lane; i0 < n; i0 += 32 * kAhead) {
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j) {
+                        const int i = i0 + 32 * j;
+                        if (i >= n) break;
+                        for (int g = 0; g < copies; ++g)
+                            *reinterpret_cast<uint4*>(smem_at + q_place<D>(i / (D / 8) + 32 * g, i % (D / 8))) = v[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j)
+                        if (i0 + 32 * (kAhead + j) < n) v[j] = q_piece<T, D>(p, u, i0 + 32 * (kAhead + j));
+                }
+                fer::dev::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_n(&sh.q_full, C::kSoft);
+            }
+            if (!ok) {
+                if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutSync);
+                *stop = 1;
+            }
         }
     } else {
-        // ---- softmax, a row a thread
-        const int x = w >> 2, r = t & 127;
+        // ---- softmax, a row a thread; of few rows (kFew) each is in all four quarters of a sub-tile: two take the first and two
+        // the second half of a block's keys, and of each two one keeps P's upper and one its lower 16 bits
+        if constexpr (C::kShift) more_registers();
+        constexpr int kChunks = C::kKeys / 32;
+        const int x = w >> 2, r = t & 127, half = (w >> 1) & 1, part = w & 1;
         const uint32_t row_at = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16), s_at = row_at + 128 * x;
         uint32_t base = 0, block = 0, n_s = 0, n_o = 0;
-        const bool wide_q = (reinterpret_cast<uintptr_t>(p.q) | (p.qs * 2)) % 16 == 0;
         const bool wide_o = (reinterpret_cast<uintptr_t>(p.out) | (p.os * 2)) % 16 == 0;
         for (int k = 0;; ++k) {
             const int slot = k % kUnitSlots;
             ok = ok && warp_wait(&sh.unit_full[slot], k / kUnitSlots);
             // both sub-tiles' warps leave together: each unit has barriers for all of them
             if (!ok) *stop = 1;
-            meet<32 * C::kSoft>();   // and the unit before is done with its queries, sums and results
+            meet<32 * C::kSoft>();   // and the unit before is done with its sums and results
             if (t == 0) sh.leave = *stop;
             meet<32 * C::kSoft>();
             if (sh.leave) {
@@ -698,114 +834,115 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
             if (u.tok0 < 0) break;
             const int nb = u.c1 - u.c0;
-            const bool alt = alternate<D>(u), fine = u.nf <= C::kFine;
-            if (nb > 0) {
-                constexpr int kPieces = D / 8;
-                for (int i = t; i < u.nf * kPieces; i += 32 * C::kSoft) {
-                    const int f = i / kPieces, pc = i % kPieces;
-                    const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + q_row(p, u, f) * p.qs +
-                                          static_cast<size_t>(q_head(p, u, f)) * D + pc * 8;
-                    uint4 v;
-                    if (wide_q) {
-                        v = *reinterpret_cast<const uint4*>(src);
-                    } else {
-                        uint32_t e[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
-                        v = make_uint4(e[0], e[1], e[2], e[3]);
-                    }
-                    *reinterpret_cast<uint4*>(smem_at + (f >> 7) * C::kQ + (pc >> 3) * 16384 + (f & 127) * 128 +
-                                              (((pc ^ f) & 7) << 4)) = v;
-                }
+            const bool alt = alternate<D>(u), few = u.nf <= kFew, fine = u.nf <= C::kFine;
+            if (nb > 0 && !loads_ahead<D>(u)) {
+                for (int i = t; i < u.nf * (D / 8); i += 32 * C::kSoft)
+                    *reinterpret_cast<uint4*>(smem_at + q_place<D>(i / (D / 8), i % (D / 8))) = q_piece<T, D>(p, u, i);
                 fer::dev::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) fer::dev::mbar_arrive(&sh.q_full);
             }
-            const int f = alt ? r : x * 128 + r, first = alt ? x : 0, step = alt ? 2 : 1;
+            const int f = few ? lane : alt ? r : x * 128 + r, first = alt ? x : 0, step = alt ? 2 : 1;
             const bool rows_here = (f & ~31) < u.nf;                       // of the warp
             const Sees sees(p, u, min(f, u.nf - 1));
             // what every row of the warp sees, for blocks that need no mask
             const int all_end = __reduce_min_sync(0xffffffffu, sees.end), all_begin = __reduce_max_sync(0xffffffffu, sees.begin);
             float m = -INFINITY, l = 0.0f;
             const int32_t* const table = table_of(c, p, u);
+
+            // a block's probabilities of N chunks of 32 keys from chunk j0 on; kind 0: rounded, 1: and what that leaves,
+            // 2: one of the two for these keys, and 0 for the others
+            const auto softmax = [&](auto chunks, auto kind, int j0, int i, int s0) {
+                constexpr int N = decltype(chunks)::value, kKind = decltype(kind)::value;
+                const bool plain = s0 + C::kKeys <= all_end && (s0 >= all_begin || s0 + C::kKeys <= sees.sink);
+                const bool bad = sh.bad[(block + i) % kBadRing] != 0;
+                float v[N][32];
+#pragma unroll
+                for (int j = 0; j < N; ++j) tmem_ld(s_at + 32 * (j0 + j), v[j]);
+                wait_ld(v);
+                if (!plain || bad) {
+                    // [b0, e0) of the window and [0, k0) of the sinks, within the chunks
+                    const int s1 = s0 + 32 * j0;
+                    const int b0 = sees.begin - s1, e0 = sees.end - s1, k0 = min(sees.sink, sees.end) - s1;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        uint32_t on = (below(e0 - 32 * j) & ~below(b0 - 32 * j)) | below(k0 - 32 * j);
+                        if (bad)
+                            for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
+                                const int page = (s1 + 32 * j + e) >> c.shift;
+                                if (!page_needed(c, u, page) || !c.is_page(table[page])) on &= ~(0xffu << e);
+                            }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(on >> e & 1u)) v[j][e] = -INFINITY;
+                    }
+                }
+                float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+#pragma unroll
+                for (int e = 4; e < 32 * N; e += 2)
+                    mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[e >> 5][e & 31], v[e >> 5][(e & 31) + 1]);
+                const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * p.scale2;
+                const bool raise = top > m + kSlack;
+                const float m1 = raise ? top : m, shift = m1 == -INFINITY ? 0.0f : m1;
+                const float a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
+                m = m1;
+                if (i > first && __any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+                    for (int j = 0; j < D / 16; ++j) {
+                        uint32_t o[16];
+                        tmem_ld16(row_at + C::kColO + x * D + 16 * j, o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                        tmem_st16(row_at + C::kColO + x * D + 16 * j, o);
+                    }
+                }
+                const uint64_t sc2 = fer::dev::f2_splat(p.scale2), nm2 = fer::dev::f2_splat(kUp - shift);
+                uint64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    uint32_t hi[16], low[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float p0, p1;
+                        const uint64_t t2 = fer::dev::f2_fma(fer::dev::f2_pack(v[j][e], v[j][e + 1]), sc2, nm2);
+                        if (kKind == 0 && (e >> 1) % kPolyOf < kPoly) {
+                            powers2(t2, p0, p1);
+                        } else {
+                            fer::dev::f2_unpack(t2, p0, p1);
+                            p0 = ex2(p0), p1 = ex2(p1);
+                        }
+                        sum[(e >> 1) & 3] = fer::dev::f2_add(sum[(e >> 1) & 3], fer::dev::f2_pack(p0, p1));
+                        hi[e >> 1] = pack2<T>(p0, p1);
+                        if constexpr (kKind > 0) {
+                            float h0, h1;
+                            unpack2<T>(hi[e >> 1], h0, h1);
+                            low[e >> 1] = pack2<T>(p0 - h0, p1 - h1);
+                            if (kKind == 2 && part) hi[e >> 1] = low[e >> 1];
+                        }
+                    }
+                    tmem_st16(s_at + 16 * (j0 + j), hi);
+                    if constexpr (kKind == 1) tmem_st16(s_at + C::kKeys / 2 + 16 * j, low);
+                    if constexpr (kKind == 2) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) low[e] = 0;
+                        tmem_st16(s_at + 16 * (N - j0 + j), low);
+                    }
+                }
+                float sm[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fer::dev::f2_unpack(sum[j], sm[2 * j], sm[2 * j + 1]);
+                l = l * a + (((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7])));
+                wait_st();
+            };
             for (int i = first; i < nb; i += step) {
                 if (ok) ok = warp_wait(&sh.s_full[x], n_s);
                 ++n_s;
                 fence_after();
                 const int s0 = block_of(u, u.c0 + i) * C::kKeys;
                 if (rows_here && ok) {
-                    const bool plain = s0 + C::kKeys <= all_end && (s0 >= all_begin || s0 + C::kKeys <= sees.sink);
-                    const bool bad = sh.bad[(block + i) % kBadRing] != 0;
-                    // [b0, e0) of the window and [0, k0) of the sinks, within the block
-                    const int b0 = sees.begin - s0, e0 = sees.end - s0, k0 = min(sees.sink, sees.end) - s0;
-                    const auto scores = [&](int j, float (&v)[32]) {   // 32 of the block, -inf where the row sees none
-                        tmem_ld(s_at + 32 * j, v);
-                        if (plain && !bad) return;
-                        uint32_t on = (below(e0 - 32 * j) & ~below(b0 - 32 * j)) | below(k0 - 32 * j);
-                        if (bad)
-                            for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
-                                const int page = (s0 + 32 * j + e) >> c.shift;
-                                if (!page_needed(c, u, page) || !c.is_page(table[page])) on &= ~(0xffu << e);
-                            }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(on >> e & 1u)) v[e] = -INFINITY;
-                    };
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int j = 0; j < C::kKeys / 32; ++j) {
-                        float v[32];
-                        scores(j, v);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[e], v[e + 1]);
-                    }
-                    const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * p.scale2;
-                    const bool raise = top > m + kSlack;
-                    const float m1 = raise ? top : m, shift = m1 == -INFINITY ? 0.0f : m1;
-                    const float a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
-                    m = m1;
-                    if (i > first && __any_sync(0xffffffffu, raise)) {
-#pragma unroll 1
-                        for (int j = 0; j < D / 16; ++j) {
-                            uint32_t o[16];
-                            tmem_ld16(row_at + C::kColO + x * D + 16 * j, o);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-                            tmem_st16(row_at + C::kColO + x * D + 16 * j, o);
-                        }
-                    }
-                    const uint64_t sc2 = fer::dev::f2_splat(p.scale2), nm2 = fer::dev::f2_splat(kUp - shift);
-                    uint64_t sum[4] = {0, 0, 0, 0};
-                    uint32_t low[C::kKeys / 2];   // kept to the end: they lie over scores
-#pragma unroll
-                    for (int j = 0; j < C::kKeys / 32; ++j) {
-                        float v[32];
-                        uint32_t hi[16];
-                        scores(j, v);
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            float p0, p1;
-                            fer::dev::f2_unpack(fer::dev::f2_fma(fer::dev::f2_pack(v[e], v[e + 1]), sc2, nm2), p0, p1);
-                            p0 = ex2(p0), p1 = ex2(p1);
-                            sum[(e >> 1) & 3] = fer::dev::f2_add(sum[(e >> 1) & 3], fer::dev::f2_pack(p0, p1));
-                            hi[e >> 1] = pack2<T>(p0, p1);
-                            if (fine) {
-                                float h0, h1;
-                                unpack2<T>(hi[e >> 1], h0, h1);
-                                low[16 * j + (e >> 1)] = pack2<T>(p0 - h0, p1 - h1);
-                            }
-                        }
-                        tmem_st16(s_at + 16 * j, hi);
-                    }
-                    if (fine)
-#pragma unroll
-                        for (int j = 0; j < C::kKeys / 32; ++j)
-                            tmem_st16(s_at + C::kKeys / 2 + 16 * j, *reinterpret_cast<uint32_t(*)[16]>(low + 16 * j));
-                    float sm[8];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) fer::dev::f2_unpack(sum[j], sm[2 * j], sm[2 * j + 1]);
-                    l = l * a + (((sm[0] + sm[1]) + (sm[2] + sm[3])) + ((sm[4] + sm[5]) + (sm[6] + sm[7])));
-                    wait_st();
+                    if (few) softmax(std::integral_constant<int, kChunks / 2>{}, std::integral_constant<int, 2>{}, half * (kChunks / 2), i, s0);
+                    else if (fine) softmax(std::integral_constant<int, kChunks>{}, std::integral_constant<int, 1>{}, 0, i, s0);
+                    else softmax(std::integral_constant<int, kChunks>{}, std::integral_constant<int, 0>{}, 0, i, s0);
                 }
                 // values of slots that no row sees count as zero, whatever is there
                 const bool behind = s0 + C::kKeys > u.hi, before = s0 < u.lo && s0 + C::kKeys > u.sink;
@@ -817,8 +954,8 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         for (int j = r; j < C::kKeys * (D / 8); j += 128) {
                             const int e = j / (D / 8), pc = j % (D / 8), s = s0 + e;
                             if (s < u.hi && (s >= u.lo || s < u.sink)) continue;
-                            *reinterpret_cast<uint4*>(smem_at + C::kSubs * C::kQ + st * C::kTile + (pc >> 3) * C::kBand +
-                                                      e * 128 + ((pc & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(smem_at + C::kRing + st * C::kTile + (pc >> 3) * C::kBand + e * 128 +
+                                                      ((pc & 7) << 4)) = make_uint4(0, 0, 0, 0);
                         }
                     fer::dev::fence_proxy_async_smem();
                 }
@@ -834,91 +971,158 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             fence_after();
             base += 2 * nb, block += nb;
 
-            // the results: where blocks alternate each sub-tile's warps take half of the dims of both sums
-            float ml = m, wa = 1.0f, wb = 0.0f, total = l;
-            int d0 = 0, d1 = D;
-            uint32_t at_a = row_at + C::kColO + x * D, at_b = at_a;
-            if (alt) {
-                // the queries' second half is free in such a unit
-                float2* const sums = reinterpret_cast<float2*>(smem_at + (C::kSubs - 1) * C::kQ);
+            // The results. Where blocks alternate, or rows are in several quarters, a row's sums meet first; everything stops
+            // at the next unit where a wait ran out.
+            float2* const sums = reinterpret_cast<float2*>(smem_at + C::kMeet);
+            const uint32_t o_at = row_at + C::kColO + x * D;
+            unsigned again = 0;     // rows of this warp's share that are computed again
+            int d0 = 0, d1 = D;     // this warp's dims of them
+            if (few) {
+                constexpr int kParts = 4 * C::kSubs;   // sums of a row; m and l are those of half of them
                 sums[t] = make_float2(m, l);
                 meet<32 * C::kSoft>();
-                const float2 sa = sums[r], sb = sums[128 + r];
-                const float ma = sa.x, mb = sb.x;
-                ml = fmaxf(ma, mb);
-                const float base2 = ml == -INFINITY ? 0.0f : ml;
-                wa = ex2(ma - base2), wb = ex2(mb - base2);
-                total = sa.y * wa + sb.y * wb;
-                d0 = x * (D / 2), d1 = d0 + D / 2;
-                at_a = row_at + C::kColO, at_b = at_a + D;
-                fence_after();
-            }
-            // (the barriers of a unit that ended early are not waited for: everything stops below)
-            const bool on = f < u.nf;
-            const int fr = min(f, u.nf - 1), head = q_head(p, u, fr);
-            const size_t tok = q_row(p, u, fr), bh = tok * p.heads + head, part = bh * p.parts + max(u.part, 0);
-            T* const out = static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D;
-            const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
-            bool nan = false;
-            if (rows_here && ok) {
-#pragma unroll 1
-                for (int d = d0; d < d1; d += 32) {
-                    float o[32];
-                    if (nb > 0) {
-                        tmem_ld(at_a + d, o);
-                        if (alt && nb > 1) {
-                            float o1[32];
-                            tmem_ld(at_b + d, o1);
+                float all = -INFINITY, total = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = fmaf(o[e], wa, o1[e] * wb);
+                for (int i = 0; i < kParts; i += 2) all = fmaxf(all, sums[32 * i + lane].x);
+                const float base2 = all == -INFINITY ? 0.0f : all;
+#pragma unroll
+                for (int i = 0; i < kParts; i += 2) total = fmaf(sums[32 * i + lane].y, ex2(sums[32 * i + lane].x - base2), total);
+                const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+                const float mine2 = mine && ok ? ex2(m - base2) * scale : 0.0f;
+                meet<32 * C::kSoft>();                 // the sums have been read
+                const bool on = lane < u.nf;
+                if (w == 0 && on) {
+                    const size_t bh = q_row(p, u, lane) * p.heads + q_head(p, u, lane);
+                    if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (bh * p.parts + u.part)) = make_float2(all, total);
+                    else if (p.lse) p.lse[bh] = total == 0.0f ? -INFINITY : (all + (log2f(total) - kUp)) * kLn2;
+                }
+                // as many dims at once as there is room for: 4 KB a warp
+                const int width = min(D, u.nf <= 8 ? 128 : u.nf <= 16 ? 64 : 32), rows = 1024 / width;
+                float* const meet_at = reinterpret_cast<float*>(smem_at + C::kMeet);
+                for (int d = 0; d < D; d += width) {
+                    for (int e0 = 0; e0 < width; e0 += 32) {
+                        float o[1][32];
+                        if (mine && ok) {
+                            tmem_ld(o_at + d + e0, o[0]);
+                            wait_ld(o);
                         }
+                        if (on) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                // 16-byte pieces of neighbouring rows in different banks
+                                float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                if (mine && ok) q = make_float4(o[0][e] * mine2, o[0][e + 1] * mine2, o[0][e + 2] * mine2, o[0][e + 3] * mine2);
+                                *reinterpret_cast<float4*>(meet_at + (w * rows + lane) * width + e0 + ((e ^ (lane << 2)) & 28)) = q;
+                            }
+                        }
+                        __syncwarp();
                     }
+                    meet<32 * C::kSoft>();
+                    for (int i = t; i < u.nf * width; i += 32 * C::kSoft) {
+                        const int row = i / width, e = i % width;
+                        const float* const from = meet_at + row * width + (e & ~31) + (((e ^ (row << 2)) & 28) | (e & 3));
+                        float v = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        o[e] = nb > 0 ? o[e] * scale : 0.0f;
-                        nan = nan || !(o[e] - o[e] == 0.0f);   // infinite ones too: they may be 0 x inf elsewhere
+                        for (int g = 0; g < kParts; ++g) v += from[g * rows * width];
+                        if (nb == 0) v = 0.0f;
+                        if (!(v - v == 0.0f)) atomicOr(&sh.again, 1u << row);   // infinite ones too: it may be 0 x inf elsewhere
+                        const size_t tok = q_row(p, u, row);
+                        const int head = q_head(p, u, row);
+                        if (u.part >= 0) p.part_o[((tok * p.heads + head) * p.parts + u.part) * D + d + e] = v;
+                        else put(static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D + d + e, v);
                     }
-                    if (on && u.part >= 0) {
-                        float4* const to = reinterpret_cast<float4*>(p.part_o + part * D + d);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                    } else if (on && wide_o) {
-                        uint4* const to = reinterpret_cast<uint4*>(out + d);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            to[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
-                                               pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
-                    } else if (on) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) put(out + d + e, o[e]);
-                    }
-                    __syncwarp();
+                    meet<32 * C::kSoft>();
                 }
-                if (on && (!alt || x == 0)) {
-                    if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * part) = make_float2(ml, total);
-                    else if (p.lse) p.lse[bh] = total == 0.0f ? -INFINITY : (ml + (log2f(total) - kUp)) * kLn2;
+                const uint32_t all_again = sh.again;
+                if (all_again) {                       // the same for all of these warps
+                    meet<32 * C::kSoft>();
+                    if (t == 0) sh.again = 0;
+                    for (int g = w; g < u.nf; g += C::kSoft)
+                        if (all_again >> g & 1u) again |= 1u << g;
                 }
-                unsigned again = __ballot_sync(0xffffffffu, on && nan && nb > 0);
-                while (again) {
-                    const int src = __ffs(again) - 1;
-                    again &= again - 1;
-                    const int g = (f & ~31) + src;
-                    float m2, l2, o2[D / 32];
-                    one_row<T, D>(c, p, u, g, m2, l2, o2);
-                    const int gh = q_head(p, u, g);
-                    const size_t gt = q_row(p, u, g), gp = (gt * p.heads + gh) * p.parts + max(u.part, 0);
+            } else {
+                float all = m, wa = 1.0f, wb = 0.0f, total = l;
+                uint32_t at_a = o_at, at_b = o_at;
+                if (alt) {   // each sub-tile's warps take half of the dims of both sums
+                    sums[t] = make_float2(m, l);
+                    meet<32 * C::kSoft>();
+                    const float2 sa = sums[r], sb = sums[128 + r];
+                    all = fmaxf(sa.x, sb.x);
+                    const float base2 = all == -INFINITY ? 0.0f : all;
+                    wa = ex2(sa.x - base2), wb = ex2(sb.x - base2);
+                    total = sa.y * wa + sb.y * wb;
+                    d0 = x * (D / 2), d1 = d0 + D / 2;
+                    at_a = row_at + C::kColO, at_b = at_a + D;
+                    fence_after();
+                }
+                const bool on = f < u.nf;
+                const int fr = min(f, u.nf - 1), head = q_head(p, u, fr);
+                const size_t tok = q_row(p, u, fr), bh = tok * p.heads + head, place = bh * p.parts + max(u.part, 0);
+                T* const out = static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D;
+                const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
+                bool nan = false;
+                if (rows_here && ok) {
+#pragma unroll 1
+                    for (int d = d0; d < d1; d += 32) {
+                        float oo[2][32];
+                        float(&o)[32] = oo[0];
+                        if (nb > 0) {
+                            tmem_ld(at_a + d, oo[0]);
+                            tmem_ld(at_b + d, oo[1]);
+                            wait_ld(oo);
+                            if (alt && nb > 1) {
 #pragma unroll
-                    for (int j = 0; j < D / 32; ++j) {
-                        const int d = 32 * j + lane;
-                        if (d < d0 || d >= d1) continue;
-                        if (u.part >= 0) p.part_o[gp * D + d] = o2[j];
-                        else put(static_cast<T*>(p.out) + gt * p.os + static_cast<size_t>(gh) * D + d, l2 == 0.0f ? 0.0f : o2[j] / l2);
+                                for (int e = 0; e < 32; ++e) o[e] = fmaf(o[e], wa, oo[1][e] * wb);
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            o[e] = nb > 0 ? o[e] * scale : 0.0f;
+                            nan = nan || !(o[e] - o[e] == 0.0f);
+                        }
+                        if (on && u.part >= 0) {
+                            float4* const to = reinterpret_cast<float4*>(p.part_o + place * D + d);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        } else if (on && wide_o) {
+                            uint4* const to = reinterpret_cast<uint4*>(out + d);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                to[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
+                                                   pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+                        } else if (on) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) put(out + d + e, o[e]);
+                        }
+                        __syncwarp();
                     }
-                    // l is of 2^(s - m + kUp) elsewhere
-                    if (lane == 0 && u.part >= 0 && (!alt || x == 0))
-                        *reinterpret_cast<float2*>(p.part_ml + 2 * gp) = make_float2(m2 + kUp, l2);
-                    __syncwarp();
+                    if (on && (!alt || x == 0)) {
+                        if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * place) = make_float2(all, total);
+                        else if (p.lse) p.lse[bh] = total == 0.0f ? -INFINITY : (all + (log2f(total) - kUp)) * kLn2;
+                    }
+                    again = __ballot_sync(0xffffffffu, on && nan && nb > 0);
                 }
+            }
+            while (again) {
+                const int src = __ffs(again) - 1;
+                again &= again - 1;
+                const int g = few ? src : (f & ~31) + src;
+                float m2, l2, o2[D / 32];
+                one_row<T, D>(c, p, u, g, m2, l2, o2);
+                const int gh = q_head(p, u, g);
+                const size_t gt = q_row(p, u, g), bh = gt * p.heads + gh, place = bh * p.parts + max(u.part, 0);
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    const int d = 32 * j + lane;
+                    if (d < d0 || d >= d1) continue;
+                    if (u.part >= 0) p.part_o[place * D + d] = o2[j];
+                    else put(static_cast<T*>(p.out) + gt * p.os + static_cast<size_t>(gh) * D + d, l2 == 0.0f ? 0.0f : o2[j] / l2);
+                }
+                if (lane == 0 && d0 == 0) {   // l is of 2^(s - m + kUp) elsewhere
+                    if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * place) = make_float2(m2 + kUp, l2);
+                    else if (p.lse) p.lse[bh] = l2 == 0.0f ? -INFINITY : (m2 + log2f(l2)) * kLn2;
+                }
+                __syncwarp();
             }
             fence_before();
         }
