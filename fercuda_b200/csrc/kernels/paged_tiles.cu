@@ -292,30 +292,37 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
 
-// Shared-memory matrix descriptor, 128-byte swizzle.
-__device__ __forceinline__ uint64_t sdesc(uint32_t at, uint32_t lbo, uint32_t sbo) {
-    return static_cast<uint64_t>((at >> 4) & 0x3FFFu) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 |
-           static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32 | 1ull << 46 | 2ull << 61;
-}
+// Shared-memory matrix descriptors, 128-byte swizzle, 1024 bytes from eight rows to the next: the upper word is the same for
+// all, the lower has the address and the bytes from one band to the next, so a step along the tile is one addition.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_low(uint32_t at, uint32_t band) { return ((at >> 4) & 0x3FFFu) | ((band >> 4) & 0x3FFFu) << 16; }
 // kind::f16, f32 sums, M = 128: N, type of both operands, and whether B has N as its contiguous dimension.
 __host__ __device__ constexpr uint32_t idesc(int n, bool bf16, bool b_by_n) {
     return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_by_n ? 1u << 16 : 0u) | (static_cast<uint32_t>(n) >> 3) << 17 |
            (128u >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"(acc), "r"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tmov.b64 y, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"(acc), "r"(kDescHigh)
         : "memory");
 }
+// One thread of the warp, the same every time.
+__device__ __forceinline__ bool elected() {
+    uint32_t on;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+    return on != 0;
+}
+// A value that the warp's threads share, known to be one.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(fer::dev::smem_addr(bar))
                  : "memory");
@@ -675,8 +682,8 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
         } else if (w > C::kSoft && w <= C::kSoft + C::kSubs) {
             // ---- products of sub-tile x. Each of these warps sees every tile of the ring, so that none can lap it, and lets go
             // of those that are the other's as soon as they are there.
-            const int x = w - C::kSoft - 1;
-            const uint32_t s_at = tmem + 128 * x, o_at = tmem + C::kColO + x * D;
+            const int x = uniform(w - C::kSoft - 1);
+            const uint32_t s_at = uniform(tmem) + 128 * x, o_at = uniform(tmem) + C::kColO + x * D;
             uint32_t tile = 0, n_q = 0, n_p = 0;   // so far
             const auto landed = [&](uint32_t i) {
                 if (ok) ok = warp_wait(&sh.full[i % C::kStages], i / C::kStages);
@@ -690,18 +697,18 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 const int slot = k % kUnitSlots;
                 ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
                 if (!ok || fer::dev::warp_flag(stop)) break;
-                const int nf = sh.unit[slot].nf, nb = sh.unit[slot].c1 - sh.unit[slot].c0;
-                const bool end = sh.unit[slot].tok0 < 0;
+                const int nf = uniform(sh.unit[slot].nf), nb = uniform(sh.unit[slot].c1 - sh.unit[slot].c0);
+                const bool end = uniform(sh.unit[slot].tok0) < 0;
                 __syncwarp();
                 if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
                 if (end) break;
                 if (nb == 0) continue;
                 const bool alt = C::kSubs == 2 && nf <= 128, fine = nf <= C::kFine && nf > kFew;
-                const uint64_t q_desc = sdesc(smem + (alt ? 0 : x * C::kQ), 16, 1024);
+                const uint32_t q_desc = desc_low(smem + (alt ? 0 : x * C::kQ), 16);
                 ok = warp_wait(&sh.q_full, n_q++);
                 // S of the tile; last: of the unit, so that other queries may come
                 const auto product_s = [&](uint32_t i, bool last) {
-                    const uint64_t kk = sdesc(ring + i % C::kStages * C::kTile, 16, 1024);
+                    const uint32_t kk = desc_low(ring + i % C::kStages * C::kTile, 16);
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j)
                         mma_ss(s_at, q_desc + ((j / 4) * 16384 + (j % 4) * 32) / 16,
@@ -711,7 +718,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     if (last) commit(&sh.q_empty);
                 };
                 const auto product_o = [&](uint32_t i, bool first) {
-                    const uint64_t v = sdesc(ring + i % C::kStages * C::kTile, C::kBand, 1024);
+                    const uint32_t v = desc_low(ring + i % C::kStages * C::kTile, C::kBand);
 #pragma unroll
                     for (int j = 0; j < C::kKeys / 16; ++j) mma_ts(o_at, s_at + 8 * j, v + j * (2048 / 16), kIdO, !first || j > 0);
                     if (fine)
@@ -732,7 +739,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 landed(tile);
                 if (ok) {
                     fence_after();
-                    if (lane == 0) product_s(tile, step >= nb - (alt ? x : 0));
+                    if (elected()) product_s(tile, step >= nb - (alt ? x : 0));
                     __syncwarp();
                 }
                 ++tile;
@@ -749,7 +756,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     ++n_p;
                     if (ok) {
                         fence_after();
-                        if (lane == 0) {
+                        if (elected()) {
                             product_o(tile, i < step);
                             if (more) product_s(tile + 1, i + 2 * step >= nb);
                             else commit(&sh.o_full[x]);
