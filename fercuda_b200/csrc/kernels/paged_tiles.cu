@@ -75,16 +75,14 @@ template <int D> struct Cut {
     static constexpr int kStages = D == 64 ? 8 : D == 128 ? 5 : 4;
     static constexpr int kQ = 128 * D * 2;           // queries of a sub-tile
     static constexpr int kSoft = 4 * kSubs;          // softmax warps
+    static constexpr int kParts = kKeys / 64;        // 64 keys at a time
     // Softmax warps, one that loads keys and values, one for each sub-tile that issues products, one that loads queries.
-    // Registers: of 168 a thread at launch the two groups of four softmax warps take 224 and leave the third group's warps
-    // 56. (One group has enough at launch.)
-    static constexpr bool kShift = kSubs == 2;
     static constexpr int kThreads = 32 * (kSoft + kSubs + 2);
     static constexpr int kRing = kSubs * kQ;         // where the ring begins
     // Where a unit's warps add up their results: the second sub-tile's queries, which such a unit does not have, or 32 KB more
     static constexpr int kMeet = D == 128 ? kQ : kRing + kStages * kTile;
     static constexpr int kSmem = kRing + kStages * kTile + (D == 128 ? 0 : 32768) + 1024;
-    static constexpr uint32_t kColO = 256;           // O of sub-tile x at kColO + x D, S and P at 128 x
+    static constexpr uint32_t kColO = 256;           // O of sub-tile x at kColO + x D, S and P of 64 keys at 128 x and 128 x + 64
     // rows up to which P's rounding is made up for
     static constexpr int kFine = kSubs == 2 ? 128 : 64;
 };
@@ -117,6 +115,7 @@ struct Unit {
     int hk, seq;       // seq -1: the prefix
     int slot0;         // the first token's slot
     int hi, lo, sink;  // visible to some row: slots below hi that are below sink or not below lo
+    int all_hi, all_lo;   // to every row: those below all_hi that are below sink or not below all_lo
     int sb, wb0;       // key blocks: 0 .. sb - 1, then wb0 ..
     int c0, c1;        // of them, counted in that order, the unit's
     int part;          // -1: the only one of its rows
@@ -159,6 +158,8 @@ __device__ __forceinline__ int tile_range(const TileParams& p, const Seq& q, int
     const int first = u.slot0 + u.f0 / p.group, last = u.slot0 + (u.f0 + u.nf - 1) / p.group;
     u.hi = max(last + 1, 0);
     u.lo = p.window == INT_MAX ? 0 : max(first + 1 - p.window, 0);
+    u.all_hi = max(first + 1, 0);
+    u.all_lo = p.window == INT_MAX ? 0 : max(last + 1 - p.window, 0);
     u.sink = min(p.sinks, u.hi);
     const int end = (u.hi + C::kKeys - 1) / C::kKeys;
     u.wb0 = min(u.lo / C::kKeys, end);
@@ -210,7 +211,7 @@ __device__ __forceinline__ Unit find_unit(const Paged& c, const TileParams& p, c
         u.seq = -1;
         u.f0 = t * C::kRows;
         u.nf = static_cast<int>(min(static_cast<long long>(C::kRows), static_cast<long long>(p.n_seq) * p.group - u.f0));
-        u.hi = pre.len;
+        u.hi = u.all_hi = pre.len;
         const int blocks = (pre.len - 1) / C::kKeys + 1;
         u.c0 = k * p.prefix_chunk;
         u.c1 = min(blocks, u.c0 + p.prefix_chunk);
@@ -264,21 +265,23 @@ __device__ __forceinline__ int block_of(const Unit& u, int i) { return i < u.sb 
 template <int D>
 __device__ __forceinline__ bool alternate(const Unit& u) { return Cut<D>::kSubs == 2 && u.nf <= 128; }
 
-// Place in the ring, from the unit's first, of a block's values: K_0 V_0 K_1 V_1 ..., or where blocks alternate K_0 K_1
-// V_0 K_2 V_1 ...
-__device__ __forceinline__ int at_v(bool alt, int i, int nb) { return alt ? min(2 * i + 2, nb + i) : 2 * i + 1; }
+// Whether the keys of two blocks come before the first's values: K_0 K_1 V_0 K_2 V_1 ... and not K_0 V_0 K_1 V_1 ...
+template <int D>
+__device__ __forceinline__ bool loads_two(const Unit& u) { return Cut<D>::kSubs == 1 || u.nf <= 128; }
+// Place in the ring, from the unit's first, of a block's values.
+__device__ __forceinline__ int at_v(bool two, int i, int nb) { return two ? min(2 * i + 2, nb + i) : 2 * i + 1; }
 
 template <int STAGES>
 struct Shared {
     uint64_t full[STAGES], empty[STAGES];
     uint64_t unit_full[kUnitSlots], unit_empty[kUnitSlots];
-    uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], o_full[2][2];
     Unit unit[kUnitSlots];
     int bad[kBadRing];
     int units[kSegments], sum[12];
     uint32_t tmem;
     int stop, leave;
-    uint32_t again;   // rows to be computed again
+    int odd;          // infinities or NaN were taken out of the unit's values
 };
 
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int r, int head, int page, uint64_t* bar) {
@@ -287,10 +290,6 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
             "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r), "r"(head), "r"(page), "r"(fer::dev::smem_addr(bar))
         : "memory");
 }
-
-// 256 threads x 224 and 128 x 56 are the 384 x 168 of the launch.
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
 
 // Shared-memory matrix descriptors, 128-byte swizzle, 1024 bytes from eight rows to the next: the upper word is the same for
 // all, the lower has the address and the bytes from one band to the next, so a step along the tile is one addition.
@@ -479,42 +478,59 @@ __device__ __forceinline__ void powers2(uint64_t t2, float& a, float& b) {
 template <typename T>
 __device__ __forceinline__ void put(T* to, float v) { *to = static_cast<T>(v); }
 
-// One row over its slots of the unit's blocks, by a warp: m, l and this lane's dims (every 32nd) of O. A probability that
-// vanishes counts as the smallest number, so that it gives an infinite value its due.
+// Whether some row of the unit does not see a slot that others, or none, see: P is 0 there, and 0 x inf would be NaN.
+__device__ __forceinline__ bool hidden(const Unit& u, int s) { return s >= u.all_hi || (s < u.all_lo && s >= u.sink); }
+template <int D>
+__device__ __forceinline__ bool any_hidden(const Unit& u, int s0, int n) {
+    return s0 + n > u.all_hi || (s0 < u.all_lo && s0 + n > u.sink);
+}
+// The halves of a word of two 16-bit floats that are infinite or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t odd_halves(uint32_t v) {
+    constexpr uint32_t kExp = __is_same(T, __half) ? 0x7c007c00u : 0x7f807f80u, kOne = __is_same(T, __half) ? 0x04000400u : 0x00800080u;
+    const uint32_t top = ((v & kExp) + kOne) & 0x80008000u;   // set where the exponent is all ones
+    return (top & 0x8000u ? 0xffffu : 0u) | (top >> 31 ? 0xffff0000u : 0u);
+}
+
+// Slots s0 .. s0 + 63 of a value tile (its rows from `at`) that are hidden from some row: those that nobody sees become 0,
+// infinite and NaN elements of the others too, noted in *odd. By the 128 threads of a sub-tile, t of them.
 template <typename T, int D>
-__device__ __noinline__ void one_row(const Paged& c, const TileParams& p, const Unit& u, int f, float& m, float& l,
-                                     float (&o)[D / 32]) {
-    const int lane = threadIdx.x & 31;
-    const T* const q = static_cast<const T*>(p.q) + q_row(p, u, f) * p.qs + static_cast<size_t>(q_head(p, u, f)) * D;
+__device__ __forceinline__ void clean_values(const Unit& u, uint8_t* at, int s0, int t, volatile int* odd) {
+    for (int j = t; j < 64 * (D / 8); j += 128) {
+        const int e = j / (D / 8), pc = j % (D / 8), s = s0 + e;
+        if (!hidden(u, s)) continue;
+        uint4* const v = reinterpret_cast<uint4*>(at + (pc >> 3) * Cut<D>::kBand + e * 128 + (((pc ^ e) & 7) << 4));
+        if (s >= u.hi || (s < u.lo && s >= u.sink)) {
+            *v = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        uint4 w = *v;
+        const uint32_t a = odd_halves<T>(w.x), b = odd_halves<T>(w.y), c = odd_halves<T>(w.z), d = odd_halves<T>(w.w);
+        if (!(a | b | c | d)) continue;
+        *odd = 1;
+        __threadfence_block();   // whoever finds the zeros finds the note
+        w.x &= ~a, w.y &= ~b, w.z &= ~c, w.w &= ~d;
+        *v = w;
+    }
+}
+
+// What clean_values took out, back into row f's results of dims d .. d + N - 1: the sum of a row that sees an infinity or NaN.
+template <typename T, int D, int N>
+__device__ __noinline__ void add_odd(const Paged& c, const TileParams& p, const Unit& u, int f, int d, float (&o)[N]) {
     const int32_t* const table = table_of(c, p, u);
     const Sees sees(p, u, f);
-    m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = 0.0f;
     for (int k = u.c0; k < u.c1; ++k) {
         const int s0 = block_of(u, k) * Cut<D>::kKeys;
+        if (!any_hidden<D>(u, s0, Cut<D>::kKeys)) continue;
         for (int s = s0; s < s0 + Cut<D>::kKeys; ++s) {
-            if (!sees(s)) continue;
+            if (!hidden(u, s) || !sees(s)) continue;
             const int id = table[s >> c.shift];
             if (!c.is_page(id)) continue;
-            const size_t at = c.row(id, u.hk, s);
-            float dot = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i)
-                dot = fmaf(static_cast<float>(q[i * 32 + lane]), static_cast<float>(static_cast<const T*>(c.k)[at + i * 32 + lane]), dot);
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, off);
-            dot *= p.scale2;
-            if (dot == -INFINITY) continue;
-            const float top = fmaxf(m, dot), base = top == -INFINITY ? 0.0f : top;
-            const float a = fmaxf(ex2(m - base), 1.17549435e-38f);
-            float w = ex2(dot - base);
-            if (w < 1.17549435e-38f) w = 1.17549435e-38f;   // NaN stays
-            m = top;
-            l = l * a + w;
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i)
-                o[i] = o[i] * a + w * static_cast<float>(static_cast<const T*>(c.v)[at + i * 32 + lane]);
+            const T* const v = static_cast<const T*>(c.v) + c.row(id, u.hk, s) + d;
+            for (int e = 0; e < N; ++e) {
+                const float x = static_cast<float>(v[e]);
+                if (!(x - x == 0.0f)) o[e] += x;
+            }
         }
     }
 }
@@ -525,7 +541,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                const __grid_constant__ CUtensorMap v_map) {
     using C = Cut<D>;
     constexpr bool kBf16 = !__is_same(T, __half);
-    constexpr uint32_t kIdS = idesc(C::kKeys, kBf16, false), kIdO = idesc(D, kBf16, true);
+    constexpr uint32_t kIdS = idesc(64, kBf16, false), kIdO = idesc(D, kBf16, true);
     // P is 2^(s - m + kUp): 16-bit floats of 5 exponent bits keep small ones so; with kSlack it stays below 2^15
     constexpr float kUp = kBf16 ? 0.0f : 8.0f;
     extern __shared__ uint8_t smem_raw[];
@@ -540,10 +556,13 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             fer::dev::mbar_init(&sh.unit_full[i], 1), fer::dev::mbar_init(&sh.unit_empty[i], C::kSoft + C::kSubs + 1);
         fer::dev::mbar_init(&sh.q_full, C::kSoft);
         fer::dev::mbar_init(&sh.q_empty, C::kSubs);
-        for (int i = 0; i < 2; ++i)
-            fer::dev::mbar_init(&sh.s_full[i], 1), fer::dev::mbar_init(&sh.p_full[i], 4), fer::dev::mbar_init(&sh.o_full[i], 1);
+        for (int i = 0; i < 2; ++i) {
+            for (int j = 0; j < 2; ++j)
+                fer::dev::mbar_init(&sh.s_full[i][j], 1), fer::dev::mbar_init(&sh.p_full[i][j], 4),
+                    fer::dev::mbar_init(&sh.o_full[i][j], 1);
+        }
         sh.stop = 0;
-        sh.again = 0;
+        sh.odd = 0;
         fer::dev::fence_mbar_init();
         fer::dev::prefetch_tmap(&k_map);
         fer::dev::prefetch_tmap(&v_map);
@@ -604,7 +623,6 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     bool ok = true;
 
     if (w >= C::kSoft) {
-        if constexpr (C::kShift) fewer_registers();   // all four warps of the group
         if (w == C::kSoft) {
             // ---- units, and their keys and values. Pages of a block: one a lane.
             const int box_rows = min(C::kKeys, c.page_size()), pages = C::kKeys / box_rows, boxes = pages * C::kBands;
@@ -624,7 +642,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 __syncwarp();
                 if (u.tok0 < 0) break;   // a later round has none either
                 const int32_t* const table = table_of(c, p, u);
-                const int nb = u.c1 - u.c0, lead = alternate<D>(u) ? 2 : 1;
+                const int nb = u.c1 - u.c0, lead = loads_two<D>(u) ? 2 : 1;
                 // this lane's page of block i: -1 where there is none to read, -2 where its id is out of range
                 const auto page_at = [&](int i) {
                     if (i >= nb || lane >= pages) return -1;
@@ -684,7 +702,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // of those that are the other's as soon as they are there.
             const int x = uniform(w - C::kSoft - 1);
             const uint32_t s_at = uniform(tmem) + 128 * x, o_at = uniform(tmem) + C::kColO + x * D;
-            uint32_t tile = 0, n_q = 0, n_p = 0;   // so far
+            uint32_t tile = 0, n_q = 0, n_p[2] = {0, 0}, n_o = 0;   // so far
             const auto landed = [&](uint32_t i) {
                 if (ok) ok = warp_wait(&sh.full[i % C::kStages], i / C::kStages);
             };
@@ -706,66 +724,113 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 const bool alt = C::kSubs == 2 && nf <= 128, fine = nf <= C::kFine && nf > kFew;
                 const uint32_t q_desc = desc_low(smem + (alt ? 0 : x * C::kQ), 16);
                 ok = warp_wait(&sh.q_full, n_q++);
-                // S of the tile; last: of the unit, so that other queries may come
-                const auto product_s = [&](uint32_t i, bool last) {
-                    const uint32_t kk = desc_low(ring + i % C::kStages * C::kTile, 16);
+                // S of 64 keys of tile i, and O += P V of 64
+                const auto product_s = [&](uint32_t i, int h, int at) {
+                    const uint32_t kk = desc_low(ring + i % C::kStages * C::kTile + h * 8192, 16);
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j)
-                        mma_ss(s_at, q_desc + ((j / 4) * 16384 + (j % 4) * 32) / 16,
+                        mma_ss(s_at + 64 * at, q_desc + ((j / 4) * 16384 + (j % 4) * 32) / 16,
                                kk + ((j / 4) * C::kBand + (j % 4) * 32) / 16, kIdS, j > 0);
-                    commit(&sh.s_full[x]);
-                    commit(&sh.empty[i % C::kStages]);
-                    if (last) commit(&sh.q_empty);
+                    commit(&sh.s_full[x][at]);
                 };
-                const auto product_o = [&](uint32_t i, bool first) {
-                    const uint32_t v = desc_low(ring + i % C::kStages * C::kTile, C::kBand);
+                const auto product_o = [&](uint32_t i, int h, int at, bool first) {
+                    const uint32_t v = desc_low(ring + i % C::kStages * C::kTile + h * 8192, C::kBand);
 #pragma unroll
-                    for (int j = 0; j < C::kKeys / 16; ++j) mma_ts(o_at, s_at + 8 * j, v + j * (2048 / 16), kIdO, !first || j > 0);
+                    for (int j = 0; j < 4; ++j)
+                        mma_ts(o_at, s_at + 64 * at + 8 * j, v + j * (2048 / 16), kIdO, !first || j > 0);
                     if (fine)
 #pragma unroll
-                        for (int j = 0; j < C::kKeys / 16; ++j)
-                            mma_ts(o_at, s_at + C::kKeys / 2 + 8 * j, v + j * (2048 / 16), kIdO, 1);
-                    commit(&sh.empty[i % C::kStages]);
+                        for (int j = 0; j < 4; ++j) mma_ts(o_at, s_at + 64 * at + 32 + 8 * j, v + j * (2048 / 16), kIdO, 1);
+                    commit(&sh.o_full[x][n_o & 1]);
                 };
-                // K_0 V_0 K_1 V_1 ..., or K_0 K_1 V_0 K_2 V_1 ... where even blocks are sub-tile 0's: either way the values
-                // of a block are followed by the keys of this sub-tile's next
-                const int step = alt ? 2 : 1;
-                if (alt && x == 1) skip();                                   // K_0
-                if (alt && x == 1 && nb == 1) {
-                    skip();                                                  // V_0
-                    if (lane == 0) fer::dev::mbar_arrive(&sh.q_empty);
-                    continue;
-                }
-                landed(tile);
-                if (ok) {
+                // the tile's last reader lets go of it
+                const auto done = [&](uint32_t i) { commit(&sh.empty[i % C::kStages]); };
+                const auto given = [&](int at) {
+                    if (ok) ok = warp_wait(&sh.p_full[x][at], n_p[at]);
+                    ++n_p[at];
                     fence_after();
-                    if (elected()) product_s(tile, step >= nb - (alt ? x : 0));
-                    __syncwarp();
-                }
-                ++tile;
-                if (alt && x == 0 && nb > 1) skip();                         // K_1
-                for (int i = alt ? x : 0; i < nb; i += step) {
-                    if (alt && i > 0) {
-                        skip();                                              // the other's V_{i-1}
-                        if (i + 1 < nb) skip();                              // and K_{i+1}
-                    }
-                    const bool more = i + step < nb;
-                    landed(tile);
-                    if (more) landed(tile + 1);
-                    if (ok) ok = warp_wait(&sh.p_full[x], n_p);
-                    ++n_p;
-                    if (ok) {
+                };
+                if constexpr (C::kSubs == 1) {
+                    // K_0 K_1 V_0 K_2 V_1 ...: a block is 64 keys, and S of the next but one follows
+                    for (int i = 0; i < min(nb, 2); ++i) {
+                        landed(tile);
                         fence_after();
-                        if (elected()) {
-                            product_o(tile, i < step);
-                            if (more) product_s(tile + 1, i + 2 * step >= nb);
-                            else commit(&sh.o_full[x]);
+                        if (ok && elected()) {
+                            product_s(tile, 0, i);
+                            done(tile);
+                            if (i + 1 == nb) commit(&sh.q_empty);
                         }
                         __syncwarp();
+                        ++tile;
                     }
-                    tile += more ? 2 : 1;
+                    for (int i = 0; i < nb; ++i) {
+                        const bool more = i + 2 < nb;
+                        landed(tile);
+                        if (more) landed(tile + 1);
+                        given(i & 1);
+                        if (ok && elected()) {
+                            product_o(tile, 0, i & 1, i == 0);
+                            done(tile);
+                            if (more) {
+                                product_s(tile + 1, 0, i & 1);
+                                done(tile + 1);
+                                if (i + 3 == nb) commit(&sh.q_empty);
+                            }
+                        }
+                        __syncwarp();
+                        ++n_o;
+                        tile += more ? 2 : 1;
+                    }
+                } else {
+                    // K_0 V_0 K_1 V_1 ..., or K_0 K_1 V_0 K_2 V_1 ... where even blocks are sub-tile 0's: either way the values
+                    // of a block are followed by the keys of this sub-tile's next
+                    const int step = alt ? 2 : 1;
+                    if (alt && x == 1) skip();                                   // K_0
+                    if (alt && x == 1 && nb == 1) {
+                        skip();                                                  // V_0
+                        if (lane == 0) fer::dev::mbar_arrive(&sh.q_empty);
+                        continue;
+                    }
+                    landed(tile);
+                    fence_after();
+                    if (ok && elected()) {
+                        product_s(tile, 0, 0);
+                        product_s(tile, 1, 1);
+                        done(tile);
+                        if (step >= nb - (alt ? x : 0)) commit(&sh.q_empty);
+                    }
+                    __syncwarp();
+                    ++tile;
+                    if (alt && x == 0 && nb > 1) skip();                         // K_1
+                    for (int i = alt ? x : 0; i < nb; i += step) {
+                        if (alt && i > 0) {
+                            skip();                                              // the other's V_{i-1}
+                            if (i + 1 < nb) skip();                              // and K_{i+1}
+                        }
+                        const bool more = i + step < nb;
+                        landed(tile);
+                        if (more) landed(tile + 1);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            given(h);
+                            if (ok && elected()) {
+                                product_o(tile, h, h, h == 0 && i < step);
+                                if (h == 1) done(tile);
+                                if (more) {
+                                    product_s(tile + 1, h, h);
+                                    if (h == 1) {
+                                        done(tile + 1);
+                                        if (i + 2 * step >= nb) commit(&sh.q_empty);
+                                    }
+                                }
+                            }
+                            __syncwarp();
+                            ++n_o;
+                        }
+                        tile += more ? 2 : 1;
+                    }
+                    if (alt && (nb - 1) % 2 != x) skip();                        // the other's last values
                 }
-                if (alt && (nb - 1) % 2 != x) skip();                        // the other's last values
             }
             if (!ok) {
                 if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
@@ -816,58 +881,53 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             }
         }
     } else {
-        // ---- softmax, a row a thread; of few rows (kFew) each is in all four quarters of a sub-tile: two take the first and two
-        // the second half of a block's keys, and of each two one keeps P's upper and one its lower 16 bits
-        if constexpr (C::kShift) more_registers();
-        constexpr int kChunks = C::kKeys / 32;
+        // ---- softmax, a row a thread, 64 keys at a time; of few rows (kFew) each is in all four quarters of a sub-tile: two take
+        // the first and two the second 32 keys, and of each two one keeps P's upper and one its lower 16 bits
         const int x = w >> 2, r = t & 127, half = (w >> 1) & 1, part = w & 1;
-        const uint32_t row_at = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16), s_at = row_at + 128 * x;
-        uint32_t base = 0, block = 0, n_s = 0, n_o = 0;
-        const bool wide_o = (reinterpret_cast<uintptr_t>(p.out) | (p.os * 2)) % 16 == 0;
+        const uint32_t row_at = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16);
+        uint32_t base = 0, block = 0, n_s[2] = {0, 0}, n_o = 0;   // n_o: P given so far
         for (int k = 0;; ++k) {
             const int slot = k % kUnitSlots;
             ok = ok && warp_wait(&sh.unit_full[slot], k / kUnitSlots);
             // both sub-tiles' warps leave together: each unit has barriers for all of them
             if (!ok) *stop = 1;
             meet<32 * C::kSoft>();   // and the unit before is done with its sums and results
-            if (t == 0) sh.leave = *stop;
+            if (t == 0) sh.leave = *stop, sh.odd = 0;
             meet<32 * C::kSoft>();
             if (sh.leave) {
                 if (!ok && lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutMma);
                 break;
             }
-            const Unit u = sh.unit[slot];
-            __syncwarp();
-            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
+            const Unit& u = sh.unit[slot];
             if (u.tok0 < 0) break;
-            const int nb = u.c1 - u.c0;
-            const bool alt = alternate<D>(u), few = u.nf <= kFew, fine = u.nf <= C::kFine;
+            const int nb = u.c1 - u.c0, nf = u.nf;
+            const bool alt = alternate<D>(u), few = nf <= kFew, fine = nf <= C::kFine;
             if (nb > 0 && !loads_ahead<D>(u)) {
-                for (int i = t; i < u.nf * (D / 8); i += 32 * C::kSoft)
+                for (int i = t; i < nf * (D / 8); i += 32 * C::kSoft)
                     *reinterpret_cast<uint4*>(smem_at + q_place<D>(i / (D / 8), i % (D / 8))) = q_piece<T, D>(p, u, i);
                 fer::dev::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) fer::dev::mbar_arrive(&sh.q_full);
             }
             const int f = few ? lane : alt ? r : x * 128 + r, first = alt ? x : 0, step = alt ? 2 : 1;
-            const bool rows_here = (f & ~31) < u.nf;                       // of the warp
-            const Sees sees(p, u, min(f, u.nf - 1));
+            const bool rows_here = (f & ~31) < nf;                         // of the warp
+            const Sees sees(p, u, min(f, nf - 1));
             // what every row of the warp sees, for blocks that need no mask
             const int all_end = __reduce_min_sync(0xffffffffu, sees.end), all_begin = __reduce_max_sync(0xffffffffu, sees.begin);
             float m = -INFINITY, l = 0.0f;
-            const int32_t* const table = table_of(c, p, u);
 
-            // a block's probabilities of N chunks of 32 keys from chunk j0 on; kind 0: rounded, 1: and what that leaves,
-            // 2: one of the two for these keys, and 0 for the others
-            const auto softmax = [&](auto chunks, auto kind, int j0, int i, int s0) {
+            // The products given so far have been added. They take turns at two barriers: where S of 64 keys is there, the
+            // products of all but the 64 before them are.
+            const auto o_added = [&]() { return warp_wait(&sh.o_full[x][(n_o - 1) & 1], (n_o - 1) >> 1); };
+            // Probabilities of 32 N of the 64 keys from slot s0 on, whose S is at s_at: those from chunk j0 on. kind 0: rounded,
+            // 1: and what that leaves, 2: one of the two for these keys, and 0 for the others.
+            const auto softmax = [&](auto chunks, auto kind, int j0, uint32_t s_at, int s0, bool bad, bool begun) {
                 constexpr int N = decltype(chunks)::value, kKind = decltype(kind)::value;
-                const bool plain = s0 + C::kKeys <= all_end && (s0 >= all_begin || s0 + C::kKeys <= sees.sink);
-                const bool bad = sh.bad[(block + i) % kBadRing] != 0;
                 float v[N][32];
 #pragma unroll
                 for (int j = 0; j < N; ++j) tmem_ld(s_at + 32 * (j0 + j), v[j]);
                 wait_ld(v);
-                if (!plain || bad) {
+                if (bad || s0 + 64 > all_end || (s0 < all_begin && s0 + 64 > sees.sink)) {
                     // [b0, e0) of the window and [0, k0) of the sinks, within the chunks
                     const int s1 = s0 + 32 * j0;
                     const int b0 = sees.begin - s1, e0 = sees.end - s1, k0 = min(sees.sink, sees.end) - s1;
@@ -877,7 +937,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         if (bad)
                             for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
                                 const int page = (s1 + 32 * j + e) >> c.shift;
-                                if (!page_needed(c, u, page) || !c.is_page(table[page])) on &= ~(0xffu << e);
+                                if (!page_needed(c, u, page) || !c.is_page(table_of(c, p, u)[page])) on &= ~(0xffu << e);
                             }
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
@@ -893,7 +953,9 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 const float m1 = raise ? top : m, shift = m1 == -INFINITY ? 0.0f : m1;
                 const float a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
                 m = m1;
-                if (i > first && __any_sync(0xffffffffu, raise)) {
+                if (begun && __any_sync(0xffffffffu, raise)) {
+                    if (ok) ok = o_added();
+                    fence_after();
 #pragma unroll 1
                     for (int j = 0; j < D / 16; ++j) {
                         uint32_t o[16];
@@ -928,11 +990,11 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         }
                     }
                     tmem_st16(s_at + 16 * (j0 + j), hi);
-                    if constexpr (kKind == 1) tmem_st16(s_at + C::kKeys / 2 + 16 * j, low);
+                    if constexpr (kKind == 1) tmem_st16(s_at + 32 + 16 * j, low);
                     if constexpr (kKind == 2) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) low[e] = 0;
-                        tmem_st16(s_at + 16 * (N - j0 + j), low);
+                        tmem_st16(s_at + 16 * (1 - j0), low);
                     }
                 }
                 float sm[8];
@@ -942,39 +1004,38 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 wait_st();
             };
             for (int i = first; i < nb; i += step) {
-                if (ok) ok = warp_wait(&sh.s_full[x], n_s);
-                ++n_s;
-                fence_after();
                 const int s0 = block_of(u, u.c0 + i) * C::kKeys;
-                if (rows_here && ok) {
-                    if (few) softmax(std::integral_constant<int, kChunks / 2>{}, std::integral_constant<int, 2>{}, half * (kChunks / 2), i, s0);
-                    else if (fine) softmax(std::integral_constant<int, kChunks>{}, std::integral_constant<int, 1>{}, 0, i, s0);
-                    else softmax(std::integral_constant<int, kChunks>{}, std::integral_constant<int, 0>{}, 0, i, s0);
+                const bool bad = sh.bad[(block + i) % kBadRing] != 0;
+#pragma unroll
+                for (int h = 0; h < C::kParts; ++h) {
+                    const int at = C::kParts == 1 ? i & 1 : h, s1 = s0 + 64 * h;
+                    if (ok) ok = warp_wait(&sh.s_full[x][at], n_s[at]);
+                    ++n_s[at];
+                    fence_after();
+                    if (rows_here && ok) {
+                        using Zero = std::integral_constant<int, 0>;
+                        using One = std::integral_constant<int, 1>;
+                        using Two = std::integral_constant<int, 2>;
+                        const uint32_t s_at = row_at + 128 * x + 64 * at;
+                        const bool begun = i > first || h > 0;
+                        if (few) softmax(One{}, Two{}, half, s_at, s1, bad, begun);
+                        else if (fine) softmax(Two{}, One{}, 0, s_at, s1, bad, begun);
+                        else softmax(Two{}, Zero{}, 0, s_at, s1, bad, begun);
+                    }
+                    if (any_hidden<D>(u, s1, 64) && ok) {
+                        const uint32_t tile = base + at_v(loads_two<D>(u), i, nb);
+                        ok = warp_wait(&sh.full[tile % C::kStages], tile / C::kStages);
+                        if (ok) clean_values<T, D>(u, smem_at + C::kRing + tile % C::kStages * C::kTile + h * 8192, s1, r, &sh.odd);
+                        fer::dev::fence_proxy_async_smem();
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) fer::dev::mbar_arrive(&sh.p_full[x][at]);
+                    ++n_o;
                 }
-                // values of slots that no row sees count as zero, whatever is there
-                const bool behind = s0 + C::kKeys > u.hi, before = s0 < u.lo && s0 + C::kKeys > u.sink;
-                if ((behind || before) && ok) {
-                    const uint32_t at = base + at_v(alt, i, nb);
-                    const int st = at % C::kStages;
-                    ok = warp_wait(&sh.full[st], at / C::kStages);
-                    if (ok)
-                        for (int j = r; j < C::kKeys * (D / 8); j += 128) {
-                            const int e = j / (D / 8), pc = j % (D / 8), s = s0 + e;
-                            if (s < u.hi && (s >= u.lo || s < u.sink)) continue;
-                            *reinterpret_cast<uint4*>(smem_at + C::kRing + st * C::kTile + (pc >> 3) * C::kBand + e * 128 +
-                                                      ((pc & 7) << 4)) = make_uint4(0, 0, 0, 0);
-                        }
-                    fer::dev::fence_proxy_async_smem();
-                }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) fer::dev::mbar_arrive(&sh.p_full[x]);
             }
             const bool mine = first < nb;
-            if (mine) {
-                if (ok) ok = warp_wait(&sh.o_full[x], n_o);
-                ++n_o;
-            }
+            if (mine && ok) ok = o_added();
             fence_after();
             base += 2 * nb, block += nb;
 
@@ -982,8 +1043,6 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // at the next unit where a wait ran out.
             float2* const sums = reinterpret_cast<float2*>(smem_at + C::kMeet);
             const uint32_t o_at = row_at + C::kColO + x * D;
-            unsigned again = 0;     // rows of this warp's share that are computed again
-            int d0 = 0, d1 = D;     // this warp's dims of them
             if (few) {
                 constexpr int kParts = 4 * C::kSubs;   // sums of a row; m and l are those of half of them
                 sums[t] = make_float2(m, l);
@@ -997,14 +1056,14 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
                 const float mine2 = mine && ok ? ex2(m - base2) * scale : 0.0f;
                 meet<32 * C::kSoft>();                 // the sums have been read
-                const bool on = lane < u.nf;
+                const bool on = lane < nf;
                 if (w == 0 && on) {
                     const size_t bh = q_row(p, u, lane) * p.heads + q_head(p, u, lane);
                     if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * (bh * p.parts + u.part)) = make_float2(all, total);
                     else if (p.lse) p.lse[bh] = total == 0.0f ? -INFINITY : (all + (log2f(total) - kUp)) * kLn2;
                 }
                 // as many dims at once as there is room for: 4 KB a warp
-                const int width = min(D, u.nf <= 8 ? 128 : u.nf <= 16 ? 64 : 32), rows = 1024 / width;
+                const int width = min(D, nf <= 8 ? 128 : nf <= 16 ? 64 : 32), rows = 1024 / width;
                 float* const meet_at = reinterpret_cast<float*>(smem_at + C::kMeet);
                 for (int d = 0; d < D; d += width) {
                     for (int e0 = 0; e0 < width; e0 += 32) {
@@ -1025,14 +1084,18 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         __syncwarp();
                     }
                     meet<32 * C::kSoft>();
-                    for (int i = t; i < u.nf * width; i += 32 * C::kSoft) {
+                    for (int i = t; i < nf * width; i += 32 * C::kSoft) {
                         const int row = i / width, e = i % width;
                         const float* const from = meet_at + row * width + (e & ~31) + (((e ^ (row << 2)) & 28) | (e & 3));
                         float v = 0.0f;
 #pragma unroll
                         for (int g = 0; g < kParts; ++g) v += from[g * rows * width];
                         if (nb == 0) v = 0.0f;
-                        if (!(v - v == 0.0f)) atomicOr(&sh.again, 1u << row);   // infinite ones too: it may be 0 x inf elsewhere
+                        if (sh.odd) {
+                            float one[1] = {v};
+                            add_odd<T, D, 1>(c, p, u, row, d + e, one);
+                            v = one[0];
+                        }
                         const size_t tok = q_row(p, u, row);
                         const int head = q_head(p, u, row);
                         if (u.part >= 0) p.part_o[((tok * p.heads + head) * p.parts + u.part) * D + d + e] = v;
@@ -1040,16 +1103,10 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     }
                     meet<32 * C::kSoft>();
                 }
-                const uint32_t all_again = sh.again;
-                if (all_again) {                       // the same for all of these warps
-                    meet<32 * C::kSoft>();
-                    if (t == 0) sh.again = 0;
-                    for (int g = w; g < u.nf; g += C::kSoft)
-                        if (all_again >> g & 1u) again |= 1u << g;
-                }
             } else {
                 float all = m, wa = 1.0f, wb = 0.0f, total = l;
                 uint32_t at_a = o_at, at_b = o_at;
+                int d0 = 0, d1 = D;
                 if (alt) {   // each sub-tile's warps take half of the dims of both sums
                     sums[t] = make_float2(m, l);
                     meet<32 * C::kSoft>();
@@ -1062,76 +1119,54 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     at_a = row_at + C::kColO, at_b = at_a + D;
                     fence_after();
                 }
-                const bool on = f < u.nf;
-                const int fr = min(f, u.nf - 1), head = q_head(p, u, fr);
+                const bool on = f < nf;
+                const int fr = min(f, nf - 1), head = q_head(p, u, fr);
                 const size_t tok = q_row(p, u, fr), bh = tok * p.heads + head, place = bh * p.parts + max(u.part, 0);
                 T* const out = static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D;
                 const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
-                bool nan = false;
+                wa *= scale, wb *= scale;
                 if (rows_here && ok) {
+                    const bool wide_o = (reinterpret_cast<uintptr_t>(p.out) | (p.os * 2)) % 16 == 0, odd = sh.odd != 0;
 #pragma unroll 1
                     for (int d = d0; d < d1; d += 32) {
-                        float oo[2][32];
-                        float(&o)[32] = oo[0];
+                        float o[2][32];
                         if (nb > 0) {
-                            tmem_ld(at_a + d, oo[0]);
-                            tmem_ld(at_b + d, oo[1]);
-                            wait_ld(oo);
-                            if (alt && nb > 1) {
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = fmaf(o[e], wa, oo[1][e] * wb);
-                            }
+                            tmem_ld(at_a + d, o[0]);
+                            if (alt && nb > 1) tmem_ld(at_b + d, o[1]);
+                            wait_ld(o);
                         }
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            o[e] = nb > 0 ? o[e] * scale : 0.0f;
-                            nan = nan || !(o[e] - o[e] == 0.0f);
+                            o[0][e] = nb > 0 ? o[0][e] * wa : 0.0f;
+                            if (alt && nb > 1) o[0][e] = fmaf(o[1][e], wb, o[0][e]);
                         }
+                        if (odd) add_odd<T, D, 32>(c, p, u, fr, d, o[0]);
                         if (on && u.part >= 0) {
                             float4* const to = reinterpret_cast<float4*>(p.part_o + place * D + d);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                            for (int e = 0; e < 8; ++e)
+                                to[e] = make_float4(o[0][4 * e], o[0][4 * e + 1], o[0][4 * e + 2], o[0][4 * e + 3]);
                         } else if (on && wide_o) {
                             uint4* const to = reinterpret_cast<uint4*>(out + d);
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                to[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
-                                                   pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+                                to[e] = make_uint4(pack2<T>(o[0][8 * e], o[0][8 * e + 1]), pack2<T>(o[0][8 * e + 2], o[0][8 * e + 3]),
+                                                   pack2<T>(o[0][8 * e + 4], o[0][8 * e + 5]), pack2<T>(o[0][8 * e + 6], o[0][8 * e + 7]));
                         } else if (on) {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) put(out + d + e, o[e]);
+                            for (int e = 0; e < 32; ++e) put(out + d + e, o[0][e]);
                         }
                         __syncwarp();
                     }
-                    if (on && (!alt || x == 0)) {
+                    if (on && d0 == 0) {
                         if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * place) = make_float2(all, total);
                         else if (p.lse) p.lse[bh] = total == 0.0f ? -INFINITY : (all + (log2f(total) - kUp)) * kLn2;
                     }
-                    again = __ballot_sync(0xffffffffu, on && nan && nb > 0);
                 }
-            }
-            while (again) {
-                const int src = __ffs(again) - 1;
-                again &= again - 1;
-                const int g = few ? src : (f & ~31) + src;
-                float m2, l2, o2[D / 32];
-                one_row<T, D>(c, p, u, g, m2, l2, o2);
-                const int gh = q_head(p, u, g);
-                const size_t gt = q_row(p, u, g), bh = gt * p.heads + gh, place = bh * p.parts + max(u.part, 0);
-#pragma unroll
-                for (int j = 0; j < D / 32; ++j) {
-                    const int d = 32 * j + lane;
-                    if (d < d0 || d >= d1) continue;
-                    if (u.part >= 0) p.part_o[place * D + d] = o2[j];
-                    else put(static_cast<T*>(p.out) + gt * p.os + static_cast<size_t>(gh) * D + d, l2 == 0.0f ? 0.0f : o2[j] / l2);
-                }
-                if (lane == 0 && d0 == 0) {   // l is of 2^(s - m + kUp) elsewhere
-                    if (u.part >= 0) *reinterpret_cast<float2*>(p.part_ml + 2 * place) = make_float2(m2 + kUp, l2);
-                    else if (p.lse) p.lse[bh] = l2 == 0.0f ? -INFINITY : (m2 + log2f(l2)) * kLn2;
-                }
-                __syncwarp();
             }
             fence_before();
+            __syncwarp();
+            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
         }
     }
 
