@@ -72,21 +72,31 @@ template <int D> struct Cut {
     static constexpr int kBands = D / 64;
     static constexpr int kTile = kKeys * D * 2;
     static constexpr int kBand = kKeys * 128;        // 64 dims of a tile's keys
-    static constexpr int kStages = D == 64 ? 8 : D == 128 ? 5 : 4;
+    static constexpr int kStages = D == 64 ? 8 : 4;
     static constexpr int kQ = 128 * D * 2;           // queries of a sub-tile
     static constexpr int kSoft = 4 * kSubs;          // softmax warps
     static constexpr int kParts = kKeys / 64;        // 64 keys at a time
     // Softmax warps, one that loads keys and values, one for each sub-tile that issues products, one that loads queries.
+    // Registers: of 168 a thread at launch the two groups of four softmax warps take 208 and leave the third group's warps
+    // 88. (One group has enough at launch.)
+    static constexpr bool kShift = kSubs == 2;
     static constexpr int kThreads = 32 * (kSoft + kSubs + 2);
     static constexpr int kRing = kSubs * kQ;         // where the ring begins
-    // Where a unit's warps add up their results: the second sub-tile's queries, which such a unit does not have, or 32 KB more
-    static constexpr int kMeet = D == 128 ? kQ : kRing + kStages * kTile;
-    static constexpr int kSmem = kRing + kStages * kTile + (D == 128 ? 0 : 32768) + 1024;
+    static constexpr int kMeet = kRing + kStages * kTile;   // 32 KB in which results are added up and turned round
+    static constexpr int kSmem = kMeet + 32768 + 1024;
     static constexpr uint32_t kColO = 256;           // O of sub-tile x at kColO + x D, S and P of 64 keys at 128 x and 128 x + 64
     // rows up to which P's rounding is made up for
     static constexpr int kFine = kSubs == 2 ? 128 : 64;
 };
 constexpr int kFew = 32;   // rows that the four warps of a sub-tile share
+
+// Division of numbers below 2^31 by one divisor, by a product and a shift (Granlund and Montgomery 1994).
+struct Divide {
+    uint32_t by, mul, shift;
+    __device__ __forceinline__ int operator()(int n) const {
+        return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+    }
+};
 
 struct TileParams {
     const void* q;
@@ -95,6 +105,7 @@ struct TileParams {
     float* lse;
     const int32_t* offsets;        // null: row b is sequence b's latest slot
     int n_seq, rows, heads, group;
+    Divide by_group;
     int window, sinks;             // INT_MAX: no window
     float scale2;                  // scale * log2 e
     int chunk;                     // key blocks a unit
@@ -155,7 +166,7 @@ __device__ __forceinline__ int tile_range(const TileParams& p, const Seq& q, int
     u.f0 = i * C::kRows;
     u.nf = static_cast<int>(min(static_cast<long long>(C::kRows), static_cast<long long>(q.n) * p.group - u.f0));
     u.slot0 = q.len - q.n;
-    const int first = u.slot0 + u.f0 / p.group, last = u.slot0 + (u.f0 + u.nf - 1) / p.group;
+    const int first = u.slot0 + p.by_group(u.f0), last = u.slot0 + p.by_group(u.f0 + u.nf - 1);
     u.hi = max(last + 1, 0);
     u.lo = p.window == INT_MAX ? 0 : max(first + 1 - p.window, 0);
     u.all_hi = max(first + 1, 0);
@@ -275,7 +286,7 @@ template <int STAGES>
 struct Shared {
     uint64_t full[STAGES], empty[STAGES];
     uint64_t unit_full[kUnitSlots], unit_empty[kUnitSlots];
-    uint64_t q_full, q_empty, s_full[2][2], p_full[2][2], o_full[2][2];
+    uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_full[2][2];
     Unit unit[kUnitSlots];
     int bad[kBadRing];
     int units[kSegments], sum[12];
@@ -290,6 +301,10 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
             "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r), "r"(head), "r"(page), "r"(fer::dev::smem_addr(bar))
         : "memory");
 }
+
+// 256 threads x 208 and 128 x 88 are the 384 x 168 of the launch.
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 
 // Shared-memory matrix descriptors, 128-byte swizzle, 1024 bytes from eight rows to the next: the upper word is the same for
 // all, the lower has the address and the bytes from one band to the next, so a step along the tile is one addition.
@@ -408,10 +423,6 @@ __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(N)
 // The bits below n, all or none of them where n is past the ends.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
 
-__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(fer::dev::smem_addr(bar)), "r"(n) : "memory");
-}
-
 // Whether some row of a unit sees a slot of the page.
 __device__ __forceinline__ bool page_needed(const Paged& c, const Unit& u, int page) {
     const int first = page << c.shift, last = first + c.page_size() - 1;
@@ -424,35 +435,17 @@ __device__ __forceinline__ const int32_t* table_of(const Paged& c, const TilePar
 struct Sees {
     int begin, end, sink;
     __device__ __forceinline__ Sees(const TileParams& p, const Unit& u, int f) {
-        end = u.seq < 0 ? u.hi : u.slot0 + (u.f0 + f) / p.group + 1;
+        end = u.seq < 0 ? u.hi : u.slot0 + p.by_group(u.f0 + f) + 1;
         begin = p.window == INT_MAX || u.seq < 0 ? 0 : max(end - p.window, 0);
         sink = p.sinks;
     }
     __device__ __forceinline__ bool operator()(int s) const { return s < end && (s >= begin || s < sink); }
 };
 __device__ __forceinline__ size_t q_row(const TileParams& p, const Unit& u, int f) {
-    return static_cast<size_t>(u.tok0) + (u.f0 + f) / p.group;
+    return static_cast<size_t>(u.tok0) + p.by_group(u.f0 + f);
 }
-__device__ __forceinline__ int q_head(const TileParams& p, const Unit& u, int f) { return u.hk * p.group + (u.f0 + f) % p.group; }
-
-// Whether a unit's queries are those of one sub-tile, which one warp loads ahead.
-template <int D>
-__device__ __forceinline__ bool loads_ahead(const Unit& u) { return Cut<D>::kSubs == 1 || u.nf <= 128; }
-// Piece i (8 elements) of a unit's queries, and its place.
-template <typename T, int D>
-__device__ __forceinline__ uint4 q_piece(const TileParams& p, const Unit& u, int i) {
-    const int f = i / (D / 8), pc = i % (D / 8);
-    const uint16_t* const src = reinterpret_cast<const uint16_t*>(p.q) + q_row(p, u, f) * p.qs +
-                                static_cast<size_t>(q_head(p, u, f)) * D + pc * 8;
-    if ((reinterpret_cast<uintptr_t>(p.q) | (p.qs * 2)) % 16 == 0) return *reinterpret_cast<const uint4*>(src);
-    uint32_t e[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) e[j] = src[2 * j] | static_cast<uint32_t>(src[2 * j + 1]) << 16;
-    return make_uint4(e[0], e[1], e[2], e[3]);
-}
-template <int D>
-__device__ __forceinline__ int q_place(int f, int pc) {
-    return (f >> 7) * Cut<D>::kQ + (pc >> 3) * 16384 + (f & 127) * 128 + (((pc ^ f) & 7) << 4);
+__device__ __forceinline__ int q_head(const TileParams& p, const Unit& u, int f) {
+    return u.hk * p.group + (u.f0 + f) - p.by_group(u.f0 + f) * p.group;
 }
 
 // 2^t for two t of at most 126, on the multipliers and adders: t = n + f with |f| <= 1/2, n by rounding in the last bits of
@@ -496,21 +489,32 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t v) {
 // infinite and NaN elements of the others too, noted in *odd. By the 128 threads of a sub-tile, t of them.
 template <typename T, int D>
 __device__ __forceinline__ void clean_values(const Unit& u, uint8_t* at, int s0, int t, volatile int* odd) {
-    for (int j = t; j < 64 * (D / 8); j += 128) {
-        const int e = j / (D / 8), pc = j % (D / 8), s = s0 + e;
-        if (!hidden(u, s)) continue;
-        uint4* const v = reinterpret_cast<uint4*>(at + (pc >> 3) * Cut<D>::kBand + e * 128 + (((pc ^ e) & 7) << 4));
-        if (s >= u.hi || (s < u.lo && s >= u.sink)) {
-            *v = make_uint4(0, 0, 0, 0);
-            continue;
+    constexpr int kPieces = D / 8, kStep = 128 / kPieces, kTimes = 64 / kStep;   // rows at once, and how often
+    const int pc = t % kPieces;
+    uint8_t* const column = at + (pc >> 3) * Cut<D>::kBand;
+#pragma unroll 1
+    for (int k0 = 0; k0 < kTimes; k0 += 4) {
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int e = (k0 + k) * kStep + t / kPieces, s = s0 + e;
+            w[k] = make_uint4(0, 0, 0, 0);
+            if (hidden(u, s)) w[k] = *reinterpret_cast<const uint4*>(column + e * 128 + (((pc ^ e) & 7) << 4));
         }
-        uint4 w = *v;
-        const uint32_t a = odd_halves<T>(w.x), b = odd_halves<T>(w.y), c = odd_halves<T>(w.z), d = odd_halves<T>(w.w);
-        if (!(a | b | c | d)) continue;
-        *odd = 1;
-        __threadfence_block();   // whoever finds the zeros finds the note
-        w.x &= ~a, w.y &= ~b, w.z &= ~c, w.w &= ~d;
-        *v = w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int e = (k0 + k) * kStep + t / kPieces, s = s0 + e;
+            const bool dead = s >= u.hi || (s < u.lo && s >= u.sink);
+            const uint32_t a = odd_halves<T>(w[k].x), b = odd_halves<T>(w[k].y), c = odd_halves<T>(w[k].z), d = odd_halves<T>(w[k].w);
+            if (dead) {
+                *reinterpret_cast<uint4*>(column + e * 128 + (((pc ^ e) & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            } else if (a | b | c | d) {
+                *odd = 1;
+                __threadfence_block();   // whoever finds the zeros finds the note
+                *reinterpret_cast<uint4*>(column + e * 128 + (((pc ^ e) & 7) << 4)) =
+                    make_uint4(w[k].x & ~a, w[k].y & ~b, w[k].z & ~c, w[k].w & ~d);
+            }
+        }
     }
 }
 
@@ -554,8 +558,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
         for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&sh.full[i], 1), fer::dev::mbar_init(&sh.empty[i], C::kSubs);
         for (int i = 0; i < kUnitSlots; ++i)
             fer::dev::mbar_init(&sh.unit_full[i], 1), fer::dev::mbar_init(&sh.unit_empty[i], C::kSoft + C::kSubs + 1);
-        fer::dev::mbar_init(&sh.q_full, C::kSoft);
-        fer::dev::mbar_init(&sh.q_empty, C::kSubs);
+        for (int i = 0; i < 2; ++i) fer::dev::mbar_init(&sh.q_full[i], 1), fer::dev::mbar_init(&sh.q_empty[i], C::kSubs);
         for (int i = 0; i < 2; ++i) {
             for (int j = 0; j < 2; ++j)
                 fer::dev::mbar_init(&sh.s_full[i][j], 1), fer::dev::mbar_init(&sh.p_full[i][j], 4),
@@ -623,6 +626,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     bool ok = true;
 
     if (w >= C::kSoft) {
+        if constexpr (C::kShift) fewer_registers();   // all four warps of the group
         if (w == C::kSoft) {
             // ---- units, and their keys and values. Pages of a block: one a lane.
             const int box_rows = min(C::kKeys, c.page_size()), pages = C::kKeys / box_rows, boxes = pages * C::kBands;
@@ -702,7 +706,8 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // of those that are the other's as soon as they are there.
             const int x = uniform(w - C::kSoft - 1);
             const uint32_t s_at = uniform(tmem) + 128 * x, o_at = uniform(tmem) + C::kColO + x * D;
-            uint32_t tile = 0, n_q = 0, n_p[2] = {0, 0}, n_o = 0;   // so far
+            uint32_t tile = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_o = 0;   // so far
+            int turn = 0;   // whose place among the queries the next unit of one sub-tile takes
             const auto landed = [&](uint32_t i) {
                 if (ok) ok = warp_wait(&sh.full[i % C::kStages], i / C::kStages);
             };
@@ -722,8 +727,14 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 if (end) break;
                 if (nb == 0) continue;
                 const bool alt = C::kSubs == 2 && nf <= 128, fine = nf <= C::kFine && nf > kFew;
-                const uint32_t q_desc = desc_low(smem + (alt ? 0 : x * C::kQ), 16);
-                ok = warp_wait(&sh.q_full, n_q++);
+                // a unit of one sub-tile has one place, they take turns; else each sub-tile has its own
+                const int q_at = C::kSubs == 1 ? 0 : alt ? turn : x;
+                const uint32_t q_desc = desc_low(smem + q_at * C::kQ, 16);
+#pragma unroll
+                for (int i = 0; i < C::kSubs; ++i)
+                    if (!alt || i == q_at) ok = ok && warp_wait(&sh.q_full[i], n_q[i]++);
+                if (C::kSubs == 2 && !alt && lane == 0) fer::dev::mbar_arrive(&sh.q_empty[x ^ 1]);   // not read here
+                if (alt) turn ^= 1;
                 // S of 64 keys of tile i, and O += P V of 64
                 const auto product_s = [&](uint32_t i, int h, int at) {
                     const uint32_t kk = desc_low(ring + i % C::kStages * C::kTile + h * 8192, 16);
@@ -758,7 +769,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         if (ok && elected()) {
                             product_s(tile, 0, i);
                             done(tile);
-                            if (i + 1 == nb) commit(&sh.q_empty);
+                            if (i + 1 == nb) commit(&sh.q_empty[q_at]);
                         }
                         __syncwarp();
                         ++tile;
@@ -774,7 +785,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                             if (more) {
                                 product_s(tile + 1, 0, i & 1);
                                 done(tile + 1);
-                                if (i + 3 == nb) commit(&sh.q_empty);
+                                if (i + 3 == nb) commit(&sh.q_empty[q_at]);
                             }
                         }
                         __syncwarp();
@@ -788,7 +799,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     if (alt && x == 1) skip();                                   // K_0
                     if (alt && x == 1 && nb == 1) {
                         skip();                                                  // V_0
-                        if (lane == 0) fer::dev::mbar_arrive(&sh.q_empty);
+                        if (lane == 0) fer::dev::mbar_arrive(&sh.q_empty[q_at]);
                         continue;
                     }
                     landed(tile);
@@ -797,7 +808,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         product_s(tile, 0, 0);
                         product_s(tile, 1, 1);
                         done(tile);
-                        if (step >= nb - (alt ? x : 0)) commit(&sh.q_empty);
+                        if (step >= nb - (alt ? x : 0)) commit(&sh.q_empty[q_at]);
                     }
                     __syncwarp();
                     ++tile;
@@ -820,7 +831,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                                     product_s(tile + 1, h, h);
                                     if (h == 1) {
                                         done(tile + 1);
-                                        if (i + 2 * step >= nb) commit(&sh.q_empty);
+                                        if (i + 2 * step >= nb) commit(&sh.q_empty[q_at]);
                                     }
                                 }
                             }
@@ -837,9 +848,10 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 *stop = 1;
             }
         } else {
-            // ---- queries of units of at most 128 rows, read while the unit before still computes; few rows go to each
-            // quarter of the sub-tile
-            uint32_t n_q = 0;
+            // ---- queries, read while the unit before still computes; few rows go to each quarter of the sub-tile
+            uint32_t n_q[2] = {0, 0};
+            int turn = 0;
+            const bool wide = (reinterpret_cast<uintptr_t>(p.q) | (p.qs * 2)) % 16 == 0;
             for (int k = 0; ok; ++k) {
                 const int slot = k % kUnitSlots;
                 ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
@@ -849,31 +861,40 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
                 if (u.tok0 < 0) break;
                 if (u.c1 == u.c0) continue;
-                const bool mine = loads_ahead<D>(u);
-                constexpr int kAhead = 4;
-                uint4 v[kAhead];
-                const int n = mine ? u.nf * (D / 8) : 0;
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    if (j * 32 + lane < n) v[j] = q_piece<T, D>(p, u, j * 32 + lane);
-                ok = warp_wait(&sh.q_empty, n_q++ ^ 1u);   // the unit before has multiplied its last keys
-                if (!mine) continue;
+                const bool alt = alternate<D>(u);
                 const int copies = u.nf <= kFew ? 4 : 1;
-                for (int i0 = lane; i0 < n; i0 += 32 * kAhead) {
+                constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;   // of a row, and rows at once
 #pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        const int i = i0 + 32 * j;
-                        if (i >= n) break;
-                        for (int g = 0; g < copies; ++g)
-                            *reinterpret_cast<uint4*>(smem_at + q_place<D>(i / (D / 8) + 32 * g, i % (D / 8))) = v[j];
+                for (int i = 0; i < C::kSubs; ++i) {
+                    if (alt && i != turn) continue;
+                    ok = ok && warp_wait(&sh.q_empty[i], n_q[i]++ ^ 1u);   // what was there has been multiplied
+                    if (!ok) break;
+                    const int first = alt ? 0 : 128 * i, rows = min(128, u.nf - first), pc = lane % kPieces;
+                    // this lane's row: token and head of the group
+                    int tok = p.by_group(u.f0 + first + lane / kPieces), g = u.f0 + first + lane / kPieces - tok * p.group;
+                    uint8_t* const to = smem_at + i * C::kQ + (pc >> 3) * 16384;
+                    for (int f = lane / kPieces; f < rows; f += kAtOnce) {
+                        const uint16_t* const src = reinterpret_cast<const uint16_t*>(p.q) + (static_cast<size_t>(u.tok0) + tok) * p.qs +
+                                                    (static_cast<size_t>(u.hk) * p.group + g) * D + pc * 8;
+                        for (int j = 0; j < copies; ++j) {
+                            uint8_t* const dst = to + (f + 32 * j) * 128 + (((pc ^ f) & 7) << 4);
+                            if (wide) {
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(fer::dev::smem_addr(dst)), "l"(src) : "memory");
+                            } else {
+                                uint32_t e[4];
+#pragma unroll
+                                for (int h = 0; h < 4; ++h) e[h] = src[2 * h] | static_cast<uint32_t>(src[2 * h + 1]) << 16;
+                                *reinterpret_cast<uint4*>(dst) = make_uint4(e[0], e[1], e[2], e[3]);
+                            }
+                        }
+                        for (g += kAtOnce; g >= p.group; g -= p.group) ++tok;
                     }
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j)
-                        if (i0 + 32 * (kAhead + j) < n) v[j] = q_piece<T, D>(p, u, i0 + 32 * (kAhead + j));
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fer::dev::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) fer::dev::mbar_arrive(&sh.q_full[i]);
                 }
-                fer::dev::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_n(&sh.q_full, C::kSoft);
+                if (alt) turn ^= 1;
             }
             if (!ok) {
                 if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutSync);
@@ -883,6 +904,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     } else {
         // ---- softmax, a row a thread, 64 keys at a time; of few rows (kFew) each is in all four quarters of a sub-tile: two take
         // the first and two the second 32 keys, and of each two one keeps P's upper and one its lower 16 bits
+        if constexpr (C::kShift) more_registers();
         const int x = w >> 2, r = t & 127, half = (w >> 1) & 1, part = w & 1;
         const uint32_t row_at = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16);
         uint32_t base = 0, block = 0, n_s[2] = {0, 0}, n_o = 0;   // n_o: P given so far
@@ -898,17 +920,12 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 if (!ok && lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutMma);
                 break;
             }
-            const Unit& u = sh.unit[slot];
+            const Unit u = sh.unit[slot];
+            __syncwarp();
+            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
             if (u.tok0 < 0) break;
             const int nb = u.c1 - u.c0, nf = u.nf;
             const bool alt = alternate<D>(u), few = nf <= kFew, fine = nf <= C::kFine;
-            if (nb > 0 && !loads_ahead<D>(u)) {
-                for (int i = t; i < nf * (D / 8); i += 32 * C::kSoft)
-                    *reinterpret_cast<uint4*>(smem_at + q_place<D>(i / (D / 8), i % (D / 8))) = q_piece<T, D>(p, u, i);
-                fer::dev::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) fer::dev::mbar_arrive(&sh.q_full);
-            }
             const int f = few ? lane : alt ? r : x * 128 + r, first = alt ? x : 0, step = alt ? 2 : 1;
             const bool rows_here = (f & ~31) < nf;                         // of the warp
             const Sees sees(p, u, min(f, nf - 1));
@@ -1115,6 +1132,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     const float base2 = all == -INFINITY ? 0.0f : all;
                     wa = ex2(sa.x - base2), wb = ex2(sb.x - base2);
                     total = sa.y * wa + sb.y * wb;
+                    meet<32 * C::kSoft>();   // the sums have been read
                     d0 = x * (D / 2), d1 = d0 + D / 2;
                     at_a = row_at + C::kColO, at_b = at_a + D;
                     fence_after();
@@ -1122,39 +1140,71 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 const bool on = f < nf;
                 const int fr = min(f, nf - 1), head = q_head(p, u, fr);
                 const size_t tok = q_row(p, u, fr), bh = tok * p.heads + head, place = bh * p.parts + max(u.part, 0);
-                T* const out = static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D;
                 const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
                 wa *= scale, wb *= scale;
                 if (rows_here && ok) {
-                    const bool wide_o = (reinterpret_cast<uintptr_t>(p.out) | (p.os * 2)) % 16 == 0, odd = sh.odd != 0;
+                    const bool odd = sh.odd != 0;
+                    // 128 bytes of each of the warp's rows at a time, turned round in shared memory, so that eight lanes write a
+                    // row's 128 bytes
+                    uint8_t* const turn = smem_at + C::kMeet + w * 4096;
+                    const unsigned long long to = u.part >= 0 ? reinterpret_cast<unsigned long long>(p.part_o + place * D)
+                                                              : reinterpret_cast<unsigned long long>(static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D);
+                    const bool whole = u.part >= 0 || (reinterpret_cast<uintptr_t>(p.out) | (p.os * 2)) % 16 == 0;
+                    const int rows = min(32, nf - (f - lane)), size = u.part >= 0 ? 4 : 2;
+                    uint8_t* const mine_at = turn + lane * 128;
+                    const int span = u.part >= 0 ? 32 : 64;   // dims in 128 bytes
 #pragma unroll 1
-                    for (int d = d0; d < d1; d += 32) {
-                        float o[2][32];
-                        if (nb > 0) {
-                            tmem_ld(at_a + d, o[0]);
-                            if (alt && nb > 1) tmem_ld(at_b + d, o[1]);
-                            wait_ld(o);
-                        }
+                    for (int d = d0; d < d1; d += 16) {
+                        float o[16];
+                        {
+                            uint32_t a[16], b[16];
+                            if (nb > 0) tmem_ld16(at_a + d, a);
+                            if (alt && nb > 1) tmem_ld16(at_b + d, b);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            o[0][e] = nb > 0 ? o[0][e] * wa : 0.0f;
-                            if (alt && nb > 1) o[0][e] = fmaf(o[1][e], wb, o[0][e]);
+                            for (int e = 0; e < 16; ++e) {
+                                o[e] = nb > 0 ? __uint_as_float(a[e]) * wa : 0.0f;
+                                if (alt && nb > 1) o[e] = fmaf(__uint_as_float(b[e]), wb, o[e]);
+                            }
                         }
-                        if (odd) add_odd<T, D, 32>(c, p, u, fr, d, o[0]);
-                        if (on && u.part >= 0) {
-                            float4* const to = reinterpret_cast<float4*>(p.part_o + place * D + d);
+                        if (odd) {
+                            float y[16];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                to[e] = make_float4(o[0][4 * e], o[0][4 * e + 1], o[0][4 * e + 2], o[0][4 * e + 3]);
-                        } else if (on && wide_o) {
-                            uint4* const to = reinterpret_cast<uint4*>(out + d);
+                            for (int e = 0; e < 16; ++e) y[e] = o[e];
+                            add_odd<T, D, 16>(c, p, u, fr, d, y);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = y[e];
+                        }
+                        const int off = (d - d0) % span;
+                        if (u.part >= 0) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                to[e] = make_uint4(pack2<T>(o[0][8 * e], o[0][8 * e + 1]), pack2<T>(o[0][8 * e + 2], o[0][8 * e + 3]),
-                                                   pack2<T>(o[0][8 * e + 4], o[0][8 * e + 5]), pack2<T>(o[0][8 * e + 6], o[0][8 * e + 7]));
-                        } else if (on) {
+                                *reinterpret_cast<float4*>(mine_at + (((off / 4 + e) ^ lane) & 7) * 16) =
+                                    make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        } else {
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) put(out + d + e, o[0][e]);
+                            for (int e = 0; e < 2; ++e)
+                                *reinterpret_cast<uint4*>(mine_at + (((off / 8 + e) ^ lane) & 7) * 16) =
+                                    make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
+                                               pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+                        }
+                        if (off + 16 < span && d + 16 < d1) continue;
+                        __syncwarp();
+                        const int begin = d - off, pieces = (off + 16) * size / 16;
+                        const unsigned long long column = static_cast<unsigned long long>(begin) * size + (lane & 7) * 16;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const int row = i + (lane >> 3);
+                            const unsigned long long at = __shfl_sync(0xffffffffu, to, row);
+                            if (row < rows && (lane & 7) < pieces) {
+                                const uint4 v = *reinterpret_cast<const uint4*>(turn + row * 128 + (((lane ^ row) & 7) << 4));
+                                if (whole) {
+                                    *reinterpret_cast<uint4*>(at + column) = v;
+                                } else {
+                                    uint16_t* const h = reinterpret_cast<uint16_t*>(at + column);
+                                    h[0] = v.x, h[1] = v.x >> 16, h[2] = v.y, h[3] = v.y >> 16;
+                                    h[4] = v.z, h[5] = v.z >> 16, h[6] = v.w, h[7] = v.w >> 16;
+                                }
+                            }
                         }
                         __syncwarp();
                     }
@@ -1165,8 +1215,6 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 }
             }
             fence_before();
-            __syncwarp();
-            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
         }
     }
 
@@ -1255,8 +1303,8 @@ Split split(long long units, long long blocks, long long tile_rows) {
     Split s{INT_MAX, 0};
     long long parts = 1;
     if (tile_rows <= 64) parts = ceil_div(blocks, 8);            // a part costs little: even shares of ragged lengths
-    else if (units < 4 * kSms) parts = ceil_div(4 * kSms, units);
-    if (tile_rows > 64 && parts > ceil_div(blocks, 16)) parts = ceil_div(blocks, 16);
+    else if (units < 8 * kSms) parts = ceil_div(8 * kSms, units);
+    if (tile_rows > 64 && parts > ceil_div(blocks, 32)) parts = ceil_div(blocks, 32);
     if (parts <= 1) return s;
     s.chunk = static_cast<int>(ceil_div(blocks, parts));
     s.parts = static_cast<int>(ceil_div(blocks, s.chunk));
@@ -1361,6 +1409,13 @@ cudaError_t run_dim(const Paged& c, const TileParams& p, cudaStream_t s) {
     }
 }
 
+Divide divide(uint32_t by) {
+    Divide d{by, 0, 0};
+    while ((1u << d.shift) < by) ++d.shift;
+    d.mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << d.shift) - by)) / by + 1);
+    return d;
+}
+
 // What both operators' arguments have in common.
 cudaError_t common(const fer_paged_view_t* cache, const void* q, void* out, size_t q_stride, size_t out_stride, int heads,
                    float scale, const float* lse, Paged* c, TileParams* p) {
@@ -1379,6 +1434,7 @@ cudaError_t common(const fer_paged_view_t* cache, const void* q, void* out, size
     p->lse = const_cast<float*>(lse);
     p->heads = heads;
     p->group = heads / c->kv_heads;
+    p->by_group = divide(static_cast<uint32_t>(p->group));
     p->scale2 = (scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c->head_dim)) : scale) * kLog2e;
     return cudaSuccess;
 }
