@@ -90,6 +90,10 @@ template <int D> struct Cut {
 };
 constexpr int kFew = 32;   // rows that the four warps of a sub-tile share
 
+// How queries are loaded: 128 (or 32) rows by a tensor copy where the group divides 32, or 128 where no unit has few rows; row
+// by row for other groups; by ordinary loads where the addresses are not multiples of 16 bytes.
+enum { kQBoxes, kQRows, kQLoads };
+
 // Division of numbers below 2^31 by one divisor, by a product and a shift (Granlund and Montgomery 1994).
 struct Divide {
     uint32_t by, mul, shift;
@@ -108,6 +112,7 @@ struct TileParams {
     Divide by_group;
     int window, sinks;             // INT_MAX: no window
     float scale2;                  // scale * log2 e
+    int q_maps;                    // kQBoxes, kQRows or kQLoads
     int chunk;                     // key blocks a unit
     int parts;                     // parts a row may have; 0: results go to out
     float* part_ml;                // [rows * heads][parts][2]
@@ -295,6 +300,12 @@ struct Shared {
     int odd;          // infinities or NaN were taken out of the unit's values
 };
 
+__device__ __forceinline__ void load_q(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(fer::dev::smem_addr(bar))
+        : "memory");
+}
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int r, int head, int page, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
@@ -477,11 +488,16 @@ template <int D>
 __device__ __forceinline__ bool any_hidden(const Unit& u, int s0, int n) {
     return s0 + n > u.all_hi || (s0 < u.all_lo && s0 + n > u.sink);
 }
-// The halves of a word of two 16-bit floats that are infinite or NaN.
+// The upper bits of those halves of a word of two 16-bit floats that are infinite or NaN (all ones in the exponent), and all
+// bits of such halves.
+template <typename T>
+__device__ __forceinline__ uint32_t odd_tops(uint32_t v) {
+    constexpr uint32_t kExp = __is_same(T, __half) ? 0x7c007c00u : 0x7f807f80u, kOne = __is_same(T, __half) ? 0x04000400u : 0x00800080u;
+    return ((v & kExp) + kOne) & 0x80008000u;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t odd_halves(uint32_t v) {
-    constexpr uint32_t kExp = __is_same(T, __half) ? 0x7c007c00u : 0x7f807f80u, kOne = __is_same(T, __half) ? 0x04000400u : 0x00800080u;
-    const uint32_t top = ((v & kExp) + kOne) & 0x80008000u;   // set where the exponent is all ones
+    const uint32_t top = odd_tops<T>(v);
     return (top & 0x8000u ? 0xffffu : 0u) | (top >> 31 ? 0xffff0000u : 0u);
 }
 
@@ -489,32 +505,32 @@ __device__ __forceinline__ uint32_t odd_halves(uint32_t v) {
 // infinite and NaN elements of the others too, noted in *odd. By the 128 threads of a sub-tile, t of them.
 template <typename T, int D>
 __device__ __forceinline__ void clean_values(const Unit& u, uint8_t* at, int s0, int t, volatile int* odd) {
-    constexpr int kPieces = D / 8, kStep = 128 / kPieces, kTimes = 64 / kStep;   // rows at once, and how often
-    const int pc = t % kPieces;
-    uint8_t* const column = at + (pc >> 3) * Cut<D>::kBand;
-#pragma unroll 1
-    for (int k0 = 0; k0 < kTimes; k0 += 4) {
-        uint4 w[4];
+    constexpr int kPieces = D / 16;   // a thread's, half a row
+    const int e = t & 63, s = s0 + e, first = (t >> 6) * kPieces;
+    if (!hidden(u, s)) return;
+    const bool dead = s >= u.hi || (s < u.lo && s >= u.sink);
+    uint8_t* const row = at + e * 128;
+    const auto piece = [&](int i) {
+        return reinterpret_cast<uint4*>(row + ((first + i) >> 3) * Cut<D>::kBand + ((((first + i) ^ e) & 7) << 4));
+    };
+    if (dead) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int e = (k0 + k) * kStep + t / kPieces, s = s0 + e;
-            w[k] = make_uint4(0, 0, 0, 0);
-            if (hidden(u, s)) w[k] = *reinterpret_cast<const uint4*>(column + e * 128 + (((pc ^ e) & 7) << 4));
-        }
+        for (int i = 0; i < kPieces; ++i) *piece(i) = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    uint32_t any = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int e = (k0 + k) * kStep + t / kPieces, s = s0 + e;
-            const bool dead = s >= u.hi || (s < u.lo && s >= u.sink);
-            const uint32_t a = odd_halves<T>(w[k].x), b = odd_halves<T>(w[k].y), c = odd_halves<T>(w[k].z), d = odd_halves<T>(w[k].w);
-            if (dead) {
-                *reinterpret_cast<uint4*>(column + e * 128 + (((pc ^ e) & 7) << 4)) = make_uint4(0, 0, 0, 0);
-            } else if (a | b | c | d) {
-                *odd = 1;
-                __threadfence_block();   // whoever finds the zeros finds the note
-                *reinterpret_cast<uint4*>(column + e * 128 + (((pc ^ e) & 7) << 4)) =
-                    make_uint4(w[k].x & ~a, w[k].y & ~b, w[k].z & ~c, w[k].w & ~d);
-            }
-        }
+    for (int i = 0; i < kPieces; ++i) {
+        const uint4 w = *piece(i);
+        any |= odd_tops<T>(w.x) | odd_tops<T>(w.y) | odd_tops<T>(w.z) | odd_tops<T>(w.w);
+    }
+    if (!any) return;
+    *odd = 1;
+    __threadfence_block();   // whoever finds the zeros finds the note
+    for (int i = 0; i < kPieces; ++i) {
+        uint4 w = *piece(i);
+        w.x &= ~odd_halves<T>(w.x), w.y &= ~odd_halves<T>(w.y), w.z &= ~odd_halves<T>(w.z), w.w &= ~odd_halves<T>(w.w);
+        *piece(i) = w;
     }
 }
 
@@ -542,7 +558,8 @@ __device__ __noinline__ void add_odd(const Paged& c, const TileParams& p, const 
 template <typename T, int D>
 __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     attn_tiles(const __grid_constant__ Paged c, const __grid_constant__ TileParams p, const __grid_constant__ CUtensorMap k_map,
-               const __grid_constant__ CUtensorMap v_map) {
+               const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap q_map,
+               const __grid_constant__ CUtensorMap q_few_map) {
     using C = Cut<D>;
     constexpr bool kBf16 = !__is_same(T, __half);
     constexpr uint32_t kIdS = idesc(64, kBf16, false), kIdO = idesc(D, kBf16, true);
@@ -569,6 +586,8 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
         fer::dev::fence_mbar_init();
         fer::dev::prefetch_tmap(&k_map);
         fer::dev::prefetch_tmap(&v_map);
+        if (p.q_maps != kQLoads) fer::dev::prefetch_tmap(&q_map);
+        if (p.q_maps == kQBoxes) fer::dev::prefetch_tmap(&q_few_map);
     }
     if (w == C::kSoft + 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(fer::dev::smem_addr(&sh.tmem)),
@@ -851,7 +870,6 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // ---- queries, read while the unit before still computes; few rows go to each quarter of the sub-tile
             uint32_t n_q[2] = {0, 0};
             int turn = 0;
-            const bool wide = (reinterpret_cast<uintptr_t>(p.q) | (p.qs * 2)) % 16 == 0;
             for (int k = 0; ok; ++k) {
                 const int slot = k % kUnitSlots;
                 ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
@@ -863,39 +881,54 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 if (u.c1 == u.c0) continue;
                 const bool alt = alternate<D>(u);
                 const int copies = u.nf <= kFew ? 4 : 1;
-                constexpr int kPieces = D / 8, kAtOnce = 32 / kPieces;   // of a row, and rows at once
 #pragma unroll
                 for (int i = 0; i < C::kSubs; ++i) {
                     if (alt && i != turn) continue;
                     ok = ok && warp_wait(&sh.q_empty[i], n_q[i]++ ^ 1u);   // what was there has been multiplied
                     if (!ok) break;
-                    const int first = alt ? 0 : 128 * i, rows = min(128, u.nf - first), pc = lane % kPieces;
-                    // this lane's row: token and head of the group
-                    int tok = p.by_group(u.f0 + first + lane / kPieces), g = u.f0 + first + lane / kPieces - tok * p.group;
-                    uint8_t* const to = smem_at + i * C::kQ + (pc >> 3) * 16384;
-                    for (int f = lane / kPieces; f < rows; f += kAtOnce) {
-                        const uint16_t* const src = reinterpret_cast<const uint16_t*>(p.q) + (static_cast<size_t>(u.tok0) + tok) * p.qs +
-                                                    (static_cast<size_t>(u.hk) * p.group + g) * D + pc * 8;
-                        for (int j = 0; j < copies; ++j) {
-                            uint8_t* const dst = to + (f + 32 * j) * 128 + (((pc ^ f) & 7) << 4);
-                            if (wide) {
-                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(fer::dev::smem_addr(dst)), "l"(src) : "memory");
-                            } else {
-                                uint32_t e[4];
-#pragma unroll
-                                for (int h = 0; h < 4; ++h) e[h] = src[2 * h] | static_cast<uint32_t>(src[2 * h + 1]) << 16;
-                                *reinterpret_cast<uint4*>(dst) = make_uint4(e[0], e[1], e[2], e[3]);
-                            }
+                    const int f0 = u.f0 + (alt ? 0 : 128 * i), rows = min(128, u.f0 + u.nf - f0);
+                    const uint32_t to = smem + i * C::kQ;
+                    if (p.q_maps == kQBoxes) {
+                        // all rows, or a quarter's for each, in one box a band: rows behind the unit's are of no matter
+                        if (lane == 0) fer::dev::mbar_arrive_expect_tx(&sh.q_full[i], C::kQ);
+                        __syncwarp();
+                        if (lane < copies * C::kBands)
+                            load_q(to + lane % C::kBands * 16384 + lane / C::kBands * 4096, copies == 1 ? &q_map : &q_few_map,
+                                   lane % C::kBands * 64, u.hk * p.group, u.tok0 + p.by_group(f0), &sh.q_full[i]);
+                    } else if (p.q_maps == kQRows) {
+                        if (lane == 0) fer::dev::mbar_arrive_expect_tx(&sh.q_full[i], rows * copies * C::kBands * 128);
+                        __syncwarp();
+                        for (int j = lane; j < rows * copies; j += 32) {
+                            const int f = copies == 1 ? j : j >> 2, row = copies == 1 ? j : f + 32 * (j & 3);
+                            const int tok = p.by_group(f0 + f), g = f0 + f - tok * p.group;
+                            for (int band = 0; band < C::kBands; ++band)
+                                load_q(to + band * 16384 + row * 128, &q_map, band * 64, u.hk * p.group + g, u.tok0 + tok, &sh.q_full[i]);
                         }
-                        for (g += kAtOnce; g >= p.group; g -= p.group) ++tok;
+                    } else {
+                        // rows at addresses that tensor copies do not take
+                        for (int j = lane; j < rows * (D / 8); j += 32) {
+                            const int f = j / (D / 8), pc = j % (D / 8), tok = p.by_group(f0 + f), g = f0 + f - tok * p.group;
+                            const uint16_t* const src = reinterpret_cast<const uint16_t*>(p.q) + (static_cast<size_t>(u.tok0) + tok) * p.qs +
+                                                        (static_cast<size_t>(u.hk) * p.group + g) * D + pc * 8;
+                            uint32_t e[4];
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) e[h] = src[2 * h] | static_cast<uint32_t>(src[2 * h + 1]) << 16;
+                            for (int c4 = 0; c4 < copies; ++c4)
+                                *reinterpret_cast<uint4*>(smem_at + i * C::kQ + (pc >> 3) * 16384 + (f + 32 * c4) * 128 +
+                                                          (((pc ^ f) & 7) << 4)) = make_uint4(e[0], e[1], e[2], e[3]);
+                        }
+                        fer::dev::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) fer::dev::mbar_arrive(&sh.q_full[i]);
                     }
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    fer::dev::fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) fer::dev::mbar_arrive(&sh.q_full[i]);
                 }
                 if (alt) turn ^= 1;
             }
+            // the copies have landed before this warp leaves, whatever became of the others
+#pragma unroll
+            for (int i = 0; i < C::kSubs; ++i)
+                if (p.q_maps != kQLoads && n_q[i] > 0 && ok) ok = warp_wait(&sh.q_full[i], n_q[i] - 1);
             if (!ok) {
                 if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutSync);
                 *stop = 1;
@@ -1154,42 +1187,42 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     uint8_t* const mine_at = turn + lane * 128;
                     const int span = u.part >= 0 ? 32 : 64;   // dims in 128 bytes
 #pragma unroll 1
-                    for (int d = d0; d < d1; d += 16) {
-                        float o[16];
-                        {
-                            uint32_t a[16], b[16];
-                            if (nb > 0) tmem_ld16(at_a + d, a);
-                            if (alt && nb > 1) tmem_ld16(at_b + d, b);
+                    for (int d = d0; d < d1; d += 32) {
+                        float o[2][32];
+                        if (nb > 0) {
+                            tmem_ld(at_a + d, o[0]);
+                            if (alt && nb > 1) tmem_ld(at_b + d, o[1]);
+                            wait_ld(o);
+                        }
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                o[e] = nb > 0 ? __uint_as_float(a[e]) * wa : 0.0f;
-                                if (alt && nb > 1) o[e] = fmaf(__uint_as_float(b[e]), wb, o[e]);
-                            }
+                        for (int e = 0; e < 32; ++e) {
+                            o[0][e] = nb > 0 ? o[0][e] * wa : 0.0f;
+                            if (alt && nb > 1) o[0][e] = fmaf(o[1][e], wb, o[0][e]);
                         }
                         if (odd) {
-                            float y[16];
+                            float y[32];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) y[e] = o[e];
-                            add_odd<T, D, 16>(c, p, u, fr, d, y);
+                            for (int e = 0; e < 32; ++e) y[e] = o[0][e];
+                            add_odd<T, D, 32>(c, p, u, fr, d, y);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = y[e];
+                            for (int e = 0; e < 32; ++e) o[0][e] = y[e];
                         }
                         const int off = (d - d0) % span;
                         if (u.part >= 0) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                *reinterpret_cast<float4*>(mine_at + (((off / 4 + e) ^ lane) & 7) * 16) =
-                                    make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                            for (int e = 0; e < 8; ++e)
+                                *reinterpret_cast<float4*>(mine_at + ((e ^ lane) & 7) * 16) =
+                                    make_float4(o[0][4 * e], o[0][4 * e + 1], o[0][4 * e + 2], o[0][4 * e + 3]);
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
+                            for (int e = 0; e < 4; ++e)
                                 *reinterpret_cast<uint4*>(mine_at + (((off / 8 + e) ^ lane) & 7) * 16) =
-                                    make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
-                                               pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+                                    make_uint4(pack2<T>(o[0][8 * e], o[0][8 * e + 1]), pack2<T>(o[0][8 * e + 2], o[0][8 * e + 3]),
+                                               pack2<T>(o[0][8 * e + 4], o[0][8 * e + 5]), pack2<T>(o[0][8 * e + 6], o[0][8 * e + 7]));
                         }
-                        if (off + 16 < span && d + 16 < d1) continue;
+                        if (off + 32 < span && d + 32 < d1) continue;
                         __syncwarp();
-                        const int begin = d - off, pieces = (off + 16) * size / 16;
+                        const int begin = d - off, pieces = (off + 32) * size / 16;
                         const unsigned long long column = static_cast<unsigned long long>(begin) * size + (lane & 7) * 16;
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
@@ -1365,6 +1398,18 @@ bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int r
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Boxes of 64 dims x `heads` heads x `tokens` rows of q; 128-byte swizzle.
+bool map_queries(CUtensorMap* m, const TileParams& p, int head_dim, uint32_t dtype, int heads, int tokens) {
+    const fer::host::EncodeTiledFn fn = fer::host::encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(p.heads), static_cast<cuuint64_t>(p.rows)};
+    const cuuint64_t strides[2] = {2ull * head_dim, 2ull * p.qs};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(tokens)}, step[3] = {1, 1, 1};
+    return fn(m, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p.q), dims,
+              strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Sets the shared-memory limit of a kernel once per device.
 cudaError_t allow(const void* kernel, int smem, std::atomic<bool>* known) {
     int dev = 0;
@@ -1378,20 +1423,30 @@ cudaError_t allow(const void* kernel, int smem, std::atomic<bool>* known) {
 }
 
 template <typename T, int D>
-cudaError_t run(const Paged& c, const TileParams& p, cudaStream_t s) {
+cudaError_t run(const Paged& c, TileParams& p, cudaStream_t s) {
     using C = Cut<D>;
     static std::atomic<bool> known[fer::host::kMaxDevices];
     cudaError_t e = allow(reinterpret_cast<const void*>(attn_tiles<T, D>), C::kSmem, known);
     if (e != cudaSuccess) return e;
-    CUtensorMap k_map, v_map;
+    CUtensorMap k_map, v_map, q_map{}, q_few_map{};
     const int rows = C::kKeys < c.page_size() ? C::kKeys : c.page_size();
     const uint32_t dtype = __is_same(T, __half) ? 1 : 2;
     if (!map_pages(&k_map, c, c.k, dtype, rows) || !map_pages(&v_map, c, c.v, dtype, rows)) return cudaErrorInvalidValue;
+    const bool aligned = (reinterpret_cast<uintptr_t>(p.q) | (p.qs * 2)) % 16 == 0 && p.qs * 2 < (1ull << 40);
+    p.q_maps = !aligned ? kQLoads : 128 % p.group == 0 ? kQBoxes : kQRows;
+    if (p.q_maps == kQBoxes) {
+        // a group of 64 or 128 has no unit of few rows
+        if (!map_queries(&q_map, p, D, dtype, p.group, 128 / p.group) ||
+            !map_queries(&q_few_map, p, D, dtype, p.group < 32 ? p.group : 32, p.group < 32 ? 32 / p.group : 1))
+            return cudaErrorInvalidValue;
+    } else if (p.q_maps == kQRows && !map_queries(&q_map, p, D, dtype, 1, 1)) {
+        return cudaErrorInvalidValue;
+    }
     // no more CTAs than there can be units
     const long long tiles = ceil_div(static_cast<long long>(p.rows) * p.group, C::kRows) + p.n_seq;
     long long most = tiles * c.kv_heads * (p.parts > 0 ? p.parts : 1);
     const int grid = static_cast<int>(most < kSms ? most : kSms);
-    e = fer::host::launch_pdl(attn_tiles<T, D>, dim3(grid), dim3(C::kThreads), C::kSmem, s, c, p, k_map, v_map);
+    e = fer::host::launch_pdl(attn_tiles<T, D>, dim3(grid), dim3(C::kThreads), C::kSmem, s, c, p, k_map, v_map, q_map, q_few_map);
     if (e == cudaSuccess && p.parts > 0) {
         const long long ctas = ceil_div(static_cast<long long>(p.rows) * p.heads, kJoinWarps);
         e = fer::host::launch_pdl(attn_join<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(32 * kJoinWarps), 0, s, c, p,
@@ -1401,7 +1456,7 @@ cudaError_t run(const Paged& c, const TileParams& p, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t run_dim(const Paged& c, const TileParams& p, cudaStream_t s) {
+cudaError_t run_dim(const Paged& c, TileParams& p, cudaStream_t s) {
     switch (c.head_dim) {
         case 64: return run<T, 64>(c, p, s);
         case 128: return run<T, 128>(c, p, s);
