@@ -54,7 +54,7 @@ namespace {
 using fer::dev::Paged;
 
 constexpr int kSms = 148;
-constexpr int kSegments = 64;        // entries of the unit table
+constexpr int kSegments = 128;       // entries of the unit table
 constexpr int kUnitSlots = 3;        // units handed from the loading warp to the others
 constexpr int kBadRing = 16;         // key blocks whose flag is kept
 constexpr int kJoinWarps = 8;
@@ -74,15 +74,16 @@ template <int D> struct Cut {
     static constexpr int kBand = kKeys * 128;        // 64 dims of a tile's keys
     static constexpr int kStages = D == 64 ? 8 : 4;
     static constexpr int kQ = 128 * D * 2;           // queries of a sub-tile
-    static constexpr int kSoft = 8 * kSubs;          // softmax warps: two of 64 keys each for 32 rows
+    static constexpr int kSoft = 4 * kSubs;          // softmax warps
     static constexpr int kParts = kKeys / 64;        // 64 keys at a time
-    // They, one that loads keys and values, one for each sub-tile that issues products, one that loads queries. Registers: of
-    // 96 a thread at launch (20 warps) the softmax warps take 104 and the others keep 64.
+    // Softmax warps, one that loads keys and values, one for each sub-tile that issues products, one that loads queries.
+    // Registers: of 168 a thread at launch the two groups of four softmax warps take 208 and leave the third group's warps
+    // 88. (One group has enough at launch.)
     static constexpr bool kShift = kSubs == 2;
     static constexpr int kThreads = 32 * (kSoft + kSubs + 2);
     static constexpr int kRing = kSubs * kQ;         // where the ring begins
     static constexpr int kMeet = kRing + kStages * kTile;   // 32 KB in which results are added up and turned round
-    static constexpr int kShared = kMeet + 32768;           // struct Shared
+    static constexpr int kSmem = kMeet + 32768 + 1024;
     static constexpr uint32_t kColO = 256;           // O of sub-tile x at kColO + x D, S and P of 64 keys at 128 x and 128 x + 64
     // rows up to which P's rounding is made up for
     static constexpr int kFine = kSubs == 2 ? 128 : 64;
@@ -293,8 +294,7 @@ struct Shared {
     uint64_t q_full[2], q_empty[2], s_full[2][2], p_full[2][2], o_full[2][2];
     Unit unit[kUnitSlots];
     int bad[kBadRing];
-    int units[kSegments], sum[20];
-    float top[2][2][128];   // of a row's two threads
+    int units[kSegments], sum[12];
     uint32_t tmem;
     int stop, leave;
     int odd;          // infinities or NaN were taken out of the unit's values
@@ -313,9 +313,9 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
-// 512 threads x 104 and 128 x 64 are the 640 x 96 of the launch.
-__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 104;"); }
-__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+// 256 threads x 208 and 128 x 88 are the 384 x 168 of the launch.
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
 
 // Shared-memory matrix descriptors, 128-byte swizzle, 1024 bytes from eight rows to the next: the upper word is the same for
 // all, the lower has the address and the bytes from one band to the next, so a step along the tile is one addition.
@@ -565,14 +565,11 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     constexpr uint32_t kIdS = idesc(64, kBf16, false), kIdO = idesc(D, kBf16, true);
     // P is 2^(s - m + kUp): 16-bit floats of 5 exponent bits keep small ones so; with kSlack it stays below 2^15
     constexpr float kUp = kBf16 ? 0.0f : 8.0f;
-    extern __shared__ __align__(1024) uint8_t smem_at[];
-    Shared<C::kStages>& sh = *reinterpret_cast<Shared<C::kStages>*>(smem_at + C::kShared);
-    const uint32_t smem = fer::dev::smem_addr(smem_at), ring = smem + C::kRing;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Shared<C::kStages> sh;
+    const uint32_t smem = (fer::dev::smem_addr(smem_raw) + 1023u) & ~1023u, ring = smem + C::kRing;
+    uint8_t* const smem_at = smem_raw + (smem - fer::dev::smem_addr(smem_raw));
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-    if (smem % 1024) {   // tiles start at multiples of 1024
-        if (t == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
-        return;
-    }
 
     if (t == 0) {
         for (int i = 0; i < C::kStages; ++i) fer::dev::mbar_init(&sh.full[i], 1), fer::dev::mbar_init(&sh.empty[i], C::kSubs);
@@ -728,7 +725,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // of those that are the other's as soon as they are there.
             const int x = uniform(w - C::kSoft - 1);
             const uint32_t s_at = uniform(tmem) + 128 * x, o_at = uniform(tmem) + C::kColO + x * D;
-            uint32_t tile = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};   // so far
+            uint32_t tile = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0}, n_o = 0;   // so far
             int turn = 0;   // whose place among the queries the next unit of one sub-tile takes
             const auto landed = [&](uint32_t i) {
                 if (ok) ok = warp_wait(&sh.full[i % C::kStages], i / C::kStages);
@@ -775,7 +772,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             mma_ts(o_at, s_at + 64 * at + 32 * (j >> 1) + 16 + 8 * (j & 1), v + j * (2048 / 16), kIdO, 1);
-                    commit(&sh.o_full[x][at]);
+                    commit(&sh.o_full[x][n_o & 1]);
                 };
                 // the tile's last reader lets go of it
                 const auto done = [&](uint32_t i) { commit(&sh.empty[i % C::kStages]); };
@@ -812,6 +809,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                             }
                         }
                         __syncwarp();
+                        ++n_o;
                         tile += more ? 2 : 1;
                     }
                 } else {
@@ -858,6 +856,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                                 }
                             }
                             __syncwarp();
+                            ++n_o;
                         }
                         tile += more ? 2 : 1;
                     }
@@ -937,25 +936,16 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             }
         }
     } else {
-        // ---- softmax, a row a thread: of the keys of a round (128) one warp takes 64 and another the other 64, on one maximum. Of
-        // few rows (kFew) each is in all four quarters of a sub-tile: two take the first and two the second half of the 64, and
-        // of each two one keeps P's upper and one its lower 16 bits.
+        // ---- softmax, a row a thread, 64 keys at a time; of few rows (kFew) each is in all four quarters of a sub-tile: two take
+        // the first and two the second 32 keys, and of each two one keeps P's upper and one its lower 16 bits
         if constexpr (C::kShift) more_registers();
-        const int x = w >> 3, side = w >> 2 & 1, quarter = w & 3, r = quarter * 32 + lane, half = quarter >> 1, part = quarter & 1;
-        const uint32_t row_at = tmem + (static_cast<uint32_t>(quarter * 32) << 16), s_at = row_at + 128 * x + 64 * side;
-        uint32_t base = 0, block = 0, n_s = 0, n_o[2] = {0, 0};   // n_o: P given so far, by this warp and the other
-        // the two warps of these rows
-        const auto pair = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + 4 * x + quarter) : "memory"); };
-        // a number of this row's other thread; this one is behind its read when it comes again, by a barrier between
-        const auto other = [&](float v) {
-            sh.top[x][side][r] = v;
-            pair();
-            return sh.top[x][side ^ 1][r];
-        };
+        const int x = w >> 2, r = t & 127, half = (w >> 1) & 1, part = w & 1;
+        const uint32_t row_at = tmem + (static_cast<uint32_t>((w & 3) * 32) << 16);
+        uint32_t base = 0, block = 0, n_s0 = 0, n_s1 = 0, n_o = 0;   // n_o: P given so far
         for (int k = 0;; ++k) {
             const int slot = k % kUnitSlots;
             ok = ok && warp_wait(&sh.unit_full[slot], k / kUnitSlots);
-            // all of these warps leave together: each unit has barriers for all of them
+            // both sub-tiles' warps leave together: each unit has barriers for all of them
             if (!ok) *stop = 1;
             meet<32 * C::kSoft>();   // and the unit before is done with its sums and results
             if (t == 0) sh.leave = *stop, sh.odd = 0;
@@ -964,88 +954,81 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 if (!ok && lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutMma);
                 break;
             }
-            const Unit& u = sh.unit[slot];
+            const Unit u = sh.unit[slot];
+            __syncwarp();
+            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
             if (u.tok0 < 0) break;
             const int nb = u.c1 - u.c0, nf = u.nf;
             const bool alt = alternate<D>(u), few = nf <= kFew, fine = nf <= C::kFine;
-            const int f = few ? lane : alt ? r : x * 128 + r, first = alt ? x : 0;
+            const int f = few ? lane : alt ? r : x * 128 + r, first = alt ? x : 0, step = alt ? 2 : 1;
             const bool rows_here = (f & ~31) < nf;                         // of the warp
             const Sees sees(p, u, min(f, nf - 1));
             // what every row of the warp sees, for blocks that need no mask
             const int all_end = __reduce_min_sync(0xffffffffu, sees.end), all_begin = __reduce_max_sync(0xffffffffu, sees.begin);
             float m = -INFINITY, l = 0.0f;
 
-            // The products given so far have been added. Those of this warp's keys come first: behind its last all of the
-            // other's but the last are added.
-            const auto o_added = [&]() {
-                bool done = true;
-                if (n_o[0] > 0) done = warp_wait(&sh.o_full[x][side], n_o[0] - 1);
-                if (done && n_o[1] > 0) done = warp_wait(&sh.o_full[x][side ^ 1], n_o[1] - 1);
-                return done;
+            // The products given so far have been added. They take turns at two barriers: where S of 64 keys is there, the
+            // products of all but the 64 before them are.
+            const auto o_added = [&]() { return warp_wait(&sh.o_full[x][(n_o - 1) & 1], (n_o - 1) >> 1); };
+            // 32 scores, -inf where the row does not see the slot (s0 is the first); masked: some row of the warp sees not all
+            const auto scores = [&](uint32_t at, int s0, bool masked, bool bad, float (&v)[1][32]) {
+                tmem_ld(at, v[0]);
+                wait_ld(v);
+                if (!masked) return;
+                // [begin, end) of the window and [0, sink) within the chunk
+                uint32_t on = (below(sees.end - s0) & ~below(sees.begin - s0)) | below(min(sees.sink, sees.end) - s0);
+                if (bad)
+                    for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
+                        const int page = (s0 + e) >> c.shift;
+                        if (!page_needed(c, u, page) || !c.is_page(table_of(c, p, u)[page])) on &= ~(0xffu << e);
+                    }
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (!(on >> e & 1u)) v[0][e] = -INFINITY;
             };
-            // Probabilities of these 64 keys, from slot s0 on, for N chunks of 32 from chunk j0 on; here: there are some (else only
-            // the maximum is agreed on). kind 0: rounded, 1: and what that leaves, 2: one of the two for these keys, and 0 for
-            // the others. P of a chunk lies over its own scores.
-            const auto softmax = [&](auto chunks, auto kind, int j0, int s0, bool here, bool bad, bool begun) {
-                constexpr int N = decltype(chunks)::value, kKind = decltype(kind)::value;
+            // Probabilities of chunks j0 .. j1 - 1 (of 32) of 64 keys from slot s0 on, whose S is at s_at. P of a chunk lies over
+            // its own scores: 16 words, and in kind 1 what rounding leaves behind them, or, of few rows, one of the two and 0
+            // over the other chunk. Loops are not unrolled: the code of a unit's whole course has to stay in the instruction
+            // cache (unrolled, a third of the fetches missed and prompts behind a window took 478 us, FIGURE so).
+            const auto softmax = [&](auto kind, int j0, int j1, uint32_t s_at, int s0, bool bad, bool begun) {
+                constexpr int kKind = decltype(kind)::value;
                 const bool masked = bad || s0 + 64 > all_end || (s0 < all_begin && s0 + 64 > sees.sink);
-                const auto scores = [&](int j, float (&v)[1][32]) {
-                    tmem_ld(s_at + 32 * (j0 + j), v[0]);
-                    wait_ld(v);
-                    if (!masked) return;
-                    // [b0, e0) of the window and [0, k0) of the sinks, within the chunk
-                    const int s1 = s0 + 32 * (j0 + j);
-                    uint32_t on = (below(sees.end - s1) & ~below(sees.begin - s1)) | below(min(sees.sink, sees.end) - s1);
-                    if (bad)
-                        for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
-                            const int page = (s1 + e) >> c.shift;
-                            if (!page_needed(c, u, page) || !c.is_page(table_of(c, p, u)[page])) on &= ~(0xffu << e);
-                        }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (!(on >> e & 1u)) v[0][e] = -INFINITY;
-                };
                 float top = -INFINITY;
-                if (here) {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        float v[1][32];
-                        scores(j, v);
-                        float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
-#pragma unroll
-                        for (int e = 4; e < 32; e += 2) mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[0][e], v[0][e + 1]);
-                        top = fmaxf(top, fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]));
-                    }
-                }
-                top = fmaxf(top, other(top)) * p.scale2;
-                const bool raise = top > m + kSlack;
-                const float m1 = raise ? top : m, shift = m1 == -INFINITY ? 0.0f : m1;
-                const float a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
-                m = m1;
-                if (begun && __any_sync(0xffffffffu, raise)) {
-                    // the same in both warps: each scales half of the sums, once all given so far are in them
-                    if (ok) ok = o_added();
-                    fence_after();
 #pragma unroll 1
-                    for (int j = side; j < D / 16; j += 2) {
-                        uint32_t o[16];
-                        tmem_ld16(row_at + C::kColO + x * D + 16 * j, o);
+                for (int j = j0; j < j1; ++j) {
+                    float v[1][32];
+                    scores(s_at + 32 * j, s0 + 32 * j, masked, bad, v);
+                    float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-                        tmem_st16(row_at + C::kColO + x * D + 16 * j, o);
-                    }
-                    wait_st();
-                    fence_before();
-                    pair();
+                    for (int e = 4; e < 32; e += 2) mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[0][e], v[0][e + 1]);
+                    top = fmaxf(top, fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]));
                 }
-                if (!here) return;
-                const uint64_t sc2 = fer::dev::f2_splat(p.scale2), nm2 = fer::dev::f2_splat(kUp - shift);
-                uint64_t sum[2] = {0, 0};
+                top *= p.scale2;
+                const bool raise = top > m + kSlack;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float m1 = raise ? top : m, a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
+                    m = m1;
+                    l *= a;
+                    if (begun) {
+                        if (ok) ok = o_added();
+                        fence_after();
+#pragma unroll 1
+                        for (int j = 0; j < D / 16; ++j) {
+                            uint32_t o[16];
+                            tmem_ld16(row_at + C::kColO + x * D + 16 * j, o);
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                            tmem_st16(row_at + C::kColO + x * D + 16 * j, o);
+                        }
+                    }
+                }
+                const uint64_t sc2 = fer::dev::f2_splat(p.scale2), nm2 = fer::dev::f2_splat(kUp - (m == -INFINITY ? 0.0f : m));
+                uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+                for (int j = j0; j < j1; ++j) {
                     float v[1][32];
                     uint32_t hi[16], low[16];
-                    scores(j, v);
+                    scores(s_at + 32 * j, s0 + 32 * j, masked, bad, v);
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         float p0, p1;
@@ -1062,58 +1045,48 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                             float h0, h1;
                             unpack2<T>(hi[e >> 1], h0, h1);
                             low[e >> 1] = pack2<T>(p0 - h0, p1 - h1);
-                            if (kKind == 2 && part) hi[e >> 1] = low[e >> 1];
                         }
                     }
-                    tmem_st16(s_at + 32 * (j0 + j), hi);
-                    if constexpr (kKind == 1) tmem_st16(s_at + 32 * j + 16, low);
-                    if constexpr (kKind == 2) {
+                    if constexpr (kKind > 0) {
+                        if (few) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) low[e] = 0;
-                        tmem_st16(s_at + 32 * (1 - j0), low);
+                            for (int e = 0; e < 16; ++e) hi[e] = part ? low[e] : hi[e], low[e] = 0;
+                        }
+                        tmem_st16(few ? s_at + 32 * (1 - j) : s_at + 32 * j + 16, low);
                     }
+                    tmem_st16(s_at + 32 * j, hi);
                 }
                 float sm[4];
                 fer::dev::f2_unpack(sum[0], sm[0], sm[1]);
                 fer::dev::f2_unpack(sum[1], sm[2], sm[3]);
-                l = l * a + ((sm[0] + sm[1]) + (sm[2] + sm[3]));
+                l += (sm[0] + sm[1]) + (sm[2] + sm[3]);
                 wait_st();
             };
-            // rounds: a block of 128 keys, or two of 64; where blocks alternate every other one
-            const int per = C::kParts == 1 ? 2 : alt ? 2 : 1;
-            for (int i0 = first; i0 < nb; i0 += per) {
-                const int i = C::kParts == 1 ? i0 + side : i0;
-                const bool here = i < nb;       // of an odd number of blocks of 64 the last has no other
-                const int s0 = block_of(u, u.c0 + min(i, nb - 1)) * C::kKeys + (C::kParts == 1 ? 0 : 64 * side);
-                if (here) {
-                    if (ok) ok = warp_wait(&sh.s_full[x][side], n_s);
-                    ++n_s;
+            for (int i = first; i < nb; i += step) {
+                const bool bad = sh.bad[(block + i) % kBadRing] != 0;
+#pragma unroll 1
+                for (int h = 0; h < C::kParts; ++h) {
+                    const int at = C::kParts == 1 ? i & 1 : h, s0 = block_of(u, u.c0 + i) * C::kKeys + 64 * h;
+                    if (ok) ok = warp_wait(&sh.s_full[x][at], at ? n_s1 : n_s0);
+                    at ? ++n_s1 : ++n_s0;
                     fence_after();
-                }
-                if (rows_here) {
-                    using Zero = std::integral_constant<int, 0>;
-                    using One = std::integral_constant<int, 1>;
-                    using Two = std::integral_constant<int, 2>;
-                    const bool bad = sh.bad[(block + i) % kBadRing] != 0, begun = i0 > first;
-                    if (few) softmax(One{}, Two{}, half, s0, here, bad, begun);
-                    else if (fine) softmax(Two{}, One{}, 0, s0, here, bad, begun);
-                    else softmax(Two{}, Zero{}, 0, s0, here, bad, begun);
-                }
-                if (here) {
+                    if (rows_here && ok) {
+                        const uint32_t s_at = row_at + 128 * x + 64 * at;
+                        const bool begun = i > first || h > 0;
+                        if (fine) softmax(std::integral_constant<int, 1>{}, few ? half : 0, few ? half + 1 : 2, s_at, s0, bad, begun);
+                        else softmax(std::integral_constant<int, 0>{}, 0, 2, s_at, s0, bad, begun);
+                    }
                     if (any_hidden<D>(u, s0, 64) && ok) {
                         const uint32_t tile = base + at_v(loads_two<D>(u), i, nb);
                         ok = warp_wait(&sh.full[tile % C::kStages], tile / C::kStages);
-                        if (ok)
-                            clean_values<T, D>(u, smem_at + C::kRing + tile % C::kStages * C::kTile + (C::kParts == 1 ? 0 : side * 8192),
-                                               s0, r, &sh.odd);
+                        if (ok) clean_values<T, D>(u, smem_at + C::kRing + tile % C::kStages * C::kTile + h * 8192, s0, r, &sh.odd);
                         fer::dev::fence_proxy_async_smem();
                     }
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) fer::dev::mbar_arrive(&sh.p_full[x][side]);
-                    ++n_o[0];
+                    if (lane == 0) fer::dev::mbar_arrive(&sh.p_full[x][at]);
+                    ++n_o;
                 }
-                if (C::kParts == 2 || i0 + (side ^ 1) < nb) ++n_o[1];
             }
             const bool mine = first < nb;
             if (mine && ok) ok = o_added();
@@ -1124,17 +1097,16 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // at the next unit where a wait ran out.
             float2* const sums = reinterpret_cast<float2*>(smem_at + C::kMeet);
             const uint32_t o_at = row_at + C::kColO + x * D;
-            if (rows_here) l += other(l);
             if (few) {
-                constexpr int kSums = 4 * C::kSubs;   // of a row; m and l are those of half of them
-                if (side == 0) sums[x * 128 + r] = make_float2(m, l);
+                constexpr int kParts = 4 * C::kSubs;   // sums of a row; m and l are those of half of them
+                sums[t] = make_float2(m, l);
                 meet<32 * C::kSoft>();
                 float all = -INFINITY, total = 0.0f;
 #pragma unroll
-                for (int i = 0; i < kSums; i += 2) all = fmaxf(all, sums[32 * i + lane].x);
+                for (int i = 0; i < kParts; i += 2) all = fmaxf(all, sums[32 * i + lane].x);
                 const float base2 = all == -INFINITY ? 0.0f : all;
 #pragma unroll
-                for (int i = 0; i < kSums; i += 2) total = fmaf(sums[32 * i + lane].y, ex2(sums[32 * i + lane].x - base2), total);
+                for (int i = 0; i < kParts; i += 2) total = fmaf(sums[32 * i + lane].y, ex2(sums[32 * i + lane].x - base2), total);
                 const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
                 const float mine2 = mine && ok ? ex2(m - base2) * scale : 0.0f;
                 meet<32 * C::kSoft>();                 // the sums have been read
@@ -1148,20 +1120,19 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 const int width = min(D, nf <= 8 ? 128 : nf <= 16 ? 64 : 32), rows = 1024 / width;
                 float* const meet_at = reinterpret_cast<float*>(smem_at + C::kMeet);
                 for (int d = 0; d < D; d += width) {
-                    for (int e0 = 16 * side; e0 < width; e0 += 32) {
-                        uint32_t o[16];
-                        if (mine && ok) tmem_ld16(o_at + d + e0, o);
+                    for (int e0 = 0; e0 < width; e0 += 32) {
+                        float o[1][32];
+                        if (mine && ok) {
+                            tmem_ld(o_at + d + e0, o[0]);
+                            wait_ld(o);
+                        }
                         if (on) {
 #pragma unroll
-                            for (int e = 0; e < 16; e += 4) {
+                            for (int e = 0; e < 32; e += 4) {
                                 // 16-byte pieces of neighbouring rows in different banks
                                 float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                if (mine && ok)
-                                    q = make_float4(__uint_as_float(o[e]) * mine2, __uint_as_float(o[e + 1]) * mine2,
-                                                    __uint_as_float(o[e + 2]) * mine2, __uint_as_float(o[e + 3]) * mine2);
-                                const int col = e0 + e;
-                                *reinterpret_cast<float4*>(meet_at + ((x * 4 + quarter) * rows + lane) * width + (col & ~31) +
-                                                           ((col ^ (lane << 2)) & 28)) = q;
+                                if (mine && ok) q = make_float4(o[0][e] * mine2, o[0][e + 1] * mine2, o[0][e + 2] * mine2, o[0][e + 3] * mine2);
+                                *reinterpret_cast<float4*>(meet_at + (w * rows + lane) * width + e0 + ((e ^ (lane << 2)) & 28)) = q;
                             }
                         }
                         __syncwarp();
@@ -1172,7 +1143,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         const float* const from = meet_at + row * width + (e & ~31) + (((e ^ (row << 2)) & 28) | (e & 3));
                         float v = 0.0f;
 #pragma unroll
-                        for (int g = 0; g < kSums; ++g) v += from[g * rows * width];
+                        for (int g = 0; g < kParts; ++g) v += from[g * rows * width];
                         if (nb == 0) v = 0.0f;
                         if (sh.odd) {
                             float one[1] = {v};
@@ -1189,9 +1160,9 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             } else {
                 float all = m, wa = 1.0f, wb = 0.0f, total = l;
                 uint32_t at_a = o_at, at_b = o_at;
-                int share = side, shares = 2;   // of the dims
-                if (alt) {   // both sub-tiles' warps share the dims of both sums
-                    if (side == 0) sums[x * 128 + r] = make_float2(m, l);
+                int d0 = 0, d1 = D;
+                if (alt) {   // each sub-tile's warps take half of the dims of both sums
+                    sums[t] = make_float2(m, l);
                     meet<32 * C::kSoft>();
                     const float2 sa = sums[r], sb = sums[128 + r];
                     all = fmaxf(sa.x, sb.x);
@@ -1199,11 +1170,10 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     wa = ex2(sa.x - base2), wb = ex2(sb.x - base2);
                     total = sa.y * wa + sb.y * wb;
                     meet<32 * C::kSoft>();   // the sums have been read
-                    share += 2 * x, shares = 4;
+                    d0 = x * (D / 2), d1 = d0 + D / 2;
                     at_a = row_at + C::kColO, at_b = at_a + D;
                     fence_after();
                 }
-                const int d0 = share * (D / shares), d1 = d0 + D / shares;
                 const bool on = f < nf;
                 const int fr = min(f, nf - 1), head = q_head(p, u, fr);
                 const size_t tok = q_row(p, u, fr), bh = tok * p.heads + head, place = bh * p.parts + max(u.part, 0);
@@ -1213,14 +1183,13 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     const bool odd = sh.odd != 0;
                     // 128 bytes of each of the warp's rows at a time, turned round in shared memory, so that eight lanes write a
                     // row's 128 bytes
-                    uint8_t* const turn = smem_at + C::kMeet + w * 2048;
+                    uint8_t* const turn = smem_at + C::kMeet + w * 4096;
                     const unsigned long long to = u.part >= 0 ? reinterpret_cast<unsigned long long>(p.part_o + place * D)
                                                               : reinterpret_cast<unsigned long long>(static_cast<T*>(p.out) + tok * p.os + static_cast<size_t>(head) * D);
                     const bool whole = u.part >= 0 || (reinterpret_cast<uintptr_t>(p.out) | (p.os * 2)) % 16 == 0;
                     const int rows = min(32, nf - (f - lane)), size = u.part >= 0 ? 4 : 2;
-                    // 64 bytes of a row at a time, four lanes a row
-                    uint8_t* const mine_at = turn + lane * 64;
-                    const int span = u.part >= 0 ? 16 : 32;
+                    uint8_t* const mine_at = turn + lane * 128;
+                    const int span = u.part >= 0 ? 32 : 64;   // dims in 128 bytes
 #pragma unroll 1
                     for (int d = d0; d < d1; d += 16) {
                         float o[16];
@@ -1246,25 +1215,25 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         if (u.part >= 0) {
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                *reinterpret_cast<float4*>(mine_at + ((e ^ (lane >> 1)) & 3) * 16) =
+                                *reinterpret_cast<float4*>(mine_at + (((off / 4 + e) ^ lane) & 7) * 16) =
                                     make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                         } else {
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
-                                *reinterpret_cast<uint4*>(mine_at + (((off / 8 + e) ^ (lane >> 1)) & 3) * 16) =
+                                *reinterpret_cast<uint4*>(mine_at + (((off / 8 + e) ^ lane) & 7) * 16) =
                                     make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
                                                pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
                         }
                         if (off + 16 < span && d + 16 < d1) continue;
                         __syncwarp();
                         const int begin = d - off, pieces = (off + 16) * size / 16;
-                        const unsigned long long column = static_cast<unsigned long long>(begin) * size + (lane & 3) * 16;
+                        const unsigned long long column = static_cast<unsigned long long>(begin) * size + (lane & 7) * 16;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            const int row = i + (lane >> 2);
+                        for (int i = 0; i < 32; i += 4) {
+                            const int row = i + (lane >> 3);
                             const unsigned long long at = __shfl_sync(0xffffffffu, to, row);
-                            if (row < rows && (lane & 3) < pieces) {
-                                const uint4 v = *reinterpret_cast<const uint4*>(turn + row * 64 + (((lane ^ (row >> 1)) & 3) << 4));
+                            if (row < rows && (lane & 7) < pieces) {
+                                const uint4 v = *reinterpret_cast<const uint4*>(turn + row * 128 + (((lane ^ row) & 7) << 4));
                                 if (whole) {
                                     *reinterpret_cast<uint4*>(at + column) = v;
                                 } else {
@@ -1283,8 +1252,6 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 }
             }
             fence_before();
-            __syncwarp();
-            if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
         }
     }
 
@@ -1463,9 +1430,7 @@ template <typename T, int D>
 cudaError_t run(const Paged& c, TileParams& p, cudaStream_t s) {
     using C = Cut<D>;
     static std::atomic<bool> known[fer::host::kMaxDevices];
-    constexpr int smem = C::kShared + static_cast<int>(sizeof(Shared<C::kStages>));
-    static_assert(smem <= 232448, "shared memory of a CTA");
-    cudaError_t e = allow(reinterpret_cast<const void*>(attn_tiles<T, D>), smem, known);
+    cudaError_t e = allow(reinterpret_cast<const void*>(attn_tiles<T, D>), C::kSmem, known);
     if (e != cudaSuccess) return e;
     CUtensorMap k_map, v_map, q_map{}, q_few_map{};
     const int rows = C::kKeys < c.page_size() ? C::kKeys : c.page_size();
@@ -1485,7 +1450,7 @@ cudaError_t run(const Paged& c, TileParams& p, cudaStream_t s) {
     const long long tiles = ceil_div(static_cast<long long>(p.rows) * p.group, C::kRows) + p.n_seq;
     long long most = tiles * c.kv_heads * (p.parts > 0 ? p.parts : 1);
     const int grid = static_cast<int>(most < kSms ? most : kSms);
-    e = fer::host::launch_pdl(attn_tiles<T, D>, dim3(grid), dim3(C::kThreads), smem, s, c, p, k_map, v_map, q_map, q_few_map);
+    e = fer::host::launch_pdl(attn_tiles<T, D>, dim3(grid), dim3(C::kThreads), C::kSmem, s, c, p, k_map, v_map, q_map, q_few_map);
     if (e == cudaSuccess && p.parts > 0) {
         const long long ctas = ceil_div(static_cast<long long>(p.rows) * p.heads, kJoinWarps);
         e = fer::host::launch_pdl(attn_join<T, D>, dim3(static_cast<unsigned>(ctas)), dim3(32 * kJoinWarps), 0, s, c, p,
