@@ -970,111 +970,111 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // The products given so far have been added. They take turns at two barriers: where S of 64 keys is there, the
             // products of all but the 64 before them are.
             const auto o_added = [&]() { return warp_wait(&sh.o_full[x][(n_o - 1) & 1], (n_o - 1) >> 1); };
-            // 32 scores, -inf where the row does not see the slot (s0 is the first); masked: some row of the warp sees not all
-            const auto scores = [&](uint32_t at, int s0, bool masked, bool bad, float (&v)[1][32]) {
-                tmem_ld(at, v[0]);
-                wait_ld(v);
-                if (!masked) return;
-                // [begin, end) of the window and [0, sink) within the chunk
-                uint32_t on = (below(sees.end - s0) & ~below(sees.begin - s0)) | below(min(sees.sink, sees.end) - s0);
-                if (bad)
-                    for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
-                        const int page = (s0 + e) >> c.shift;
-                        if (!page_needed(c, u, page) || !c.is_page(table_of(c, p, u)[page])) on &= ~(0xffu << e);
-                    }
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    if (!(on >> e & 1u)) v[0][e] = -INFINITY;
-            };
-            // Probabilities of chunks j0 .. j1 - 1 (of 32) of 64 keys from slot s0 on, whose S is at s_at. P of a chunk lies over
-            // its own scores: 16 words, and in kind 1 what rounding leaves behind them, or, of few rows, one of the two and 0
-            // over the other chunk. Loops are not unrolled: the code of a unit's whole course has to stay in the instruction
-            // cache (unrolled, a third of the fetches missed and prompts behind a window took 478 us, FIGURE so).
-            const auto softmax = [&](auto kind, int j0, int j1, uint32_t s_at, int s0, bool bad, bool begun) {
-                constexpr int kKind = decltype(kind)::value;
-                const bool masked = bad || s0 + 64 > all_end || (s0 < all_begin && s0 + 64 > sees.sink);
-                float top = -INFINITY;
-#pragma unroll 1
-                for (int j = j0; j < j1; ++j) {
-                    float v[1][32];
-                    scores(s_at + 32 * j, s0 + 32 * j, masked, bad, v);
-                    float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
-#pragma unroll
-                    for (int e = 4; e < 32; e += 2) mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[0][e], v[0][e + 1]);
-                    top = fmaxf(top, fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]));
-                }
-                top *= p.scale2;
-                const bool raise = top > m + kSlack;
-                if (__any_sync(0xffffffffu, raise)) {
-                    const float m1 = raise ? top : m, a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
-                    m = m1;
-                    l *= a;
-                    if (begun) {
-                        if (ok) ok = o_added();
-                        fence_after();
-#pragma unroll 1
-                        for (int j = 0; j < D / 16; ++j) {
-                            uint32_t o[16];
-                            tmem_ld16(row_at + C::kColO + x * D + 16 * j, o);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-                            tmem_st16(row_at + C::kColO + x * D + 16 * j, o);
-                        }
-                    }
-                }
-                const uint64_t sc2 = fer::dev::f2_splat(p.scale2), nm2 = fer::dev::f2_splat(kUp - (m == -INFINITY ? 0.0f : m));
-                uint64_t sum[2] = {0, 0};
-#pragma unroll 1
-                for (int j = j0; j < j1; ++j) {
-                    float v[1][32];
-                    uint32_t hi[16], low[16];
-                    scores(s_at + 32 * j, s0 + 32 * j, masked, bad, v);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float p0, p1;
-                        const uint64_t t2 = fer::dev::f2_fma(fer::dev::f2_pack(v[0][e], v[0][e + 1]), sc2, nm2);
-                        if (kKind == 0 && (e >> 1) % kPolyOf < kPoly) {
-                            powers2(t2, p0, p1);
-                        } else {
-                            fer::dev::f2_unpack(t2, p0, p1);
-                            p0 = ex2(p0), p1 = ex2(p1);
-                        }
-                        sum[(e >> 1) & 1] = fer::dev::f2_add(sum[(e >> 1) & 1], fer::dev::f2_pack(p0, p1));
-                        hi[e >> 1] = pack2<T>(p0, p1);
-                        if constexpr (kKind > 0) {
-                            float h0, h1;
-                            unpack2<T>(hi[e >> 1], h0, h1);
-                            low[e >> 1] = pack2<T>(p0 - h0, p1 - h1);
-                        }
-                    }
-                    if constexpr (kKind > 0) {
-                        if (few) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) hi[e] = part ? low[e] : hi[e], low[e] = 0;
-                        }
-                        tmem_st16(few ? s_at + 32 * (1 - j) : s_at + 32 * j + 16, low);
-                    }
-                    tmem_st16(s_at + 32 * j, hi);
-                }
-                float sm[4];
-                fer::dev::f2_unpack(sum[0], sm[0], sm[1]);
-                fer::dev::f2_unpack(sum[1], sm[2], sm[3]);
-                l += (sm[0] + sm[1]) + (sm[2] + sm[3]);
-                wait_st();
-            };
-            for (int i = first; i < nb; i += step) {
-                const bool bad = sh.bad[(block + i) % kBadRing] != 0;
-#pragma unroll 1
-                for (int h = 0; h < C::kParts; ++h) {
-                    const int at = C::kParts == 1 ? i & 1 : h, s0 = block_of(u, u.c0 + i) * C::kKeys + 64 * h;
+            // The blocks, 64 keys at a time, N chunks of 32 of them from chunk j0 on. kind 0: P is rounded, 1: what that leaves is
+            // kept too, 2: one of the two for these keys, and 0 for the others. P of a chunk lies over its own scores: 16 words,
+            // and what is left behind them. The next scores are on their way while P is handed over.
+            // Where both sub-tiles have rows of their own their exponentials take turns, so that one's are computed while the
+            // other's scores and products are on their way: left alone the two fall into step (FIGURE).
+            const auto my_turn = [&]() { if (C::kSubs == 2 && !alt) asm volatile("bar.sync %0, 256;" ::"r"(2 + x) : "memory"); };
+            const auto your_turn = [&]() { if (C::kSubs == 2 && !alt) asm volatile("bar.arrive %0, 256;" ::"r"(3 - x) : "memory"); };
+            if (!alt && nb > 0 && x == 1) your_turn();
+            const auto blocks = [&](auto chunks, auto kind, int j0) {
+                constexpr int N = decltype(chunks)::value, kKind = decltype(kind)::value;
+                float v[N][32];
+                const auto load = [&](int at) {   // scores of 64 keys, when they are there
                     if (ok) ok = warp_wait(&sh.s_full[x][at], at ? n_s1 : n_s0);
                     at ? ++n_s1 : ++n_s0;
                     fence_after();
-                    if (rows_here && ok) {
-                        const uint32_t s_at = row_at + 128 * x + 64 * at;
-                        const bool begun = i > first || h > 0;
-                        if (fine) softmax(std::integral_constant<int, 1>{}, few ? half : 0, few ? half + 1 : 2, s_at, s0, bad, begun);
-                        else softmax(std::integral_constant<int, 0>{}, 0, 2, s_at, s0, bad, begun);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) tmem_ld(row_at + 128 * x + 64 * at + 32 * (j0 + j), v[j]);
+                };
+                const auto hand_over = [&](int at) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) fer::dev::mbar_arrive(&sh.p_full[x][at]);
+                    ++n_o;
+                };
+                int i = first, h = 0;
+                load(C::kParts == 1 ? i & 1 : 0);
+                wait_ld(v);
+#pragma unroll 1
+                for (;;) {
+                    const int at = C::kParts == 1 ? i & 1 : h, s0 = block_of(u, u.c0 + i) * C::kKeys + 64 * h;
+                    const uint32_t s_at = row_at + 128 * x + 64 * at;
+                    {
+                        const bool bad = sh.bad[(block + i) % kBadRing] != 0;
+                        if (bad || s0 + 64 > all_end || (s0 < all_begin && s0 + 64 > sees.sink)) {
+#pragma unroll
+                            for (int j = 0; j < N; ++j) {
+                                // [begin, end) of the window and [0, sink) within the chunk
+                                const int s1 = s0 + 32 * (j0 + j);
+                                uint32_t on = (below(sees.end - s1) & ~below(sees.begin - s1)) | below(min(sees.sink, sees.end) - s1);
+                                if (bad)
+                                    for (int e = 0; e < 32; e += 8) {   // pages are of 8 slots and more
+                                        const int page = (s1 + e) >> c.shift;
+                                        if (!page_needed(c, u, page) || !c.is_page(table_of(c, p, u)[page])) on &= ~(0xffu << e);
+                                    }
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (!(on >> e & 1u)) v[j][e] = -INFINITY;
+                            }
+                        }
+                        float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+#pragma unroll
+                        for (int e = 4; e < 32 * N; e += 2)
+                            mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[e >> 5][e & 31], v[e >> 5][(e & 31) + 1]);
+                        const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * p.scale2;
+                        const bool raise = top > m + kSlack;
+                        if (__any_sync(0xffffffffu, raise)) {
+                            const float m1 = raise ? top : m, a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
+                            m = m1;
+                            l *= a;
+                            if (i > first || h > 0) {
+                                if (ok) ok = o_added();
+                                fence_after();
+#pragma unroll 1
+                                for (int j = 0; j < D / 16; ++j) {
+                                    uint32_t o[16];
+                                    tmem_ld16(row_at + C::kColO + x * D + 16 * j, o);
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                                    tmem_st16(row_at + C::kColO + x * D + 16 * j, o);
+                                }
+                            }
+                        }
+                        if (kKind == 0) my_turn();
+                        const uint64_t sc2 = fer::dev::f2_splat(p.scale2), nm2 = fer::dev::f2_splat(kUp - (m == -INFINITY ? 0.0f : m));
+                        uint64_t sum[2] = {0, 0};
+#pragma unroll
+                        for (int j = 0; j < N; ++j) {
+                            uint32_t hi[16], low[16];
+#pragma unroll
+                            for (int e = 0; e < 32; e += 2) {
+                                float p0, p1;
+                                const uint64_t t2 = fer::dev::f2_fma(fer::dev::f2_pack(v[j][e], v[j][e + 1]), sc2, nm2);
+                                if (kKind == 0 && (e >> 1) % kPolyOf < kPoly) {
+                                    powers2(t2, p0, p1);
+                                } else {
+                                    fer::dev::f2_unpack(t2, p0, p1);
+                                    p0 = ex2(p0), p1 = ex2(p1);
+                                }
+                                sum[(e >> 1) & 1] = fer::dev::f2_add(sum[(e >> 1) & 1], fer::dev::f2_pack(p0, p1));
+                                hi[e >> 1] = pack2<T>(p0, p1);
+                                if constexpr (kKind > 0) {
+                                    float h0, h1;
+                                    unpack2<T>(hi[e >> 1], h0, h1);
+                                    low[e >> 1] = pack2<T>(p0 - h0, p1 - h1);
+                                    if (kKind == 2) hi[e >> 1] = part ? low[e >> 1] : hi[e >> 1], low[e >> 1] = 0;
+                                }
+                            }
+                            tmem_st16(s_at + 32 * (j0 + j), hi);
+                            if constexpr (kKind > 0) tmem_st16(kKind == 1 ? s_at + 32 * j + 16 : s_at + 32 * (1 - j0), low);
+                        }
+                        if (kKind == 0 && (x == 0 || i + 1 < nb || h + 1 < C::kParts)) your_turn();
+                        float sm[4];
+                        fer::dev::f2_unpack(sum[0], sm[0], sm[1]);
+                        fer::dev::f2_unpack(sum[1], sm[2], sm[3]);
+                        l += (sm[0] + sm[1]) + (sm[2] + sm[3]);
                     }
                     if (any_hidden<D>(u, s0, 64) && ok) {
                         const uint32_t tile = base + at_v(loads_two<D>(u), i, nb);
@@ -1082,11 +1082,26 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         if (ok) clean_values<T, D>(u, smem_at + C::kRing + tile % C::kStages * C::kTile + h * 8192, s0, r, &sh.odd);
                         fer::dev::fence_proxy_async_smem();
                     }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) fer::dev::mbar_arrive(&sh.p_full[x][at]);
-                    ++n_o;
+                    if (++h == C::kParts) h = 0, i += step;
+                    if (i >= nb) {
+                        wait_st();
+                        hand_over(at);
+                        break;
+                    }
+                    // S of the next 64 keys lies elsewhere, and has been on its way since P before this was handed over
+                    load(C::kParts == 1 ? i & 1 : h);
+                    wait_st();
+                    hand_over(at);
+                    wait_ld(v);
                 }
+            };
+            if (first < nb) {
+                using Zero = std::integral_constant<int, 0>;
+                using One = std::integral_constant<int, 1>;
+                using Two = std::integral_constant<int, 2>;
+                if (few) blocks(One{}, Two{}, half);
+                else if (fine) blocks(Two{}, One{}, 0);
+                else blocks(Two{}, Zero{}, 0);
             }
             const bool mine = first < nb;
             if (mine && ok) ok = o_added();
