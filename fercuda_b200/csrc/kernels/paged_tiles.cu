@@ -647,38 +647,35 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     if (w >= C::kSoft) {
         if constexpr (C::kShift) fewer_registers();   // all four warps of the group
         if (w == C::kSoft) {
-            // ---- units, and their keys and values. Pages of a block: one a lane.
+            // ---- keys and values. Pages of a block: one a lane.
             const int box_rows = min(C::kKeys, c.page_size()), pages = C::kKeys / box_rows, boxes = pages * C::kBands;
             uint32_t tile = 0, block = 0;   // so far
-            for (int k = 0; ok; ++k) {
+            const auto take = [&](int k) {
                 const int slot = k % kUnitSlots;
-                ok = warp_wait(&sh.unit_empty[slot], (k / kUnitSlots & 1) ^ 1);
-                if (!ok || fer::dev::warp_flag(stop)) break;
-                const long long x = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
-                Unit u{};
-                u.tok0 = -1;
-                if (x < units) u = find_unit<D>(c, p, pre, sh.units, segments, seg, static_cast<int>(x));
-                if (lane == 0) {
-                    sh.unit[slot] = u;
-                    fer::dev::mbar_arrive(&sh.unit_full[slot]);
-                }
+                if (ok) ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
+                Unit u = sh.unit[slot];
                 __syncwarp();
-                if (u.tok0 < 0) break;   // a later round has none either
-                const int32_t* const table = table_of(c, p, u);
+                if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
+                if (!ok || fer::dev::warp_flag(stop)) u.tok0 = -1;
+                return u;
+            };
+            // this lane's page of block i of a unit: -1 where there is none to read
+            const auto page_at = [&](const Unit& u, int i) {
+                if (u.tok0 < 0 || i >= u.c1 - u.c0 || lane >= pages) return -1;
+                const int page = ((block_of(u, u.c0 + i) * C::kKeys) >> c.shift) + lane;
+                if (!page_needed(c, u, page)) return -1;
+                const int id = table_of(c, p, u)[page];
+                return id < 0 ? INT_MAX : id;   // out of range either way
+            };
+            Unit u = take(0);
+            int id0 = page_at(u, 0), id1 = page_at(u, 1), id2 = page_at(u, 2);   // of blocks i, i + 1, i + 2
+            for (int k = 0; ok && u.tok0 >= 0; ++k) {
                 const int nb = u.c1 - u.c0, lead = loads_two<D>(u) ? 2 : 1;
-                // this lane's page of block i: -1 where there is none to read, -2 where its id is out of range
-                const auto page_at = [&](int i) {
-                    if (i >= nb || lane >= pages) return -1;
-                    const int page = ((block_of(u, u.c0 + i) * C::kKeys) >> c.shift) + lane;
-                    if (!page_needed(c, u, page)) return -1;
-                    const int id = table[page];
-                    return c.is_page(id) ? id : -2;
-                };
                 const auto load = [&](int i, int mine, bool value) {
                     const int st = tile % C::kStages;
                     if (ok) ok = warp_wait(&sh.empty[st], (tile / C::kStages & 1) ^ 1);
                     if (!ok) return;
-                    const bool bad = __any_sync(0xffffffffu, mine == -2);
+                    const bool bad = __any_sync(0xffffffffu, mine >= c.pages);
                     if (lane == 0) {
                         if (!value) {
                             sh.bad[block % kBadRing] = bad;
@@ -694,21 +691,28 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                         // slots of no page are read as page `pages`, outside the map: zeros
                         if (j < boxes)
                             load_box(ring + st * C::kTile + band * C::kBand + pg * box_rows * 128, value ? &v_map : &k_map,
-                                     band * 64, s0 & (c.page_size() - 1), u.hk, id < 0 ? c.pages : id, &sh.full[st]);
+                                     band * 64, s0 & (c.page_size() - 1), u.hk, c.is_page(id) ? id : c.pages, &sh.full[st]);
                     }
                     ++tile;
                     if (!value) ++block;
                 };
-                // ids of four blocks: i .. i + 3 when values i are loaded
-                int id0 = page_at(0), id1 = page_at(1), id2 = page_at(2);
                 if (nb > 0) load(0, id0, false);
                 if (lead == 2 && nb > 1) load(1, id1, false);
-                for (int i = 0; i < nb && ok; ++i) {
-                    const int id3 = page_at(i + 3);
-                    load(i, id0, true);
+                // the next unit's first ids are on their way while this one's last tiles wait for room
+                Unit next{};
+                int n0 = -1, n1 = -1, n2 = -1;
+                for (int i = 0; i < max(nb, 1) && ok; ++i) {
+                    const int id3 = page_at(u, i + 3);
+                    if (i + 1 >= nb) {
+                        next = take(k + 1);
+                        n0 = page_at(next, 0), n1 = page_at(next, 1), n2 = page_at(next, 2);
+                    }
+                    if (nb > 0) load(i, id0, true);
                     if (i + lead < nb) load(i + lead, lead == 2 ? id2 : id1, false);
                     id0 = id1, id1 = id2, id2 = id3;
                 }
+                u = next;
+                id0 = n0, id1 = n1, id2 = n2;
             }
             if (!ok) {
                 if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutSync);
@@ -868,18 +872,27 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 *stop = 1;
             }
         } else {
-            // ---- queries, read while the unit before still computes; few rows go to each quarter of the sub-tile
+            // ---- units, one ahead, and their queries, read while the unit before still computes; few rows go to each quarter of
+            // the sub-tile
             uint32_t n_q[2] = {0, 0};
             int turn = 0;
-            for (int k = 0; ok; ++k) {
+            const auto publish = [&](int k) {
                 const int slot = k % kUnitSlots;
-                ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
-                if (!ok || fer::dev::warp_flag(stop)) break;
-                const Unit u = sh.unit[slot];
+                if (ok) ok = warp_wait(&sh.unit_empty[slot], (k / kUnitSlots & 1) ^ 1);
+                const long long x = static_cast<long long>(k) * grid + (k & 1 ? grid - 1 - blockIdx.x : blockIdx.x);
+                Unit u{};
+                u.tok0 = -1;
+                if (!ok || fer::dev::warp_flag(stop)) return u;
+                if (x < units) u = find_unit<D>(c, p, pre, sh.units, segments, seg, static_cast<int>(x));
+                if (lane == 0) {
+                    sh.unit[slot] = u;
+                    fer::dev::mbar_arrive(&sh.unit_full[slot]);
+                }
                 __syncwarp();
-                if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
-                if (u.tok0 < 0) break;
-                if (u.c1 == u.c0) continue;
+                return u;   // the last: a later round has none either
+            };
+            const auto queries = [&](const Unit& u) {
+                if (u.c1 == u.c0) return;
                 const bool alt = alternate<D>(u);
                 const int copies = u.nf <= kFew ? 4 : 1;
 #pragma unroll
@@ -925,6 +938,16 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     __syncwarp();
                 }
                 if (alt) turn ^= 1;
+            };
+            Unit u = publish(0);
+            if (u.tok0 >= 0) {
+                queries(u);
+                u = publish(1);
+            }
+            for (int k = 1; ok && u.tok0 >= 0; ++k) {
+                const Unit next = publish(k + 1);
+                queries(u);
+                u = next;
             }
             // the copies have landed before this warp leaves, whatever became of the others
 #pragma unroll
@@ -1354,9 +1377,14 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 Split split(long long units, long long blocks, long long tile_rows) {
     Split s{INT_MAX, 0};
     long long parts = 1;
-    if (tile_rows <= 64) parts = ceil_div(blocks, 8);            // a part costs little: even shares of ragged lengths
-    else if (units < 8 * kSms) parts = ceil_div(8 * kSms, units);
-    if (tile_rows > 64 && parts > ceil_div(blocks, 32)) parts = ceil_div(blocks, 32);
+    if (tile_rows <= 64) {
+        // a part costs little: even shares of ragged lengths
+        parts = ceil_div(blocks, 8);
+        if (parts > ceil_div(6 * kSms, units)) parts = ceil_div(6 * kSms, units);
+    } else if (units < 8 * kSms) {
+        parts = ceil_div(8 * kSms, units);
+        if (parts > ceil_div(blocks, 32)) parts = ceil_div(blocks, 32);
+    }
     if (parts <= 1) return s;
     s.chunk = static_cast<int>(ceil_div(blocks, parts));
     s.parts = static_cast<int>(ceil_div(blocks, s.chunk));
