@@ -497,9 +497,9 @@ KERNEL_PROTOTYPES = {
     "fer_paged_attention": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_attention_args_t), P, P]),
     "fer_paged_evict_workspace_bytes": (sz, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "fer_paged_evict": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_evict_args_t), P, P]),
-    "fer_norm_rotary": (C.c_int, [C.POINTER(fer_norm_rotary_args_t), P]),
+    "fer_norm_rotary": (C.c_int, [C.POINTER(fer_norm_rotary_args_t), P, P]),
     "fer_norm_rotary_grad_workspace_bytes": (sz, [C.c_int, C.c_int, C.c_int]),
-    "fer_norm_rotary_grad": (C.c_int, [C.POINTER(fer_norm_rotary_args_t), C.POINTER(fer_norm_rotary_grad_t), P]),
+    "fer_norm_rotary_grad": (C.c_int, [C.POINTER(fer_norm_rotary_args_t), C.POINTER(fer_norm_rotary_grad_t), P, P]),
     "fer_paged_plan": (C.c_int, [C.POINTER(fer_paged_plan_args_t), P, P]),
     "fer_paged_window_attention_workspace_bytes": (sz, [C.c_int] * 8),
     "fer_paged_window_attention": (C.c_int, [C.POINTER(fer_paged_view_t), C.POINTER(fer_paged_window_args_t), P, P]),

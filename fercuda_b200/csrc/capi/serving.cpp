@@ -256,7 +256,7 @@ fer_status_t submit_norm_rotary(Session& S, const fer_norm_rotary_request_t& r, 
     const fer_status_t st = open_norm(S, r.rotary, r.q_gamma, r.k_gamma, r.k_heads, r.eps, &t, gamma, &a);
     if (st.code != FER_STATUS_OK) return st;
     if (capturing(S)) return invalid(kCapturing);
-    return finish(S, fer_norm_rotary(&a, S.stream), out_job_id);
+    return finish(S, fer_norm_rotary(&a, S.dev_err, S.stream), out_job_id);
 }
 
 fer_status_t submit_norm_rotary_grad(Session& S, const fer_norm_rotary_grad_request_t& r, uint64_t* out_job_id) {
@@ -299,7 +299,7 @@ fer_status_t submit_norm_rotary_grad(Session& S, const fer_norm_rotary_grad_requ
     d.workspace = ws->ptr;
     d.workspace_bytes = ws->bytes;
     if (capturing(S)) return invalid(kCapturing);
-    return finish(S, fer_norm_rotary_grad(&a, &d, S.stream), out_job_id);
+    return finish(S, fer_norm_rotary_grad(&a, &d, S.dev_err, S.stream), out_job_id);
 }
 
 fer_status_t submit_plan(Session& S, const fer_paged_plan_request_t& r, uint64_t* out_job_id) {

@@ -20,8 +20,10 @@
 // holds a unit: the elements of V pairs, as two pieces of V elements; what lies
 // behind the turned part is in units that do not turn. kAhead heads a lane are
 // loaded before the first is needed.
+#include "f32x2.cuh"
 #include "pdl.cuh"
 #include "pieces.cuh"
+#include "sm100_util.cuh"
 
 #include "fercuda/b200/native.h"
 
@@ -32,6 +34,11 @@
 
 namespace {
 
+using fer::dev::f2_fma;
+using fer::dev::f2_mul;
+using fer::dev::f2_pack;
+using fer::dev::f2_splat;
+using fer::dev::f2_unpack;
 using fer::dev::Piece;
 
 constexpr int kThreads = 256;
@@ -40,6 +47,8 @@ constexpr int kSms = 148;
 constexpr int kMostDim = 256;
 constexpr int kGradCtas = 3 * kSms;      // at most that many partial sums of dgamma
 constexpr int kSumThreads = 1024;
+// The form with copies: warps of a CTA (one an SM), stages of a warp, bytes of a stage's part of a row.
+constexpr int kCopyWarps = 12, kStages = 3, kSegment = 5632;
 
 struct NormParams {
     const void* x;
@@ -54,6 +63,7 @@ struct NormParams {
     int turning, units;      // units of a head, those that turn first
     int lanes_log2;          // lanes a head
     int split, share;        // warps a row, heads of one of them
+    int step_rows, step_parts;   // from a warp's part of a row to its next
     float base, eps;
     uint32_t flags;
 };
@@ -96,7 +106,9 @@ __device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float2 
 
 // A sum over the lanes of a head.
 __device__ __forceinline__ float over_head(float v, int lanes) {
-    for (int off = 1; off < lanes; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1)
+        if (off < lanes) v += __shfl_xor_sync(0xffffffffu, v, off);
     return v;
 }
 
@@ -197,7 +209,8 @@ __global__ void __launch_bounds__(kThreads, V < 4 ? 2 : 3) norm_rotary(const Nor
                     if (hb + j * hp >= hi) break;                     // of the whole warp
                     const int h = hb + j * hp + h0;
                     const bool on = h < hi;
-                    float a[K][2][V], b[GRAD ? K : 1][2][V], squares = 0.0f, dot = 0.0f;
+                    float a[K][2][V], squares = 0.0f;
+                    [[maybe_unused]] float b[GRAD ? K : 1][2][V], dot = 0.0f;
 #pragma unroll
                     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -320,10 +333,319 @@ __global__ void __launch_bounds__(kSumThreads) sum_partials(const float* partial
     if (to) to[c < head_dim ? c : c - head_dim] = static_cast<float>(v);
 }
 
+// The same with rows fetched and results written by bulk copies: every warp has kStages parts of rows in shared memory, one it
+// works on, one that is arriving and one that is leaving, so that far more is in flight than lanes could keep in registers
+// (32768 rows of 32 + 8 heads x 128: 176 us with loads in registers, FIGURE so). x, dy and out are at multiples of 16 bytes.
+template <typename T, bool INTER, bool GRAD>
+__global__ void __launch_bounds__(32 * kCopyWarps, 1) norm_rotary_copies(const NormParams p, uint32_t* err) {
+    constexpr int V = 16 / sizeof(T), kSize = sizeof(T), kBuffers = GRAD ? 2 : 1, kStage = kSegment;   // of all buffers
+    using P = Piece<T, V, V>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t s_full[kCopyWarps][kStages];
+    __shared__ float s_gamma[2][kMostDim];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, half4 = (p.half + 3) & ~3;
+    uint8_t* const mine = smem + w * (kStages * kStage);
+    double* const freq = reinterpret_cast<double*>(smem + kCopyWarps * kStages * kStage);              // [half] turns a position
+    float2* const table = reinterpret_cast<float2*>(freq + half4) + w * half4;
+    const double inv_two_pi = 0.15915494309189535;
+    for (int i = threadIdx.x; i < p.half; i += 32 * kCopyWarps) {
+        int a = 0, lo = 0;
+        while (a + 1 < p.axes && i >= p.bound[a]) lo = p.bound[a++];
+        const double e = (p.flags & FER_ROTARY_FLAG_AXIS_FREQS) ? static_cast<double>(i - lo) / (p.bound[a] - lo)
+                                                                : static_cast<double>(i) / p.half;
+        freq[i] = (GRAD ? -inv_two_pi : inv_two_pi) * exp2(-e * log2(static_cast<double>(p.base)));
+    }
+    if (lane < kStages) fer::dev::mbar_init(&s_full[w][lane], 1);
+    fer::dev::fence_mbar_init();
+    fer::dev::pdl_begin();
+    for (int i = threadIdx.x; i < 2 * p.head_dim; i += 32 * kCopyWarps) {
+        const int k = i >= p.head_dim, d = i - k * p.head_dim;
+        s_gamma[k][d] = p.gamma[k] ? p.gamma[k][d] : 1.0f;
+    }
+    __syncthreads();
+
+    const int lanes = 1 << p.lanes_log2, hp = 32 >> p.lanes_log2;
+    const int u0 = lane & (lanes - 1), h0 = lane >> p.lanes_log2;
+    int at0, at1;
+    place<V, INTER>(p, u0, at0, at1);
+    const bool turning = u0 < p.turning;
+    [[maybe_unused]] uint64_t sum[GRAD ? 2 : 1][2][V / 2] = {};   // dgamma of this lane's elements
+    const float inv_dim = 1.0f / p.head_dim;
+    bool ok = true;
+    // a part of a row, and the one that is a step of all warps behind it
+    struct Part {
+        int row, part;
+        __device__ __forceinline__ void advance(const NormParams& p) {
+            row += p.step_rows;
+            part += p.step_parts;
+            if (part >= p.split) part -= p.split, ++row;
+        }
+    };
+    // a part into a stage
+    const auto fetch = [&](const Part& at, int stage) {
+        if (at.row >= p.rows || lane != 0) return;
+        const int first = at.part * p.share;
+        const uint32_t bytes = static_cast<uint32_t>(min(p.heads - first, p.share)) * p.head_dim * kSize;
+        fer::dev::mbar_arrive_expect_tx(&s_full[w][stage], kBuffers * bytes);
+        uint8_t* const to = mine + stage * kStage;
+        fer::dev::bulk_g2s(to, static_cast<const T*>(p.x) + static_cast<size_t>(at.row) * p.xs + first * p.head_dim, bytes, &s_full[w][stage]);
+        if constexpr (GRAD)
+            fer::dev::bulk_g2s(to + kStage / 2, static_cast<const T*>(p.dy) + static_cast<size_t>(at.row) * p.ys + first * p.head_dim, bytes,
+                               &s_full[w][stage]);
+    };
+    // lane i < axes: the position on axis i
+    const auto position = [&](const Part& at) {
+        return at.row < p.rows && lane < p.axes ? p.positions[static_cast<size_t>(at.row) * p.axes + lane] : 0;
+    };
+    const long long begin = static_cast<long long>(blockIdx.x) * kCopyWarps + w;
+    Part now{static_cast<int>(begin / p.split), static_cast<int>(begin % p.split)}, next = now, ahead = now;
+    next.advance(p);
+    static_assert(kStages == 3, "two parts ahead");
+    fetch(now, 0);
+    fetch(next, 1);
+    ahead = next;
+    ahead.advance(p);
+    int pos = position(now), stage = 0;
+    uint32_t phase = 0;
+    while (now.row < p.rows) {
+        const int first = now.part * p.share, n = min(p.heads - first, p.share);
+        const int next_pos = position(next);
+        __syncwarp();                                                 // the part before has read the table
+        for (int i0 = 0; i0 < p.half; i0 += 32) {
+            const int i = i0 + lane;
+            int a = 0;
+            while (a + 1 < p.axes && i >= p.bound[a]) ++a;
+            const int at = __shfl_sync(0xffffffffu, pos, a);
+            if (i < p.half) {
+                const double turns = static_cast<double>(at) * freq[i];
+                float s, c;
+                sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
+                table[i] = make_float2(c, s);
+            }
+        }
+        __syncwarp();
+        pos = next_pos;
+        // cosines and sines of this lane's pairs, two side by side, and the sines' negatives
+        uint64_t cos2[V / 2], sin2[V / 2], neg2[V / 2];
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+            const int i = u0 * V + e;
+            const float2 c0 = i < p.half ? table[i] : make_float2(1.0f, 0.0f), c1 = i + 1 < p.half ? table[i + 1] : make_float2(1.0f, 0.0f);
+            cos2[e / 2] = f2_pack(c0.x, c1.x);
+            sin2[e / 2] = f2_pack(c0.y, c1.y);
+            neg2[e / 2] = f2_pack(-c0.y, -c1.y);
+        }
+        if (ok) ok = __all_sync(0xffffffffu, fer::dev::mbar_wait(&s_full[w][stage], phase));
+        if (!ok) break;
+        T* const x_at = reinterpret_cast<T*>(mine + stage * kStage);
+        const T* const y_at = reinterpret_cast<const T*>(mine + stage * kStage + kStage / 2);
+        // a and b, the two pieces of a unit, turned
+        const auto turn2 = [&](uint64_t (&a)[V / 2], uint64_t (&b)[V / 2]) {
+            if constexpr (INTER) {
+                // pairs lie side by side: the first V / 2 of the unit's in a
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const auto one = [&](uint64_t& z, int i) {
+                        float x, y, c, d, sn, m;
+                        f2_unpack(z, x, y);
+                        f2_unpack(cos2[i / 2], c, d);
+                        f2_unpack(sin2[i / 2], sn, m);
+                        if (i & 1) c = d, sn = m;
+                        z = f2_pack(x * c - y * sn, x * sn + y * c);
+                    };
+                    one(a[e], e);
+                    one(b[e], V / 2 + e);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V / 2; ++e) {
+                    const uint64_t a0 = a[e];
+                    a[e] = f2_fma(b[e], neg2[e], f2_mul(a0, cos2[e]));
+                    b[e] = f2_fma(a0, sin2[e], f2_mul(b[e], cos2[e]));
+                }
+            }
+        };
+        // the heads of one kind: s 0 query, 1 key; places in the part
+        const auto heads = [&](auto kind, int lo, int hi) {
+            constexpr int s = decltype(kind)::value;
+            if (lo >= hi) return;
+            uint64_t gamma[2][V / 2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int at = c ? at1 : at0;
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    const float4 g = at >= 0 ? *reinterpret_cast<const float4*>(&s_gamma[s][at + e]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    gamma[c][e / 2] = f2_pack(g.x, g.y);
+                    gamma[c][e / 2 + 1] = f2_pack(g.z, g.w);
+                }
+            }
+#pragma unroll 2
+            for (int hb = lo; hb < hi; hb += hp) {
+                const int h = hb + h0;
+                const bool on = h < hi;
+                T* const head = x_at + h * p.head_dim;
+                uint64_t a[2][V / 2], squares = 0;
+                [[maybe_unused]] uint64_t b[GRAD ? 2 : 1][V / 2], dot = 0;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int at = c ? at1 : at0;
+                    float x[V] = {};
+                    [[maybe_unused]] float y[V] = {};
+                    if (on && at >= 0) {
+                        reinterpret_cast<const P*>(head + at)->get(x);
+                        if constexpr (GRAD) reinterpret_cast<const P*>(y_at + h * p.head_dim + at)->get(y);
+                    }
+#pragma unroll
+                    for (int e = 0; e < V / 2; ++e) {
+                        a[c][e] = f2_pack(x[2 * e], x[2 * e + 1]);
+                        if constexpr (GRAD) b[c][e] = f2_pack(y[2 * e], y[2 * e + 1]);
+                        squares = f2_fma(a[c][e], a[c][e], squares);
+                    }
+                }
+                float s0, s1;
+                f2_unpack(squares, s0, s1);
+                // lanes without a head add nothing to dgamma, whatever eps is
+                const float mean = fmaf(over_head(s0 + s1, lanes), inv_dim, p.eps), rr = on ? rsqrtf(mean) : 0.0f;
+                const uint64_t rr2 = f2_splat(rr);
+                if constexpr (GRAD) {
+                    if (turning) turn2(b[0], b[1]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < V / 2; ++e) {
+                            a[c][e] = f2_mul(a[c][e], rr2);
+                            sum[s][c][e] = f2_fma(b[c][e], a[c][e], sum[s][c][e]);
+                            b[c][e] = f2_mul(b[c][e], gamma[c][e]);
+                            dot = f2_fma(b[c][e], a[c][e], dot);
+                        }
+                    f2_unpack(dot, s0, s1);
+                    const uint64_t d2 = f2_splat(-over_head(s0 + s1, lanes) * inv_dim);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < V / 2; ++e) a[c][e] = f2_mul(rr2, f2_fma(d2, a[c][e], b[c][e]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < V / 2; ++e) a[c][e] = f2_mul(f2_mul(a[c][e], rr2), gamma[c][e]);
+                    if (turning) turn2(a[0], a[1]);
+                }
+                if (on) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = c ? at1 : at0;
+                        float x[V];
+#pragma unroll
+                        for (int e = 0; e < V / 2; ++e) f2_unpack(a[c][e], x[2 * e], x[2 * e + 1]);
+                        P y;
+                        y.put(x);
+                        if (at >= 0) *reinterpret_cast<P*>(head + at) = y;
+                    }
+                }
+            }
+        };
+        const int q_end = min(max(p.q_heads - first, 0), n);
+        heads(std::integral_constant<int, 0>{}, 0, q_end);
+        heads(std::integral_constant<int, 1>{}, q_end, n);
+        fer::dev::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            T* const to = static_cast<T*>(p.out) + static_cast<size_t>(now.row) * p.os + first * p.head_dim;
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;" ::"l"(to),
+                         "r"(fer::dev::smem_addr(x_at)), "r"(n * p.head_dim * kSize)
+                         : "memory");
+            // the part before has left its stage
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        }
+        __syncwarp();
+        fetch(ahead, stage == 0 ? kStages - 1 : stage - 1);
+        now = next, next = ahead;
+        ahead.advance(p);
+        if (++stage == kStages) stage = 0, phase ^= 1u;
+    }
+    if (!ok && lane == 0) fer::dev::report(err, fer::dev::kErrTimeoutLoad);
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");   // written before the kernel ends
+
+    if constexpr (GRAD) {
+        // over the heads a warp takes at once, then the warps in order
+        __syncthreads();
+        float(*const s_sum)[2][kMostDim] = reinterpret_cast<float(*)[2][kMostDim]>(smem);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int at = c ? at1 : at0;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    float v, other;
+                    f2_unpack(sum[s][c][e / 2], v, other);
+                    if (e & 1) v = other;
+                    for (int off = lanes; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+                    if (h0 == 0 && at >= 0) s_sum[w][s][at + e] = v;
+                }
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * p.head_dim; i += 32 * kCopyWarps) {
+            const int k = i >= p.head_dim, d = i - k * p.head_dim;
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kCopyWarps; ++j) v += s_sum[j][k][d];
+            p.partial[static_cast<size_t>(blockIdx.x) * 2 * p.head_dim + i] = v;
+        }
+    }
+}
+
 // CTAs of a pass over so many rows and heads; the gradient's workspace has a place for each.
 int grad_ctas(long long warps) {
     const long long ctas = (warps + kWarps - 1) / kWarps;
     return static_cast<int>(ctas < kGradCtas ? ctas : kGradCtas);
+}
+
+cudaError_t sum_up(const NormParams& p, int ctas, float* dq, float* dk, cudaStream_t s) {
+    if (!dq && !dk) return cudaSuccess;
+    return fer::host::launch_pdl(sum_partials, dim3((2 * p.head_dim + 31) / 32), dim3(kSumThreads), 0, s,
+                                 static_cast<const float*>(p.partial), ctas, p.head_dim, dq, dk);
+}
+
+// Units of V pairs a head, and the lanes that take them.
+template <int V>
+void set_units(NormParams& p) {
+    const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
+    p.turning = inter ? (2 * p.half + 2 * V - 1) / (2 * V) : p.half / V;
+    p.units = p.turning + (p.head_dim - 2 * p.half + 2 * V - 1) / (2 * V);
+    p.lanes_log2 = 0;
+    while (p.lanes_log2 < 5 && (1 << p.lanes_log2) < p.units) ++p.lanes_log2;
+}
+
+// The form with copies, for as many parts of rows as its warps' stages have room for and more; false: not taken.
+template <typename T, bool GRAD>
+bool launch_copies(NormParams& p, float* dq, float* dk, uint32_t* err, cudaStream_t s, cudaError_t* result) {
+    constexpr int V = 16 / sizeof(T);
+    set_units<V>(p);
+    const int hp = 32 >> p.lanes_log2, most = kSegment / (GRAD ? 2 : 1) / (p.head_dim * static_cast<int>(sizeof(T)));
+    if (p.units > 32 || most < 1) return false;
+    // equal parts of whole turns of a warp's heads, where a part has room for one
+    int split = (p.heads + most - 1) / most;
+    p.share = (p.heads + split - 1) / split;
+    if (most >= hp) p.share = (p.share + hp - 1) / hp * hp;
+    if (p.share > most) p.share = most >= hp ? most / hp * hp : most;
+    p.split = (p.heads + p.share - 1) / p.share;
+    const long long items = static_cast<long long>(p.rows) * p.split;
+    if (items < 2ll * kSms * kCopyWarps) return false;
+    p.step_rows = kSms * kCopyWarps / p.split;
+    p.step_parts = kSms * kCopyWarps % p.split;
+    if (p.rows > INT_MAX - 3 * kSms * kCopyWarps) return false;
+    const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
+    const int smem = kCopyWarps * kStages * kSegment + ((p.half + 3) & ~3) * static_cast<int>(sizeof(double) + kCopyWarps * sizeof(float2));
+    void (*const kernel)(NormParams, uint32_t*) = inter ? norm_rotary_copies<T, true, GRAD> : norm_rotary_copies<T, false, GRAD>;
+    // the limit is the kernel's on the current device; setting it again costs little beside such a pass
+    *result = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (*result != cudaSuccess) return true;
+    *result = fer::host::launch_pdl(kernel, dim3(kSms), dim3(32 * kCopyWarps), smem, s, p, err);
+    if (*result == cudaSuccess && GRAD) *result = sum_up(p, kSms, dq, dk, s);
+    return true;
 }
 
 template <typename T, int V, int A, bool GRAD>
@@ -332,10 +654,7 @@ cudaError_t launch(NormParams& p, float* dq, float* dk, cudaStream_t s) {
     constexpr int K = V >= 4 ? 1 : V == 2 ? 3 : 4;
     constexpr int kAhead = V < 4 ? 1 : V == 4 && !GRAD ? 4 : 2;
     const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
-    p.turning = inter ? (2 * p.half + 2 * V - 1) / (2 * V) : p.half / V;
-    p.units = p.turning + (p.head_dim - 2 * p.half + 2 * V - 1) / (2 * V);
-    p.lanes_log2 = 0;
-    while (p.lanes_log2 < 5 && (1 << p.lanes_log2) < p.units) ++p.lanes_log2;
+    set_units<V>(p);
     const int hp = 32 >> p.lanes_log2;
     // a warp a row; where that leaves SMs without work, a part of the row's heads
     int split = 1, turns = (p.heads + hp - 1) / hp;
@@ -351,20 +670,20 @@ cudaError_t launch(NormParams& p, float* dq, float* dk, cudaStream_t s) {
     if constexpr (V > 1)
         if (inter) kernel = norm_rotary<T, V, A, true, GRAD, K, kAhead>;
     cudaError_t e = fer::host::launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, s, p);
-    if (e == cudaSuccess && GRAD && (dq || dk))
-        e = fer::host::launch_pdl(sum_partials, dim3((2 * p.head_dim + 31) / 32), dim3(kSumThreads), 0, s,
-                                  static_cast<const float*>(p.partial), grid, p.head_dim, dq, dk);
+    if (e == cudaSuccess && GRAD) e = sum_up(p, grid, dq, dk, s);
     return e;
 }
 
 // The widest power-of-two V elements that every address and size allows.
 template <typename T, bool GRAD>
-cudaError_t dispatch(NormParams& p, float* dq, float* dk, cudaStream_t s) {
+cudaError_t dispatch(NormParams& p, float* dq, float* dk, uint32_t* err, cudaStream_t s) {
     const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
     const uintptr_t addr = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.out) |
                            (GRAD ? reinterpret_cast<uintptr_t>(p.dy) : 0);
     const size_t all = addr / sizeof(T) | p.xs | p.os | (GRAD ? p.ys : 0) | static_cast<size_t>(p.head_dim) |
                        static_cast<size_t>(inter ? 2 * p.half : p.half);
+    cudaError_t result = cudaSuccess;
+    if (all % (16 / sizeof(T)) == 0 && launch_copies<T, GRAD>(p, dq, dk, err, s, &result)) return result;
     if constexpr (sizeof(T) == 2 && !GRAD)   // the gradient has no registers for units of sixteen
         if (all % 8 == 0) return launch<T, 8, 8, GRAD>(p, dq, dk, s);
     const bool whole = !inter || 2 * p.half % 8 == 0;   // else there may be 33 units of 8
@@ -375,7 +694,7 @@ cudaError_t dispatch(NormParams& p, float* dq, float* dk, cudaStream_t s) {
 }
 
 template <bool GRAD>
-cudaError_t run(const fer_norm_rotary_args_t* a, const fer_norm_rotary_grad_t* d, cudaStream_t s) {
+cudaError_t run(const fer_norm_rotary_args_t* a, const fer_norm_rotary_grad_t* d, uint32_t* err, cudaStream_t s) {
     if (!a) return cudaErrorInvalidValue;
     const fer_rotary_args_t& r = a->rotary;
     if (!r.x || !r.out || !r.positions) return cudaErrorInvalidValue;
@@ -440,9 +759,9 @@ cudaError_t run(const fer_norm_rotary_args_t* a, const fer_norm_rotary_grad_t* d
     p.eps = a->eps;
     p.flags = r.flags;
     switch (r.dtype) {
-        case 0: return dispatch<float, GRAD>(p, dq, dk, s);
-        case 1: return dispatch<__half, GRAD>(p, dq, dk, s);
-        default: return dispatch<__nv_bfloat16, GRAD>(p, dq, dk, s);
+        case 0: return dispatch<float, GRAD>(p, dq, dk, err, s);
+        case 1: return dispatch<__half, GRAD>(p, dq, dk, err, s);
+        default: return dispatch<__nv_bfloat16, GRAD>(p, dq, dk, err, s);
     }
 }
 
@@ -454,11 +773,11 @@ extern "C" size_t fer_norm_rotary_grad_workspace_bytes(int rows, int heads, int 
     return static_cast<size_t>(grad_ctas(static_cast<long long>(rows) * heads)) * 2 * head_dim * sizeof(float);
 }
 
-extern "C" cudaError_t fer_norm_rotary(const fer_norm_rotary_args_t* args, cudaStream_t s) {
-    return run<false>(args, nullptr, s);
+extern "C" cudaError_t fer_norm_rotary(const fer_norm_rotary_args_t* args, uint32_t* err, cudaStream_t s) {
+    return run<false>(args, nullptr, err, s);
 }
 
 extern "C" cudaError_t fer_norm_rotary_grad(const fer_norm_rotary_args_t* args, const fer_norm_rotary_grad_t* grad,
-                                            cudaStream_t s) {
-    return run<true>(args, grad, s);
+                                            uint32_t* err, cudaStream_t s) {
+    return run<true>(args, grad, err, s);
 }

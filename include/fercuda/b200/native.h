@@ -204,8 +204,9 @@ typedef struct fer_norm_rotary_grad {
     size_t workspace_bytes;
 } fer_norm_rotary_grad_t;
 size_t fer_norm_rotary_grad_workspace_bytes(int rows, int heads, int head_dim);
-cudaError_t fer_norm_rotary(const fer_norm_rotary_args_t* args, cudaStream_t s);
-cudaError_t fer_norm_rotary_grad(const fer_norm_rotary_args_t* args, const fer_norm_rotary_grad_t* grad, cudaStream_t s);
+cudaError_t fer_norm_rotary(const fer_norm_rotary_args_t* args, uint32_t* err, cudaStream_t s);
+cudaError_t fer_norm_rotary_grad(const fer_norm_rotary_args_t* args, const fer_norm_rotary_grad_t* grad, uint32_t* err,
+                                 cudaStream_t s);
 
 /* ---- paged key-value cache ----------------------------------------------------------
  * K and V in pages [pages][kv_heads][page_size][head_dim] (f16 or bf16, 16-byte
