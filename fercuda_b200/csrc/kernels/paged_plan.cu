@@ -15,7 +15,8 @@
 // neighbouring sequences, the sums are a scan over the cluster's threads, page
 // ids are moved by whole warps, and a row finds its sequence by a search among
 // every few sequences' first rows in shared memory. One CTA does it where there
-// are few rows and sequences.
+// are few rows and sequences; where there are many rows a second launch spreads
+// them over the GPU (1024 requests with 236000 rows: 30 us by the cluster, FIGURE so).
 #include "paged.cuh"
 #include "pdl.cuh"
 
@@ -28,11 +29,12 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
 constexpr int kCtas = 8;             // of a cluster
 constexpr int kStarts = 4096;        // first rows in shared memory
-constexpr int kOneSequences = 1024, kOneRows = 4096;   // what one CTA does alone
+constexpr int kFewSequences = 256, kFewRows = 1024;     // what a small CTA does alone
+constexpr int kOneRows = 4096;       // rows that a CTA fills alone
+constexpr int kManyRows = 16384;     // rows with a launch of their own
+constexpr int kRowThreads = 256;
 
 struct PlanParams {
     int32_t* table;
@@ -41,7 +43,7 @@ struct PlanParams {
     const int32_t* state;
     int32_t *new_held, *new_state, *offsets, *sequences, *positions, *slots;
     int batch, max_pages, pages, shift, rows;
-    int each;        // sequences a thread
+    int each, across;   // sequences a thread, and lanes of a warp that have some
     uint32_t* err;
 };
 
@@ -72,8 +74,8 @@ struct Request {
 __device__ __forceinline__ long long shfl_up(long long v, int off) { return __shfl_up_sync(0xffffffffu, v, off); }
 
 // The sums of the threads before this one over the whole cluster, and the total.
-template <int CTAS>
-__device__ __forceinline__ Sums scan(Sums mine, Sums (&s_warp)[kWarps], Sums& s_cta, Sums& total) {
+template <int CTAS, int THREADS>
+__device__ __forceinline__ Sums scan(Sums mine, Sums (&s_warp)[32], Sums& s_cta, Sums& total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     Sums x = mine;
 #pragma unroll
@@ -85,8 +87,7 @@ __device__ __forceinline__ Sums scan(Sums mine, Sums (&s_warp)[kWarps], Sums& s_
     __syncthreads();
     Sums before{}, all{};
     {
-        Sums v = s_warp[lane];   // kWarps is 32
-        Sums y = v;
+        Sums y = lane < THREADS / 32 ? s_warp[lane] : Sums{};
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
             const Sums z{shfl_up(y.ask, off), shfl_up(y.rows, off), shfl_up(y.give, off)};
@@ -122,14 +123,18 @@ __device__ __forceinline__ size_t ring_at(int first, unsigned i, int n) {
     return at >= static_cast<unsigned>(n) ? at - n : at;
 }
 
-template <int CTAS>
-__global__ void __launch_bounds__(kThreads) plan(const PlanParams p) {
-    __shared__ Sums s_warp[kWarps], s_cta[2];
-    __shared__ int s_start[kStarts];
+// Rows from r0 on, four a thread, step apart; s_start: first rows of every few sequences.
+__device__ __forceinline__ void fill_rows(const PlanParams& p, int* s_start, int starts_most, long long r0, long long step_rows,
+                                          long long total);
+
+template <int CTAS, int THREADS>
+__global__ void __launch_bounds__(THREADS) plan(const PlanParams p, const int fill) {
+    __shared__ Sums s_warp[32], s_cta[2];
+    __shared__ int s_start[CTAS > 1 ? kStarts : kFewSequences];
     const int t = threadIdx.x, lane = t & 31;
     int rank = 0;
     if constexpr (CTAS > 1) rank = static_cast<int>(cg::this_cluster().block_rank());
-    const int thread = rank * kThreads + t;
+    const int thread = rank * THREADS + t;
     fer::dev::pdl_begin();
 
     // a ring that cannot be gives and takes nothing
@@ -139,11 +144,14 @@ __global__ void __launch_bounds__(kThreads) plan(const PlanParams p) {
     const int room = broken ? 0 : p.pages - free;
     const int kept_first = first, kept_free = free;
     if (broken) first = free = 0;
-    const int b0 = thread * p.each, b1 = min(p.batch, b0 + p.each);
+    // few sequences are spread over all warps, as a warp moves the page ids of one at a time
+    const long long place = (static_cast<long long>(thread >> 5) * p.across + lane) * p.each;
+    const int b0 = lane < p.across ? static_cast<int>(min(place, static_cast<long long>(p.batch))) : p.batch;
+    const int b1 = min(p.batch, b0 + p.each);
 
     Sums mine{}, total{};
     for (int b = b0; b < b1; ++b) mine.ask += Request(p, b).ask();
-    const Sums asked = scan<CTAS>(mine, s_warp, s_cta[0], total);
+    const Sums asked = scan<CTAS, THREADS>(mine, s_warp, s_cta[0], total);
     const auto granted = [&](long long before, int ask) { return ask == 0 || before + ask <= free; };
     // what a sequence holds afterwards; where the ring cannot be, nothing goes back
     const auto pages_after = [&](const Request& r, bool on) { return broken ? r.held : on ? r.need : min(r.held, r.keep); };
@@ -160,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) plan(const PlanParams p) {
             mine.give += r.held - min(r.held, pages_after(r, on));
         }
     }
-    Sums at = scan<CTAS>(mine, s_warp, s_cta[1], total);
+    Sums at = scan<CTAS, THREADS>(mine, s_warp, s_cta[1], total);
     if (thread == 0) {
         if (broken) {
             p.new_state[0] = kept_first, p.new_state[1] = kept_free;
@@ -177,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) plan(const PlanParams p) {
     // offsets and pages; a warp moves one sequence's page ids at a time
     long long before = asked.ask;
     for (int i = 0; i < p.each; ++i) {
-        const int b = b0 + i;
+        const int b = b0 + i;   // of lanes without one behind the last
         int held = 0, now = 0;
         long long take_at = 0, give_at = 0;
         if (b < b1) {
@@ -218,16 +226,18 @@ __global__ void __launch_bounds__(kThreads) plan(const PlanParams p) {
     // offsets and page ids are there for every CTA; and each has read the others' shared memory
     if constexpr (CTAS > 1) cg::this_cluster().sync();
     else __syncthreads();
-    if (!p.sequences && !p.positions && !p.slots) return;
+    if (fill) fill_rows(p, s_start, CTAS > 1 ? kStarts : kFewSequences, 4ll * thread, 4ll * CTAS * THREADS, total.rows);
+}
 
-    // rows, four a thread
-    const int step = (p.batch + kStarts - 1) / kStarts, starts = (p.batch + step - 1) / step;
-    for (int i = t; i < starts; i += kThreads) s_start[i] = __ldcg(p.offsets + static_cast<size_t>(i) * step);
+__device__ __forceinline__ void fill_rows(const PlanParams& p, int* s_start, int starts_most, long long r0, long long step_rows,
+                                          long long total) {
+    const int t = threadIdx.x, step = (p.batch + starts_most - 1) / starts_most, starts = (p.batch + step - 1) / step;
+    for (int i = t; i < starts; i += blockDim.x) s_start[i] = __ldcg(p.offsets + static_cast<size_t>(i) * step);
     __syncthreads();
     const bool wide = (reinterpret_cast<uintptr_t>(p.sequences) | reinterpret_cast<uintptr_t>(p.positions) |
                        reinterpret_cast<uintptr_t>(p.slots)) % 16 == 0;
-    const int rows = static_cast<int>(min(total.rows, static_cast<long long>(p.rows)));
-    for (long long r0 = 4ll * thread; r0 < p.rows; r0 += 4ll * CTAS * kThreads) {
+    const int rows = static_cast<int>(min(total, static_cast<long long>(p.rows)));
+    for (; r0 < p.rows; r0 += step_rows) {
         int seq[4], pos[4], slot[4];
         int b = -1, begin = 0, end = 0, length = 0, seen = 0, base = -1, page = -1;
 #pragma unroll
@@ -283,6 +293,14 @@ __global__ void __launch_bounds__(kThreads) plan(const PlanParams p) {
     }
 }
 
+// The rows of a plan whose offsets and pages are there.
+__global__ void __launch_bounds__(kRowThreads) plan_rows(const PlanParams p) {
+    __shared__ int s_start[kStarts];
+    fer::dev::pdl_begin();
+    const long long thread = static_cast<long long>(blockIdx.x) * kRowThreads + threadIdx.x;
+    fill_rows(p, s_start, kStarts, 4 * thread, 4ll * gridDim.x * kRowThreads, __ldcg(p.offsets + p.batch));
+}
+
 }  // namespace
 
 extern "C" cudaError_t fer_paged_plan(const fer_paged_plan_args_t* a, uint32_t* err, cudaStream_t s) {
@@ -320,9 +338,26 @@ extern "C" cudaError_t fer_paged_plan(const fer_paged_plan_args_t* a, uint32_t* 
     p.shift = shift;
     p.rows = a->sequences || a->positions || a->slots ? a->rows : INT_MAX;
     p.err = err;
-    const bool one = a->batch <= kOneSequences && (p.rows <= kOneRows || p.rows == INT_MAX);
-    const int ctas = one ? 1 : kCtas;
-    p.each = (a->batch + ctas * kThreads - 1) / (ctas * kThreads);
-    if (one) return fer::host::launch_pdl(plan<1>, dim3(1), dim3(kThreads), 0, s, p);
-    return fer::host::launch_pdl_cluster(plan<kCtas>, dim3(kCtas), dim3(kThreads), 0, kCtas, s, p);
+    const int fill = a->sequences || a->positions || a->slots;
+    const int alone = fill ? a->rows : 0;
+    p.each = 1;
+    const auto spread = [&](int warps) {
+        p.across = (a->batch + warps - 1) / warps;
+        if (p.across > 32) p.each = (p.across + 31) / 32, p.across = 32;
+    };
+    if (a->batch <= kFewSequences && alone <= kFewRows) {
+        spread(kFewSequences / 32);
+        return fer::host::launch_pdl(plan<1, kFewSequences>, dim3(1), dim3(kFewSequences), 0, s, p, fill);
+    }
+    cudaError_t e;
+    if (a->batch <= kFewSequences && (alone <= kOneRows || alone > kManyRows)) {
+        spread(32);
+        e = fer::host::launch_pdl(plan<1, 1024>, dim3(1), dim3(1024), 0, s, p, alone > kManyRows ? 0 : fill);
+    } else {
+        spread(32 * kCtas);
+        e = fer::host::launch_pdl_cluster(plan<kCtas, 1024>, dim3(kCtas), dim3(1024), 0, kCtas, s, p, alone > kManyRows ? 0 : fill);
+    }
+    if (e != cudaSuccess || alone <= kManyRows) return e;
+    const int ctas = (a->rows - 1) / (4 * kRowThreads) + 1;
+    return fer::host::launch_pdl(plan_rows, dim3(ctas < 4 * 148 ? ctas : 4 * 148), dim3(kRowThreads), 0, s, p);
 }

@@ -47,8 +47,13 @@ constexpr int kSms = 148;
 constexpr int kMostDim = 256;
 constexpr int kGradCtas = 3 * kSms;      // at most that many partial sums of dgamma
 constexpr int kSumThreads = 1024;
-// The form with copies: warps of a CTA (one an SM), stages of a warp, bytes of a stage's part of a row.
-constexpr int kCopyWarps = 12, kStages = 3, kSegment = 5632;
+// The form with copies: warps of a CTA (one an SM), stages of a warp, bytes of a stage's part of a row (x and dy together),
+// heads a lane works on at once. Fewer warps with two heads each suit the gradient's registers: 10007 rows of 24 + 16 heads x
+// 128 take 146 us with the forward's numbers and 101 so, and the forward 160 with the gradient's and 145 so.
+constexpr int kStages = 3;
+template <bool GRAD> struct Copies {
+    static constexpr int kWarps = GRAD ? 12 : 16, kSegment = GRAD ? 5632 : 4096, kAtOnce = GRAD ? 2 : 1;
+};
 
 struct NormParams {
     const void* x;
@@ -63,7 +68,6 @@ struct NormParams {
     int turning, units;      // units of a head, those that turn first
     int lanes_log2;          // lanes a head
     int split, share;        // warps a row, heads of one of them
-    int step_rows, step_parts;   // from a warp's part of a row to its next
     float base, eps;
     uint32_t flags;
 };
@@ -110,6 +114,20 @@ __device__ __forceinline__ float over_head(float v, int lanes) {
     for (int off = 1; off < 32; off <<= 1)
         if (off < lanes) v += __shfl_xor_sync(0xffffffffu, v, off);
     return v;
+}
+
+// The same for several heads at once.
+template <int N>
+__device__ __forceinline__ void over_heads(float (&v)[N], int lanes) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1)
+        if (off < lanes) {
+            float w[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = __shfl_xor_sync(0xffffffffu, v[j], off);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] += w[j];
+        }
 }
 
 // K: units a lane; kAhead: heads a lane loads before it uses the first
@@ -336,9 +354,11 @@ __global__ void __launch_bounds__(kSumThreads) sum_partials(const float* partial
 // The same with rows fetched and results written by bulk copies: every warp has kStages parts of rows in shared memory, one it
 // works on, one that is arriving and one that is leaving, so that far more is in flight than lanes could keep in registers
 // (32768 rows of 32 + 8 heads x 128: 176 us with loads in registers, FIGURE so). x, dy and out are at multiples of 16 bytes.
-template <typename T, bool INTER, bool GRAD>
-__global__ void __launch_bounds__(32 * kCopyWarps, 1) norm_rotary_copies(const NormParams p, uint32_t* err) {
-    constexpr int V = 16 / sizeof(T), kSize = sizeof(T), kBuffers = GRAD ? 2 : 1, kStage = kSegment;   // of all buffers
+// TAIL: not all of a head turns
+template <typename T, bool INTER, bool GRAD, bool TAIL>
+__global__ void __launch_bounds__(32 * Copies<GRAD>::kWarps, 1) norm_rotary_copies(const NormParams p, uint32_t* err) {
+    constexpr int V = 16 / sizeof(T), kSize = sizeof(T), kBuffers = GRAD ? 2 : 1, kStage = Copies<GRAD>::kSegment;
+    constexpr int kAtOnce = Copies<GRAD>::kAtOnce, kCopyWarps = Copies<GRAD>::kWarps;
     using P = Piece<T, V, V>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t s_full[kCopyWarps][kStages];
@@ -372,13 +392,11 @@ __global__ void __launch_bounds__(32 * kCopyWarps, 1) norm_rotary_copies(const N
     [[maybe_unused]] uint64_t sum[GRAD ? 2 : 1][2][V / 2] = {};   // dgamma of this lane's elements
     const float inv_dim = 1.0f / p.head_dim;
     bool ok = true;
-    // a part of a row, and the one that is a step of all warps behind it
+    // a part of a row, and the warp's next: all of a row's, so that its cosines and sines are computed once
     struct Part {
         int row, part;
         __device__ __forceinline__ void advance(const NormParams& p) {
-            row += p.step_rows;
-            part += p.step_parts;
-            if (part >= p.split) part -= p.split, ++row;
+            if (++part == p.split) part = 0, row += gridDim.x * kCopyWarps;
         }
     };
     // a part into a stage
@@ -397,8 +415,7 @@ __global__ void __launch_bounds__(32 * kCopyWarps, 1) norm_rotary_copies(const N
     const auto position = [&](const Part& at) {
         return at.row < p.rows && lane < p.axes ? p.positions[static_cast<size_t>(at.row) * p.axes + lane] : 0;
     };
-    const long long begin = static_cast<long long>(blockIdx.x) * kCopyWarps + w;
-    Part now{static_cast<int>(begin / p.split), static_cast<int>(begin % p.split)}, next = now, ahead = now;
+    Part now{static_cast<int>(blockIdx.x) * kCopyWarps + w, 0}, next = now, ahead = now;
     next.advance(p);
     static_assert(kStages == 3, "two parts ahead");
     fetch(now, 0);
@@ -407,33 +424,34 @@ __global__ void __launch_bounds__(32 * kCopyWarps, 1) norm_rotary_copies(const N
     ahead.advance(p);
     int pos = position(now), stage = 0;
     uint32_t phase = 0;
+    uint64_t cos2[V / 2], sin2[V / 2], neg2[V / 2];
     while (now.row < p.rows) {
         const int first = now.part * p.share, n = min(p.heads - first, p.share);
-        const int next_pos = position(next);
-        __syncwarp();                                                 // the part before has read the table
-        for (int i0 = 0; i0 < p.half; i0 += 32) {
-            const int i = i0 + lane;
-            int a = 0;
-            while (a + 1 < p.axes && i >= p.bound[a]) ++a;
-            const int at = __shfl_sync(0xffffffffu, pos, a);
-            if (i < p.half) {
-                const double turns = static_cast<double>(at) * freq[i];
-                float s, c;
-                sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-                table[i] = make_float2(c, s);
+        if (now.part == 0) {
+            __syncwarp();                                                 // the part before has read the table
+            for (int i0 = 0; i0 < p.half; i0 += 32) {
+                const int i = i0 + lane;
+                int a = 0;
+                while (a + 1 < p.axes && i >= p.bound[a]) ++a;
+                const int at = __shfl_sync(0xffffffffu, pos, a);
+                if (i < p.half) {
+                    const double turns = static_cast<double>(at) * freq[i];
+                    float s, c;
+                    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
+                    table[i] = make_float2(c, s);
+                }
             }
-        }
-        __syncwarp();
-        pos = next_pos;
-        // cosines and sines of this lane's pairs, two side by side, and the sines' negatives
-        uint64_t cos2[V / 2], sin2[V / 2], neg2[V / 2];
+            __syncwarp();
+            pos = position(Part{now.row + static_cast<int>(gridDim.x) * kCopyWarps, 0});
+            // cosines and sines of this lane's pairs, two side by side, and the sines' negatives
 #pragma unroll
-        for (int e = 0; e < V; e += 2) {
-            const int i = u0 * V + e;
-            const float2 c0 = i < p.half ? table[i] : make_float2(1.0f, 0.0f), c1 = i + 1 < p.half ? table[i + 1] : make_float2(1.0f, 0.0f);
-            cos2[e / 2] = f2_pack(c0.x, c1.x);
-            sin2[e / 2] = f2_pack(c0.y, c1.y);
-            neg2[e / 2] = f2_pack(-c0.y, -c1.y);
+            for (int e = 0; e < V; e += 2) {
+                const int i = u0 * V + e;
+                const float2 c0 = i < p.half ? table[i] : make_float2(1.0f, 0.0f), c1 = i + 1 < p.half ? table[i + 1] : make_float2(1.0f, 0.0f);
+                cos2[e / 2] = f2_pack(c0.x, c1.x);
+                sin2[e / 2] = f2_pack(c0.y, c1.y);
+                neg2[e / 2] = f2_pack(-c0.y, -c1.y);
+            }
         }
         if (ok) ok = __all_sync(0xffffffffu, fer::dev::mbar_wait(&s_full[w][stage], phase));
         if (!ok) break;
@@ -480,68 +498,89 @@ __global__ void __launch_bounds__(32 * kCopyWarps, 1) norm_rotary_copies(const N
                     gamma[c][e / 2 + 1] = f2_pack(g.z, g.w);
                 }
             }
-#pragma unroll 2
-            for (int hb = lo; hb < hi; hb += hp) {
-                const int h = hb + h0;
-                const bool on = h < hi;
-                T* const head = x_at + h * p.head_dim;
-                uint64_t a[2][V / 2], squares = 0;
-                [[maybe_unused]] uint64_t b[GRAD ? 2 : 1][V / 2], dot = 0;
+            // kAtOnce heads a lane, whose sums over lanes overlap
+#pragma unroll 1
+            for (int hb = lo; hb < hi; hb += kAtOnce * hp) {
+                uint64_t a[kAtOnce][2][V / 2];
+                [[maybe_unused]] uint64_t b[GRAD ? kAtOnce : 1][2][V / 2];
+                float total[kAtOnce], rr[kAtOnce];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int at = c ? at1 : at0;
-                    float x[V] = {};
-                    [[maybe_unused]] float y[V] = {};
-                    if (on && at >= 0) {
-                        reinterpret_cast<const P*>(head + at)->get(x);
-                        if constexpr (GRAD) reinterpret_cast<const P*>(y_at + h * p.head_dim + at)->get(y);
-                    }
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const int h = hb + j * hp + h0;
+                    uint64_t squares = 0;
 #pragma unroll
-                    for (int e = 0; e < V / 2; ++e) {
-                        a[c][e] = f2_pack(x[2 * e], x[2 * e + 1]);
-                        if constexpr (GRAD) b[c][e] = f2_pack(y[2 * e], y[2 * e + 1]);
-                        squares = f2_fma(a[c][e], a[c][e], squares);
-                    }
-                }
-                float s0, s1;
-                f2_unpack(squares, s0, s1);
-                // lanes without a head add nothing to dgamma, whatever eps is
-                const float mean = fmaf(over_head(s0 + s1, lanes), inv_dim, p.eps), rr = on ? rsqrtf(mean) : 0.0f;
-                const uint64_t rr2 = f2_splat(rr);
-                if constexpr (GRAD) {
-                    if (turning) turn2(b[0], b[1]);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = c ? at1 : at0;
+                        float x[V] = {};
+                        [[maybe_unused]] float y[V] = {};
+                        if (h < hi && at >= 0) {
+                            reinterpret_cast<const P*>(x_at + h * p.head_dim + at)->get(x);
+                            if constexpr (GRAD) reinterpret_cast<const P*>(y_at + h * p.head_dim + at)->get(y);
+                        }
 #pragma unroll
                         for (int e = 0; e < V / 2; ++e) {
-                            a[c][e] = f2_mul(a[c][e], rr2);
-                            sum[s][c][e] = f2_fma(b[c][e], a[c][e], sum[s][c][e]);
-                            b[c][e] = f2_mul(b[c][e], gamma[c][e]);
-                            dot = f2_fma(b[c][e], a[c][e], dot);
+                            a[j][c][e] = f2_pack(x[2 * e], x[2 * e + 1]);
+                            if constexpr (GRAD) b[j][c][e] = f2_pack(y[2 * e], y[2 * e + 1]);
+                            squares = f2_fma(a[j][c][e], a[j][c][e], squares);
                         }
-                    f2_unpack(dot, s0, s1);
-                    const uint64_t d2 = f2_splat(-over_head(s0 + s1, lanes) * inv_dim);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int e = 0; e < V / 2; ++e) a[c][e] = f2_mul(rr2, f2_fma(d2, a[c][e], b[c][e]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int e = 0; e < V / 2; ++e) a[c][e] = f2_mul(f2_mul(a[c][e], rr2), gamma[c][e]);
-                    if (turning) turn2(a[0], a[1]);
+                    }
+                    float s0, s1;
+                    f2_unpack(squares, s0, s1);
+                    total[j] = s0 + s1;
                 }
-                if (on) {
+                over_heads(total, lanes);
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    // lanes without a head add nothing to dgamma, whatever eps is
+                    rr[j] = hb + j * hp + h0 < hi ? rsqrtf(fmaf(total[j], inv_dim, p.eps)) : 0.0f;
+                    const uint64_t rr2 = f2_splat(rr[j]);
+                    if constexpr (GRAD) {
+                        if (!TAIL || turning) turn2(b[j][0], b[j][1]);
+                        uint64_t dot = 0;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int e = 0; e < V / 2; ++e) {
+                                a[j][c][e] = f2_mul(a[j][c][e], rr2);
+                                sum[s][c][e] = f2_fma(b[j][c][e], a[j][c][e], sum[s][c][e]);
+                                b[j][c][e] = f2_mul(b[j][c][e], gamma[c][e]);
+                                dot = f2_fma(b[j][c][e], a[j][c][e], dot);
+                            }
+                        float s0, s1;
+                        f2_unpack(dot, s0, s1);
+                        total[j] = s0 + s1;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int e = 0; e < V / 2; ++e) a[j][c][e] = f2_mul(f2_mul(a[j][c][e], rr2), gamma[c][e]);
+                        if (!TAIL || turning) turn2(a[j][0], a[j][1]);
+                    }
+                }
+                if constexpr (GRAD) {
+                    over_heads(total, lanes);
+#pragma unroll
+                    for (int j = 0; j < kAtOnce; ++j) {
+                        const uint64_t d2 = f2_splat(-total[j] * inv_dim), rr2 = f2_splat(rr[j]);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int e = 0; e < V / 2; ++e) a[j][c][e] = f2_mul(rr2, f2_fma(d2, a[j][c][e], b[j][c][e]));
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < kAtOnce; ++j) {
+                    const int h = hb + j * hp + h0;
+                    if (h >= hi) continue;
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int at = c ? at1 : at0;
                         float x[V];
 #pragma unroll
-                        for (int e = 0; e < V / 2; ++e) f2_unpack(a[c][e], x[2 * e], x[2 * e + 1]);
+                        for (int e = 0; e < V / 2; ++e) f2_unpack(a[j][c][e], x[2 * e], x[2 * e + 1]);
                         P y;
                         y.put(x);
-                        if (at >= 0) *reinterpret_cast<P*>(head + at) = y;
+                        if (at >= 0) *reinterpret_cast<P*>(x_at + h * p.head_dim + at) = y;
                     }
                 }
             }
@@ -622,7 +661,7 @@ void set_units(NormParams& p) {
 // The form with copies, for as many parts of rows as its warps' stages have room for and more; false: not taken.
 template <typename T, bool GRAD>
 bool launch_copies(NormParams& p, float* dq, float* dk, uint32_t* err, cudaStream_t s, cudaError_t* result) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), kCopyWarps = Copies<GRAD>::kWarps, kSegment = Copies<GRAD>::kSegment;
     set_units<V>(p);
     const int hp = 32 >> p.lanes_log2, most = kSegment / (GRAD ? 2 : 1) / (p.head_dim * static_cast<int>(sizeof(T)));
     if (p.units > 32 || most < 1) return false;
@@ -632,14 +671,14 @@ bool launch_copies(NormParams& p, float* dq, float* dk, uint32_t* err, cudaStrea
     if (most >= hp) p.share = (p.share + hp - 1) / hp * hp;
     if (p.share > most) p.share = most >= hp ? most / hp * hp : most;
     p.split = (p.heads + p.share - 1) / p.share;
-    const long long items = static_cast<long long>(p.rows) * p.split;
-    if (items < 2ll * kSms * kCopyWarps) return false;
-    p.step_rows = kSms * kCopyWarps / p.split;
-    p.step_parts = kSms * kCopyWarps % p.split;
-    if (p.rows > INT_MAX - 3 * kSms * kCopyWarps) return false;
+    // every warp has a row or two at least, else the form above shares rows out among warps
+    if (p.rows < kSms * kCopyWarps || p.rows > INT_MAX - 4 * kSms * kCopyWarps) return false;
     const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
     const int smem = kCopyWarps * kStages * kSegment + ((p.half + 3) & ~3) * static_cast<int>(sizeof(double) + kCopyWarps * sizeof(float2));
-    void (*const kernel)(NormParams, uint32_t*) = inter ? norm_rotary_copies<T, true, GRAD> : norm_rotary_copies<T, false, GRAD>;
+    const bool tail = 2 * p.half < p.head_dim;
+    void (*const kernel)(NormParams, uint32_t*) =
+        inter ? (tail ? norm_rotary_copies<T, true, GRAD, true> : norm_rotary_copies<T, true, GRAD, false>)
+              : (tail ? norm_rotary_copies<T, false, GRAD, true> : norm_rotary_copies<T, false, GRAD, false>);
     // the limit is the kernel's on the current device; setting it again costs little beside such a pass
     *result = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (*result != cudaSuccess) return true;
