@@ -173,9 +173,10 @@ __device__ __forceinline__ int tile_range(const TileParams& p, const Seq& q, int
     u.slot0 = q.len - q.n;
     const int first = u.slot0 + p.by_group(u.f0), last = u.slot0 + p.by_group(u.f0 + u.nf - 1);
     u.hi = max(last + 1, 0);
-    u.lo = p.window == INT_MAX ? 0 : max(first + 1 - p.window, 0);
     u.all_hi = max(first + 1, 0);
-    u.all_lo = p.window == INT_MAX ? 0 : max(last + 1 - p.window, 0);
+    // rows may lie before slot 0, so that a difference to the window could pass 32 bits
+    u.lo = p.window == INT_MAX ? 0 : max(u.all_hi - p.window, 0);
+    u.all_lo = p.window == INT_MAX ? 0 : max(u.hi - p.window, 0);
     u.sink = min(p.sinks, u.hi);
     const int end = (u.hi + C::kKeys - 1) / C::kKeys;
     u.wb0 = min(u.lo / C::kKeys, end);
@@ -403,9 +404,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) 
         : "memory");
 }
 
+// NaN if one of them is.
 __device__ __forceinline__ float max3f(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 template <typename T>
@@ -447,7 +449,7 @@ struct Sees {
     int begin, end, sink;
     __device__ __forceinline__ Sees(const TileParams& p, const Unit& u, int f) {
         end = u.seq < 0 ? u.hi : u.slot0 + p.by_group(u.f0 + f) + 1;
-        begin = p.window == INT_MAX || u.seq < 0 ? 0 : max(end - p.window, 0);
+        begin = p.window == INT_MAX || u.seq < 0 ? 0 : max(max(end, 0) - p.window, 0);
         sink = p.sinks;
     }
     __device__ __forceinline__ bool operator()(int s) const { return s < end && (s >= begin || s < sink); }
@@ -985,6 +987,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             const bool alt = alternate<D>(u), few = nf <= kFew, fine = nf <= C::kFine;
             const int f = few ? lane : alt ? r : x * 128 + r, first = alt ? x : 0, step = alt ? 2 : 1;
             const bool rows_here = (f & ~31) < nf;                         // of the warp
+            const bool real = f < nf;                                      // rows behind the unit's hold anything
             const Sees sees(p, u, min(f, nf - 1));
             // what every row of the warp sees, for blocks that need no mask
             const int all_end = __reduce_min_sync(0xffffffffu, sees.end), all_begin = __reduce_max_sync(0xffffffffu, sees.begin);
@@ -1046,8 +1049,10 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
 #pragma unroll
                         for (int e = 4; e < 32 * N; e += 2)
                             mx[(e >> 1) & 3] = max3f(mx[(e >> 1) & 3], v[e >> 5][e & 31], v[e >> 5][(e & 31) + 1]);
-                        const float top = fmaxf(max3f(mx[0], mx[1], mx[2]), mx[3]) * p.scale2;
-                        const bool raise = top > m + kSlack;
+                        // a score of +inf or NaN makes the row NaN: by its maximum, as powers2 does not hand a NaN on
+                        float top = max3f(max3f(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale2;
+                        if (top == INFINITY) top = NAN;
+                        const bool raise = real && !(top <= m + kSlack);
                         if (__any_sync(0xffffffffu, raise)) {
                             const float m1 = raise ? top : m, a = raise ? ex2(m - m1) : 1.0f;   // 0 while m is -inf
                             m = m1;

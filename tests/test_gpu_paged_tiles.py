@@ -188,6 +188,51 @@ def test_scores_of_lowest_and_infinite_values(session):
     assert bool(((out[0].cpu().double() - v).abs() <= ref.half_step(v, F16)).all())
 
 
+@pytest.mark.parametrize("D,group,new", [(64, 4, 70), (128, 4, 70), (256, 4, 70), (128, 2, 50), (64, 3, 5), (256, 2, 1), (128, 1, None)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_scores_of_infinity_and_nan(session, D, group, new, bad):
+    """They make the rows that see them NaN, wherever they stand, and no other."""
+    n = 300
+    rows, offsets = (1, None) if new is None else (new, [0, new])
+    q = queries(rows, group * D, BF16).abs()
+    for at in (*range(n - 19, n), 0, 5, 130, n - 40):
+        c = ref.Cache([n], 1, D, 16, BF16)
+        poison(c, 0, 0, [at], k=torch.tensor([bad] + [1.0] * (D - 1), dtype=BF16, device="cuda"))
+        sees = torch.arange(n - rows, n) >= at
+        for win in (0, 200):
+            out, lse = window(session, c, q, group, offsets, win, 1)
+            see = sees & (torch.arange(n - rows, n) - win < at) if win and at else sees
+            got = out.view(rows, group, D).cpu()
+            assert bool(got[see].isnan().all()) and bool(lse.cpu()[see].isnan().all())
+            assert bool(got[~see].isfinite().all()) and bool(lse.cpu()[~see].isfinite().all())
+
+
+def test_prefix_scores_of_infinity_and_nan(session):
+    for bad in (math.nan, math.inf):
+        c = Shared(300, [20] * 40, 1, 128, 16, BF16)
+        q = queries(40, 4 * 128, BF16).abs()
+        p = int(c.table[3, 0])
+        c.k[p, 0, 8, 5] = bad
+        out, lse = prefix(session, c, c.prefix, 300, q, 4)
+        see = torch.arange(40) == 3
+        assert bool(out.cpu()[see].isnan().all()) and bool(lse.cpu()[see].isnan().all())
+        assert bool(out.cpu()[~see].isfinite().all()) and bool(lse.cpu()[~see].isfinite().all())
+        c.k[c.prefix[9], 0, 0, 5] = bad
+        out, lse = prefix(session, c, c.prefix, 300, q, 4)
+        assert bool(out.isnan().all()) and bool(lse.isnan().all())
+
+
+def test_rows_without_slots_behind_a_long_window(session):
+    """Rows before slot 0 and a window near 2^31."""
+    c = ref.Cache([20, 50], 2, 64, 16, F16)
+    q = queries(300, 4 * 64, F16)
+    offsets = [0, 200, 300]
+    want = window(session, c, q, 4, offsets, 0, 0)
+    for win in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 100):
+        got = check_window(session, c, q, 4, offsets, win, 3)
+        assert ref.same_bits(got[0], want[0]) and ref.same_bits(got[1], want[1])
+
+
 def test_growing_scores(session):
     """Every block's maximum is far above the one before, and far below at the end."""
     c = ref.Cache([1400], 1, 128, 64, BF16)
