@@ -88,6 +88,7 @@ template <int D> struct Cut {
     // rows up to which P's rounding is made up for
     static constexpr int kFine = kSubs == 2 ? 128 : 64;
 };
+constexpr int kUnitBlocks = 3;   // a unit's queries, first scores and results take about as long as so many blocks
 constexpr int kFew = 32;   // rows that the four warps of a sub-tile share
 
 // How queries are loaded: 128 (or 32) rows by a tensor copy where the group divides 32, or 128 where no unit has few rows; row
@@ -1377,6 +1378,18 @@ constexpr int rows_of(int head_dim) { return head_dim == 256 ? 128 : 256; }
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
+// Into how many parts to cut `blocks` key blocks of each of `tiles` tiles: the number of at most `most` with which the GPU is
+// done first, by the rounds of its SMs times the blocks of a part and what a unit costs beside them.
+long long fewest_rounds(long long tiles, long long blocks, long long most) {
+    long long best = 1, least = LLONG_MAX;
+    for (long long parts = 1; parts <= most; ++parts) {
+        const long long chunk = ceil_div(blocks, parts), units = tiles * ceil_div(blocks, chunk);
+        const long long time = ceil_div(units, kSms) * (chunk + kUnitBlocks);
+        if (time < least) least = time, best = parts;
+    }
+    return best;
+}
+
 // Cuts of a row's key blocks, of which there are at most `blocks`, where `units` tiles of rows and heads are to be
 // shared out and a tile has about tile_rows rows.
 Split split(long long units, long long blocks, long long tile_rows) {
@@ -1389,6 +1402,7 @@ Split split(long long units, long long blocks, long long tile_rows) {
     } else if (units < 8 * kSms) {
         parts = ceil_div(8 * kSms, units);
         if (parts > ceil_div(blocks, 32)) parts = ceil_div(blocks, 32);
+        parts = fewest_rounds(units, blocks, parts);
     }
     if (parts <= 1) return s;
     s.chunk = static_cast<int>(ceil_div(blocks, parts));
@@ -1421,13 +1435,11 @@ PrefixSplit prefix_split(long long n_seq, int heads, int kv_heads, int head_dim,
     PrefixSplit s{};
     s.own = split(n_seq * kv_heads * ceil_div(group, tile), ceil_div(max_slots, keys), group < tile ? group : tile);
     if (s.own.parts == 0) s.own = Split{INT_MAX, 1};
-    // a CTA's equal share of the prefix, if that is not less than a few blocks
+    // a few units a CTA at most, and of no less than a few blocks
     const long long blocks = ceil_div(max_prefix, keys), tiles = kv_heads * ceil_div(n_seq * group, tile);
-    long long chunk = ceil_div(blocks * tiles, kSms);
-    if (chunk < 4) chunk = 4;
-    if (chunk > blocks) chunk = blocks;
-    s.chunk = static_cast<int>(chunk);
-    s.parts = static_cast<int>(ceil_div(blocks, chunk));
+    const long long a = ceil_div(4 * kSms, tiles), b = ceil_div(blocks, 4);
+    s.chunk = static_cast<int>(ceil_div(blocks, fewest_rounds(tiles, blocks, a < b ? a : b)));
+    s.parts = static_cast<int>(ceil_div(blocks, s.chunk));
     return s;
 }
 
