@@ -298,8 +298,8 @@ struct Shared {
     int bad[kBadRing];
     int units[kSegments], sum[12];
     uint32_t tmem;
-    int stop, leave;
-    int odd;          // infinities or NaN were taken out of the unit's values
+    int stop;
+    int odd[2];       // infinities or NaN were taken out of the values of an even or odd unit
 };
 
 __device__ __forceinline__ void load_q(uint32_t dst, const CUtensorMap* map, int x, int head, int row, uint64_t* bar) {
@@ -433,6 +433,17 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
 }
 template <int N>
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
+
+// The same, and whether some thread says so.
+template <int N>
+__device__ __forceinline__ bool meet_or(bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r)
+                 : "r"(static_cast<uint32_t>(v)), "n"(N)
+                 : "memory");
+    return r != 0;
+}
 
 // The bits below n, all or none of them where n is past the ends.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
@@ -585,7 +596,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     fer::dev::mbar_init(&sh.o_full[i][j], 1);
         }
         sh.stop = 0;
-        sh.odd = 0;
+        sh.odd[0] = sh.odd[1] = 0;
         fer::dev::fence_mbar_init();
         fer::dev::prefetch_tmap(&k_map);
         fer::dev::prefetch_tmap(&v_map);
@@ -973,10 +984,11 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             ok = ok && warp_wait(&sh.unit_full[slot], k / kUnitSlots);
             // both sub-tiles' warps leave together: each unit has barriers for all of them
             if (!ok) *stop = 1;
-            meet<32 * C::kSoft>();   // and the unit before is done with its sums and results
-            if (t == 0) sh.leave = *stop, sh.odd = 0;
-            meet<32 * C::kSoft>();
-            if (sh.leave) {
+            // and the unit before is done with its sums and results
+            const bool leave = meet_or<32 * C::kSoft>(!ok || *stop);
+            volatile int* const odd_here = &sh.odd[k & 1];
+            if (t == 0) sh.odd[(k + 1) & 1] = 0;
+            if (leave) {
                 if (!ok && lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutMma);
                 break;
             }
@@ -1108,7 +1120,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     if (any_hidden<D>(u, s0, 64) && ok) {
                         const uint32_t tile = base + at_v(loads_two<D>(u), i, nb);
                         ok = warp_wait(&sh.full[tile % C::kStages], tile / C::kStages);
-                        if (ok) clean_values<T, D>(u, smem_at + C::kRing + tile % C::kStages * C::kTile + h * 8192, s0, r, &sh.odd);
+                        if (ok) clean_values<T, D>(u, smem_at + C::kRing + tile % C::kStages * C::kTile + h * 8192, s0, r, odd_here);
                         fer::dev::fence_proxy_async_smem();
                     }
                     if (++h == C::kParts) h = 0, i += step;
@@ -1163,24 +1175,30 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 // as many dims at once as there is room for: 4 KB a warp
                 const int width = min(D, nf <= 8 ? 128 : nf <= 16 ? 64 : 32), rows = 1024 / width;
                 float* const meet_at = reinterpret_cast<float*>(smem_at + C::kMeet);
-                for (int d = 0; d < D; d += width) {
-                    for (int e0 = 0; e0 < width; e0 += 32) {
-                        float o[1][32];
-                        if (mine && ok) {
-                            tmem_ld(o_at + d + e0, o[0]);
-                            wait_ld(o);
-                        }
-                        if (on) {
+                // the dims of this warp from d + e0 on, several loads under way at once
+                const auto gather = [&](auto loads, int d, int e0) {
+                    constexpr int N = decltype(loads)::value;
+                    float o[N][32];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4) {
-                                // 16-byte pieces of neighbouring rows in different banks
-                                float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                if (mine && ok) q = make_float4(o[0][e] * mine2, o[0][e + 1] * mine2, o[0][e + 2] * mine2, o[0][e + 3] * mine2);
-                                *reinterpret_cast<float4*>(meet_at + (w * rows + lane) * width + e0 + ((e ^ (lane << 2)) & 28)) = q;
-                            }
+                    for (int j = 0; j < N; ++j) tmem_ld(o_at + d + e0 + 32 * j, o[j]);   // without sums: anything
+                    wait_ld(o);
+                    if (on) {
+#pragma unroll
+                        for (int e = 0; e < 32 * N; e += 4) {
+                            // 16-byte pieces of neighbouring rows in different banks
+                            float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            const float* const from = o[e >> 5] + (e & 31);
+                            if (mine && ok) q = make_float4(from[0] * mine2, from[1] * mine2, from[2] * mine2, from[3] * mine2);
+                            *reinterpret_cast<float4*>(meet_at + (w * rows + lane) * width + e0 + (e & ~31) + ((e ^ (lane << 2)) & 28)) = q;
                         }
-                        __syncwarp();
                     }
+                    __syncwarp();
+                };
+                const bool odd = *odd_here != 0;
+                for (int d = 0; d < D; d += width) {
+                    if (width == 32) gather(std::integral_constant<int, 1>{}, d, 0);
+                    else
+                        for (int e0 = 0; e0 < width; e0 += 64) gather(std::integral_constant<int, 2>{}, d, e0);
                     meet<32 * C::kSoft>();
                     for (int i = t; i < nf * width; i += 32 * C::kSoft) {
                         const int row = i / width, e = i % width;
@@ -1189,7 +1207,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
 #pragma unroll
                         for (int g = 0; g < kParts; ++g) v += from[g * rows * width];
                         if (nb == 0) v = 0.0f;
-                        if (sh.odd) {
+                        if (odd) {
                             float one[1] = {v};
                             add_odd<T, D, 1>(c, p, u, row, d + e, one);
                             v = one[0];
@@ -1224,7 +1242,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 const float scale = u.part >= 0 ? 1.0f : total == 0.0f ? 0.0f : 1.0f / total;
                 wa *= scale, wb *= scale;
                 if (rows_here && ok) {
-                    const bool odd = sh.odd != 0;
+                    const bool odd = *odd_here != 0;
                     // 128 bytes of each of the warp's rows at a time, turned round in shared memory, so that eight lanes write a
                     // row's 128 bytes
                     uint8_t* const turn = smem_at + C::kMeet + w * 4096;
@@ -1235,42 +1253,43 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     uint8_t* const mine_at = turn + lane * 128;
                     const int span = u.part >= 0 ? 32 : 64;   // dims in 128 bytes
 #pragma unroll 1
-                    for (int d = d0; d < d1; d += 16) {
-                        float o[16];
+                    for (int d = d0; d < d1; d += 32) {
+                        float o[32];
                         {
-                            uint32_t a[16], b[16];
-                            if (nb > 0) tmem_ld16(at_a + d, a);
-                            if (alt && nb > 1) tmem_ld16(at_b + d, b);
+                            float a[2][32];
+                            tmem_ld(at_a + d, a[0]);   // without sums: anything
+                            tmem_ld(at_b + d, a[1]);
+                            wait_ld(a);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                o[e] = nb > 0 ? __uint_as_float(a[e]) * wa : 0.0f;
-                                if (alt && nb > 1) o[e] = fmaf(__uint_as_float(b[e]), wb, o[e]);
+                            for (int e = 0; e < 32; ++e) {
+                                o[e] = nb > 0 ? a[0][e] * wa : 0.0f;
+                                if (alt && nb > 1) o[e] = fmaf(a[1][e], wb, o[e]);
                             }
                         }
                         if (odd) {
-                            float y[16];
+                            float y[32];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) y[e] = o[e];
-                            add_odd<T, D, 16>(c, p, u, fr, d, y);
+                            for (int e = 0; e < 32; ++e) y[e] = o[e];
+                            add_odd<T, D, 32>(c, p, u, fr, d, y);
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = y[e];
+                            for (int e = 0; e < 32; ++e) o[e] = y[e];
                         }
                         const int off = (d - d0) % span;
                         if (u.part >= 0) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
+                            for (int e = 0; e < 8; ++e)
                                 *reinterpret_cast<float4*>(mine_at + (((off / 4 + e) ^ lane) & 7) * 16) =
                                     make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
+                            for (int e = 0; e < 4; ++e)
                                 *reinterpret_cast<uint4*>(mine_at + (((off / 8 + e) ^ lane) & 7) * 16) =
                                     make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
                                                pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
                         }
-                        if (off + 16 < span && d + 16 < d1) continue;
+                        if (off + 32 < span && d + 32 < d1) continue;
                         __syncwarp();
-                        const int begin = d - off, pieces = (off + 16) * size / 16;
+                        const int begin = d - off, pieces = (off + 32) * size / 16;
                         const unsigned long long column = static_cast<unsigned long long>(begin) * size + (lane & 7) * 16;
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
