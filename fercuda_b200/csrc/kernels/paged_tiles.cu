@@ -136,6 +136,7 @@ struct Unit {
     int sb, wb0;       // key blocks: 0 .. sb - 1, then wb0 ..
     int c0, c1;        // of them, counted in that order, the unit's
     int part;          // -1: the only one of its rows
+    bool last;         // of the CTA's
 };
 
 __device__ __forceinline__ float ex2(float v) {
@@ -216,12 +217,16 @@ struct Prefix {
     __device__ __forceinline__ int units(const Paged& c) const { return c.kv_heads * tiles * chunks; }
 };
 
-// Unit x of the call; s_units: units before every segment of seg sequences.
+// Whether every sequence has the same number of units, whatever its length: they need not be counted.
+__device__ __forceinline__ bool alike(const TileParams& p) { return !p.offsets && p.chunk == INT_MAX; }
+
+// Unit x of the call; s_units: units before every segment of seg sequences, where they are not alike.
 template <int D>
 __device__ __forceinline__ Unit find_unit(const Paged& c, const TileParams& p, const Prefix<D>& pre, const int* s_units,
-                                          int segments, int seg, int x) {
+                                          int segments, int seg, int x, bool& bad) {
     using C = Cut<D>;
     Unit u{};
+    bad = false;
     if (x < pre.units(c)) {
         // tiles that read the same keys next to one another
         const int t = x % pre.tiles, rest = x / pre.tiles, k = rest % pre.chunks;
@@ -237,6 +242,16 @@ __device__ __forceinline__ Unit find_unit(const Paged& c, const TileParams& p, c
         return u;
     }
     x -= pre.units(c);
+    if (alike(p)) {
+        const int tiles = (p.group - 1) / C::kRows + 1, rest = x / tiles;
+        u.seq = rest / c.kv_heads;
+        u.hk = rest - u.seq * c.kv_heads;
+        const Seq q(c, p, u.seq);
+        bad = q.bad;
+        u.c1 = tile_range<D>(p, q, x - rest * tiles, u);
+        u.part = p.prefix_pages ? 0 : -1;
+        return u;
+    }
     int lo = 0, hi = segments;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -613,8 +628,14 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
 
     // units before every segment of sequences
     const Prefix<D> pre(c, p);
-    const int seg = (p.n_seq + kSegments - 1) / kSegments, segments = (p.n_seq + seg - 1) / seg;
-    {
+    int seg = 1, segments = 1;
+    if (alike(p)) {
+        if (t == 0) {
+            sh.sum[0] = p.n_seq * c.kv_heads * ((p.group - 1) / C::kRows + 1);
+            if (pre.bad && blockIdx.x == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
+        }
+    } else {
+        seg = (p.n_seq + kSegments - 1) / kSegments, segments = (p.n_seq + seg - 1) / seg;
         int mine[(kSegments + C::kThreads - 1) / C::kThreads] = {};
         bool bad = pre.bad, broken = false;
         int carry = 0;
@@ -717,7 +738,9 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 int n0 = -1, n1 = -1, n2 = -1;
                 for (int i = 0; i < max(nb, 1) && ok; ++i) {
                     const int id3 = page_at(u, i + 3);
-                    if (i + 1 >= nb) {
+                    if (i + 1 >= nb && u.last) {
+                        next.tok0 = -1;
+                    } else if (i + 1 >= nb) {
                         next = take(k + 1);
                         n0 = page_at(next, 0), n1 = page_at(next, 1), n2 = page_at(next, 2);
                     }
@@ -758,11 +781,14 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 ok = warp_wait(&sh.unit_full[slot], k / kUnitSlots);
                 if (!ok || fer::dev::warp_flag(stop)) break;
                 const int nf = uniform(sh.unit[slot].nf), nb = uniform(sh.unit[slot].c1 - sh.unit[slot].c0);
-                const bool end = uniform(sh.unit[slot].tok0) < 0;
+                const bool end = uniform(sh.unit[slot].tok0) < 0, last = uniform(sh.unit[slot].last) != 0;
                 __syncwarp();
                 if (lane == 0) fer::dev::mbar_arrive(&sh.unit_empty[slot]);
                 if (end) break;
-                if (nb == 0) continue;
+                if (nb == 0) {
+                    if (last) break;
+                    continue;
+                }
                 const bool alt = C::kSubs == 2 && nf <= 128, fine = nf <= C::kFine && nf > kFew;
                 // a unit of one sub-tile has one place, they take turns; else each sub-tile has its own
                 const int q_at = C::kSubs == 1 ? 0 : alt ? turn : x;
@@ -838,6 +864,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     if (alt && x == 1 && nb == 1) {
                         skip();                                                  // V_0
                         if (lane == 0) fer::dev::mbar_arrive(&sh.q_empty[q_at]);
+                        if (last) break;
                         continue;
                     }
                     landed(tile);
@@ -880,6 +907,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                     }
                     if (alt && (nb - 1) % 2 != x) skip();                        // the other's last values
                 }
+                if (last) break;
             }
             if (!ok) {
                 if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutLoad);
@@ -897,8 +925,12 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 Unit u{};
                 u.tok0 = -1;
                 if (!ok || fer::dev::warp_flag(stop)) return u;
-                if (x < units) u = find_unit<D>(c, p, pre, sh.units, segments, seg, static_cast<int>(x));
+                bool bad = false;
+                if (x < units) u = find_unit<D>(c, p, pre, sh.units, segments, seg, static_cast<int>(x), bad);
+                // the next round's is one of the next grid's
+                u.last = static_cast<long long>(k + 1) * grid + (k & 1 ? blockIdx.x : grid - 1 - blockIdx.x) >= units;
                 if (lane == 0) {
+                    if (bad) fer::dev::report(p.err, fer::dev::kErrBadShape);
                     sh.unit[slot] = u;
                     fer::dev::mbar_arrive(&sh.unit_full[slot]);
                 }
@@ -956,10 +988,13 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             Unit u = publish(0);
             if (u.tok0 >= 0) {
                 queries(u);
-                u = publish(1);
+                if (u.last) u.tok0 = -1;
+                else u = publish(1);
             }
             for (int k = 1; ok && u.tok0 >= 0; ++k) {
-                const Unit next = publish(k + 1);
+                Unit next = u;
+                next.tok0 = -1;
+                if (!u.last) next = publish(k + 1);
                 queries(u);
                 u = next;
             }
@@ -1315,6 +1350,13 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
                 }
             }
             fence_before();
+            if (u.last) {
+                if (!ok) {
+                    *stop = 1;
+                    if (lane == 0) fer::dev::report(p.err, fer::dev::kErrTimeoutMma);
+                }
+                break;
+            }
         }
     }
 
