@@ -62,7 +62,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMostScale = 2.0e38f;   // times log2 e it is still finite
 constexpr float kSlack = 7.0f;          // log2 units the subtracted maximum may lag
-constexpr int kPoly = 1, kPolyOf = 4;   // of so many pairs of exponentials so many go to the multipliers
+constexpr int kPoly = 1, kPolyOf = 16;   // of so many pairs of exponentials so many go to the multipliers
 
 // Sizes of a head_dim: keys a block, sub-tiles of rows, tiles of the ring.
 template <int D> struct Cut {
@@ -547,13 +547,14 @@ __device__ __forceinline__ void clean_values(const Unit& u, uint8_t* at, int s0,
         for (int i = 0; i < kPieces; ++i) *piece(i) = make_uint4(0, 0, 0, 0);
         return;
     }
-    uint32_t any = 0;
+    uint32_t most[2] = {0, 0};   // of all 16-bit magnitudes, by halves
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
         const uint4 w = *piece(i);
-        any |= odd_tops<T>(w.x) | odd_tops<T>(w.y) | odd_tops<T>(w.z) | odd_tops<T>(w.w);
+        most[0] = __vmaxu2(most[0], w.x & 0x7fff7fffu), most[1] = __vmaxu2(most[1], w.y & 0x7fff7fffu);
+        most[0] = __vmaxu2(most[0], w.z & 0x7fff7fffu), most[1] = __vmaxu2(most[1], w.w & 0x7fff7fffu);
     }
-    if (!any) return;
+    if (!odd_tops<T>(__vmaxu2(most[0], most[1]))) return;
     *odd = 1;
     __threadfence_block();   // whoever finds the zeros finds the note
     for (int i = 0; i < kPieces; ++i) {
@@ -1452,14 +1453,17 @@ long long fewest_rounds(long long tiles, long long blocks, long long most) {
 }
 
 // Cuts of a row's key blocks, of which there are at most `blocks`, where `units` tiles of rows and heads are to be
-// shared out and a tile has about tile_rows rows.
-Split split(long long units, long long blocks, long long tile_rows) {
+// shared out and a tile has about tile_rows rows. A tile of few rows is bound by HBM, and a part costs it what reading some
+// 300 keys does, so cuts are for even shares: of 1024 keys or more where there are fewer tiles than SMs, else of 2560 (64
+// sequences x 8 key heads behind a window of 2048: whole 146 us, in halves 158; over 8192 slots: whole 421, in parts 282).
+Split split(long long units, long long blocks, long long tile_rows, int keys) {
     Split s{INT_MAX, 0};
     long long parts = 1;
     if (tile_rows <= 64) {
-        // a part costs little: even shares of ragged lengths
-        parts = ceil_div(blocks, 8);
-        if (parts > ceil_div(6 * kSms, units)) parts = ceil_div(6 * kSms, units);
+        const bool many = units >= kSms;
+        const long long most = ceil_div((many ? 12 : 6) * kSms, units);
+        parts = ceil_div(blocks, (many ? 2560 : 1024) / keys);
+        if (parts > most) parts = most;
     } else if (units < 8 * kSms) {
         parts = ceil_div(8 * kSms, units);
         if (parts > ceil_div(blocks, 32)) parts = ceil_div(blocks, 32);
@@ -1482,7 +1486,7 @@ Split window_split(long long rows, long long n_seq, int heads, int kv_heads, int
     }
     const long long tiles = n_seq > ceil_div(rows * group, tile) ? n_seq : ceil_div(rows * group, tile);
     const long long each = ceil_div(rows, n_seq) * group;
-    return split(tiles * kv_heads, blocks, each < tile ? each : tile);
+    return split(tiles * kv_heads, blocks, each < tile ? each : tile, keys);
 }
 
 struct PrefixSplit {
@@ -1494,7 +1498,7 @@ PrefixSplit prefix_split(long long n_seq, int heads, int kv_heads, int head_dim,
     const int keys = keys_of(head_dim), tile = rows_of(head_dim);
     const long long group = heads / kv_heads;
     PrefixSplit s{};
-    s.own = split(n_seq * kv_heads * ceil_div(group, tile), ceil_div(max_slots, keys), group < tile ? group : tile);
+    s.own = split(n_seq * kv_heads * ceil_div(group, tile), ceil_div(max_slots, keys), group < tile ? group : tile, keys);
     if (s.own.parts == 0) s.own = Split{INT_MAX, 1};
     // a few units a CTA at most, and of no less than a few blocks
     const long long blocks = ceil_div(max_prefix, keys), tiles = kv_heads * ceil_div(n_seq * group, tile);
