@@ -86,4 +86,9 @@ inline cudaError_t paged_params(const fer_paged_view_t* c, fer::dev::Paged* p) {
     return cudaSuccess;
 }
 
+// Attention of one token a sequence behind a window (a.window, 0: none, and a.sinks; a.offsets is not used), and the bytes of
+// its workspace. Arguments but the workspace have been checked.
+size_t window_token_bytes(int n_seq, int heads, int head_dim, int max_slots, int window, int sinks);
+cudaError_t window_token(const dev::Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, uint32_t* err, cudaStream_t s);
+
 }  // namespace fer::host

@@ -92,6 +92,7 @@ struct AttnParams {
     float* part_ml;      // [n_seq * heads][chunks][2]
     float* part_o;       // [n_seq * heads][chunks][head_dim]
     float* scores;       // [n_seq * heads][max_slots], with weights
+    int window, sinks;   // of the kernels for windows
     uint32_t* err;
 };
 
@@ -212,27 +213,47 @@ struct Units {
     }
 };
 
+// What a window (WIN) lets the latest slot of `len` see: the slots from lo on and those below the sinks. Chunks begin at
+// `begin`, a multiple of a round, behind chunks of the `head` first slots; head is 0 where the two meet or there is no window.
+template <bool WIN>
+struct Visible {
+    int begin = 0, head = 0, lo = 0;
+    __device__ __forceinline__ Visible(const AttnParams& p, int len) {
+        if constexpr (WIN) {
+            lo = max(len - p.window, 0);
+            const int first = lo & -kRound, sinks = min(p.sinks, len);
+            if (first > ((sinks + kRound - 1) & -kRound)) begin = first, head = sinks;
+        }
+    }
+    __device__ __forceinline__ int head_chunks(const AttnParams& p) const { return WIN ? p.chunks_of(head) : 0; }
+    __device__ __forceinline__ int rounds(int len) const { return rounds_of(len - begin) + (WIN ? rounds_of(head) : 0); }
+};
+
 // One sequence's units: head blocks, chunks of each, and the cost of a block.
+template <bool WIN>
 struct Seq {
-    int len, chunks, heads;
+    int len, chunks, heads, rounds;
     __device__ __forceinline__ Seq(const Paged& c, const AttnParams& p, int b) {
         bool bad;
         len = c.length(b, &bad);
-        chunks = p.chunks_of(len);
+        const Visible<WIN> v(p, len);
+        chunks = v.head_chunks(p) + p.chunks_of(len - v.begin);
         heads = c.kv_heads * p.blocks;
+        rounds = v.rounds(len);
     }
     __device__ __forceinline__ int units() const { return chunks * heads; }
-    __device__ __forceinline__ int block_cost() const { return rounds_of(len) + chunks * kUnitCost; }
+    __device__ __forceinline__ int block_cost() const { return rounds + chunks * kUnitCost; }
     __device__ __forceinline__ int cost() const { return block_cost() * heads; }
 };
 
-// The first unit whose cost begins at or behind x.
+// The first unit whose cost begins at or behind x (of a window about that: what counts is that runs meet).
+template <bool WIN>
 __device__ __forceinline__ int unit_at(const Paged& c, const AttnParams& p, const Units& t, int x) {
     const int s = t.find(t.cost, x);
     int u = t.units[s];
     x -= t.cost[s];
     for (int b = s * t.seg; b < min(p.n_seq, (s + 1) * t.seg); ++b) {
-        const Seq q(c, p, b);
+        const Seq<WIN> q(c, p, b);
         if (x < q.cost()) {
             const int block = x / q.block_cost(), rest = x - block * q.block_cost();
             const int each = rounds_of(p.chunk()) + kUnitCost;
@@ -247,16 +268,36 @@ __device__ __forceinline__ int unit_at(const Paged& c, const AttnParams& p, cons
 // One unit.
 struct Unit {
     int b, hk, blk, chunk, chunks, n;   // n: slots
+    int k0, lo;                         // of a window: first slot, and what Visible says
 };
 
+template <bool WIN>
+__device__ __forceinline__ int first_slot(const AttnParams& p, const Unit& x) { return WIN ? x.k0 : x.chunk << p.chunk_log2; }
+
+// Its slots, from the others.
+template <bool WIN>
+__device__ __forceinline__ void set_slots(const AttnParams& p, int len, Unit& x) {
+    if constexpr (WIN) {
+        const Visible<WIN> v(p, len);
+        const int head = v.head_chunks(p);
+        const bool first = x.chunk < head;
+        x.k0 = first ? x.chunk << p.chunk_log2 : v.begin + ((x.chunk - head) << p.chunk_log2);
+        x.n = min(p.chunk(), (first ? v.head : len) - x.k0);
+        x.lo = v.lo;
+    } else {
+        x.n = min(p.chunk(), len - (x.chunk << p.chunk_log2));
+    }
+}
+
+template <bool WIN>
 __device__ __forceinline__ Unit find_unit(const Paged& c, const AttnParams& p, const Units& t, int u) {
     const int s = t.find(t.units, u);
     int r = u - t.units[s];
     int b = s * t.seg;
-    Seq q(c, p, b);
+    Seq<WIN> q(c, p, b);
     while (r >= q.units() && b + 1 < p.n_seq) {
         r -= q.units();
-        q = Seq(c, p, ++b);
+        q = Seq<WIN>(c, p, ++b);
     }
     Unit x;
     x.b = b;
@@ -265,19 +306,20 @@ __device__ __forceinline__ Unit find_unit(const Paged& c, const AttnParams& p, c
     x.chunk = r - hb * q.chunks;
     x.hk = hb / p.blocks;
     x.blk = hb - x.hk * p.blocks;
-    x.n = min(p.chunk(), q.len - (x.chunk << p.chunk_log2));
+    set_slots<WIN>(p, q.len, x);
     return x;
 }
 
 // The units of a run, found 32 at a time, one a lane, and handed to the whole
 // warp one by one.
+template <bool WIN>
 struct UnitRun {
     int from = -1;   // unit of lane 0
     Unit x{};
     __device__ __forceinline__ Unit get(const Paged& c, const AttnParams& p, const Units& t, int u, int last) {
         if (from < 0 || u >= from + 32) {
             from = u;
-            x = find_unit(c, p, t, min(u + static_cast<int>(threadIdx.x & 31), last));
+            x = find_unit<WIN>(c, p, t, min(u + static_cast<int>(threadIdx.x & 31), last));
         }
         const int i = u - from;
         Unit y;
@@ -287,6 +329,7 @@ struct UnitRun {
         y.chunk = __shfl_sync(0xffffffffu, x.chunk, i);
         y.chunks = __shfl_sync(0xffffffffu, x.chunks, i);
         y.n = __shfl_sync(0xffffffffu, x.n, i);
+        if constexpr (WIN) y.k0 = __shfl_sync(0xffffffffu, x.k0, i), y.lo = __shfl_sync(0xffffffffu, x.lo, i);
         return y;
     }
 };
@@ -302,22 +345,36 @@ struct ChunkPages {
         const int x = __shfl_sync(0xffffffffu, a, i & 31), y = __shfl_sync(0xffffffffu, b, i & 31);
         return i < 32 ? x : y;
     }
-    __device__ __forceinline__ bool all_good(const Paged& c, const Unit& x, int k0) const {
-        const int lane = threadIdx.x & 31, last = ((k0 + x.n - 1) >> c.shift) - (k0 >> c.shift);
-        return !__any_sync(0xffffffffu, (lane <= last && !c.is_page(a)) || (lane + 32 <= last && !c.is_page(b)));
-    }
+    template <bool WIN>
+    __device__ __forceinline__ bool all_good(const Paged& c, const AttnParams& p, const Unit& x, int k0) const;
 };
 
-__device__ __forceinline__ ChunkPages load_pages(const Paged& c, const Unit& x, int k0) {
-    const int lane = threadIdx.x & 31, last = ((k0 + x.n - 1) >> c.shift) - (k0 >> c.shift);
+// Whether the chunk's i-th page is one that it reads: a page without a visible slot is not, nor is its id.
+template <bool WIN>
+__device__ __forceinline__ bool page_needed(const Paged& c, const AttnParams& p, const Unit& x, int k0, int i) {
+    if (i > ((k0 + x.n - 1) >> c.shift) - (k0 >> c.shift)) return false;
+    const int first = ((k0 >> c.shift) + i) << c.shift;
+    return !WIN || first + c.page_size() > x.lo || first < p.sinks;
+}
+
+template <bool WIN>
+__device__ __forceinline__ bool ChunkPages::all_good(const Paged& c, const AttnParams& p, const Unit& x, int k0) const {
+    const int lane = threadIdx.x & 31;
+    return !__any_sync(0xffffffffu, (page_needed<WIN>(c, p, x, k0, lane) && !c.is_page(a)) ||
+                                        (page_needed<WIN>(c, p, x, k0, lane + 32) && !c.is_page(b)));
+}
+
+template <bool WIN>
+__device__ __forceinline__ ChunkPages load_pages(const Paged& c, const AttnParams& p, const Unit& x, int k0) {
+    const int lane = threadIdx.x & 31;
     const int32_t* row = c.table + static_cast<size_t>(x.b) * c.max_pages + (k0 >> c.shift) + lane;
     ChunkPages g{-1, -1};
-    if (lane <= last) g.a = row[0];
-    if (lane + 32 <= last) g.b = row[32];
+    if (page_needed<WIN>(c, p, x, k0, lane)) g.a = row[0];
+    if (page_needed<WIN>(c, p, x, k0, lane + 32)) g.b = row[32];
     return g;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool WIN>
 __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
     attn_units(const Paged c, const AttnParams p, const __grid_constant__ CUtensorMap k_map,
                const __grid_constant__ CUtensorMap v_map) {
@@ -361,16 +418,17 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
             for (int i = t; i < p.heads; i += kThreads) p.lse[static_cast<size_t>(b) * p.heads + i] = -INFINITY;
     }
     Units table{s_units, s_cost, 0, 0};
-    UnitRun run;
+    UnitRun<WIN> run;
     int u0 = 0, u1 = 1;
     if (p.direct) {
         // no table: this CTA's unit by its index
         const int heads = c.kv_heads * p.blocks, chunk = blockIdx.x % p.chunks, hb = blockIdx.x / p.chunks;
         const int b = hb / heads, h = hb - b * heads;
-        const Seq q(c, p, b);
+        const Seq<WIN> q(c, p, b);
         if (chunk >= q.chunks) return;
         run.from = 0;
-        run.x = Unit{b, h / p.blocks, h % p.blocks, chunk, q.chunks, min(p.chunk(), q.len - (chunk << p.chunk_log2))};
+        run.x = Unit{b, h / p.blocks, h % p.blocks, chunk, q.chunks};
+        set_slots<WIN>(p, q.len, run.x);
         __syncthreads();   // the barriers are set up
     } else {
         // how many units each segment of sequences has and what they cost, and the sums before them
@@ -384,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
             const int s = s0 + t;
             if (s < table.segments) {
                 for (int b = s * table.seg; b < min(p.n_seq, (s + 1) * table.seg); ++b) {
-                    const Seq q(c, p, b);
+                    const Seq<WIN> q(c, p, b);
                     mine += q.units();
                     cost += q.cost();
                 }
@@ -413,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
         {
             const int x = static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(cost_carry)) *
                                            (blockIdx.x + (lane & 1)) / gridDim.x);
-            const int u = x >= cost_carry ? carry : unit_at(c, p, table, x);
+            const int u = x >= cost_carry ? carry : unit_at<WIN>(c, p, table, x);
             u0 = __shfl_sync(0xffffffffu, u, 0);
             u1 = __shfl_sync(0xffffffffu, u, 1);
         }
@@ -434,15 +492,15 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
         if (p.blocks == 1) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
         else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
         Unit x = run.get(c, p, table, u0, u1 - 1), next = x;
-        ChunkPages pages = load_pages(c, x, x.chunk << p.chunk_log2), ahead = pages;
+        ChunkPages pages = load_pages<WIN>(c, p, x, first_slot<WIN>(p, x)), ahead = pages;
         int q = 0;
         for (int u = u0; u < u1 && alive; ++u) {
             if (u + 1 < u1) {   // the next unit's page ids are on their way meanwhile
                 next = run.get(c, p, table, u + 1, u1 - 1);
-                ahead = load_pages(c, next, next.chunk << p.chunk_log2);
+                ahead = load_pages<WIN>(c, p, next, first_slot<WIN>(p, next));
             }
-            const int k0 = x.chunk << p.chunk_log2;
-            const int good = pages.all_good(c, x, k0);
+            const int k0 = first_slot<WIN>(p, x);
+            const int good = pages.all_good<WIN>(c, p, x, k0);
             if (!good && lane == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
             for (int r0 = 0; r0 < x.n; r0 += kRound, ++q) {
                 const int stage = q % C::kStages;
@@ -505,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
     for (int u = u0; u < u1; ++u) {
         const int h0 = x.hk * p.group + x.blk * 8 * NT;          // first head of the block
         const int nh = min(8 * NT, p.group - x.blk * 8 * NT);    // its heads
-        const int k0 = x.chunk << p.chunk_log2;
+        const int k0 = first_slot<WIN>(p, x);
         const Unit next = u + 1 < u1 ? run.get(c, p, table, u + 1, u1 - 1) : x;
         const bool turn = next.b != x.b || next.hk != x.hk || next.blk != x.blk;
         if (kAhead && turn) load_q(next, qn);
@@ -547,8 +605,12 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
             }
             const int j = r0 + 16 * w + lane / 4;   // this lane's slots of the chunk: j, j + 8
             bool on0 = j < x.n, on1 = j + 8 < x.n;
+            if constexpr (WIN) {
+                on0 = on0 && (k0 + j >= x.lo || k0 + j < p.sinks);
+                on1 = on1 && (k0 + j + 8 >= x.lo || k0 + j + 8 < p.sinks);
+            }
             if (!good) {
-                const ChunkPages pg = load_pages(c, x, k0);
+                const ChunkPages pg = load_pages<WIN>(c, p, x, k0);
                 const int p0 = pg.of(c, k0, min(j, x.n - 1)), p1 = pg.of(c, k0, min(j + 8, x.n - 1));
                 on0 = on0 && c.is_page(p0);
                 on1 = on1 && c.is_page(p1);
@@ -565,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
                     if (lane < 4) s_top[w][nt * 8 + 2 * lane + e] = v;
                 }
-            if (p.scores) {
+            if (!WIN && p.scores) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -615,6 +677,13 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
                 for (int nt = 0; nt < NT; ++nt) f[nt] = s_p[v][nt][lane];
                 const int r = 16 * v + (lane & 7) + ((lane >> 4) << 3);
                 const int left = rows - 16 * v - 2 * (lane & 3);   // a lane has slots 0, 1, 8 and 9 from there
+                uint32_t seen0 = ~0u, seen1 = ~0u;                 // their bits, and those of 8 and 9: of slots that are seen
+                if constexpr (WIN) {
+                    const int s = k0 + r0 + 16 * v + 2 * (lane & 3);
+                    const auto seen = [&](int i) { return s + i >= x.lo || s + i < p.sinks; };
+                    seen0 = (seen(0) ? 0xffffu : 0u) | (seen(1) ? 0xffff0000u : 0u);
+                    seen1 = (seen(8) ? 0xffffu : 0u) | (seen(9) ? 0xffff0000u : 0u);
+                }
 #pragma unroll
                 for (int k = 0; k < kMine; ++k) {
                     uint32_t a[4];
@@ -624,6 +693,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
                         const uint32_t m1 = left > 9 ? ~0u : left > 8 ? 0xffffu : 0u;
                         a[0] &= m0, a[1] &= m0, a[2] &= m1, a[3] &= m1;
                     }
+                    if constexpr (WIN) a[0] &= seen0, a[1] &= seen0, a[2] &= seen1, a[3] &= seen1;   // and those not seen
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         mma<T>(kTwo ? low[nt][k] : o[nt][k], a, f[nt].z, f[nt].w);
@@ -737,7 +807,7 @@ __device__ __forceinline__ float chunks_lse2(const float* ml, int chunks) {
 // of its own, are added in order. The others add
 // probabilities to the weights of four slots a thread, with what does not
 // depend on the total in flight before they wait for it.
-template <typename T, int D, int kFinish, int DIMS, int kW>
+template <typename T, int D, int kFinish, int DIMS, int kW, bool WIN>
 __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const AttnParams p) {
     constexpr int kWarpsIn = kFinish / 32, kV = DIMS / 32, kBands = D / DIMS, kHeads = 4;
     // Chunks that share a maximum, and batches of lse's loads: functions of D and kW, so not of the batch.
@@ -751,7 +821,7 @@ __global__ void __launch_bounds__(kFinish) attn_finish(const Paged c, const Attn
     fer::dev::pdl_begin();
     bool bad;
     const int len = c.length(b, &bad);
-    const int chunks = p.chunks_of(len);
+    const int chunks = WIN ? Seq<WIN>(c, p, b).chunks : p.chunks_of(len);
     const size_t bh0 = static_cast<size_t>(b) * p.heads + static_cast<size_t>(hk) * p.group;
     if (static_cast<int>(blockIdx.x) < p.group * kBands) {
         if (chunks <= 1) return;                      // written already
@@ -891,22 +961,22 @@ bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int r
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int D, int THREADS, int DIMS, int kW>
+template <typename T, int D, int THREADS, int DIMS, int kW, bool WIN>
 cudaError_t finish(const Paged& c, const AttnParams& p, cudaStream_t s) {
     // as many tiles a (key head, sequence) as there are, within kTiles CTAs: a wide table has mostly empty ones
     // (those 64 x 32 heads with weights: 66 us in all with every tile its CTA, 37 so)
     const long long pairs = static_cast<long long>(c.kv_heads) * p.n_seq;
     const int all = p.weights ? (c.max_slots() - 1) / (4 * THREADS) + 1 : 0, least = static_cast<int>(kTiles / pairs) + 1;
     const int tiles = all < least ? all : least;
-    return fer::host::launch_pdl(attn_finish<T, D, THREADS, DIMS, kW>,
+    return fer::host::launch_pdl(attn_finish<T, D, THREADS, DIMS, kW, WIN>,
                                  dim3(p.group * (D / DIMS) + tiles, c.kv_heads, p.n_seq), dim3(THREADS), 0, s, c, p);
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool WIN>
 cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
     constexpr int smem = Cut<D>::kSmem;
     static std::atomic<int> known[fer::host::kMaxDevices];
-    const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT>), smem, known);
+    const int ctas = resident(reinterpret_cast<const void*>(attn_units<T, D, NT, WIN>), smem, known);
     if (ctas <= 0) return cudaErrorInvalidConfiguration;
     CUtensorMap k_map, v_map;
     const int rows = kRound < c.page_size() ? kRound : c.page_size();
@@ -914,16 +984,16 @@ cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
     if (!map_pages(&k_map, c, c.k, dtype, rows) || !map_pages(&v_map, c, c.v, dtype, rows)) return cudaErrorInvalidValue;
     const long long most = static_cast<long long>(p.n_seq) * c.kv_heads * p.blocks * p.chunks;
     p.direct = most <= ctas;
-    cudaError_t e = fer::host::launch_pdl(attn_units<T, D, NT>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
+    cudaError_t e = fer::host::launch_pdl(attn_units<T, D, NT, WIN>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
                                           dim3(kThreads), smem, s, c, p, k_map, v_map);
     if (e == cudaSuccess && (p.weights || p.chunks > 1)) {
         // few chunks or many heads: a head a CTA; else sixteen warps for 32 dims, whose loads one SM could not have
         // in flight (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA; 64 x 32
         // heads of up to 512 slots in a table of 32768: 52 us in all so, 33 with a head a CTA)
         // Which warp takes which chunk, and with it every rounding, is a function of the table's width.
-        if (p.chunks <= 32) e = finish<T, D, 256, D, 8>(c, p, s);
-        else if (static_cast<long long>(p.n_seq) * p.heads >= kManyHeads) e = finish<T, D, 256, D, 16>(c, p, s);
-        else e = finish<T, D, 512, 32, 16>(c, p, s);
+        if (p.chunks <= 32) e = finish<T, D, 256, D, 8, WIN>(c, p, s);
+        else if (static_cast<long long>(p.n_seq) * p.heads >= kManyHeads) e = finish<T, D, 256, D, 16, WIN>(c, p, s);
+        else e = finish<T, D, 512, 32, 16, WIN>(c, p, s);
     }
     return e;
 }
@@ -931,23 +1001,81 @@ cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
 // Head blocks a key head: of up to 8 heads, or of up to 16 where it has more.
 int blocks_of(int group) { return group <= 8 ? 1 : (group - 1) / 16 + 1; }
 
-template <typename T, int D>
+template <typename T, int D, bool WIN>
 cudaError_t run_heads(const Paged& c, AttnParams& p, cudaStream_t s) {
-    return p.group <= 8 ? run<T, D, 1>(c, p, s) : run<T, D, 2>(c, p, s);
+    return p.group <= 8 ? run<T, D, 1, WIN>(c, p, s) : run<T, D, 2, WIN>(c, p, s);
 }
 
-template <typename T>
+template <typename T, bool WIN>
 cudaError_t run_dim(const Paged& c, AttnParams& p, cudaStream_t s) {
     switch (c.head_dim) {
-        case 64: return run_heads<T, 64>(c, p, s);
-        case 128: return run_heads<T, 128>(c, p, s);
-        default: return run_heads<T, 256>(c, p, s);
+        case 64: return run_heads<T, 64, WIN>(c, p, s);
+        case 128: return run_heads<T, 128, WIN>(c, p, s);
+        default: return run_heads<T, 256, WIN>(c, p, s);
     }
 }
 
+// Slots and the most chunks of a sequence that a window lets its latest slot see.
+struct WindowChunks {
+    int chunk, chunks;
+    WindowChunks(int max_slots, int window, int sinks) {
+        const long long slots = max_slots, win = window < slots ? window : slots, head = sinks < slots ? sinks : slots;
+        const auto up = [](long long v, long long by) { return (v + by - 1) / by * by; };
+        const long long span = win + head < slots ? win + head : slots;
+        chunk = chunk_of(static_cast<int>(span));
+        // the same test as Visible's for the longest sequence: the others' windows begin no later
+        const bool meet = ((slots - win) & -static_cast<long long>(kRound)) <= up(head, kRound);
+        const long long all = up(slots, chunk) / chunk;
+        const long long apart = up(head, chunk) / chunk + up(win + kRound, chunk) / chunk + 1;
+        chunks = static_cast<int>(meet || all < apart ? all + !meet : apart);
+    }
+};
+
 size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
 
+// Units and their cost are counted in 31 bits.
+bool countable(const Paged& c, int n_seq, int group, long long chunks) {
+    return static_cast<long long>(n_seq) * c.kv_heads * blocks_of(group) * (rounds_of(c.max_slots()) + kUnitCost * chunks) <= 0x7fffffffll;
+}
+
 }  // namespace
+
+// Attention of one token a sequence behind a window, by a.window > 0 or 0 and a.sinks; arguments are checked but for what follows.
+size_t fer::host::window_token_bytes(int n_seq, int heads, int head_dim, int max_slots, int window, int sinks) {
+    const size_t bh = static_cast<size_t>(n_seq) * heads;
+    const size_t chunks = WindowChunks(max_slots, window > 0 ? window : max_slots, window > 0 ? sinks : 0).chunks;
+    return up16(bh * chunks * 2 * sizeof(float)) + up16(bh * chunks * head_dim * sizeof(float));
+}
+
+cudaError_t fer::host::window_token(const Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, uint32_t* err, cudaStream_t s) {
+    const bool win = a.window > 0;
+    const WindowChunks w(c.max_slots(), win ? a.window : c.max_slots(), win ? a.sinks : 0);
+    AttnParams p{};
+    p.q = a.q;
+    p.out = a.out;
+    p.qs = a.q_stride;
+    p.os = a.out_stride;
+    p.n_seq = a.n_seq;
+    p.heads = a.heads;
+    p.group = a.heads / c.kv_heads;
+    p.blocks = blocks_of(p.group);
+    while ((1 << p.chunk_log2) < w.chunk) ++p.chunk_log2;
+    p.chunks = w.chunks;
+    p.scale2 = (a.scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c.head_dim)) : a.scale) * kLog2e;
+    p.lse = a.lse;
+    p.window = a.window;
+    p.sinks = a.sinks;
+    p.err = err;
+    if (!countable(c, a.n_seq, p.group, p.chunks)) return cudaErrorNotSupported;
+    if (!a.workspace || reinterpret_cast<uintptr_t>(a.workspace) % 16 ||
+        a.workspace_bytes < window_token_bytes(a.n_seq, a.heads, c.head_dim, c.max_slots(), a.window, a.sinks))
+        return cudaErrorInvalidValue;
+    char* const at = static_cast<char*>(a.workspace);
+    p.part_ml = reinterpret_cast<float*>(at);
+    p.part_o = reinterpret_cast<float*>(at + up16(static_cast<size_t>(a.n_seq) * a.heads * p.chunks * 2 * sizeof(float)));
+    if (win) return dtype == 1 ? run_dim<__half, true>(c, p, s) : run_dim<__nv_bfloat16, true>(c, p, s);
+    return dtype == 1 ? run_dim<__half, false>(c, p, s) : run_dim<__nv_bfloat16, false>(c, p, s);
+}
 
 extern "C" size_t fer_paged_attention_workspace_bytes(int n_seq, int heads, int kv_heads, int head_dim, int max_slots,
                                                       int with_weights) {
@@ -974,11 +1102,8 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     if (a->n_seq == 0) return cudaSuccess;
     if (c.kv_heads > 65535 || a->n_seq > 65535) return cudaErrorNotSupported;
     const int max_slots = c.max_slots();
-    // units and their cost are counted in 31 bits
     const int group = a->heads / c.kv_heads;
-    const long long blocks = static_cast<long long>(a->n_seq) * c.kv_heads * blocks_of(group);
-    if (blocks * (rounds_of(max_slots) + kUnitCost * ((max_slots - 1ll) / chunk_of(max_slots) + 1)) > 0x7fffffffll)
-        return cudaErrorNotSupported;
+    if (!countable(c, a->n_seq, group, (max_slots - 1ll) / chunk_of(max_slots) + 1)) return cudaErrorNotSupported;
     const size_t need = fer_paged_attention_workspace_bytes(a->n_seq, a->heads, c.kv_heads, c.head_dim, max_slots,
                                                             a->weights != nullptr);
     if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 || a->workspace_bytes < need)
@@ -1005,5 +1130,5 @@ extern "C" cudaError_t fer_paged_attention(const fer_paged_view_t* cache, const 
     p.part_o = reinterpret_cast<float*>(w);
     w += up16(bh * p.chunks * c.head_dim * sizeof(float));
     if (a->weights) p.scores = reinterpret_cast<float*>(w);
-    return cache->dtype == 1 ? run_dim<__half>(c, p, s) : run_dim<__nv_bfloat16>(c, p, s);
+    return cache->dtype == 1 ? run_dim<__half, false>(c, p, s) : run_dim<__nv_bfloat16, false>(c, p, s);
 }

@@ -1526,6 +1526,10 @@ PrefixSplit prefix_split(long long n_seq, int heads, int kv_heads, int head_dim,
     return s;
 }
 
+// Single tokens of groups up to so many heads go to the kernel for them, which hides latencies with several small CTAs an SM
+// (behind a window of 2048, 64 x 8 groups of 4 heads: 90 us there, 145 here); it reads a larger group's pages more than once.
+constexpr int kTokenGroup = 16;
+
 size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
 size_t parts_bytes(size_t rows, size_t heads, size_t head_dim, size_t parts) {
     return up16(rows * heads * parts * 2 * sizeof(float)) + rows * heads * parts * head_dim * sizeof(float);
@@ -1669,7 +1673,12 @@ extern "C" size_t fer_paged_window_attention_workspace_bytes(int rows, int n_seq
                                                              int max_slots, int window, int sinks) {
     if (rows <= 0 || n_seq <= 0 || max_slots <= 0 || window < 0 || sinks < 0 || !sizes_ok(heads, kv_heads, head_dim)) return 0;
     const Split s = window_split(rows, n_seq, heads, kv_heads, head_dim, max_slots, window, sinks);
-    return s.parts > 0 ? parts_bytes(rows, heads, head_dim, s.parts) : 16;
+    size_t n = s.parts > 0 ? parts_bytes(rows, heads, head_dim, s.parts) : 16;
+    if (rows == n_seq && heads / kv_heads <= kTokenGroup) {   // there may be no offsets
+        const size_t m = fer::host::window_token_bytes(n_seq, heads, head_dim, max_slots, window, sinks);
+        if (m > n) n = m;
+    }
+    return n;
 }
 
 extern "C" cudaError_t fer_paged_window_attention(const fer_paged_view_t* cache, const fer_paged_window_args_t* a, uint32_t* err,
@@ -1684,6 +1693,7 @@ extern "C" cudaError_t fer_paged_window_attention(const fer_paged_view_t* cache,
         return cudaErrorInvalidValue;
     if (a->rows == 0 || a->n_seq == 0) return cudaSuccess;
     if (a->n_seq > 65535) return cudaErrorNotSupported;
+    if (!a->offsets && p.group <= kTokenGroup) return fer::host::window_token(c, cache->dtype, *a, err, s);
     p.offsets = a->offsets;
     p.rows = a->rows;
     p.n_seq = a->n_seq;

@@ -79,6 +79,41 @@ def test_window_of_single_tokens(session, dtype, D, H, group, page, lens, win, s
     check_window(session, c, queries(len(lens), H * group * D, dtype), H * group, None, win, sinks)
 
 
+# sinks in chunks of their own, or meeting the window's; windows that begin inside a page; more units than CTAs; no slot or page
+# outside is any number
+@pytest.mark.parametrize("dtype,D,H,group,page,lens,win,sinks", [
+    (BF16, 64, 2, 4, 256, [2000, 1500, 700, 257], 100, 600),
+    (F16, 128, 2, 8, 8, [3000, 1290, 1300, 20], 1000, 300),
+    (BF16, 128, 1, 9, 128, [1000, 999, 64, 65], 64, 1),
+    (BF16, 256, 2, 16, 16, [1200, 130, 0, 513], 300, 64),
+    (F16, 64, 16, 1, 16, [(i * 37) % 900 for i in range(70)], 200, 5),
+    (BF16, 128, 8, 4, 64, [(i * 211) % 2000 for i in range(40)], 1024, 4),
+    (BF16, 128, 2, 17, 16, [1200, 130, 700], 300, 64),
+    (F16, 64, 1, 2, 8, [70000, 66000, 3], 66000, 3),      # longer chunks
+])
+def test_window_of_single_tokens_reads_nothing_else(session, dtype, D, H, group, page, lens, win, sinks):
+    c = ref.Cache(lens, H, D, page, dtype, seed=win)
+    q = queries(len(lens), H * group * D, dtype)
+    dev, k, v, table = (c.k, c.v, c.table), c.k.cpu(), c.v.cpu(), c.table.cpu()
+    c.k, c.v, c.table = k, v, table      # read over and over
+    want = tiles_ref.window(c, q, H * group, None, win, sinks)
+    c.k, c.v, c.table = dev
+    for b, n in enumerate(lens):
+        gone = torch.arange(n)
+        gone = gone[(gone >= sinks) & (gone <= n - 1 - win)]
+        at = table[b, gone // page].long()
+        k[at, :, gone % page], v[at, :, gone % page] = math.nan, math.inf
+        for i in (gone // page).unique().tolist():
+            if i * page >= sinks and (i + 1) * page <= n - win:
+                table[b, i] = [-1, 10 ** 9, -2 ** 31][i % 3]
+    c.k.copy_(k), c.v.copy_(v), c.table.copy_(table)
+    out, lse = window(session, c, q, H * group, None, win, sinks)
+    agree(out, lse, *want, dtype)
+    if lens[0] > win:      # a page that is read is reported
+        c.table[0, (lens[0] - 1) // page] = -1
+        window(session, c, q, H * group, None, win, sinks, errors=ERR_BAD)
+
+
 # prompts: ragged rows, sequences without any, rows behind the last, more rows than slots
 @pytest.mark.parametrize("dtype,D,H,group,page,lens,new,win,sinks,tail", [
     (BF16, 64, 2, 1, 16, [5], [5], 0, 0, 0),
