@@ -90,5 +90,7 @@ inline cudaError_t paged_params(const fer_paged_view_t* c, fer::dev::Paged* p) {
 // its workspace. Arguments but the workspace have been checked.
 size_t window_token_bytes(int n_seq, int heads, int head_dim, int max_slots, int window, int sinks);
 cudaError_t window_token(const dev::Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, uint32_t* err, cudaStream_t s);
+int token_parts_chunk(int max_slots);
+cudaError_t token_parts(const dev::Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, uint32_t* err, cudaStream_t s);
 
 }  // namespace fer::host

@@ -56,6 +56,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <climits>
 #include <cstdint>
 
 namespace {
@@ -93,6 +94,7 @@ struct AttnParams {
     float* part_o;       // [n_seq * heads][chunks][head_dim]
     float* scores;       // [n_seq * heads][max_slots], with weights
     int window, sinks;   // of the kernels for windows
+    int apart;           // there: results stay parts
     uint32_t* err;
 };
 
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, Cut<D>::kCtas)
                 if (lane < 4) s_l[w][nt * 8 + 2 * lane + e] = l[nt][e];
             }
         meet_warps();
-        const bool whole = x.chunks == 1;
+        const bool whole = x.chunks == 1 && !(WIN && p.apart);
         constexpr float kBack = 1.0f / kScaleP<T>;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -986,7 +988,7 @@ cudaError_t run(const Paged& c, AttnParams& p, cudaStream_t s) {
     p.direct = most <= ctas;
     cudaError_t e = fer::host::launch_pdl(attn_units<T, D, NT, WIN>, dim3(static_cast<unsigned>(most < ctas ? most : ctas)),
                                           dim3(kThreads), smem, s, c, p, k_map, v_map);
-    if (e == cudaSuccess && (p.weights || p.chunks > 1)) {
+    if (e == cudaSuccess && !p.apart && (p.weights || p.chunks > 1)) {
         // few chunks or many heads: a head a CTA; else sixteen warps for 32 dims, whose loads one SM could not have
         // in flight (256 chunks: 8.9 us with a head a CTA, 6.0 so; 4 chunks: 6.2 so, 5.2 with a head a CTA; 64 x 32
         // heads of up to 512 slots in a table of 32768: 52 us in all so, 33 with a head a CTA)
@@ -1047,9 +1049,11 @@ size_t fer::host::window_token_bytes(int n_seq, int heads, int head_dim, int max
     return up16(bh * chunks * 2 * sizeof(float)) + up16(bh * chunks * head_dim * sizeof(float));
 }
 
-cudaError_t fer::host::window_token(const Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, uint32_t* err, cudaStream_t s) {
+namespace {
+
+cudaError_t launch_window(const Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, int chunk, int chunks, bool apart,
+                          uint32_t* err, cudaStream_t s) {
     const bool win = a.window > 0;
-    const WindowChunks w(c.max_slots(), win ? a.window : c.max_slots(), win ? a.sinks : 0);
     AttnParams p{};
     p.q = a.q;
     p.out = a.out;
@@ -1059,22 +1063,39 @@ cudaError_t fer::host::window_token(const Paged& c, uint32_t dtype, const fer_pa
     p.heads = a.heads;
     p.group = a.heads / c.kv_heads;
     p.blocks = blocks_of(p.group);
-    while ((1 << p.chunk_log2) < w.chunk) ++p.chunk_log2;
-    p.chunks = w.chunks;
+    while ((1 << p.chunk_log2) < chunk) ++p.chunk_log2;
+    p.chunks = chunks;
     p.scale2 = (a.scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c.head_dim)) : a.scale) * kLog2e;
     p.lse = a.lse;
-    p.window = a.window;
-    p.sinks = a.sinks;
+    p.window = win ? a.window : INT_MAX;
+    p.sinks = win ? a.sinks : 0;
+    p.apart = apart;
     p.err = err;
     if (!countable(c, a.n_seq, p.group, p.chunks)) return cudaErrorNotSupported;
-    if (!a.workspace || reinterpret_cast<uintptr_t>(a.workspace) % 16 ||
-        a.workspace_bytes < window_token_bytes(a.n_seq, a.heads, c.head_dim, c.max_slots(), a.window, a.sinks))
-        return cudaErrorInvalidValue;
     char* const at = static_cast<char*>(a.workspace);
     p.part_ml = reinterpret_cast<float*>(at);
     p.part_o = reinterpret_cast<float*>(at + up16(static_cast<size_t>(a.n_seq) * a.heads * p.chunks * 2 * sizeof(float)));
-    if (win) return dtype == 1 ? run_dim<__half, true>(c, p, s) : run_dim<__nv_bfloat16, true>(c, p, s);
+    if (win || apart) return dtype == 1 ? run_dim<__half, true>(c, p, s) : run_dim<__nv_bfloat16, true>(c, p, s);
     return dtype == 1 ? run_dim<__half, false>(c, p, s) : run_dim<__nv_bfloat16, false>(c, p, s);
+}
+
+}  // namespace
+
+cudaError_t fer::host::window_token(const Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, uint32_t* err, cudaStream_t s) {
+    if (!a.workspace || reinterpret_cast<uintptr_t>(a.workspace) % 16 ||
+        a.workspace_bytes < window_token_bytes(a.n_seq, a.heads, c.head_dim, c.max_slots(), a.window, a.sinks))
+        return cudaErrorInvalidValue;
+    const WindowChunks w(c.max_slots(), a.window > 0 ? a.window : c.max_slots(), a.window > 0 ? a.sinks : 0);
+    return launch_window(c, dtype, a, w.chunk, w.chunks, false, err, s);
+}
+
+// The parts of held slots for attention that goes on elsewhere: chunks of token_parts_chunk(max_slots), of a sequence's length
+// rounded up; workspace as window_token's with window 0, m and l [n_seq * heads][chunks][2], then o.
+int fer::host::token_parts_chunk(int max_slots) { return chunk_of(max_slots); }
+
+cudaError_t fer::host::token_parts(const Paged& c, uint32_t dtype, const fer_paged_window_args_t& a, uint32_t* err, cudaStream_t s) {
+    const int chunk = chunk_of(c.max_slots());
+    return launch_window(c, dtype, a, chunk, (c.max_slots() - 1) / chunk + 1, true, err, s);
 }
 
 extern "C" size_t fer_paged_attention_workspace_bytes(int n_seq, int heads, int kv_heads, int head_dim, int max_slots,

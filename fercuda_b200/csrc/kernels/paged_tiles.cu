@@ -139,6 +139,9 @@ struct TileParams {
     const int32_t* prefix_pages;   // null: no prefix
     const int32_t* prefix_length;
     int prefix_max, prefix_chunk, own_parts;
+    int own_chunk_log2;            // >= 0: sequences' own slots are another kernel's parts, in chunks of 2^that
+    const float* own_ml;           // [rows * heads][own_parts][2]
+    const float* own_o;
     uint32_t* err;
 };
 
@@ -256,7 +259,7 @@ __device__ __forceinline__ Unit find_unit(const Paged& c, const TileParams& p, c
         const int blocks = (pre.len - 1) / C::kKeys + 1;
         u.c0 = k * p.prefix_chunk;
         u.c1 = min(blocks, u.c0 + p.prefix_chunk);
-        u.part = p.own_parts + k;
+        u.part = (p.own_chunk_log2 >= 0 ? 0 : p.own_parts) + k;
         return u;
     }
     x -= pre.units(c);
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
     int seg = 1, segments = 1;
     if (alike(p)) {
         if (t == 0) {
-            sh.sum[0] = p.n_seq * c.kv_heads * ((p.group - 1) / C::kRows + 1);
+            sh.sum[0] = p.own_chunk_log2 >= 0 ? 0 : p.n_seq * c.kv_heads * ((p.group - 1) / C::kRows + 1);
             if (pre.bad && blockIdx.x == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
         }
     } else {
@@ -1414,15 +1417,26 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join(const Paged c, cons
         if (tok < q.tok0 || tok >= q.tok0 + q.n) return;   // of no sequence
         const long long f = static_cast<long long>(tok - q.tok0) * p.group + head % p.group;
         Unit u;
-        own = chunks_of(tile_range<D>(p, q, static_cast<int>(f / Cut<D>::kRows), u), p.chunk);
+        if (p.own_chunk_log2 >= 0) own = (q.len + (1 << p.own_chunk_log2) - 1) >> p.own_chunk_log2;
+        else own = chunks_of(tile_range<D>(p, q, static_cast<int>(f / Cut<D>::kRows), u), p.chunk);
     }
     if (p.prefix_pages) shared = Prefix<D>(c, p).chunks;
     else if (own == 1) return;   // written already
-    const float2* const ml = reinterpret_cast<const float2*>(p.part_ml) + item * p.parts;
-    const float* const po = p.part_o + item * p.parts * D + kV * lane;
+    // the other kernel's parts are not 2^up times as large
+    const bool other = p.own_chunk_log2 >= 0;
+    const float2* const ml = reinterpret_cast<const float2*>(p.part_ml) + item * p.parts + (other ? 0 : p.own_parts);
+    const float* const po = p.part_o + (item * p.parts + (other ? 0 : p.own_parts)) * D + kV * lane;
+    const float2* const own_ml = other ? reinterpret_cast<const float2*>(p.own_ml) + item * p.own_parts : ml - p.own_parts;
+    const float* const own_o = other ? p.own_o + item * p.own_parts * D + kV * lane : po - static_cast<size_t>(p.own_parts) * D;
+    const float lift = other ? up : 0.0f;
+    const auto part_ml = [&](int i) {
+        float2 v = i < own ? own_ml[i] : ml[i - own];
+        if (i < own) v.x += lift;
+        return v;
+    };
     const int n = own + shared;
     float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, ml[i < own ? i : p.own_parts + i - own].x);
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, part_ml(i).x);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     const float base = top == -INFINITY ? 0.0f : top;
@@ -1430,9 +1444,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join(const Paged c, cons
     Dims o{};
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
-        const int at = i < own ? i : p.own_parts + i - own;
-        const float2 v = ml[at];
-        const Dims d = *reinterpret_cast<const Dims*>(po + static_cast<size_t>(at) * D);
+        const float2 v = part_ml(i);
+        const Dims d = *reinterpret_cast<const Dims*>(i < own ? own_o + static_cast<size_t>(i) * D : po + static_cast<size_t>(i - own) * D);
         const float y = ex2(v.x - base);
         l = fmaf(v.y, y, l);
         // a part without a key counts as nothing, and one that vanishes gives an infinite value its due
@@ -1527,8 +1540,13 @@ PrefixSplit prefix_split(long long n_seq, int heads, int kv_heads, int head_dim,
 }
 
 // Single tokens of groups up to so many heads go to the kernel for them, which hides latencies with several small CTAs an SM
-// (behind a window of 2048, 64 x 8 groups of 4 heads: 90 us there, 145 here); it reads a larger group's pages more than once.
+// (behind a window of 2048, 64 x 8 groups of 4 heads: 86 us there, 145 here); it reads a larger group's pages more than once.
 constexpr int kTokenGroup = 16;
+
+// Whether the sequences' own slots behind a prefix go to that kernel too: where they are units enough to fill the GPU, for which
+// another launch pays (us here and there: 160 units of up to 400 slots 29 and 33, 320 of up to 30 33 and 28, 512 of up to 1024 85
+// and 64).
+bool own_by_tokens(long long n_seq, int heads, int kv_heads) { return heads / kv_heads <= kTokenGroup && n_seq * kv_heads >= 2 * kSms; }
 
 size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
 size_t parts_bytes(size_t rows, size_t heads, size_t head_dim, size_t parts) {
@@ -1641,17 +1659,21 @@ cudaError_t common(const fer_paged_view_t* cache, const void* q, void* out, size
     p->heads = heads;
     p->group = heads / c->kv_heads;
     p->by_group = divide(static_cast<uint32_t>(p->group));
+    p->own_chunk_log2 = -1;
     p->scale2 = (scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c->head_dim)) : scale) * kLog2e;
     return cudaSuccess;
 }
 
-cudaError_t go(const Paged& c, TileParams& p, uint32_t dtype, void* workspace, size_t bytes, cudaStream_t s) {
-    // units are counted in 31 bits, and so are the joining's CTAs
+// Units are counted in 31 bits, and so are the joining's CTAs.
+bool countable(const Paged& c, const TileParams& p) {
     const long long tiles = ceil_div(static_cast<long long>(p.rows) * p.group, rows_of(c.head_dim)) + p.n_seq;
-    if (tiles * c.kv_heads * (p.parts > 0 ? p.parts : 1) > INT_MAX - 65536ll ||
-        static_cast<long long>(p.rows) * p.group > INT_MAX - 65536ll ||
-        ceil_div(static_cast<long long>(p.rows) * p.heads, kJoinWarps) > INT_MAX)
-        return cudaErrorNotSupported;
+    return tiles * c.kv_heads * (p.parts > 0 ? p.parts : 1) <= INT_MAX - 65536ll &&
+           static_cast<long long>(p.rows) * p.group <= INT_MAX - 65536ll &&
+           ceil_div(static_cast<long long>(p.rows) * p.heads, kJoinWarps) <= INT_MAX;
+}
+
+cudaError_t go(const Paged& c, TileParams& p, uint32_t dtype, void* workspace, size_t bytes, cudaStream_t s) {
+    if (!countable(c, p)) return cudaErrorNotSupported;
     if (p.parts > 0) {
         if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
             bytes < parts_bytes(p.rows, p.heads, c.head_dim, p.parts))
@@ -1710,6 +1732,8 @@ extern "C" size_t fer_paged_prefix_attention_workspace_bytes(int n_seq, int head
                                                              int max_prefix_slots) {
     if (n_seq <= 0 || max_slots <= 0 || max_prefix_slots <= 0 || !sizes_ok(heads, kv_heads, head_dim)) return 0;
     const PrefixSplit s = prefix_split(n_seq, heads, kv_heads, head_dim, max_slots, max_prefix_slots);
+    if (own_by_tokens(n_seq, heads, kv_heads))
+        return parts_bytes(n_seq, heads, head_dim, s.parts) + fer::host::window_token_bytes(n_seq, heads, head_dim, max_slots, 0, 0);
     return parts_bytes(n_seq, heads, head_dim, static_cast<size_t>(s.own.parts) + s.parts);
 }
 
@@ -1733,9 +1757,38 @@ extern "C" cudaError_t fer_paged_prefix_attention(const fer_paged_view_t* cache,
     p.prefix_length = a->prefix_length;
     p.prefix_max = a->max_prefix_pages;
     const PrefixSplit sp = prefix_split(a->n_seq, a->heads, c.kv_heads, c.head_dim, c.max_slots(), most);
+    p.prefix_chunk = sp.chunk;
+    if (own_by_tokens(a->n_seq, a->heads, c.kv_heads)) {
+        const int max_slots = c.max_slots(), chunk = fer::host::token_parts_chunk(max_slots);
+        p.chunk = INT_MAX;
+        p.parts = sp.parts;
+        if (!countable(c, p)) return cudaErrorNotSupported;
+        const size_t mine = parts_bytes(a->n_seq, a->heads, c.head_dim, sp.parts);
+        if (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16 ||
+            a->workspace_bytes < mine + fer::host::window_token_bytes(a->n_seq, a->heads, c.head_dim, max_slots, 0, 0))
+            return cudaErrorInvalidValue;
+        char* const at = static_cast<char*>(a->workspace) + mine;
+        p.own_parts = (max_slots - 1) / chunk + 1;
+        p.own_chunk_log2 = 0;
+        while ((1 << p.own_chunk_log2) < chunk) ++p.own_chunk_log2;
+        p.own_ml = reinterpret_cast<const float*>(at);
+        p.own_o = reinterpret_cast<const float*>(at + up16(static_cast<size_t>(a->n_seq) * a->heads * p.own_parts * 2 * sizeof(float)));
+        fer_paged_window_args_t own{};
+        own.q = a->q;
+        own.out = a->out;
+        own.q_stride = a->q_stride;
+        own.out_stride = a->out_stride;
+        own.rows = own.n_seq = a->n_seq;
+        own.heads = a->heads;
+        own.scale = a->scale;
+        own.lse = a->lse;
+        own.workspace = at;
+        const cudaError_t t = fer::host::token_parts(c, cache->dtype, own, err, s);
+        if (t != cudaSuccess) return t;
+        return go(c, p, cache->dtype, a->workspace, mine, s);
+    }
     p.chunk = sp.own.chunk;
     p.own_parts = sp.own.parts;
-    p.prefix_chunk = sp.chunk;
     p.parts = sp.own.parts + sp.parts;
     return go(c, p, cache->dtype, a->workspace, a->workspace_bytes, s);
 }

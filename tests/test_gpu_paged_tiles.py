@@ -397,6 +397,13 @@ class Shared(ref.Cache):
     (BF16, 256, 1, 5, 32, 515, [64, 65, 0] * 10),
     (F16, 128, 3, 1, 256, 1000, [700, 2, 0]),
     (BF16, 128, 1, 300, 16, 140, [20, 3]),
+    # sequences enough that their own slots are the other kernel's work: one chunk, several, none
+    (BF16, 128, 8, 4, 16, 700, [(i * 53) % 300 for i in range(40)]),
+    (F16, 64, 32, 1, 8, 300, [600, 0, 257, 256, 1, 511, 512, 513, 30, 800]),
+    (BF16, 256, 6, 2, 64, 130, [(i * 7) % 70 for i in range(50)]),
+    (F16, 128, 150, 16, 32, 200, [400, 33]),
+    (F16, 128, 150, 17, 32, 200, [40, 33]),
+    (BF16, 64, 300, 2, 16, 50, [0]),
 ])
 def test_prefix(session, dtype, D, H, group, page, length, lens):
     c = Shared(length, lens, H, D, page, dtype, width=-(-length // page) + 2, seed=length)
@@ -412,6 +419,58 @@ def test_prefix_of_nothing(session):
     out, lse = prefix(session, c, c.prefix, 0, q, 2)
     agree(out, lse, *tiles_ref.prefix(c, c.prefix, 0, q, 2), F16)
     assert bool((out[1] == 0).all()) and bool((lse[1] == -math.inf).all())
+
+
+def test_prefix_own_pages_out_of_range(session):
+    """Of many sequences: reported, and of no weight."""
+    c = Shared(100, [40] * 50, 6, 64, 16, BF16)
+    q = queries(50, 12 * 64, BF16)
+    c.table[7, 1] = -1
+    out, lse = prefix(session, c, c.prefix, 100, q, 12, errors=ERR_BAD)
+    c.table[7, 1] = 0
+    others = torch.arange(50) != 7
+    want, wlse, err, ds = tiles_ref.prefix(c, c.prefix, 100, q, 12)
+    agree(out.view(50, 12, 64)[others], lse[others], want[others], wlse[others], err[others], ds, BF16)
+    assert bool(out.isfinite().all())
+    c.lengths[9] = -3
+    prefix(session, c, c.prefix, 100, q, 12, errors=ERR_BAD)
+
+
+def test_prefix_the_same_bits_every_time(session):
+    c = Shared(3000, [(i * 97) % 900 for i in range(64)], 8, 128, 16, F16)
+    q = queries(64, 32 * 128, F16)
+    first = prefix(session, c, c.prefix, 3000, q, 32)
+    for _ in range(3):
+        again = prefix(session, c, c.prefix, 3000, q, 32)
+        assert ref.same_bits(first[0], again[0]) and ref.same_bits(first[1], again[1])
+
+
+def test_prefix_captured_and_replayed(session):
+    """With another prefix, other lengths and other pages in each replay."""
+    c = Shared(700, [200] * 40, 8, 128, 16, BF16)
+    q = queries(40, 32 * 128, BF16)
+    out, lse = torch.zeros(40, 32 * 128, dtype=BF16, device="cuda"), torch.zeros(40, 32, device="cuda")
+    pages, length = i32(c.prefix), i32([700])
+    ws = torch.full((capi.paged_prefix_attention_workspace_bytes(40, 32, 8, 128, c.slots, len(c.prefix) * 16),), 255,
+                    dtype=torch.uint8, device="cuda")
+    v, a = views(c), capi.fer_paged_prefix_args_t(q.data_ptr(), out.data_ptr(), 32 * 128, 32 * 128, 40, 32, pages.data_ptr(),
+                                                  length.data_ptr(), len(c.prefix), 0.0, lse.data_ptr(), ws.data_ptr(), ws.numel())
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert capi.kernels().fer_paged_prefix_attention(C.byref(v), C.byref(a), err.data_ptr(),
+                                                         torch.cuda.current_stream().cuda_stream) == 0
+    for n, lens in ((700, [200] * 40), (33, [(i * 31) % 200 for i in range(40)]), (0, [i % 3 for i in range(40)])):
+        length.copy_(i32([n])), c.lengths.copy_(i32(lens))
+        pages.copy_(i32(c.prefix[::-1] if n == 33 else c.prefix))
+        if n == 33:   # the last page of the text is its only part full
+            pages[0], pages[-1] = pages[-1].clone(), pages[0].clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.lens = lens
+        agree(out, lse, *tiles_ref.prefix(c, pages.tolist(), n, q, 32), BF16)
+    assert err.item() == 0
+    del graph
 
 
 def test_prefix_is_what_attention_over_a_joined_table_gives(session):
