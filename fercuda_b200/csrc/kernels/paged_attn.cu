@@ -42,6 +42,12 @@
 // 32 to 33.2 us (20.6): 3.5 us pass until the first rows arrive, CTAs end between 18
 // and 29 us as they have a unit more or less, and 5 us go to the joining.
 //
+// Behind a window (kernels with WIN) chunks of the sinks come first, then chunks
+// from the window's first slot, rounded down to a round; where the two meet they
+// are one run. Slots that are not seen count as -inf and their values as zeros,
+// and pages without one that is seen are not looked up: 64 sequences of 1 to 8192
+// slots behind 2048 read 470 MB in 86 to 90 us, 5.3 TB/s.
+//
 // Scores are kept in base-2 units (scale * log2 e folded into one factor).
 // When weights are wanted they go to the workspace as well, and the second
 // kernel adds 2^(s - lse) of a group's heads, in head order.

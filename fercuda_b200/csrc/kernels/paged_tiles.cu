@@ -28,12 +28,15 @@
 // What bounds it. Wide units: the latency of a sub-tile's 64 keys (scores from
 // tensor memory, maximum, exponentials, P back, about 1900 cycles, while the
 // tensor cores are busy 58% of the time and the issue slots 45%): a piece of 4001
-// tokens behind 28000, 32 heads x 128, takes 1948 us, 1009 TFLOP/s. Loops that
-// stay in the instruction cache matter as much as their length (prompts behind a
-// window 478 -> 372 us by chunks that are looped over instead of unrolled). Prompts behind a window of 512 lose a
-// third to masked blocks, whose slots are tested one by one, and 6000 cycles a
-// unit to its results. Single tokens: latency and uneven shares; 64 sequences
-// behind a window of 2048 read 470 MB in 146 us, 3.2 TB/s.
+// tokens behind 28000, 32 heads x 128, takes 1940 to 1965 us, 1009 TFLOP/s.
+// Loops that stay in the instruction cache matter as much as their length
+// (prompts behind a window 478 -> 372 us by chunks that are looped over instead
+// of unrolled). Prompts behind a window of 512 (320 to 345 us for 16 of up to
+// 2048) lose a third to masked blocks, whose slots are tested one by one, and
+// 6000 cycles a unit to its results. Units of few rows: latency and uneven
+// shares (3.2 TB/s); where all rows are single tokens of small groups, and
+// where own slots behind a prefix are many, the kernel of one-token attention
+// takes them, which has three or four small CTAs an SM.
 //
 // P is rounded to 16 bits once, by half a step of the type at most, and l sums it
 // unrounded; where rows are few (kFine) what rounding leaves is multiplied as a
@@ -1715,7 +1718,10 @@ extern "C" cudaError_t fer_paged_window_attention(const fer_paged_view_t* cache,
         return cudaErrorInvalidValue;
     if (a->rows == 0 || a->n_seq == 0) return cudaSuccess;
     if (a->n_seq > 65535) return cudaErrorNotSupported;
-    if (!a->offsets && p.group <= kTokenGroup) return fer::host::window_token(c, cache->dtype, *a, err, s);
+    if (!a->offsets && p.group <= kTokenGroup) {
+        const cudaError_t t = fer::host::window_token(c, cache->dtype, *a, err, s);
+        if (t != cudaErrorNotSupported) return t;   // its units are counted by the table's width, here by what is seen
+    }
     p.offsets = a->offsets;
     p.rows = a->rows;
     p.n_seq = a->n_seq;
