@@ -242,6 +242,26 @@ def test_the_same_bits_every_time(session):
         assert all(ref.same_bits(a, b) for a, b in zip(first, (dx, dq, dk)))
 
 
+def test_rows_behind_two_to_the_31_elements(session):
+    rows, width = 2400, 1 << 20
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB")
+    few, dy, pos, qg, kg = setup(rows, 3, 64, BF16, 1)
+    x = torch.zeros(rows, width, dtype=BF16, device="cuda")
+    x[:, -192:] = few.cuda()
+    out = torch.empty(rows, 192, dtype=BF16, device="cuda")
+    want = torch.empty_like(out)
+    kw = dict(k_heads=1, qg=qg.cuda(), kg=kg.cuda())
+    call(session, few.cuda(), want, pos.cuda(), 3, 64, **kw)
+    call(session, x, out, pos.cuda(), 3, 64, x_col=width - 192, **kw)
+    assert ref.same_bits(out, want)
+    call_grad(session, few.cuda(), dy.cuda(), want, pos.cuda(), 3, 64, **kw)
+    call_grad(session, x, dy.cuda(), out, pos.cuda(), 3, 64, x_col=width - 192, **kw)
+    assert ref.same_bits(out, want)
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_no_rows(session):
     one = torch.zeros(1, 128, dtype=BF16, device="cuda")
     args = capi.fer_norm_rotary_args_t
