@@ -1048,7 +1048,6 @@ bool countable(const Paged& c, int n_seq, int group, long long chunks) {
 
 }  // namespace
 
-// Attention of one token a sequence behind a window, by a.window > 0 or 0 and a.sinks; arguments are checked but for what follows.
 size_t fer::host::window_token_bytes(int n_seq, int heads, int head_dim, int max_slots, int window, int sinks) {
     const size_t bh = static_cast<size_t>(n_seq) * heads;
     const size_t chunks = WindowChunks(max_slots, window > 0 ? window : max_slots, window > 0 ? sinks : 0).chunks;

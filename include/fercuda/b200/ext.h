@@ -434,8 +434,8 @@ fer_status_t fer_submit_paged_evict(fer_session_t* session, const fer_paged_evic
  * behind the last). page_size: a power of two from 8 to 256. Error bit 4: a
  * length, count or number of pages out of range (clamped; more slots than a row
  * of the table holds: no rows for that sequence), a page id or free_state out of
- * range, more rows than the arrays have (dropped). A free_state out of range moves no page; a
- * page id out of range moves as it is, and slots of it are -1. */
+ * range, more rows than the arrays have (dropped). A free_state out of range
+ * moves no page; a page id out of range moves as it is, and slots of it are -1. */
 typedef struct fer_paged_plan_request {
     uint64_t page_table;
     uint64_t lengths;
@@ -501,7 +501,9 @@ fer_status_t fer_submit_paged_window_attention(fer_session_t* session, const fer
  * hold the sequences' own slots alone; a prefix enters its pages once, as a
  * sequence of a cache view of its own. Other arguments and rules as
  * fer_submit_paged_attention's (no weights); a prefix_length out of range is
- * clamped and sets error bit 4. Bit-identical run to run. workspace: u8 buffer (16-byte aligned) of at least
+ * clamped and sets error bit 4. Scores of +inf or NaN and rounding as in
+ * fer_submit_paged_window_attention. Bit-identical run to run. workspace: u8
+ * buffer (16-byte aligned) of at least
  * fer_paged_prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim,
  * max_pages * page_size, prefix pages * page_size) bytes, any contents; calls on
  * different streams need one each. */
