@@ -5,6 +5,7 @@
 
 #include "fercuda/b200/native.h"
 #include "sm100_util.cuh"
+#include "smem_limit.cuh"
 
 #include <cstdint>
 #include <initializer_list>
@@ -48,9 +49,6 @@ struct Paged {
 }  // namespace fer::dev
 
 namespace fer::host {
-
-// Devices for which a launcher keeps what it asked the runtime once.
-constexpr int kMaxDevices = 64;
 
 // Whether all of these arrays of 32-bit numbers start at a multiple of 4 bytes (null does).
 inline bool words_aligned(std::initializer_list<const void*> arrays) {

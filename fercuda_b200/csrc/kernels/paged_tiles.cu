@@ -1582,23 +1582,11 @@ bool map_queries(CUtensorMap* m, const TileParams& p, int head_dim, uint32_t dty
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Sets the shared-memory limit of a kernel once per device.
-cudaError_t allow(const void* kernel, int smem, std::atomic<bool>* known) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= fer::host::kMaxDevices) return cudaErrorInvalidDevice;
-    if (known[dev].load(std::memory_order_relaxed)) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) known[dev].store(true, std::memory_order_relaxed);
-    return e;
-}
-
 template <typename T, int D>
 cudaError_t run(const Paged& c, TileParams& p, cudaStream_t s) {
     using C = Cut<D>;
     static std::atomic<bool> known[fer::host::kMaxDevices];
-    cudaError_t e = allow(reinterpret_cast<const void*>(attn_tiles<T, D>), C::kSmem, known);
+    cudaError_t e = fer::host::allow_smem(reinterpret_cast<const void*>(attn_tiles<T, D>), C::kSmem, known);
     if (e != cudaSuccess) return e;
     CUtensorMap k_map, v_map, q_map{}, q_few_map{};
     const int rows = C::kKeys < c.page_size() ? C::kKeys : c.page_size();

@@ -24,9 +24,11 @@
 #include "pdl.cuh"
 #include "pieces.cuh"
 #include "sm100_util.cuh"
+#include "smem_limit.cuh"
 
 #include "fercuda/b200/native.h"
 
+#include <atomic>
 #include <cfloat>
 #include <climits>
 #include <cmath>
@@ -674,15 +676,17 @@ bool launch_copies(NormParams& p, float* dq, float* dk, uint32_t* err, cudaStrea
     // every warp has a row or two at least, else the form above shares rows out among warps
     if (p.rows < kSms * kCopyWarps || p.rows > INT_MAX - 4 * kSms * kCopyWarps) return false;
     const bool inter = p.flags & FER_ROTARY_FLAG_INTERLEAVED;
-    const int smem = kCopyWarps * kStages * kSegment + ((p.half + 3) & ~3) * static_cast<int>(sizeof(double) + kCopyWarps * sizeof(float2));
+    const auto smem_of = [](int half) {
+        return kCopyWarps * kStages * kSegment + ((half + 3) & ~3) * static_cast<int>(sizeof(double) + kCopyWarps * sizeof(float2));
+    };
     const bool tail = 2 * p.half < p.head_dim;
     void (*const kernel)(NormParams, uint32_t*) =
         inter ? (tail ? norm_rotary_copies<T, true, GRAD, true> : norm_rotary_copies<T, true, GRAD, false>)
               : (tail ? norm_rotary_copies<T, false, GRAD, true> : norm_rotary_copies<T, false, GRAD, false>);
-    // the limit is the kernel's on the current device; setting it again costs little beside such a pass
-    *result = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<bool> known[4][fer::host::kMaxDevices];   // of the four kernels
+    *result = fer::host::allow_smem(reinterpret_cast<const void*>(kernel), smem_of(kMostDim / 2), known[2 * inter + tail]);
     if (*result != cudaSuccess) return true;
-    *result = fer::host::launch_pdl(kernel, dim3(kSms), dim3(32 * kCopyWarps), smem, s, p, err);
+    *result = fer::host::launch_pdl(kernel, dim3(kSms), dim3(32 * kCopyWarps), smem_of(p.half), s, p, err);
     if (*result == cudaSuccess && GRAD) *result = sum_up(p, kSms, dq, dk, s);
     return true;
 }
