@@ -139,6 +139,7 @@ struct TileParams {
     int parts;                     // parts a row may have; 0: results go to out
     float* part_ml;                // [rows * heads][parts][2]
     float* part_o;                 // [rows * heads][parts][head_dim]
+    int* broken;                   // parts of rows with offsets: whether those cannot be, for the joining
     const int32_t* prefix_pages;   // null: no prefix
     const int32_t* prefix_length;
     int prefix_max, prefix_chunk, own_parts;
@@ -691,9 +692,12 @@ __global__ void __launch_bounds__(Cut<D>::kThreads, 1)
             if (s < segments) sh.units[s] = x;
             __syncthreads();
         }
-        // with offsets that cannot be nothing is done
+        // with offsets that cannot be nothing is done, here or by the joining
         broken = __syncthreads_or(broken);
-        if (t == 0) sh.sum[0] = broken ? 0 : carry;
+        if (t == 0) {
+            sh.sum[0] = broken ? 0 : carry;
+            if (p.broken && blockIdx.x == 0) *p.broken = broken;
+        }
         if ((bad || broken) && blockIdx.x == 0) fer::dev::report(p.err, fer::dev::kErrBadShape);
     }
     fence_before();
@@ -1401,7 +1405,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attn_join(const Paged c, cons
     fer::dev::pdl_begin();
     const int lane = threadIdx.x & 31;
     const long long item = static_cast<long long>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
-    if (item >= static_cast<long long>(p.rows) * p.heads) return;
+    if (item >= static_cast<long long>(p.rows) * p.heads || (p.broken && *p.broken)) return;
     const int tok = static_cast<int>(item / p.heads), head = static_cast<int>(item - static_cast<long long>(tok) * p.heads);
     int own = 0, shared = 0;
     {
@@ -1555,6 +1559,7 @@ size_t up16(size_t v) { return (v + 15) & ~size_t(15); }
 size_t parts_bytes(size_t rows, size_t heads, size_t head_dim, size_t parts) {
     return up16(rows * heads * parts * 2 * sizeof(float)) + rows * heads * parts * head_dim * sizeof(float);
 }
+constexpr size_t kBrokenBytes = 16;   // of TileParams::broken, behind the parts
 
 // Boxes of 64 dims x `rows` rows of one page; 128-byte swizzle.
 bool map_pages(CUtensorMap* m, const Paged& c, void* base, uint32_t dtype, int rows) {
@@ -1666,9 +1671,10 @@ bool countable(const Paged& c, const TileParams& p) {
 cudaError_t go(const Paged& c, TileParams& p, uint32_t dtype, void* workspace, size_t bytes, cudaStream_t s) {
     if (!countable(c, p)) return cudaErrorNotSupported;
     if (p.parts > 0) {
-        if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
-            bytes < parts_bytes(p.rows, p.heads, c.head_dim, p.parts))
+        const size_t all = parts_bytes(p.rows, p.heads, c.head_dim, p.parts);
+        if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || bytes < all + (p.offsets ? kBrokenBytes : 0))
             return cudaErrorInvalidValue;
+        if (p.offsets) p.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + all);
         p.part_ml = static_cast<float*>(workspace);
         p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                             up16(static_cast<size_t>(p.rows) * p.heads * p.parts * 2 * sizeof(float)));
@@ -1686,7 +1692,7 @@ extern "C" size_t fer_paged_window_attention_workspace_bytes(int rows, int n_seq
                                                              int max_slots, int window, int sinks) {
     if (rows <= 0 || n_seq <= 0 || max_slots <= 0 || window < 0 || sinks < 0 || !sizes_ok(heads, kv_heads, head_dim)) return 0;
     const Split s = window_split(rows, n_seq, heads, kv_heads, head_dim, max_slots, window, sinks);
-    size_t n = s.parts > 0 ? parts_bytes(rows, heads, head_dim, s.parts) : 16;
+    size_t n = s.parts > 0 ? parts_bytes(rows, heads, head_dim, s.parts) + kBrokenBytes : 16;
     if (rows == n_seq && heads / kv_heads <= kTokenGroup) {   // there may be no offsets
         const size_t m = fer::host::window_token_bytes(n_seq, heads, head_dim, max_slots, window, sinks);
         if (m > n) n = m;

@@ -470,7 +470,7 @@ fer_status_t fer_submit_paged_plan(fer_session_t* session, const fer_paged_plan_
  * are rounded to the cache's dtype once before they meet the values (where a
  * sequence has few rows to twice its bits), sums are f32. What lies in slots that a
  * row does not see does not touch it. Bit-identical run to run. Offsets that decrease
- * or leave 0 .. rows set error bit 4, and the results are then not to be used.
+ * or leave 0 .. rows set error bit 4, and out and lse are then left as they were.
  * workspace: u8 buffer (16-byte aligned) of at least
  * fer_paged_window_attention_workspace_bytes(rows, sequences, heads, kv_heads,
  * head_dim, max_pages * page_size, window, sinks) bytes, any contents; calls on

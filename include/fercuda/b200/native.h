@@ -340,8 +340,8 @@ cudaError_t fer_paged_plan(const fer_paged_plan_args_t* args, uint32_t* err, cud
  * that one of the call's rows sees are not read, nor are their entries. Other
  * arguments as fer_paged_attention's; lse [rows, heads]. A row that sees nothing
  * gives zeros, lse -inf; rows behind the last offset are left as they were.
- * Offsets that decrease or leave 0 .. rows set error bit 4, and results are then
- * not to be used. The same bits run to run. workspace:
+ * Offsets that decrease or leave 0 .. rows set error bit 4, and out and lse are
+ * then left as they were. The same bits run to run. workspace:
  * fer_paged_window_attention_workspace_bytes, rules as above. */
 typedef struct fer_paged_window_args {
     const void* q;
