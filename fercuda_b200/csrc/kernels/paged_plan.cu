@@ -261,7 +261,7 @@ __device__ __forceinline__ void fill_rows(const PlanParams& p, int* s_start, int
                 }
                 for (end = __ldcg(p.offsets + b + 1); r >= end; end = __ldcg(p.offsets + b + 1)) ++b, begin = end;
                 length = min(max(p.lengths[b], 0), p.max_pages << p.shift);
-                seen = p.positions ? (p.seen ? p.seen : p.lengths)[b] : 0;
+                seen = p.positions && p.seen ? p.seen[b] : length;
                 base = -1;
             }
             const int i = static_cast<int>(r) - begin, s = length + i;
