@@ -635,14 +635,14 @@ def norm_rotary_grad_workspace_bytes(rows: int, heads: int, head_dim: int) -> in
 
 def paged_window_attention_workspace_bytes(rows: int, sequences: int, heads: int, kv_heads: int, head_dim: int,
                                            max_slots: int, window: int, sinks: int) -> int:
-    """Bytes of workspace of Session.paged_window_attention; max_slots is max_pages * page_size."""
+    """Bytes of workspace of Session.paged_window_attention; max_slots is max_pages * page_size. Fewer rows may need more."""
     return kernels().fer_paged_window_attention_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, max_slots,
                                                                 window, sinks)
 
 
 def paged_prefix_attention_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_slots: int,
                                            max_prefix_slots: int) -> int:
-    """Bytes of workspace of Session.paged_prefix_attention; slots are pages * page_size."""
+    """Bytes of workspace of Session.paged_prefix_attention; slots are pages * page_size. Fewer rows may need more."""
     return kernels().fer_paged_prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim, max_slots,
                                                                 max_prefix_slots)
 

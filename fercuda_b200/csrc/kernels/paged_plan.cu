@@ -14,7 +14,8 @@
 // so that two cluster barriers stand where launches would: each thread has a few
 // neighbouring sequences, the sums are a scan over the cluster's threads, page
 // ids are moved by whole warps, and a row finds its sequence by a search among
-// every few sequences' first rows in shared memory. One CTA does it where there
+// every few sequences' first rows in shared memory (a thread's next rows walk on from
+// there, over sequences without rows one by one). One CTA does it where there
 // are few rows and sequences; where there are many rows a second launch spreads
 // them over the GPU (1024 requests with 236000 rows: 30 us by the cluster, 21 so).
 #include "paged.cuh"

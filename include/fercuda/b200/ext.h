@@ -474,7 +474,9 @@ fer_status_t fer_submit_paged_plan(fer_session_t* session, const fer_paged_plan_
  * workspace: u8 buffer (16-byte aligned) of at least
  * fer_paged_window_attention_workspace_bytes(rows, sequences, heads, kv_heads,
  * head_dim, max_pages * page_size, window, sinks) bytes, any contents; calls on
- * different streams need one each. */
+ * different streams need one each. Fewer rows may need more bytes, as their keys
+ * are cut into more parts: a buffer for calls of several sizes has to be as large as
+ * the largest of their needs. */
 typedef struct fer_paged_window_attention_request {
     fer_paged_cache_t cache;
     uint64_t q;
@@ -506,7 +508,7 @@ fer_status_t fer_submit_paged_window_attention(fer_session_t* session, const fer
  * buffer (16-byte aligned) of at least
  * fer_paged_prefix_attention_workspace_bytes(rows, heads, kv_heads, head_dim,
  * max_pages * page_size, prefix pages * page_size) bytes, any contents; calls on
- * different streams need one each. */
+ * different streams need one each; fewer rows may need more bytes here too. */
 typedef struct fer_paged_prefix_attention_request {
     fer_paged_cache_t cache;
     uint64_t q;

@@ -342,7 +342,9 @@ cudaError_t fer_paged_plan(const fer_paged_plan_args_t* args, uint32_t* err, cud
  * gives zeros, lse -inf; rows behind the last offset are left as they were.
  * Offsets that decrease or leave 0 .. rows set error bit 4, and out and lse are
  * then left as they were. The same bits run to run. workspace:
- * fer_paged_window_attention_workspace_bytes, rules as above. */
+ * fer_paged_window_attention_workspace_bytes, rules as above; fewer rows may need
+ * more bytes, so a buffer for calls of several sizes is as large as the largest of
+ * their needs. The same holds for the prefix's workspace. */
 typedef struct fer_paged_window_args {
     const void* q;
     void* out;
