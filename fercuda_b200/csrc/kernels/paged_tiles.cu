@@ -28,7 +28,7 @@
 // What bounds it. Wide units: the latency of a sub-tile's 64 keys (scores from
 // tensor memory, maximum, exponentials, P back, about 1900 cycles, while the
 // tensor cores are busy 58% of the time and the issue slots 45%): a piece of 4001
-// tokens behind 28000, 32 heads x 128, takes 1940 to 1986 us, 990 to 1013 TFLOP/s.
+// tokens behind 28000, 32 heads x 128, takes 1940 to 1998 us, 984 to 1013 TFLOP/s.
 // Loops that stay in the instruction cache matter as much as their length
 // (prompts behind a window 478 -> 372 us by chunks that are looped over instead
 // of unrolled). Prompts behind a window of 512 (320 to 345 us for 16 of up to
